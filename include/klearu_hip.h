@@ -678,6 +678,124 @@ int kh_dejavu_attn_block_batch(const kh_predictor* p, kh_sparse_attn* a, float* 
                                int32_t* heads_dev, float* norm_ws_dev, void* stream);
 
 /* ======================================================================== */
+/* Rotary positions, and a paged K/V cache held in 4 bits with its attention */
+/* (dense attention over prompts, chunks and single tokens; the reference    */
+/* keeps its cache in f32, model/kv_cache.rs, and rotates inside the step,   */
+/* model/rope.rs: no counterpart there)                                      */
+/* ======================================================================== */
+
+/* These calls take dtype KH_DT_F32 or KH_DT_BF16 (KH_DT_* below) for rows x of
+ * heads x head_dim elements: element (t, h, i) lies at t * row_stride +
+ * h * head_stride + i, strides in elements, any that are not negative (an
+ * output's heads must not overlap).  The handles belong to the device that was
+ * current when they were created, and calls with another current device are
+ * KH_ERR_ARG.  Nothing is allocated after creation and no scratch is shared, so
+ * calls may be captured in HIP graphs and run at once on several streams, as
+ * long as nobody reads a cache's positions while they are written. */
+
+typedef struct kh_rope kh_rope;
+
+#define KH_ROPE_HALF 0        /* element i is rotated with i + rot_dim / 2 (rope.rs:75-87) */
+#define KH_ROPE_INTERLEAVED 1 /* 2 i with 2 i + 1 */
+
+/* Frequencies f_i = theta^(-2 i / rot_dim), i < rot_dim / 2, of positions past
+ * the trained ones: */
+#define KH_ROPE_SCALE_NONE 0
+#define KH_ROPE_SCALE_LINEAR 1   /* f_i / factor */
+#define KH_ROPE_SCALE_BASE 2     /* theta * factor^(r / (r - 2)) for theta, r = rot_dim > 2 */
+#define KH_ROPE_SCALE_BY_PARTS 3 /* f_i (g + (1 - g) / factor), g = clamp((n_i - low) / (high - low), 0, 1), \
+                                    n_i = f_i original_len / (2 pi) the turns over the trained length */
+
+/* A rotation by positions 0 .. max_pos - 1: cos and sin of p f_i, in f64 and
+ * rounded to f32 once, times `magnitude` (1 leaves lengths as they are).
+ * rot_dim even, 2..1024.  Keeps max_pos * rot_dim * 4 bytes.  Synchronous. */
+int kh_rope_create(int rot_dim, int64_t max_pos, int layout, double theta, int scaling, double factor,
+                   int64_t original_len, double low, double high, double magnitude, kh_rope** out);
+int kh_rope_destroy(kh_rope* r);
+/* Rotates the first rot_dim elements of every head of row t by position
+ * pos_dev[t] and copies the others: y = R x, or y = R^T x with `transpose`, which
+ * takes the gradient with respect to y to the one with respect to x.  A row
+ * with a negative position is padding and left as it was; so is one with a
+ * position past the table, which kh_rope_status reports.  y may be x itself
+ * (with the same strides); otherwise the two must not overlap. */
+int kh_rope_apply(const kh_rope* r, int dtype, const void* x_dev, int64_t x_row_stride,
+                  int64_t x_head_stride, int64_t rows, int heads, int head_dim, const int64_t* pos_dev,
+                  void* y_dev, int64_t y_row_stride, int64_t y_head_stride, int transpose, void* stream);
+/* Synchronises the device; KH_ERR_ARG (clearing the record) if a call since the
+ * last status call met a position past the table, else KH_OK. */
+int kh_rope_status(const kh_rope* r);
+
+typedef struct kh_paged_kv kh_paged_kv;
+
+/* num_pages pages of page_size positions (16, 32, 64, 128 or 256) of every kv
+ * head; head_dim 64, 128 or 256.  32 neighbouring values of a head share m =
+ * their minimum rounded down to BF16 and s = (maximum - m) / 15 rounded up to
+ * BF16; x is held as the 4-bit c = rint((x - m) / s) and stands for s c + m:
+ * 5 bits a value.  A group with a value that is not finite stands for NaN.
+ * Positions that were never written stand for 0.  Synchronous.
+ *
+ * Which pages belong to a sequence is the caller's: row b of an int32 page
+ * table (table_dev, table_cols columns in use, rows table_stride apart) lists
+ * sequence b's pages, position p lying in page table[b][p / page_size].  Rows
+ * of a call belong to sequences by off_dev[batch + 1] (int64, ascending): rows
+ * off[b] .. off[b + 1] - 1 are sequence b's; rows outside all of them are padding
+ * and their outputs are left as they were.  Places outside the table and page
+ * ids outside the pool are not accessed, and kh_paged_kv_status reports them. */
+int kh_paged_kv_create(int num_kv_heads, int head_dim, int page_size, int64_t num_pages,
+                       kh_paged_kv** out);
+int kh_paged_kv_destroy(kh_paged_kv* c);
+/* Synchronises the device; KH_ERR_ARG (clearing the record) if a call since the
+ * last status call met a place outside its sequence's table, a length that the
+ * table cannot hold or a page id outside the pool, else KH_OK. */
+int kh_paged_kv_status(const kh_paged_kv* c);
+/* Puts keys and values k, v [rows][kv heads][head_dim] into the cache: row
+ * off[b] + i at position start_dev[b] + i of sequence b.  With a rotation the
+ * keys are rotated on the way, in f32 and before they are held in 4 bits, by
+ * pos_dev[row], or by their positions in the cache where pos_dev is NULL; rows
+ * whose rotary position is negative or past the rotation's table are not
+ * appended (kh_rope_status reports them).  Two rows of one call must not have the
+ * same place (two sequences may share pages, but not write to them). */
+int kh_paged_kv_append(kh_paged_kv* c, const kh_rope* rope, int dtype, const void* k_dev,
+                       int64_t k_row_stride, int64_t k_head_stride, const void* v_dev,
+                       int64_t v_row_stride, int64_t v_head_stride, int64_t rows, const int64_t* off_dev,
+                       int64_t batch, const int64_t* start_dev, const int64_t* pos_dev,
+                       const int32_t* table_dev, int64_t table_cols, int64_t table_stride, void* stream);
+/* The values that the same places stand for, into contiguous k, v
+ * [rows][kv heads][head_dim] (16-byte aligned). */
+int kh_paged_kv_gather(const kh_paged_kv* c, int dtype, int64_t rows, const int64_t* off_dev,
+                       int64_t batch, const int64_t* start_dev, const int32_t* table_dev,
+                       int64_t table_cols, int64_t table_stride, void* k_dev, void* v_dev, void* stream);
+/* Bytes of workspace that kh_paged_kv_attention needs for these arguments (0
+ * where one pass does it). */
+int kh_paged_kv_attention_workspace(const kh_paged_kv* c, int dtype, int64_t rows, int64_t batch,
+                                    int num_heads, int64_t max_rows, int64_t max_len, int64_t* bytes);
+/* Attention of q [rows][num_heads][head_dim] over the cache: sequence b has
+ * len_dev[b] positions there (int64, its rows of this call among them, so row i
+ * of its n rows is at position len - n + i), and
+ *   out = sum_j softmax_j(scale q . k_j) v_j
+ * over the j that the row sees: j < len; with `causal` j <= its position; with a
+ * window w > 0 (causal only) j > its position - w.  Query head h reads kv head
+ * h / (num_heads / kv heads).  lse_dev (NULL, or [rows][num_heads] f32) gets
+ * log sum_j exp(scale q . k_j).  A row that sees nothing gives 0 and -inf.
+ * heads_dev (NULL: all heads; else [rows][n_heads] int32 as
+ * kh_predictor_select_top_k gives them, ids outside [0, num_heads) skipped,
+ * repeated ids counted once): heads that a row does not list give 0 and -inf
+ * and their share of the cache is not read.
+ * max_rows and max_len are the caller's guess of the most rows and the longest
+ * length of a sequence; a wrong one costs time, not correctness.  Sums and
+ * softmax statistics are f32; BF16 rows have their weights p rounded to BF16.
+ * The result does not depend on the run.  ws_dev: 16-byte aligned,
+ * kh_paged_kv_attention_workspace bytes (fewer are KH_ERR_CAPACITY), not shared
+ * by calls that may run at once; its contents do not matter. */
+int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void* q_dev, int64_t q_row_stride,
+                          int64_t q_head_stride, int num_heads, int64_t rows, const int64_t* off_dev,
+                          int64_t batch, const int64_t* len_dev, const int32_t* table_dev,
+                          int64_t table_cols, int64_t table_stride, int64_t max_rows, int64_t max_len,
+                          float scale, int causal, int64_t window, const int32_t* heads_dev, int n_heads,
+                          void* out_dev, int64_t out_row_stride, int64_t out_head_stride, float* lse_dev,
+                          void* ws_dev, int64_t ws_bytes, void* stream);
+
+/* ======================================================================== */
 /* On-disk formats: safetensors weights and predictor JSON files            */
 /* ======================================================================== */
 

@@ -152,6 +152,18 @@ SIGS = {
     "kh_sparse_attn_cache_len": (I, [P, I64, P]),
     "kh_sparse_attn_clear": (I, [P, P]),
     "kh_sparse_attn_forward": (I, [P, P, I64, P, P, I, P, I, P]),
+    "kh_rope_create": (I, [I, I64, I, C.c_double, I, C.c_double, I64, C.c_double, C.c_double, C.c_double, PP]),
+    "kh_rope_destroy": (I, [P]),
+    "kh_rope_apply": (I, [P, I, P, I64, I64, I64, I, I, P, P, I64, I64, I, P]),
+    "kh_rope_status": (I, [P]),
+    "kh_paged_kv_create": (I, [I, I, I, I64, PP]),
+    "kh_paged_kv_destroy": (I, [P]),
+    "kh_paged_kv_status": (I, [P]),
+    "kh_paged_kv_append": (I, [P, P, I, P, I64, I64, P, I64, I64, I64, P, I64, P, P, P, I64, I64, P]),
+    "kh_paged_kv_gather": (I, [P, I, I64, P, I64, P, P, I64, I64, P, P, P]),
+    "kh_paged_kv_attention_workspace": (I, [P, I, I64, I64, I, I64, I64, P]),
+    "kh_paged_kv_attention": (I, [P, I, P, I64, I64, I, I64, P, I64, P, P, I64, I64, I64, I64, F, I, I64, P, I, P,
+                                  I64, I64, P, P, I64, P]),
     "kh_safetensors_open": (I, [S, PP]),
     "kh_safetensors_close": (I, [P]),
     "kh_safetensors_count": (I, [P, C.POINTER(I64)]),

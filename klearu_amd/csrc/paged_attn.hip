@@ -1,0 +1,654 @@
+// paged_attn.hip -- attention over the paged 4-bit cache (gfx950).
+//
+// For row i of a sequence with n new rows and L cached positions (the new rows'
+// own among them), at position p = L - n + i:
+//   o = sum_j softmax_j(scale q . k_j) v_j,  lse = log sum_j exp(scale q . k_j)
+// over the positions j that the row sees: j < L, with `causal` j <= p, with a
+// window w also j > p - w.  A row that sees nothing gives 0 and -inf.
+//
+// The codes go into the matrix cores as they are.  A nibble c behind the bits
+// 0x43 is the BF16 number 128 + c, so with group sums A_g = sum_d q_d (128 + c_d)
+//   q . k = sum_g s_g A_g + sum_g (m_g - 128 s_g) Q_g,   Q_g = sum_{d in g} q_d
+// where the second sum is one more product, of the (s, m) pairs as they lie in
+// the page with (-128 Q_g, Q_g) in three BF16 terms.  Values alike, with R the
+// rounded products p_j s_jg that the matrix core takes:
+//   o_d = sum_j R_jg (128 + c_jd) - 128 sum_j R_jg + sum_j p_j m_jg
+// where the rounding of R cancels in the 128s.  The middle sum is one more
+// product with ones, per group: a group that stands for NaN touches no other.
+//
+// Row tiles are 16 rows of one kv head: the queries of its heads, of one
+// sequence.  Scores come out of the matrix core with positions along registers
+// and rows along lanes, which is the layout that the second product takes its P
+// in when the positions of a step are numbered 4 g + i and 16 + 4 g + i; nothing
+// is exchanged between lanes but the running maximum.
+#include <cmath>
+#include <type_traits>
+
+#include "mfma.hpp"
+#include "paged_kv.hpp"
+
+namespace kh {
+
+constexpr int kPaWaves = 4;
+constexpr int kPaStep = 32;        // positions a wave takes at a time
+constexpr int kPaMaxSplit = 128;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+struct PaArgs {
+  const char* pool;
+  int64_t block, pages;
+  int nkv, ps_log2;
+  int* err;
+  const void* q;
+  int64_t qs, qh;
+  const int64_t *off, *len;
+  int64_t batch, rows;
+  const int32_t* table;
+  int64_t cols, table_stride;
+  const int32_t* heads;
+  int nsel, nh, gs;
+  float c1;  // scale * log2(e)
+  int causal;
+  int64_t window;
+  void* out;
+  int64_t os, oh;
+  float* lse;
+  float* part_o;
+  float2* part_ml;
+  int nsplit, tiles;
+  int qvec, ovec;
+};
+
+template <int N>
+__device__ __forceinline__ void ld_words(const char* p, uint32_t (&w)[N]) {
+  if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  }
+}
+
+__device__ __forceinline__ kh_f32x4 mfma16(const uint4& a, const uint4& b, kh_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+}
+
+// Two codes (nibble n of each half of w) as BF16 128 + c.
+__device__ __forceinline__ uint32_t codes2(uint32_t w, int n) { return ((w >> (4 * n)) & 0x000f000fu) | 0x43004300u; }
+
+// Eight f32 in BF16 terms: x = t[0] + t[1] + ... to 8 more bits each.
+template <int NT>
+__device__ __forceinline__ void terms8(const float (&f)[8], uint4 (&t)[NT]) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = f[i];
+#pragma unroll
+  for (int k = 0; k < NT; ++k) {
+    t[k] = make_uint4(cvt_bf16x2(r[0], r[1]), cvt_bf16x2(r[2], r[3]), cvt_bf16x2(r[4], r[5]), cvt_bf16x2(r[6], r[7]));
+    if (k + 1 < NT) {
+      r[0] -= bf16_lo(t[k].x); r[1] -= bf16_hi(t[k].x); r[2] -= bf16_lo(t[k].y); r[3] -= bf16_hi(t[k].y);
+      r[4] -= bf16_lo(t[k].z); r[5] -= bf16_hi(t[k].z); r[6] -= bf16_lo(t[k].w); r[7] -= bf16_hi(t[k].w);
+    }
+  }
+}
+
+__device__ __forceinline__ float across_groups_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float across_groups_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// The lane's value of lane N of its row of sixteen.
+template <int N>
+__device__ __forceinline__ uint32_t row_bcast(uint32_t v) {
+  return (uint32_t)dpp<0x150 + N>((int)v);
+}
+template <int N>
+__device__ __forceinline__ uint32_t quad_bcast(uint32_t v) {
+  return (uint32_t)dpp<N * 0x55>((int)v);
+}
+
+// What a wave holds of 32 positions.
+template <int D>
+struct PaStepData {
+  static constexpr int NG = D / kKvGroup, HN = D / 64;
+  uint32_t kw[2][NG];       // codes of key lane % 16, the lane group's words
+  uint32_t kpa[2][NG];      // pairs of that key
+  uint32_t kpc[2][NG];      // pairs of key 4 g + lane % 4
+  uint32_t vw[2][2 * HN];   // codes of positions 4 g .. 4 g + 3
+  uint32_t vp[2][2];        // row lane % (2 NG) of the value pairs, those positions
+};
+
+template <int D>
+__device__ __forceinline__ void pa_load(const PaArgs& a, int64_t pg0, int64_t pg1, int tok, int h, int ps, int lane,
+                                        PaStepData<D>& x) {
+  using P = KvParts<D>;
+  constexpr int NG = D / kKvGroup, HN = D / 64;
+  const int g = lane >> 4, r = lane & 15, in = tok & (ps - 1);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const char* blk = a.pool + ((t ? pg1 : pg0) * a.nkv + h) * a.block;
+    const int t0 = ps == 16 ? 0 : in + 16 * t;
+    ld_words<NG>(blk + P::kc() + (t0 + r) * (D / 2) + g * NG * 4, x.kw[t]);
+    ld_words<NG>(blk + P::kp(ps) + (t0 + r) * NG * 4, x.kpa[t]);
+    ld_words<NG>(blk + P::kp(ps) + (t0 + 4 * g + (lane & 3)) * NG * 4, x.kpc[t]);
+    ld_words<2 * HN>(blk + P::vc(ps) + (((t0 >> 2) + g) * 16 + r) * (HN * 8), x.vw[t]);
+    ld_words<2>(blk + P::vp(ps) + ((r & (2 * NG - 1)) * ps + t0 + 4 * g) * 2, x.vp[t]);
+  }
+}
+
+// Whether head h of row t is in the row's list; every lane of the wave takes part.
+__device__ __forceinline__ bool pa_selected(const PaArgs& a, int64_t t, int h, int lane) {
+  for (int j0 = 0; j0 < a.nsel; j0 += 64) {
+    const bool hit = j0 + lane < a.nsel && a.heads[t * a.nsel + j0 + lane] == h;
+    if (__ballot(hit)) return true;
+  }
+  return false;
+}
+
+template <int D, typename T>
+__device__ __forceinline__ void pa_store4(T* y, bool vec, float a, float b, float c, float d) {
+  if constexpr (sizeof(T) == 4) {
+    if (vec) {
+      *reinterpret_cast<float4*>(y) = make_float4(a, b, c, d);
+      return;
+    }
+  } else {
+    if (vec) {
+      *reinterpret_cast<uint2*>(y) = make_uint2(cvt_bf16x2(a, b), cvt_bf16x2(c, d));
+      return;
+    }
+  }
+  store_f32(y, a);
+  store_f32(y + 1, b);
+  store_f32(y + 2, c);
+  store_f32(y + 3, d);
+}
+
+// Block: one row tile of one (sequence, kv head), one of nsplit parts of the
+// positions that the tile sees; its waves take every fourth step of 32.
+template <int D, typename T>
+__global__ __launch_bounds__(64 * kPaWaves) void paged_rows_kernel(PaArgs a) {
+  constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16;
+  constexpr int NQ = sizeof(T) == 4 ? 3 : 1;  // terms of q: all of its bits
+  constexpr int NP = sizeof(T) == 4 ? 3 : 1;  // of P: all of its bits for f32 rows, 8 for BF16 ones, as their output
+  __shared__ float s_m[kPaWaves][16], s_l[kPaWaves][16];
+  __shared__ __align__(16) float s_o[2][16 * D];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
+  int64_t id = blockIdx.x;
+  const int split = (int)(id % a.nsplit);
+  id /= a.nsplit;
+  const int tile0 = (int)(id % a.tiles);
+  id /= a.tiles;
+  const int h = (int)(id % a.nkv);
+  const int64_t b = id / a.nkv;
+  const int ps = 1 << a.ps_log2;
+  const uint32_t odd = (col & 1) ? 0xffffffffu : 0u;
+  int64_t o0 = a.off[b], o1 = a.off[b + 1];
+  o0 = o0 < 0 ? 0 : o0;
+  o1 = o1 > a.rows ? a.rows : o1;
+  if (o1 <= o0) return;
+  const int64_t n = o1 - o0, nr = n * a.gs;
+  const int64_t cap = a.cols << a.ps_log2;
+  int64_t L = a.len[b];
+  if (L < 0 || L > cap) {
+    if (threadIdx.x == 0) atomicOr(a.err, 1);
+    L = L < 0 ? 0 : cap;
+  }
+  const int32_t* __restrict__ table = a.table + b * a.table_stride;
+
+  for (int64_t tile = tile0; tile * 16 < nr; tile += a.tiles) {
+    // the lane's row (column of the products)
+    const int64_t rr = tile * 16 + col;
+    const bool inside = rr < nr;
+    const int64_t i = (inside ? rr : 0) / a.gs, t = o0 + i;
+    const int head = h * a.gs + (int)((inside ? rr : 0) - i * a.gs);
+    bool on = inside;
+    if (a.heads) {
+      uint64_t sel = 0;
+      for (int c = 0; c < 16; ++c) {
+        const int64_t cr = tile * 16 + c;
+        if (cr >= nr) break;
+        const int64_t ci = cr / a.gs;
+        if (pa_selected(a, o0 + ci, h * a.gs + (int)(cr - ci * a.gs), lane)) sel |= 1ull << c;
+      }
+      on = on && (sel >> col & 1);
+    }
+    int lo = 0, hi = 0;
+    if (on) {
+      const int64_t p = L - n + i;
+      const int64_t e = a.causal ? (p + 1 < L ? p + 1 : L) : L;
+      const int64_t s = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
+      if (e > s) lo = (int)s, hi = (int)e;
+    }
+    const bool some = hi > lo;
+    // the tile's range, and the part of it that every row sees (the rows that see anything)
+    const int tlo = (int)wave_min_u32(some ? (uint32_t)lo : 0x7fffffffu);
+    const int thi = (int)wave_max_u32(some ? (uint32_t)hi : 0u);
+    const int all_lo = (int)wave_max_u32(some ? (uint32_t)lo : 0u);
+    const int all_hi = (int)wave_min_u32(some ? (uint32_t)hi : 0x7fffffffu);
+
+    float m = -INFINITY, l = 0.0f;
+    kh_f32x4 o[NF], om, os[NG];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) o[f] = kh_f32x4{0, 0, 0, 0};
+    om = kh_f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < NG; ++j) os[j] = kh_f32x4{0, 0, 0, 0};
+
+    const int first = tlo / kPaStep, steps = thi > tlo ? (thi + kPaStep - 1) / kPaStep - first : 0;
+    const int per = (steps + a.nsplit - 1) / a.nsplit;
+    const int sb = first + split * per, se = min(first + steps, sb + per);
+    if (sb < se) {
+      // q as the second operand: slots (0,4,1,5,2,6,3,7) of eight neighbouring
+      // elements, the order in which codes2 takes the nibbles of a word
+      uint4 qf[NG][NQ];
+      uint4 qm[(NG + 3) / 4];
+      {
+        float qsum[NG];
+        const T* q = static_cast<const T*>(a.q) + t * a.qs + head * a.qh;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          float f[8];
+          load8(q + 32 * j + 8 * g, a.qvec, f);
+          const float e[8] = {f[0], f[4], f[1], f[5], f[2], f[6], f[3], f[7]};
+          terms8<NQ>(e, qf[j]);
+          qsum[j] = across_groups_sum(((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7])));
+        }
+#pragma unroll
+        for (int k = 0; k < (NG + 3) / 4; ++k) {
+          float e[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float s = 4 * k + j < NG ? qsum[4 * k + j < NG ? 4 * k + j : 0] : 0.0f;
+            e[2 * j] = -128.0f * s;
+            e[2 * j + 1] = s;
+          }
+          uint4 tm[3];
+          terms8<3>(e, tm);
+          const uint4 z = make_uint4(0, 0, 0, 0);
+          qm[k] = g == 0 ? tm[0] : g == 1 ? tm[1] : g == 2 ? tm[2] : z;
+        }
+      }
+
+      const auto page = [&](int tok) -> int64_t {
+        const int c = min(tok >> a.ps_log2, (int)a.cols - 1);
+        return table[__builtin_amdgcn_readfirstlane(c)];
+      };
+      const auto clean = [&](int64_t pg, bool* ok) -> int64_t {
+        *ok = pg >= 0 && pg < a.pages;
+        if (*ok) return pg;
+        if (lane == 0) atomicOr(a.err, 2);
+        return 0;
+      };
+      const auto step = [&](const PaStepData<D>& x, int tok, bool ok0, bool ok1) {
+        const bool whole = tok >= all_lo && tok + kPaStep <= all_hi && ok0 && ok1;
+        // scores: positions 16 t + 4 g + r along registers, rows along lanes
+        float s[2][4];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+          kh_f32x4 base = {0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < (NG + 3) / 4; ++k) {
+            uint4 av;
+            if constexpr (NG == 2) av = make_uint4(x.kpa[tt][0], x.kpa[tt][1], 0, 0);
+            else av = make_uint4(x.kpa[tt][4 * k], x.kpa[tt][4 * k + 1], x.kpa[tt][4 * k + 2], x.kpa[tt][4 * k + 3]);
+            base = mfma16(av, qm[k], base);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[tt][r] = base[r];
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            const uint32_t w = x.kw[tt][j];
+            const uint4 kf = make_uint4(codes2(w, 0), codes2(w, 1), codes2(w, 2), codes2(w, 3));
+            kh_f32x4 c = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = NQ - 1; k >= 0; --k) c = mfma16(kf, qf[j][k], c);
+            const uint32_t pr = x.kpc[tt][j];
+            s[tt][0] = fmaf(__uint_as_float(quad_bcast<0>(pr) << 16), c[0], s[tt][0]);
+            s[tt][1] = fmaf(__uint_as_float(quad_bcast<1>(pr) << 16), c[1], s[tt][1]);
+            s[tt][2] = fmaf(__uint_as_float(quad_bcast<2>(pr) << 16), c[2], s[tt][2]);
+            s[tt][3] = fmaf(__uint_as_float(quad_bcast<3>(pr) << 16), c[3], s[tt][3]);
+          }
+        }
+        bool see[2][4];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            s[tt][r] *= a.c1;
+            if (!whole) {
+              const int j = tok + 16 * tt + 4 * g + r;
+              see[tt][r] = j >= lo && j < hi && (tt ? ok1 : ok0);
+              if (!see[tt][r]) s[tt][r] = -INFINITY;
+            }
+            mx = fmaxf(mx, s[tt][r]);
+          }
+        const float mn = fmaxf(m, across_groups_max(mx));
+        const float mu = mn == -INFINITY ? 0.0f : mn;
+        if (__ballot(mn != m)) {
+          const float alpha = __builtin_amdgcn_exp2f(m - mu);
+          l *= alpha;
+          om *= alpha;
+#pragma unroll
+          for (int j = 0; j < NG; ++j) os[j] *= alpha;
+#pragma unroll
+          for (int f = 0; f < NF; ++f) o[f] *= alpha;
+          m = mn;
+        }
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - mu);
+        l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+
+        uint4 pt[NP];
+        terms8<NP>(p, pt);
+        const uint4 vm = make_uint4(x.vp[0][0] & odd, x.vp[0][1] & odd, x.vp[1][0] & odd, x.vp[1][1] & odd);
+#pragma unroll
+        for (int k = NP - 1; k >= 0; --k) om = mfma16(vm, pt[k], om);
+
+        const auto group = [&](auto G) {
+          constexpr int gi = decltype(G)::value;
+          float ps8[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t w = row_bcast<2 * gi>(x.vp[e >> 1][e & 1]);
+            ps8[2 * e] = p[2 * e] * __uint_as_float(w << 16);
+            ps8[2 * e + 1] = p[2 * e + 1] * __uint_as_float(w & 0xffff0000u);
+          }
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ps8[e] = see[e >> 2][e & 3] ? ps8[e] : 0.0f;
+          }
+          uint4 pg[NP];
+          terms8<NP>(ps8, pg);
+          const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+#pragma unroll
+          for (int k = NP - 1; k >= 0; --k) os[gi] = mfma16(ones, pg[k], os[gi]);
+#pragma unroll
+          for (int ff = 0; ff < 2; ++ff) {
+            const int f = 2 * gi + ff, hf = f >> 2, nb = f & 3;
+            const uint4 vf = make_uint4(codes2(x.vw[0][hf], nb), codes2(x.vw[0][HN + hf], nb),
+                                        codes2(x.vw[1][hf], nb), codes2(x.vw[1][HN + hf], nb));
+#pragma unroll
+            for (int k = NP - 1; k >= 0; --k) o[f] = mfma16(vf, pg[k], o[f]);
+          }
+        };
+        group(std::integral_constant<int, 0>{});
+        group(std::integral_constant<int, 1>{});
+        if constexpr (NG >= 4) {
+          group(std::integral_constant<int, 2>{});
+          group(std::integral_constant<int, 3>{});
+        }
+        if constexpr (NG >= 8) {
+          group(std::integral_constant<int, 4>{});
+          group(std::integral_constant<int, 5>{});
+          group(std::integral_constant<int, 6>{});
+          group(std::integral_constant<int, 7>{});
+        }
+      };
+
+      for (int st = sb + wave; st < se; st += kPaWaves) {
+        const int tok = st * kPaStep;
+        // a half of the step that no row of the tile sees takes the other half's page:
+        // the table need not name one there
+        bool ok0, ok1;
+        const int64_t pg0 = clean(page(tok + 16 <= tlo ? tok + 16 : tok), &ok0);
+        const int64_t pg1 = clean(page(tok + 16 >= thi ? tok : tok + 16), &ok1);
+        PaStepData<D> x;
+        pa_load<D>(a, pg0, pg1, tok, h, ps, lane, x);
+        step(x, tok, ok0, ok1);
+      }
+    }
+
+    // -128 sum R + sum p m: row 2 j + 1 of om lies with lane group j / 2
+    l = across_groups_sum(l);
+    {
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi) {
+        const float c = __shfl((gi & 1) ? om[3] : om[1], (gi >> 1) * 16 + col) - 128.0f * os[gi][0];
+#pragma unroll
+        for (int ff = 0; ff < 2; ++ff)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[2 * gi + ff][r] += c;
+      }
+    }
+    // the four waves' parts, joined in a fixed order
+    if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l;
+    __syncthreads();
+    float M = s_m[0][col];
+#pragma unroll
+    for (int w = 1; w < kPaWaves; ++w) M = fmaxf(M, s_m[w][col]);
+    const float Mu = M == -INFINITY ? 0.0f : M;
+    float tot = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kPaWaves; ++w) tot += s_l[w][col] * __builtin_amdgcn_exp2f(s_m[w][col] - Mu);
+    const float fac = __builtin_amdgcn_exp2f(m - Mu);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) o[f] *= fac;
+#pragma unroll
+    for (int half = 2; half >= 1; half >>= 1) {
+      if (wave >= half && wave < 2 * half) {
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+          *reinterpret_cast<kh_f32x4*>(&s_o[wave - half][(f * 64 + lane) * 4]) = o[f];
+      }
+      __syncthreads();
+      if (wave < half) {
+#pragma unroll
+        for (int f = 0; f < NF; ++f) o[f] += *reinterpret_cast<const kh_f32x4*>(&s_o[wave][(f * 64 + lane) * 4]);
+      }
+      if (half == 2) __syncthreads();
+    }
+    if (wave == 0 && inside) {
+      const int64_t row = t * a.nh + head;
+      if (a.nsplit > 1) {
+        const int64_t at = row * a.nsplit + split;
+        if (g == 0) a.part_ml[at] = make_float2(some ? M : -INFINITY, some ? tot : 0.0f);
+        if (some && sb < se) {
+#pragma unroll
+          for (int f = 0; f < NF; ++f)
+            *reinterpret_cast<float4*>(a.part_o + at * D + 16 * f + 4 * g) = make_float4(o[f][0], o[f][1], o[f][2], o[f][3]);
+        }
+      } else {
+        const bool any = some && (M != -INFINITY || tot != 0.0f);  // NaN scores leave M behind
+        T* y = static_cast<T*>(a.out) + t * a.os + head * a.oh + 4 * g;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = any ? o[f][r] / tot : 0.0f;
+          pa_store4<D, T>(y + 16 * f, a.ovec, v[0], v[1], v[2], v[3]);
+        }
+        if (a.lse && g == 0) a.lse[row] = any ? kLn2 * (M + __builtin_amdgcn_logf(tot)) : -INFINITY;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Joins the parts of each row: one wave a (row, head), D / 64 elements a lane.
+template <int D, typename T>
+__global__ __launch_bounds__(256) void paged_join_kernel(PaArgs a) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t t = row / a.nh;
+  if (t >= a.rows || t < a.off[0] || t >= a.off[a.batch]) return;
+  const int head = (int)(row - t * a.nh);
+  const float2* __restrict__ ml = a.part_ml + row * a.nsplit;
+  float2 x[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    x[k] = lane + 64 * k < a.nsplit ? ml[lane + 64 * k] : make_float2(-INFINITY, 0.0f);
+  const float M = wave_max(fmaxf(x[0].x, x[1].x)), Mu = M == -INFINITY ? 0.0f : M;
+  float w[2], tot = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    w[k] = __builtin_amdgcn_exp2f(x[k].x - Mu);
+    tot += w[k] * x[k].y;
+  }
+  tot = wave_sum(tot);
+  // parts without a key were not written; where NaN scores left no maximum, tot is NaN
+  float acc[E] = {};
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float ws = __shfl(s < 64 ? w[0] : w[1], s & 63);
+    const float ms = __shfl(s < 64 ? x[0].x : x[1].x, s & 63);
+    if (ms == -INFINITY) continue;
+    const float* __restrict__ p = a.part_o + (row * a.nsplit + s) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(ws, p[e], acc[e]);
+  }
+  const bool any = M != -INFINITY || tot != 0.0f;
+  T* y = static_cast<T*>(a.out) + t * a.os + head * a.oh + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) store_f32(y + e, any ? acc[e] / tot : 0.0f);
+  if (a.lse && lane == 0) a.lse[row] = any ? kLn2 * (M + __builtin_amdgcn_logf(tot)) : -INFINITY;
+}
+
+// How a call is cut: row tiles per (sequence, kv head) as the caller expects
+// them, and parts along the positions when the tiles alone do not fill the chip.
+struct PaPlan {
+  int64_t tiles, base;
+  int nsplit;
+};
+static PaPlan pa_plan(int nkv, int nh, int64_t rows, int64_t batch, int64_t max_rows, int64_t max_len) {
+  PaPlan p;
+  const int64_t gs = nh / nkv;
+  if (max_rows > rows) max_rows = rows;
+  p.tiles = (max_rows * gs + 15) / 16;
+  if (p.tiles < 1) p.tiles = 1;
+  if (p.tiles > 65536) p.tiles = 65536;
+  p.base = batch * nkv * p.tiles;
+  int64_t want = p.base >= 1024 ? 1 : (2048 + p.base - 1) / p.base;
+  const int64_t most = (max_len + 255) / 256;
+  if (want > most) want = most;
+  if (want > kPaMaxSplit) want = kPaMaxSplit;
+  p.nsplit = want < 1 ? 1 : (int)want;
+  return p;
+}
+static int64_t pa_bytes(const PaPlan& p, int64_t rows, int nh, int d) {
+  return p.nsplit > 1 ? rows * nh * p.nsplit * (int64_t)(4 * d + 8) : 0;
+}
+
+template <int D, typename T>
+static void pa_launch(const PaArgs& a, int64_t blocks, hipStream_t st) {
+  hipLaunchKernelGGL((paged_rows_kernel<D, T>), dim3((unsigned)blocks), dim3(64 * kPaWaves), 0, st, a);
+  if (a.nsplit > 1)
+    hipLaunchKernelGGL((paged_join_kernel<D, T>), dim3((unsigned)((a.rows * a.nh + 3) / 4)), dim3(256), 0, st, a);
+}
+template <typename T>
+static void pa_launch_d(int d, const PaArgs& a, int64_t blocks, hipStream_t st) {
+  if (d == 64) pa_launch<64, T>(a, blocks, st);
+  else if (d == 128) pa_launch<128, T>(a, blocks, st);
+  else pa_launch<256, T>(a, blocks, st);
+}
+
+static int pa_shape(const kh_paged_kv* c, int dtype, int64_t rows, int64_t batch, int num_heads, int64_t max_rows,
+                    int64_t max_len) {
+  KH_CHECK_ARG(c != nullptr, "null handle");
+  KH_CHECK_ARG(dtype == KH_DT_F32 || dtype == KH_DT_BF16, "dtype %d: f32 and BF16 are supported", dtype);
+  KH_CHECK_ARG(rows >= 0 && rows < (int64_t)1 << 31 && batch >= 0 && batch < (int64_t)1 << 31,
+               "rows %lld, batch %lld not in [0,2^31)", (long long)rows, (long long)batch);
+  KH_CHECK_ARG(num_heads >= c->nkv && num_heads % c->nkv == 0 && num_heads <= 65536,
+               "num_heads %d is no multiple of the cache's %d", num_heads, c->nkv);
+  KH_CHECK_ARG(max_rows >= 0 && max_len >= 0, "max_rows %lld, max_len %lld", (long long)max_rows, (long long)max_len);
+  return KH_OK;
+}
+
+}  // namespace kh
+
+using namespace kh;
+
+extern "C" int kh_paged_kv_attention_workspace(const kh_paged_kv* c, int dtype, int64_t rows, int64_t batch,
+                                               int num_heads, int64_t max_rows, int64_t max_len, int64_t* bytes) {
+  KH_CHECK_ARG(bytes != nullptr, "null output");
+  const int rc = pa_shape(c, dtype, rows, batch, num_heads, max_rows, max_len);
+  if (rc != KH_OK) return rc;
+  *bytes = rows && batch ? pa_bytes(pa_plan(c->nkv, num_heads, rows, batch, max_rows, max_len), rows, num_heads, c->d)
+                         : 0;
+  return KH_OK;
+}
+
+extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void* q_dev, int64_t q_row_stride,
+                                     int64_t q_head_stride, int num_heads, int64_t rows, const int64_t* off_dev,
+                                     int64_t batch, const int64_t* len_dev, const int32_t* table_dev,
+                                     int64_t table_cols, int64_t table_stride, int64_t max_rows, int64_t max_len,
+                                     float scale, int causal, int64_t window, const int32_t* heads_dev, int n_heads,
+                                     void* out_dev, int64_t out_row_stride, int64_t out_head_stride, float* lse_dev,
+                                     void* ws_dev, int64_t ws_bytes, void* stream) {
+  int rc = pa_shape(c, dtype, rows, batch, num_heads, max_rows, max_len);
+  if (rc != KH_OK) return rc;
+  KH_CHECK_ARG(table_cols >= 1 && table_stride >= table_cols, "page table of %lld columns, %lld apart",
+               (long long)table_cols, (long long)table_stride);
+  KH_CHECK_ARG((table_cols << c->ps_log2) <= INT32_MAX - 64, "a page table of %lld columns holds 2^31 positions",
+               (long long)table_cols);
+  KH_CHECK_ARG(std::isfinite(scale) && scale > 0, "scale must be positive and finite");
+  KH_CHECK_ARG(window >= 0 && (window == 0 || causal), "a window (%lld) needs causal attention", (long long)window);
+  KH_CHECK_ARG(q_row_stride >= 0 && q_head_stride >= 0, "negative stride");
+  KH_CHECK_ARG(n_heads >= 0 && n_heads <= 4 * num_heads, "n_heads %d not in [0,%d]", n_heads, 4 * num_heads);
+  KH_CHECK_ARG(strides_disjoint(rows, out_row_stride, num_heads, out_head_stride, c->d),
+               "output strides (%lld, %lld) let heads overlap", (long long)out_row_stride,
+               (long long)out_head_stride);
+  if (rows == 0 || batch == 0) return KH_OK;
+  KH_CHECK_ARG(q_dev && off_dev && len_dev && table_dev && out_dev, "null argument");
+  KH_CHECK_ARG(heads_dev || n_heads == 0, "null head list");
+  const PaPlan p = pa_plan(c->nkv, num_heads, rows, batch, max_rows, max_len);
+  const int64_t need = pa_bytes(p, rows, num_heads, c->d);
+  if (need > 0 && (!ws_dev || ws_bytes < need)) {
+    set_error("the workspace holds %lld bytes, %lld are needed", (long long)(ws_dev ? ws_bytes : 0),
+              (long long)need);
+    return KH_ERR_CAPACITY;
+  }
+  KH_CHECK_ARG((reinterpret_cast<uintptr_t>(ws_dev) & 15) == 0, "the workspace must be 16-byte aligned");
+  const int64_t blocks = p.base * p.nsplit;
+  KH_CHECK_ARG(blocks < (int64_t)1 << 31 && rows * num_heads < (int64_t)1 << 33, "too many rows for one call");
+  KH_ON_DEVICE(c->device, "the cache");
+  PaArgs a;
+  a.pool = c->pool;
+  a.block = c->block;
+  a.pages = c->pages;
+  a.nkv = c->nkv;
+  a.ps_log2 = c->ps_log2;
+  a.err = c->err;
+  a.q = q_dev;
+  a.qs = q_row_stride;
+  a.qh = q_head_stride;
+  a.off = off_dev;
+  a.len = len_dev;
+  a.batch = batch;
+  a.rows = rows;
+  a.table = table_dev;
+  a.cols = table_cols;
+  a.table_stride = table_stride;
+  a.heads = heads_dev;
+  a.nsel = n_heads;
+  a.nh = num_heads;
+  a.gs = num_heads / c->nkv;
+  a.c1 = scale * kLog2e;
+  a.causal = causal ? 1 : 0;
+  a.window = window;
+  a.out = out_dev;
+  a.os = out_row_stride;
+  a.oh = out_head_stride;
+  a.lse = lse_dev;
+  a.nsplit = p.nsplit;
+  a.tiles = (int)p.tiles;
+  a.part_o = static_cast<float*>(ws_dev);
+  a.part_ml = need ? reinterpret_cast<float2*>(a.part_o + rows * num_heads * p.nsplit * c->d) : nullptr;
+  a.qvec = aligned16(q_dev, dtype, q_row_stride, q_head_stride) ? 1 : 0;
+  a.ovec = aligned16(out_dev, dtype, out_row_stride, out_head_stride) ? 1 : 0;
+  if (dtype == KH_DT_F32) pa_launch_d<float>(c->d, a, blocks, as_stream(stream));
+  else pa_launch_d<uint16_t>(c->d, a, blocks, as_stream(stream));
+  KH_LAUNCHED();
+  return KH_OK;
+}

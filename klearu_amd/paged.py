@@ -1,0 +1,288 @@
+"""Rotary positions, and a paged K/V cache held in 4 bits with the attention that reads it.
+
+The framework's decode step (attention.SparseAttention) keeps a contiguous cache per sequence in
+BF16 / f32 and rotates inside the step.  Here the cache is a pool of pages that sequences share,
+5 bits a value (include/klearu_hip.h has the format), rows are put in with their rotation on the
+way, and attention takes any number of rows per sequence: prompts, chunks of them, single tokens.
+
+    rope = Rope(128, max_pos=32768)
+    cache = PagedKv(num_kv_heads=8, head_dim=128, num_pages=4096)
+    cache.append(k, v, off, start, table, rope=rope)     # rows off[b]..off[b+1]-1 -> start[b], ...
+    q = rope.apply(q, pos)
+    y = cache.attention(q, off, start + n_new, table)
+
+All compute runs in libklearu_hip.so on the current torch stream of the tensors' device (or
+`stream`).  Rows are tensors [rows, heads, head_dim], f32 or bfloat16, of any non-negative strides
+but 1 along the last dimension.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+HALF, INTERLEAVED = 0, 1
+SCALE_NONE, SCALE_LINEAR, SCALE_BASE, SCALE_BY_PARTS = 0, 1, 2, 3
+
+_DT = {torch.float32: 0, torch.bfloat16: 2}
+
+
+def _rows(t: torch.Tensor, what: str, device, dtype=None):
+    """(pointer, row stride, head stride, dtype code) of a tensor [rows, heads, head_dim]."""
+    if not t.is_cuda:
+        raise ValueError(f"{what}: expected a device tensor")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the handle on {device}")
+    if t.dim() != 3:
+        raise ValueError(f"{what}: expected [rows, heads, head_dim], got {tuple(t.shape)}")
+    code = _DT.get(t.dtype)
+    if code is None or (dtype is not None and t.dtype != dtype):
+        raise TypeError(f"{what}: dtype {t.dtype}, expected {dtype or 'float32 or bfloat16'}")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 and t.shape[2] > 1 and t.numel():
+        raise ValueError(f"{what}: the elements of a head must be contiguous")
+    return t.data_ptr(), s0, s1, code
+
+
+def _index(t: torch.Tensor, what: str, device, dtype, shape):
+    """Pointer of a contiguous index tensor of a given dtype and shape."""
+    if not t.is_cuda:
+        raise ValueError(f"{what}: expected a device tensor")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the handle on {device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: dtype {t.dtype}, expected {dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous tensor")
+    return t.data_ptr()
+
+
+def _table(t: torch.Tensor, device, batch):
+    """(pointer, columns, row stride) of an int32 page table [batch, columns]."""
+    if not t.is_cuda:
+        raise ValueError("table: expected a device tensor")
+    if t.device != device:
+        raise ValueError(f"table is on {t.device}, the handle on {device}")
+    if t.dtype != torch.int32:
+        raise TypeError(f"table: dtype {t.dtype}, expected torch.int32")
+    if t.dim() != 2 or t.shape[0] != batch:
+        raise ValueError(f"table: shape {tuple(t.shape)}, expected [{batch}, columns]")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError("table: the columns of a row must be contiguous")
+    return t.data_ptr(), t.shape[1], max(t.stride(0), t.shape[1]) if batch <= 1 else t.stride(0)
+
+
+class _On:
+    """The handle's device and `stream` (None: the current one) made current, where they are not."""
+
+    __slots__ = ("ctx",)
+
+    def __init__(self, device, stream):
+        self.ctx = []
+        if torch.cuda.current_device() != device.index:
+            self.ctx.append(torch.cuda.device(device))
+        if stream is not None:
+            if stream.device != device:
+                raise ValueError(f"stream is on {stream.device}, the handle on {device}")
+            self.ctx.append(torch.cuda.stream(stream))
+
+    def __enter__(self):
+        for c in self.ctx:
+            c.__enter__()
+
+    def __exit__(self, *e):
+        for c in reversed(self.ctx):
+            c.__exit__(*e)
+
+
+class _Handle:
+    _destroy = ""
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h:
+            try:
+                getattr(_lib.load(), self._destroy)(h)
+            except Exception:
+                pass
+
+    def _adopt(self, h):
+        self._h = h
+        self.device = torch.device("cuda", torch.cuda.current_device())
+
+    def _call(self, stream, fn, *inputs):
+        """fn(stream pointer) with the handle's device and the stream current: results are
+        allocated there, so their memory is the stream's, and the inputs' memory is not given
+        to others before the stream has passed."""
+        if stream is None and torch.cuda.current_device() == self.device.index:
+            return fn(torch.cuda.current_stream().cuda_stream)
+        with _On(self.device, stream):
+            for t in inputs:
+                if t is not None and stream is not None:
+                    t.record_stream(stream)
+            return fn(torch.cuda.current_stream().cuda_stream)
+
+
+class Rope(_Handle):
+    """Rotation of the first `rot_dim` elements of heads by positions 0 .. max_pos - 1.
+
+    layout HALF rotates element i with i + rot_dim / 2 (crates/klearu-llm/src/model/rope.rs:75-87),
+    INTERLEAVED 2 i with 2 i + 1.  Frequencies theta^(-2 i / rot_dim) are stretched for contexts
+    longer than the trained one by `factor`: SCALE_LINEAR all of them, SCALE_BASE through theta,
+    SCALE_BY_PARTS those that turn less than `low` times over `original_len` positions, those
+    over `high` turns not, in between in proportion.  `magnitude` scales the rotated elements."""
+
+    _destroy = "kh_rope_destroy"
+
+    def __init__(self, rot_dim, max_pos, layout=HALF, theta=10000.0, scaling=SCALE_NONE, factor=1.0, original_len=0,
+                 low=1.0, high=32.0, magnitude=1.0):
+        h = C.c_void_p()
+        _lib.call("kh_rope_create", rot_dim, max_pos, layout, theta, scaling, factor, original_len, low, high,
+                  magnitude, C.byref(h))
+        self._adopt(h)
+        self.rot_dim, self.max_pos, self.layout = rot_dim, max_pos, layout
+
+    def apply(self, x: torch.Tensor, pos: torch.Tensor, out: torch.Tensor | None = None, transpose: bool = False,
+              stream=None) -> torch.Tensor:
+        """x [rows, heads, head_dim] rotated by pos [rows] (int64), into `out` (x itself rotates in
+        place) or a new tensor.  `transpose` takes gradients back: the transposed rotation.  Rows of
+        a negative position are padding and left as they were, as are (reported by status()) rows
+        past max_pos; in a new tensor those hold no value."""
+        xp, x0, x1, dt = _rows(x, "x", self.device)
+        n, heads, dim = x.shape
+        pp = _index(pos, "pos", self.device, torch.int64, (n,))
+        if out is not None and out.shape != x.shape:
+            raise ValueError(f"out: shape {tuple(out.shape)}, expected {tuple(x.shape)}")
+
+        def go(s):
+            y = out if out is not None else torch.empty((n, heads, dim), dtype=x.dtype, device=x.device)
+            yp, y0, y1, _ = _rows(y, "out", self.device, x.dtype)
+            _lib.call("kh_rope_apply", self._h, dt, xp, x0, x1, n, heads, dim, pp, yp, y0, y1, 1 if transpose else 0,
+                      s)
+            return y
+
+        return self._call(stream, go, x, pos, out)
+
+    def status(self):
+        """Raise KlearuError (KH_ERR_ARG) if a call since the last check met a position past max_pos."""
+        self._call(None, lambda s: _lib.call("kh_rope_status", self._h))
+
+
+class PagedKv(_Handle):
+    """num_pages pages of page_size positions of every kv head, keys and values in 4 bits.
+
+    A page table [batch, columns] (int32) names each sequence's pages, and off [batch + 1] (int64)
+    the rows of a call that are its own: off[b] .. off[b + 1] - 1.  Rows outside are padding.
+    Which page is whose is the caller's; pages may be shared by sequences that only read them."""
+
+    _destroy = "kh_paged_kv_destroy"
+
+    def __init__(self, num_kv_heads, head_dim, num_pages, page_size=64):
+        h = C.c_void_p()
+        _lib.call("kh_paged_kv_create", num_kv_heads, head_dim, page_size, num_pages, C.byref(h))
+        self._adopt(h)
+        self.num_kv_heads, self.head_dim = num_kv_heads, head_dim
+        self.num_pages, self.page_size = num_pages, page_size
+
+    def _shape(self, t, what, rows):
+        if tuple(t.shape) != (rows, self.num_kv_heads, self.head_dim):
+            raise ValueError(f"{what}: shape {tuple(t.shape)}, expected "
+                             f"({rows}, {self.num_kv_heads}, {self.head_dim})")
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, off: torch.Tensor, start: torch.Tensor, table: torch.Tensor,
+               rope: Rope | None = None, pos: torch.Tensor | None = None, stream=None) -> None:
+        """Row off[b] + i of k and v [rows, num_kv_heads, head_dim] becomes position start[b] + i of
+        sequence b; `rope` rotates the keys on the way, by pos [rows] or by their places in the
+        cache.  Two rows of one call must not have the same place."""
+        n = k.shape[0]
+        kp, k0, k1, dt = _rows(k, "k", self.device)
+        vp, v0, v1, _ = _rows(v, "v", self.device, k.dtype)
+        self._shape(k, "k", n)
+        self._shape(v, "v", n)
+        batch = start.shape[0]
+        op = _index(off, "off", self.device, torch.int64, (batch + 1,))
+        sp = _index(start, "start", self.device, torch.int64, (batch,))
+        tp, cols, ts = _table(table, self.device, batch)
+        if pos is not None and rope is None:
+            raise ValueError("pos: rotary positions without a rotation")
+        pp = None if pos is None else _index(pos, "pos", self.device, torch.int64, (n,))
+        self._call(stream, lambda s: _lib.call(
+            "kh_paged_kv_append", self._h, None if rope is None else rope._h, dt, kp, k0, k1, vp, v0, v1, n, op,
+            batch, sp, pp, tp, cols, ts, s), k, v, off, start, table, pos)
+
+    def gather(self, off: torch.Tensor, start: torch.Tensor, table: torch.Tensor, rows: int,
+               dtype: torch.dtype = torch.float32, k: torch.Tensor | None = None, v: torch.Tensor | None = None,
+               stream=None):
+        """The values that those places hold: (k, v) [rows, num_kv_heads, head_dim], new or given.
+        Rows outside all sequences, or without a place, are left as they were."""
+        batch = start.shape[0]
+        op = _index(off, "off", self.device, torch.int64, (batch + 1,))
+        sp = _index(start, "start", self.device, torch.int64, (batch,))
+        tp, cols, ts = _table(table, self.device, batch)
+        if dtype not in _DT:
+            raise TypeError(f"dtype {dtype}: expected float32 or bfloat16")
+        shape = (rows, self.num_kv_heads, self.head_dim)
+
+        def go(s):
+            a = k if k is not None else torch.empty(shape, dtype=dtype, device=self.device)
+            b = v if v is not None else torch.empty(shape, dtype=dtype, device=self.device)
+            _lib.call("kh_paged_kv_gather", self._h, _DT[dtype], rows, op, batch, sp, tp, cols, ts,
+                      _index(a, "k", self.device, dtype, shape), _index(b, "v", self.device, dtype, shape), s)
+            return a, b
+
+        return self._call(stream, go, off, start, table, k, v)
+
+    def attention(self, q: torch.Tensor, off: torch.Tensor, lens: torch.Tensor, table: torch.Tensor,
+                  scale: float | None = None, causal: bool = True, window: int = 0,
+                  heads: torch.Tensor | None = None, max_rows: int | None = None, max_len: int | None = None,
+                  out: torch.Tensor | None = None, return_lse: bool = False, stream=None):
+        """Attention of q [rows, num_heads, head_dim] over the cache: sequence b holds lens[b]
+        positions, the last of them its rows' own (append first).  scale defaults to
+        head_dim ** -0.5.  heads [rows, n] (int32, SparsityPredictor.select_top_k's lists) leaves
+        the other heads 0.  max_rows and max_len guess the most rows and the longest length of a
+        sequence (default: an even share of the rows, the table's reach); wrong guesses cost
+        time only.  Returns out, or (out, lse) with lse [rows, num_heads] f32: a row that sees nothing
+        gives 0 and -inf."""
+        n, nh = q.shape[0], q.shape[1] if q.dim() == 3 else 0
+        qp, q0, q1, dt = _rows(q, "q", self.device)
+        if q.shape[2] != self.head_dim:
+            raise ValueError(f"q: head_dim {q.shape[2]}, expected {self.head_dim}")
+        batch = lens.shape[0]
+        op = _index(off, "off", self.device, torch.int64, (batch + 1,))
+        lp = _index(lens, "lens", self.device, torch.int64, (batch,))
+        tp, cols, ts = _table(table, self.device, batch)
+        if out is not None and out.shape != q.shape:
+            raise ValueError(f"out: shape {tuple(out.shape)}, expected {tuple(q.shape)}")
+        hp, nsel = None, 0
+        if heads is not None:
+            nsel = heads.shape[-1]
+            hp = _index(heads, "heads", self.device, torch.int32, (n, nsel)) or op  # an empty list is no list of all
+        if max_rows is None:
+            max_rows = -(-n // max(1, batch))
+        if max_len is None:
+            max_len = cols * self.page_size
+        if scale is None:
+            scale = self.head_dim ** -0.5
+        need = C.c_int64()
+        _lib.call("kh_paged_kv_attention_workspace", self._h, dt, n, batch, nh, max_rows, max_len, C.byref(need))
+
+        def go(s):
+            y = out if out is not None else torch.empty((n, nh, self.head_dim), dtype=q.dtype, device=q.device)
+            yp, y0, y1, _ = _rows(y, "out", self.device, q.dtype)
+            ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+            lse = torch.empty((n, nh), dtype=torch.float32, device=q.device) if return_lse else None
+            _lib.call("kh_paged_kv_attention", self._h, dt, qp, q0, q1, nh, n, op, batch, lp, tp, cols, ts, max_rows,
+                      max_len, scale, 1 if causal else 0, window, hp, nsel, yp, y0, y1,
+                      None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), need.value, s)
+            return (y, lse) if return_lse else y
+
+        return self._call(stream, go, q, off, lens, table, heads, out)
+
+    def status(self):
+        """Raise KlearuError (KH_ERR_ARG) if a call since the last check met a place outside its
+        sequence's table, a length the table cannot hold, or a page id outside the pool."""
+        self._call(None, lambda s: _lib.call("kh_paged_kv_status", self._h))
