@@ -7,7 +7,7 @@
 // window w also j > p - w.  A row that sees nothing gives 0 and -inf.
 //
 // The codes go into the matrix cores as they are.  A nibble c behind the bits
-// 0x43 is the BF16 number 128 + c, so with group sums A_g = sum_d q_d (128 + c_d)
+// 0x43 is the BF16 number 128 + c (f32 rows: 16 + c), so with group sums A_g = sum_d q_d (128 + c_d)
 //   q . k = sum_g s_g A_g + sum_g (m_g - 128 s_g) Q_g,   Q_g = sum_{d in g} q_d
 // where the second sum is one more product, of the (s, m) pairs as they lie in
 // the page with (-128 Q_g, Q_g) in three BF16 terms.  Values alike, with R the
@@ -78,8 +78,15 @@ __device__ __forceinline__ kh_f32x4 mfma16(const uint4& a, const uint4& b, kh_f3
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
 }
 
-// Two codes (nibble n of each half of w) as BF16 128 + c.
-__device__ __forceinline__ uint32_t codes2(uint32_t w, int n) { return ((w >> (4 * n)) & 0x000f000fu) | 0x43004300u; }
+// Two codes (nibble n of each half of w) as BF16 numbers BIAS + c: behind the
+// bits 0x43 a nibble counts ones above 128, three bits higher behind 0x418 above
+// 16.  The bias leaves the sums again, with the rounding errors of numbers of its
+// size: f32 rows take 16, which costs a shift more per word.
+template <int BIAS>
+__device__ __forceinline__ uint32_t codes2(uint32_t w, int n) {
+  if constexpr (BIAS == 128) return ((w >> (4 * n)) & 0x000f000fu) | 0x43004300u;
+  return ((n == 0 ? w << 3 : w >> (4 * n - 3)) & 0x00780078u) | 0x41804180u;
+}
 
 // Eight f32 in BF16 terms: x = t[0] + t[1] + ... to 8 more bits each.
 template <int NT>
@@ -97,52 +104,75 @@ __device__ __forceinline__ void terms8(const float (&f)[8], uint4 (&t)[NT]) {
   }
 }
 
+// c plus the two BF16 numbers of w.
+__device__ __forceinline__ float add2(uint32_t w, float c) {
+  typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, w), __builtin_bit_cast(v2, 0x3f803f80u), c, false);
+}
+
+// Over the four lanes of a column, one in each group of sixteen: a row of
+// sixteen is exchanged with its neighbour, then halves of the wave.
+template <typename F>
+__device__ __forceinline__ float across_groups(float v, F f) {
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t w = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ __forceinline__ float across_groups_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  return across_groups(v, [](float x, float y) { return fmaxf(x, y); });
 }
 __device__ __forceinline__ float across_groups_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  return across_groups(v, [](float x, float y) { return x + y; });
 }
 
-// The lane's value of lane N of its row of sixteen.
+// a times the lane's row's (of sixteen) lane N of s; c plus a times the quad's lane N of s.
 template <int N>
-__device__ __forceinline__ uint32_t row_bcast(uint32_t v) {
-  return (uint32_t)dpp<0x150 + N>((int)v);
+__device__ __forceinline__ float mul_row(float a, uint32_t s) {
+  return a * __int_as_float(__builtin_amdgcn_mov_dpp((int)s, 0x150 + N, 0xf, 0xf, true));
 }
 template <int N>
-__device__ __forceinline__ uint32_t quad_bcast(uint32_t v) {
-  return (uint32_t)dpp<N * 0x55>((int)v);
+__device__ __forceinline__ float fma_quad(float a, uint32_t s, float c) {
+  return fmaf(__int_as_float(__builtin_amdgcn_mov_dpp((int)s, N * 0x55, 0xf, 0xf, true)), a, c);
 }
 
-// What a wave holds of 32 positions.
+// What a wave holds of 32 positions, two tiles of 16.
 template <int D>
 struct PaStepData {
   static constexpr int NG = D / kKvGroup, HN = D / 64;
-  uint32_t kw[2][NG];       // codes of key lane % 16, the lane group's words
-  uint32_t kpa[2][NG];      // pairs of that key
-  uint32_t kpc[2][NG];      // pairs of key 4 g + lane % 4
-  uint32_t vw[2][2 * HN];   // codes of positions 4 g .. 4 g + 3
-  uint32_t vp[2][2];        // row lane % (2 NG) of the value pairs, those positions
+  uint32_t kw[2][NG];      // codes of key lane % 16, the lane group's words
+  uint32_t kpa[2][NG];     // pairs of that key
+  uint32_t kpc[2][NG];     // pairs of key 4 g + lane % 4
+  uint32_t vw[2][2 * HN];  // codes of positions 4 g .. 4 g + 3
+  uint32_t vp[2][4];       // pairs of group lane % NG, those positions
 };
 
+// Where a lane's words lie in a block, from the first of 16 positions on.
 template <int D>
-__device__ __forceinline__ void pa_load(const PaArgs& a, int64_t pg0, int64_t pg1, int tok, int h, int ps, int lane,
-                                        PaStepData<D>& x) {
-  using P = KvParts<D>;
-  constexpr int NG = D / kKvGroup, HN = D / 64;
-  const int g = lane >> 4, r = lane & 15, in = tok & (ps - 1);
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const char* blk = a.pool + ((t ? pg1 : pg0) * a.nkv + h) * a.block;
-    const int t0 = ps == 16 ? 0 : in + 16 * t;
-    ld_words<NG>(blk + P::kc() + (t0 + r) * (D / 2) + g * NG * 4, x.kw[t]);
-    ld_words<NG>(blk + P::kp(ps) + (t0 + r) * NG * 4, x.kpa[t]);
-    ld_words<NG>(blk + P::kp(ps) + (t0 + 4 * g + (lane & 3)) * NG * 4, x.kpc[t]);
-    ld_words<2 * HN>(blk + P::vc(ps) + (((t0 >> 2) + g) * 16 + r) * (HN * 8), x.vw[t]);
-    ld_words<2>(blk + P::vp(ps) + ((r & (2 * NG - 1)) * ps + t0 + 4 * g) * 2, x.vp[t]);
+struct PaLane {
+  static constexpr int NG = D / kKvGroup, HN = D / 64;
+  uint32_t kc, kpa, kpc, vc, vp;
+  __device__ __forceinline__ PaLane(int lane, int ps) {
+    using P = KvParts<D>;
+    const int g = lane >> 4, r = lane & 15;
+    kc = P::kc() + r * (D / 2) + g * NG * 4;
+    kpa = P::kp(ps) + r * NG * 4;
+    kpc = P::kp(ps) + (4 * g + (lane & 3)) * NG * 4;
+    vc = P::vc(ps) + (g * 16 + r) * (HN * 8);
+    vp = P::vp(ps) + ((r & (NG - 1)) * ps + 4 * g) * 4;
   }
+};
+
+// Tile T of a step; blk: the block of its positions, in: the first one's place in the page (both the wave's).
+template <int D, int T>
+__device__ __forceinline__ void pa_load(const char* blk, int in, const PaLane<D>& o, PaStepData<D>& x) {
+  constexpr int NG = D / kKvGroup, HN = D / 64;
+  ld_words<NG>(blk + in * (D / 2) + o.kc, x.kw[T]);
+  ld_words<NG>(blk + in * (NG * 4) + o.kpa, x.kpa[T]);
+  ld_words<NG>(blk + in * (NG * 4) + o.kpc, x.kpc[T]);
+  ld_words<2 * HN>(blk + in * (D / 2) + o.vc, x.vw[T]);
+  ld_words<4>(blk + in * 4 + o.vp, x.vp[T]);
 }
 
 // Whether head h of row t is in the row's list; every lane of the wave takes part.
@@ -176,27 +206,28 @@ __device__ __forceinline__ void pa_store4(T* y, bool vec, float a, float b, floa
 // Block: one row tile of one (sequence, kv head), one of nsplit parts of the
 // positions that the tile sees; its waves take every fourth step of 32.
 template <int D, typename T>
-__global__ __launch_bounds__(64 * kPaWaves) void paged_rows_kernel(PaArgs a) {
+__global__ __launch_bounds__(64 * kPaWaves, D == 64 ? 3 : D == 128 ? 2 : 1) void paged_rows_kernel(PaArgs a) {
   constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16;
+  constexpr int BIAS = sizeof(T) == 4 ? 16 : 128;
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1;  // terms of q: all of its bits
   constexpr int NP = sizeof(T) == 4 ? 3 : 1;  // of P: all of its bits for f32 rows, 8 for BF16 ones, as their output
   __shared__ float s_m[kPaWaves][16], s_l[kPaWaves][16];
   __shared__ __align__(16) float s_o[2][16 * D];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
-  int64_t id = blockIdx.x;
-  const int split = (int)(id % a.nsplit);
-  id /= a.nsplit;
-  const int tile0 = (int)(id % a.tiles);
-  id /= a.tiles;
-  const int h = (int)(id % a.nkv);
-  const int64_t b = id / a.nkv;
+  const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t id = blockIdx.x;
+  const int split = (int)(id % (uint32_t)a.nsplit);
+  id /= (uint32_t)a.nsplit;
+  const int tile0 = (int)(id % (uint32_t)a.tiles);
+  id /= (uint32_t)a.tiles;
+  const int h = (int)(id % (uint32_t)a.nkv);
+  const int64_t b = id / (uint32_t)a.nkv;
   const int ps = 1 << a.ps_log2;
-  const uint32_t odd = (col & 1) ? 0xffffffffu : 0u;
   int64_t o0 = a.off[b], o1 = a.off[b + 1];
   o0 = o0 < 0 ? 0 : o0;
   o1 = o1 > a.rows ? a.rows : o1;
   if (o1 <= o0) return;
-  const int64_t n = o1 - o0, nr = n * a.gs;
+  const int n = (int)(o1 - o0), nr = n * a.gs;  // rows x heads of a kv head: below 2^31
   const int64_t cap = a.cols << a.ps_log2;
   int64_t L = a.len[b];
   if (L < 0 || L > cap) {
@@ -205,20 +236,21 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_rows_kernel(PaArgs a) {
   }
   const int32_t* __restrict__ table = a.table + b * a.table_stride;
 
-  for (int64_t tile = tile0; tile * 16 < nr; tile += a.tiles) {
+  const PaLane<D> lo_(lane, ps);
+
+  for (int tile = tile0; tile < (nr + 15) >> 4; tile += a.tiles) {
     // the lane's row (column of the products)
-    const int64_t rr = tile * 16 + col;
+    const int rr = tile * 16 + col;
     const bool inside = rr < nr;
-    const int64_t i = (inside ? rr : 0) / a.gs, t = o0 + i;
-    const int head = h * a.gs + (int)((inside ? rr : 0) - i * a.gs);
+    const int i = (int)((uint32_t)(inside ? rr : 0) / (uint32_t)a.gs);
+    const int64_t t = o0 + i;
+    const int head = h * a.gs + ((inside ? rr : 0) - i * a.gs);
     bool on = inside;
     if (a.heads) {
-      uint64_t sel = 0;
-      for (int c = 0; c < 16; ++c) {
-        const int64_t cr = tile * 16 + c;
-        if (cr >= nr) break;
-        const int64_t ci = cr / a.gs;
-        if (pa_selected(a, o0 + ci, h * a.gs + (int)(cr - ci * a.gs), lane)) sel |= 1ull << c;
+      uint32_t sel = 0;
+      for (int c = 0; c < 16 && tile * 16 + c < nr; ++c) {
+        const int cr = tile * 16 + c, ci = (int)((uint32_t)cr / (uint32_t)a.gs);
+        if (pa_selected(a, o0 + ci, h * a.gs + (cr - ci * a.gs), lane)) sel |= 1u << c;
       }
       on = on && (sel >> col & 1);
     }
@@ -237,12 +269,13 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_rows_kernel(PaArgs a) {
     const int all_hi = (int)wave_min_u32(some ? (uint32_t)hi : 0x7fffffffu);
 
     float m = -INFINITY, l = 0.0f;
-    kh_f32x4 o[NF], om, os[NG];
+    kh_f32x4 o[NF], om;
+    float os[NG];  // of the lane's positions
 #pragma unroll
     for (int f = 0; f < NF; ++f) o[f] = kh_f32x4{0, 0, 0, 0};
     om = kh_f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < NG; ++j) os[j] = kh_f32x4{0, 0, 0, 0};
+    for (int j = 0; j < NG; ++j) os[j] = 0.0f;
 
     const int first = tlo / kPaStep, steps = thi > tlo ? (thi + kPaStep - 1) / kPaStep - first : 0;
     const int per = (steps + a.nsplit - 1) / a.nsplit;
@@ -269,27 +302,18 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_rows_kernel(PaArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float s = 4 * k + j < NG ? qsum[4 * k + j < NG ? 4 * k + j : 0] : 0.0f;
-            e[2 * j] = -128.0f * s;
-            e[2 * j + 1] = s;
+            e[2 * j] = s;
+            e[2 * j + 1] = -(float)BIAS * s;
           }
           uint4 tm[3];
           terms8<3>(e, tm);
-          const uint4 z = make_uint4(0, 0, 0, 0);
-          qm[k] = g == 0 ? tm[0] : g == 1 ? tm[1] : g == 2 ? tm[2] : z;
+          const auto pick = [g](uint32_t x, uint32_t y, uint32_t z) { return g == 0 ? x : g == 1 ? y : g == 2 ? z : 0u; };
+          qm[k] = make_uint4(pick(tm[0].x, tm[1].x, tm[2].x), pick(tm[0].y, tm[1].y, tm[2].y),
+                             pick(tm[0].z, tm[1].z, tm[2].z), pick(tm[0].w, tm[1].w, tm[2].w));
         }
       }
 
-      const auto page = [&](int tok) -> int64_t {
-        const int c = min(tok >> a.ps_log2, (int)a.cols - 1);
-        return table[__builtin_amdgcn_readfirstlane(c)];
-      };
-      const auto clean = [&](int64_t pg, bool* ok) -> int64_t {
-        *ok = pg >= 0 && pg < a.pages;
-        if (*ok) return pg;
-        if (lane == 0) atomicOr(a.err, 2);
-        return 0;
-      };
-      const auto step = [&](const PaStepData<D>& x, int tok, bool ok0, bool ok1) {
+      const auto step = [&](PaStepData<D>& x, int tok, bool ok0, bool ok1) {
         const bool whole = tok >= all_lo && tok + kPaStep <= all_hi && ok0 && ok1;
         // scores: positions 16 t + 4 g + r along registers, rows along lanes
         float s[2][4];
@@ -308,15 +332,15 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_rows_kernel(PaArgs a) {
 #pragma unroll
           for (int j = 0; j < NG; ++j) {
             const uint32_t w = x.kw[tt][j];
-            const uint4 kf = make_uint4(codes2(w, 0), codes2(w, 1), codes2(w, 2), codes2(w, 3));
+            const uint4 kf = make_uint4(codes2<BIAS>(w, 0), codes2<BIAS>(w, 1), codes2<BIAS>(w, 2), codes2<BIAS>(w, 3));
             kh_f32x4 c = {0, 0, 0, 0};
 #pragma unroll
             for (int k = NQ - 1; k >= 0; --k) c = mfma16(kf, qf[j][k], c);
-            const uint32_t pr = x.kpc[tt][j];
-            s[tt][0] = fmaf(__uint_as_float(quad_bcast<0>(pr) << 16), c[0], s[tt][0]);
-            s[tt][1] = fmaf(__uint_as_float(quad_bcast<1>(pr) << 16), c[1], s[tt][1]);
-            s[tt][2] = fmaf(__uint_as_float(quad_bcast<2>(pr) << 16), c[2], s[tt][2]);
-            s[tt][3] = fmaf(__uint_as_float(quad_bcast<3>(pr) << 16), c[3], s[tt][3]);
+            const uint32_t ks = x.kpc[tt][j] & 0xffff0000u;
+            s[tt][0] = fma_quad<0>(c[0], ks, s[tt][0]);
+            s[tt][1] = fma_quad<1>(c[1], ks, s[tt][1]);
+            s[tt][2] = fma_quad<2>(c[2], ks, s[tt][2]);
+            s[tt][3] = fma_quad<3>(c[3], ks, s[tt][3]);
           }
         }
         bool see[2][4];
@@ -325,7 +349,6 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_rows_kernel(PaArgs a) {
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            s[tt][r] *= a.c1;
             if (!whole) {
               const int j = tok + 16 * tt + 4 * g + r;
               see[tt][r] = j >= lo && j < hi && (tt ? ok1 : ok0);
@@ -333,10 +356,10 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_rows_kernel(PaArgs a) {
             }
             mx = fmaxf(mx, s[tt][r]);
           }
-        const float mn = fmaxf(m, across_groups_max(mx));
-        const float mu = mn == -INFINITY ? 0.0f : mn;
-        if (__ballot(mn != m)) {
-          const float alpha = __builtin_amdgcn_exp2f(m - mu);
+        // a new maximum is looked for across the lanes only where one passes the old
+        if (__ballot(mx > m)) {
+          const float mn = fmaxf(m, across_groups_max(mx));
+          const float alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.c1);
           l *= alpha;
           om *= alpha;
 #pragma unroll
@@ -345,40 +368,43 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_rows_kernel(PaArgs a) {
           for (int f = 0; f < NF; ++f) o[f] *= alpha;
           m = mn;
         }
+        const float mc = m == -INFINITY ? 0.0f : m * a.c1;
         float p[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - mu);
+        for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], a.c1, -mc));
         l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 
         uint4 pt[NP];
         terms8<NP>(p, pt);
-        const uint4 vm = make_uint4(x.vp[0][0] & odd, x.vp[0][1] & odd, x.vp[1][0] & odd, x.vp[1][1] & odd);
+        // rows m_g, then the scales alone
+        const uint4 vm = make_uint4(__builtin_amdgcn_perm(x.vp[0][1], x.vp[0][0], 0x05040100u),
+                                    __builtin_amdgcn_perm(x.vp[0][3], x.vp[0][2], 0x05040100u),
+                                    __builtin_amdgcn_perm(x.vp[1][1], x.vp[1][0], 0x05040100u),
+                                    __builtin_amdgcn_perm(x.vp[1][3], x.vp[1][2], 0x05040100u));
 #pragma unroll
         for (int k = NP - 1; k >= 0; --k) om = mfma16(vm, pt[k], om);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x.vp[e >> 2][e & 3] &= 0xffff0000u;
 
         const auto group = [&](auto G) {
           constexpr int gi = decltype(G)::value;
           float ps8[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t w = row_bcast<2 * gi>(x.vp[e >> 1][e & 1]);
-            ps8[2 * e] = p[2 * e] * __uint_as_float(w << 16);
-            ps8[2 * e + 1] = p[2 * e + 1] * __uint_as_float(w & 0xffff0000u);
-          }
+          for (int e = 0; e < 8; ++e) ps8[e] = mul_row<gi>(p[e], x.vp[e >> 2][e & 3]);
           if (!whole) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) ps8[e] = see[e >> 2][e & 3] ? ps8[e] : 0.0f;
           }
           uint4 pg[NP];
           terms8<NP>(ps8, pg);
-          const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
 #pragma unroll
-          for (int k = NP - 1; k >= 0; --k) os[gi] = mfma16(ones, pg[k], os[gi]);
+          for (int k = NP - 1; k >= 0; --k)
+            os[gi] = add2(pg[k].w, add2(pg[k].z, add2(pg[k].y, add2(pg[k].x, os[gi]))));
 #pragma unroll
           for (int ff = 0; ff < 2; ++ff) {
             const int f = 2 * gi + ff, hf = f >> 2, nb = f & 3;
-            const uint4 vf = make_uint4(codes2(x.vw[0][hf], nb), codes2(x.vw[0][HN + hf], nb),
-                                        codes2(x.vw[1][hf], nb), codes2(x.vw[1][HN + hf], nb));
+            const uint4 vf = make_uint4(codes2<BIAS>(x.vw[0][hf], nb), codes2<BIAS>(x.vw[0][HN + hf], nb),
+                                        codes2<BIAS>(x.vw[1][hf], nb), codes2<BIAS>(x.vw[1][HN + hf], nb));
 #pragma unroll
             for (int k = NP - 1; k >= 0; --k) o[f] = mfma16(vf, pg[k], o[f]);
           }
@@ -397,32 +423,66 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_rows_kernel(PaArgs a) {
         }
       };
 
-      for (int st = sb + wave; st < se; st += kPaWaves) {
-        const int tok = st * kPaStep;
+      // The wave's steps sb + wave, + kPaWaves, ...: lane k holds the pages of the
+      // k-th of the next 64, and a step's words are loaded while the one before it
+      // is worked on.
+      const int mine = (se - sb - wave + kPaWaves - 1) / kPaWaves;
+      int pg0 = 0, pg1 = 0;
+      const auto pages = [&](int k0) {
+        const int k = k0 + lane, tok = (sb + wave + k * kPaWaves) * kPaStep;
+        if (k >= mine) return;
         // a half of the step that no row of the tile sees takes the other half's page:
         // the table need not name one there
-        bool ok0, ok1;
-        const int64_t pg0 = clean(page(tok + 16 <= tlo ? tok + 16 : tok), &ok0);
-        const int64_t pg1 = clean(page(tok + 16 >= thi ? tok : tok + 16), &ok1);
-        PaStepData<D> x;
-        pa_load<D>(a, pg0, pg1, tok, h, ps, lane, x);
-        step(x, tok, ok0, ok1);
+        pg0 = table[(tok + 16 <= tlo ? tok + 16 : tok) >> a.ps_log2];
+        pg1 = table[(tok + 16 >= thi ? tok : tok + 16) >> a.ps_log2];
+        if (pg0 < 0 || pg0 >= a.pages) pg0 = -1;
+        if (pg1 < 0 || pg1 >= a.pages) pg1 = -1;
+        if ((pg0 | pg1) < 0) atomicOr(a.err, 2);
+      };
+      const auto load = [&](int k, PaStepData<D>& x) {
+        const int tok = (sb + wave + k * kPaWaves) * kPaStep;
+        const int p0 = max(__builtin_amdgcn_readlane(pg0, k & 63), 0), p1 = max(__builtin_amdgcn_readlane(pg1, k & 63), 0);
+        pa_load<D, 0>(a.pool + ((int64_t)p0 * a.nkv + h) * a.block, tok & (ps - 1), lo_, x);
+        pa_load<D, 1>(a.pool + ((int64_t)p1 * a.nkv + h) * a.block, (tok + 16) & (ps - 1), lo_, x);
+      };
+      const auto work = [&](int k, int q0, int q1, PaStepData<D>& x) {
+        step(x, (sb + wave + k * kPaWaves) * kPaStep, q0 >= 0, q1 >= 0);
+      };
+      if (mine > 0) {
+        PaStepData<D> x[2];
+        pages(0);
+        load(0, x[0]);
+        for (int k = 0; k < mine; k += 2) {
+          int q0 = __builtin_amdgcn_readlane(pg0, k & 63), q1 = __builtin_amdgcn_readlane(pg1, k & 63);
+          if (k + 1 < mine) load(k + 1, x[1]);  // 64 is even: of the same pages
+          work(k, q0, q1, x[0]);
+          if (k + 1 >= mine) break;
+          q0 = __builtin_amdgcn_readlane(pg0, (k + 1) & 63);
+          q1 = __builtin_amdgcn_readlane(pg1, (k + 1) & 63);
+          if (k + 2 < mine) {
+            if (((k + 2) & 63) == 0) pages(k + 2);
+            load(k + 2, x[0]);
+          }
+          work(k + 1, q0, q1, x[1]);
+        }
       }
     }
 
-    // -128 sum R + sum p m: row 2 j + 1 of om lies with lane group j / 2
+    // -128 sum R + sum p m: row j of om lies with lane group j / 4
     l = across_groups_sum(l);
     {
 #pragma unroll
       for (int gi = 0; gi < NG; ++gi) {
-        const float c = __shfl((gi & 1) ? om[3] : om[1], (gi >> 1) * 16 + col) - 128.0f * os[gi][0];
+        const float c = __shfl(om[gi & 3], (gi >> 2) * 16 + col) -
+                        (float)BIAS * across_groups_sum(os[gi]);
 #pragma unroll
         for (int ff = 0; ff < 2; ++ff)
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[2 * gi + ff][r] += c;
       }
     }
-    // the four waves' parts, joined in a fixed order
+    // the four waves' parts, joined in a fixed order; maxima in powers of two from here
+    m *= a.c1;
     if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l;
     __syncthreads();
     float M = s_m[0][col];
@@ -476,42 +536,64 @@ __global__ __launch_bounds__(64 * kPaWaves) void paged_rows_kernel(PaArgs a) {
   }
 }
 
-// Joins the parts of each row: one wave a (row, head), D / 64 elements a lane.
-template <int D, typename T>
+// Joins the parts of each row: W waves a (row, head), four elements a lane, so
+// that 256 / D parts of a wave are in flight at once.
+template <int D, typename T, int W>
 __global__ __launch_bounds__(256) void paged_join_kernel(PaArgs a) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t t = row / a.nh;
+  constexpr int C = D / 4, NS = 64 / C;
+  __shared__ __align__(16) float s_acc[W > 1 ? W : 1][D];
+  const int lane = threadIdx.x & 63, c = lane % C, sub = lane / C;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  const uint32_t t = (uint32_t)(row / a.nh);
   if (t >= a.rows || t < a.off[0] || t >= a.off[a.batch]) return;
-  const int head = (int)(row - t * a.nh);
+  const int head = (int)(row - (int64_t)t * a.nh);
   const float2* __restrict__ ml = a.part_ml + row * a.nsplit;
+  const float* __restrict__ po = a.part_o + row * a.nsplit * D + 4 * c;
   float2 x[2];
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    x[k] = lane + 64 * k < a.nsplit ? ml[lane + 64 * k] : make_float2(-INFINITY, 0.0f);
+  for (int k = 0; k < 2; ++k) x[k] = lane + 64 * k < a.nsplit ? ml[lane + 64 * k] : make_float2(-INFINITY, 0.0f);
   const float M = wave_max(fmaxf(x[0].x, x[1].x)), Mu = M == -INFINITY ? 0.0f : M;
-  float w[2], tot = 0.0f;
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    w[k] = __builtin_amdgcn_exp2f(x[k].x - Mu);
-    tot += w[k] * x[k].y;
+  const float tot = wave_sum(__builtin_amdgcn_exp2f(x[0].x - Mu) * x[0].y + __builtin_amdgcn_exp2f(x[1].x - Mu) * x[1].y);
+  float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+  for (int s = (W > 1 ? wave : 0) * NS + sub; s < a.nsplit; s += (W > 1 ? W : 1) * NS) {
+    const float ms = ml[s].x, w = __builtin_amdgcn_exp2f(ms - Mu);
+    const float4 v = *reinterpret_cast<const float4*>(po + (int64_t)s * D);
+    // a part without a key was not written; where NaN scores left no maximum, tot is NaN
+    const bool none = ms == -INFINITY;
+    acc.x = fmaf(w, none ? 0.0f : v.x, acc.x);
+    acc.y = fmaf(w, none ? 0.0f : v.y, acc.y);
+    acc.z = fmaf(w, none ? 0.0f : v.z, acc.z);
+    acc.w = fmaf(w, none ? 0.0f : v.w, acc.w);
   }
-  tot = wave_sum(tot);
-  // parts without a key were not written; where NaN scores left no maximum, tot is NaN
-  float acc[E] = {};
-  for (int s = 0; s < a.nsplit; ++s) {
-    const float ws = __shfl(s < 64 ? w[0] : w[1], s & 63);
-    const float ms = __shfl(s < 64 ? x[0].x : x[1].x, s & 63);
-    if (ms == -INFINITY) continue;
-    const float* __restrict__ p = a.part_o + (row * a.nsplit + s) * D + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(ws, p[e], acc[e]);
+  for (int m = C; m < 64; m <<= 1) {
+    acc.x += __shfl_xor(acc.x, m);
+    acc.y += __shfl_xor(acc.y, m);
+    acc.z += __shfl_xor(acc.z, m);
+    acc.w += __shfl_xor(acc.w, m);
+  }
+  if (W > 1) {
+    if (sub == 0) *reinterpret_cast<float4*>(&s_acc[wave][4 * c]) = acc;
+    __syncthreads();
+    if (wave > 0) return;
+    acc = *reinterpret_cast<const float4*>(&s_acc[0][4 * c]);
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(&s_acc[w][4 * c]);
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
+    }
   }
   const bool any = M != -INFINITY || tot != 0.0f;
-  T* y = static_cast<T*>(a.out) + t * a.os + head * a.oh + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) store_f32(y + e, any ? acc[e] / tot : 0.0f);
+  if (sub == 0) {
+    T* y = static_cast<T*>(a.out) + t * a.os + head * a.oh + 4 * c;
+    pa_store4<D, T>(y, a.ovec, any ? acc.x / tot : 0.0f, any ? acc.y / tot : 0.0f, any ? acc.z / tot : 0.0f,
+                    any ? acc.w / tot : 0.0f);
+  }
   if (a.lse && lane == 0) a.lse[row] = any ? kLn2 * (M + __builtin_amdgcn_logf(tot)) : -INFINITY;
 }
 
@@ -529,7 +611,7 @@ static PaPlan pa_plan(int nkv, int nh, int64_t rows, int64_t batch, int64_t max_
   if (p.tiles < 1) p.tiles = 1;
   if (p.tiles > 65536) p.tiles = 65536;
   p.base = batch * nkv * p.tiles;
-  int64_t want = p.base >= 1024 ? 1 : (2048 + p.base - 1) / p.base;
+  int64_t want = (512 + p.base - 1) / p.base;
   const int64_t most = (max_len + 255) / 256;
   if (want > most) want = most;
   if (want > kPaMaxSplit) want = kPaMaxSplit;
@@ -543,8 +625,10 @@ static int64_t pa_bytes(const PaPlan& p, int64_t rows, int nh, int d) {
 template <int D, typename T>
 static void pa_launch(const PaArgs& a, int64_t blocks, hipStream_t st) {
   hipLaunchKernelGGL((paged_rows_kernel<D, T>), dim3((unsigned)blocks), dim3(64 * kPaWaves), 0, st, a);
-  if (a.nsplit > 1)
-    hipLaunchKernelGGL((paged_join_kernel<D, T>), dim3((unsigned)((a.rows * a.nh + 3) / 4)), dim3(256), 0, st, a);
+  if (a.nsplit > 16)
+    hipLaunchKernelGGL((paged_join_kernel<D, T, 4>), dim3((unsigned)(a.rows * a.nh)), dim3(256), 0, st, a);
+  else if (a.nsplit > 1)
+    hipLaunchKernelGGL((paged_join_kernel<D, T, 1>), dim3((unsigned)((a.rows * a.nh + 3) / 4)), dim3(256), 0, st, a);
 }
 template <typename T>
 static void pa_launch_d(int d, const PaArgs& a, int64_t blocks, hipStream_t st) {
@@ -561,6 +645,8 @@ static int pa_shape(const kh_paged_kv* c, int dtype, int64_t rows, int64_t batch
                "rows %lld, batch %lld not in [0,2^31)", (long long)rows, (long long)batch);
   KH_CHECK_ARG(num_heads >= c->nkv && num_heads % c->nkv == 0 && num_heads <= 65536,
                "num_heads %d is no multiple of the cache's %d", num_heads, c->nkv);
+  KH_CHECK_ARG(rows * (num_heads / c->nkv) < (int64_t)1 << 31, "%lld rows of %d heads: too many for one call",
+               (long long)rows, num_heads);
   KH_CHECK_ARG(max_rows >= 0 && max_len >= 0, "max_rows %lld, max_len %lld", (long long)max_rows, (long long)max_len);
   return KH_OK;
 }
@@ -611,7 +697,7 @@ extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void
   }
   KH_CHECK_ARG((reinterpret_cast<uintptr_t>(ws_dev) & 15) == 0, "the workspace must be 16-byte aligned");
   const int64_t blocks = p.base * p.nsplit;
-  KH_CHECK_ARG(blocks < (int64_t)1 << 31 && rows * num_heads < (int64_t)1 << 33, "too many rows for one call");
+  KH_CHECK_ARG(blocks < (int64_t)1 << 31 && rows * num_heads < (int64_t)1 << 31, "too many rows for one call");
   KH_ON_DEVICE(c->device, "the cache");
   PaArgs a;
   a.pool = c->pool;

@@ -25,15 +25,15 @@ __device__ __forceinline__ uint32_t bf16_down(float x) {
 }
 __device__ __forceinline__ uint32_t bf16_up(float x) { return (__float_as_uint(x) + 0xffffu) >> 16; }
 
-// scale | minimum << 16 of a group with range [lo, hi]; bad: it holds a value that is not finite.
+// minimum | scale << 16 of a group with range [lo, hi]; bad: it holds a value that is not finite.
 __device__ __forceinline__ uint32_t kv_pair(float lo, float hi, bool bad) {
   const uint32_t m = bf16_down(lo);
   const uint32_t s = bf16_up(__fdiv_rn(__fsub_rn(hi, __uint_as_float(m << 16)), 15.0f));
-  if (bad || s >= 0x7f80u) return 0x7fc0u;  // negative s cannot be: hi >= m
-  return s | m << 16;
+  if (bad || s >= 0x7f80u) return 0x7fc00000u;  // negative s cannot be: hi >= m
+  return m | s << 16;
 }
 __device__ __forceinline__ uint32_t kv_code(float x, uint32_t pair) {
-  const float s = __uint_as_float(pair << 16), m = __uint_as_float(pair & 0xffff0000u);
+  const float s = __uint_as_float(pair & 0xffff0000u), m = __uint_as_float(pair << 16);
   if (!(s > 0.0f)) return 0;
   const float q = rintf(__fdiv_rn(__fsub_rn(x, m), s));
   return (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f);
@@ -232,11 +232,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a) {
       }
       uint16_t* vc = reinterpret_cast<uint16_t*>(blk + P::vc(ps));
       vc[((((at >> 2) * 16 + r) * 2 + ((at >> 1) & 1)) * HN + hf) * 2 + (at & 1)] = (uint16_t)w;
-      if (r < 4) {  // row 2 group + (0: scale, 1: minimum)
-        uint16_t* vp = reinterpret_cast<uint16_t*>(blk + P::vp(ps));
-        const uint32_t pr = pairs[r >> 1];
-        vp[(4 * hf + r) * ps + at] = (uint16_t)((r & 1) ? pr >> 16 : pr);
-      }
+      if (r < 2) *reinterpret_cast<uint32_t*>(blk + P::vp(ps) + ((2 * hf + r) * ps + at) * 4) = r ? pairs[1] : pairs[0];
     }
   }
 }
@@ -267,15 +263,15 @@ __global__ __launch_bounds__(kKvThreads) void kv_gather_kernel(GatherArgs a) {
     if (blockIdx.y == 0) {
       const uint32_t w = *reinterpret_cast<const uint32_t*>(blk + P::kc() + at * (D / 2) + ((c & 3) * NG + j) * 4);
       const uint32_t pr = *reinterpret_cast<const uint32_t*>(blk + P::kp(ps) + (at * NG + j) * 4);
-      const float s = __uint_as_float(pr << 16), m = __uint_as_float(pr & 0xffff0000u);
+      const float s = __uint_as_float(pr & 0xffff0000u), m = __uint_as_float(pr << 16);
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = s * (float)((w >> (4 * i)) & 15) + m;
     } else {
       // d = 8 c + i = 64 hf + 16 n + r: one nibble of eight neighbouring r
       const int hf = c >> 3, n = (c >> 1) & 3, r0 = 8 * (c & 1);
       const uint16_t* vc = reinterpret_cast<const uint16_t*>(blk + P::vc(ps));
-      const uint16_t* vp = reinterpret_cast<const uint16_t*>(blk + P::vp(ps));
-      const float s = bf16_to_f32(vp[2 * j * ps + at]), m = bf16_to_f32(vp[(2 * j + 1) * ps + at]);
+      const uint32_t pr = *reinterpret_cast<const uint32_t*>(blk + P::vp(ps) + (j * ps + at) * 4);
+      const float s = __uint_as_float(pr & 0xffff0000u), m = __uint_as_float(pr << 16);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t w = vc[((((at >> 2) * 16 + r0 + i) * 2 + ((at >> 1) & 1)) * HN + hf) * 2 + (at & 1)];

@@ -8,8 +8,8 @@
 //   K codes [ps][g][j] u32: nibble n is the code of d = 32 j + 8 g + n
 //   V codes [ps / 4][r][token / 2 % 2][h][token % 2] u16, h < D / 64: nibble n
 //           is the code of d = 64 h + 16 n + r
-//   K pairs [ps][j] u32: scale | minimum << 16 (BF16 bits)
-//   V pairs [j][2][ps] u16: the scales of group j, then its minima
+//   K pairs [ps][j] u32: minimum | scale << 16 (BF16 bits)
+//   V pairs [j][ps] u32: the same
 // Every part of a position is written by whole u16 or u32 stores of its own, so
 // positions of one page may be appended from different blocks.
 #pragma once
