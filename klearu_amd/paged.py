@@ -27,19 +27,19 @@ HALF, INTERLEAVED = 0, 1
 SCALE_NONE, SCALE_LINEAR, SCALE_BASE, SCALE_BY_PARTS = 0, 1, 2, 3
 
 _DT = {torch.float32: 0, torch.bfloat16: 2}
+_I64, _I32 = torch.int64, torch.int32
 
 
 def _rows(t: torch.Tensor, what: str, device, dtype=None):
     """(pointer, row stride, head stride, dtype code) of a tensor [rows, heads, head_dim]."""
-    if not t.is_cuda:
-        raise ValueError(f"{what}: expected a device tensor")
+    dt = t.dtype
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, the handle on {device}")
     if t.dim() != 3:
         raise ValueError(f"{what}: expected [rows, heads, head_dim], got {tuple(t.shape)}")
-    code = _DT.get(t.dtype)
-    if code is None or (dtype is not None and t.dtype != dtype):
-        raise TypeError(f"{what}: dtype {t.dtype}, expected {dtype or 'float32 or bfloat16'}")
+    code = _DT.get(dt)
+    if code is None or (dtype is not None and dt is not dtype):
+        raise TypeError(f"{what}: dtype {dt}, expected {dtype or 'float32 or bfloat16'}")
     s0, s1, s2 = t.stride()
     if s2 != 1 and t.shape[2] > 1 and t.numel():
         raise ValueError(f"{what}: the elements of a head must be contiguous")
@@ -48,13 +48,11 @@ def _rows(t: torch.Tensor, what: str, device, dtype=None):
 
 def _index(t: torch.Tensor, what: str, device, dtype, shape):
     """Pointer of a contiguous index tensor of a given dtype and shape."""
-    if not t.is_cuda:
-        raise ValueError(f"{what}: expected a device tensor")
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, the handle on {device}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{what}: dtype {t.dtype}, expected {dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
     if not t.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous tensor")
@@ -63,40 +61,55 @@ def _index(t: torch.Tensor, what: str, device, dtype, shape):
 
 def _table(t: torch.Tensor, device, batch):
     """(pointer, columns, row stride) of an int32 page table [batch, columns]."""
-    if not t.is_cuda:
-        raise ValueError("table: expected a device tensor")
     if t.device != device:
         raise ValueError(f"table is on {t.device}, the handle on {device}")
-    if t.dtype != torch.int32:
+    if t.dtype is not _I32:
         raise TypeError(f"table: dtype {t.dtype}, expected torch.int32")
     if t.dim() != 2 or t.shape[0] != batch:
         raise ValueError(f"table: shape {tuple(t.shape)}, expected [{batch}, columns]")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    cols = t.shape[1]
+    s0, s1 = t.stride()
+    if cols > 1 and s1 != 1:
         raise ValueError("table: the columns of a row must be contiguous")
-    return t.data_ptr(), t.shape[1], max(t.stride(0), t.shape[1]) if batch <= 1 else t.stride(0)
+    return t.data_ptr(), cols, max(s0, cols) if batch <= 1 else s0
+
+
+def _check(rc: int) -> None:
+    if rc < 0:
+        raise _lib.KlearuError(rc, _lib.load().kh_last_error().decode(errors="replace"))
 
 
 class _On:
-    """The handle's device and `stream` (None: the current one) made current, where they are not."""
+    """Makes a handle's device and `stream` (None: the current one) current, and holds the memory
+    of `tensors` for that stream; as a value, the stream's pointer."""
 
-    __slots__ = ("ctx",)
-
-    def __init__(self, device, stream):
-        self.ctx = []
-        if torch.cuda.current_device() != device.index:
-            self.ctx.append(torch.cuda.device(device))
+    def __init__(self, device, stream, tensors):
+        if stream is not None and stream.device != device:
+            raise ValueError(f"stream is on {stream.device}, the handle on {device}")
+        self.ctx = [torch.cuda.device(device)]
         if stream is not None:
-            if stream.device != device:
-                raise ValueError(f"stream is on {stream.device}, the handle on {device}")
             self.ctx.append(torch.cuda.stream(stream))
+        self.stream, self.tensors = stream, tensors
 
     def __enter__(self):
         for c in self.ctx:
             c.__enter__()
+        if self.stream is not None:
+            for t in self.tensors:
+                if t is not None:
+                    t.record_stream(self.stream)
+        return torch.cuda.current_stream().cuda_stream
 
     def __exit__(self, *e):
         for c in reversed(self.ctx):
             c.__exit__(*e)
+
+
+# torch.cuda.current_stream(index).cuda_stream and torch.cuda.current_device(), without the
+# objects (a call of a few microseconds is mostly this)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda i: torch.cuda.current_stream(i).cuda_stream)
+_raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 class _Handle:
@@ -112,19 +125,13 @@ class _Handle:
 
     def _adopt(self, h):
         self._h = h
-        self.device = torch.device("cuda", torch.cuda.current_device())
+        self._lib = _lib.load()
+        self._dev = torch.cuda.current_device()
+        self.device = torch.device("cuda", self._dev)
 
-    def _call(self, stream, fn, *inputs):
-        """fn(stream pointer) with the handle's device and the stream current: results are
-        allocated there, so their memory is the stream's, and the inputs' memory is not given
-        to others before the stream has passed."""
-        if stream is None and torch.cuda.current_device() == self.device.index:
-            return fn(torch.cuda.current_stream().cuda_stream)
-        with _On(self.device, stream):
-            for t in inputs:
-                if t is not None and stream is not None:
-                    t.record_stream(stream)
-            return fn(torch.cuda.current_stream().cuda_stream)
+    def _status(self, name):
+        with _On(self.device, None, ()):
+            _check(getattr(self._lib, name)(self._h))
 
 
 class Rope(_Handle):
@@ -152,24 +159,27 @@ class Rope(_Handle):
         place) or a new tensor.  `transpose` takes gradients back: the transposed rotation.  Rows of
         a negative position are padding and left as they were, as are (reported by status()) rows
         past max_pos; in a new tensor those hold no value."""
-        xp, x0, x1, dt = _rows(x, "x", self.device)
+        dev = self.device
+        xp, x0, x1, dt = _rows(x, "x", dev)
         n, heads, dim = x.shape
-        pp = _index(pos, "pos", self.device, torch.int64, (n,))
-        if out is not None and out.shape != x.shape:
+        pp = _index(pos, "pos", dev, _I64, (n,))
+        if stream is not None or _raw_device() != self._dev:
+            with _On(dev, stream, (x, pos, out)):
+                return self.apply(x, pos, out, transpose)
+        if out is None:
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+            yp, y0, y1 = out.data_ptr(), heads * dim, dim
+        elif out.shape != x.shape:
             raise ValueError(f"out: shape {tuple(out.shape)}, expected {tuple(x.shape)}")
-
-        def go(s):
-            y = out if out is not None else torch.empty((n, heads, dim), dtype=x.dtype, device=x.device)
-            yp, y0, y1, _ = _rows(y, "out", self.device, x.dtype)
-            _lib.call("kh_rope_apply", self._h, dt, xp, x0, x1, n, heads, dim, pp, yp, y0, y1, 1 if transpose else 0,
-                      s)
-            return y
-
-        return self._call(stream, go, x, pos, out)
+        else:
+            yp, y0, y1, _ = _rows(out, "out", dev, x.dtype)
+        _check(self._lib.kh_rope_apply(self._h, dt, xp, x0, x1, n, heads, dim, pp, yp, y0, y1, 1 if transpose else 0,
+                                       _raw_stream(self._dev)))
+        return out
 
     def status(self):
         """Raise KlearuError (KH_ERR_ARG) if a call since the last check met a position past max_pos."""
-        self._call(None, lambda s: _lib.call("kh_rope_status", self._h))
+        self._status("kh_rope_status")
 
 
 class PagedKv(_Handle):
@@ -187,54 +197,56 @@ class PagedKv(_Handle):
         self._adopt(h)
         self.num_kv_heads, self.head_dim = num_kv_heads, head_dim
         self.num_pages, self.page_size = num_pages, page_size
+        self._ws = {}
 
-    def _shape(self, t, what, rows):
-        if tuple(t.shape) != (rows, self.num_kv_heads, self.head_dim):
-            raise ValueError(f"{what}: shape {tuple(t.shape)}, expected "
-                             f"({rows}, {self.num_kv_heads}, {self.head_dim})")
+    def _places(self, off, start, table):
+        """What every call over rows of sequences checks: (batch, off, start, table, columns, stride)."""
+        dev, batch = self.device, start.shape[0]
+        return (batch, _index(off, "off", dev, _I64, (batch + 1,)), _index(start, "start", dev, _I64, (batch,)),
+                *_table(table, dev, batch))
 
     def append(self, k: torch.Tensor, v: torch.Tensor, off: torch.Tensor, start: torch.Tensor, table: torch.Tensor,
                rope: Rope | None = None, pos: torch.Tensor | None = None, stream=None) -> None:
         """Row off[b] + i of k and v [rows, num_kv_heads, head_dim] becomes position start[b] + i of
         sequence b; `rope` rotates the keys on the way, by pos [rows] or by their places in the
         cache.  Two rows of one call must not have the same place."""
+        dev = self.device
+        kp, k0, k1, dt = _rows(k, "k", dev)
+        vp, v0, v1, _ = _rows(v, "v", dev, k.dtype)
         n = k.shape[0]
-        kp, k0, k1, dt = _rows(k, "k", self.device)
-        vp, v0, v1, _ = _rows(v, "v", self.device, k.dtype)
-        self._shape(k, "k", n)
-        self._shape(v, "v", n)
-        batch = start.shape[0]
-        op = _index(off, "off", self.device, torch.int64, (batch + 1,))
-        sp = _index(start, "start", self.device, torch.int64, (batch,))
-        tp, cols, ts = _table(table, self.device, batch)
+        shape = (n, self.num_kv_heads, self.head_dim)
+        if k.shape != shape or v.shape != shape:
+            raise ValueError(f"k, v: shapes {tuple(k.shape)}, {tuple(v.shape)}, expected {shape}")
+        batch, op, sp, tp, cols, ts = self._places(off, start, table)
         if pos is not None and rope is None:
             raise ValueError("pos: rotary positions without a rotation")
-        pp = None if pos is None else _index(pos, "pos", self.device, torch.int64, (n,))
-        self._call(stream, lambda s: _lib.call(
-            "kh_paged_kv_append", self._h, None if rope is None else rope._h, dt, kp, k0, k1, vp, v0, v1, n, op,
-            batch, sp, pp, tp, cols, ts, s), k, v, off, start, table, pos)
+        pp = None if pos is None else _index(pos, "pos", dev, _I64, (n,))
+        if stream is not None or _raw_device() != self._dev:
+            with _On(dev, stream, (k, v, off, start, table, pos)):
+                return self.append(k, v, off, start, table, rope, pos)
+        _check(self._lib.kh_paged_kv_append(self._h, None if rope is None else rope._h, dt, kp, k0, k1, vp, v0, v1, n, op,
+                                            batch, sp, pp, tp, cols, ts, _raw_stream(self._dev)))
 
     def gather(self, off: torch.Tensor, start: torch.Tensor, table: torch.Tensor, rows: int,
                dtype: torch.dtype = torch.float32, k: torch.Tensor | None = None, v: torch.Tensor | None = None,
                stream=None):
         """The values that those places hold: (k, v) [rows, num_kv_heads, head_dim], new or given.
         Rows outside all sequences, or without a place, are left as they were."""
-        batch = start.shape[0]
-        op = _index(off, "off", self.device, torch.int64, (batch + 1,))
-        sp = _index(start, "start", self.device, torch.int64, (batch,))
-        tp, cols, ts = _table(table, self.device, batch)
-        if dtype not in _DT:
+        dev = self.device
+        batch, op, sp, tp, cols, ts = self._places(off, start, table)
+        dt = _DT.get(dtype)
+        if dt is None:
             raise TypeError(f"dtype {dtype}: expected float32 or bfloat16")
+        if stream is not None or _raw_device() != self._dev:
+            with _On(dev, stream, (off, start, table, k, v)):
+                return self.gather(off, start, table, rows, dtype, k, v)
         shape = (rows, self.num_kv_heads, self.head_dim)
-
-        def go(s):
-            a = k if k is not None else torch.empty(shape, dtype=dtype, device=self.device)
-            b = v if v is not None else torch.empty(shape, dtype=dtype, device=self.device)
-            _lib.call("kh_paged_kv_gather", self._h, _DT[dtype], rows, op, batch, sp, tp, cols, ts,
-                      _index(a, "k", self.device, dtype, shape), _index(b, "v", self.device, dtype, shape), s)
-            return a, b
-
-        return self._call(stream, go, off, start, table, k, v)
+        k = torch.empty(shape, dtype=dtype, device=dev) if k is None else k
+        v = torch.empty(shape, dtype=dtype, device=dev) if v is None else v
+        _check(self._lib.kh_paged_kv_gather(self._h, dt, rows, op, batch, sp, tp, cols, ts,
+                                            _index(k, "k", dev, dtype, shape), _index(v, "v", dev, dtype, shape),
+                                            _raw_stream(self._dev)))
+        return k, v
 
     def attention(self, q: torch.Tensor, off: torch.Tensor, lens: torch.Tensor, table: torch.Tensor,
                   scale: float | None = None, causal: bool = True, window: int = 0,
@@ -247,42 +259,54 @@ class PagedKv(_Handle):
         sequence (default: an even share of the rows, the table's reach); wrong guesses cost
         time only.  Returns out, or (out, lse) with lse [rows, num_heads] f32: a row that sees nothing
         gives 0 and -inf."""
-        n, nh = q.shape[0], q.shape[1] if q.dim() == 3 else 0
-        qp, q0, q1, dt = _rows(q, "q", self.device)
-        if q.shape[2] != self.head_dim:
-            raise ValueError(f"q: head_dim {q.shape[2]}, expected {self.head_dim}")
-        batch = lens.shape[0]
-        op = _index(off, "off", self.device, torch.int64, (batch + 1,))
-        lp = _index(lens, "lens", self.device, torch.int64, (batch,))
-        tp, cols, ts = _table(table, self.device, batch)
-        if out is not None and out.shape != q.shape:
-            raise ValueError(f"out: shape {tuple(out.shape)}, expected {tuple(q.shape)}")
+        dev = self.device
+        qp, q0, q1, dt = _rows(q, "q", dev)
+        n, nh, dim = q.shape
+        if dim != self.head_dim:
+            raise ValueError(f"q: head_dim {dim}, expected {self.head_dim}")
+        batch, op, lp, tp, cols, ts = self._places(off, lens, table)
         hp, nsel = None, 0
         if heads is not None:
             nsel = heads.shape[-1]
-            hp = _index(heads, "heads", self.device, torch.int32, (n, nsel)) or op  # an empty list is no list of all
+            hp = _index(heads, "heads", dev, _I32, (n, nsel)) or op  # an empty list is no list of all
+        if stream is not None or _raw_device() != self._dev:
+            with _On(dev, stream, (q, off, lens, table, heads, out)):
+                return self.attention(q, off, lens, table, scale, causal, window, heads, max_rows, max_len, out,
+                                      return_lse)
         if max_rows is None:
             max_rows = -(-n // max(1, batch))
         if max_len is None:
             max_len = cols * self.page_size
         if scale is None:
-            scale = self.head_dim ** -0.5
-        need = C.c_int64()
-        _lib.call("kh_paged_kv_attention_workspace", self._h, dt, n, batch, nh, max_rows, max_len, C.byref(need))
+            scale = dim ** -0.5
+        need = self._workspace(dt, n, batch, nh, max_rows, max_len)
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            yp, y0, y1 = out.data_ptr(), nh * dim, dim
+        elif out.shape != q.shape:
+            raise ValueError(f"out: shape {tuple(out.shape)}, expected {tuple(q.shape)}")
+        else:
+            yp, y0, y1, _ = _rows(out, "out", dev, q.dtype)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        lse = torch.empty((n, nh), dtype=torch.float32, device=dev) if return_lse else None
+        _check(self._lib.kh_paged_kv_attention(
+            self._h, dt, qp, q0, q1, nh, n, op, batch, lp, tp, cols, ts, max_rows, max_len, scale, 1 if causal else 0,
+            window, hp, nsel, yp, y0, y1, None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(),
+            need, _raw_stream(self._dev)))
+        return (out, lse) if return_lse else out
 
-        def go(s):
-            y = out if out is not None else torch.empty((n, nh, self.head_dim), dtype=q.dtype, device=q.device)
-            yp, y0, y1, _ = _rows(y, "out", self.device, q.dtype)
-            ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-            lse = torch.empty((n, nh), dtype=torch.float32, device=q.device) if return_lse else None
-            _lib.call("kh_paged_kv_attention", self._h, dt, qp, q0, q1, nh, n, op, batch, lp, tp, cols, ts, max_rows,
-                      max_len, scale, 1 if causal else 0, window, hp, nsel, yp, y0, y1,
-                      None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), need.value, s)
-            return (y, lse) if return_lse else y
-
-        return self._call(stream, go, q, off, lens, table, heads, out)
+    def _workspace(self, *sizes) -> int:
+        """kh_paged_kv_attention_workspace: bytes by the call's sizes."""
+        need = self._ws.get(sizes)
+        if need is None:
+            x = C.c_int64()
+            _check(self._lib.kh_paged_kv_attention_workspace(self._h, *sizes, C.byref(x)))
+            if len(self._ws) >= 1024:
+                self._ws.clear()
+            need = self._ws[sizes] = x.value
+        return need
 
     def status(self):
         """Raise KlearuError (KH_ERR_ARG) if a call since the last check met a place outside its
         sequence's table, a length the table cannot hold, or a page id outside the pool."""
-        self._call(None, lambda s: _lib.call("kh_paged_kv_status", self._h))
+        self._status("kh_paged_kv_status")
