@@ -731,7 +731,8 @@ typedef struct kh_paged_kv kh_paged_kv;
  * head; head_dim 64, 128 or 256.  32 neighbouring values of a head share m =
  * their minimum rounded down to BF16 and s = (maximum - m) / 15 rounded up to
  * BF16; x is held as the 4-bit c = rint((x - m) / s) and stands for s c + m:
- * 5 bits a value.  A group with a value that is not finite stands for NaN.
+ * 5 bits a value.  A group with a value that is not finite, or of 2^100 and
+ * more, stands for NaN.
  * Positions that were never written stand for 0.  Synchronous.
  *
  * Which pages belong to a sequence is the caller's: row b of an int32 page

@@ -22,6 +22,7 @@
 // in when the positions of a step are numbered 4 g + i and 16 + 4 g + i; nothing
 // is exchanged between lanes but the running maximum.
 #include <cmath>
+#include <mutex>
 #include <type_traits>
 
 #include "mfma.hpp"
@@ -536,6 +537,400 @@ __global__ __launch_bounds__(64 * kPaWaves, D == 64 ? 3 : D == 128 ? 2 : 1) void
   }
 }
 
+// ---------------------------------------------------------------- many rows
+// Tiles of many rows (prompts and chunks, BF16): a block's waves put 64 positions
+// at a time into LDS as BF16 numbers s c + m, in the order of the matrix core's
+// first operand, and every wave runs its own rows (16 CT columns) over them, so
+// the work of unpacking is shared by all rows of the block.  Rounding a key or a
+// value to BF16 is off by at most 2^-8 of it, as in a BF16 cache, and queries and
+// weights are BF16 themselves.  Codes of the next 64 positions are loaded while
+// these are worked on; two LDS buffers, one barrier per 64 positions.
+//
+// A value's group that stands for NaN is unpacked as 0 and marked in a mask of its
+// positions: rows that see one of them get their NaN from the mask.
+constexpr int kPtKeys = 64;
+constexpr float kPtSlack = 6.0f;  // a maximum that is passed by less (in powers of two) is kept
+
+template <int D>
+struct PtShape {
+  static constexpr int CT = D == 256 ? 1 : 2;  // column tiles of 16 rows a wave holds
+  static constexpr int RW = 16 * CT;
+  static constexpr int kBufBytes = 2 * kPtKeys * D * 2;  // keys, then values
+  template <int NW>
+  static constexpr int lds() {
+    return 2 * kBufBytes;
+  }
+};
+
+typedef _Float16 kh_f16x2 __attribute__((ext_vector_type(2)));
+
+// Nibble n of each half of w as f32 (1024 + c), halves of a pair of f16.
+__device__ __forceinline__ kh_f16x2 codes_f16(uint32_t w, int n) {
+  return __builtin_bit_cast(kh_f16x2, ((w >> (4 * n)) & 0x000f000fu) | 0x64006400u);
+}
+
+template <int D, int NW>
+struct PtCodes {
+  static constexpr int NG = D / kKvGroup, HN = D / 64;
+  static constexpr int KF = 4 * NG / NW, VF = 4 * NG / NW;  // fragments a wave unpacks
+  static constexpr int VG = VF < 2 ? 1 : VF / 2, VH = VF <= 4 ? 1 : VF / 4;
+  uint32_t kw[KF], kp[KF];
+  uint32_t vw[VH][4], vp[VG][8];
+};
+
+template <int N>
+__device__ __forceinline__ void ld_n(const char* p, uint32_t* w) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  }
+}
+
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
+  using S = PtShape<D>;
+  using C = PtCodes<D, NW>;
+  using P = KvParts<D>;
+  constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16, CT = S::CT, RW = S::RW, RB = RW * NW;
+  constexpr int KF = C::KF, VF = C::VF;
+  extern __shared__ __align__(16) char s_buf[];
+  __shared__ int s_lo[NW], s_hi[NW];
+  __shared__ uint32_t s_nan[2][NG][2];  // positions whose value group stands for NaN
+  const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t id = blockIdx.x;
+  const int h = (int)(id % (uint32_t)a.nkv);
+  id /= (uint32_t)a.nkv;
+  const int split = (int)(id % (uint32_t)a.nsplit);
+  id /= (uint32_t)a.nsplit;
+  const int64_t b = id % (uint32_t)a.batch;
+  const int tile0 = a.tiles - 1 - (int)(id / (uint32_t)a.batch);  // the longest first
+  const int ps = 1 << a.ps_log2;
+  int64_t o0 = a.off[b], o1 = a.off[b + 1];
+  o0 = o0 < 0 ? 0 : o0;
+  o1 = o1 > a.rows ? a.rows : o1;
+  if (o1 <= o0) return;
+  const int n = (int)(o1 - o0), nr = n * a.gs;
+  const int64_t cap = a.cols << a.ps_log2;
+  int64_t L = a.len[b];
+  if (L < 0 || L > cap) {
+    if (threadIdx.x == 0) atomicOr(a.err, 1);
+    L = L < 0 ? 0 : cap;
+  }
+  const int32_t* __restrict__ table = a.table + b * a.table_stride;
+  const int ktile = wave / (NW / 4), kj0 = (wave % (NW / 4)) * KF;  // the fragments this wave unpacks
+  const int vtb = wave / (NW / 2), vf0 = (wave % (NW / 2)) * VF;
+
+  for (int tile = tile0; tile < (nr + RB - 1) / RB; tile += a.tiles) {
+    int lo[CT], hi[CT];
+    uint32_t row[CT];  // t * nh + head, below 2^31
+    bool inside[CT];
+    uint32_t wlo = 0x7fffffffu, whi = 0, all_lo = 0, all_hi = 0x7fffffffu;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const int r0 = tile * RB + wave * RW + c * 16, rr = r0 + col;
+      inside[c] = rr < nr;
+      const int i = (int)((uint32_t)(inside[c] ? rr : 0) / (uint32_t)a.gs);
+      const int head = h * a.gs + ((inside[c] ? rr : 0) - i * a.gs);
+      row[c] = (uint32_t)((o0 + i) * a.nh + head);
+      bool on = inside[c];
+      if (a.heads) {
+        uint32_t sel = 0;
+        for (int k = 0; k < 16 && r0 + k < nr; ++k) {
+          const int ci = (int)((uint32_t)(r0 + k) / (uint32_t)a.gs);
+          if (pa_selected(a, o0 + ci, h * a.gs + (r0 + k - ci * a.gs), lane)) sel |= 1u << k;
+        }
+        on = on && (sel >> col & 1);
+      }
+      lo[c] = hi[c] = 0;
+      if (on) {
+        const int64_t p = L - n + i;
+        const int64_t e = a.causal ? (p + 1 < L ? p + 1 : L) : L;
+        const int64_t s = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
+        if (e > s) lo[c] = (int)s, hi[c] = (int)e;
+      }
+      const bool some = hi[c] > lo[c];
+      wlo = min(wlo, wave_min_u32(some ? (uint32_t)lo[c] : 0x7fffffffu));
+      whi = max(whi, wave_max_u32(some ? (uint32_t)hi[c] : 0u));
+      all_lo = max(all_lo, wave_max_u32(some ? (uint32_t)lo[c] : 0u));
+      all_hi = min(all_hi, wave_min_u32(some ? (uint32_t)hi[c] : 0x7fffffffu));
+    }
+    __syncthreads();  // the last tile's readers of s_lo, s_hi and the buffers
+    if (lane == 0) s_lo[wave] = (int)wlo, s_hi[wave] = (int)whi;
+    __syncthreads();
+    int tlo = 0x7fffffff, thi = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) tlo = min(tlo, s_lo[w]), thi = max(thi, s_hi[w]);
+    tlo = __builtin_amdgcn_readfirstlane(tlo);
+    thi = __builtin_amdgcn_readfirstlane(thi);
+
+    float m[CT], l[CT];
+    kh_f32x4 o[CT][NF];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      m[c] = -INFINITY;
+      l[c] = 0.0f;
+#pragma unroll
+      for (int f = 0; f < NF; ++f) o[c][f] = kh_f32x4{0, 0, 0, 0};
+    }
+    const int first = tlo / kPtKeys, steps = thi > tlo ? (thi + kPtKeys - 1) / kPtKeys - first : 0;
+    const int per = (steps + a.nsplit - 1) / a.nsplit;
+    const int sb = first + split * per, se = min(first + steps, sb + per);
+    if (sb < se) {
+      uint4 qf[CT][NG];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)(row[c] / (uint32_t)a.nh) * a.qs +
+                            (int64_t)(row[c] % (uint32_t)a.nh) * a.qh + 8 * g;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          if (a.qvec) {
+            qf[c][j] = *reinterpret_cast<const uint4*>(q + 32 * j);
+          } else {
+            uint32_t e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = q[32 * j + i];
+            qf[c][j] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+          }
+        }
+      }
+      // lane i holds the page of the i-th of 64 tiles of 16 positions
+      int pgv = 0;
+      const auto pages = [&](int st) {
+        const int tok = min(max(st * kPtKeys + lane * 16, tlo & ~15), (thi - 1) & ~15);
+        const int col0 = max(tok, tlo) >> a.ps_log2;
+        const int pg = table[col0];
+        pgv = pg < 0 || pg >= a.pages ? -1 : pg;
+        if (pgv < 0) atomicOr(a.err, 2);
+      };
+      const auto page = [&](int st, int k) { return __builtin_amdgcn_readlane(pgv, ((st - sb) & 15) * 4 + k); };
+      const auto blk = [&](int pg) { return a.pool + ((int64_t)max(pg, 0) * a.nkv + h) * a.block; };
+      const auto load = [&](int st, C& x) {
+        const int in = (st * kPtKeys + ktile * 16) & (ps - 1);
+        const char* kb = blk(page(st, ktile));
+        ld_n<KF>(kb + P::kc() + (in + col) * (D / 2) + (g * NG + kj0) * 4, x.kw);
+        ld_n<KF>(kb + P::kp(ps) + ((in + col) * NG + kj0) * 4, x.kp);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int iv = (st * kPtKeys + vtb * 32 + q * 16) & (ps - 1);
+          const char* vb = blk(page(st, 2 * vtb + q));
+          const char* vw = vb + P::vc(ps) + (((iv >> 2) + g) * 16 + col) * (HN * 8) + (vf0 >> 2) * 4;
+#pragma unroll
+          for (int hh = 0; hh < C::VH; ++hh) {
+            x.vw[hh][2 * q] = *reinterpret_cast<const uint32_t*>(vw + hh * 4);
+            x.vw[hh][2 * q + 1] = *reinterpret_cast<const uint32_t*>(vw + HN * 4 + hh * 4);
+          }
+#pragma unroll
+          for (int gi = 0; gi < C::VG; ++gi)
+            ld_n<4>(vb + P::vp(ps) + (((vf0 >> 1) + gi) * ps + iv + 4 * g) * 4, &x.vp[gi][4 * q]);
+        }
+      };
+      const auto unpack = [&](int st, C& x) {
+        char* kbuf = s_buf + (st & 1) * S::kBufBytes;
+        char* vbuf = kbuf + kPtKeys * D * 2;
+#pragma unroll
+        for (int f = 0; f < KF; ++f) {
+          const float s = __uint_as_float(x.kp[f] & 0xffff0000u);
+          const float t = fmaf(-1024.0f, s, __uint_as_float(x.kp[f] << 16));
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const kh_f16x2 c = codes_f16(x.kw[f], i);
+            v[i] = fmaf((float)c.x, s, t);
+            v[i + 4] = fmaf((float)c.y, s, t);
+          }
+          uint4 w[1];
+          terms8<1>(v, w);
+          *reinterpret_cast<uint4*>(kbuf + ((ktile * NG + kj0 + f) * 64 + lane) * 16) = w[0];
+        }
+#pragma unroll
+        for (int gi = 0; gi < C::VG; ++gi) {
+          uint32_t top = x.vp[gi][0];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) top = max(top, x.vp[gi][e]);
+          uint32_t nan = 0;
+          if (__ballot(top >= 0x7fc00000u)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint64_t bal = __ballot(x.vp[gi][e] >= 0x7fc00000u);  // lanes of group g agree
+              if (x.vp[gi][e] >= 0x7fc00000u) x.vp[gi][e] = 0;
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (bal >> (16 * q) & 1) nan |= 1u << ((e < 4 ? 0 : 16) + 4 * q + (e & 3));
+            }
+          }
+          if (lane == 0 && (VF > 1 || (vf0 & 1) == 0)) s_nan[st & 1][(vf0 >> 1) + gi][vtb] = nan;
+          float s[8], t[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            s[e] = __uint_as_float(x.vp[gi][e] & 0xffff0000u);
+            t[e] = fmaf(-1024.0f, s[e], __uint_as_float(x.vp[gi][e] << 16));
+          }
+#pragma unroll
+          for (int ff = 0; ff < (VF < 2 ? 1 : 2); ++ff) {
+            const int fi = 2 * gi + ff;  // of the wave's
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const kh_f16x2 c = codes_f16(x.vw[VF <= 4 ? 0 : fi >> 2][e], (vf0 + fi) & 3);
+              v[2 * e] = fmaf((float)c.x, s[2 * e], t[2 * e]);
+              v[2 * e + 1] = fmaf((float)c.y, s[2 * e + 1], t[2 * e + 1]);
+            }
+            uint4 w[1];
+            terms8<1>(v, w);
+            *reinterpret_cast<uint4*>(vbuf + ((vtb * NF + vf0 + fi) * 64 + lane) * 16) = w[0];
+          }
+        }
+      };
+      const auto work = [&](int st) {
+        const int tok = st * kPtKeys;
+        if (tok + kPtKeys <= (int)wlo || tok >= (int)whi) return;
+        int okp = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) okp |= (page(st, k) >= 0 ? 1 : 0) << k;
+        const bool whole = tok >= (int)all_lo && tok + kPtKeys <= (int)all_hi && okp == 15;
+        const char* kbuf = s_buf + (st & 1) * S::kBufBytes;
+        const char* vbuf = kbuf + kPtKeys * D * 2;
+        kh_f32x4 s[CT][4];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+          for (int c = 0; c < CT; ++c) s[c][kt] = kh_f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            const uint4 kf = *reinterpret_cast<const uint4*>(kbuf + ((kt * NG + j) * 64 + lane) * 16);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) s[c][kt] = mfma16(kf, qf[c][j], s[c][kt]);
+          }
+        }
+        uint4 pf[CT][2];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          if (!whole) {
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const int j = tok + 16 * kt + 4 * g + r;
+                if (!(j >= lo[c] && j < hi[c] && (okp >> kt & 1))) s[c][kt][r] = -INFINITY;
+              }
+          }
+          float mx = s[c][0][0];
+#pragma unroll
+          for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[c][e >> 2][e & 3]);
+          if (__ballot((mx - m[c]) * a.c1 > kPtSlack)) {
+            const float mn = fmaxf(m[c], across_groups_max(mx));
+            const float alpha = mn == m[c] ? 1.0f : __builtin_amdgcn_exp2f((m[c] - mn) * a.c1);
+            l[c] *= alpha;
+#pragma unroll
+            for (int f = 0; f < NF; ++f) o[c][f] *= alpha;
+            m[c] = mn;
+          }
+          const float mc = m[c] == -INFINITY ? 0.0f : m[c] * a.c1;
+          float sum = 0.0f;
+#pragma unroll
+          for (int tb = 0; tb < 2; ++tb) {
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[c][2 * tb + (e >> 2)][e & 3], a.c1, -mc));
+            sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            uint4 w[1];
+            terms8<1>(p, w);
+            pf[c][tb] = w[0];
+          }
+          l[c] += sum;
+        }
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+          for (int f = 0; f < NF; ++f) {
+            const uint4 vf = *reinterpret_cast<const uint4*>(vbuf + ((tb * NF + f) * 64 + lane) * 16);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) o[c][f] = mfma16(vf, pf[c][tb], o[c][f]);
+          }
+        uint32_t any = 0;
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) any |= s_nan[st & 1][gi][0] | s_nan[st & 1][gi][1];
+        if (__builtin_amdgcn_readfirstlane(any)) {
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi) {
+            const uint64_t mask = s_nan[st & 1][gi][0] | (uint64_t)s_nan[st & 1][gi][1] << 32;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+              const int from = max(lo[c] - tok, 0), to = min(hi[c] - tok, kPtKeys);  // of the 64 positions
+              uint64_t see = to > from ? (~0ull >> (64 - (to - from))) << from : 0;
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (!(okp >> k & 1)) see &= ~(0xffffull << (16 * k));
+              if (mask & see) {
+                const float x = __uint_as_float(0x7fc00000u);
+                o[c][2 * gi] = o[c][2 * gi + 1] = kh_f32x4{x, x, x, x};
+              }
+            }
+          }
+        }
+      };
+
+      C x;
+      pages(sb);
+      load(sb, x);
+      unpack(sb, x);
+      for (int st = sb; st < se; ++st) {
+        __syncthreads();
+        // the pages of this step are read by work() below: new ones come after it, with
+        // the step's own load then
+        const bool more = st + 1 < se, turn = ((st + 1 - sb) & 15) == 0;
+        if (more && !turn) load(st + 1, x);
+        work(st);
+        if (more) {
+          if (turn) {
+            pages(st + 1);
+            load(st + 1, x);
+          }
+          unpack(st + 1, x);
+        }
+      }
+    }
+
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const float tot = across_groups_sum(l[c]);
+      const float M = m[c] * a.c1;
+      const bool some = hi[c] > lo[c];
+      if (!inside[c]) continue;
+      const int64_t t = row[c] / (uint32_t)a.nh;
+      const int head = (int)(row[c] - t * a.nh);
+      if (a.nsplit > 1) {
+        const int64_t at = (int64_t)row[c] * a.nsplit + split;
+        if (g == 0) a.part_ml[at] = make_float2(some ? M : -INFINITY, some ? tot : 0.0f);
+        if (some && sb < se) {
+#pragma unroll
+          for (int f = 0; f < NF; ++f)
+            *reinterpret_cast<float4*>(a.part_o + at * D + 16 * f + 4 * g) =
+                make_float4(o[c][f][0], o[c][f][1], o[c][f][2], o[c][f][3]);
+        }
+      } else {
+        const bool any = some && (M != -INFINITY || tot != 0.0f);
+        const float inv = any ? 1.0f / tot : 0.0f;
+        uint16_t* y = static_cast<uint16_t*>(a.out) + t * a.os + head * a.oh + 4 * g;
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+          pa_store4<D, uint16_t>(y + 16 * f, a.ovec, any ? o[c][f][0] * inv : 0.0f, any ? o[c][f][1] * inv : 0.0f,
+                                 any ? o[c][f][2] * inv : 0.0f, any ? o[c][f][3] * inv : 0.0f);
+        if (a.lse && g == 0) a.lse[row[c]] = any ? kLn2 * (M + __builtin_amdgcn_logf(tot)) : -INFINITY;
+      }
+    }
+  }
+}
+
 // Joins the parts of each row: W waves a (row, head), four elements a lane, so
 // that 256 / D parts of a wave are in flight at once.
 template <int D, typename T, int W>
@@ -599,20 +994,26 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaArgs a) {
 
 // How a call is cut: row tiles per (sequence, kv head) as the caller expects
 // them, and parts along the positions when the tiles alone do not fill the chip.
+constexpr int kPtWaves = 8;
+constexpr int kPtMinRows = 64;
 struct PaPlan {
+  bool many;  // paged_tile_kernel
   int64_t tiles, base;
   int nsplit;
 };
-static PaPlan pa_plan(int nkv, int nh, int64_t rows, int64_t batch, int64_t max_rows, int64_t max_len) {
+static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int64_t batch, int64_t max_rows,
+                      int64_t max_len) {
   PaPlan p;
-  const int64_t gs = nh / nkv;
+  const int64_t gs = nh / c->nkv;
   if (max_rows > rows) max_rows = rows;
-  p.tiles = (max_rows * gs + 15) / 16;
+  p.many = dtype == KH_DT_BF16 && max_rows * gs >= kPtMinRows;
+  const int64_t rb = p.many ? (c->d == 256 ? 16 : 32) * kPtWaves : 16;
+  p.tiles = (max_rows * gs + rb - 1) / rb;
   if (p.tiles < 1) p.tiles = 1;
   if (p.tiles > 65536) p.tiles = 65536;
-  p.base = batch * nkv * p.tiles;
-  int64_t want = (512 + p.base - 1) / p.base;
-  const int64_t most = (max_len + 255) / 256;
+  p.base = batch * c->nkv * p.tiles;
+  int64_t want = ((p.many ? 256 : 512) + p.base - 1) / p.base;
+  const int64_t most = p.many ? (max_len + 511) / 512 : (max_len + 255) / 256;
   if (want > most) want = most;
   if (want > kPaMaxSplit) want = kPaMaxSplit;
   p.nsplit = want < 1 ? 1 : (int)want;
@@ -623,18 +1024,34 @@ static int64_t pa_bytes(const PaPlan& p, int64_t rows, int nh, int d) {
 }
 
 template <int D, typename T>
-static void pa_launch(const PaArgs& a, int64_t blocks, hipStream_t st) {
-  hipLaunchKernelGGL((paged_rows_kernel<D, T>), dim3((unsigned)blocks), dim3(64 * kPaWaves), 0, st, a);
+static int pa_launch(const PaArgs& a, bool many, int64_t blocks, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (many) {
+      constexpr int lds = PtShape<D>::template lds<kPtWaves>();
+      static std::once_flag once;
+      static hipError_t arc = hipSuccess;
+      std::call_once(once, [] {
+        arc = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_tile_kernel<D, kPtWaves>),
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      });
+      KH_HIP(arc);
+      hipLaunchKernelGGL((paged_tile_kernel<D, kPtWaves>), dim3((unsigned)blocks), dim3(64 * kPtWaves), lds, st, a);
+    }
+  }
+  if (!many)
+    hipLaunchKernelGGL((paged_rows_kernel<D, T>), dim3((unsigned)blocks), dim3(64 * kPaWaves), 0, st, a);
   if (a.nsplit > 16)
     hipLaunchKernelGGL((paged_join_kernel<D, T, 4>), dim3((unsigned)(a.rows * a.nh)), dim3(256), 0, st, a);
   else if (a.nsplit > 1)
     hipLaunchKernelGGL((paged_join_kernel<D, T, 1>), dim3((unsigned)((a.rows * a.nh + 3) / 4)), dim3(256), 0, st, a);
+  KH_LAUNCHED();
+  return KH_OK;
 }
 template <typename T>
-static void pa_launch_d(int d, const PaArgs& a, int64_t blocks, hipStream_t st) {
-  if (d == 64) pa_launch<64, T>(a, blocks, st);
-  else if (d == 128) pa_launch<128, T>(a, blocks, st);
-  else pa_launch<256, T>(a, blocks, st);
+static int pa_launch_d(int d, const PaArgs& a, bool many, int64_t blocks, hipStream_t st) {
+  if (d == 64) return pa_launch<64, T>(a, many, blocks, st);
+  if (d == 128) return pa_launch<128, T>(a, many, blocks, st);
+  return pa_launch<256, T>(a, many, blocks, st);
 }
 
 static int pa_shape(const kh_paged_kv* c, int dtype, int64_t rows, int64_t batch, int num_heads, int64_t max_rows,
@@ -660,7 +1077,7 @@ extern "C" int kh_paged_kv_attention_workspace(const kh_paged_kv* c, int dtype, 
   KH_CHECK_ARG(bytes != nullptr, "null output");
   const int rc = pa_shape(c, dtype, rows, batch, num_heads, max_rows, max_len);
   if (rc != KH_OK) return rc;
-  *bytes = rows && batch ? pa_bytes(pa_plan(c->nkv, num_heads, rows, batch, max_rows, max_len), rows, num_heads, c->d)
+  *bytes = rows && batch ? pa_bytes(pa_plan(c, dtype, num_heads, rows, batch, max_rows, max_len), rows, num_heads, c->d)
                          : 0;
   return KH_OK;
 }
@@ -688,7 +1105,7 @@ extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void
   if (rows == 0 || batch == 0) return KH_OK;
   KH_CHECK_ARG(q_dev && off_dev && len_dev && table_dev && out_dev, "null argument");
   KH_CHECK_ARG(heads_dev || n_heads == 0, "null head list");
-  const PaPlan p = pa_plan(c->nkv, num_heads, rows, batch, max_rows, max_len);
+  const PaPlan p = pa_plan(c, dtype, num_heads, rows, batch, max_rows, max_len);
   const int64_t need = pa_bytes(p, rows, num_heads, c->d);
   if (need > 0 && (!ws_dev || ws_bytes < need)) {
     set_error("the workspace holds %lld bytes, %lld are needed", (long long)(ws_dev ? ws_bytes : 0),
@@ -733,8 +1150,6 @@ extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void
   a.part_ml = need ? reinterpret_cast<float2*>(a.part_o + rows * num_heads * p.nsplit * c->d) : nullptr;
   a.qvec = aligned16(q_dev, dtype, q_row_stride, q_head_stride) ? 1 : 0;
   a.ovec = aligned16(out_dev, dtype, out_row_stride, out_head_stride) ? 1 : 0;
-  if (dtype == KH_DT_F32) pa_launch_d<float>(c->d, a, blocks, as_stream(stream));
-  else pa_launch_d<uint16_t>(c->d, a, blocks, as_stream(stream));
-  KH_LAUNCHED();
-  return KH_OK;
+  return dtype == KH_DT_F32 ? pa_launch_d<float>(c->d, a, p.many, blocks, as_stream(stream))
+                            : pa_launch_d<uint16_t>(c->d, a, p.many, blocks, as_stream(stream));
 }

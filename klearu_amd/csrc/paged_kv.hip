@@ -7,8 +7,8 @@
 // m below every value and 15 s above every distance from it, no value is
 // clipped and each is off by at most s / 2.  Differences and quotients are f32
 // with one rounding each, so the codes are a function of x alone.  A group that
-// holds a value that is not finite, or whose range BF16 cannot hold, has s =
-// NaN, m = 0 and stands for NaN: no infinity ever enters the cache.
+// holds a value that is not finite, or of 2^100 and more, has s = NaN, m = 0 and
+// stands for NaN: no infinity ever enters the cache, and none comes of its sums.
 #include <new>
 
 #include "paged_kv.hpp"
@@ -25,12 +25,11 @@ __device__ __forceinline__ uint32_t bf16_down(float x) {
 }
 __device__ __forceinline__ uint32_t bf16_up(float x) { return (__float_as_uint(x) + 0xffffu) >> 16; }
 
-// minimum | scale << 16 of a group with range [lo, hi]; bad: it holds a value that is not finite.
+// minimum | scale << 16 of a group with range [lo, hi]; bad: it stands for NaN.
 __device__ __forceinline__ uint32_t kv_pair(float lo, float hi, bool bad) {
   const uint32_t m = bf16_down(lo);
   const uint32_t s = bf16_up(__fdiv_rn(__fsub_rn(hi, __uint_as_float(m << 16)), 15.0f));
-  if (bad || s >= 0x7f80u) return 0x7fc00000u;  // negative s cannot be: hi >= m
-  return m | s << 16;
+  return bad ? 0x7fc00000u : m | s << 16;  // s >= 0: hi >= m
 }
 __device__ __forceinline__ uint32_t kv_code(float x, uint32_t pair) {
   const float s = __uint_as_float(pair & 0xffff0000u), m = __uint_as_float(pair << 16);
@@ -38,7 +37,7 @@ __device__ __forceinline__ uint32_t kv_code(float x, uint32_t pair) {
   const float q = rintf(__fdiv_rn(__fsub_rn(x, m), s));
   return (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f);
 }
-__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ bool too_large(float x) { return (__float_as_uint(x) & 0x7fffffffu) >= 0x71800000u; }  // 2^100
 
 struct KvRows {
   char* pool;
@@ -175,7 +174,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a) {
       for (int i = 0; i < 8; ++i) {
         lo = fminf(lo, f[i]);
         hi = fmaxf(hi, f[i]);
-        bad |= not_finite(f[i]);
+        bad |= too_large(f[i]);
       }
       lo = fminf(lo, dppf<kDppQuadSwap1>(lo));
       hi = fmaxf(hi, dppf<kDppQuadSwap1>(hi));
@@ -213,7 +212,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a) {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         float lo = fminf(f[2 * q], f[2 * q + 1]), hi = fmaxf(f[2 * q], f[2 * q + 1]);
-        int bad = not_finite(f[2 * q]) || not_finite(f[2 * q + 1]);
+        int bad = too_large(f[2 * q]) || too_large(f[2 * q + 1]);
         lo = fminf(lo, dppf<kDppQuadSwap1>(lo));
         hi = fmaxf(hi, dppf<kDppQuadSwap1>(hi));
         bad |= dpp<kDppQuadSwap1>(bad);

@@ -21,7 +21,7 @@ def quantize(x):
     with np.errstate(all="ignore"):
         m = bf16_down(g.min(-1, keepdims=True))
         s = -bf16_down(-((g.max(-1, keepdims=True) - m) / np.float32(15)))
-        bad = ~np.isfinite(g).all(-1, keepdims=True) | ~np.isfinite(s)
+        bad = ~(np.abs(g) < np.float32(2.0 ** 100)).all(-1, keepdims=True)
         c = np.clip(np.rint((g - m) / s), 0, 15)
     c = np.where(s > 0, c, 0)
     c, s, m = np.where(bad, 0, c), np.where(bad, np.nan, s), np.where(bad, 0, m)
@@ -46,7 +46,7 @@ def seen(n, length, causal, window):
     return ok
 
 
-def attention(q, kraw, vraw, scale, causal=True, window=0, bf16=True):
+def attention(q, kraw, vraw, scale, causal=True, window=0, bf16=True, many=False):
     """One sequence: q [n, heads, dim] f64, kraw, vraw [length, kv, dim] f32 as appended ->
     (out, lse, tolerance of out, tolerance of lse), f64.
 
@@ -54,7 +54,8 @@ def attention(q, kraw, vraw, scale, causal=True, window=0, bf16=True):
     q (m - 128 s), so their magnitudes are B = scale sum |q| (271 s + |m|), summed by at most dim + 16
     additions; an exponential is off by 2^-21 and by 2^-22 of its argument; a weight that the second product
     takes is rounded to 8 bits (2^-8; f32 rows: three times 8, 2^-24) of p s c + p |m|; its sums over the positions have
-    magnitudes sum p (271 s + |m|) and at most length / 4 + 64 additions in a row; out is rounded last."""
+    magnitudes sum p (271 s + |m|) and at most length / 4 + 64 additions in a row; out is rounded last.  Tiles of
+    many BF16 rows (`many`) take keys and values rounded to 8 bits: 2^-8 of |q| |k| and of p |v| more."""
     n, heads, dim = q.shape
     length, kv = kraw.shape[:2]
     kc, ks, km = quantize(kraw)
@@ -79,10 +80,14 @@ def attention(q, kraw, vraw, scale, causal=True, window=0, bf16=True):
             w = p / np.where(some, tot, 1.0)[:, None]
             o = np.where(ok[:, :, None], w[:, :, None] * v[None, :, g], 0.0).sum(1)
             err = (dim + 16) * u * big + 2.0 ** -21 + 2.0 ** -22 * np.abs(np.where(ok, t - top[:, None], 0.0))
+            if many:
+                err = err + 2.0 ** -8 * scale * (np.abs(q[:, h]) @ np.abs(np.nan_to_num(k[:, g])).T)
             err = np.where(ok, err, 0.0)
             depth = (length / 4 + 64) * u
             sg = np.nan_to_num(vs[:, g])  # groups that stand for NaN have no tolerance
             mag = sg * vc[:, g] + np.abs(vm[:, g])
+            if many:
+                mag = mag + np.abs(np.nan_to_num(v[:, g]))
             tol[:, h] = ((w * err) @ np.abs(np.nan_to_num(v[:, g])) + (w * err).sum(-1)[:, None] * np.abs(o)
                          + up * (w @ mag) + depth * (w @ (271 * sg + np.abs(vm[:, g]))) + uo * np.abs(o))
         out[:, h] = np.where(some[:, None], o, 0.0)

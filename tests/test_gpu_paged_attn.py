@@ -26,10 +26,13 @@ class Case:
         zero = torch.zeros(len(lens), dtype=torch.int64).cuda()
         if sum(lens):
             self.cache.append(torch.cat(self.k).cuda(), torch.cat(self.v).cuda(), offsets(lens).cuda(), zero, self.table)
+        self.many = False  # whether the call takes tiles of many rows
         self.q = torch.from_numpy((rng.normal(0, qscale, (sum(rows), heads, dim))).astype(np.float32)).to(dtype)
 
     def run(self, **kw):
         kw.setdefault("return_lse", True)
+        n = max(1, -(-sum(self.rows) // len(self.rows)))
+        self.many = self.dtype == BF16 and min(kw.get("max_rows", n), sum(self.rows)) * self.heads // self.kv >= 64
         return self.cache.attention(self.q.cuda(), self.off, self.len, self.table, **kw)
 
     def check(self, got, causal=True, window=0, scale=None, on=None):
@@ -45,7 +48,7 @@ class Case:
             assert (out[at:at + first] == 0).all() and (lse[at:at + first] == -np.inf).all()
             if length:
                 o, l, to, tl = attention(q[first:], k.float().numpy(), v.float().numpy(),
-                                         self.dim ** -0.5 if scale is None else scale, causal, window, self.dtype == BF16)
+                                         self.dim ** -0.5 if scale is None else scale, causal, window, self.dtype == BF16, self.many)
                 if on is not None:
                     off = ~on[keep]
                     o[off], l[off], to[off], tl[off] = 0, -np.inf, 0, 0

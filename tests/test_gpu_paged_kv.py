@@ -100,12 +100,15 @@ def test_hard_values(kh):
     x[9, 0, :32] = -1000.0 - rng.random(32)
     x[10, 0, 0] = 1e30
     x[11, 0, :32] = np.float32(2.0 ** -126) * rng.random(32)
+    x[0, 0, 40] = -np.float32(2.0 ** 100)
+    x[1, 0, 40] = np.nextafter(np.float32(2.0 ** 100), np.float32(0))
     c = cache_of(1, 64, 1, 16)
     t, o, z = torch.zeros(1, 1, dtype=torch.int32).cuda(), offsets([12]).cuda(), torch.zeros(1, dtype=torch.int64).cuda()
     xd = torch.from_numpy(x).cuda()
     c.append(xd, xd, o, z, t)
     want = values(x)
     assert np.isnan(want[[4, 5, 7], 0, :32]).all() and np.isnan(want[6, 0, 32:]).all() and np.isfinite(want[6, 0, :32]).all()
+    assert np.isnan(want[0, 0, 32:]).all() and np.isfinite(want[1]).all()
     for got in c.gather(o, z, t, 12):
         same(got, want)
         g = got.cpu().numpy()
