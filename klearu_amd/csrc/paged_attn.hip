@@ -128,6 +128,13 @@ __device__ __forceinline__ float across_groups_sum(float v) {
   return across_groups(v, [](float x, float y) { return x + y; });
 }
 
+__device__ __forceinline__ uint32_t across_groups_or(uint32_t u) {
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t w = a[0] | a[1];
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return b[0] | b[1];
+}
+
 // a times the lane's row's (of sixteen) lane N of s; c plus a times the quad's lane N of s.
 template <int N>
 __device__ __forceinline__ float mul_row(float a, uint32_t s) {
@@ -549,17 +556,15 @@ __global__ __launch_bounds__(64 * kPaWaves, D == 64 ? 3 : D == 128 ? 2 : 1) void
 // A value's group that stands for NaN is unpacked as 0 and marked in a mask of its
 // positions: rows that see one of them get their NaN from the mask.
 constexpr int kPtKeys = 64;
+constexpr int kOnlyAlu = 0x6;  // what a scheduling barrier lets pass: vector and scalar arithmetic
 constexpr float kPtSlack = 6.0f;  // a maximum that is passed by less (in powers of two) is kept
 
 template <int D>
 struct PtShape {
   static constexpr int CT = D == 256 ? 1 : 2;  // column tiles of 16 rows a wave holds
   static constexpr int RW = 16 * CT;
-  static constexpr int kBufBytes = 2 * kPtKeys * D * 2;  // keys, then values
-  template <int NW>
-  static constexpr int lds() {
-    return 2 * kBufBytes;
-  }
+  static constexpr int kBuf = kPtKeys * D * 2;  // bytes of 64 keys or values
+  static constexpr int kLds = 4 * kBuf;         // two buffers of keys, two of values
 };
 
 typedef _Float16 kh_f16x2 __attribute__((ext_vector_type(2)));
@@ -672,12 +677,12 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
     tlo = __builtin_amdgcn_readfirstlane(tlo);
     thi = __builtin_amdgcn_readfirstlane(thi);
 
-    float m[CT], l[CT];
-    kh_f32x4 o[CT][NF];
+    float m[CT];
+    kh_f32x4 l[CT], o[CT][NF];  // l: a product with ones, all four alike
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       m[c] = -INFINITY;
-      l[c] = 0.0f;
+      l[c] = kh_f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int f = 0; f < NF; ++f) o[c][f] = kh_f32x4{0, 0, 0, 0};
     }
@@ -702,40 +707,49 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
           }
         }
       }
-      // lane i holds the page of the i-th of 64 tiles of 16 positions
-      int pgv = 0;
+      // Lane i holds the offset of the block of the i-th of 64 tiles of 16 positions: the next sixteen
+      // steps'.  Bits of okm say which pages there are, of these steps and (high) the next.
+      uint32_t blk_lo = 0, blk_hi = 0;
+      uint64_t okm = 0, okn = 0;
       const auto pages = [&](int st) {
         const int tok = min(max(st * kPtKeys + lane * 16, tlo & ~15), (thi - 1) & ~15);
-        const int col0 = max(tok, tlo) >> a.ps_log2;
-        const int pg = table[col0];
-        pgv = pg < 0 || pg >= a.pages ? -1 : pg;
-        if (pgv < 0) atomicOr(a.err, 2);
+        const int pg = table[max(tok, tlo) >> a.ps_log2];
+        const bool there = pg >= 0 && pg < a.pages;
+        if (!there) atomicOr(a.err, 2);
+        const uint64_t p = ((int64_t)(there ? pg : 0) * a.nkv + h) * a.block;
+        blk_lo = (uint32_t)p;
+        blk_hi = (uint32_t)(p >> 32);
+        okn = __ballot(there);
       };
-      const auto page = [&](int st, int k) { return __builtin_amdgcn_readlane(pgv, ((st - sb) & 15) * 4 + k); };
-      const auto blk = [&](int pg) { return a.pool + ((int64_t)max(pg, 0) * a.nkv + h) * a.block; };
+      const auto blk = [&](int st, int k) {
+        const int l = ((st - sb) & 15) * 4 + k;
+        const uint32_t x = __builtin_amdgcn_readlane(blk_lo, l), y = __builtin_amdgcn_readlane(blk_hi, l);
+        return a.pool + ((uint64_t)y << 32 | x);
+      };
+      const uint32_t koff = P::kc() + col * (D / 2) + (g * NG + kj0) * 4, kpoff = P::kp(ps) + (col * NG + kj0) * 4;
+      const uint32_t voff = P::vc(ps) + (g * 16 + col) * (HN * 8) + (vf0 >> 2) * 4;
+      const uint32_t vpoff = P::vp(ps) + ((vf0 >> 1) * ps + 4 * g) * 4;
       const auto load = [&](int st, C& x) {
         const int in = (st * kPtKeys + ktile * 16) & (ps - 1);
-        const char* kb = blk(page(st, ktile));
-        ld_n<KF>(kb + P::kc() + (in + col) * (D / 2) + (g * NG + kj0) * 4, x.kw);
-        ld_n<KF>(kb + P::kp(ps) + ((in + col) * NG + kj0) * 4, x.kp);
+        const char* kb = blk(st, ktile);
+        ld_n<KF>(kb + in * (D / 2) + koff, x.kw);
+        ld_n<KF>(kb + in * (NG * 4) + kpoff, x.kp);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const int iv = (st * kPtKeys + vtb * 32 + q * 16) & (ps - 1);
-          const char* vb = blk(page(st, 2 * vtb + q));
-          const char* vw = vb + P::vc(ps) + (((iv >> 2) + g) * 16 + col) * (HN * 8) + (vf0 >> 2) * 4;
+          const char* vb = blk(st, 2 * vtb + q);
+          const char* vw = vb + iv * (D / 2) + voff;
 #pragma unroll
           for (int hh = 0; hh < C::VH; ++hh) {
             x.vw[hh][2 * q] = *reinterpret_cast<const uint32_t*>(vw + hh * 4);
             x.vw[hh][2 * q + 1] = *reinterpret_cast<const uint32_t*>(vw + HN * 4 + hh * 4);
           }
 #pragma unroll
-          for (int gi = 0; gi < C::VG; ++gi)
-            ld_n<4>(vb + P::vp(ps) + (((vf0 >> 1) + gi) * ps + iv + 4 * g) * 4, &x.vp[gi][4 * q]);
+          for (int gi = 0; gi < C::VG; ++gi) ld_n<4>(vb + iv * 4 + gi * ps * 4 + vpoff, &x.vp[gi][4 * q]);
         }
       };
-      const auto unpack = [&](int st, C& x) {
-        char* kbuf = s_buf + (st & 1) * S::kBufBytes;
-        char* vbuf = kbuf + kPtKeys * D * 2;
+      const auto unpack_k = [&](int st, const C& x) {
+        char* kbuf = s_buf + (st & 1) * S::kBuf;
 #pragma unroll
         for (int f = 0; f < KF; ++f) {
           const float s = __uint_as_float(x.kp[f] & 0xffff0000u);
@@ -751,6 +765,9 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
           terms8<1>(v, w);
           *reinterpret_cast<uint4*>(kbuf + ((ktile * NG + kj0 + f) * 64 + lane) * 16) = w[0];
         }
+      };
+      // A group that stands for NaN counts as 0, and its positions go to the masks.
+      const auto mark_nan = [&](int st, C& x) {
 #pragma unroll
         for (int gi = 0; gi < C::VG; ++gi) {
           uint32_t top = x.vp[gi][0];
@@ -758,16 +775,23 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
           for (int e = 1; e < 8; ++e) top = max(top, x.vp[gi][e]);
           uint32_t nan = 0;
           if (__ballot(top >= 0x7fc00000u)) {
+            uint32_t from = 0x7fc00000u;
+            asm volatile("" : "+s"(from));  // keeps this behind its branch
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const uint64_t bal = __ballot(x.vp[gi][e] >= 0x7fc00000u);  // lanes of group g agree
-              if (x.vp[gi][e] >= 0x7fc00000u) x.vp[gi][e] = 0;
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                if (bal >> (16 * q) & 1) nan |= 1u << ((e < 4 ? 0 : 16) + 4 * q + (e & 3));
+              const uint32_t is = x.vp[gi][e] >= from ? 1u : 0u;
+              nan |= is << ((e < 4 ? 0 : 16) + 4 * g + (e & 3));
+              x.vp[gi][e] &= is - 1u;
             }
+            nan = across_groups_or(nan);
           }
           if (lane == 0 && (VF > 1 || (vf0 & 1) == 0)) s_nan[st & 1][(vf0 >> 1) + gi][vtb] = nan;
+        }
+      };
+      const auto unpack_v = [&](int st, const C& x) {
+        char* vbuf = s_buf + (2 + (st & 1)) * S::kBuf;
+#pragma unroll
+        for (int gi = 0; gi < C::VG; ++gi) {
           float s[8], t[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -790,119 +814,178 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
           }
         }
       };
-      const auto work = [&](int st) {
-        const int tok = st * kPtKeys;
-        if (tok + kPtKeys <= (int)wlo || tok >= (int)whi) return;
-        int okp = 0;
+      kh_f32x4 sc[CT][4];
+      uint4 pf[CT][2];
+      float mc[CT];
+      // Fragments are read one group ahead of the products that take them.
+      const auto scores = [&](int st) {
+        const char* kbuf = s_buf + (st & 1) * S::kBuf + lane * 16;
+        uint4 kf[2][NG];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) okp |= (page(st, k) >= 0 ? 1 : 0) << k;
-        const bool whole = tok >= (int)all_lo && tok + kPtKeys <= (int)all_hi && okp == 15;
-        const char* kbuf = s_buf + (st & 1) * S::kBufBytes;
-        const char* vbuf = kbuf + kPtKeys * D * 2;
-        kh_f32x4 s[CT][4];
+        for (int j = 0; j < NG; ++j) kf[0][j] = *reinterpret_cast<const uint4*>(kbuf + j * 1024);
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
+          if (kt < 3) {
 #pragma unroll
-          for (int c = 0; c < CT; ++c) s[c][kt] = kh_f32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int j = 0; j < NG; ++j) {
-            const uint4 kf = *reinterpret_cast<const uint4*>(kbuf + ((kt * NG + j) * 64 + lane) * 16);
-#pragma unroll
-            for (int c = 0; c < CT; ++c) s[c][kt] = mfma16(kf, qf[c][j], s[c][kt]);
+            for (int j = 0; j < NG; ++j)
+              kf[(kt + 1) & 1][j] = *reinterpret_cast<const uint4*>(kbuf + ((kt + 1) * NG + j) * 1024);
           }
+          __builtin_amdgcn_sched_barrier(kOnlyAlu);
+#pragma unroll
+          for (int c = 0; c < CT; ++c) sc[c][kt] = kh_f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int c = 0; c < CT; ++c) sc[c][kt] = mfma16(kf[kt & 1][j], qf[c][j], sc[c][kt]);
+          __builtin_amdgcn_sched_barrier(kOnlyAlu);
         }
-        uint4 pf[CT][2];
+      };
+      const auto whole = [&](int st, int ok) {
+        return st * kPtKeys >= (int)all_lo && (st + 1) * kPtKeys <= (int)all_hi && ok == 15;
+      };
+      const auto hide = [&](int st, int ok) {
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-          if (!whole) {
+          int from = lo[c] - st * kPtKeys - 4 * g;
+          asm volatile("" : "+v"(from));  // keeps this behind its branch: 32 selects of every step otherwise
+          const uint32_t span = (uint32_t)(hi[c] - lo[c]);
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt)
+          for (int kt = 0; kt < 4; ++kt) {
+            const uint32_t n = ok >> kt & 1 ? span : 0u;
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const int j = tok + 16 * kt + 4 * g + r;
-                if (!(j >= lo[c] && j < hi[c] && (okp >> kt & 1))) s[c][kt][r] = -INFINITY;
-              }
+            for (int r = 0; r < 4; ++r)
+              if ((uint32_t)(16 * kt + r - from) >= n) sc[c][kt][r] = -INFINITY;
           }
-          float mx = s[c][0][0];
+        }
+      };
+      float mx[CT];
+      const auto top = [&]() {
 #pragma unroll
-          for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[c][e >> 2][e & 3]);
-          if (__ballot((mx - m[c]) * a.c1 > kPtSlack)) {
-            const float mn = fmaxf(m[c], across_groups_max(mx));
+        for (int c = 0; c < CT; ++c) {
+          mx[c] = sc[c][0][0];
+#pragma unroll
+          for (int e = 1; e < 16; ++e) mx[c] = fmaxf(mx[c], sc[c][e >> 2][e & 3]);
+        }
+      };
+      const auto rescale = [&]() {
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          if (__ballot((mx[c] - m[c]) * a.c1 > kPtSlack)) {
+            const float mn = fmaxf(m[c], across_groups_max(mx[c]));
             const float alpha = mn == m[c] ? 1.0f : __builtin_amdgcn_exp2f((m[c] - mn) * a.c1);
             l[c] *= alpha;
 #pragma unroll
             for (int f = 0; f < NF; ++f) o[c][f] *= alpha;
             m[c] = mn;
+            mc[c] = mn == -INFINITY ? 0.0f : mn * a.c1;
           }
-          const float mc = m[c] == -INFINITY ? 0.0f : m[c] * a.c1;
-          float sum = 0.0f;
-#pragma unroll
-          for (int tb = 0; tb < 2; ++tb) {
-            float p[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[c][2 * tb + (e >> 2)][e & 3], a.c1, -mc));
-            sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-            uint4 w[1];
-            terms8<1>(p, w);
-            pf[c][tb] = w[0];
-          }
-          l[c] += sum;
         }
+      };
+      const auto weights = [&](int tb) {
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
+        for (int c = 0; c < CT; ++c) {
+          float p[8];
 #pragma unroll
-          for (int f = 0; f < NF; ++f) {
-            const uint4 vf = *reinterpret_cast<const uint4*>(vbuf + ((tb * NF + f) * 64 + lane) * 16);
+          for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(sc[c][2 * tb + (e >> 2)][e & 3], a.c1, -mc[c]));
+          uint4 w[1];
+          terms8<1>(p, w);
+          pf[c][tb] = w[0];
+        }
+      };
+      constexpr int VQ = 4;  // value fragments of a group
+      uint4 vf[2][VQ];
+      const auto values = [&](int st, int k) {  // group k of step st's
+        const char* vbuf = s_buf + (2 + (st & 1)) * S::kBuf + lane * 16;
 #pragma unroll
-            for (int c = 0; c < CT; ++c) o[c][f] = mfma16(vf, pf[c][tb], o[c][f]);
+        for (int i = 0; i < VQ; ++i) vf[k & 1][i] = *reinterpret_cast<const uint4*>(vbuf + (k * VQ + i) * 1024);
+      };
+      const auto sum_values = [&](int st) {  // values(st, 0) is under way
+        const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+#pragma unroll
+        for (int k = 0; k < 2 * NF / VQ; ++k) {
+          const int tb = k * VQ / NF;
+          if (k + 1 < 2 * NF / VQ) values(st, k + 1);
+          __builtin_amdgcn_sched_barrier(kOnlyAlu);
+          if (k * VQ % NF == 0) {
+#pragma unroll
+            for (int c = 0; c < CT; ++c) l[c] = mfma16(ones, pf[c][tb], l[c]);
           }
+#pragma unroll
+          for (int i = 0; i < VQ; ++i)
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+              const int f = (k * VQ + i) % NF;
+              o[c][f] = mfma16(vf[k & 1][i], pf[c][tb], o[c][f]);
+            }
+          __builtin_amdgcn_sched_barrier(kOnlyAlu);
+        }
+      };
+      const auto spread_nan = [&](int st, int ok) {
         uint32_t any = 0;
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi) any |= s_nan[st & 1][gi][0] | s_nan[st & 1][gi][1];
-        if (__builtin_amdgcn_readfirstlane(any)) {
+        if (!__builtin_amdgcn_readfirstlane(any)) return;
+        int tok = st * kPtKeys;
+        asm volatile("" : "+s"(tok));  // keeps this behind its branch
 #pragma unroll
-          for (int gi = 0; gi < NG; ++gi) {
-            const uint64_t mask = s_nan[st & 1][gi][0] | (uint64_t)s_nan[st & 1][gi][1] << 32;
+        for (int gi = 0; gi < NG; ++gi) {
+          const uint64_t mask = s_nan[st & 1][gi][0] | (uint64_t)s_nan[st & 1][gi][1] << 32;
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-              const int from = max(lo[c] - tok, 0), to = min(hi[c] - tok, kPtKeys);  // of the 64 positions
-              uint64_t see = to > from ? (~0ull >> (64 - (to - from))) << from : 0;
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (!(okp >> k & 1)) see &= ~(0xffffull << (16 * k));
-              if (mask & see) {
-                const float x = __uint_as_float(0x7fc00000u);
-                o[c][2 * gi] = o[c][2 * gi + 1] = kh_f32x4{x, x, x, x};
-              }
+          for (int c = 0; c < CT; ++c) {
+            const int from = max(lo[c] - tok, 0), to = min(hi[c] - tok, kPtKeys);  // of the 64 positions
+            uint64_t see = to > from ? (~0ull >> (64 - (to - from))) << from : 0;
+            for (int k = 0; k < 4; ++k)
+              if (!(ok >> k & 1)) see &= ~(0xffffull << (16 * k));
+            if (mask & see) {
+              const float x = __uint_as_float(0x7fc00000u);
+              o[c][2 * gi] = o[c][2 * gi + 1] = kh_f32x4{x, x, x, x};
             }
           }
         }
       };
 
+#pragma unroll
+      for (int c = 0; c < CT; ++c) mc[c] = 0.0f;
+      const bool busy = whi > wlo;  // some row of the wave sees something
       C x;
       pages(sb);
       load(sb, x);
-      unpack(sb, x);
+      unpack_k(sb, x);
+      mark_nan(sb, x);
+      unpack_v(sb, x);
+      if (sb + 1 < se) load(sb + 1, x);
       for (int st = sb; st < se; ++st) {
         __syncthreads();
-        // the pages of this step are read by work() below: new ones come after it, with
-        // the step's own load then
-        const bool more = st + 1 < se, turn = ((st + 1 - sb) & 15) == 0;
-        if (more && !turn) load(st + 1, x);
-        work(st);
-        if (more) {
-          if (turn) {
-            pages(st + 1);
-            load(st + 1, x);
-          }
-          unpack(st + 1, x);
+        if (st + 1 < se) {
+          unpack_k(st + 1, x);
+          mark_nan(st + 1, x);
+          unpack_v(st + 1, x);
+        }
+        // pages() for the next sixteen steps comes two steps before them
+        const int i = (st - sb) & 15;
+        if (i == 14) okm = okn;
+        if (st + 2 < se) {
+          if (i == 14) pages(st + 2);
+          load(st + 2, x);
+        }
+        const int ok = (int)((i >= 14 ? okm : okn) >> (4 * i)) & 15;
+        if (busy) {
+          scores(st);
+          values(st, 0);
+          if (!whole(st, ok)) hide(st, ok);
+          top();
+          rescale();
+          weights(0);
+          weights(1);
+          sum_values(st);
+          spread_nan(st, ok);
         }
       }
     }
 
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      const float tot = across_groups_sum(l[c]);
+      const float tot = l[c][0];
       const float M = m[c] * a.c1;
       const bool some = hi[c] > lo[c];
       if (!inside[c]) continue;
@@ -1027,7 +1110,7 @@ template <int D, typename T>
 static int pa_launch(const PaArgs& a, bool many, int64_t blocks, hipStream_t st) {
   if constexpr (sizeof(T) == 2) {
     if (many) {
-      constexpr int lds = PtShape<D>::template lds<kPtWaves>();
+      constexpr int lds = PtShape<D>::kLds;
       static std::once_flag once;
       static hipError_t arc = hipSuccess;
       std::call_once(once, [] {
