@@ -31,11 +31,31 @@ __device__ __forceinline__ uint32_t kv_pair(float lo, float hi, bool bad) {
   const uint32_t s = bf16_up(__fdiv_rn(__fsub_rn(hi, __uint_as_float(m << 16)), 15.0f));
   return bad ? 0x7fc00000u : m | s << 16;  // s >= 0: hi >= m
 }
-__device__ __forceinline__ uint32_t kv_code(float x, uint32_t pair) {
-  const float s = __uint_as_float(pair & 0xffff0000u), m = __uint_as_float(pair << 16);
+__device__ __forceinline__ uint32_t kv_code(float x, float m, float s) {
   if (!(s > 0.0f)) return 0;
   const float q = rintf(__fdiv_rn(__fsub_rn(x, m), s));
   return (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f);
+}
+// The codes of eight values, four bits each.  x - m over s lies in [0, 15 + 2^-20]
+// and a product with the reciprocal is off by less than 1e-5 from it, so its
+// nearest whole number is the quotient's unless it lies that near to a half (or s
+// has no reciprocal): those eight are divided.
+__device__ __forceinline__ uint32_t kv_codes8(const float (&f)[8], uint32_t pair) {
+  const float s = __uint_as_float(pair & 0xffff0000u), m = __uint_as_float(pair << 16);
+  const float inv = __builtin_amdgcn_rcpf(s);
+  bool sure = true;
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 7; i >= 0; --i) {
+    const float q = (f[i] - m) * inv, c = rintf(q);
+    sure = sure && fabsf(q - c) < 0.49999f;  // not where it is NaN
+    w = w << 4 | (uint32_t)(int)c;
+  }
+  if (sure) return w;
+  w = 0;
+#pragma unroll
+  for (int i = 7; i >= 0; --i) w = w << 4 | kv_code(f[i], m, s);
+  return w;
 }
 __device__ __forceinline__ bool too_large(float x) { return (__float_as_uint(x) & 0x7fffffffu) >= 0x71800000u; }  // 2^100
 
@@ -86,7 +106,7 @@ struct AppendArgs {
   const int64_t* pos;  // rotary positions of the rows, or nullptr: their places in the cache
   const float2* table;
   int64_t max_pos;
-  int rot, half_layout;
+  int rot, half_layout, mode;
   int* rope_err;
   int kvec, vvec;  // 16-byte loads
 };
@@ -132,108 +152,264 @@ __device__ __forceinline__ void rotated8(const T* __restrict__ x, int d, int rot
   }
 }
 
-// Blocks with blockIdx.y = 0 append keys, D / 8 lanes a row with eight
-// neighbouring values each (four lanes share a group); the others append
-// values, D / 4 lanes a row with the four values of one u16 each (the sixteen
-// lanes of a DPP row share two groups).
-template <typename T, int D>
-__global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a) {
-  __shared__ int64_t s_off[kSeqLds];
-  constexpr int NG = D / kKvGroup, HN = D / 64;
-  using P = KvParts<D>;
-  const int64_t* off = stage_off(a.r, s_off);
-  const int ps = 1 << a.r.ps_log2;
-  const int64_t units = a.r.rows * a.r.nkv;
-  if (blockIdx.y == 0) {
-    constexpr int L = D / 8, R = kKvThreads / L;
-    const int c = threadIdx.x % L, j = c >> 2, g = c & 3;
-    for (int64_t u = (int64_t)blockIdx.x * R + threadIdx.x / L; u < units; u += (int64_t)gridDim.x * R) {
-      const int64_t t = u / a.r.nkv;
-      const int h = (int)(u - t * a.r.nkv);
-      char* blk = nullptr;
-      int64_t p = 0;
-      int at = kv_place(a.r, off, t, h, &blk, &p);
-      const float2* tab = a.table;
-      if (tab && at >= 0) {
-        if (a.pos) p = a.pos[t];
-        if (p < 0 || p >= a.max_pos) {
-          atomicOr(a.rope_err, 1);
-          at = -1;
-        } else
-          tab += p * (a.rot >> 1);
-      }
-      float f[8];
-      // the lanes of a group take the same way: `at` is the row's
-      if (at < 0) continue;
-      const T* x = static_cast<const T*>(a.k) + t * a.ks + h * a.kh;
-      if (tab) rotated8(x, 8 * c, a.rot, a.half_layout, a.kvec, tab, f);
-      else load8(x + 8 * c, a.kvec, f);
-      float lo = f[0], hi = f[0];
-      int bad = 0;
+// The quads (four positions that share bytes) that the rows of sequences c0 ..
+// c0 + nb - 1 touch: s_q[i] of them lie before sequence c0 + i.  The whole block
+// takes part; returns their number.
+constexpr int kSeqChunk = 1024;
+__device__ __forceinline__ int quads_of(int64_t n, int64_t start) {
+  if (n <= 0) return 0;
+  // a start past 2^40 is out of every table: one quad reports it
+  if (start <= -((int64_t)1 << 40) || start >= (int64_t)1 << 40) return 1;
+  return (int)(((start + n - 1) >> 2) - (start >> 2) + 1);
+}
+__device__ __forceinline__ int stage_quads(const KvRows& a, int64_t c0, int nb, int* s_q, int* wsum, int* s_tot) {
+  constexpr int E = kSeqChunk / kKvThreads;
+  int n[E], sum = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        lo = fminf(lo, f[i]);
-        hi = fmaxf(hi, f[i]);
-        bad |= too_large(f[i]);
-      }
-      lo = fminf(lo, dppf<kDppQuadSwap1>(lo));
-      hi = fmaxf(hi, dppf<kDppQuadSwap1>(hi));
-      bad |= dpp<kDppQuadSwap1>(bad);
-      lo = fminf(lo, dppf<kDppQuadSwap2>(lo));
-      hi = fmaxf(hi, dppf<kDppQuadSwap2>(hi));
-      bad |= dpp<kDppQuadSwap2>(bad);
-      const uint32_t pair = kv_pair(lo, hi, bad != 0);
-      uint32_t w = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w |= kv_code(f[i], pair) << (4 * i);
-      *reinterpret_cast<uint32_t*>(blk + P::kc() + at * (D / 2) + (g * NG + j) * 4) = w;
-      if (g == 0) *reinterpret_cast<uint32_t*>(blk + P::kp(ps) + (at * NG + j) * 4) = pair;
+  for (int e = 0; e < E; ++e) {
+    const int i = threadIdx.x * E + e;
+    n[e] = 0;
+    if (i < nb) {
+      n[e] = quads_of(min(a.off[c0 + i + 1], a.rows) - max(a.off[c0 + i], (int64_t)0), a.start[c0 + i]);
     }
-  } else {
-    constexpr int L = D / 4, R = kKvThreads / L;
-    const int c = threadIdx.x % L, r = c & 15, hf = c >> 4;
-    for (int64_t u = (int64_t)blockIdx.x * R + threadIdx.x / L; u < units; u += (int64_t)gridDim.x * R) {
-      const int64_t t = u / a.r.nkv;
-      const int h = (int)(u - t * a.r.nkv);
-      char* blk = nullptr;
-      int64_t p = 0;
-      int at = kv_place(a.r, off, t, h, &blk, &p);
-      if (a.table && at >= 0) {  // a row without a rotation is not appended at all
-        if (a.pos) p = a.pos[t];
-        if (p < 0 || p >= a.max_pos) at = -1;
-      }
-      if (at < 0) continue;
-      const T* x = static_cast<const T*>(a.v) + t * a.vs + h * a.vh + 64 * hf + r;
-      float f[4];
+    sum += n[e];
+  }
+  int at = block_excl_scan(sum, wsum, s_tot);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) f[n] = load_f32(x + 16 * n);
-      uint32_t w = 0;
-      uint32_t pairs[2];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        float lo = fminf(f[2 * q], f[2 * q + 1]), hi = fmaxf(f[2 * q], f[2 * q + 1]);
-        int bad = too_large(f[2 * q]) || too_large(f[2 * q + 1]);
-        lo = fminf(lo, dppf<kDppQuadSwap1>(lo));
-        hi = fmaxf(hi, dppf<kDppQuadSwap1>(hi));
-        bad |= dpp<kDppQuadSwap1>(bad);
-        lo = fminf(lo, dppf<kDppQuadSwap2>(lo));
-        hi = fmaxf(hi, dppf<kDppQuadSwap2>(hi));
-        bad |= dpp<kDppQuadSwap2>(bad);
-        lo = fminf(lo, dppf<kDppRowHalfMirror>(lo));
-        hi = fmaxf(hi, dppf<kDppRowHalfMirror>(hi));
-        bad |= dpp<kDppRowHalfMirror>(bad);
-        lo = fminf(lo, dppf<kDppRowMirror>(lo));
-        hi = fmaxf(hi, dppf<kDppRowMirror>(hi));
-        bad |= dpp<kDppRowMirror>(bad);
-        pairs[q] = kv_pair(lo, hi, bad != 0);
-        w |= kv_code(f[2 * q], pairs[q]) << (8 * q);
-        w |= kv_code(f[2 * q + 1], pairs[q]) << (8 * q + 4);
+  for (int e = 0; e < E; ++e) {
+    s_q[threadIdx.x * E + e] = at;
+    at += n[e];
+  }
+  __syncthreads();
+  return *s_tot;
+}
+
+// How the rows' keys are rotated: not at all, pieces of eight elements by their
+// pairs, or element by element (any rot).
+constexpr int kRotNone = 0, kRotHalf = 1, kRotInterleaved = 2, kRotAny = 3;
+
+// Up to 64 sequences: lane i holds sequence i's quads and those before it.
+struct WaveSeqs {
+  int before = 0, n = 0, o0 = 0, o1 = 0;
+  int64_t start = 0;
+};
+__device__ __forceinline__ int64_t readlane64(int64_t v, int l) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, l), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), l);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// A wave takes a quad and the heads of one unit: D / 8 lanes a position with eight
+// neighbouring values each, so four lanes share a group.  blockIdx.y: keys, values.
+// Keys leave as they are, a word a lane.  The u16 of a value's layout gathers the
+// nibbles of four lanes (c, c ^ 2, c ^ 4, c ^ 6), and a quad's four positions
+// share 16-byte pieces: they are put together in LDS and stored whole where all
+// four are appended, and as u16 where they are not.
+template <typename T, int D, int MODE, bool VAL>
+__device__ __forceinline__ void append_part(const AppendArgs& a, int units, int hpu, int* s_q, int* s_wsum, int* s_tot,
+                                            uint16_t* s_v) {
+  using P = KvParts<D>;
+  constexpr int NG = D / kKvGroup, HN = D / 64, L = D / 8;
+  constexpr int TP = 64 / L < 4 ? 64 / L : 4, PASS = 4 / TP;  // positions at a time
+  constexpr int HW = D == 64 ? 2 : 1;                         // heads at a time
+  const int lane = threadIdx.x & 63, c = lane % L, j = c >> 2, g = c & 3;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int sub = D == 64 ? lane >> 5 : 0, tp = (lane / L) % TP;
+  const int ps = 1 << a.r.ps_log2;
+  const bool vec = VAL ? a.vvec : a.kvec;
+  const int64_t srow = VAL ? a.vs : a.ks, shead = VAL ? a.vh : a.kh;
+  const T* src = static_cast<const T*>(VAL ? a.v : a.k) + tp * srow + 8 * c;
+  const bool first_half = 8 * c < (a.rot >> 1);
+  const bool turns = MODE == kRotHalf || MODE == kRotInterleaved ? 8 * c < a.rot : false;
+  const int other = first_half ? a.rot >> 1 : -(a.rot >> 1);  // the pairs' other elements (kRotHalf)
+  const bool few = a.r.batch <= 64;
+  for (int64_t c0 = 0; c0 < a.r.batch; c0 += kSeqChunk) {
+    const int nb = (int)min((int64_t)kSeqChunk, a.r.batch - c0);
+    WaveSeqs ws;
+    int quads;
+    if (few) {
+      if (lane < nb) {
+        ws.o0 = (int)max(a.r.off[lane], (int64_t)0);
+        ws.o1 = (int)min(a.r.off[lane + 1], a.r.rows);
+        ws.start = a.r.start[lane];
+        ws.n = quads_of(ws.o1 - ws.o0, ws.start);
       }
-      uint16_t* vc = reinterpret_cast<uint16_t*>(blk + P::vc(ps));
-      vc[((((at >> 2) * 16 + r) * 2 + ((at >> 1) & 1)) * HN + hf) * 2 + (at & 1)] = (uint16_t)w;
-      if (r < 2) *reinterpret_cast<uint32_t*>(blk + P::vp(ps) + ((2 * hf + r) * ps + at) * 4) = r ? pairs[1] : pairs[0];
+      const int incl = wave_incl_scan(ws.n);
+      ws.before = incl - ws.n;
+      quads = __builtin_amdgcn_readlane(incl, 63);
+    } else {
+      if (c0) __syncthreads();
+      quads = stage_quads(a.r, c0, nb, s_q, s_wsum, s_tot);
+    }
+    const uint32_t end = (uint32_t)quads * (uint32_t)units;  // below 2^31 (checked on the host)
+    for (uint32_t u = blockIdx.x * (kKvThreads / 64) + wave; u < end; u += gridDim.x * (kKvThreads / 64)) {
+      const int qi = (int)(u / (uint32_t)units), h0 = (int)(u - (uint32_t)qi * (uint32_t)units) * hpu;
+      int lo = 0;  // the sequence: the last one with no more than qi quads before it, and some of its own
+      int o0, o1, first;
+      int64_t start;
+      if (few) {
+        lo = 63 - __builtin_clzll(__ballot(ws.n > 0 && ws.before <= qi));
+        o0 = __builtin_amdgcn_readlane(ws.o0, lo);
+        o1 = __builtin_amdgcn_readlane(ws.o1, lo);
+        start = readlane64(ws.start, lo);
+        first = __builtin_amdgcn_readlane(ws.before, lo);
+      } else {
+        int hi = nb;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (s_q[mid] <= qi) lo = mid;
+          else hi = mid;
+        }
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        o0 = (int)max(a.r.off[c0 + lo], (int64_t)0);
+        o1 = (int)min(a.r.off[c0 + lo + 1], a.r.rows);
+        start = a.r.start[c0 + lo];
+        first = __builtin_amdgcn_readfirstlane(s_q[lo]);
+      }
+      const int64_t p0 = ((start >> 2) + (qi - first)) * 4;  // the quad's first position
+      const int t0 = (int)(o0 + (p0 - start));               // and its row, which may lie up to 3 before o0
+      const int64_t colm = p0 >> a.r.ps_log2;
+      int pg = -1;
+      if (p0 < 0 || colm >= a.r.cols) {
+        if (lane == 0) atomicOr(a.r.err, 1);
+      } else {
+        pg = __builtin_amdgcn_readfirstlane(a.r.table[(c0 + lo) * a.r.table_stride + colm]);
+        if (pg < 0 || pg >= a.r.pages) {
+          pg = -1;
+          if (lane == 0) atomicOr(a.r.err, 2);
+        }
+      }
+      if (pg < 0) continue;
+      const int at0 = (int)(p0 & (ps - 1));
+      // the lane's positions
+      bool on[PASS];
+      const float2* tab[PASS];
+      float2 cs[MODE == kRotHalf || MODE == kRotInterleaved ? PASS : 1][8];
+      bool mine = true;
+#pragma unroll
+      for (int k = 0; k < PASS; ++k) {
+        const int t = t0 + k * TP + tp;
+        on[k] = t >= o0 && t < o1;
+        tab[k] = nullptr;
+        if (a.table && on[k]) {  // a row without a rotation is not appended at all
+          const int64_t r = a.pos ? a.pos[t] : p0 + k * TP + tp;
+          if (r < 0 || r >= a.max_pos) {
+            if (!VAL) atomicOr(a.rope_err, 1);
+            on[k] = false;
+          } else
+            tab[k] = a.table + r * (a.rot >> 1);
+        }
+        mine = mine && on[k];
+        // the pairs of the lane's piece, for every head
+        if (MODE == kRotHalf && on[k] && turns) {
+          const int e = first_half ? 8 * c : 8 * c - (a.rot >> 1);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            cs[k][i] = tab[k][e + i];
+            cs[k][i].y = first_half ? -cs[k][i].y : cs[k][i].y;
+          }
+        }
+        if (MODE == kRotInterleaved && on[k] && turns) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) cs[k][i] = tab[k][4 * c + i];
+        }
+      }
+      const bool all = __ballot(!mine) == 0;
+      const T* x0 = src + t0 * srow + (h0 + sub) * shead;
+      const int nh = min(hpu, a.r.nkv - h0);  // heads of this unit
+      char* blk = a.r.pool + ((int64_t)pg * a.r.nkv + h0 + sub) * a.r.block;
+      for (int h1 = 0; h1 < nh; h1 += HW, x0 += HW * shead, blk += HW * a.r.block) {
+        const bool there = HW == 1 || h1 + sub < nh;
+#pragma unroll
+        for (int k = 0; k < PASS; ++k) {
+          const bool act = on[k] && there;
+          const int at = at0 + k * TP + tp;
+          float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+          if (act) {
+            const T* x = x0 + k * TP * srow;
+            if (MODE == kRotAny) {
+              rotated8(x - 8 * c, 8 * c, a.rot, a.half_layout, vec, tab[k], f);
+            } else {
+              load8(x, vec, f);
+              if (MODE == kRotHalf && turns) {
+                float o[8];
+                load8(x + other, vec, o);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = f[i] * cs[k][i].x + o[i] * cs[k][i].y;
+              }
+              if (MODE == kRotInterleaved && turns) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float y0 = f[2 * i], y1 = f[2 * i + 1];
+                  f[2 * i] = y0 * cs[k][i].x - y1 * cs[k][i].y;
+                  f[2 * i + 1] = y1 * cs[k][i].x + y0 * cs[k][i].y;
+                }
+              }
+            }
+          }
+          float lo8 = fminf(fminf(fminf(f[0], f[1]), fminf(f[2], f[3])), fminf(fminf(f[4], f[5]), fminf(f[6], f[7])));
+          float hi8 = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+          int bad = __builtin_isunordered(f[0], f[1]) | __builtin_isunordered(f[2], f[3]) |
+                    __builtin_isunordered(f[4], f[5]) | __builtin_isunordered(f[6], f[7]);
+          lo8 = fminf(lo8, dppf<kDppQuadSwap1>(lo8));
+          hi8 = fmaxf(hi8, dppf<kDppQuadSwap1>(hi8));
+          bad |= dpp<kDppQuadSwap1>(bad);
+          lo8 = fminf(lo8, dppf<kDppQuadSwap2>(lo8));
+          hi8 = fmaxf(hi8, dppf<kDppQuadSwap2>(hi8));
+          bad |= dpp<kDppQuadSwap2>(bad);
+          const bool nan = bad || too_large(lo8) || too_large(hi8);
+          const uint32_t pair = kv_pair(lo8, hi8, nan);
+          const uint32_t w = nan ? 0 : kv_codes8(f, pair);
+          if (!VAL) {
+            if (act) {
+              *reinterpret_cast<uint32_t*>(blk + P::kc() + at * (D / 2) + (g * NG + j) * 4) = w;
+              if (g == 0) *reinterpret_cast<uint32_t*>(blk + P::kp(ps) + (at * NG + j) * 4) = pair;
+            }
+            continue;
+          }
+          // d = 8 c + i = 64 hf + 16 n + r: nibble n of the u16 of r = 8 (c & 1) + i
+          const int n = (c >> 1) & 3, hf = c >> 3;
+          uint32_t v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = w >> (8 * i);
+            v[i] = ((x & 15u) | (x & 0xf0u) << 12) << (4 * n);
+            v[i] |= (uint32_t)dpp<kDppQuadSwap2>((int)v[i]);
+            // lane c ^ 4: the mirror of eight lanes, then of four
+            v[i] |= (uint32_t)dpp<0x1B>(dpp<kDppRowHalfMirror>((int)v[i]));
+          }
+          // of the four lanes that now hold the same eight u16, each takes two
+          const uint32_t two = n == 0 ? v[0] : n == 1 ? v[1] : n == 2 ? v[2] : v[3];
+          const int r = 8 * (c & 1) + 2 * n, tk = at & 3;
+          const int o = ((r * 2 + (tk >> 1)) * HN + hf) * 2 + (tk & 1);
+          if (all) {
+            s_v[sub * D + o] = (uint16_t)two;
+            s_v[sub * D + o + 4 * HN] = (uint16_t)(two >> 16);
+          } else if (act) {
+            uint16_t* vc = reinterpret_cast<uint16_t*>(blk + P::vc(ps)) + (at >> 2) * D;
+            vc[o] = (uint16_t)two;
+            vc[o + 4 * HN] = (uint16_t)(two >> 16);
+          }
+          if (act && g == 0) *reinterpret_cast<uint32_t*>(blk + P::vp(ps) + (j * ps + at) * 4) = pair;
+        }
+        if (VAL && all) {
+          __builtin_amdgcn_wave_barrier();
+          const int l = lane & (D == 64 ? 31 : 63);
+          if (l < D / 8 && there)
+            *reinterpret_cast<uint4*>(blk + P::vc(ps) + (at0 >> 2) * (2 * D) + l * 16) =
+                *reinterpret_cast<const uint4*>(&s_v[sub * D + l * 8]);
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
     }
   }
+}
+
+template <typename T, int D, int MODE>
+__global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a, int units, int hpu) {
+  __shared__ int s_q[kSeqChunk], s_wsum[kKvThreads / 64], s_tot;
+  __shared__ __align__(16) uint16_t s_v[kKvThreads / 64][D == 64 ? 2 * D : D];
+  if (blockIdx.y == 0) append_part<T, D, MODE, false>(a, units, hpu, s_q, s_wsum, &s_tot, nullptr);
+  else append_part<T, D, kRotNone, true>(a, units, hpu, s_q, s_wsum, &s_tot, s_v[threadIdx.x >> 6]);
 }
 
 struct GatherArgs {
@@ -282,11 +458,20 @@ __global__ __launch_bounds__(kKvThreads) void kv_gather_kernel(GatherArgs a) {
   }
 }
 
+template <typename T, int D>
+static void append_launch_m(const AppendArgs& a, dim3 g, int units, int hpu, hipStream_t st) {
+  const dim3 blk(kKvThreads);
+  if (a.mode == kRotNone) hipLaunchKernelGGL((kv_append_kernel<T, D, kRotNone>), g, blk, 0, st, a, units, hpu);
+  else if (a.mode == kRotHalf) hipLaunchKernelGGL((kv_append_kernel<T, D, kRotHalf>), g, blk, 0, st, a, units, hpu);
+  else if (a.mode == kRotInterleaved)
+    hipLaunchKernelGGL((kv_append_kernel<T, D, kRotInterleaved>), g, blk, 0, st, a, units, hpu);
+  else hipLaunchKernelGGL((kv_append_kernel<T, D, kRotAny>), g, blk, 0, st, a, units, hpu);
+}
 template <typename T>
-static void append_launch(int d, const AppendArgs& a, dim3 g, hipStream_t st) {
-  if (d == 64) hipLaunchKernelGGL((kv_append_kernel<T, 64>), g, dim3(kKvThreads), 0, st, a);
-  else if (d == 128) hipLaunchKernelGGL((kv_append_kernel<T, 128>), g, dim3(kKvThreads), 0, st, a);
-  else hipLaunchKernelGGL((kv_append_kernel<T, 256>), g, dim3(kKvThreads), 0, st, a);
+static void append_launch(int d, const AppendArgs& a, dim3 g, int units, int hpu, hipStream_t st) {
+  if (d == 64) append_launch_m<T, 64>(a, g, units, hpu, st);
+  else if (d == 128) append_launch_m<T, 128>(a, g, units, hpu, st);
+  else append_launch_m<T, 256>(a, g, units, hpu, st);
 }
 template <typename T>
 static void gather_launch(int d, const GatherArgs& a, dim3 g, hipStream_t st) {
@@ -301,7 +486,7 @@ static int rows_args(const kh_paged_kv* c, int dtype, int64_t rows, const int64_
   KH_CHECK_ARG(c != nullptr, "null handle");
   KH_CHECK_ARG(dtype == KH_DT_F32 || dtype == KH_DT_BF16, "dtype %d: f32 and BF16 are supported", dtype);
   KH_CHECK_ARG(rows >= 0 && batch >= 0, "rows %lld, batch %lld", (long long)rows, (long long)batch);
-  KH_CHECK_ARG(rows <= (int64_t)1 << 40, "too many rows");
+  KH_CHECK_ARG(rows < (int64_t)1 << 31, "%lld rows: too many for one call", (long long)rows);
   KH_CHECK_ARG(rows == 0 || batch == 0 || (off && start && table), "null argument");
   KH_CHECK_ARG(cols >= 1 && table_stride >= cols, "page table of %lld columns, %lld apart", (long long)cols,
                (long long)table_stride);
@@ -425,14 +610,24 @@ extern "C" int kh_paged_kv_append(kh_paged_kv* c, const kh_rope* rope, int dtype
   a.max_pos = rope ? rope->max_pos : 0;
   a.rot = rope ? rope->rot : 0;
   a.half_layout = rope && rope->layout == KH_ROPE_HALF ? 1 : 0;
+  a.mode = !rope ? kRotNone
+           : rope->rot % (a.half_layout ? 16 : 8) ? kRotAny
+           : a.half_layout ? kRotHalf : kRotInterleaved;
   a.rope_err = rope ? rope->err : nullptr;
   a.kvec = aligned16(k_dev, dtype, k_row_stride, k_head_stride) ? 1 : 0;
   a.vvec = aligned16(v_dev, dtype, v_row_stride, v_head_stride) ? 1 : 0;
-  const int64_t per = kKvThreads / (c->d / 4);
-  const int64_t blocks = (rows * c->nkv + per - 1) / per;
-  const dim3 g((unsigned)(blocks < 16384 ? blocks : 16384), 2);
-  if (dtype == KH_DT_F32) append_launch<float>(c->d, a, g, as_stream(stream));
-  else append_launch<uint16_t>(c->d, a, g, as_stream(stream));
+  // one head (two of 64 elements) a wave until there are waves enough, then up to
+  // eight in turn, which share the search for the quad's sequence and page
+  const int hw = c->d == 64 ? 2 : 1;
+  const int64_t waves = (rows / 4 + batch) * ((c->nkv + hw - 1) / hw);
+  int hpu = hw;
+  while (hpu < 8 && hpu < c->nkv && waves * hw / hpu > 16384) hpu *= 2;
+  const int units = (c->nkv + hpu - 1) / hpu;
+  const int64_t blocks = ((rows / 4 + 2 * batch) * units + 3) / 4;
+  KH_CHECK_ARG(blocks < (int64_t)1 << 28, "too many rows for one call");
+  const dim3 g((unsigned)(blocks < 1024 ? blocks : 1024), 2);
+  if (dtype == KH_DT_F32) append_launch<float>(c->d, a, g, units, hpu, as_stream(stream));
+  else append_launch<uint16_t>(c->d, a, g, units, hpu, as_stream(stream));
   KH_LAUNCHED();
   return KH_OK;
 }
