@@ -16,7 +16,6 @@
 namespace kh {
 
 constexpr int kKvThreads = 256;
-constexpr int kSeqLds = 1025;  // offsets staged in LDS for the search of a row's sequence
 
 // BF16 bits of x rounded towards minus infinity, and of x >= 0 towards plus infinity.
 __device__ __forceinline__ uint32_t bf16_down(float x) {
@@ -68,36 +67,6 @@ struct KvRows {
   const int32_t* table;
   int64_t batch, rows, cols, table_stride;
 };
-
-// Where row t of head h lies: its block, and its place in the page (-1: the
-// row lies in no sequence, or its place is not in the cache, which is recorded).
-__device__ __forceinline__ int kv_place(const KvRows& a, const int64_t* off, int64_t t, int h, char** blk,
-                                        int64_t* pos) {
-  const int64_t b = seq_of_row(off, a.batch, t);
-  if (b < 0) return -1;
-  const int64_t p = a.start[b] + (t - off[b]);
-  const int64_t col = p >> a.ps_log2;
-  if (p < 0 || col >= a.cols) {
-    atomicOr(a.err, 1);
-    return -1;
-  }
-  const int64_t pg = a.table[b * a.table_stride + col];
-  if (pg < 0 || pg >= a.pages) {
-    atomicOr(a.err, 2);
-    return -1;
-  }
-  *pos = p;
-  *blk = a.pool + (pg * a.nkv + h) * a.block;
-  return (int)(p & ((1 << a.ps_log2) - 1));
-}
-
-// The offsets the block searches: an LDS copy where they fit.
-__device__ __forceinline__ const int64_t* stage_off(const KvRows& a, int64_t* lds) {
-  if (a.batch >= kSeqLds) return a.off;
-  for (int i = threadIdx.x; i <= a.batch; i += blockDim.x) lds[i] = a.off[i];
-  __syncthreads();
-  return lds;
-}
 
 struct AppendArgs {
   KvRows r;
@@ -204,33 +173,23 @@ __device__ __forceinline__ int64_t readlane64(int64_t v, int l) {
 // nibbles of four lanes (c, c ^ 2, c ^ 4, c ^ 6), and a quad's four positions
 // share 16-byte pieces: they are put together in LDS and stored whole where all
 // four are appended, and as u16 where they are not.
-template <typename T, int D, int MODE, bool VAL>
-__device__ __forceinline__ void append_part(const AppendArgs& a, int units, int hpu, int* s_q, int* s_wsum, int* s_tot,
-                                            uint16_t* s_v) {
-  using P = KvParts<D>;
-  constexpr int NG = D / kKvGroup, HN = D / 64, L = D / 8;
-  constexpr int TP = 64 / L < 4 ? 64 / L : 4, PASS = 4 / TP;  // positions at a time
-  constexpr int HW = D == 64 ? 2 : 1;                         // heads at a time
-  const int lane = threadIdx.x & 63, c = lane % L, j = c >> 2, g = c & 3;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int sub = D == 64 ? lane >> 5 : 0, tp = (lane / L) % TP;
-  const int ps = 1 << a.r.ps_log2;
-  const bool vec = VAL ? a.vvec : a.kvec;
-  const int64_t srow = VAL ? a.vs : a.ks, shead = VAL ? a.vh : a.kh;
-  const T* src = static_cast<const T*>(VAL ? a.v : a.k) + tp * srow + 8 * c;
-  const bool first_half = 8 * c < (a.rot >> 1);
-  const bool turns = MODE == kRotHalf || MODE == kRotInterleaved ? 8 * c < a.rot : false;
-  const int other = first_half ? a.rot >> 1 : -(a.rot >> 1);  // the pairs' other elements (kRotHalf)
-  const bool few = a.r.batch <= 64;
-  for (int64_t c0 = 0; c0 < a.r.batch; c0 += kSeqChunk) {
-    const int nb = (int)min((int64_t)kSeqChunk, a.r.batch - c0);
+// Gives the waves of the grid their quads, one unit (hpu heads) at a time:
+// f(p0, t0, o0, o1, pg, h0, nh), with the quad's first position and its row, the
+// sequence's rows, the page, and the unit's heads.  Rows t0 .. t0 + 3 that lie in
+// [o0, o1) are the quad's.  Places that are not there are recorded and skipped.
+template <typename F>
+__device__ __forceinline__ void walk_quads(const KvRows& r, int units, int hpu, int* s_q, int* s_wsum, int* s_tot, F f) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool few = r.batch <= 64;
+  for (int64_t c0 = 0; c0 < r.batch; c0 += kSeqChunk) {
+    const int nb = (int)min((int64_t)kSeqChunk, r.batch - c0);
     WaveSeqs ws;
     int quads;
     if (few) {
       if (lane < nb) {
-        ws.o0 = (int)max(a.r.off[lane], (int64_t)0);
-        ws.o1 = (int)min(a.r.off[lane + 1], a.r.rows);
-        ws.start = a.r.start[lane];
+        ws.o0 = (int)max(r.off[lane], (int64_t)0);
+        ws.o1 = (int)min(r.off[lane + 1], r.rows);
+        ws.start = r.start[lane];
         ws.n = quads_of(ws.o1 - ws.o0, ws.start);
       }
       const int incl = wave_incl_scan(ws.n);
@@ -238,7 +197,7 @@ __device__ __forceinline__ void append_part(const AppendArgs& a, int units, int 
       quads = __builtin_amdgcn_readlane(incl, 63);
     } else {
       if (c0) __syncthreads();
-      quads = stage_quads(a.r, c0, nb, s_q, s_wsum, s_tot);
+      quads = stage_quads(r, c0, nb, s_q, s_wsum, s_tot);
     }
     const uint32_t end = (uint32_t)quads * (uint32_t)units;  // below 2^31 (checked on the host)
     for (uint32_t u = blockIdx.x * (kKvThreads / 64) + wave; u < end; u += gridDim.x * (kKvThreads / 64)) {
@@ -260,25 +219,52 @@ __device__ __forceinline__ void append_part(const AppendArgs& a, int units, int 
           else hi = mid;
         }
         lo = __builtin_amdgcn_readfirstlane(lo);
-        o0 = (int)max(a.r.off[c0 + lo], (int64_t)0);
-        o1 = (int)min(a.r.off[c0 + lo + 1], a.r.rows);
-        start = a.r.start[c0 + lo];
+        o0 = (int)max(r.off[c0 + lo], (int64_t)0);
+        o1 = (int)min(r.off[c0 + lo + 1], r.rows);
+        start = r.start[c0 + lo];
         first = __builtin_amdgcn_readfirstlane(s_q[lo]);
       }
-      const int64_t p0 = ((start >> 2) + (qi - first)) * 4;  // the quad's first position
-      const int t0 = (int)(o0 + (p0 - start));               // and its row, which may lie up to 3 before o0
-      const int64_t colm = p0 >> a.r.ps_log2;
-      int pg = -1;
-      if (p0 < 0 || colm >= a.r.cols) {
-        if (lane == 0) atomicOr(a.r.err, 1);
-      } else {
-        pg = __builtin_amdgcn_readfirstlane(a.r.table[(c0 + lo) * a.r.table_stride + colm]);
-        if (pg < 0 || pg >= a.r.pages) {
-          pg = -1;
-          if (lane == 0) atomicOr(a.r.err, 2);
-        }
+      const int64_t p0 = ((start >> 2) + (qi - first)) * 4;
+      const int64_t colm = p0 >> r.ps_log2;
+      if (p0 < 0 || colm >= r.cols) {
+        if (lane == 0) atomicOr(r.err, 1);
+        continue;
       }
-      if (pg < 0) continue;
+      const int pg = __builtin_amdgcn_readfirstlane(r.table[(c0 + lo) * r.table_stride + colm]);
+      if (pg < 0 || pg >= r.pages) {
+        if (lane == 0) atomicOr(r.err, 2);
+        continue;
+      }
+      f(p0, (int)(o0 + (p0 - start)), o0, o1, pg, h0, min(hpu, r.nkv - h0));
+    }
+  }
+}
+
+// The lanes of a wave over a quad: D / 8 lanes a position, eight neighbouring
+// elements each.
+template <int D>
+struct QuadLanes {
+  static constexpr int L = D / 8;
+  static constexpr int TP = 64 / L < 4 ? 64 / L : 4, PASS = 4 / TP;  // positions at a time
+  static constexpr int HW = D == 64 ? 2 : 1;                         // heads at a time
+};
+
+template <typename T, int D, int MODE, bool VAL>
+__device__ __forceinline__ void append_part(const AppendArgs& a, int units, int hpu, int* s_q, int* s_wsum, int* s_tot,
+                                            uint16_t* s_v) {
+  using P = KvParts<D>;
+  constexpr int NG = D / kKvGroup, HN = D / 64, L = QuadLanes<D>::L;
+  constexpr int TP = QuadLanes<D>::TP, PASS = QuadLanes<D>::PASS, HW = QuadLanes<D>::HW;
+  const int lane = threadIdx.x & 63, c = lane % L, j = c >> 2, g = c & 3;
+  const int sub = D == 64 ? lane >> 5 : 0, tp = (lane / L) % TP;
+  const int ps = 1 << a.r.ps_log2;
+  const bool vec = VAL ? a.vvec : a.kvec;
+  const int64_t srow = VAL ? a.vs : a.ks, shead = VAL ? a.vh : a.kh;
+  const T* src = static_cast<const T*>(VAL ? a.v : a.k) + tp * srow + 8 * c;
+  const bool first_half = 8 * c < (a.rot >> 1);
+  const bool turns = MODE == kRotHalf || MODE == kRotInterleaved ? 8 * c < a.rot : false;
+  const int other = first_half ? a.rot >> 1 : -(a.rot >> 1);  // the pairs' other elements (kRotHalf)
+  walk_quads(a.r, units, hpu, s_q, s_wsum, s_tot, [&](int64_t p0, int t0, int o0, int o1, int pg, int h0, int nh) {
       const int at0 = (int)(p0 & (ps - 1));
       // the lane's positions
       bool on[PASS];
@@ -315,7 +301,6 @@ __device__ __forceinline__ void append_part(const AppendArgs& a, int units, int 
       }
       const bool all = __ballot(!mine) == 0;
       const T* x0 = src + t0 * srow + (h0 + sub) * shead;
-      const int nh = min(hpu, a.r.nkv - h0);  // heads of this unit
       char* blk = a.r.pool + ((int64_t)pg * a.r.nkv + h0 + sub) * a.r.block;
       for (int h1 = 0; h1 < nh; h1 += HW, x0 += HW * shead, blk += HW * a.r.block) {
         const bool there = HW == 1 || h1 + sub < nh;
@@ -400,8 +385,7 @@ __device__ __forceinline__ void append_part(const AppendArgs& a, int units, int 
           __builtin_amdgcn_wave_barrier();
         }
       }
-    }
-  }
+  });
 }
 
 template <typename T, int D, int MODE>
@@ -417,45 +401,70 @@ struct GatherArgs {
   void *k, *v;
 };
 
-// The inverse walk, eight neighbouring values a lane.
-template <typename T, int D>
-__global__ __launch_bounds__(kKvThreads) void kv_gather_kernel(GatherArgs a) {
-  __shared__ int64_t s_off[kSeqLds];
-  constexpr int NG = D / kKvGroup, HN = D / 64, L = D / 8, R = kKvThreads / L;
+// The inverse: the same quads and lanes.  Of the four lanes that need the same eight
+// u16 of a value's codes each loads two, and they exchange them.
+template <typename T, int D, bool VAL>
+__device__ __forceinline__ void gather_part(const GatherArgs& a, int units, int hpu, int* s_q, int* s_wsum, int* s_tot) {
   using P = KvParts<D>;
-  const int64_t* off = stage_off(a.r, s_off);
+  constexpr int NG = D / kKvGroup, HN = D / 64, L = QuadLanes<D>::L;
+  constexpr int TP = QuadLanes<D>::TP, PASS = QuadLanes<D>::PASS, HW = QuadLanes<D>::HW;
+  const int lane = threadIdx.x & 63, c = lane % L, j = c >> 2, g = c & 3;
+  const int sub = D == 64 ? lane >> 5 : 0, tp = (lane / L) % TP;
   const int ps = 1 << a.r.ps_log2;
-  const int c = threadIdx.x % L, j = c >> 2;
-  const int64_t units = a.r.rows * a.r.nkv;
-  for (int64_t u = (int64_t)blockIdx.x * R + threadIdx.x / L; u < units; u += (int64_t)gridDim.x * R) {
-    const int64_t t = u / a.r.nkv;
-    const int h = (int)(u - t * a.r.nkv);
-    char* blk = nullptr;
-    int64_t p = 0;
-    const int at = kv_place(a.r, off, t, h, &blk, &p);
-    if (at < 0) continue;
-    float f[8];
-    if (blockIdx.y == 0) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(blk + P::kc() + at * (D / 2) + ((c & 3) * NG + j) * 4);
-      const uint32_t pr = *reinterpret_cast<const uint32_t*>(blk + P::kp(ps) + (at * NG + j) * 4);
-      const float s = __uint_as_float(pr & 0xffff0000u), m = __uint_as_float(pr << 16);
+  const int64_t srow = (int64_t)a.r.nkv * D;
+  T* dst = static_cast<T*>(VAL ? a.v : a.k) + tp * srow + 8 * c;
+  const int n = (c >> 1) & 3, hf = c >> 3, r = 8 * (c & 1) + 2 * n;
+  walk_quads(a.r, units, hpu, s_q, s_wsum, s_tot, [&](int64_t p0, int t0, int o0, int o1, int pg, int h0, int nh) {
+    const int at0 = (int)(p0 & (ps - 1));
+    T* y0 = dst + t0 * srow + (int64_t)(h0 + sub) * D;
+    const char* blk = a.r.pool + ((int64_t)pg * a.r.nkv + h0) * a.r.block;
+#pragma unroll 2
+    for (int h1 = 0; h1 < nh; h1 += HW, y0 += HW * D, blk += HW * a.r.block) {
+      const bool there = HW == 1 || h1 + sub < nh;
+      const char* mine = blk + (there ? sub : 0) * a.r.block;  // lanes without a head read the first one's
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = s * (float)((w >> (4 * i)) & 15) + m;
-    } else {
-      // d = 8 c + i = 64 hf + 16 n + r: one nibble of eight neighbouring r
-      const int hf = c >> 3, n = (c >> 1) & 3, r0 = 8 * (c & 1);
-      const uint16_t* vc = reinterpret_cast<const uint16_t*>(blk + P::vc(ps));
-      const uint32_t pr = *reinterpret_cast<const uint32_t*>(blk + P::vp(ps) + (j * ps + at) * 4);
-      const float s = __uint_as_float(pr & 0xffff0000u), m = __uint_as_float(pr << 16);
+      for (int k = 0; k < PASS; ++k) {
+        const int t = t0 + k * TP + tp, at = at0 + k * TP + tp;
+        const bool act = there && t >= o0 && t < o1;
+        uint32_t pr, q[4];
+        if (VAL) {
+          const uint16_t* vc = reinterpret_cast<const uint16_t*>(mine + P::vc(ps)) + (at >> 2) * D;
+          const int o = ((r * 2 + ((at >> 1) & 1)) * HN + hf) * 2 + (at & 1);
+          const uint32_t w0 = vc[o] | (uint32_t)vc[o + 4 * HN] << 16;
+          pr = *reinterpret_cast<const uint32_t*>(mine + P::vp(ps) + (j * ps + at) * 4);
+          // of lanes c, c ^ 2, c ^ 4, c ^ 6, put in the order of their n
+          const uint32_t w1 = (uint32_t)dpp<kDppQuadSwap2>((int)w0);
+          const uint32_t w2 = (uint32_t)dpp<0x1B>(dpp<kDppRowHalfMirror>((int)w0));
+          const uint32_t w3 = (uint32_t)dpp<kDppQuadSwap2>((int)w2);
+          const uint32_t a0 = (n & 1) ? w1 : w0, a1 = (n & 1) ? w0 : w1, a2 = (n & 1) ? w3 : w2, a3 = (n & 1) ? w2 : w3;
+          q[0] = (n & 2) ? a2 : a0;
+          q[1] = (n & 2) ? a3 : a1;
+          q[2] = (n & 2) ? a0 : a2;
+          q[3] = (n & 2) ? a1 : a3;
+        } else {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(mine + P::kc() + at * (D / 2) + (g * NG + j) * 4);
+          pr = *reinterpret_cast<const uint32_t*>(mine + P::kp(ps) + (at * NG + j) * 4);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t w = vc[((((at >> 2) * 16 + r0 + i) * 2 + ((at >> 1) & 1)) * HN + hf) * 2 + (at & 1)];
-        f[i] = s * (float)((w >> (4 * n)) & 15) + m;
+          for (int i = 0; i < 4; ++i) q[i] = w >> (8 * i);
+        }
+        const float s = __uint_as_float(pr & 0xffff0000u), m = __uint_as_float(pr << 16);
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[2 * i] = s * (float)(VAL ? (q[i] >> (4 * n)) & 15 : q[i] & 15) + m;
+          f[2 * i + 1] = s * (float)(VAL ? (q[i] >> (4 * n + 16)) & 15 : (q[i] >> 4) & 15) + m;
+        }
+        if (act) store8(y0 + k * TP * srow, true, f);
       }
     }
-    T* y = static_cast<T*>(blockIdx.y == 0 ? a.k : a.v) + u * D + 8 * c;
-    store8(y, true, f);
-  }
+  });
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kKvThreads) void kv_gather_kernel(GatherArgs a, int units, int hpu) {
+  __shared__ int s_q[kSeqChunk], s_wsum[kKvThreads / 64], s_tot;
+  if (blockIdx.y == 0) gather_part<T, D, false>(a, units, hpu, s_q, s_wsum, &s_tot);
+  else gather_part<T, D, true>(a, units, hpu, s_q, s_wsum, &s_tot);
 }
 
 template <typename T, int D>
@@ -474,10 +483,25 @@ static void append_launch(int d, const AppendArgs& a, dim3 g, int units, int hpu
   else append_launch_m<T, 256>(a, g, units, hpu, st);
 }
 template <typename T>
-static void gather_launch(int d, const GatherArgs& a, dim3 g, hipStream_t st) {
-  if (d == 64) hipLaunchKernelGGL((kv_gather_kernel<T, 64>), g, dim3(kKvThreads), 0, st, a);
-  else if (d == 128) hipLaunchKernelGGL((kv_gather_kernel<T, 128>), g, dim3(kKvThreads), 0, st, a);
-  else hipLaunchKernelGGL((kv_gather_kernel<T, 256>), g, dim3(kKvThreads), 0, st, a);
+static void gather_launch(int d, const GatherArgs& a, dim3 g, int units, int hpu, hipStream_t st) {
+  if (d == 64) hipLaunchKernelGGL((kv_gather_kernel<T, 64>), g, dim3(kKvThreads), 0, st, a, units, hpu);
+  else if (d == 128) hipLaunchKernelGGL((kv_gather_kernel<T, 128>), g, dim3(kKvThreads), 0, st, a, units, hpu);
+  else hipLaunchKernelGGL((kv_gather_kernel<T, 256>), g, dim3(kKvThreads), 0, st, a, units, hpu);
+}
+
+// The grid: one head (two of 64 elements) a wave until there are waves enough,
+// then up to eight in turn, which share the search for the quad's sequence and page.
+static int quad_grid(const kh_paged_kv* c, int64_t rows, int64_t batch, int* units, int* hpu, dim3* g) {
+  const int hw = c->d == 64 ? 2 : 1;
+  const int64_t waves = (rows / 4 + batch) * ((c->nkv + hw - 1) / hw);
+  int n = hw;
+  while (n < 8 && n < c->nkv && waves * hw / n > 16384) n *= 2;
+  *hpu = n;
+  *units = (c->nkv + n - 1) / n;
+  const int64_t blocks = ((rows / 4 + 2 * batch) * *units + 3) / 4;
+  KH_CHECK_ARG(blocks < (int64_t)1 << 28, "too many rows for one call");
+  *g = dim3((unsigned)(blocks < 1024 ? blocks : 1024), 2);
+  return KH_OK;
 }
 
 // The arguments every call over rows of sequences checks.
@@ -616,16 +640,10 @@ extern "C" int kh_paged_kv_append(kh_paged_kv* c, const kh_rope* rope, int dtype
   a.rope_err = rope ? rope->err : nullptr;
   a.kvec = aligned16(k_dev, dtype, k_row_stride, k_head_stride) ? 1 : 0;
   a.vvec = aligned16(v_dev, dtype, v_row_stride, v_head_stride) ? 1 : 0;
-  // one head (two of 64 elements) a wave until there are waves enough, then up to
-  // eight in turn, which share the search for the quad's sequence and page
-  const int hw = c->d == 64 ? 2 : 1;
-  const int64_t waves = (rows / 4 + batch) * ((c->nkv + hw - 1) / hw);
-  int hpu = hw;
-  while (hpu < 8 && hpu < c->nkv && waves * hw / hpu > 16384) hpu *= 2;
-  const int units = (c->nkv + hpu - 1) / hpu;
-  const int64_t blocks = ((rows / 4 + 2 * batch) * units + 3) / 4;
-  KH_CHECK_ARG(blocks < (int64_t)1 << 28, "too many rows for one call");
-  const dim3 g((unsigned)(blocks < 1024 ? blocks : 1024), 2);
+  int units, hpu;
+  dim3 g;
+  const int grc = quad_grid(c, rows, batch, &units, &hpu, &g);
+  if (grc != KH_OK) return grc;
   if (dtype == KH_DT_F32) append_launch<float>(c->d, a, g, units, hpu, as_stream(stream));
   else append_launch<uint16_t>(c->d, a, g, units, hpu, as_stream(stream));
   KH_LAUNCHED();
@@ -645,11 +663,12 @@ extern "C" int kh_paged_kv_gather(const kh_paged_kv* c, int dtype, int64_t rows,
   KH_ON_DEVICE(c->device, "the cache");
   a.k = k_dev;
   a.v = v_dev;
-  const int64_t per = kKvThreads / (c->d / 8);
-  const int64_t blocks = (rows * c->nkv + per - 1) / per;
-  const dim3 g((unsigned)(blocks < 16384 ? blocks : 16384), 2);
-  if (dtype == KH_DT_F32) gather_launch<float>(c->d, a, g, as_stream(stream));
-  else gather_launch<uint16_t>(c->d, a, g, as_stream(stream));
+  int units, hpu;
+  dim3 g;
+  const int grc = quad_grid(c, rows, batch, &units, &hpu, &g);
+  if (grc != KH_OK) return grc;
+  if (dtype == KH_DT_F32) gather_launch<float>(c->d, a, g, units, hpu, as_stream(stream));
+  else gather_launch<uint16_t>(c->d, a, g, units, hpu, as_stream(stream));
   KH_LAUNCHED();
   return KH_OK;
 }

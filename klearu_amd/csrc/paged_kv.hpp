@@ -54,19 +54,6 @@ struct KvParts {
   static __host__ __device__ constexpr int vp(int ps) { return ps * D + ps * NG * 4; }
 };
 
-// The sequence of row `t`: the last b with off[b] <= t (off ascending), or -1
-// when t lies in no sequence.  `off` may be an LDS copy.
-__device__ __forceinline__ int64_t seq_of_row(const int64_t* off, int64_t batch, int64_t t) {
-  if (t < off[0] || t >= off[batch]) return -1;
-  int64_t lo = 0, hi = batch;  // off[lo] <= t < off[hi]
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (off[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
 // The handle's device must be the current one: its memory and the stream
 // belong there.
 inline int check_device(int device, const char* what) {
