@@ -35,26 +35,26 @@ __device__ __forceinline__ uint32_t kv_code(float x, float m, float s) {
   const float q = rintf(__fdiv_rn(__fsub_rn(x, m), s));
   return (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f);
 }
-// The codes of eight values, four bits each.  x - m over s lies in [0, 15 + 2^-20]
-// and a product with the reciprocal is off by less than 1e-5 from it, so its
-// nearest whole number is the quotient's unless it lies that near to a half (or s
-// has no reciprocal): those eight are divided.
+// The codes of eight values, four bits each.  The quotient without a division
+// (Markstein): with y the correctly rounded reciprocal of s and q = d y within an
+// ulp of d / s, q + (d - q s) y rounds to the correctly rounded d / s.  One step
+// from the hardware's reciprocal gives y (for significands that are not all ones; s
+// has eight bits), where nothing underflows: scales below 2^-90 are divided.
 __device__ __forceinline__ uint32_t kv_codes8(const float (&f)[8], uint32_t pair) {
   const float s = __uint_as_float(pair & 0xffff0000u), m = __uint_as_float(pair << 16);
-  const float inv = __builtin_amdgcn_rcpf(s);
-  bool sure = true;
   uint32_t w = 0;
+  if (s > 0.0f && s < 0x1p-90f) {
+#pragma unroll
+    for (int i = 7; i >= 0; --i) w = w << 4 | kv_code(f[i], m, s);
+    return w;
+  }
+  const float y0 = __builtin_amdgcn_rcpf(s), y = fmaf(fmaf(-s, y0, 1.0f), y0, y0);
 #pragma unroll
   for (int i = 7; i >= 0; --i) {
-    const float q = (f[i] - m) * inv, c = rintf(q);
-    sure = sure && fabsf(q - c) < 0.49999f;  // not where it is NaN
-    w = w << 4 | (uint32_t)(int)c;
+    const float d = f[i] - m, q = d * y;
+    w = w << 4 | (uint32_t)(int)rintf(fmaf(fmaf(-q, s, d), y, q));
   }
-  if (sure) return w;
-  w = 0;
-#pragma unroll
-  for (int i = 7; i >= 0; --i) w = w << 4 | kv_code(f[i], m, s);
-  return w;
+  return s > 0.0f ? w : 0;
 }
 __device__ __forceinline__ bool too_large(float x) { return (__float_as_uint(x) & 0x7fffffffu) >= 0x71800000u; }  // 2^100
 
