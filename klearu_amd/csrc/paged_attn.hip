@@ -30,7 +30,15 @@
 
 namespace kh {
 
-constexpr int kPaWaves = 4;
+// Waves of a block, and waves that a SIMD's registers hold.
+template <int D>
+struct PaShape {
+  static constexpr int NW = D == 128 ? 8 : 4;
+  static constexpr int kPerSimd = D == 64 ? 3 : D == 128 ? 2 : 1;
+  static constexpr int kFill = 256 * 4 * kPerSimd / NW;  // blocks that the chip holds at once
+  static constexpr int kOS = D + 4;                      // floats between rows in LDS: other banks for each
+  static constexpr int kLds = NW * 16 * (kOS + 2) * 4;
+};
 constexpr int kPaStep = 32;        // positions a wave takes at a time
 constexpr int kPaMaxSplit = 128;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -74,6 +82,40 @@ __device__ __forceinline__ void ld_words(const char* p, uint32_t (&w)[N]) {
     }
   }
 }
+
+// Eight neighbouring elements as they lie in memory.
+template <typename T>
+struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p, bool vec) {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+      float f[8];
+      load8(p, false, f);
+      put(f);
+    }
+  }
+  __device__ __forceinline__ void put(const float (&f)[8]) {
+    if constexpr (sizeof(T) == 4) {
+      w[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+      w[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+    } else {
+      w[0] = make_uint4(__float_as_uint(f[0]) >> 16 | __float_as_uint(f[1]), __float_as_uint(f[2]) >> 16 | __float_as_uint(f[3]),
+                        __float_as_uint(f[4]) >> 16 | __float_as_uint(f[5]), __float_as_uint(f[6]) >> 16 | __float_as_uint(f[7]));
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+      f[0] = __uint_as_float(w[0].x); f[1] = __uint_as_float(w[0].y); f[2] = __uint_as_float(w[0].z); f[3] = __uint_as_float(w[0].w);
+      f[4] = __uint_as_float(w[1].x); f[5] = __uint_as_float(w[1].y); f[6] = __uint_as_float(w[1].z); f[7] = __uint_as_float(w[1].w);
+    } else {
+      f[0] = bf16_lo(w[0].x); f[1] = bf16_hi(w[0].x); f[2] = bf16_lo(w[0].y); f[3] = bf16_hi(w[0].y);
+      f[4] = bf16_lo(w[0].z); f[5] = bf16_hi(w[0].z); f[6] = bf16_lo(w[0].w); f[7] = bf16_hi(w[0].w);
+    }
+  }
+};
 
 __device__ __forceinline__ kh_f32x4 mfma16(const uint4& a, const uint4& b, kh_f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
@@ -212,45 +254,44 @@ __device__ __forceinline__ void pa_store4(T* y, bool vec, float a, float b, floa
 }
 
 // Block: one row tile of one (sequence, kv head), one of nsplit parts of the
-// positions that the tile sees; its waves take every fourth step of 32.
+// positions that the tile sees; its waves take every NW-th step of 32.
 template <int D, typename T>
-__global__ __launch_bounds__(64 * kPaWaves, D == 64 ? 3 : D == 128 ? 2 : 1) void paged_rows_kernel(PaArgs a) {
-  constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16;
+__global__ __launch_bounds__(64 * PaShape<D>::NW, PaShape<D>::kPerSimd) void paged_rows_kernel(PaArgs a) {
+  constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16, NW = PaShape<D>::NW;
   constexpr int BIAS = sizeof(T) == 4 ? 16 : 128;
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1;  // terms of q: all of its bits
   constexpr int NP = sizeof(T) == 4 ? 3 : 1;  // of P: all of its bits for f32 rows, 8 for BF16 ones, as their output
-  __shared__ float s_m[kPaWaves][16], s_l[kPaWaves][16];
-  __shared__ __align__(16) float s_o[2][16 * D];
+  constexpr int OS = PaShape<D>::kOS;
+  extern __shared__ __align__(16) float s_o[];  // [NW][16][OS], then the maxima and sums
+  float* s_m = s_o + NW * 16 * OS;
+  float* s_l = s_m + NW * 16;
   const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint32_t id = blockIdx.x;
-  const int split = (int)(id % (uint32_t)a.nsplit);
-  id /= (uint32_t)a.nsplit;
-  const int tile0 = (int)(id % (uint32_t)a.tiles);
-  id /= (uint32_t)a.tiles;
-  const int h = (int)(id % (uint32_t)a.nkv);
-  const int64_t b = id / (uint32_t)a.nkv;
+  const int split = blockIdx.x, h = blockIdx.y;
   const int ps = 1 << a.ps_log2;
-  int64_t o0 = a.off[b], o1 = a.off[b + 1];
+  const int64_t cap = a.cols << a.ps_log2;
+  const PaLane<D> lo_(lane, ps);
+  for (int64_t bt = blockIdx.z; bt < a.batch * a.tiles; bt += gridDim.z) {
+  const int64_t b = a.tiles == 1 ? bt : bt / a.tiles;
+  const int tile0 = a.tiles == 1 ? 0 : (int)(bt - b * a.tiles);
+  // the first of the chain's loads together: rows, length, the first 64 pages
+  const int32_t* __restrict__ table = a.table + b * a.table_stride;
+  const int pre = lane < a.cols ? table[lane] : -1;
+  int64_t o0 = a.off[b], o1 = a.off[b + 1], L = a.len[b];
   o0 = o0 < 0 ? 0 : o0;
   o1 = o1 > a.rows ? a.rows : o1;
-  if (o1 <= o0) return;
+  if (o1 <= o0) continue;
   const int n = (int)(o1 - o0), nr = n * a.gs;  // rows x heads of a kv head: below 2^31
-  const int64_t cap = a.cols << a.ps_log2;
-  int64_t L = a.len[b];
   if (L < 0 || L > cap) {
     if (threadIdx.x == 0) atomicOr(a.err, 1);
     L = L < 0 ? 0 : cap;
   }
-  const int32_t* __restrict__ table = a.table + b * a.table_stride;
-
-  const PaLane<D> lo_(lane, ps);
 
   for (int tile = tile0; tile < (nr + 15) >> 4; tile += a.tiles) {
     // the lane's row (column of the products)
     const int rr = tile * 16 + col;
     const bool inside = rr < nr;
-    const int i = (int)((uint32_t)(inside ? rr : 0) / (uint32_t)a.gs);
+    const int i = a.gs == 1 ? (inside ? rr : 0) : (int)((uint32_t)(inside ? rr : 0) / (uint32_t)a.gs);
     const int64_t t = o0 + i;
     const int head = h * a.gs + ((inside ? rr : 0) - i * a.gs);
     bool on = inside;
@@ -289,17 +330,48 @@ __global__ __launch_bounds__(64 * kPaWaves, D == 64 ? 3 : D == 128 ? 2 : 1) void
     const int per = (steps + a.nsplit - 1) / a.nsplit;
     const int sb = first + split * per, se = min(first + steps, sb + per);
     if (sb < se) {
+      // The wave's steps sb + wave, + NW, ...: lane k holds the pages of the k-th of
+      // the next 64, and a step's words are loaded while the one before it is worked on.
+      const int mine = (se - sb - wave + NW - 1) / NW;
+      const bool known = ((thi - 1) >> a.ps_log2) < 64;  // every page is among the first 64
+      int pg0 = 0, pg1 = 0;
+      const auto pages = [&](int k0) {
+        const int k = k0 + lane, tok = (sb + wave + min(k, mine - 1) * NW) * kPaStep;
+        // a half of the step that no row of the tile sees takes the other half's page:
+        // the table need not name one there
+        const int c0 = (tok + 16 <= tlo ? tok + 16 : tok) >> a.ps_log2;
+        const int c1 = (tok + 16 >= thi ? tok : tok + 16) >> a.ps_log2;
+        pg0 = known ? __shfl(pre, c0) : table[c0];
+        pg1 = known ? __shfl(pre, c1) : table[c1];
+        if (pg0 < 0 || pg0 >= a.pages) pg0 = -1;
+        if (pg1 < 0 || pg1 >= a.pages) pg1 = -1;
+        if ((pg0 | pg1) < 0) atomicOr(a.err, 2);
+      };
+      const auto load = [&](int k, PaStepData<D>& x) {
+        const int tok = (sb + wave + k * NW) * kPaStep;
+        const int p0 = max(__builtin_amdgcn_readlane(pg0, k & 63), 0), p1 = max(__builtin_amdgcn_readlane(pg1, k & 63), 0);
+        pa_load<D, 0>(a.pool + ((int64_t)p0 * a.nkv + h) * a.block, tok & (ps - 1), lo_, x);
+        pa_load<D, 1>(a.pool + ((int64_t)p1 * a.nkv + h) * a.block, (tok + 16) & (ps - 1), lo_, x);
+      };
+      PaStepData<D> x[2];
+      Raw8<T> qr[NG];
+      const T* q = static_cast<const T*>(a.q) + t * a.qs + head * a.qh;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) qr[j].load(q + 32 * j + 8 * g, a.qvec);
+      if (mine > 0) {
+        pages(0);
+        load(0, x[0]);
+      }
       // q as the second operand: slots (0,4,1,5,2,6,3,7) of eight neighbouring
       // elements, the order in which codes2 takes the nibbles of a word
       uint4 qf[NG][NQ];
       uint4 qm[(NG + 3) / 4];
       {
         float qsum[NG];
-        const T* q = static_cast<const T*>(a.q) + t * a.qs + head * a.qh;
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
           float f[8];
-          load8(q + 32 * j + 8 * g, a.qvec, f);
+          qr[j].get(f);
           const float e[8] = {f[0], f[4], f[1], f[5], f[2], f[6], f[3], f[7]};
           terms8<NQ>(e, qf[j]);
           qsum[j] = across_groups_sum(((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7])));
@@ -431,48 +503,21 @@ __global__ __launch_bounds__(64 * kPaWaves, D == 64 ? 3 : D == 128 ? 2 : 1) void
         }
       };
 
-      // The wave's steps sb + wave, + kPaWaves, ...: lane k holds the pages of the
-      // k-th of the next 64, and a step's words are loaded while the one before it
-      // is worked on.
-      const int mine = (se - sb - wave + kPaWaves - 1) / kPaWaves;
-      int pg0 = 0, pg1 = 0;
-      const auto pages = [&](int k0) {
-        const int k = k0 + lane, tok = (sb + wave + k * kPaWaves) * kPaStep;
-        if (k >= mine) return;
-        // a half of the step that no row of the tile sees takes the other half's page:
-        // the table need not name one there
-        pg0 = table[(tok + 16 <= tlo ? tok + 16 : tok) >> a.ps_log2];
-        pg1 = table[(tok + 16 >= thi ? tok : tok + 16) >> a.ps_log2];
-        if (pg0 < 0 || pg0 >= a.pages) pg0 = -1;
-        if (pg1 < 0 || pg1 >= a.pages) pg1 = -1;
-        if ((pg0 | pg1) < 0) atomicOr(a.err, 2);
-      };
-      const auto load = [&](int k, PaStepData<D>& x) {
-        const int tok = (sb + wave + k * kPaWaves) * kPaStep;
-        const int p0 = max(__builtin_amdgcn_readlane(pg0, k & 63), 0), p1 = max(__builtin_amdgcn_readlane(pg1, k & 63), 0);
-        pa_load<D, 0>(a.pool + ((int64_t)p0 * a.nkv + h) * a.block, tok & (ps - 1), lo_, x);
-        pa_load<D, 1>(a.pool + ((int64_t)p1 * a.nkv + h) * a.block, (tok + 16) & (ps - 1), lo_, x);
-      };
       const auto work = [&](int k, int q0, int q1, PaStepData<D>& x) {
-        step(x, (sb + wave + k * kPaWaves) * kPaStep, q0 >= 0, q1 >= 0);
+        step(x, (sb + wave + k * NW) * kPaStep, q0 >= 0, q1 >= 0);
       };
-      if (mine > 0) {
-        PaStepData<D> x[2];
-        pages(0);
-        load(0, x[0]);
-        for (int k = 0; k < mine; k += 2) {
-          int q0 = __builtin_amdgcn_readlane(pg0, k & 63), q1 = __builtin_amdgcn_readlane(pg1, k & 63);
-          if (k + 1 < mine) load(k + 1, x[1]);  // 64 is even: of the same pages
-          work(k, q0, q1, x[0]);
-          if (k + 1 >= mine) break;
-          q0 = __builtin_amdgcn_readlane(pg0, (k + 1) & 63);
-          q1 = __builtin_amdgcn_readlane(pg1, (k + 1) & 63);
-          if (k + 2 < mine) {
-            if (((k + 2) & 63) == 0) pages(k + 2);
-            load(k + 2, x[0]);
-          }
-          work(k + 1, q0, q1, x[1]);
+      for (int k = 0; k < mine; k += 2) {
+        int q0 = __builtin_amdgcn_readlane(pg0, k & 63), q1 = __builtin_amdgcn_readlane(pg1, k & 63);
+        if (k + 1 < mine) load(k + 1, x[1]);  // 64 is even: of the same pages
+        work(k, q0, q1, x[0]);
+        if (k + 1 >= mine) break;
+        q0 = __builtin_amdgcn_readlane(pg0, (k + 1) & 63);
+        q1 = __builtin_amdgcn_readlane(pg1, (k + 1) & 63);
+        if (k + 2 < mine) {
+          if (((k + 2) & 63) == 0) pages(k + 2);
+          load(k + 2, x[0]);
         }
+        work(k + 1, q0, q1, x[1]);
       }
     }
 
@@ -489,58 +534,50 @@ __global__ __launch_bounds__(64 * kPaWaves, D == 64 ? 3 : D == 128 ? 2 : 1) void
           for (int r = 0; r < 4; ++r) o[2 * gi + ff][r] += c;
       }
     }
-    // the four waves' parts, joined in a fixed order; maxima in powers of two from here
-    m *= a.c1;
-    if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l;
+    // The waves' parts go to LDS as they are, and behind one barrier every thread
+    // joins four elements of a row, in the order of the waves; maxima in powers of two.
+    if (g == 0) s_m[wave * 16 + col] = some ? m * a.c1 : -INFINITY, s_l[wave * 16 + col] = some ? l : 0.0f;
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+      *reinterpret_cast<kh_f32x4*>(s_o + (wave * 16 + col) * OS + 16 * f + 4 * g) = o[f];
     __syncthreads();
-    float M = s_m[0][col];
 #pragma unroll
-    for (int w = 1; w < kPaWaves; ++w) M = fmaxf(M, s_m[w][col]);
-    const float Mu = M == -INFINITY ? 0.0f : M;
-    float tot = 0.0f;
+    for (int it = 0; it < (4 * D + 64 * NW - 1) / (64 * NW); ++it) {
+      const int e = it * 64 * NW + (int)threadIdx.x, r = e / (D / 4), d = (e - r * (D / 4)) * 4;
+      const int row16 = tile * 16 + r;
+      if (r >= 16 || row16 >= nr) break;
+      float M = -INFINITY, tot = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kPaWaves; ++w) tot += s_l[w][col] * __builtin_amdgcn_exp2f(s_m[w][col] - Mu);
-    const float fac = __builtin_amdgcn_exp2f(m - Mu);
+      for (int w = 0; w < NW; ++w) M = fmaxf(M, s_m[w * 16 + r]);
+      const float Mu = M == -INFINITY ? 0.0f : M;
+      kh_f32x4 v = {0, 0, 0, 0};
 #pragma unroll
-    for (int f = 0; f < NF; ++f) o[f] *= fac;
+      for (int w = 0; w < NW; ++w) {
+        const float fac = __builtin_amdgcn_exp2f(s_m[w * 16 + r] - Mu);
+        tot = fmaf(s_l[w * 16 + r], fac, tot);
+        const kh_f32x4 x = *reinterpret_cast<const kh_f32x4*>(s_o + (w * 16 + r) * OS + d);
 #pragma unroll
-    for (int half = 2; half >= 1; half >>= 1) {
-      if (wave >= half && wave < 2 * half) {
-#pragma unroll
-        for (int f = 0; f < NF; ++f)
-          *reinterpret_cast<kh_f32x4*>(&s_o[wave - half][(f * 64 + lane) * 4]) = o[f];
+        for (int k = 0; k < 4; ++k) v[k] = fmaf(x[k], fac, v[k]);
       }
-      __syncthreads();
-      if (wave < half) {
-#pragma unroll
-        for (int f = 0; f < NF; ++f) o[f] += *reinterpret_cast<const kh_f32x4*>(&s_o[wave][(f * 64 + lane) * 4]);
-      }
-      if (half == 2) __syncthreads();
-    }
-    if (wave == 0 && inside) {
-      const int64_t row = t * a.nh + head;
+      const int ri = a.gs == 1 ? row16 : (int)((uint32_t)row16 / (uint32_t)a.gs);
+      const int64_t rt = o0 + ri;
+      const int rh = h * a.gs + (row16 - ri * a.gs);
+      const int64_t row = rt * a.nh + rh;
+      // a row that sees nothing (here): no maximum and no sum; NaN scores leave the maximum behind
+      const bool any = M != -INFINITY || tot != 0.0f;
       if (a.nsplit > 1) {
         const int64_t at = row * a.nsplit + split;
-        if (g == 0) a.part_ml[at] = make_float2(some ? M : -INFINITY, some ? tot : 0.0f);
-        if (some && sb < se) {
-#pragma unroll
-          for (int f = 0; f < NF; ++f)
-            *reinterpret_cast<float4*>(a.part_o + at * D + 16 * f + 4 * g) = make_float4(o[f][0], o[f][1], o[f][2], o[f][3]);
-        }
+        if (d == 0) a.part_ml[at] = make_float2(M, tot);
+        if (any) *reinterpret_cast<float4*>(a.part_o + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
-        const bool any = some && (M != -INFINITY || tot != 0.0f);  // NaN scores leave M behind
-        T* y = static_cast<T*>(a.out) + t * a.os + head * a.oh + 4 * g;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          float v[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = any ? o[f][r] / tot : 0.0f;
-          pa_store4<D, T>(y + 16 * f, a.ovec, v[0], v[1], v[2], v[3]);
-        }
-        if (a.lse && g == 0) a.lse[row] = any ? kLn2 * (M + __builtin_amdgcn_logf(tot)) : -INFINITY;
+        const float inv = any ? 1.0f / tot : 0.0f;
+        pa_store4<D, T>(static_cast<T*>(a.out) + rt * a.os + rh * a.oh + d, a.ovec, any ? v[0] * inv : 0.0f,
+                        any ? v[1] * inv : 0.0f, any ? v[2] * inv : 0.0f, any ? v[3] * inv : 0.0f);
+        if (a.lse && d == 0) a.lse[row] = any ? kLn2 * (M + __builtin_amdgcn_logf(tot)) : -INFINITY;
       }
     }
     __syncthreads();
+  }
   }
 }
 
@@ -1095,8 +1132,9 @@ static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int
   if (p.tiles < 1) p.tiles = 1;
   if (p.tiles > 65536) p.tiles = 65536;
   p.base = batch * c->nkv * p.tiles;
-  int64_t want = ((p.many ? 256 : 512) + p.base - 1) / p.base;
-  const int64_t most = p.many ? (max_len + 511) / 512 : (max_len + 255) / 256;
+  const int64_t fill = p.many ? 256 : c->d == 64 ? PaShape<64>::kFill : c->d == 128 ? PaShape<128>::kFill : PaShape<256>::kFill;
+  int64_t want = (fill + p.base - 1) / p.base;
+  const int64_t most = p.many ? (max_len + 511) / 512 : c->d == 256 ? (max_len + 127) / 128 : (max_len + 255) / 256;
   if (want > most) want = most;
   if (want > kPaMaxSplit) want = kPaMaxSplit;
   p.nsplit = want < 1 ? 1 : (int)want;
@@ -1106,23 +1144,31 @@ static int64_t pa_bytes(const PaPlan& p, int64_t rows, int nh, int d) {
   return p.nsplit > 1 ? rows * nh * p.nsplit * (int64_t)(4 * d + 8) : 0;
 }
 
+// Dynamic LDS of more than 64 KB has to be asked for, once a kernel.
+template <typename K>
+static hipError_t allow_lds(K* kernel, int bytes) {
+  return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
 template <int D, typename T>
 static int pa_launch(const PaArgs& a, bool many, int64_t blocks, hipStream_t st) {
-  if constexpr (sizeof(T) == 2) {
-    if (many) {
-      constexpr int lds = PtShape<D>::kLds;
-      static std::once_flag once;
-      static hipError_t arc = hipSuccess;
-      std::call_once(once, [] {
-        arc = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_tile_kernel<D, kPtWaves>),
-                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-      });
-      KH_HIP(arc);
-      hipLaunchKernelGGL((paged_tile_kernel<D, kPtWaves>), dim3((unsigned)blocks), dim3(64 * kPtWaves), lds, st, a);
+  static std::once_flag once;
+  static hipError_t arc = hipSuccess;
+  std::call_once(once, [] {
+    arc = allow_lds(&paged_rows_kernel<D, T>, PaShape<D>::kLds);
+    if constexpr (sizeof(T) == 2) {
+      if (arc == hipSuccess) arc = allow_lds(&paged_tile_kernel<D, kPtWaves>, PtShape<D>::kLds);
     }
+  });
+  KH_HIP(arc);
+  if constexpr (sizeof(T) == 2) {
+    if (many)
+      hipLaunchKernelGGL((paged_tile_kernel<D, kPtWaves>), dim3((unsigned)blocks), dim3(64 * kPtWaves), PtShape<D>::kLds, st, a);
   }
   if (!many)
-    hipLaunchKernelGGL((paged_rows_kernel<D, T>), dim3((unsigned)blocks), dim3(64 * kPaWaves), 0, st, a);
+    hipLaunchKernelGGL((paged_rows_kernel<D, T>),
+                       dim3((unsigned)a.nsplit, (unsigned)a.nkv, (unsigned)(a.batch * a.tiles < 65535 ? a.batch * a.tiles : 65535)),
+                       dim3(64 * PaShape<D>::NW), PaShape<D>::kLds, st, a);
   if (a.nsplit > 16)
     hipLaunchKernelGGL((paged_join_kernel<D, T, 4>), dim3((unsigned)(a.rows * a.nh)), dim3(256), 0, st, a);
   else if (a.nsplit > 1)
