@@ -31,10 +31,12 @@
 namespace kh {
 
 // Waves of a block, and waves that a SIMD's registers hold.
-template <int D>
+template <int D, typename T>
 struct PaShape {
-  static constexpr int NW = D == 128 ? 8 : 4;
-  static constexpr int kPerSimd = D == 64 ? 3 : D == 128 ? 2 : 1;
+  static constexpr bool kF32 = sizeof(T) == 4;
+  static constexpr int NW = D == (kF32 ? 64 : 128) ? 8 : 4;
+  static constexpr int kPerSimd = D == 256 || (kF32 && D == 128) ? 1 : D == 64 && !kF32 ? 3 : 2;
+  static constexpr int kAhead = D == 256 ? 0 : 1;        // steps loaded ahead of the one that is worked on
   static constexpr int kFill = 256 * 4 * kPerSimd / NW;  // blocks that the chip holds at once
   static constexpr int kOS = D + 4;                      // floats between rows in LDS: other banks for each
   static constexpr int kLds = NW * 16 * (kOS + 2) * 4;
@@ -256,12 +258,12 @@ __device__ __forceinline__ void pa_store4(T* y, bool vec, float a, float b, floa
 // Block: one row tile of one (sequence, kv head), one of nsplit parts of the
 // positions that the tile sees; its waves take every NW-th step of 32.
 template <int D, typename T>
-__global__ __launch_bounds__(64 * PaShape<D>::NW, PaShape<D>::kPerSimd) void paged_rows_kernel(PaArgs a) {
-  constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16, NW = PaShape<D>::NW;
+__global__ __launch_bounds__((64 * PaShape<D, T>::NW), (PaShape<D, T>::kPerSimd)) void paged_rows_kernel(PaArgs a) {
+  constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16, NW = PaShape<D, T>::NW;
   constexpr int BIAS = sizeof(T) == 4 ? 16 : 128;
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1;  // terms of q: all of its bits
   constexpr int NP = sizeof(T) == 4 ? 3 : 1;  // of P: all of its bits for f32 rows, 8 for BF16 ones, as their output
-  constexpr int OS = PaShape<D>::kOS;
+  constexpr int OS = PaShape<D, T>::kOS;
   extern __shared__ __align__(16) float s_o[];  // [NW][16][OS], then the maxima and sums
   float* s_m = s_o + NW * 16 * OS;
   float* s_l = s_m + NW * 16;
@@ -353,7 +355,8 @@ __global__ __launch_bounds__(64 * PaShape<D>::NW, PaShape<D>::kPerSimd) void pag
         pa_load<D, 0>(a.pool + ((int64_t)p0 * a.nkv + h) * a.block, tok & (ps - 1), lo_, x);
         pa_load<D, 1>(a.pool + ((int64_t)p1 * a.nkv + h) * a.block, (tok + 16) & (ps - 1), lo_, x);
       };
-      PaStepData<D> x[2];
+      constexpr bool ahead = PaShape<D, T>::kAhead > 0;
+      PaStepData<D> x[ahead ? 2 : 1];
       Raw8<T> qr[NG];
       const T* q = static_cast<const T*>(a.q) + t * a.qs + head * a.qh;
 #pragma unroll
@@ -506,18 +509,28 @@ __global__ __launch_bounds__(64 * PaShape<D>::NW, PaShape<D>::kPerSimd) void pag
       const auto work = [&](int k, int q0, int q1, PaStepData<D>& x) {
         step(x, (sb + wave + k * NW) * kPaStep, q0 >= 0, q1 >= 0);
       };
-      for (int k = 0; k < mine; k += 2) {
-        int q0 = __builtin_amdgcn_readlane(pg0, k & 63), q1 = __builtin_amdgcn_readlane(pg1, k & 63);
-        if (k + 1 < mine) load(k + 1, x[1]);  // 64 is even: of the same pages
-        work(k, q0, q1, x[0]);
-        if (k + 1 >= mine) break;
-        q0 = __builtin_amdgcn_readlane(pg0, (k + 1) & 63);
-        q1 = __builtin_amdgcn_readlane(pg1, (k + 1) & 63);
-        if (k + 2 < mine) {
-          if (((k + 2) & 63) == 0) pages(k + 2);
-          load(k + 2, x[0]);
+      if constexpr (ahead) {
+        for (int k = 0; k < mine; k += 2) {
+          int q0 = __builtin_amdgcn_readlane(pg0, k & 63), q1 = __builtin_amdgcn_readlane(pg1, k & 63);
+          if (k + 1 < mine) load(k + 1, x[1]);  // 64 is even: of the same pages
+          work(k, q0, q1, x[0]);
+          if (k + 1 >= mine) break;
+          q0 = __builtin_amdgcn_readlane(pg0, (k + 1) & 63);
+          q1 = __builtin_amdgcn_readlane(pg1, (k + 1) & 63);
+          if (k + 2 < mine) {
+            if (((k + 2) & 63) == 0) pages(k + 2);
+            load(k + 2, x[0]);
+          }
+          work(k + 1, q0, q1, x[1]);
         }
-        work(k + 1, q0, q1, x[1]);
+      } else {
+        for (int k = 0; k < mine; ++k) {
+          work(k, __builtin_amdgcn_readlane(pg0, k & 63), __builtin_amdgcn_readlane(pg1, k & 63), x[0]);
+          if (k + 1 < mine) {
+            if (((k + 1) & 63) == 0) pages(k + 1);
+            load(k + 1, x[0]);
+          }
+        }
       }
     }
 
@@ -1061,27 +1074,42 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   const uint32_t t = (uint32_t)(row / a.nh);
-  if (t >= a.rows || t < a.off[0] || t >= a.off[a.batch]) return;
+  if (t >= a.rows) return;
   const int head = (int)(row - (int64_t)t * a.nh);
   const float2* __restrict__ ml = a.part_ml + row * a.nsplit;
   const float* __restrict__ po = a.part_o + row * a.nsplit * D + 4 * c;
+  // every load that the first parts need at once, whether the row is one of a sequence or not
+  const int s0 = (W > 1 ? wave : 0) * NS + sub;
+  constexpr int ST = (W > 1 ? W : 1) * NS, U = 4;
+  const int64_t first = a.off[0], last = a.off[a.batch];
+  float4 v[U];
+  float ms[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int s = min(s0 + u * ST, a.nsplit - 1);
+    ms[u] = ml[s].x;
+    v[u] = *reinterpret_cast<const float4*>(po + (int64_t)s * D);
+  }
   float2 x[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) x[k] = lane + 64 * k < a.nsplit ? ml[lane + 64 * k] : make_float2(-INFINITY, 0.0f);
+  if (t < first || t >= last) return;
   const float M = wave_max(fmaxf(x[0].x, x[1].x)), Mu = M == -INFINITY ? 0.0f : M;
   const float tot = wave_sum(__builtin_amdgcn_exp2f(x[0].x - Mu) * x[0].y + __builtin_amdgcn_exp2f(x[1].x - Mu) * x[1].y);
   float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-  for (int s = (W > 1 ? wave : 0) * NS + sub; s < a.nsplit; s += (W > 1 ? W : 1) * NS) {
-    const float ms = ml[s].x, w = __builtin_amdgcn_exp2f(ms - Mu);
-    const float4 v = *reinterpret_cast<const float4*>(po + (int64_t)s * D);
+  const auto add = [&](float m, const float4& y, bool there) {
     // a part without a key was not written; where NaN scores left no maximum, tot is NaN
-    const bool none = ms == -INFINITY;
-    acc.x = fmaf(w, none ? 0.0f : v.x, acc.x);
-    acc.y = fmaf(w, none ? 0.0f : v.y, acc.y);
-    acc.z = fmaf(w, none ? 0.0f : v.z, acc.z);
-    acc.w = fmaf(w, none ? 0.0f : v.w, acc.w);
-  }
+    const bool none = !there || m == -INFINITY;
+    const float w = none ? 0.0f : __builtin_amdgcn_exp2f(m - Mu);
+    acc.x = fmaf(w, none ? 0.0f : y.x, acc.x);
+    acc.y = fmaf(w, none ? 0.0f : y.y, acc.y);
+    acc.z = fmaf(w, none ? 0.0f : y.z, acc.z);
+    acc.w = fmaf(w, none ? 0.0f : y.w, acc.w);
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) add(ms[u], v[u], s0 + u * ST < a.nsplit);
+#pragma unroll 4
+  for (int s = s0 + U * ST; s < a.nsplit; s += ST) add(ml[s].x, *reinterpret_cast<const float4*>(po + (int64_t)s * D), true);
 #pragma unroll
   for (int m = C; m < 64; m <<= 1) {
     acc.x += __shfl_xor(acc.x, m);
@@ -1116,6 +1144,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaArgs a) {
 // them, and parts along the positions when the tiles alone do not fill the chip.
 constexpr int kPtWaves = 8;
 constexpr int kPtMinRows = 64;
+template <typename T>
+static int pa_fill_t(int d) {
+  return d == 64 ? PaShape<64, T>::kFill : d == 128 ? PaShape<128, T>::kFill : PaShape<256, T>::kFill;
+}
+static int pa_waves(int d, int dtype) {
+  return d == 64 ? (dtype == KH_DT_F32 ? PaShape<64, float>::NW : PaShape<64, uint16_t>::NW)
+       : d == 128 ? (dtype == KH_DT_F32 ? PaShape<128, float>::NW : PaShape<128, uint16_t>::NW)
+                  : PaShape<256, uint16_t>::NW;
+}
+static int pa_fill(int d, int dtype) { return dtype == KH_DT_F32 ? pa_fill_t<float>(d) : pa_fill_t<uint16_t>(d); }
 struct PaPlan {
   bool many;  // paged_tile_kernel
   int64_t tiles, base;
@@ -1132,9 +1170,11 @@ static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int
   if (p.tiles < 1) p.tiles = 1;
   if (p.tiles > 65536) p.tiles = 65536;
   p.base = batch * c->nkv * p.tiles;
-  const int64_t fill = p.many ? 256 : c->d == 64 ? PaShape<64>::kFill : c->d == 128 ? PaShape<128>::kFill : PaShape<256>::kFill;
+  const int64_t fill = p.many ? 256 : pa_fill(c->d, dtype);
   int64_t want = (fill + p.base - 1) / p.base;
-  const int64_t most = p.many ? (max_len + 511) / 512 : c->d == 256 ? (max_len + 127) / 128 : (max_len + 255) / 256;
+  // parts of fewer than four steps a wave do not pay for the join
+  const int64_t step = p.many ? 512 : 32 * pa_waves(c->d, dtype);
+  const int64_t most = max_len < 4 * step ? 1 : (max_len + step - 1) / step;
   if (want > most) want = most;
   if (want > kPaMaxSplit) want = kPaMaxSplit;
   p.nsplit = want < 1 ? 1 : (int)want;
@@ -1155,7 +1195,7 @@ static int pa_launch(const PaArgs& a, bool many, int64_t blocks, hipStream_t st)
   static std::once_flag once;
   static hipError_t arc = hipSuccess;
   std::call_once(once, [] {
-    arc = allow_lds(&paged_rows_kernel<D, T>, PaShape<D>::kLds);
+    arc = allow_lds(&paged_rows_kernel<D, T>, PaShape<D, T>::kLds);
     if constexpr (sizeof(T) == 2) {
       if (arc == hipSuccess) arc = allow_lds(&paged_tile_kernel<D, kPtWaves>, PtShape<D>::kLds);
     }
@@ -1168,7 +1208,7 @@ static int pa_launch(const PaArgs& a, bool many, int64_t blocks, hipStream_t st)
   if (!many)
     hipLaunchKernelGGL((paged_rows_kernel<D, T>),
                        dim3((unsigned)a.nsplit, (unsigned)a.nkv, (unsigned)(a.batch * a.tiles < 65535 ? a.batch * a.tiles : 65535)),
-                       dim3(64 * PaShape<D>::NW), PaShape<D>::kLds, st, a);
+                       dim3((64 * PaShape<D, T>::NW)), (PaShape<D, T>::kLds), st, a);
   if (a.nsplit > 16)
     hipLaunchKernelGGL((paged_join_kernel<D, T, 4>), dim3((unsigned)(a.rows * a.nh)), dim3(256), 0, st, a);
   else if (a.nsplit > 1)
