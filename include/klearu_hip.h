@@ -767,9 +767,10 @@ int kh_paged_kv_gather(const kh_paged_kv* c, int dtype, int64_t rows, const int6
                        int64_t batch, const int64_t* start_dev, const int32_t* table_dev,
                        int64_t table_cols, int64_t table_stride, void* k_dev, void* v_dev, void* stream);
 /* Bytes of workspace that kh_paged_kv_attention needs for these arguments (0
- * where one pass does it). */
+ * where one pass does it); with_lse: whether lse_dev will be given. */
 int kh_paged_kv_attention_workspace(const kh_paged_kv* c, int dtype, int64_t rows, int64_t batch,
-                                    int num_heads, int64_t max_rows, int64_t max_len, int64_t* bytes);
+                                    int num_heads, int64_t max_rows, int64_t max_len, int with_lse,
+                                    int64_t* bytes);
 /* Attention of q [rows][num_heads][head_dim] over the cache: sequence b has
  * len_dev[b] positions there (int64, its rows of this call among them, so row i
  * of its n rows is at position len - n + i), and
@@ -785,7 +786,10 @@ int kh_paged_kv_attention_workspace(const kh_paged_kv* c, int dtype, int64_t row
  * max_rows and max_len are the caller's guess of the most rows and the longest
  * length of a sequence; a wrong one costs time, not correctness.  Sums and
  * softmax statistics are f32; BF16 rows have their weights p rounded to BF16.
- * The result does not depend on the run.  ws_dev: 16-byte aligned,
+ * BF16 calls of many rows (max_rows times the query heads of a kv head of 64 or
+ * more) take keys and values rounded to BF16 as well; with lse_dev their keys are
+ * held to 2^-16 instead, so that out may differ from a call without it in the
+ * rounding.  The result does not depend on the run.  ws_dev: 16-byte aligned,
  * kh_paged_kv_attention_workspace bytes (fewer are KH_ERR_CAPACITY), not shared
  * by calls that may run at once; its contents do not matter. */
 int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void* q_dev, int64_t q_row_stride,

@@ -161,7 +161,7 @@ SIGS = {
     "kh_paged_kv_status": (I, [P]),
     "kh_paged_kv_append": (I, [P, P, I, P, I64, I64, P, I64, I64, I64, P, I64, P, P, P, I64, I64, P]),
     "kh_paged_kv_gather": (I, [P, I, I64, P, I64, P, P, I64, I64, P, P, P]),
-    "kh_paged_kv_attention_workspace": (I, [P, I, I64, I64, I, I64, I64, P]),
+    "kh_paged_kv_attention_workspace": (I, [P, I, I64, I64, I, I64, I64, I, P]),
     "kh_paged_kv_attention": (I, [P, I, P, I64, I64, I, I64, P, I64, P, P, I64, I64, I64, I64, F, I, I64, P, I, P,
                                   I64, I64, P, P, I64, P]),
     "kh_safetensors_open": (I, [S, PP]),

@@ -69,6 +69,9 @@ struct PaArgs {
   float2* part_ml;
   int nsplit, tiles;
   int qvec, ovec;
+  char* un;  // unpacked positions (tiles of many rows): un_steps steps of each sequence
+  uint32_t* un_nan;
+  int un_steps;
 };
 
 template <int N>
@@ -595,42 +598,63 @@ __global__ __launch_bounds__((64 * PaShape<D, T>::NW), (PaShape<D, T>::kPerSimd)
 }
 
 // ---------------------------------------------------------------- many rows
-// Tiles of many rows (prompts and chunks, BF16): a block's waves put 64 positions
-// at a time into LDS as BF16 numbers s c + m, in the order of the matrix core's
-// first operand, and every wave runs its own rows (16 CT columns) over them, so
-// the work of unpacking is shared by all rows of the block.  Rounding a key or a
-// value to BF16 is off by at most 2^-8 of it, as in a BF16 cache, and queries and
-// weights are BF16 themselves.  Codes of the next 64 positions are loaded while
-// these are worked on; two LDS buffers, one barrier per 64 positions.
+// Tiles of many rows (prompts and chunks, BF16): a step's 64 positions lie in LDS as
+// BF16 numbers s c + m, in the order of the matrix core's first operand, and every wave
+// runs its own rows (16 CT columns) over them, so the work of unpacking is shared by all
+// rows of the block.  Rounding a key or a value to BF16 is off by at most 2^-8 of it, as
+// in a BF16 cache, and queries and weights are BF16 themselves.  The next step's codes are
+// loaded and unpacked while this one is worked on: two LDS buffers, one barrier a step.
+//
+// Where three row tiles or more see the same positions, a kernel unpacks them once into
+// the workspace and the tiles copy them to LDS as they are: 4096 causal rows of 32 heads
+// of 128 take 13 + 166 us so, 210 us where each tile unpacks them; three chunks of 256-wide
+// heads 11 + 72 us against 103.  The copies go through registers: for a load straight to
+// LDS the compiler waits before the next read of any LDS (178 us).
 //
 // A value's group that stands for NaN is unpacked as 0 and marked in a mask of its
 // positions: rows that see one of them get their NaN from the mask.
-constexpr int kPtKeys = 64;
+//
+// Bound by its own latency: two waves a SIMD (registers), each with its products (41% of
+// the time), exponentials and roundings (29%) and waits one after the other.  Half of the
+// waves a phase later (177 us), exponentials between the products of the step before
+// (spills), blocks of four waves (187 us) and raised priority for products (no change)
+// did not help.
 constexpr int kOnlyAlu = 0x6;  // what a scheduling barrier lets pass: vector and scalar arithmetic
 constexpr float kPtSlack = 6.0f;  // a maximum that is passed by less (in powers of two) is kept
 
-template <int D>
+// KT: BF16 terms that a key is held in.  One gives outputs as exact as their type
+// holds; two (to 2^-16) and sums of weights that are not rounded are for callers who
+// want the log-sum-exp, which is f32.
+template <int D, int KT>
 struct PtShape {
+  static constexpr int NW = 8;
+  static constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16;
   static constexpr int CT = D == 256 ? 1 : 2;  // column tiles of 16 rows a wave holds
-  static constexpr int RW = 16 * CT;
-  static constexpr int kBuf = kPtKeys * D * 2;  // bytes of 64 keys or values
-  static constexpr int kLds = 4 * kBuf;         // two buffers of keys, two of values
+  static constexpr int RW = 16 * CT, RB = RW * NW;
+  static constexpr int KEYS = D == 256 && KT == 2 ? 32 : 64;  // positions of a step: two steps' fit in LDS
+  static constexpr int TK = KEYS / 16, TV = KEYS / 32;        // tiles of 16, halves of 32
+  static constexpr int kKeyPart = KEYS * D * 2, kKeys = KT * kKeyPart, kValues = KEYS * D * 2;
+  static constexpr int kStep = kKeys + kValues;               // bytes of a step
+  static constexpr int kLds = 2 * kStep;
+  static constexpr int KF = TK * NG / NW, VF = TV * NF / NW;  // fragments a wave unpacks
+  static constexpr int VG = VF < 2 ? 1 : VF / 2, VH = VF <= 4 ? 1 : VF / 4;
 };
 
+typedef int kh_i32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 kh_f16x2 __attribute__((ext_vector_type(2)));
 
-// Nibble n of each half of w as f32 (1024 + c), halves of a pair of f16.
+// Nibble n of each half of w as 16 + c, a pair of f16: six bits up it counts ones
+// behind the bits of 16.
 __device__ __forceinline__ kh_f16x2 codes_f16(uint32_t w, int n) {
-  return __builtin_bit_cast(kh_f16x2, ((w >> (4 * n)) & 0x000f000fu) | 0x64006400u);
+  const uint32_t x = n == 0 ? w << 6 : n == 1 ? w << 2 : n == 2 ? w >> 2 : w >> 6;
+  return __builtin_bit_cast(kh_f16x2, (x & 0x03c003c0u) | 0x4c004c00u);
 }
 
-template <int D, int NW>
+template <int D, int KT>
 struct PtCodes {
-  static constexpr int NG = D / kKvGroup, HN = D / 64;
-  static constexpr int KF = 4 * NG / NW, VF = 4 * NG / NW;  // fragments a wave unpacks
-  static constexpr int VG = VF < 2 ? 1 : VF / 2, VH = VF <= 4 ? 1 : VF / 4;
-  uint32_t kw[KF], kp[KF];
-  uint32_t vw[VH][4], vp[VG][8];
+  using S = PtShape<D, KT>;
+  uint32_t kw[S::KF], kp[S::KF];
+  uint32_t vw[S::VH][4], vp[S::VG][8];
 };
 
 template <int N>
@@ -649,40 +673,179 @@ __device__ __forceinline__ void ld_n(const char* p, uint32_t* w) {
   }
 }
 
-template <int D, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
-  using S = PtShape<D>;
-  using C = PtCodes<D, NW>;
+// What wave `wave` of NW does to a step's positions: KF fragments of keys of one of
+// their tiles of 16, VF of values of one half of 32.  A fragment is what the 64 lanes of
+// a wave hold of a matrix-core operand, 16 bytes each: of keys, tile by tile, NG; of
+// values, half by half, D / 16.
+template <int D, int KT>
+struct PtUnpack {
+  using S = PtShape<D, KT>;
+  using C = PtCodes<D, KT>;
   using P = KvParts<D>;
-  constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16, CT = S::CT, RW = S::RW, RB = RW * NW;
-  constexpr int KF = C::KF, VF = C::VF;
-  extern __shared__ __align__(16) char s_buf[];
-  __shared__ int s_lo[NW], s_hi[NW];
-  __shared__ uint32_t s_nan[2][NG][2];  // positions whose value group stands for NaN
+  static constexpr int NG = S::NG, HN = S::HN, NF = S::NF, KF = S::KF, VF = S::VF, NW = S::NW;
+  int ps, g, ktile, kj0, vtb, vf0;
+  uint32_t koff, kpoff, voff, vpoff;  // the lane's words in a block
+  __device__ __forceinline__ PtUnpack(int lane, int wave, int page_size) : ps(page_size), g(lane >> 4) {
+    const int col = lane & 15;
+    ktile = wave / (NW / S::TK);
+    kj0 = (wave % (NW / S::TK)) * KF;
+    vtb = wave / (NW / S::TV);
+    vf0 = (wave % (NW / S::TV)) * VF;
+    koff = P::kc() + col * (D / 2) + (g * NG + kj0) * 4;
+    kpoff = P::kp(ps) + (col * NG + kj0) * 4;
+    voff = P::vc(ps) + (g * 16 + col) * (HN * 8) + (vf0 >> 2) * 4;
+    vpoff = P::vp(ps) + ((vf0 >> 1) * ps + 4 * g) * 4;
+  }
+  // tok: the first of the step's positions; blk(k): the block of their k-th tile of 16.
+  template <typename B>
+  __device__ __forceinline__ void load(int tok, B blk, C& x) const {
+    const int in = (tok + ktile * 16) & (ps - 1);
+    const char* kb = blk(ktile);
+    ld_n<KF>(kb + in * (D / 2) + koff, x.kw);
+    ld_n<KF>(kb + in * (NG * 4) + kpoff, x.kp);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int iv = (tok + vtb * 32 + q * 16) & (ps - 1);
+      const char* vb = blk(2 * vtb + q);
+      const char* vw = vb + iv * (D / 2) + voff;
+#pragma unroll
+      for (int hh = 0; hh < S::VH; ++hh) {
+        x.vw[hh][2 * q] = *reinterpret_cast<const uint32_t*>(vw + hh * 4);
+        x.vw[hh][2 * q + 1] = *reinterpret_cast<const uint32_t*>(vw + HN * 4 + hh * 4);
+      }
+#pragma unroll
+      for (int gi = 0; gi < S::VG; ++gi) ld_n<4>(vb + iv * 4 + gi * ps * 4 + vpoff, &x.vp[gi][4 * q]);
+    }
+  }
+  // put(term, fragment, the lane's 16 bytes)
+  template <typename F>
+  __device__ __forceinline__ void keys(const C& x, F put) const {
+#pragma unroll
+    for (int f = 0; f < KF; ++f) {
+      const float s = __uint_as_float(x.kp[f] & 0xffff0000u);
+      const float t = fmaf(-16.0f, s, __uint_as_float(x.kp[f] << 16));
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const kh_f16x2 c = codes_f16(x.kw[f], i);
+        v[i] = fmaf((float)c.x, s, t);
+        v[i + 4] = fmaf((float)c.y, s, t);
+      }
+      uint4 w[KT];
+      terms8<KT>(v, w);
+#pragma unroll
+      for (int k = 0; k < KT; ++k) put(k, ktile * NG + kj0 + f, w[k]);
+    }
+  }
+  // A group that stands for NaN counts as 0 from here on: mask(group, half, its
+  // positions among the half's 32).
+  template <typename F>
+  __device__ __forceinline__ void nan(C& x, F mask) const {
+#pragma unroll
+    for (int gi = 0; gi < S::VG; ++gi) {
+      uint32_t top = x.vp[gi][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) top = max(top, x.vp[gi][e]);
+      uint32_t nan = 0;
+      if (__ballot(top >= 0x7fc00000u)) {
+        uint32_t from = 0x7fc00000u;
+        asm volatile("" : "+s"(from));  // keeps this behind its branch
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t is = x.vp[gi][e] >= from ? 1u : 0u;
+          nan |= is << ((e < 4 ? 0 : 16) + 4 * g + (e & 3));
+          x.vp[gi][e] &= is - 1u;
+        }
+        nan = across_groups_or(nan);
+      }
+      if (VF > 1 || (vf0 & 1) == 0) mask((vf0 >> 1) + gi, vtb, nan);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void values(const C& x, F put) const {
+#pragma unroll
+    for (int gi = 0; gi < S::VG; ++gi) {
+      float s[8], t[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s[e] = __uint_as_float(x.vp[gi][e] & 0xffff0000u);
+        t[e] = fmaf(-16.0f, s[e], __uint_as_float(x.vp[gi][e] << 16));
+      }
+#pragma unroll
+      for (int ff = 0; ff < (VF < 2 ? 1 : 2); ++ff) {
+        const int fi = 2 * gi + ff;  // of the wave's
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const kh_f16x2 c = codes_f16(x.vw[VF <= 4 ? 0 : fi >> 2][e], (vf0 + fi) & 3);
+          v[2 * e] = fmaf((float)c.x, s[2 * e], t[2 * e]);
+          v[2 * e + 1] = fmaf((float)c.y, s[2 * e + 1], t[2 * e + 1]);
+        }
+        uint4 w[1];
+        terms8<1>(v, w);
+        put(vtb * NF + vf0 + fi, w[0]);
+      }
+    }
+  }
+};
+
+// Where a step's positions of one (sequence, kv head) lie in the workspace once they
+// are unpacked for all tiles, kStep bytes each: their keys' fragments, term by term,
+// then their values'.  Behind all steps: the masks [NG][2] of value groups that
+// stand for NaN.
+__device__ __forceinline__ int64_t pt_step(const PaArgs& a, int64_t b, int h, int st) {
+  return (b * a.nkv + h) * a.un_steps + st;
+}
+
+// The positions that some row of the call sees, unpacked once for all of its row
+// tiles: a block a step of a (sequence, kv head).
+template <int D, int KT>
+__global__ __launch_bounds__((64 * PtShape<D, KT>::NW)) void paged_unpack_kernel(PaArgs a) {
+  using S = PtShape<D, KT>;
+  using U = PtUnpack<D, KT>;
+  constexpr int NG = S::NG, KEYS = S::KEYS;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int st = blockIdx.x, h = blockIdx.y;
+  const U u(lane, wave, 1 << a.ps_log2);
+  for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
+    const int32_t* __restrict__ table = a.table + b * a.table_stride;
+    const int64_t n = min(a.off[b + 1], a.rows) - max(a.off[b], (int64_t)0), L = a.len[b];
+    if (n <= 0 || L > (a.cols << a.ps_log2) || L > (int64_t)a.un_steps * KEYS) continue;
+    const int64_t first = a.window > 0 && L - n - a.window + 1 > 0 ? L - n - a.window + 1 : 0;
+    if ((int64_t)(st + 1) * KEYS <= first || (int64_t)st * KEYS >= L) continue;
+    const auto blk = [&](int k) -> const char* {
+      const int tok = min(max(st * KEYS + k * 16, (int)first), (int)L - 1);
+      int pg = __builtin_amdgcn_readfirstlane(table[tok >> a.ps_log2]);
+      if (pg < 0 || pg >= a.pages) pg = 0;  // the tiles' rows know that it is not there
+      return a.pool + ((int64_t)pg * a.nkv + h) * a.block;
+    };
+    typename U::C x;
+    u.load(st * KEYS, blk, x);
+    const int64_t at = pt_step(a, b, h, st);
+    char* to = a.un + at * S::kStep + lane * 16;
+    u.keys(x, [&](int k, int f, const uint4& w) { *reinterpret_cast<uint4*>(to + k * S::kKeyPart + f * 1024) = w; });
+    u.nan(x, [&](int gi, int half, uint32_t m) {
+      if (lane == 0) a.un_nan[(at * NG + gi) * 2 + half] = m;
+    });
+    u.values(x, [&](int f, const uint4& w) { *reinterpret_cast<uint4*>(to + S::kKeys + f * 1024) = w; });
+  }
+}
+
+// UN: the positions lie unpacked in the workspace, and go from there to LDS as they
+// are.
+template <int D, int KT, bool UN>
+__device__ __forceinline__ void pt_tiles(const PaArgs& a, char* s_buf, int* s_lo, int* s_hi,
+                                         uint32_t (*s_nan)[D / kKvGroup][2], int64_t b, int h, int split, int tile0,
+                                         int64_t o0, int64_t o1, int64_t L) {
+  using S = PtShape<D, KT>;
+  constexpr int NG = S::NG, NF = S::NF, CT = S::CT, RW = S::RW, RB = S::RB, NW = S::NW;
+  constexpr int KEYS = S::KEYS, TK = S::TK, TV = S::TV;
+  constexpr int kRound = 64 / TK;  // steps whose tiles' pages the lanes hold
   const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint32_t id = blockIdx.x;
-  const int h = (int)(id % (uint32_t)a.nkv);
-  id /= (uint32_t)a.nkv;
-  const int split = (int)(id % (uint32_t)a.nsplit);
-  id /= (uint32_t)a.nsplit;
-  const int64_t b = id % (uint32_t)a.batch;
-  const int tile0 = a.tiles - 1 - (int)(id / (uint32_t)a.batch);  // the longest first
-  const int ps = 1 << a.ps_log2;
-  int64_t o0 = a.off[b], o1 = a.off[b + 1];
-  o0 = o0 < 0 ? 0 : o0;
-  o1 = o1 > a.rows ? a.rows : o1;
-  if (o1 <= o0) return;
   const int n = (int)(o1 - o0), nr = n * a.gs;
-  const int64_t cap = a.cols << a.ps_log2;
-  int64_t L = a.len[b];
-  if (L < 0 || L > cap) {
-    if (threadIdx.x == 0) atomicOr(a.err, 1);
-    L = L < 0 ? 0 : cap;
-  }
   const int32_t* __restrict__ table = a.table + b * a.table_stride;
-  const int ktile = wave / (NW / 4), kj0 = (wave % (NW / 4)) * KF;  // the fragments this wave unpacks
-  const int vtb = wave / (NW / 2), vf0 = (wave % (NW / 2)) * VF;
+  const PtUnpack<D, KT> un(lane, wave, 1 << a.ps_log2);
 
   for (int tile = tile0; tile < (nr + RB - 1) / RB; tile += a.tiles) {
     int lo[CT], hi[CT];
@@ -728,7 +891,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
     thi = __builtin_amdgcn_readfirstlane(thi);
 
     float m[CT];
-    kh_f32x4 l[CT], o[CT][NF];  // l: a product with ones, all four alike
+    kh_f32x4 l[CT], o[CT][NF];  // l: a product with ones, all four alike; KT > 1: [0] of the lane's own weights
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       m[c] = -INFINITY;
@@ -736,7 +899,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
 #pragma unroll
       for (int f = 0; f < NF; ++f) o[c][f] = kh_f32x4{0, 0, 0, 0};
     }
-    const int first = tlo / kPtKeys, steps = thi > tlo ? (thi + kPtKeys - 1) / kPtKeys - first : 0;
+    const int first = tlo / KEYS, steps = thi > tlo ? (thi + KEYS - 1) / KEYS - first : 0;
     const int per = (steps + a.nsplit - 1) / a.nsplit;
     const int sb = first + split * per, se = min(first + steps, sb + per);
     if (sb < se) {
@@ -757,12 +920,12 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
           }
         }
       }
-      // Lane i holds the offset of the block of the i-th of 64 tiles of 16 positions: the next sixteen
-      // steps'.  Bits of okm say which pages there are, of these steps and (high) the next.
+      // Lane i holds the offset of the block of the i-th of 64 tiles of 16 positions, the next
+      // kRound steps'.  Bits of okn say which pages there are, those of okm the round before.
       uint32_t blk_lo = 0, blk_hi = 0;
       uint64_t okm = 0, okn = 0;
       const auto pages = [&](int st) {
-        const int tok = min(max(st * kPtKeys + lane * 16, tlo & ~15), (thi - 1) & ~15);
+        const int tok = min(max(st * KEYS + lane * 16, tlo & ~15), (thi - 1) & ~15);
         const int pg = table[max(tok, tlo) >> a.ps_log2];
         const bool there = pg >= 0 && pg < a.pages;
         if (!there) atomicOr(a.err, 2);
@@ -772,135 +935,77 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
         okn = __ballot(there);
       };
       const auto blk = [&](int st, int k) {
-        const int l = ((st - sb) & 15) * 4 + k;
+        const int l = ((st - sb) & (kRound - 1)) * TK + k;
         const uint32_t x = __builtin_amdgcn_readlane(blk_lo, l), y = __builtin_amdgcn_readlane(blk_hi, l);
         return a.pool + ((uint64_t)y << 32 | x);
       };
-      const uint32_t koff = P::kc() + col * (D / 2) + (g * NG + kj0) * 4, kpoff = P::kp(ps) + (col * NG + kj0) * 4;
-      const uint32_t voff = P::vc(ps) + (g * 16 + col) * (HN * 8) + (vf0 >> 2) * 4;
-      const uint32_t vpoff = P::vp(ps) + ((vf0 >> 1) * ps + 4 * g) * 4;
-      const auto load = [&](int st, C& x) {
-        const int in = (st * kPtKeys + ktile * 16) & (ps - 1);
-        const char* kb = blk(st, ktile);
-        ld_n<KF>(kb + in * (D / 2) + koff, x.kw);
-        ld_n<KF>(kb + in * (NG * 4) + kpoff, x.kp);
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int iv = (st * kPtKeys + vtb * 32 + q * 16) & (ps - 1);
-          const char* vb = blk(st, 2 * vtb + q);
-          const char* vw = vb + iv * (D / 2) + voff;
-#pragma unroll
-          for (int hh = 0; hh < C::VH; ++hh) {
-            x.vw[hh][2 * q] = *reinterpret_cast<const uint32_t*>(vw + hh * 4);
-            x.vw[hh][2 * q + 1] = *reinterpret_cast<const uint32_t*>(vw + HN * 4 + hh * 4);
-          }
-#pragma unroll
-          for (int gi = 0; gi < C::VG; ++gi) ld_n<4>(vb + iv * 4 + gi * ps * 4 + vpoff, &x.vp[gi][4 * q]);
-        }
+      PtCodes<D, KT> x;
+      const auto load = [&](int st) { un.load(st * KEYS, [&](int k) { return blk(st, k); }, x); };
+      const auto unpack = [&](int st) {
+        char* buf = s_buf + (st & 1) * S::kStep + lane * 16;
+        un.keys(x, [&](int k, int f, const uint4& w) { *reinterpret_cast<uint4*>(buf + k * S::kKeyPart + f * 1024) = w; });
+        un.nan(x, [&](int gi, int half, uint32_t m) {
+          if (lane == 0) s_nan[st & 1][gi][half] = m;
+        });
+        un.values(x, [&](int f, const uint4& w) { *reinterpret_cast<uint4*>(buf + S::kKeys + f * 1024) = w; });
       };
-      const auto unpack_k = [&](int st, const C& x) {
-        char* kbuf = s_buf + (st & 1) * S::kBuf;
+      // UN: a wave's share of the step's bytes, and the masks
+      constexpr int SHARE = S::kStep / 1024 / NW;
+      kh_i32x4 raw[SHARE];
+      uint32_t nan0 = 0, nan1 = 0, nan2 = 0;  // of the step that is worked on, and the next two
+      const auto fetch = [&](int st) {
+        const int64_t at = pt_step(a, b, h, st);
+        const char* from = a.un + at * S::kStep + wave * SHARE * 1024 + lane * 16;
 #pragma unroll
-        for (int f = 0; f < KF; ++f) {
-          const float s = __uint_as_float(x.kp[f] & 0xffff0000u);
-          const float t = fmaf(-1024.0f, s, __uint_as_float(x.kp[f] << 16));
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const kh_f16x2 c = codes_f16(x.kw[f], i);
-            v[i] = fmaf((float)c.x, s, t);
-            v[i + 4] = fmaf((float)c.y, s, t);
-          }
-          uint4 w[1];
-          terms8<1>(v, w);
-          *reinterpret_cast<uint4*>(kbuf + ((ktile * NG + kj0 + f) * 64 + lane) * 16) = w[0];
-        }
+        for (int i = 0; i < SHARE; ++i) raw[i] = *reinterpret_cast<const kh_i32x4*>(from + i * 1024);
+        nan2 = a.un_nan[at * (2 * NG) + (lane & (2 * NG - 1))];
       };
-      // A group that stands for NaN counts as 0, and its positions go to the masks.
-      const auto mark_nan = [&](int st, C& x) {
+      const auto place = [&](int st) {
+        char* to = s_buf + (st & 1) * S::kStep + wave * SHARE * 1024 + lane * 16;
 #pragma unroll
-        for (int gi = 0; gi < C::VG; ++gi) {
-          uint32_t top = x.vp[gi][0];
-#pragma unroll
-          for (int e = 1; e < 8; ++e) top = max(top, x.vp[gi][e]);
-          uint32_t nan = 0;
-          if (__ballot(top >= 0x7fc00000u)) {
-            uint32_t from = 0x7fc00000u;
-            asm volatile("" : "+s"(from));  // keeps this behind its branch
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const uint32_t is = x.vp[gi][e] >= from ? 1u : 0u;
-              nan |= is << ((e < 4 ? 0 : 16) + 4 * g + (e & 3));
-              x.vp[gi][e] &= is - 1u;
-            }
-            nan = across_groups_or(nan);
-          }
-          if (lane == 0 && (VF > 1 || (vf0 & 1) == 0)) s_nan[st & 1][(vf0 >> 1) + gi][vtb] = nan;
-        }
+        for (int i = 0; i < SHARE; ++i) *reinterpret_cast<kh_i32x4*>(to + i * 1024) = raw[i];
       };
-      const auto unpack_v = [&](int st, const C& x) {
-        char* vbuf = s_buf + (2 + (st & 1)) * S::kBuf;
-#pragma unroll
-        for (int gi = 0; gi < C::VG; ++gi) {
-          float s[8], t[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            s[e] = __uint_as_float(x.vp[gi][e] & 0xffff0000u);
-            t[e] = fmaf(-1024.0f, s[e], __uint_as_float(x.vp[gi][e] << 16));
-          }
-#pragma unroll
-          for (int ff = 0; ff < (VF < 2 ? 1 : 2); ++ff) {
-            const int fi = 2 * gi + ff;  // of the wave's
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const kh_f16x2 c = codes_f16(x.vw[VF <= 4 ? 0 : fi >> 2][e], (vf0 + fi) & 3);
-              v[2 * e] = fmaf((float)c.x, s[2 * e], t[2 * e]);
-              v[2 * e + 1] = fmaf((float)c.y, s[2 * e + 1], t[2 * e + 1]);
-            }
-            uint4 w[1];
-            terms8<1>(v, w);
-            *reinterpret_cast<uint4*>(vbuf + ((vtb * NF + vf0 + fi) * 64 + lane) * 16) = w[0];
-          }
-        }
-      };
-      kh_f32x4 sc[CT][4];
-      uint4 pf[CT][2];
+      kh_f32x4 sc[CT][TK];
+      uint4 pf[CT][TV];
       float mc[CT];
       // Fragments are read one group ahead of the products that take them.
       const auto scores = [&](int st) {
-        const char* kbuf = s_buf + (st & 1) * S::kBuf + lane * 16;
+        const char* kbuf = s_buf + (st & 1) * S::kStep + lane * 16;
+        constexpr int R = TK * KT;  // groups of NG fragments: a tile's last term first
         uint4 kf[2][NG];
+        const auto at = [&](int r, int j) { return kbuf + (KT - 1 - r % KT) * S::kKeyPart + (r / KT * NG + j) * 1024; };
 #pragma unroll
-        for (int j = 0; j < NG; ++j) kf[0][j] = *reinterpret_cast<const uint4*>(kbuf + j * 1024);
+        for (int j = 0; j < NG; ++j) kf[0][j] = *reinterpret_cast<const uint4*>(at(0, j));
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          if (kt < 3) {
+        for (int r = 0; r < R; ++r) {
+          if (r + 1 < R) {
 #pragma unroll
-            for (int j = 0; j < NG; ++j)
-              kf[(kt + 1) & 1][j] = *reinterpret_cast<const uint4*>(kbuf + ((kt + 1) * NG + j) * 1024);
+            for (int j = 0; j < NG; ++j) kf[(r + 1) & 1][j] = *reinterpret_cast<const uint4*>(at(r + 1, j));
           }
           __builtin_amdgcn_sched_barrier(kOnlyAlu);
+          const int kt = r / KT;
+          if (r % KT == 0) {
 #pragma unroll
-          for (int c = 0; c < CT; ++c) sc[c][kt] = kh_f32x4{0, 0, 0, 0};
+            for (int c = 0; c < CT; ++c) sc[c][kt] = kh_f32x4{0, 0, 0, 0};
+          }
 #pragma unroll
           for (int j = 0; j < NG; ++j)
 #pragma unroll
-            for (int c = 0; c < CT; ++c) sc[c][kt] = mfma16(kf[kt & 1][j], qf[c][j], sc[c][kt]);
+            for (int c = 0; c < CT; ++c) sc[c][kt] = mfma16(kf[r & 1][j], qf[c][j], sc[c][kt]);
           __builtin_amdgcn_sched_barrier(kOnlyAlu);
         }
       };
       const auto whole = [&](int st, int ok) {
-        return st * kPtKeys >= (int)all_lo && (st + 1) * kPtKeys <= (int)all_hi && ok == 15;
+        return st * KEYS >= (int)all_lo && (st + 1) * KEYS <= (int)all_hi && ok == (1 << TK) - 1;
       };
       const auto hide = [&](int st, int ok) {
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-          int from = lo[c] - st * kPtKeys - 4 * g;
+          int from = lo[c] - st * KEYS - 4 * g;
           asm volatile("" : "+v"(from));  // keeps this behind its branch: 32 selects of every step otherwise
           const uint32_t span = (uint32_t)(hi[c] - lo[c]);
 #pragma unroll
-          for (int kt = 0; kt < 4; ++kt) {
+          for (int kt = 0; kt < TK; ++kt) {
             const uint32_t n = ok >> kt & 1 ? span : 0u;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -914,7 +1019,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
         for (int c = 0; c < CT; ++c) {
           mx[c] = sc[c][0][0];
 #pragma unroll
-          for (int e = 1; e < 16; ++e) mx[c] = fmaxf(mx[c], sc[c][e >> 2][e & 3]);
+          for (int e = 1; e < 4 * TK; ++e) mx[c] = fmaxf(mx[c], sc[c][e >> 2][e & 3]);
         }
       };
       const auto rescale = [&]() {
@@ -940,23 +1045,24 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
           uint4 w[1];
           terms8<1>(p, w);
           pf[c][tb] = w[0];
+          if (KT > 1) l[c][0] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
         }
       };
       constexpr int VQ = 4;  // value fragments of a group
       uint4 vf[2][VQ];
       const auto values = [&](int st, int k) {  // group k of step st's
-        const char* vbuf = s_buf + (2 + (st & 1)) * S::kBuf + lane * 16;
+        const char* vbuf = s_buf + (st & 1) * S::kStep + S::kKeys + lane * 16;
 #pragma unroll
         for (int i = 0; i < VQ; ++i) vf[k & 1][i] = *reinterpret_cast<const uint4*>(vbuf + (k * VQ + i) * 1024);
       };
       const auto sum_values = [&](int st) {  // values(st, 0) is under way
         const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
 #pragma unroll
-        for (int k = 0; k < 2 * NF / VQ; ++k) {
+        for (int k = 0; k < TV * NF / VQ; ++k) {
           const int tb = k * VQ / NF;
-          if (k + 1 < 2 * NF / VQ) values(st, k + 1);
+          if (k + 1 < TV * NF / VQ) values(st, k + 1);
           __builtin_amdgcn_sched_barrier(kOnlyAlu);
-          if (k * VQ % NF == 0) {
+          if (KT == 1 && k * VQ % NF == 0) {
 #pragma unroll
             for (int c = 0; c < CT; ++c) l[c] = mfma16(ones, pf[c][tb], l[c]);
           }
@@ -972,19 +1078,27 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
       };
       const auto spread_nan = [&](int st, int ok) {
         uint32_t any = 0;
+        if constexpr (UN) {
+          any = __ballot(nan0 != 0) != 0;
+        } else {
 #pragma unroll
-        for (int gi = 0; gi < NG; ++gi) any |= s_nan[st & 1][gi][0] | s_nan[st & 1][gi][1];
+          for (int gi = 0; gi < NG; ++gi) any |= s_nan[st & 1][gi][0] | s_nan[st & 1][gi][1];
+        }
         if (!__builtin_amdgcn_readfirstlane(any)) return;
-        int tok = st * kPtKeys;
+        int tok = st * KEYS;
         asm volatile("" : "+s"(tok));  // keeps this behind its branch
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi) {
-          const uint64_t mask = s_nan[st & 1][gi][0] | (uint64_t)s_nan[st & 1][gi][1] << 32;
+          uint64_t mask;
+          if constexpr (UN)
+            mask = (uint32_t)__builtin_amdgcn_readlane(nan0, 2 * gi) |
+                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane(nan0, 2 * gi + 1) << 32;
+          else mask = s_nan[st & 1][gi][0] | (uint64_t)s_nan[st & 1][gi][1] << 32;
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
-            const int from = max(lo[c] - tok, 0), to = min(hi[c] - tok, kPtKeys);  // of the 64 positions
+            const int from = max(lo[c] - tok, 0), to = min(hi[c] - tok, KEYS);  // of the 64 positions
             uint64_t see = to > from ? (~0ull >> (64 - (to - from))) << from : 0;
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < TK; ++k)
               if (!(ok >> k & 1)) see &= ~(0xffffull << (16 * k));
             if (mask & see) {
               const float x = __uint_as_float(0x7fc00000u);
@@ -997,36 +1111,42 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
 #pragma unroll
       for (int c = 0; c < CT; ++c) mc[c] = 0.0f;
       const bool busy = whi > wlo;  // some row of the wave sees something
-      C x;
       pages(sb);
-      load(sb, x);
-      unpack_k(sb, x);
-      mark_nan(sb, x);
-      unpack_v(sb, x);
-      if (sb + 1 < se) load(sb + 1, x);
+      if constexpr (UN) {
+        fetch(sb);
+        place(sb);
+        nan1 = nan2;
+        if (sb + 1 < se) fetch(sb + 1);
+      } else {
+        load(sb);
+        unpack(sb);
+        if (sb + 1 < se) load(sb + 1);
+      }
       for (int st = sb; st < se; ++st) {
+        // pages() for the next round comes two steps before it
+        const int i = (st - sb) & (kRound - 1);
         __syncthreads();
+        nan0 = nan1;
+        nan1 = nan2;
         if (st + 1 < se) {
-          unpack_k(st + 1, x);
-          mark_nan(st + 1, x);
-          unpack_v(st + 1, x);
+          if constexpr (UN) place(st + 1);
+          else unpack(st + 1);
         }
-        // pages() for the next sixteen steps comes two steps before them
-        const int i = (st - sb) & 15;
-        if (i == 14) okm = okn;
+        if (i == kRound - 2) okm = okn;
         if (st + 2 < se) {
-          if (i == 14) pages(st + 2);
-          load(st + 2, x);
+          if (i == kRound - 2) pages(st + 2);
+          if constexpr (UN) fetch(st + 2);
+          else load(st + 2);
         }
-        const int ok = (int)((i >= 14 ? okm : okn) >> (4 * i)) & 15;
+        const int ok = (int)((i >= kRound - 2 ? okm : okn) >> (TK * i)) & ((1 << TK) - 1);
         if (busy) {
           scores(st);
           values(st, 0);
           if (!whole(st, ok)) hide(st, ok);
           top();
           rescale();
-          weights(0);
-          weights(1);
+#pragma unroll
+          for (int tb = 0; tb < TV; ++tb) weights(tb);
           sum_values(st);
           spread_nan(st, ok);
         }
@@ -1035,7 +1155,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
 
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      const float tot = l[c][0];
+      const float tot = KT > 1 ? across_groups_sum(l[c][0]) : l[c][0];
       const float M = m[c] * a.c1;
       const bool some = hi[c] > lo[c];
       if (!inside[c]) continue;
@@ -1062,6 +1182,36 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_tile_kernel(PaArgs a) {
       }
     }
   }
+}
+
+// Blocks of the same kv head lie on the same XCD (h is what varies fastest, and
+// there are eight), and the longest tiles begin first.
+template <int D, int KT, bool UN>
+__global__ __launch_bounds__((64 * PtShape<D, KT>::NW), 2) void paged_tile_kernel(PaArgs a) {
+  extern __shared__ __align__(16) char s_buf[];
+  __shared__ int s_lo[PtShape<D, KT>::NW], s_hi[PtShape<D, KT>::NW];
+  __shared__ uint32_t s_nan[2][D / kKvGroup][2];  // positions whose value group stands for NaN
+  uint32_t id = blockIdx.x;
+  const int h = (int)(id % (uint32_t)a.nkv);
+  id /= (uint32_t)a.nkv;
+  const int split = (int)(id % (uint32_t)a.nsplit);
+  id /= (uint32_t)a.nsplit;
+  const int64_t b = id % (uint32_t)a.batch;
+  const int tile0 = a.tiles - 1 - (int)(id / (uint32_t)a.batch);
+  int64_t o0 = a.off[b], o1 = a.off[b + 1], L = a.len[b];
+  o0 = o0 < 0 ? 0 : o0;
+  o1 = o1 > a.rows ? a.rows : o1;
+  if (o1 <= o0) return;
+  const int64_t cap = a.cols << a.ps_log2;
+  if (L < 0 || L > cap) {
+    if (threadIdx.x == 0) atomicOr(a.err, 1);
+    L = L < 0 ? 0 : cap;
+  }
+  // a sequence that is longer than the caller said was not unpacked
+  if (UN && a.len[b] <= (int64_t)a.un_steps * PtShape<D, KT>::KEYS && a.len[b] <= cap)
+    pt_tiles<D, KT, true>(a, s_buf, s_lo, s_hi, s_nan, b, h, split, tile0, o0, o1, L);
+  else
+    pt_tiles<D, KT, false>(a, s_buf, s_lo, s_hi, s_nan, b, h, split, tile0, o0, o1, L);
 }
 
 // Joins the parts of each row: W waves a (row, head), four elements a lane, so
@@ -1142,8 +1292,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaArgs a) {
 
 // How a call is cut: row tiles per (sequence, kv head) as the caller expects
 // them, and parts along the positions when the tiles alone do not fill the chip.
-constexpr int kPtWaves = 8;
 constexpr int kPtMinRows = 64;
+constexpr int kPtUnpackTiles = 3;                    // row tiles from which on positions are unpacked ahead of them
+constexpr int64_t kPtUnpackMost = (int64_t)1 << 30;  // bytes of them
 template <typename T>
 static int pa_fill_t(int d) {
   return d == 64 ? PaShape<64, T>::kFill : d == 128 ? PaShape<128, T>::kFill : PaShape<256, T>::kFill;
@@ -1154,23 +1305,40 @@ static int pa_waves(int d, int dtype) {
                   : PaShape<256, uint16_t>::NW;
 }
 static int pa_fill(int d, int dtype) { return dtype == KH_DT_F32 ? pa_fill_t<float>(d) : pa_fill_t<uint16_t>(d); }
+struct PtSize {
+  int keys, step, rows, fill;  // positions of a step, their bytes, rows of a block, blocks that the chip holds
+};
+template <int D, int KT>
+static PtSize pt_size_dk() {
+  using S = PtShape<D, KT>;
+  return {S::KEYS, S::kStep, S::RB, 256 * 8 / S::NW};
+}
+template <int D>
+static PtSize pt_size_d(bool lse) {
+  return lse ? pt_size_dk<D, 2>() : pt_size_dk<D, 1>();
+}
+static PtSize pt_size(int d, bool lse) {
+  return d == 64 ? pt_size_d<64>(lse) : d == 128 ? pt_size_d<128>(lse) : pt_size_d<256>(lse);
+}
 struct PaPlan {
   bool many;  // paged_tile_kernel
   int64_t tiles, base;
   int nsplit;
+  int64_t un_steps;  // steps of each sequence that are unpacked ahead, or 0
 };
 static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int64_t batch, int64_t max_rows,
-                      int64_t max_len) {
+                      int64_t max_len, bool lse) {
   PaPlan p;
   const int64_t gs = nh / c->nkv;
   if (max_rows > rows) max_rows = rows;
   p.many = dtype == KH_DT_BF16 && max_rows * gs >= kPtMinRows;
-  const int64_t rb = p.many ? (c->d == 256 ? 16 : 32) * kPtWaves : 16;
+  const PtSize z = pt_size(c->d, lse);
+  const int64_t rb = p.many ? z.rows : 16;
   p.tiles = (max_rows * gs + rb - 1) / rb;
   if (p.tiles < 1) p.tiles = 1;
   if (p.tiles > 65536) p.tiles = 65536;
   p.base = batch * c->nkv * p.tiles;
-  const int64_t fill = p.many ? 256 : pa_fill(c->d, dtype);
+  const int64_t fill = p.many ? z.fill : pa_fill(c->d, dtype);
   int64_t want = (fill + p.base - 1) / p.base;
   // parts of fewer than four steps a wave do not pay for the join
   const int64_t step = p.many ? 512 : 32 * pa_waves(c->d, dtype);
@@ -1178,10 +1346,25 @@ static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int
   if (want > most) want = most;
   if (want > kPaMaxSplit) want = kPaMaxSplit;
   p.nsplit = want < 1 ? 1 : (int)want;
+  p.un_steps = 0;
+  if (p.many && p.tiles >= kPtUnpackTiles) {
+    const int64_t steps = (max_len + z.keys - 1) / z.keys;
+    if (steps > 0 && steps <= INT32_MAX / z.keys && batch * c->nkv * steps <= kPtUnpackMost / z.step) p.un_steps = steps;
+  }
   return p;
 }
-static int64_t pa_bytes(const PaPlan& p, int64_t rows, int nh, int d) {
-  return p.nsplit > 1 ? rows * nh * p.nsplit * (int64_t)(4 * d + 8) : 0;
+// The workspace: parts of rows, their maxima and sums, unpacked positions, their masks.
+struct PaSpace {
+  int64_t ml, un, nan, bytes;
+};
+static PaSpace pa_space(const PaPlan& p, int64_t rows, int64_t batch, int nkv, int nh, int d, bool lse) {
+  const int64_t parts = p.nsplit > 1 ? rows * nh * p.nsplit : 0, steps = batch * nkv * p.un_steps;
+  PaSpace s;
+  s.ml = parts * 4 * d;
+  s.un = (s.ml + parts * 8 + 15) / 16 * 16;
+  s.nan = s.un + steps * pt_size(d, lse).step;
+  s.bytes = s.nan + steps * (d / kKvGroup) * 8;
+  return s;
 }
 
 // Dynamic LDS of more than 64 KB has to be asked for, once a kernel.
@@ -1190,20 +1373,40 @@ static hipError_t allow_lds(K* kernel, int bytes) {
   return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
+template <int D, int KT>
+static int pt_launch(const PaArgs& a, int64_t blocks, hipStream_t st) {
+  constexpr int lds = PtShape<D, KT>::kLds;
+  static std::once_flag once;
+  static hipError_t arc = hipSuccess;
+  std::call_once(once, [] {
+    arc = allow_lds(&paged_tile_kernel<D, KT, false>, PtShape<D, KT>::kLds);
+    if (arc == hipSuccess) arc = allow_lds(&paged_tile_kernel<D, KT, true>, PtShape<D, KT>::kLds);
+  });
+  KH_HIP(arc);
+  const dim3 g((unsigned)blocks), blk(64 * PtShape<D, KT>::NW);
+  if (a.un_steps) {
+    hipLaunchKernelGGL((paged_unpack_kernel<D, KT>),
+                       dim3((unsigned)a.un_steps, (unsigned)a.nkv, (unsigned)(a.batch < 65535 ? a.batch : 65535)), blk,
+                       0, st, a);
+    hipLaunchKernelGGL((paged_tile_kernel<D, KT, true>), g, blk, lds, st, a);
+  } else {
+    hipLaunchKernelGGL((paged_tile_kernel<D, KT, false>), g, blk, lds, st, a);
+  }
+  KH_LAUNCHED();
+  return KH_OK;
+}
+
 template <int D, typename T>
 static int pa_launch(const PaArgs& a, bool many, int64_t blocks, hipStream_t st) {
   static std::once_flag once;
   static hipError_t arc = hipSuccess;
-  std::call_once(once, [] {
-    arc = allow_lds(&paged_rows_kernel<D, T>, PaShape<D, T>::kLds);
-    if constexpr (sizeof(T) == 2) {
-      if (arc == hipSuccess) arc = allow_lds(&paged_tile_kernel<D, kPtWaves>, PtShape<D>::kLds);
-    }
-  });
+  std::call_once(once, [] { arc = allow_lds(&paged_rows_kernel<D, T>, PaShape<D, T>::kLds); });
   KH_HIP(arc);
   if constexpr (sizeof(T) == 2) {
-    if (many)
-      hipLaunchKernelGGL((paged_tile_kernel<D, kPtWaves>), dim3((unsigned)blocks), dim3(64 * kPtWaves), PtShape<D>::kLds, st, a);
+    if (many) {
+      const int rc = a.lse ? pt_launch<D, 2>(a, blocks, st) : pt_launch<D, 1>(a, blocks, st);
+      if (rc != KH_OK) return rc;
+    }
   }
   if (!many)
     hipLaunchKernelGGL((paged_rows_kernel<D, T>),
@@ -1242,12 +1445,15 @@ static int pa_shape(const kh_paged_kv* c, int dtype, int64_t rows, int64_t batch
 using namespace kh;
 
 extern "C" int kh_paged_kv_attention_workspace(const kh_paged_kv* c, int dtype, int64_t rows, int64_t batch,
-                                               int num_heads, int64_t max_rows, int64_t max_len, int64_t* bytes) {
+                                               int num_heads, int64_t max_rows, int64_t max_len, int with_lse,
+                                               int64_t* bytes) {
   KH_CHECK_ARG(bytes != nullptr, "null output");
   const int rc = pa_shape(c, dtype, rows, batch, num_heads, max_rows, max_len);
   if (rc != KH_OK) return rc;
-  *bytes = rows && batch ? pa_bytes(pa_plan(c, dtype, num_heads, rows, batch, max_rows, max_len), rows, num_heads, c->d)
-                         : 0;
+  *bytes = 0;
+  if (rows && batch)
+    *bytes = pa_space(pa_plan(c, dtype, num_heads, rows, batch, max_rows, max_len, with_lse != 0), rows, batch, c->nkv,
+                      num_heads, c->d, with_lse != 0).bytes;
   return KH_OK;
 }
 
@@ -1274,8 +1480,9 @@ extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void
   if (rows == 0 || batch == 0) return KH_OK;
   KH_CHECK_ARG(q_dev && off_dev && len_dev && table_dev && out_dev, "null argument");
   KH_CHECK_ARG(heads_dev || n_heads == 0, "null head list");
-  const PaPlan p = pa_plan(c, dtype, num_heads, rows, batch, max_rows, max_len);
-  const int64_t need = pa_bytes(p, rows, num_heads, c->d);
+  const PaPlan p = pa_plan(c, dtype, num_heads, rows, batch, max_rows, max_len, lse_dev != nullptr);
+  const PaSpace sp = pa_space(p, rows, batch, c->nkv, num_heads, c->d, lse_dev != nullptr);
+  const int64_t need = sp.bytes;
   if (need > 0 && (!ws_dev || ws_bytes < need)) {
     set_error("the workspace holds %lld bytes, %lld are needed", (long long)(ws_dev ? ws_bytes : 0),
               (long long)need);
@@ -1315,8 +1522,12 @@ extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void
   a.lse = lse_dev;
   a.nsplit = p.nsplit;
   a.tiles = (int)p.tiles;
-  a.part_o = static_cast<float*>(ws_dev);
-  a.part_ml = need ? reinterpret_cast<float2*>(a.part_o + rows * num_heads * p.nsplit * c->d) : nullptr;
+  char* ws = static_cast<char*>(ws_dev);
+  a.part_o = reinterpret_cast<float*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + sp.ml);
+  a.un = ws + sp.un;
+  a.un_nan = reinterpret_cast<uint32_t*>(ws + sp.nan);
+  a.un_steps = (int)p.un_steps;
   a.qvec = aligned16(q_dev, dtype, q_row_stride, q_head_stride) ? 1 : 0;
   a.ovec = aligned16(out_dev, dtype, out_row_stride, out_head_stride) ? 1 : 0;
   return dtype == KH_DT_F32 ? pa_launch_d<float>(c->d, a, p.many, blocks, as_stream(stream))

@@ -279,7 +279,7 @@ class PagedKv(_Handle):
             max_len = cols * self.page_size
         if scale is None:
             scale = dim ** -0.5
-        need = self._workspace(dt, n, batch, nh, max_rows, max_len)
+        need = self._workspace(dt, n, batch, nh, max_rows, max_len, 1 if return_lse else 0)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
             yp, y0, y1 = out.data_ptr(), nh * dim, dim

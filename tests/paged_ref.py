@@ -55,7 +55,8 @@ def attention(q, kraw, vraw, scale, causal=True, window=0, bf16=True, many=False
     additions; an exponential is off by 2^-21 and by 2^-22 of its argument; a weight that the second product
     takes is rounded to 8 bits (2^-8; f32 rows: three times 8, 2^-24) of p s c + p |m|; its sums over the positions have
     magnitudes sum p (271 s + |m|) and at most length / 4 + 64 additions in a row; out is rounded last.  Tiles of
-    many BF16 rows (`many`) take keys and values rounded to 8 bits: 2^-8 of |q| |k| and of p |v| more."""
+    many BF16 rows (`many`) take keys and values rounded to 8 bits: 2^-8 of |q| |k| and of p |v| more, and divide by
+    the sum of the rounded weights: 2^-8 of |o| <= sum p |v| once more."""
     n, heads, dim = q.shape
     length, kv = kraw.shape[:2]
     kc, ks, km = quantize(kraw)
@@ -87,7 +88,7 @@ def attention(q, kraw, vraw, scale, causal=True, window=0, bf16=True, many=False
             sg = np.nan_to_num(vs[:, g])  # groups that stand for NaN have no tolerance
             mag = sg * vc[:, g] + np.abs(vm[:, g])
             if many:
-                mag = mag + np.abs(np.nan_to_num(v[:, g]))
+                mag = mag + 2 * np.abs(np.nan_to_num(v[:, g]))
             tol[:, h] = ((w * err) @ np.abs(np.nan_to_num(v[:, g])) + (w * err).sum(-1)[:, None] * np.abs(o)
                          + up * (w @ mag) + depth * (w @ (271 * sg + np.abs(vm[:, g]))) + uo * np.abs(o))
         out[:, h] = np.where(some[:, None], o, 0.0)

@@ -36,7 +36,7 @@ class Case:
         return self.cache.attention(self.q.cuda(), self.off, self.len, self.table, **kw)
 
     def check(self, got, causal=True, window=0, scale=None, on=None):
-        out, lse = (x.double().cpu().numpy() for x in got)
+        out, lse = (None if x is None else x.double().cpu().numpy() for x in ((got, None) if torch.is_tensor(got) else got))
         at, worst = 0, 0.0
         for n, length, k, v in zip(self.rows, self.lens, self.k, self.v):
             if n == 0:
@@ -45,7 +45,7 @@ class Case:
             first = max(0, n - length)  # rows before the cache's first position see nothing
             keep = slice(at + first, at + n)
             assert causal or not first
-            assert (out[at:at + first] == 0).all() and (lse[at:at + first] == -np.inf).all()
+            assert (out[at:at + first] == 0).all() and (lse is None or (lse[at:at + first] == -np.inf).all())
             if length:
                 o, l, to, tl = attention(q[first:], k.float().numpy(), v.float().numpy(),
                                          self.dim ** -0.5 if scale is None else scale, causal, window, self.dtype == BF16, self.many)
@@ -58,6 +58,9 @@ class Case:
                 assert (d[fine] <= to[fine]).all(), float(np.nanmax(np.where(fine, d - to, 0)))
                 worst = max(worst, float(np.max(np.where(fine & (to > 0), d / np.where(to > 0, to, 1), 0), initial=0)))
                 some = np.isfinite(l)
+                if lse is None:
+                    at += n
+                    continue
                 assert (lse[keep][~some & ~np.isnan(l)] == -np.inf).all()
                 assert (np.abs(lse[keep][some] - l[some]) <= tl[some]).all()
             at += n
@@ -87,6 +90,7 @@ def test_many_rows(kh, dtype, heads, kv, dim, page, causal, window):
     rows, lens = [70, 0, 1, 33, 5], [70, 40, 90, 133, 200]
     c = Case(dtype, heads, kv, dim, page, rows, lens)
     c.check(c.run(causal=causal, window=window), causal, window)
+    c.check(c.run(causal=causal, window=window, return_lse=False), causal, window)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -210,13 +214,16 @@ def test_strides(kh, dtype, shift):
         got = c.cache.attention(buf[:, 2:10], c.off, c.len, c.table, out=out, return_lse=True)
         assert got[0] is out and torch.equal(out, want[0]) and torch.equal(got[1], want[1])
         assert (flat[:, n] == 4).all()
+        # without the log-sum-exp tiles of many rows hold their keys in one BF16 term
+        alone = c.cache.attention(c.q.cuda(), c.off, c.len, c.table)
+        c.check(alone)
         wide = torch.full((n, 12, 128), 4.0, dtype=dtype, device="cuda")
         c.cache.attention(c.q.cuda(), c.off, c.len, c.table, out=wide[:, :8])
-        assert torch.equal(wide[:, :8], want[0]) and (wide[:, 8:] == 4).all()
+        assert torch.equal(wide[:, :8], alone) and (wide[:, 8:] == 4).all()
         # a table's columns inside a wider one
         big = torch.full((len(rows), c.table.shape[1] + 3), -9, dtype=torch.int32, device="cuda")
         big[:, 2:-1] = c.table
-        assert torch.equal(c.cache.attention(c.q.cuda(), c.off, c.len, big[:, 2:-1]), want[0])
+        assert torch.equal(c.cache.attention(c.q.cuda(), c.off, c.len, big[:, 2:-1]), alone)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -379,3 +386,82 @@ def test_two_graphs_of_one_stream(kh):
                 g.replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+# Row tiles enough that the positions are unpacked ahead of them (BF16)
+AHEAD = [(32, 2, 64, [60, 40], [60, 300]), (64, 4, 128, [40, 0, 70], [40, 9, 450]), (32, 2, 256, [50, 33], [180, 33])]
+
+
+@pytest.mark.parametrize("heads,kv,dim,rows,lens", AHEAD)
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 70), (False, 0)])
+def test_unpacked_ahead(kh, heads, kv, dim, rows, lens, page, causal, window):
+    c = Case(BF16, heads, kv, dim, page, rows, lens)
+    for lse in (True, False):
+        c.check(c.run(causal=causal, window=window, max_rows=max(rows), max_len=max(lens), return_lse=lse), causal, window)
+    # a sequence longer than the caller says, and lengths far shorter
+    for most in (max(lens) - 64, 64, 10 ** 5):
+        for lse in (True, False):
+            c.check(c.run(causal=causal, window=window, max_rows=max(rows), max_len=most, return_lse=lse), causal, window)
+
+
+@pytest.mark.parametrize("heads,kv,dim,rows,lens", AHEAD)
+def test_unpacked_ahead_values_that_are_not_finite(kh, heads, kv, dim, rows, lens):
+    c = Case(BF16, heads, kv, dim, 16, rows, lens)
+    for b, n in enumerate(lens):
+        if n > 20:
+            c.v[b][n - 3, kv - 1, dim - 1] = float("nan")  # the last rows see it, and one group of them turns
+            c.v[b][n - rows[b] // 2, 0, 33] = float("inf")
+            c.k[b][n - rows[b] // 3, kv // 2, 5] = float("nan")
+    c.cache.append(torch.cat(c.k).cuda(), torch.cat(c.v).cuda(), offsets(lens).cuda(),
+                   torch.zeros(len(lens), dtype=torch.int64).cuda(), c.table)
+    for lse in (True, False):
+        c.check(c.run(max_rows=max(rows), max_len=max(lens), return_lse=lse))
+        c.check(c.run(max_rows=max(rows), max_len=max(lens), window=30, return_lse=lse), window=30)
+
+
+@pytest.mark.parametrize("heads,kv,dim,rows,lens", AHEAD)
+def test_unpacked_ahead_pages_and_heads(kh, heads, kv, dim, rows, lens):
+    """A page that is not there leaves the rest; freed pages before a window are not looked at; listed heads alone."""
+    from klearu_amd import KlearuError
+    c = Case(BF16, heads, kv, dim, 16, rows, lens)
+    c.many = True
+    q, most = c.q.cuda(), dict(max_rows=max(rows), max_len=max(lens))
+    last = len(lens) - 1
+    bad = c.table.clone()
+    bad[last, 0] = -7
+    got = c.cache.attention(q, c.off, c.len, bad, **most)
+    with pytest.raises(KlearuError, match="page id"):
+        c.cache.status()
+    at, n, length = sum(rows[:last]), rows[last], lens[last]
+    late = [i for i in range(n) if length - n + i >= 16]
+    qs = c.q[[at + i for i in late]].double().numpy()
+    for i, row in list(zip(late, qs))[:: max(1, len(late) // 5)]:
+        k, v = (x[last][16:length - n + i + 1].float().numpy() for x in (c.k, c.v))
+        o, _, to, _ = attention(row[None], k, v, dim ** -0.5, many=True)
+        assert (np.abs(got[at + i].double().cpu().numpy() - o[0]) <= to[0]).all()
+    if length - n - 20 >= 16:
+        c.check(c.cache.attention(q, c.off, c.len, bad, window=20, return_lse=True, **most), window=20)
+    rng = np.random.default_rng(2)
+    sel = np.stack([rng.permutation(heads)[:5] for _ in range(sum(rows))]).astype(np.int32)
+    on = np.zeros((sum(rows), heads), bool)
+    np.put_along_axis(on, sel.astype(np.int64), True, 1)
+    c.check(c.run(heads=torch.from_numpy(sel).cuda(), **most), on=on)
+
+
+def test_unpacked_ahead_in_a_graph(kh):
+    """A prompt's attention captured and replayed, eager calls between: no workspace is shared."""
+    c = Case(BF16, 32, 2, 128, 64, [70, 30], [70, 200])
+    q, out = c.q.cuda(), torch.zeros_like(c.q, device="cuda")
+    kw = dict(max_rows=70, max_len=200)
+    want = c.cache.attention(q, c.off, c.len, c.table, **kw)
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        c.cache.attention(q, c.off, c.len, c.table, out=out, **kw)
+    for _ in range(4):
+        out.zero_()
+        g.replay()
+        other = c.cache.attention(q * 0.5, c.off, c.len, c.table, **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and not torch.equal(other, want)

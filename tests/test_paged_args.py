@@ -114,8 +114,8 @@ def test_attention():
         refused("kh_paged_kv_attention", change(base, **kw), ARG, text)
     need = C.c_int64()
     call = _lib.load().kh_paged_kv_attention_workspace
-    assert call(cache(), 0, 3, 3, 4, 1, 64, C.byref(need)) == 0 and need.value == 0
-    assert call(cache(), 0, 3, 3, 4, 1, 100000, C.byref(need)) == 0 and need.value > 0
+    assert call(cache(), 0, 3, 3, 4, 1, 64, 0, C.byref(need)) == 0 and need.value == 0
+    assert call(cache(), 0, 3, 3, 4, 1, 100000, 0, C.byref(need)) == 0 and need.value > 0
     refused("kh_paged_kv_attention", change(base, max_len=100000, ws=P, wsb=need.value - 1), CAP, "workspace")
     refused("kh_paged_kv_attention", change(base, max_len=100000), CAP, "workspace")
     refused("kh_paged_kv_attention", change(base, max_len=100000, ws=P + 4, wsb=need.value), ARG, "aligned")
