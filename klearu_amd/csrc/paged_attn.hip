@@ -68,6 +68,7 @@ struct PaArgs {
   float* part_o;
   float2* part_ml;
   int nsplit, tiles;
+  int share;  // 0, or the parts that a kv head's sequences get by their lengths, up to nsplit each
   int qvec, ovec;
   char* un;  // unpacked positions (tiles of many rows): un_steps steps of each sequence
   uint32_t* un_nan;
@@ -258,6 +259,32 @@ __device__ __forceinline__ void pa_store4(T* y, bool vec, float a, float b, floa
   store_f32(y + 3, d);
 }
 
+// Which part of which sequence block blockIdx.x of a kv head takes where the parts are
+// dealt out by length: a sequence gets one for every `per` steps of 32 positions, such
+// that all of them are about `share`.  The sequence, or -1 for a block without one.
+__device__ __forceinline__ int pa_share(const PaArgs& a, int lane, int waves, int* split, int* parts) {
+  const int64_t cap = a.cols << a.ps_log2;
+  uint32_t steps = 0, mine = 0;
+  if (lane < a.batch) {
+    const int64_t o0 = max(a.off[lane], (int64_t)0), o1 = min(a.off[lane + 1], a.rows), n = o1 - o0;
+    const int64_t L = min(max(a.len[lane], (int64_t)0), cap);
+    const int64_t from = a.window > 0 && L - n - a.window + 1 > 0 ? L - n - a.window + 1 : 0;
+    if (n > 0) mine = 1, steps = (uint32_t)((L + kPaStep - 1) / kPaStep - from / kPaStep);
+  }
+  // halves of steps: 64 lanes' sum stays below 2^31
+  const uint32_t all = __builtin_amdgcn_readlane(wave_incl_scan((int)((steps + 1) >> 1)), 63);
+  uint32_t per = all / (uint32_t)a.share * 2 + 2;
+  per = (per + waves - 1) / waves * waves;
+  mine = mine ? min(max((steps + per - 1) / per, 1u), (uint32_t)a.nsplit) : 0u;
+  const uint32_t upto = (uint32_t)wave_incl_scan((int)mine);
+  const uint64_t past = __ballot(upto > blockIdx.x);
+  if (!past) return -1;
+  const int b = __builtin_ctzll(past);
+  *parts = (int)__builtin_amdgcn_readlane(mine, b);
+  *split = (int)(blockIdx.x - (__builtin_amdgcn_readlane(upto, b) - *parts));
+  return b;
+}
+
 // Block: one row tile of one (sequence, kv head), one of nsplit parts of the
 // positions that the tile sees; its waves take every NW-th step of 32.
 template <int D, typename T>
@@ -272,11 +299,18 @@ __global__ __launch_bounds__((64 * PaShape<D, T>::NW), (PaShape<D, T>::kPerSimd)
   float* s_l = s_m + NW * 16;
   const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int split = blockIdx.x, h = blockIdx.y;
+  const int h = blockIdx.y;
   const int ps = 1 << a.ps_log2;
   const int64_t cap = a.cols << a.ps_log2;
   const PaLane<D> lo_(lane, ps);
-  for (int64_t bt = blockIdx.z; bt < a.batch * a.tiles; bt += gridDim.z) {
+  int split = blockIdx.x, parts = a.nsplit;
+  int64_t z0 = blockIdx.z;
+  if (a.share) {
+    const int s = pa_share(a, lane, NW, &split, &parts);
+    if (s < 0) return;
+    z0 = s;
+  }
+  for (int64_t bt = z0; bt < a.batch * a.tiles; bt += a.share ? a.batch : gridDim.z) {
   const int64_t b = a.tiles == 1 ? bt : bt / a.tiles;
   const int tile0 = a.tiles == 1 ? 0 : (int)(bt - b * a.tiles);
   // the first of the chain's loads together: rows, length, the first 64 pages
@@ -332,7 +366,7 @@ __global__ __launch_bounds__((64 * PaShape<D, T>::NW), (PaShape<D, T>::kPerSimd)
     for (int j = 0; j < NG; ++j) os[j] = 0.0f;
 
     const int first = tlo / kPaStep, steps = thi > tlo ? (thi + kPaStep - 1) / kPaStep - first : 0;
-    const int per = (steps + a.nsplit - 1) / a.nsplit;
+    const int per = (steps + parts - 1) / parts;
     const int sb = first + split * per, se = min(first + steps, sb + per);
     if (sb < se) {
       // The wave's steps sb + wave, + NW, ...: lane k holds the pages of the k-th of
@@ -583,7 +617,10 @@ __global__ __launch_bounds__((64 * PaShape<D, T>::NW), (PaShape<D, T>::kPerSimd)
       const bool any = M != -INFINITY || tot != 0.0f;
       if (a.nsplit > 1) {
         const int64_t at = row * a.nsplit + split;
-        if (d == 0) a.part_ml[at] = make_float2(M, tot);
+        if (d == 0) {
+          a.part_ml[at] = make_float2(M, tot);
+          for (int s = split + parts; s < a.nsplit; s += parts) a.part_ml[row * a.nsplit + s] = make_float2(-INFINITY, 0.0f);
+        }
         if (any) *reinterpret_cast<float4*>(a.part_o + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
         const float inv = any ? 1.0f / tot : 0.0f;
@@ -1323,7 +1360,7 @@ static PtSize pt_size(int d, bool lse) {
 struct PaPlan {
   bool many;  // paged_tile_kernel
   int64_t tiles, base;
-  int nsplit;
+  int nsplit, share;
   int64_t un_steps;  // steps of each sequence that are unpacked ahead, or 0
 };
 static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int64_t batch, int64_t max_rows,
@@ -1346,6 +1383,15 @@ static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int
   if (want > most) want = most;
   if (want > kPaMaxSplit) want = kPaMaxSplit;
   p.nsplit = want < 1 ? 1 : (int)want;
+  p.share = 0;
+  // Single rows of several sequences: parts by length, which every block works out from
+  // the lengths for itself (64 sequences of 1 to 4096 positions: 25 us with three parts
+  // for each, 21 with eight at most; lengths that are all alike cost it 1 us).
+  if (!p.many && p.nsplit > 1 && p.tiles == 1 && batch > 1 && batch <= 64) {
+    p.share = (int)(fill / c->nkv - batch / 2);
+    p.nsplit = 2 * p.nsplit + 2;
+    if (p.nsplit > most) p.nsplit = (int)most;
+  }
   p.un_steps = 0;
   if (p.many && p.tiles >= kPtUnpackTiles) {
     const int64_t steps = (max_len + z.keys - 1) / z.keys;
@@ -1410,7 +1456,8 @@ static int pa_launch(const PaArgs& a, bool many, int64_t blocks, hipStream_t st)
   }
   if (!many)
     hipLaunchKernelGGL((paged_rows_kernel<D, T>),
-                       dim3((unsigned)a.nsplit, (unsigned)a.nkv, (unsigned)(a.batch * a.tiles < 65535 ? a.batch * a.tiles : 65535)),
+                       dim3((unsigned)(a.share ? a.share + a.batch : a.nsplit), (unsigned)a.nkv,
+                            (unsigned)(a.share ? 1 : a.batch * a.tiles < 65535 ? a.batch * a.tiles : 65535)),
                        dim3((64 * PaShape<D, T>::NW)), (PaShape<D, T>::kLds), st, a);
   if (a.nsplit > 16)
     hipLaunchKernelGGL((paged_join_kernel<D, T, 4>), dim3((unsigned)(a.rows * a.nh)), dim3(256), 0, st, a);
@@ -1468,7 +1515,7 @@ extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void
   if (rc != KH_OK) return rc;
   KH_CHECK_ARG(table_cols >= 1 && table_stride >= table_cols, "page table of %lld columns, %lld apart",
                (long long)table_cols, (long long)table_stride);
-  KH_CHECK_ARG((table_cols << c->ps_log2) <= INT32_MAX - 64, "a page table of %lld columns holds 2^31 positions",
+  KH_CHECK_ARG(table_cols <= (INT32_MAX - 64) >> c->ps_log2, "a page table of %lld columns holds 2^31 positions",
                (long long)table_cols);
   KH_CHECK_ARG(std::isfinite(scale) && scale > 0, "scale must be positive and finite");
   KH_CHECK_ARG(window >= 0 && (window == 0 || causal), "a window (%lld) needs causal attention", (long long)window);
@@ -1521,6 +1568,7 @@ extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void
   a.oh = out_head_stride;
   a.lse = lse_dev;
   a.nsplit = p.nsplit;
+  a.share = p.share;
   a.tiles = (int)p.tiles;
   char* ws = static_cast<char*>(ws_dev);
   a.part_o = reinterpret_cast<float*>(ws);

@@ -465,3 +465,22 @@ def test_unpacked_ahead_in_a_graph(kh):
         other = c.cache.attention(q * 0.5, c.off, c.len, c.table, **kw)
         torch.cuda.synchronize()
         assert torch.equal(out, want) and not torch.equal(other, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("heads,kv,dim,lens", [
+    (8, 2, 64, [4000, 1, 700, 0, 33, 1300, 64, 2600]), (4, 1, 128, [3000, 3000]), (2, 2, 256, [1, 5000, 0, 1]),
+    (4, 4, 64, [1 + 61 * i for i in range(40)])])
+@pytest.mark.parametrize("window", [0, 500])
+def test_ragged_lengths_share_the_parts(kh, dtype, heads, kv, dim, lens, window):
+    """Single rows whose parts are dealt out by length, one sequence without a row, two rows in another; a guess of
+    the longest that is far too large."""
+    rows = [1] * len(lens)
+    rows[-1] = 2 if lens[-1] >= 2 else 1
+    rows[len(lens) // 2] = 0 if len(lens) > 2 else 1
+    c = Case(dtype, heads, kv, dim, 32, rows, lens)
+    for most in (max(lens), 10 ** 6):
+        got = c.run(window=window, max_rows=1, max_len=most)
+        c.check(got, window=window)
+        again = c.run(window=window, max_rows=1, max_len=most)
+        assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
