@@ -30,11 +30,15 @@ _DT = {torch.float32: 0, torch.bfloat16: 2}
 _I64, _I32 = torch.int64, torch.int32
 
 
-def _rows(t: torch.Tensor, what: str, device, dtype=None):
+def _elsewhere(t: torch.Tensor, what: str, device: int):
+    raise ValueError(f"{what} is on {t.device}, the handle on cuda:{device}")
+
+
+def _rows(t: torch.Tensor, what: str, device: int, dtype=None):
     """(pointer, row stride, head stride, dtype code) of a tensor [rows, heads, head_dim]."""
     dt = t.dtype
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, the handle on {device}")
+    if t.get_device() != device:
+        _elsewhere(t, what, device)
     if t.dim() != 3:
         raise ValueError(f"{what}: expected [rows, heads, head_dim], got {tuple(t.shape)}")
     code = _DT.get(dt)
@@ -46,10 +50,10 @@ def _rows(t: torch.Tensor, what: str, device, dtype=None):
     return t.data_ptr(), s0, s1, code
 
 
-def _index(t: torch.Tensor, what: str, device, dtype, shape):
-    """Pointer of a contiguous index tensor of a given dtype and shape."""
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, the handle on {device}")
+def _index(t: torch.Tensor, what: str, device: int, dtype, shape):
+    """Pointer of a contiguous tensor of a given dtype and shape."""
+    if t.get_device() != device:
+        _elsewhere(t, what, device)
     if t.dtype is not dtype:
         raise TypeError(f"{what}: dtype {t.dtype}, expected {dtype}")
     if t.shape != shape:
@@ -59,15 +63,16 @@ def _index(t: torch.Tensor, what: str, device, dtype, shape):
     return t.data_ptr()
 
 
-def _table(t: torch.Tensor, device, batch):
+def _table(t: torch.Tensor, device: int, batch):
     """(pointer, columns, row stride) of an int32 page table [batch, columns]."""
-    if t.device != device:
-        raise ValueError(f"table is on {t.device}, the handle on {device}")
+    if t.get_device() != device:
+        _elsewhere(t, "table", device)
     if t.dtype is not _I32:
         raise TypeError(f"table: dtype {t.dtype}, expected torch.int32")
-    if t.dim() != 2 or t.shape[0] != batch:
-        raise ValueError(f"table: shape {tuple(t.shape)}, expected [{batch}, columns]")
-    cols = t.shape[1]
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != batch:
+        raise ValueError(f"table: shape {tuple(shape)}, expected [{batch}, columns]")
+    cols = shape[1]
     s0, s1 = t.stride()
     if cols > 1 and s1 != 1:
         raise ValueError("table: the columns of a row must be contiguous")
@@ -159,12 +164,12 @@ class Rope(_Handle):
         place) or a new tensor.  `transpose` takes gradients back: the transposed rotation.  Rows of
         a negative position are padding and left as they were, as are (reported by status()) rows
         past max_pos; in a new tensor those hold no value."""
-        dev = self.device
+        dev = self._dev
         xp, x0, x1, dt = _rows(x, "x", dev)
         n, heads, dim = x.shape
         pp = _index(pos, "pos", dev, _I64, (n,))
-        if stream is not None or _raw_device() != self._dev:
-            with _On(dev, stream, (x, pos, out)):
+        if stream is not None or _raw_device() != dev:
+            with _On(self.device, stream, (x, pos, out)):
                 return self.apply(x, pos, out, transpose)
         if out is None:
             out = torch.empty_like(x, memory_format=torch.contiguous_format)
@@ -174,7 +179,7 @@ class Rope(_Handle):
         else:
             yp, y0, y1, _ = _rows(out, "out", dev, x.dtype)
         _check(self._lib.kh_rope_apply(self._h, dt, xp, x0, x1, n, heads, dim, pp, yp, y0, y1, 1 if transpose else 0,
-                                       _raw_stream(self._dev)))
+                                       _raw_stream(dev)))
         return out
 
     def status(self):
@@ -201,7 +206,7 @@ class PagedKv(_Handle):
 
     def _places(self, off, start, table):
         """What every call over rows of sequences checks: (batch, off, start, table, columns, stride)."""
-        dev, batch = self.device, start.shape[0]
+        dev, batch = self._dev, start.shape[0]
         return (batch, _index(off, "off", dev, _I64, (batch + 1,)), _index(start, "start", dev, _I64, (batch,)),
                 *_table(table, dev, batch))
 
@@ -210,7 +215,7 @@ class PagedKv(_Handle):
         """Row off[b] + i of k and v [rows, num_kv_heads, head_dim] becomes position start[b] + i of
         sequence b; `rope` rotates the keys on the way, by pos [rows] or by their places in the
         cache.  Two rows of one call must not have the same place."""
-        dev = self.device
+        dev = self._dev
         kp, k0, k1, dt = _rows(k, "k", dev)
         vp, v0, v1, _ = _rows(v, "v", dev, k.dtype)
         n = k.shape[0]
@@ -221,31 +226,37 @@ class PagedKv(_Handle):
         if pos is not None and rope is None:
             raise ValueError("pos: rotary positions without a rotation")
         pp = None if pos is None else _index(pos, "pos", dev, _I64, (n,))
-        if stream is not None or _raw_device() != self._dev:
-            with _On(dev, stream, (k, v, off, start, table, pos)):
+        if stream is not None or _raw_device() != dev:
+            with _On(self.device, stream, (k, v, off, start, table, pos)):
                 return self.append(k, v, off, start, table, rope, pos)
         _check(self._lib.kh_paged_kv_append(self._h, None if rope is None else rope._h, dt, kp, k0, k1, vp, v0, v1, n, op,
-                                            batch, sp, pp, tp, cols, ts, _raw_stream(self._dev)))
+                                            batch, sp, pp, tp, cols, ts, _raw_stream(dev)))
 
     def gather(self, off: torch.Tensor, start: torch.Tensor, table: torch.Tensor, rows: int,
                dtype: torch.dtype = torch.float32, k: torch.Tensor | None = None, v: torch.Tensor | None = None,
                stream=None):
         """The values that those places hold: (k, v) [rows, num_kv_heads, head_dim], new or given.
         Rows outside all sequences, or without a place, are left as they were."""
-        dev = self.device
+        dev = self._dev
         batch, op, sp, tp, cols, ts = self._places(off, start, table)
         dt = _DT.get(dtype)
         if dt is None:
             raise TypeError(f"dtype {dtype}: expected float32 or bfloat16")
-        if stream is not None or _raw_device() != self._dev:
-            with _On(dev, stream, (off, start, table, k, v)):
+        if stream is not None or _raw_device() != dev:
+            with _On(self.device, stream, (off, start, table, k, v)):
                 return self.gather(off, start, table, rows, dtype, k, v)
         shape = (rows, self.num_kv_heads, self.head_dim)
-        k = torch.empty(shape, dtype=dtype, device=dev) if k is None else k
-        v = torch.empty(shape, dtype=dtype, device=dev) if v is None else v
-        _check(self._lib.kh_paged_kv_gather(self._h, dt, rows, op, batch, sp, tp, cols, ts,
-                                            _index(k, "k", dev, dtype, shape), _index(v, "v", dev, dtype, shape),
-                                            _raw_stream(self._dev)))
+        if k is None:
+            k = torch.empty(shape, dtype=dtype, device=self.device)
+            kp = k.data_ptr()
+        else:
+            kp = _index(k, "k", dev, dtype, shape)
+        if v is None:
+            v = torch.empty(shape, dtype=dtype, device=self.device)
+            vp = v.data_ptr()
+        else:
+            vp = _index(v, "v", dev, dtype, shape)
+        _check(self._lib.kh_paged_kv_gather(self._h, dt, rows, op, batch, sp, tp, cols, ts, kp, vp, _raw_stream(dev)))
         return k, v
 
     def attention(self, q: torch.Tensor, off: torch.Tensor, lens: torch.Tensor, table: torch.Tensor,
@@ -259,7 +270,7 @@ class PagedKv(_Handle):
         sequence (default: an even share of the rows, the table's reach); wrong guesses cost
         time only.  Returns out, or (out, lse) with lse [rows, num_heads] f32: a row that sees nothing
         gives 0 and -inf."""
-        dev = self.device
+        dev = self._dev
         qp, q0, q1, dt = _rows(q, "q", dev)
         n, nh, dim = q.shape
         if dim != self.head_dim:
@@ -269,8 +280,8 @@ class PagedKv(_Handle):
         if heads is not None:
             nsel = heads.shape[-1]
             hp = _index(heads, "heads", dev, _I32, (n, nsel)) or op  # an empty list is no list of all
-        if stream is not None or _raw_device() != self._dev:
-            with _On(dev, stream, (q, off, lens, table, heads, out)):
+        if stream is not None or _raw_device() != dev:
+            with _On(self.device, stream, (q, off, lens, table, heads, out)):
                 return self.attention(q, off, lens, table, scale, causal, window, heads, max_rows, max_len, out,
                                       return_lse)
         if max_rows is None:
@@ -287,12 +298,12 @@ class PagedKv(_Handle):
             raise ValueError(f"out: shape {tuple(out.shape)}, expected {tuple(q.shape)}")
         else:
             yp, y0, y1, _ = _rows(out, "out", dev, q.dtype)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        lse = torch.empty((n, nh), dtype=torch.float32, device=dev) if return_lse else None
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        lse = torch.empty((n, nh), dtype=torch.float32, device=self.device) if return_lse else None
         _check(self._lib.kh_paged_kv_attention(
             self._h, dt, qp, q0, q1, nh, n, op, batch, lp, tp, cols, ts, max_rows, max_len, scale, 1 if causal else 0,
             window, hp, nsel, yp, y0, y1, None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(),
-            need, _raw_stream(self._dev)))
+            need, _raw_stream(dev)))
         return (out, lse) if return_lse else out
 
     def _workspace(self, *sizes) -> int:
