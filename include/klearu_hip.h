@@ -787,8 +787,8 @@ int kh_paged_kv_attention_workspace(const kh_paged_kv* c, int dtype, int64_t row
  * length of a sequence; a wrong one costs time, not correctness.  Sums and
  * softmax statistics are f32; BF16 rows have their weights p rounded to BF16.
  * BF16 calls of many rows (max_rows times the query heads of a kv head of 64 or
- * more) take keys and values rounded to BF16 as well; with lse_dev their keys are
- * held to 2^-16 instead, so that out may differ from a call without it in the
+ * more) may take keys and values rounded to BF16 as well; with lse_dev their keys
+ * are held to 2^-16 instead, so that out may differ from a call without it in the
  * rounding.  The result does not depend on the run.  ws_dev: 16-byte aligned,
  * kh_paged_kv_attention_workspace bytes (fewer are KH_ERR_CAPACITY), not shared
  * by calls that may run at once; its contents do not matter. */

@@ -1329,8 +1329,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaArgs a) {
 
 // How a call is cut: row tiles per (sequence, kv head) as the caller expects
 // them, and parts along the positions when the tiles alone do not fill the chip.
+//
+// Tiles of many rows pay where the tiles of 16 rows do not fit on the chip at once, or
+// have far to go: below, each goes over its positions from the start (12 against 30 us for
+// 64 rows of 32 heads of 128 over 564 positions, 25 against 33 for 128 over 2176, 38
+// against 50 for 256 over 2304, where the 16-row tiles need two rounds; 46 against 36 for
+// 64 over 8064).  Sizes are in rows times positions.
 constexpr int kPtMinRows = 64;
-constexpr int kPtUnpackTiles = 3;                    // row tiles from which on positions are unpacked ahead of them
+constexpr int64_t kPtMinWork = 3000;  // positions of a full chip of 16-row tiles
+// Positions are unpacked ahead where three row tiles or more see them and there are
+// enough: it takes 10 us (8 sequences of 256 rows: 42 against 37 us over 556 positions,
+// 101 against 110 over 2304).
+constexpr int kPtUnpackTiles = 3;
+constexpr int64_t kPtUnpackWork = 1 << 18;           // row tiles times positions
 constexpr int64_t kPtUnpackMost = (int64_t)1 << 30;  // bytes of them
 template <typename T>
 static int pa_fill_t(int d) {
@@ -1368,7 +1379,9 @@ static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int
   PaPlan p;
   const int64_t gs = nh / c->nkv;
   if (max_rows > rows) max_rows = rows;
-  p.many = dtype == KH_DT_BF16 && max_rows * gs >= kPtMinRows;
+  const int64_t tiles16 = batch * c->nkv * ((max_rows * gs + 15) / 16), held = pa_fill(c->d, dtype);
+  p.many = dtype == KH_DT_BF16 && max_rows * gs >= kPtMinRows &&
+           (tiles16 > held || (max_len > 0 && tiles16 > kPtMinWork * held / max_len));
   const PtSize z = pt_size(c->d, lse);
   const int64_t rb = p.many ? z.rows : 16;
   p.tiles = (max_rows * gs + rb - 1) / rb;
@@ -1376,7 +1389,7 @@ static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int
   if (p.tiles > 65536) p.tiles = 65536;
   p.base = batch * c->nkv * p.tiles;
   const int64_t fill = p.many ? z.fill : pa_fill(c->d, dtype);
-  int64_t want = (fill + p.base - 1) / p.base;
+  int64_t want = fill / p.base;  // one round of blocks: a second would begin with its own latency
   // parts of fewer than four steps a wave do not pay for the join
   const int64_t step = p.many ? 512 : 32 * pa_waves(c->d, dtype);
   const int64_t most = max_len < 4 * step ? 1 : (max_len + step - 1) / step;
@@ -1386,14 +1399,14 @@ static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int
   p.share = 0;
   // Single rows of several sequences: parts by length, which every block works out from
   // the lengths for itself (64 sequences of 1 to 4096 positions: 25 us with three parts
-  // for each, 21 with eight at most; lengths that are all alike cost it 1 us).
+  // for each, 21 with eight at most; where all have 4096, 33 and 34).
   if (!p.many && p.nsplit > 1 && p.tiles == 1 && batch > 1 && batch <= 64) {
     p.share = (int)(fill / c->nkv - batch / 2);
     p.nsplit = 2 * p.nsplit + 2;
     if (p.nsplit > most) p.nsplit = (int)most;
   }
   p.un_steps = 0;
-  if (p.many && p.tiles >= kPtUnpackTiles) {
+  if (p.many && p.tiles >= kPtUnpackTiles && max_len >= kPtUnpackWork / p.base) {
     const int64_t steps = (max_len + z.keys - 1) / z.keys;
     if (steps > 0 && steps <= INT32_MAX / z.keys && batch * c->nkv * steps <= kPtUnpackMost / z.step) p.un_steps = steps;
   }

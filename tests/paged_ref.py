@@ -79,7 +79,8 @@ def attention(q, kraw, vraw, scale, causal=True, window=0, bf16=True, many=False
             p = np.where(ok, p, 0.0)
             tot = p.sum(-1)
             w = p / np.where(some, tot, 1.0)[:, None]
-            o = np.where(ok[:, :, None], w[:, :, None] * v[None, :, g], 0.0).sum(1)
+            o = w @ np.nan_to_num(v[:, g])
+            o[(ok.astype(np.float64) @ np.isnan(v[:, g])) > 0] = np.nan
             err = (dim + 16) * u * big + 2.0 ** -21 + 2.0 ** -22 * np.abs(np.where(ok, t - top[:, None], 0.0))
             if many:
                 err = err + 2.0 ** -8 * scale * (np.abs(q[:, h]) @ np.abs(np.nan_to_num(k[:, g])).T)

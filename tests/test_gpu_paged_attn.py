@@ -484,3 +484,60 @@ def test_ragged_lengths_share_the_parts(kh, dtype, heads, kv, dim, lens, window)
         c.check(got, window=window)
         again = c.run(window=window, max_rows=1, max_len=most)
         assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+# Row tiles enough, or said to go far enough, for the tiles of many rows (BF16): the guess of the longest length
+# decides whether they are split along the positions and whether these are unpacked ahead.
+TILES = [(64, 4, 64, [70, 0, 50, 1], [70, 40, 333, 20]), (64, 4, 128, [160, 30, 0, 95], [160, 30, 9, 450]),
+         (32, 2, 256, [150, 0, 90, 100], [180, 5, 90, 333])]
+
+
+@pytest.mark.parametrize("heads,kv,dim,rows,lens", TILES)
+@pytest.mark.parametrize("guess", [500, 1999, 10 ** 5])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 1), (True, 70), (False, 0)])
+@pytest.mark.parametrize("lse", [True, False])
+def test_tiles_of_many_rows(kh, heads, kv, dim, rows, lens, guess, causal, window, lse):
+    c = Case(BF16, heads, kv, dim, 16 if causal else 64, rows, lens)
+    c.check(c.run(causal=causal, window=window, max_rows=max(rows), max_len=guess, return_lse=lse), causal, window)
+
+
+@pytest.mark.parametrize("heads,kv,dim,rows,lens", TILES)
+@pytest.mark.parametrize("guess", [500, 1999, 10 ** 5])
+def test_tiles_of_many_rows_not_finite_lists_pages(kh, heads, kv, dim, rows, lens, guess):
+    """Groups that stand for NaN reach the rows that see them alone; unlisted heads; a page that is not there
+    before the window."""
+    c = Case(BF16, heads, kv, dim, 16, rows, lens)
+    last = len(lens) - 1
+    c.v[2 if lens[2] > 50 else last][lens[2] - 3 if lens[2] > 50 else lens[last] - 3, kv - 1, dim - 1] = float("nan")
+    c.k[0][lens[0] - 10, 0, 5] = float("inf")
+    c.cache.append(torch.cat(c.k).cuda(), torch.cat(c.v).cuda(), offsets(lens).cuda(),
+                   torch.zeros(len(lens), dtype=torch.int64).cuda(), c.table)
+    most = dict(max_rows=max(rows), max_len=guess)
+    for lse in (True, False):
+        c.check(c.run(return_lse=lse, **most))
+    rng = np.random.default_rng(2)
+    sel = np.stack([rng.permutation(heads)[:5] for _ in range(sum(rows))]).astype(np.int32)
+    on = np.zeros((sum(rows), heads), bool)
+    np.put_along_axis(on, sel.astype(np.int64), True, 1)
+    c.check(c.run(heads=torch.from_numpy(sel).cuda(), **most), on=on)
+    if lens[last] - rows[last] - 20 >= 16:
+        c.table[last, 0] = -7
+        c.check(c.run(window=20, **most), window=20)
+
+
+@pytest.mark.parametrize("guess", [1999, 10 ** 5])
+def test_tiles_of_many_rows_in_a_graph(kh, guess):
+    c = Case(BF16, *TILES[1][:3], 64, *TILES[1][3:])
+    q, out = c.q.cuda(), torch.zeros_like(c.q, device="cuda")
+    kw = dict(max_rows=160, max_len=guess)
+    want = c.cache.attention(q, c.off, c.len, c.table, **kw)
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        c.cache.attention(q, c.off, c.len, c.table, out=out, **kw)
+    for _ in range(4):
+        out.zero_()
+        g.replay()
+        other = c.cache.attention(q * 0.5, c.off, c.len, c.table, **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and not torch.equal(other, want)
