@@ -21,8 +21,8 @@
 // and rows along lanes, which is the layout that the second product takes its P
 // in when the positions of a step are numbered 4 g + i and 16 + 4 g + i; nothing
 // is exchanged between lanes but the running maximum.
+#include <algorithm>
 #include <cmath>
-#include <mutex>
 #include <type_traits>
 
 #include "mfma.hpp"
@@ -1379,7 +1379,8 @@ static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int
   PaPlan p;
   const int64_t gs = nh / c->nkv;
   if (max_rows > rows) max_rows = rows;
-  const int64_t tiles16 = batch * c->nkv * ((max_rows * gs + 15) / 16), held = pa_fill(c->d, dtype);
+  if (max_len > INT32_MAX) max_len = INT32_MAX;  // more than a table holds
+  const int64_t tiles16 = std::min<int64_t>((max_rows * gs + 15) / 16, 65536) * batch * c->nkv, held = pa_fill(c->d, dtype);
   p.many = dtype == KH_DT_BF16 && max_rows * gs >= kPtMinRows &&
            (tiles16 > held || (max_len > 0 && tiles16 > kPtMinWork * held / max_len));
   const PtSize z = pt_size(c->d, lse);
@@ -1408,7 +1409,7 @@ static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int
   p.un_steps = 0;
   if (p.many && p.tiles >= kPtUnpackTiles && max_len >= kPtUnpackWork / p.base) {
     const int64_t steps = (max_len + z.keys - 1) / z.keys;
-    if (steps > 0 && steps <= INT32_MAX / z.keys && batch * c->nkv * steps <= kPtUnpackMost / z.step) p.un_steps = steps;
+    if (steps <= kPtUnpackMost / z.step / (batch * c->nkv)) p.un_steps = steps;
   }
   return p;
 }
@@ -1426,22 +1427,9 @@ static PaSpace pa_space(const PaPlan& p, int64_t rows, int64_t batch, int nkv, i
   return s;
 }
 
-// Dynamic LDS of more than 64 KB has to be asked for, once a kernel.
-template <typename K>
-static hipError_t allow_lds(K* kernel, int bytes) {
-  return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 template <int D, int KT>
 static int pt_launch(const PaArgs& a, int64_t blocks, hipStream_t st) {
   constexpr int lds = PtShape<D, KT>::kLds;
-  static std::once_flag once;
-  static hipError_t arc = hipSuccess;
-  std::call_once(once, [] {
-    arc = allow_lds(&paged_tile_kernel<D, KT, false>, PtShape<D, KT>::kLds);
-    if (arc == hipSuccess) arc = allow_lds(&paged_tile_kernel<D, KT, true>, PtShape<D, KT>::kLds);
-  });
-  KH_HIP(arc);
   const dim3 g((unsigned)blocks), blk(64 * PtShape<D, KT>::NW);
   if (a.un_steps) {
     hipLaunchKernelGGL((paged_unpack_kernel<D, KT>),
@@ -1457,10 +1445,6 @@ static int pt_launch(const PaArgs& a, int64_t blocks, hipStream_t st) {
 
 template <int D, typename T>
 static int pa_launch(const PaArgs& a, bool many, int64_t blocks, hipStream_t st) {
-  static std::once_flag once;
-  static hipError_t arc = hipSuccess;
-  std::call_once(once, [] { arc = allow_lds(&paged_rows_kernel<D, T>, PaShape<D, T>::kLds); });
-  KH_HIP(arc);
   if constexpr (sizeof(T) == 2) {
     if (many) {
       const int rc = a.lse ? pt_launch<D, 2>(a, blocks, st) : pt_launch<D, 1>(a, blocks, st);
@@ -1485,6 +1469,25 @@ static int pa_launch_d(int d, const PaArgs& a, bool many, int64_t blocks, hipStr
   if (d == 128) return pa_launch<128, T>(a, many, blocks, st);
   return pa_launch<256, T>(a, many, blocks, st);
 }
+
+// Dynamic LDS of more than 64 KB has to be asked for, a kernel and device: when a cache
+// is made, so that no call does it inside a capture.
+template <typename K>
+static int allow_lds(K* kernel, int bytes) {
+  KH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  return KH_OK;
+}
+template <int D>
+static int allow_lds_d() {
+  int rc = allow_lds(&paged_rows_kernel<D, float>, PaShape<D, float>::kLds);
+  if (rc == KH_OK) rc = allow_lds(&paged_rows_kernel<D, uint16_t>, PaShape<D, uint16_t>::kLds);
+  if (rc == KH_OK) rc = allow_lds(&paged_tile_kernel<D, 1, false>, PtShape<D, 1>::kLds);
+  if (rc == KH_OK) rc = allow_lds(&paged_tile_kernel<D, 1, true>, PtShape<D, 1>::kLds);
+  if (rc == KH_OK) rc = allow_lds(&paged_tile_kernel<D, 2, false>, PtShape<D, 2>::kLds);
+  if (rc == KH_OK) rc = allow_lds(&paged_tile_kernel<D, 2, true>, PtShape<D, 2>::kLds);
+  return rc;
+}
+int paged_attn_prepare(int d) { return d == 64 ? allow_lds_d<64>() : d == 128 ? allow_lds_d<128>() : allow_lds_d<256>(); }
 
 static int pa_shape(const kh_paged_kv* c, int dtype, int64_t rows, int64_t batch, int num_heads, int64_t max_rows,
                     int64_t max_len) {
@@ -1530,7 +1533,7 @@ extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void
                (long long)table_cols, (long long)table_stride);
   KH_CHECK_ARG(table_cols <= (INT32_MAX - 64) >> c->ps_log2, "a page table of %lld columns holds 2^31 positions",
                (long long)table_cols);
-  KH_CHECK_ARG(std::isfinite(scale) && scale > 0, "scale must be positive and finite");
+  KH_CHECK_ARG(std::isfinite(scale * kLog2e) && scale > 0, "scale must be positive and finite");
   KH_CHECK_ARG(window >= 0 && (window == 0 || causal), "a window (%lld) needs causal attention", (long long)window);
   KH_CHECK_ARG(q_row_stride >= 0 && q_head_stride >= 0, "negative stride");
   KH_CHECK_ARG(n_heads >= 0 && n_heads <= 4 * num_heads, "n_heads %d not in [0,%d]", n_heads, 4 * num_heads);

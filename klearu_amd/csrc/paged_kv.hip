@@ -187,8 +187,8 @@ __device__ __forceinline__ void walk_quads(const KvRows& r, int units, int hpu, 
     int quads;
     if (few) {
       if (lane < nb) {
-        ws.o0 = (int)max(r.off[lane], (int64_t)0);
-        ws.o1 = (int)min(r.off[lane + 1], r.rows);
+        ws.o0 = (int)min(max(r.off[lane], (int64_t)0), r.rows);
+        ws.o1 = (int)min(max(r.off[lane + 1], (int64_t)0), r.rows);
         ws.start = r.start[lane];
         ws.n = quads_of(ws.o1 - ws.o0, ws.start);
       }
@@ -580,7 +580,7 @@ extern "C" int kh_paged_kv_create(int num_kv_heads, int head_dim, int page_size,
     KH_HIP(hipMemset(c->pool, 0, bytes));
     KH_HIP(hipMemset(c->err, 0, sizeof(int)));
     KH_HIP(hipStreamSynchronize(nullptr));
-    return KH_OK;
+    return paged_attn_prepare(c->d);
   };
   const int rc = fill();
   if (rc != KH_OK) {

@@ -68,6 +68,9 @@ inline int check_device(int device, const char* what) {
     if (dev_rc_ != KH_OK) return dev_rc_;                    \
   } while (0)
 
+// What the attention kernels of a head_dim need of the current device.
+int paged_attn_prepare(int d);
+
 inline size_t dtype_bytes(int dtype) { return dtype == KH_DT_F32 ? 4 : 2; }
 
 // Whether 16-byte accesses of whole 16-byte pieces are aligned: the base and

@@ -249,7 +249,8 @@ extern "C" int kh_rope_apply(const kh_rope* r, int dtype, const void* x_dev, int
                              void* stream) {
   KH_CHECK_ARG(r != nullptr, "null handle");
   KH_CHECK_ARG(dtype == KH_DT_F32 || dtype == KH_DT_BF16, "dtype %d: f32 and BF16 are supported", dtype);
-  KH_CHECK_ARG(rows >= 0 && heads >= 1 && heads <= 65536, "rows %lld, heads %d", (long long)rows, heads);
+  KH_CHECK_ARG(rows >= 0 && rows < (int64_t)1 << 31 && heads >= 1 && heads <= 65536, "rows %lld, heads %d",
+               (long long)rows, heads);
   KH_CHECK_ARG(head_dim >= r->rot && head_dim <= 65536, "head_dim %d not in [%d,65536]", head_dim, r->rot);
   if (rows == 0) return KH_OK;
   KH_CHECK_ARG(x_dev && y_dev && pos_dev, "null argument");

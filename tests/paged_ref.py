@@ -17,7 +17,7 @@ def bf16_down(x):
 def quantize(x):
     """x [..., dim] f32 -> (c, s, m) of every element, f64; s NaN and c = m = 0 where a group stands for NaN."""
     x = np.asarray(x, np.float32)
-    g = x.reshape(*x.shape[:-1], -1, G)
+    g = x.reshape(*x.shape[:-1], x.shape[-1] // G, G)
     with np.errstate(all="ignore"):
         m = bf16_down(g.min(-1, keepdims=True))
         s = -bf16_down(-((g.max(-1, keepdims=True) - m) / np.float32(15)))

@@ -217,3 +217,28 @@ def test_pool_past_4_gib(kh):
     gk, gv = c.gather(o, z, tb, n)
     same(gk, values(k.float().cpu().numpy()))
     same(gv, values(v.float().cpu().numpy()))
+
+
+@pytest.mark.parametrize("batch", [2, 70])
+def test_offsets_past_the_rows(kh, batch):
+    """Offsets before the first and past the last row, and past 32 bits: the rows between them, and no others."""
+    rng = np.random.default_rng(11)
+    c = cache_of(2, 64, 2 * batch, 16)
+    k, v = (torch.from_numpy(keys(rng, 9, 2, 64)).cuda() for _ in range(2))
+    far = [(-2 ** 40, 5, 2 ** 31), (-2 ** 32 - 5, 9, 2 ** 40), (4, 9, 2 ** 32 + 3), (2 ** 31, 2 ** 31 + 7, 2 ** 33)]
+    tb = torch.arange(2 * batch, dtype=torch.int32).view(batch, 2).cuda()
+    st = torch.zeros(batch, dtype=torch.int64).cuda()
+    for a, b, e in far:
+        off = torch.tensor([a, b, e] + [e] * (batch - 2)).cuda()
+        c.append(k, v, off, st, tb)
+        gk, gv = (torch.full((9, 2, 64), 3.0, device="cuda") for _ in range(2))
+        c.gather(off, st, tb, 9, k=gk, v=gv)
+        c.status()
+        one, two = slice(max(a, 0), min(max(b, 0), 9)), slice(min(b, 9), 9)
+        for got, x in ((gk, k), (gv, v)):
+            for s in (one, two):
+                same(got[s], values(x[s].cpu().numpy()))
+            assert (got[: min(max(a, 0), 9)] == 3).all()
+        got = c.attention(k.repeat(1, 2, 1), off, torch.full((batch,), 9).cuda(), tb, max_rows=9, max_len=9)
+        assert torch.isfinite(got[min(max(a, 0), 9):]).all()
+        c.status()

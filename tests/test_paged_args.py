@@ -120,3 +120,22 @@ def test_attention():
     refused("kh_paged_kv_attention", change(base, max_len=100000), CAP, "workspace")
     refused("kh_paged_kv_attention", change(base, max_len=100000, ws=P + 4, wsb=need.value), ARG, "aligned")
     assert _lib.load().kh_paged_kv_attention(*change(base, rows=0)) == 0
+
+
+def test_sizes_past_the_types():
+    base = dict(r=rope(), dtype=0, x=P, xs=0, xh=64, rows=2 ** 31, heads=2, dim=64, pos=P, y=2 * P, ys=128, yh=64, tr=0,
+                st=None)
+    refused("kh_rope_apply", list(base.values()), ARG, "rows")
+    base = dict(c=cache(), dtype=0, q=P, qs=256, qh=64, nh=4, rows=3, off=P, batch=3, len=P, table=P, cols=4, ts=4,
+                max_rows=1, max_len=64, scale=0.1, causal=1, window=0, heads=None, nsel=0, out=2 * P, os=256, oh=64,
+                lse=None, ws=None, wsb=0, st=None)
+    for kw, text in ((dict(cols=2 ** 60, ts=2 ** 60), "positions"), (dict(scale=3e38), "scale")):
+        refused("kh_paged_kv_attention", change(base, **kw), ARG, text)
+    need, same = C.c_int64(), C.c_int64()
+    call = _lib.load().kh_paged_kv_attention_workspace
+    for dtype, rows, most, lse in ((0, 3, 1, 0), (2, 3, 1, 1), (2, 5000, 5000, 0), (2, 5000, 2 ** 62, 1)):
+        assert call(cache(), dtype, rows, 3, 4, most, 2 ** 31 - 1, lse, C.byref(need)) == 0
+        assert call(cache(), dtype, rows, 3, 4, most, 2 ** 63 - 1, lse, C.byref(same)) == 0
+        assert need.value == same.value and (need.value > 0 or rows == 5000)
+    assert call(cache(), 2, 2 ** 31 - 1, 2 ** 31 - 1, 2, 2 ** 31 - 1, 2 ** 63 - 1, 1, C.byref(need)) == 0
+    assert 0 <= need.value < 2 ** 62
