@@ -43,6 +43,7 @@ struct PaShape {
 };
 constexpr int kPaStep = 32;        // positions a wave takes at a time
 constexpr int kPaMaxSplit = 128;
+constexpr int kPaFine = 512;      // positions up to which BF16 rows hold their weights in two terms
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -68,6 +69,7 @@ struct PaArgs {
   float* part_o;
   float2* part_ml;
   int nsplit, tiles;
+  int fine;   // two terms of P for BF16 rows
   int share;  // 0, or the parts that a kv head's sequences get by their lengths, up to nsplit each
   int qvec, ovec;
   char* un;  // unpacked positions (tiles of many rows): un_steps steps of each sequence
@@ -287,12 +289,18 @@ __device__ __forceinline__ int pa_share(const PaArgs& a, int lane, int waves, in
 
 // Block: one row tile of one (sequence, kv head), one of nsplit parts of the
 // positions that the tile sees; its waves take every NW-th step of 32.
-template <int D, typename T>
+//
+// NP: BF16 terms of the weights P.  f32 rows take three, all of their bits.  BF16 rows
+// take one, as their output has, where the roundings of many positions cancel, and two
+// where the caller says that they see 512 or fewer: the error against 64 bits was 1.9
+// times that of rounding the output alone for 20 positions, 1.4 for 180, 1.04 for 570 (two
+// terms: 1.00).  Eight sequences of 2048 take 25 us with one, 30 with two; both in one
+// kernel spill registers (33 us).
+template <int D, typename T, int NP>
 __global__ __launch_bounds__((64 * PaShape<D, T>::NW), (PaShape<D, T>::kPerSimd)) void paged_rows_kernel(PaArgs a) {
   constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16, NW = PaShape<D, T>::NW;
   constexpr int BIAS = sizeof(T) == 4 ? 16 : 128;
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1;  // terms of q: all of its bits
-  constexpr int NP = sizeof(T) == 4 ? 3 : 1;  // of P: all of its bits for f32 rows, 8 for BF16 ones, as their output
   constexpr int OS = PaShape<D, T>::kOS;
   extern __shared__ __align__(16) float s_o[];  // [NW][16][OS], then the maxima and sums
   float* s_m = s_o + NW * 16 * OS;
@@ -1451,11 +1459,15 @@ static int pa_launch(const PaArgs& a, bool many, int64_t blocks, hipStream_t st)
       if (rc != KH_OK) return rc;
     }
   }
-  if (!many)
-    hipLaunchKernelGGL((paged_rows_kernel<D, T>),
-                       dim3((unsigned)(a.share ? a.share + a.batch : a.nsplit), (unsigned)a.nkv,
-                            (unsigned)(a.share ? 1 : a.batch * a.tiles < 65535 ? a.batch * a.tiles : 65535)),
-                       dim3((64 * PaShape<D, T>::NW)), (PaShape<D, T>::kLds), st, a);
+  if (!many) {
+    const dim3 g((unsigned)(a.share ? a.share + a.batch : a.nsplit), (unsigned)a.nkv,
+                 (unsigned)(a.share ? 1 : a.batch * a.tiles < 65535 ? a.batch * a.tiles : 65535));
+    const dim3 blk((64 * PaShape<D, T>::NW));
+    constexpr int lds = PaShape<D, T>::kLds;
+    if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((paged_rows_kernel<D, T, 3>), g, blk, lds, st, a);
+    else if (a.fine) hipLaunchKernelGGL((paged_rows_kernel<D, T, 2>), g, blk, lds, st, a);
+    else hipLaunchKernelGGL((paged_rows_kernel<D, T, 1>), g, blk, lds, st, a);
+  }
   if (a.nsplit > 16)
     hipLaunchKernelGGL((paged_join_kernel<D, T, 4>), dim3((unsigned)(a.rows * a.nh)), dim3(256), 0, st, a);
   else if (a.nsplit > 1)
@@ -1479,8 +1491,9 @@ static int allow_lds(K* kernel, int bytes) {
 }
 template <int D>
 static int allow_lds_d() {
-  int rc = allow_lds(&paged_rows_kernel<D, float>, PaShape<D, float>::kLds);
-  if (rc == KH_OK) rc = allow_lds(&paged_rows_kernel<D, uint16_t>, PaShape<D, uint16_t>::kLds);
+  int rc = allow_lds(&paged_rows_kernel<D, float, 3>, PaShape<D, float>::kLds);
+  if (rc == KH_OK) rc = allow_lds(&paged_rows_kernel<D, uint16_t, 1>, PaShape<D, uint16_t>::kLds);
+  if (rc == KH_OK) rc = allow_lds(&paged_rows_kernel<D, uint16_t, 2>, PaShape<D, uint16_t>::kLds);
   if (rc == KH_OK) rc = allow_lds(&paged_tile_kernel<D, 1, false>, PtShape<D, 1>::kLds);
   if (rc == KH_OK) rc = allow_lds(&paged_tile_kernel<D, 1, true>, PtShape<D, 1>::kLds);
   if (rc == KH_OK) rc = allow_lds(&paged_tile_kernel<D, 2, false>, PtShape<D, 2>::kLds);
@@ -1585,6 +1598,7 @@ extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void
   a.lse = lse_dev;
   a.nsplit = p.nsplit;
   a.share = p.share;
+  a.fine = max_len <= kPaFine || (window > 0 && window <= kPaFine) ? 1 : 0;
   a.tiles = (int)p.tiles;
   char* ws = static_cast<char*>(ws_dev);
   a.part_o = reinterpret_cast<float*>(ws);

@@ -46,7 +46,7 @@ def seen(n, length, causal, window):
     return ok
 
 
-def attention(q, kraw, vraw, scale, causal=True, window=0, bf16=True, many=False):
+def attention(q, kraw, vraw, scale, causal=True, window=0, bf16=True, many=False, fine=False):
     """One sequence: q [n, heads, dim] f64, kraw, vraw [length, kv, dim] f32 as appended ->
     (out, lse, tolerance of out, tolerance of lse), f64.
 
@@ -56,7 +56,8 @@ def attention(q, kraw, vraw, scale, causal=True, window=0, bf16=True, many=False
     takes is rounded to 8 bits (2^-8; f32 rows: three times 8, 2^-24) of p s c + p |m|; its sums over the positions have
     magnitudes sum p (271 s + |m|) and at most length / 4 + 64 additions in a row; out is rounded last.  Tiles of
     many BF16 rows (`many`) take keys and values rounded to 8 bits: 2^-8 of |q| |k| and of p |v| more, and divide by
-    the sum of the rounded weights: 2^-8 of |o| <= sum p |v| once more."""
+    the sum of the rounded weights: 2^-8 of |o| <= sum p |v| once more.  Few positions (`fine`): weights in two
+    terms, 2^-16."""
     n, heads, dim = q.shape
     length, kv = kraw.shape[:2]
     kc, ks, km = quantize(kraw)
@@ -66,7 +67,7 @@ def attention(q, kraw, vraw, scale, causal=True, window=0, bf16=True, many=False
     out, lse = np.zeros((n, heads, dim)), np.full((n, heads), -np.inf)
     tol, tol_l = np.zeros((n, heads, dim)), np.zeros((n, heads))
     u = 2.0 ** -24
-    up, uo = (2.0 ** -8, 2.0 ** -8) if bf16 else (u, u)
+    up, uo = (2.0 ** -16 if fine else 2.0 ** -8, 2.0 ** -8) if bf16 else (u, u)
     for h in range(heads):
         g = h * kv // heads
         with np.errstate(all="ignore"):

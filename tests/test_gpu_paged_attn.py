@@ -26,6 +26,7 @@ class Case:
         zero = torch.zeros(len(lens), dtype=torch.int64).cuda()
         if sum(lens):
             self.cache.append(torch.cat(self.k).cuda(), torch.cat(self.v).cuda(), offsets(lens).cuda(), zero, self.table)
+        self.fine = False  # whether BF16 rows hold their weights in two terms
         self.many = False  # whether the call takes tiles of many rows
         self.q = torch.from_numpy((rng.normal(0, qscale, (sum(rows), heads, dim))).astype(np.float32)).to(dtype)
 
@@ -48,7 +49,7 @@ class Case:
             assert (out[at:at + first] == 0).all() and (lse is None or (lse[at:at + first] == -np.inf).all())
             if length:
                 o, l, to, tl = attention(q[first:], k.float().numpy(), v.float().numpy(),
-                                         self.dim ** -0.5 if scale is None else scale, causal, window, self.dtype == BF16, self.many)
+                                         self.dim ** -0.5 if scale is None else scale, causal, window, self.dtype == BF16, self.many, self.fine)
                 if on is not None:
                     off = ~on[keep]
                     o[off], l[off], to[off], tl[off] = 0, -np.inf, 0, 0
@@ -541,3 +542,15 @@ def test_tiles_of_many_rows_in_a_graph(kh, guess):
         other = c.cache.attention(q * 0.5, c.off, c.len, c.table, **kw)
         torch.cuda.synchronize()
         assert torch.equal(out, want) and not torch.equal(other, want)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 4, 128), (8, 2, 64), (6, 2, 256)])
+@pytest.mark.parametrize("rows,lens,window", [([1] * 6, [1, 7, 20, 33, 150, 512], 0), ([9, 1, 4], [9, 40, 333], 0),
+                                              ([1, 3, 1], [2000, 900, 31], 24)])
+def test_few_positions(kh, heads, kv, dim, rows, lens, window):
+    """BF16 rows of 512 positions or fewer, by their lengths or a window: weights to 2^-16."""
+    c = Case(BF16, heads, kv, dim, 32, rows, lens)
+    c.fine = True
+    got = c.run(window=window, max_len=max(lens))
+    c.many = False
+    c.check(got, window=window)
