@@ -881,7 +881,7 @@ __global__ __launch_bounds__((64 * PtShape<D, KT>::NW)) void paged_unpack_kernel
 template <int D, int KT, bool UN>
 __device__ __forceinline__ void pt_tiles(const PaArgs& a, char* s_buf, int* s_lo, int* s_hi,
                                          uint32_t (*s_nan)[D / kKvGroup][2], int64_t b, int h, int split, int tile0,
-                                         int64_t o0, int64_t o1, int64_t L) {
+                                         int every, int64_t o0, int64_t o1, int64_t L) {
   using S = PtShape<D, KT>;
   constexpr int NG = S::NG, NF = S::NF, CT = S::CT, RW = S::RW, RB = S::RB, NW = S::NW;
   constexpr int KEYS = S::KEYS, TK = S::TK, TV = S::TV;
@@ -892,7 +892,8 @@ __device__ __forceinline__ void pt_tiles(const PaArgs& a, char* s_buf, int* s_lo
   const int32_t* __restrict__ table = a.table + b * a.table_stride;
   const PtUnpack<D, KT> un(lane, wave, 1 << a.ps_log2);
 
-  for (int tile = tile0; tile < (nr + RB - 1) / RB; tile += a.tiles) {
+  for (int64_t tl = tile0; tl < (nr + RB - 1) / RB; tl += every) {
+    const int tile = (int)tl;
     int lo[CT], hi[CT];
     uint32_t row[CT];  // t * nh + head, below 2^31
     bool inside[CT];
@@ -1229,8 +1230,35 @@ __device__ __forceinline__ void pt_tiles(const PaArgs& a, char* s_buf, int* s_lo
   }
 }
 
+// The u-th row tile of up to 64 sequences, the last tiles (which see the most) of all of
+// them first: false where there are no more.  Grids of every sequence's most tiles left
+// compute units empty behind blocks without rows (chunks of 331, 255, 41 and 286 rows:
+// 232 blocks with rows among 336 began in two rounds, 71 us instead of 37).
+__device__ __forceinline__ bool pt_tile(const PaArgs& a, int lane, int rb, uint32_t u, int* b, int* tile) {
+  uint32_t n = 0;
+  if (lane < a.batch) {
+    const int64_t rows = min(a.off[lane + 1], a.rows) - max(a.off[lane], (int64_t)0);
+    if (rows > 0) n = (uint32_t)((rows * a.gs + rb - 1) / rb);
+  }
+  const auto from = [&](uint32_t t) {  // tiles t and later of all sequences
+    return (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan((int)(n > t ? n - t : 0u)), 63);
+  };
+  if (u >= from(0)) return false;
+  uint32_t lo = 0, hi = wave_max_u32(n);  // from(lo) > u >= from(hi)
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) >> 1;
+    if (from(mid) > u) lo = mid;
+    else hi = mid;
+  }
+  const uint64_t level = __ballot(n > lo);
+  const uint32_t k = u - from(hi), rank = __builtin_popcountll(level & ((1ull << lane) - 1));
+  *b = __builtin_ctzll(__ballot(n > lo && rank == k));
+  *tile = (int)lo;
+  return true;
+}
+
 // Blocks of the same kv head lie on the same XCD (h is what varies fastest, and
-// there are eight), and the longest tiles begin first.
+// there are eight XCDs).
 template <int D, int KT, bool UN>
 __global__ __launch_bounds__((64 * PtShape<D, KT>::NW), 2) void paged_tile_kernel(PaArgs a) {
   extern __shared__ __align__(16) char s_buf[];
@@ -1241,8 +1269,17 @@ __global__ __launch_bounds__((64 * PtShape<D, KT>::NW), 2) void paged_tile_kerne
   id /= (uint32_t)a.nkv;
   const int split = (int)(id % (uint32_t)a.nsplit);
   id /= (uint32_t)a.nsplit;
-  const int64_t b = id % (uint32_t)a.batch;
-  const int tile0 = a.tiles - 1 - (int)(id / (uint32_t)a.batch);
+  int tile0, every = a.tiles;
+  int64_t b;
+  if (a.batch <= 64) {
+    int s;
+    if (!pt_tile(a, threadIdx.x & 63, PtShape<D, KT>::RB, id, &s, &tile0)) return;
+    b = s;
+    every = INT32_MAX;
+  } else {
+    b = id % (uint32_t)a.batch;
+    tile0 = a.tiles - 1 - (int)(id / (uint32_t)a.batch);
+  }
   int64_t o0 = a.off[b], o1 = a.off[b + 1], L = a.len[b];
   o0 = o0 < 0 ? 0 : o0;
   o1 = o1 > a.rows ? a.rows : o1;
@@ -1254,9 +1291,9 @@ __global__ __launch_bounds__((64 * PtShape<D, KT>::NW), 2) void paged_tile_kerne
   }
   // a sequence that is longer than the caller said was not unpacked
   if (UN && a.len[b] <= (int64_t)a.un_steps * PtShape<D, KT>::KEYS && a.len[b] <= cap)
-    pt_tiles<D, KT, true>(a, s_buf, s_lo, s_hi, s_nan, b, h, split, tile0, o0, o1, L);
+    pt_tiles<D, KT, true>(a, s_buf, s_lo, s_hi, s_nan, b, h, split, tile0, every, o0, o1, L);
   else
-    pt_tiles<D, KT, false>(a, s_buf, s_lo, s_hi, s_nan, b, h, split, tile0, o0, o1, L);
+    pt_tiles<D, KT, false>(a, s_buf, s_lo, s_hi, s_nan, b, h, split, tile0, every, o0, o1, L);
 }
 
 // Joins the parts of each row: W waves a (row, head), four elements a lane, so
@@ -1398,6 +1435,7 @@ static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int
   if (p.tiles > 65536) p.tiles = 65536;
   p.base = batch * c->nkv * p.tiles;
   const int64_t fill = p.many ? z.fill : pa_fill(c->d, dtype);
+  if (p.many && batch <= 64) p.base = c->nkv * ((rows * gs + batch * (rb - 1)) / rb);  // as pt_tile counts them
   int64_t want = fill / p.base;  // one round of blocks: a second would begin with its own latency
   // parts of fewer than four steps a wave do not pay for the join
   const int64_t step = p.many ? 512 : 32 * pa_waves(c->d, dtype);
