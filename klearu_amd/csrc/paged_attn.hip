@@ -21,6 +21,13 @@
 // and rows along lanes, which is the layout that the second product takes its P
 // in when the positions of a step are numbered 4 g + i and 16 + 4 g + i; nothing
 // is exchanged between lanes but the running maximum.
+//
+// Few rows (paged_rows_kernel) are bound by the cache's bytes where it is long and by a
+// chain of some 6.5 us where it is short: launch, lengths, pages, codes, one step, the
+// join of the waves.  32 heads of 128, BF16: eight sequences of 2048 positions (84 MB)
+// 24.4 us, 131072 positions of 8 kv heads (168 MB) 44.4 + 5.2 us of join (3.7 TB/s; a copy
+// runs at 4.8, read and write), 64 positions 7 us.  16 of 32 heads, f32, 2000 positions:
+// 11.3 + 3.7 us.  Many rows: below.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -288,7 +295,9 @@ __device__ __forceinline__ int pa_share(const PaArgs& a, int lane, int waves, in
 }
 
 // Block: one row tile of one (sequence, kv head), one of nsplit parts of the
-// positions that the tile sees; its waves take every NW-th step of 32.
+// positions that the tile sees; its waves take every NW-th step of 32, the next step's
+// codes under way.  As many blocks as the registers let the chip hold at once: twice as
+// many parts were slower (64 sequences: 26.9 us instead of 25), each begins with the chain.
 //
 // NP: BF16 terms of the weights P.  f32 rows take three, all of their bits.  BF16 rows
 // take one, as their output has, where the roundings of many positions cancel, and two
@@ -652,15 +661,17 @@ __global__ __launch_bounds__((64 * PaShape<D, T>::NW), (PaShape<D, T>::kPerSimd)
 //
 // Where three row tiles or more see the same positions, a kernel unpacks them once into
 // the workspace and the tiles copy them to LDS as they are: 4096 causal rows of 32 heads
-// of 128 take 13 + 166 us so, 210 us where each tile unpacks them; three chunks of 256-wide
-// heads 11 + 72 us against 103.  The copies go through registers: for a load straight to
-// LDS the compiler waits before the next read of any LDS (178 us).
+// of 128 take 13 + 166 us so, 210 us where each tile unpacks them (at 137 GFLOP 0.83
+// PFLOP/s; a call in a stream of them 149 us).  The copies go through registers: for a
+// load straight to LDS the compiler waits before the next read of any LDS (178 us).
 //
 // A value's group that stands for NaN is unpacked as 0 and marked in a mask of its
 // positions: rows that see one of them get their NaN from the mask.
 //
-// Bound by its own latency: two waves a SIMD (registers), each with its products (41% of
-// the time), exponentials and roundings (29%) and waits one after the other.  Half of the
+// Bound by its own latency: two waves a SIMD (registers), each with its products (42% of
+// the time), other vector instructions (29%) and waits one after the other; at D = 256 by
+// reading LDS, where a fragment feeds one product a wave (four chunks of 41 to 331 rows of
+// 16 heads over 2, window 1024: 11 + 41 us and 8 of join).  Half of the
 // waves a phase later (177 us), exponentials between the products of the step before
 // (spills), blocks of four waves (187 us) and raised priority for products (no change)
 // did not help.
@@ -1142,7 +1153,7 @@ __device__ __forceinline__ void pt_tiles(const PaArgs& a, char* s_buf, int* s_lo
           else mask = s_nan[st & 1][gi][0] | (uint64_t)s_nan[st & 1][gi][1] << 32;
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
-            const int from = max(lo[c] - tok, 0), to = min(hi[c] - tok, KEYS);  // of the 64 positions
+            const int from = max(lo[c] - tok, 0), to = min(hi[c] - tok, KEYS);  // of the step's positions
             uint64_t see = to > from ? (~0ull >> (64 - (to - from))) << from : 0;
             for (int k = 0; k < TK; ++k)
               if (!(ok >> k & 1)) see &= ~(0xffffull << (16 * k));
@@ -1297,7 +1308,8 @@ __global__ __launch_bounds__((64 * PtShape<D, KT>::NW), 2) void paged_tile_kerne
 }
 
 // Joins the parts of each row: W waves a (row, head), four elements a lane, so
-// that 256 / D parts of a wave are in flight at once.
+// that 256 / D parts of a wave are in flight at once.  4 us, latency: the parts come
+// from other XCDs' caches.
 template <int D, typename T, int W>
 __global__ __launch_bounds__(256) void paged_join_kernel(PaArgs a) {
   constexpr int C = D / 4, NS = 64 / C;

@@ -167,12 +167,6 @@ __device__ __forceinline__ int64_t readlane64(int64_t v, int l) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// A wave takes a quad and the heads of one unit: D / 8 lanes a position with eight
-// neighbouring values each, so four lanes share a group.  blockIdx.y: keys, values.
-// Keys leave as they are, a word a lane.  The u16 of a value's layout gathers the
-// nibbles of four lanes (c, c ^ 2, c ^ 4, c ^ 6), and a quad's four positions
-// share 16-byte pieces: they are put together in LDS and stored whole where all
-// four are appended, and as u16 where they are not.
 // Gives the waves of the grid their quads, one unit (hpu heads) at a time:
 // f(p0, t0, o0, o1, pg, h0, nh), with the quad's first position and its row, the
 // sequence's rows, the page, and the unit's heads.  Rows t0 .. t0 + 3 that lie in
@@ -249,6 +243,18 @@ struct QuadLanes {
   static constexpr int HW = D == 64 ? 2 : 1;                         // heads at a time
 };
 
+// A wave takes a quad and the heads of one unit: D / 8 lanes a position with eight
+// neighbouring values each, so four lanes share a group.  blockIdx.y: keys, values.
+// Keys leave as they are, a word a lane.  The u16 of a value's layout gathers the
+// nibbles of four lanes (c, c ^ 2, c ^ 4, c ^ 6), and a quad's four positions
+// share 16-byte pieces: they are put together in LDS and stored whole where all
+// four are appended, and as u16 where they are not.
+//
+// 14460 BF16 rows of 8 heads of 128 (59 MB in, 18.5 MB out, interleaved rotation): 32.4 us,
+// 2.4 TB/s.  28 vector instructions a value, for ranges, quotients, codes and their places,
+// take 55% of the issue slots, and loads wait behind them (a position a lane took 77 us;
+// quads with correctly rounded quotients by a division 38, by a corrected reciprocal 33).
+// One row: 4 us, the chain of offsets, page id and table.
 template <typename T, int D, int MODE, bool VAL>
 __device__ __forceinline__ void append_part(const AppendArgs& a, int units, int hpu, int* s_q, int* s_wsum, int* s_tot,
                                             uint16_t* s_v) {
@@ -402,7 +408,8 @@ struct GatherArgs {
 };
 
 // The inverse: the same quads and lanes.  Of the four lanes that need the same eight
-// u16 of a value's codes each loads two, and they exchange them.
+// u16 of a value's codes each loads two, and they exchange them.  14460 rows of 8 heads of
+// 128 to BF16 (18.5 MB in, 59 MB out): 22.8 us, 3.4 TB/s; 3.6 us for one.
 template <typename T, int D, bool VAL>
 __device__ __forceinline__ void gather_part(const GatherArgs& a, int units, int hpu, int* s_q, int* s_wsum, int* s_tot) {
   using P = KvParts<D>;
