@@ -49,7 +49,7 @@ struct PaShape {
   static constexpr int kLds = NW * 16 * (kOS + 2) * 4;
 };
 constexpr int kPaStep = 32;        // positions a wave takes at a time
-constexpr int kPaMaxSplit = 128;
+constexpr int kPaMaxSplit = 128;  // parts of a row that the join takes: two a lane
 constexpr int kPaFine = 512;      // positions up to which BF16 rows hold their weights in two terms
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -1461,8 +1461,7 @@ static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int
   // for each, 21 with eight at most; where all have 4096, 33 and 34).
   if (!p.many && p.nsplit > 1 && p.tiles == 1 && batch > 1 && batch <= 64) {
     p.share = (int)(fill / c->nkv - batch / 2);
-    p.nsplit = 2 * p.nsplit + 2;
-    if (p.nsplit > most) p.nsplit = (int)most;
+    p.nsplit = (int)std::min<int64_t>(std::min(2 * p.nsplit + 2, kPaMaxSplit), most);
   }
   p.un_steps = 0;
   if (p.many && p.tiles >= kPtUnpackTiles && max_len >= kPtUnpackWork / p.base) {

@@ -554,3 +554,22 @@ def test_few_positions(kh, heads, kv, dim, rows, lens, window):
     got = c.run(window=window, max_len=max(lens))
     c.many = False
     c.check(got, window=window)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("heads,kv,dim,lens", [(1, 1, 64, [40000, 25001]), (2, 1, 128, [30000, 1, 17])])
+def test_most_parts_of_a_row(kh, dtype, heads, kv, dim, lens):
+    """Few sequences of one kv head over long caches: as many parts as the join takes."""
+    c = Case(dtype, heads, kv, dim, 256, [1] * len(lens), lens)
+    for most in (max(lens), 2 ** 31):
+        c.check(c.run(max_len=most))
+        c.check(c.run(max_len=most, return_lse=False))
+
+
+@pytest.mark.parametrize("rows,guess", [(5, 40), (33, 1999)])
+def test_many_rows_of_many_sequences(kh, rows, guess):
+    """More than 64 sequences in tiles of many rows, some without rows."""
+    n = [0 if i % 7 == 3 else 1 + i % rows for i in range(70)]
+    c = Case(BF16, 64, 4, 64, 16, n, [r + i % 9 for i, r in enumerate(n)])
+    for lse in (True, False):
+        c.check(c.run(max_rows=rows, max_len=guess, return_lse=lse))
