@@ -250,9 +250,9 @@ struct QuadLanes {
 // share 16-byte pieces: they are put together in LDS and stored whole where all
 // four are appended, and as u16 where they are not.
 //
-// 14460 BF16 rows of 8 heads of 128 (59 MB in, 18.5 MB out, interleaved rotation): 32.4 us,
-// 2.4 TB/s.  28 vector instructions a value, for ranges, quotients, codes and their places,
-// take 55% of the issue slots, and loads wait behind them (a position a lane took 77 us;
+// 14460 BF16 rows of 8 heads of 128 (59 MB in, 18.5 MB out, interleaved rotation): 28.9 us,
+// 2.7 TB/s.  28 vector instructions a value, for ranges, quotients, codes and their places,
+// take 60% of the issue slots, and loads wait behind them (a position a lane took 77 us;
 // quads with correctly rounded quotients by a division 38, by a corrected reciprocal 33).
 // One row: 4 us, the chain of offsets, page id and table.
 template <typename T, int D, int MODE, bool VAL>
@@ -409,7 +409,8 @@ struct GatherArgs {
 
 // The inverse: the same quads and lanes.  Of the four lanes that need the same eight
 // u16 of a value's codes each loads two, and they exchange them.  14460 rows of 8 heads of
-// 128 to BF16 (18.5 MB in, 59 MB out): 22.8 us, 3.4 TB/s; 3.6 us for one.
+// 128 to BF16 (18.5 MB in, 59 MB out): 21.7 us, 3.6 TB/s, 3.6 us for one.  The rows leave
+// past the caches (22.8 us through them, and the append behind them 32.4 instead of 28.9).
 template <typename T, int D, bool VAL>
 __device__ __forceinline__ void gather_part(const GatherArgs& a, int units, int hpu, int* s_q, int* s_wsum, int* s_tot) {
   using P = KvParts<D>;
@@ -461,7 +462,7 @@ __device__ __forceinline__ void gather_part(const GatherArgs& a, int units, int 
           f[2 * i] = s * (float)(VAL ? (q[i] >> (4 * n)) & 15 : q[i] & 15) + m;
           f[2 * i + 1] = s * (float)(VAL ? (q[i] >> (4 * n + 16)) & 15 : (q[i] >> 4) & 15) + m;
         }
-        if (act) store8(y0 + k * TP * srow, true, f);
+        if (act) stream8(y0 + k * TP * srow, f);
       }
     }
   });
