@@ -247,12 +247,12 @@ class PagedKv(_Handle):
                 return self.gather(off, start, table, rows, dtype, k, v)
         shape = (rows, self.num_kv_heads, self.head_dim)
         if k is None:
-            k = torch.empty(shape, dtype=dtype, device=self.device)
+            k = torch.empty_strided(shape, (shape[1] * shape[2], shape[2], 1), dtype=dtype, device=self.device)
             kp = k.data_ptr()
         else:
             kp = _index(k, "k", dev, dtype, shape)
         if v is None:
-            v = torch.empty(shape, dtype=dtype, device=self.device)
+            v = torch.empty_like(k)
             vp = v.data_ptr()
         else:
             vp = _index(v, "v", dev, dtype, shape)
