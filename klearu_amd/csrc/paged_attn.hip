@@ -50,7 +50,7 @@ struct PaShape {
 };
 constexpr int kPaStep = 32;        // positions a wave takes at a time
 constexpr int kPaMaxSplit = 128;  // parts of a row that the join takes: two a lane
-constexpr int kPaFine = 512;      // positions up to which BF16 rows hold their weights in two terms
+constexpr int kPaFine = 1024;     // positions up to which BF16 rows hold their weights in two terms
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -301,10 +301,10 @@ __device__ __forceinline__ int pa_share(const PaArgs& a, int lane, int waves, in
 //
 // NP: BF16 terms of the weights P.  f32 rows take three, all of their bits.  BF16 rows
 // take one, as their output has, where the roundings of many positions cancel, and two
-// where the caller says that they see 512 or fewer: the error against 64 bits was 1.9
-// times that of rounding the output alone for 20 positions, 1.4 for 180, 1.04 for 570 (two
-// terms: 1.00).  Eight sequences of 2048 take 25 us with one, 30 with two; both in one
-// kernel spill registers (33 us).
+// where the caller says that they see 1024 or fewer: with one the error against 64 bits was
+// 1.9 times that of rounding the output alone for 20 positions, 1.4 for 180 and 1.5 for
+// lengths up to 650 mixed (two terms: 1.00).  Eight sequences of 1024 take 16.2 us with
+// one, 18.3 with two, of 2048 25 and 30; both in one kernel spill registers (33 us).
 template <int D, typename T, int NP>
 __global__ __launch_bounds__((64 * PaShape<D, T>::NW), (PaShape<D, T>::kPerSimd)) void paged_rows_kernel(PaArgs a) {
   constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16, NW = PaShape<D, T>::NW;
