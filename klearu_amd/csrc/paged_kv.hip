@@ -426,7 +426,6 @@ __device__ __forceinline__ void gather_part(const GatherArgs& a, int units, int 
     const int at0 = (int)(p0 & (ps - 1));
     T* y0 = dst + t0 * srow + (int64_t)(h0 + sub) * D;
     const char* blk = a.r.pool + ((int64_t)pg * a.r.nkv + h0) * a.r.block;
-#pragma unroll 2
     for (int h1 = 0; h1 < nh; h1 += HW, y0 += HW * D, blk += HW * a.r.block) {
       const bool there = HW == 1 || h1 + sub < nh;
       const char* mine = blk + (there ? sub : 0) * a.r.block;  // lanes without a head read the first one's
