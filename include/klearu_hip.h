@@ -784,9 +784,9 @@ int kh_paged_kv_attention_workspace(const kh_paged_kv* c, int dtype, int64_t row
  * repeated ids counted once): heads that a row does not list give 0 and -inf
  * and their share of the cache is not read.
  * max_rows and max_len are the caller's guess of the most rows and the longest
- * length of a sequence; a wrong one costs time, or the roundings below.  Sums and
- * softmax statistics are f32; BF16 rows have their weights p rounded to BF16 (to
- * 2^-16 where max_len or the window is 1024 or less, but for the next).
+ * length of a sequence; a wrong one costs time and workspace.  Sums and softmax statistics
+ * are f32; BF16 rows have their weights p rounded to BF16 (to 2^-16 in sequences of
+ * 1024 positions or fewer and with such a window, but for the next).
  * BF16 calls of many rows (max_rows times the query heads of a kv head of 64 or
  * more) may take keys and values rounded to BF16 as well; with lse_dev their keys
  * are held to 2^-16 instead, so that out may differ from a call without it in the

@@ -76,7 +76,6 @@ struct PaArgs {
   float* part_o;
   float2* part_ml;
   int nsplit, tiles;
-  int fine;   // two terms of P for BF16 rows
   int share;  // 0, or the parts that a kv head's sequences get by their lengths, up to nsplit each
   int qvec, ovec;
   char* un;  // unpacked positions (tiles of many rows): un_steps steps of each sequence
@@ -294,55 +293,22 @@ __device__ __forceinline__ int pa_share(const PaArgs& a, int lane, int waves, in
   return b;
 }
 
-// Block: one row tile of one (sequence, kv head), one of nsplit parts of the
-// positions that the tile sees; its waves take every NW-th step of 32, the next step's
-// codes under way.  As many blocks as the registers let the chip hold at once: twice as
-// many parts were slower (64 sequences: 26.9 us instead of 25), each begins with the chain.
-//
-// NP: BF16 terms of the weights P.  f32 rows take three, all of their bits.  BF16 rows
-// take one, as their output has, where the roundings of many positions cancel, and two
-// where the caller says that they see 1024 or fewer: with one the error against 64 bits was
-// 1.9 times that of rounding the output alone for 20 positions, 1.4 for 180 and 1.5 for
-// lengths up to 650 mixed (two terms: 1.00).  Eight sequences of 1024 take 16.2 us with
-// one, 18.3 with two, of 2048 25 and 30; both in one kernel spill registers (33 us).
+// Row tiles tile0, + tiles, ... of one (sequence, kv head): part `split` of `parts` of the
+// positions that each sees.  pre: the first 64 of the sequence's pages, one a lane.
+// NP: BF16 terms of the weights; each NP has the whole body to itself, from the queries to
+// the join: one loop for either in a body that both share spills 276 registers.
 template <int D, typename T, int NP>
-__global__ __launch_bounds__((64 * PaShape<D, T>::NW), (PaShape<D, T>::kPerSimd)) void paged_rows_kernel(PaArgs a) {
+__device__ __forceinline__ void pa_tiles(const PaArgs& a, float* s_o, const PaLane<D>& lo_, const int32_t* __restrict__ table,
+                                         int pre, int h, int split, int parts, int tile0, int64_t o0, int n, int64_t L) {
   constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16, NW = PaShape<D, T>::NW;
   constexpr int BIAS = sizeof(T) == 4 ? 16 : 128;
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1;  // terms of q: all of its bits
   constexpr int OS = PaShape<D, T>::kOS;
-  extern __shared__ __align__(16) float s_o[];  // [NW][16][OS], then the maxima and sums
   float* s_m = s_o + NW * 16 * OS;
   float* s_l = s_m + NW * 16;
   const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.y;
-  const int ps = 1 << a.ps_log2;
-  const int64_t cap = a.cols << a.ps_log2;
-  const PaLane<D> lo_(lane, ps);
-  int split = blockIdx.x, parts = a.nsplit;
-  int64_t z0 = blockIdx.z;
-  if (a.share) {
-    const int s = pa_share(a, lane, NW, &split, &parts);
-    if (s < 0) return;
-    z0 = s;
-  }
-  for (int64_t bt = z0; bt < a.batch * a.tiles; bt += a.share ? a.batch : gridDim.z) {
-  const int64_t b = a.tiles == 1 ? bt : bt / a.tiles;
-  const int tile0 = a.tiles == 1 ? 0 : (int)(bt - b * a.tiles);
-  // the first of the chain's loads together: rows, length, the first 64 pages
-  const int32_t* __restrict__ table = a.table + b * a.table_stride;
-  const int pre = lane < a.cols ? table[lane] : -1;
-  int64_t o0 = a.off[b], o1 = a.off[b + 1], L = a.len[b];
-  o0 = o0 < 0 ? 0 : o0;
-  o1 = o1 > a.rows ? a.rows : o1;
-  if (o1 <= o0) continue;
-  const int n = (int)(o1 - o0), nr = n * a.gs;  // rows x heads of a kv head: below 2^31
-  if (L < 0 || L > cap) {
-    if (threadIdx.x == 0) atomicOr(a.err, 1);
-    L = L < 0 ? 0 : cap;
-  }
-
+  const int ps = 1 << a.ps_log2, nr = n * a.gs;  // rows x heads of a kv head: below 2^31
   for (int tile = tile0; tile < (nr + 15) >> 4; tile += a.tiles) {
     // the lane's row (column of the products)
     const int rr = tile * 16 + col;
@@ -648,6 +614,56 @@ __global__ __launch_bounds__((64 * PaShape<D, T>::NW), (PaShape<D, T>::kPerSimd)
     }
     __syncthreads();
   }
+}
+
+// Block: one row tile of one (sequence, kv head), one of nsplit parts of the
+// positions that the tile sees; its waves take every NW-th step of 32, the next step's
+// codes under way.  As many blocks as the registers let the chip hold at once: twice as
+// many parts were slower (64 sequences: 26.9 us instead of 25), each begins with the chain.
+//
+// BF16 terms of the weights P: f32 rows take three, all of their bits.  BF16 rows
+// take one, as their output has, where the roundings of many positions cancel, and two
+// where the sequence's length, or the window, lets them see 1024 or fewer: with one the
+// error against 64 bits was 1.9 times that of rounding the output alone for 20 positions,
+// 1.4 for 180 and 1.5 for lengths up to 650 mixed (two terms: 1.00).  Eight sequences of
+// 1024 take 16.2 us with one, 18.3 with two, of 2048 25 and 30.
+template <int D, typename T>
+__global__ __launch_bounds__((64 * PaShape<D, T>::NW), (PaShape<D, T>::kPerSimd)) void paged_rows_kernel(PaArgs a) {
+  constexpr int NW = PaShape<D, T>::NW;
+  extern __shared__ __align__(16) float s_o[];  // [NW][16][OS], then the maxima and sums
+  const int lane = threadIdx.x & 63;
+  const int h = blockIdx.y;
+  const int64_t cap = a.cols << a.ps_log2;
+  const PaLane<D> lo_(lane, 1 << a.ps_log2);
+  int split = blockIdx.x, parts = a.nsplit;
+  int64_t z0 = blockIdx.z;
+  if (a.share) {
+    const int s = pa_share(a, lane, NW, &split, &parts);
+    if (s < 0) return;
+    z0 = s;
+  }
+  for (int64_t bt = z0; bt < a.batch * a.tiles; bt += a.share ? a.batch : gridDim.z) {
+  const int64_t b = a.tiles == 1 ? bt : bt / a.tiles;
+  const int tile0 = a.tiles == 1 ? 0 : (int)(bt - b * a.tiles);
+  // the first of the chain's loads together: rows, length, the first 64 pages
+  const int32_t* __restrict__ table = a.table + b * a.table_stride;
+  const int pre = lane < a.cols ? table[lane] : -1;
+  int64_t o0 = a.off[b], o1 = a.off[b + 1], L = a.len[b];
+  o0 = o0 < 0 ? 0 : o0;
+  o1 = o1 > a.rows ? a.rows : o1;
+  if (o1 <= o0) continue;
+  const int n = (int)(o1 - o0);
+  if (L < 0 || L > cap) {
+    if (threadIdx.x == 0) atomicOr(a.err, 1);
+    L = L < 0 ? 0 : cap;
+  }
+
+  const auto run = [&](auto terms) {
+    pa_tiles<D, T, decltype(terms)::value>(a, s_o, lo_, table, pre, h, split, parts, tile0, o0, n, L);
+  };
+  if constexpr (sizeof(T) == 4) run(std::integral_constant<int, 3>{});
+  else if ((a.window > 0 && a.window < L ? a.window : L) <= kPaFine) run(std::integral_constant<int, 2>{});
+  else run(std::integral_constant<int, 1>{});
   }
 }
 
@@ -1513,9 +1529,7 @@ static int pa_launch(const PaArgs& a, bool many, int64_t blocks, hipStream_t st)
                  (unsigned)(a.share ? 1 : a.batch * a.tiles < 65535 ? a.batch * a.tiles : 65535));
     const dim3 blk((64 * PaShape<D, T>::NW));
     constexpr int lds = PaShape<D, T>::kLds;
-    if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((paged_rows_kernel<D, T, 3>), g, blk, lds, st, a);
-    else if (a.fine) hipLaunchKernelGGL((paged_rows_kernel<D, T, 2>), g, blk, lds, st, a);
-    else hipLaunchKernelGGL((paged_rows_kernel<D, T, 1>), g, blk, lds, st, a);
+    hipLaunchKernelGGL((paged_rows_kernel<D, T>), g, blk, lds, st, a);
   }
   if (a.nsplit > 16)
     hipLaunchKernelGGL((paged_join_kernel<D, T, 4>), dim3((unsigned)(a.rows * a.nh)), dim3(256), 0, st, a);
@@ -1540,9 +1554,8 @@ static int allow_lds(K* kernel, int bytes) {
 }
 template <int D>
 static int allow_lds_d() {
-  int rc = allow_lds(&paged_rows_kernel<D, float, 3>, PaShape<D, float>::kLds);
-  if (rc == KH_OK) rc = allow_lds(&paged_rows_kernel<D, uint16_t, 1>, PaShape<D, uint16_t>::kLds);
-  if (rc == KH_OK) rc = allow_lds(&paged_rows_kernel<D, uint16_t, 2>, PaShape<D, uint16_t>::kLds);
+  int rc = allow_lds(&paged_rows_kernel<D, float>, PaShape<D, float>::kLds);
+  if (rc == KH_OK) rc = allow_lds(&paged_rows_kernel<D, uint16_t>, PaShape<D, uint16_t>::kLds);
   if (rc == KH_OK) rc = allow_lds(&paged_tile_kernel<D, 1, false>, PtShape<D, 1>::kLds);
   if (rc == KH_OK) rc = allow_lds(&paged_tile_kernel<D, 1, true>, PtShape<D, 1>::kLds);
   if (rc == KH_OK) rc = allow_lds(&paged_tile_kernel<D, 2, false>, PtShape<D, 2>::kLds);
@@ -1647,7 +1660,6 @@ extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void
   a.lse = lse_dev;
   a.nsplit = p.nsplit;
   a.share = p.share;
-  a.fine = max_len <= kPaFine || (window > 0 && window <= kPaFine) ? 1 : 0;
   a.tiles = (int)p.tiles;
   char* ws = static_cast<char*>(ws_dev);
   a.part_o = reinterpret_cast<float*>(ws);

@@ -268,8 +268,8 @@ class PagedKv(_Handle):
         head_dim ** -0.5.  heads [rows, n] (int32, SparsityPredictor.select_top_k's lists) leaves
         the other heads 0.  max_rows and max_len guess the most rows and the longest length of a
         sequence (default: an even share of the rows, the table's reach); wrong guesses cost
-        time (BF16 weights are held finer where max_len or window is 1024 or less).  Returns out,
-        or (out, lse) with lse [rows, num_heads] f32: a row that sees nothing gives 0 and -inf."""
+        time and workspace.  Returns out, or (out, lse) with lse [rows, num_heads] f32: a row that
+        sees nothing gives 0 and -inf."""
         dev = self._dev
         qp, q0, q1, dt = _rows(q, "q", dev)
         n, nh, dim = q.shape
