@@ -863,8 +863,8 @@ struct PtUnpack {
 
 // Where a step's positions of one (sequence, kv head) lie in the workspace once they
 // are unpacked for all tiles, kStep bytes each: their keys' fragments, term by term,
-// then their values'.  Behind all steps: the masks [NG][2] of value groups that
-// stand for NaN.
+// then their values'.  Behind all steps: the masks [NG][TV] of value groups that
+// stand for NaN, one bit for each of 32 positions.
 __device__ __forceinline__ int64_t pt_step(const PaArgs& a, int64_t b, int h, int st) {
   return (b * a.nkv + h) * a.un_steps + st;
 }
@@ -897,7 +897,7 @@ __global__ __launch_bounds__((64 * PtShape<D, KT>::NW)) void paged_unpack_kernel
     char* to = a.un + at * S::kStep + lane * 16;
     u.keys(x, [&](int k, int f, const uint4& w) { *reinterpret_cast<uint4*>(to + k * S::kKeyPart + f * 1024) = w; });
     u.nan(x, [&](int gi, int half, uint32_t m) {
-      if (lane == 0) a.un_nan[(at * NG + gi) * 2 + half] = m;
+      if (lane == 0) a.un_nan[(at * NG + gi) * S::TV + half] = m;
     });
     u.values(x, [&](int f, const uint4& w) { *reinterpret_cast<uint4*>(to + S::kKeys + f * 1024) = w; });
   }
@@ -907,7 +907,7 @@ __global__ __launch_bounds__((64 * PtShape<D, KT>::NW)) void paged_unpack_kernel
 // are.
 template <int D, int KT, bool UN>
 __device__ __forceinline__ void pt_tiles(const PaArgs& a, char* s_buf, int* s_lo, int* s_hi,
-                                         uint32_t (*s_nan)[D / kKvGroup][2], int64_t b, int h, int split, int tile0,
+                                         uint32_t (*s_nan)[D / kKvGroup][PtShape<D, KT>::TV], int64_t b, int h, int split, int tile0,
                                          int every, int64_t o0, int64_t o1, int64_t L) {
   using S = PtShape<D, KT>;
   constexpr int NG = S::NG, NF = S::NF, CT = S::CT, RW = S::RW, RB = S::RB, NW = S::NW;
@@ -1031,7 +1031,7 @@ __device__ __forceinline__ void pt_tiles(const PaArgs& a, char* s_buf, int* s_lo
         const char* from = a.un + at * S::kStep + wave * SHARE * 1024 + lane * 16;
 #pragma unroll
         for (int i = 0; i < SHARE; ++i) raw[i] = *reinterpret_cast<const kh_i32x4*>(from + i * 1024);
-        nan2 = a.un_nan[at * (2 * NG) + (lane & (2 * NG - 1))];
+        nan2 = a.un_nan[at * (TV * NG) + (lane & (TV * NG - 1))];
       };
       const auto place = [&](int st) {
         char* to = s_buf + (st & 1) * S::kStep + wave * SHARE * 1024 + lane * 16;
@@ -1155,18 +1155,21 @@ __device__ __forceinline__ void pt_tiles(const PaArgs& a, char* s_buf, int* s_lo
           any = __ballot(nan0 != 0) != 0;
         } else {
 #pragma unroll
-          for (int gi = 0; gi < NG; ++gi) any |= s_nan[st & 1][gi][0] | s_nan[st & 1][gi][1];
+          for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+            for (int tb = 0; tb < TV; ++tb) any |= s_nan[st & 1][gi][tb];
         }
         if (!__builtin_amdgcn_readfirstlane(any)) return;
         int tok = st * KEYS;
         asm volatile("" : "+s"(tok));  // keeps this behind its branch
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi) {
-          uint64_t mask;
-          if constexpr (UN)
-            mask = (uint32_t)__builtin_amdgcn_readlane(nan0, 2 * gi) |
-                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane(nan0, 2 * gi + 1) << 32;
-          else mask = s_nan[st & 1][gi][0] | (uint64_t)s_nan[st & 1][gi][1] << 32;
+          uint64_t mask = 0;
+#pragma unroll
+          for (int tb = 0; tb < TV; ++tb) {
+            if constexpr (UN) mask |= (uint64_t)(uint32_t)__builtin_amdgcn_readlane(nan0, TV * gi + tb) << (32 * tb);
+            else mask |= (uint64_t)s_nan[st & 1][gi][tb] << (32 * tb);
+          }
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
             const int from = max(lo[c] - tok, 0), to = min(hi[c] - tok, KEYS);  // of the step's positions
@@ -1290,7 +1293,7 @@ template <int D, int KT, bool UN>
 __global__ __launch_bounds__((64 * PtShape<D, KT>::NW), 2) void paged_tile_kernel(PaArgs a) {
   extern __shared__ __align__(16) char s_buf[];
   __shared__ int s_lo[PtShape<D, KT>::NW], s_hi[PtShape<D, KT>::NW];
-  __shared__ uint32_t s_nan[2][D / kKvGroup][2];  // positions whose value group stands for NaN
+  __shared__ uint32_t s_nan[2][D / kKvGroup][PtShape<D, KT>::TV];  // positions whose value group stands for NaN
   uint32_t id = blockIdx.x;
   const int h = (int)(id % (uint32_t)a.nkv);
   id /= (uint32_t)a.nkv;
@@ -1427,12 +1430,12 @@ static int pa_waves(int d, int dtype) {
 }
 static int pa_fill(int d, int dtype) { return dtype == KH_DT_F32 ? pa_fill_t<float>(d) : pa_fill_t<uint16_t>(d); }
 struct PtSize {
-  int keys, step, rows, fill;  // positions of a step, their bytes, rows of a block, blocks that the chip holds
+  int keys, step, masks, rows, fill;  // positions of a step, their bytes and their masks', rows of a block, blocks that the chip holds
 };
 template <int D, int KT>
 static PtSize pt_size_dk() {
   using S = PtShape<D, KT>;
-  return {S::KEYS, S::kStep, S::RB, 256 * 8 / S::NW};
+  return {S::KEYS, S::kStep, S::NG * S::TV * 4, S::RB, 256 * 8 / S::NW};
 }
 template <int D>
 static PtSize pt_size_d(bool lse) {
@@ -1496,7 +1499,7 @@ static PaSpace pa_space(const PaPlan& p, int64_t rows, int64_t batch, int nkv, i
   s.ml = parts * 4 * d;
   s.un = (s.ml + parts * 8 + 15) / 16 * 16;
   s.nan = s.un + steps * pt_size(d, lse).step;
-  s.bytes = s.nan + steps * (d / kKvGroup) * 8;
+  s.bytes = s.nan + steps * pt_size(d, lse).masks;
   return s;
 }
 

@@ -49,3 +49,44 @@ def test_weights_by_the_lengths(kh, heads, kv, dim, lens, window):
     for guess in (None, max(lens), 64, 4096, 10 ** 5):
         hold(c, c.run(window=window, max_len=guess), window=window)
         hold(c, c.run(window=window, max_len=guess, max_rows=1, return_lse=False), window=window)
+
+
+# ---------------------------------------------------------------- positions unpacked ahead (BF16 tiles of many rows)
+def unpacked(c, most_rows, most_len, lse):
+    """(bytes of unpacked positions, bytes of their masks) where the plan takes that path in one part, as its workspace
+    says: steps of 64 positions (32 of 256-wide heads with the log-sum-exp) of values, and of keys in one or two terms,
+    and one bit of 32 positions for each group of 32 elements."""
+    keys = 32 if c.dim == 256 and lse else 64
+    steps = -(-most_len // keys) * len(c.rows) * c.kv
+    step, masks = keys * c.dim * 2 * (3 if lse else 2), c.dim // 32 * (keys // 32) * 4
+    need = c.cache._workspace(2, sum(c.rows), len(c.rows), c.heads, most_rows, most_len, 1 if lse else 0)
+    assert need == steps * (step + masks), (need, steps, step, masks)
+    return steps * step, steps * masks
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lse", [False, True])
+def test_masks_are_written_whole(kh, dim, lse):
+    """No word of a workspace is read that was not written: every mask word of a whole sequence is, and the bits that
+    lay there before do not matter."""
+    from klearu_amd import _lib
+    c = Case(BF16, 512, 4, dim, 64, [210], [704])
+    c.v[0][5, 1, 40] = float("nan")
+    c.cache.append(c.k[0].cuda(), c.v[0].cuda(), torch.tensor([0, 704]).cuda(), torch.zeros(1, dtype=torch.int64).cuda(), c.table)
+    data, masks = unpacked(c, 210, 704, lse)
+    q, got = c.q.cuda(), []
+    for fill in (0x5A, 0x00, 0xFF):
+        ws = torch.full((data + masks,), fill, dtype=torch.uint8, device="cuda")
+        out = torch.zeros_like(q)
+        l = torch.zeros(210, 512, device="cuda") if lse else None
+        rc = _lib.load().kh_paged_kv_attention(
+            c.cache._h, 2, q.data_ptr(), 512 * dim, dim, 512, 210, c.off.data_ptr(), 1, c.len.data_ptr(), c.table.data_ptr(),
+            c.table.shape[1], c.table.shape[1], 210, 704, dim ** -0.5, 1, 0, None, 0, out.data_ptr(), 512 * dim, dim,
+            None if l is None else l.data_ptr(), ws.data_ptr(), data + masks, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        torch.cuda.synchronize()
+        assert (ws[data:].view(torch.int32) != 0x5A5A5A5A).all()
+        got.append((out, l))
+    for o, l in got[1:]:
+        assert torch.equal(o.view(torch.int16), got[0][0].view(torch.int16)) and (l is None or torch.equal(l, got[0][1]))
+    assert torch.isnan(got[0][0]).any()
