@@ -68,6 +68,10 @@ inline int check_device(int device, const char* what) {
     if (dev_rc_ != KH_OK) return dev_rc_;                    \
   } while (0)
 
+// Threads that a grid may have along x: of more the launch keeps the lower 32 bits of
+// their number, and reports nothing.
+constexpr int64_t kGridThreads = ((int64_t)1 << 32) - 1;
+
 // What the attention kernels of a head_dim need of the current device.
 int paged_attn_prepare(int d);
 

@@ -12,6 +12,7 @@
 // 128, 138 MB with the table: 24.7 us, 5.6 TB/s, a copy of 4 GiB runs at 4.8; 2049 f32 rows
 // of 32 heads of 64, interleaved, half of a head rotated: 7.5 us) and by the launch for one
 // (2.2 us of kernel, 6.8 us a call).
+#include <algorithm>
 #include <cmath>
 #include <new>
 
@@ -19,10 +20,13 @@
 
 namespace kh {
 
-__global__ void rope_table_kernel(const double* __restrict__ freq, int half, int64_t max_pos, double mag,
+constexpr int64_t kMostBlocks = kGridThreads / 256;  // larger work is launched in parts
+
+// Entries first and later of the table of n.
+__global__ void rope_table_kernel(const double* __restrict__ freq, int half, int64_t first, int64_t n, double mag,
                                   float2* __restrict__ table) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= max_pos * half) return;
+  const int64_t i = first + (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
   const double a = (double)(i / half) * freq[i % half];
   double s, c;
   sincos(a, &s, &c);
@@ -133,24 +137,27 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a, int half_layo
 }
 
 template <typename T>
-static int rope_launch(const RopeArgs& a, int layout, bool vec, hipStream_t st) {
-  if (vec) {
-    const int pieces = layout == KH_ROPE_HALF ? a.rot / 16 + (a.copy ? (a.dim - a.rot) / 8 : 0)
-                                              : (a.copy ? a.dim : a.rot) / 8;
-    const int64_t blocks = (a.rows * a.heads * pieces + 255) / 256;
-    KH_CHECK_ARG(blocks < (int64_t)1 << 31, "too many rows for one call");
-    if (layout == KH_ROPE_HALF)
-      hipLaunchKernelGGL((rope_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, st, a, pieces);
+static int rope_launch(const RopeArgs& all, int layout, bool vec, hipStream_t st) {
+  const int pieces = !vec ? all.rot / 2 + (all.copy ? all.dim - all.rot : 0)
+                     : layout == KH_ROPE_HALF ? all.rot / 16 + (all.copy ? (all.dim - all.rot) / 8 : 0)
+                                              : (all.copy ? all.dim : all.rot) / 8;
+  // rows of a launch; one row is below 2^32 threads (65536 heads of fewer than 65536 pieces)
+  const int64_t most = kMostBlocks * 256 / ((int64_t)all.heads * pieces);
+  for (int64_t t0 = 0; t0 < all.rows; t0 += most) {
+    RopeArgs a = all;
+    a.rows = all.rows - t0 < most ? all.rows - t0 : most;
+    a.x = static_cast<const T*>(all.x) + t0 * all.xs;
+    a.y = static_cast<T*>(all.y) + t0 * all.ys;
+    a.pos = all.pos + t0;
+    const unsigned blocks = (unsigned)((a.rows * a.heads * pieces + 255) / 256);
+    if (!vec)
+      hipLaunchKernelGGL(rope_any_kernel<T>, dim3(blocks), dim3(256), 0, st, a, layout == KH_ROPE_HALF ? 1 : 0, pieces);
+    else if (layout == KH_ROPE_HALF)
+      hipLaunchKernelGGL((rope_kernel<T, true>), dim3(blocks), dim3(256), 0, st, a, pieces);
     else
-      hipLaunchKernelGGL((rope_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, st, a, pieces);
-  } else {
-    const int units = a.rot / 2 + (a.copy ? a.dim - a.rot : 0);
-    const int64_t blocks = (a.rows * a.heads * units + 255) / 256;
-    KH_CHECK_ARG(blocks < (int64_t)1 << 31, "too many rows for one call");
-    hipLaunchKernelGGL(rope_any_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, a,
-                       layout == KH_ROPE_HALF ? 1 : 0, units);
+      hipLaunchKernelGGL((rope_kernel<T, false>), dim3(blocks), dim3(256), 0, st, a, pieces);
+    KH_LAUNCHED();
   }
-  KH_LAUNCHED();
   return KH_OK;
 }
 
@@ -216,11 +223,12 @@ extern "C" int kh_rope_create(int rot_dim, int64_t max_pos, int layout, double t
     if (!r->table || !r->err || !freq_dev) return KH_ERR_ALLOC;
     KH_HIP(hipMemset(r->err, 0, sizeof(int)));
     KH_HIP(hipMemcpy(freq_dev, freq, sizeof(double) * half, hipMemcpyHostToDevice));
-    const int64_t blocks = (n + 255) / 256;
-    KH_CHECK_ARG(blocks < (int64_t)1 << 31, "max_pos * rot_dim too large");
-    hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)blocks), dim3(256), 0, nullptr, freq_dev, half, max_pos,
-                       magnitude, r->table);
-    KH_LAUNCHED();
+    for (int64_t i = 0; i < n; i += kMostBlocks * 256) {
+      const int64_t blocks = std::min((n - i + 255) / 256, kMostBlocks);
+      hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)blocks), dim3(256), 0, nullptr, freq_dev, half, i, n,
+                         magnitude, r->table);
+      KH_LAUNCHED();
+    }
     KH_HIP(hipStreamSynchronize(nullptr));
     return KH_OK;
   };
