@@ -1326,16 +1326,16 @@ __global__ __launch_bounds__((64 * PtShape<D, KT>::NW), 2) void paged_tile_kerne
     pt_tiles<D, KT, false>(a, s_buf, s_lo, s_hi, s_nan, b, h, split, tile0, every, o0, o1, L);
 }
 
-// Joins the parts of each row: W waves a (row, head), four elements a lane, so
+// Joins the parts of each row from first_row on: W waves a (row, head), four elements a lane, so
 // that 256 / D parts of a wave are in flight at once.  4 us, latency: the parts come
 // from other XCDs' caches.
 template <int D, typename T, int W>
-__global__ __launch_bounds__(256) void paged_join_kernel(PaArgs a) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PaArgs a, int64_t first_row) {
   constexpr int C = D / 4, NS = 64 / C;
   __shared__ __align__(16) float s_acc[W > 1 ? W : 1][D];
   const int lane = threadIdx.x & 63, c = lane % C, sub = lane / C;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  const int64_t row = first_row + (W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave);
   const uint32_t t = (uint32_t)(row / a.nh);
   if (t >= a.rows) return;
   const int head = (int)(row - (int64_t)t * a.nh);
@@ -1419,6 +1419,7 @@ constexpr int64_t kPtMinWork = 3000;  // positions of a full chip of 16-row tile
 constexpr int kPtUnpackTiles = 3;
 constexpr int64_t kPtUnpackWork = 1 << 18;           // row tiles times positions
 constexpr int64_t kPtUnpackMost = (int64_t)1 << 30;  // bytes of them
+constexpr int64_t kPtMostBlocks = (int64_t)1 << 20;  // tiles of more than 64 sequences, as guessed
 template <typename T>
 static int pa_fill_t(int d) {
   return d == 64 ? PaShape<64, T>::kFill : d == 128 ? PaShape<128, T>::kFill : PaShape<256, T>::kFill;
@@ -1460,10 +1461,12 @@ static PaPlan pa_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int
   p.many = dtype == KH_DT_BF16 && max_rows * gs >= kPtMinRows &&
            (tiles16 > held || (max_len > 0 && tiles16 > kPtMinWork * held / max_len));
   const PtSize z = pt_size(c->d, lse);
+  // a block of its own for each tile that the guess allows, as far as a grid goes: past
+  // that a block takes every tiles-th
+  const int64_t most_tiles = p.many && batch > 64 ? kPtMostBlocks / (batch * c->nkv) : 65535 / batch;
+  if (p.many && most_tiles < 1) p.many = false;
   const int64_t rb = p.many ? z.rows : 16;
-  p.tiles = (max_rows * gs + rb - 1) / rb;
-  if (p.tiles < 1) p.tiles = 1;
-  if (p.tiles > 65536) p.tiles = 65536;
+  p.tiles = std::max<int64_t>(std::min<int64_t>((max_rows * gs + rb - 1) / rb, most_tiles), 1);
   p.base = batch * c->nkv * p.tiles;
   const int64_t fill = p.many ? z.fill : pa_fill(c->d, dtype);
   if (p.many && batch <= 64) p.base = c->nkv * ((rows * gs + batch * (rb - 1)) / rb);  // as pt_tile counts them
@@ -1534,10 +1537,14 @@ static int pa_launch(const PaArgs& a, bool many, int64_t blocks, hipStream_t st)
     constexpr int lds = PaShape<D, T>::kLds;
     hipLaunchKernelGGL((paged_rows_kernel<D, T>), g, blk, lds, st, a);
   }
-  if (a.nsplit > 16)
-    hipLaunchKernelGGL((paged_join_kernel<D, T, 4>), dim3((unsigned)(a.rows * a.nh)), dim3(256), 0, st, a);
-  else if (a.nsplit > 1)
-    hipLaunchKernelGGL((paged_join_kernel<D, T, 1>), dim3((unsigned)((a.rows * a.nh + 3) / 4)), dim3(256), 0, st, a);
+  if (a.nsplit > 1) {
+    const int64_t all = a.rows * a.nh, each = a.nsplit > 16 ? 1 : 4, most = kGridThreads / 256 * each;
+    for (int64_t row = 0; row < all; row += most) {
+      const dim3 g((unsigned)((std::min(all - row, most) + each - 1) / each));
+      if (each == 1) hipLaunchKernelGGL((paged_join_kernel<D, T, 4>), g, dim3(256), 0, st, a, row);
+      else hipLaunchKernelGGL((paged_join_kernel<D, T, 1>), g, dim3(256), 0, st, a, row);
+    }
+  }
   KH_LAUNCHED();
   return KH_OK;
 }
@@ -1630,8 +1637,9 @@ extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void
     return KH_ERR_CAPACITY;
   }
   KH_CHECK_ARG((reinterpret_cast<uintptr_t>(ws_dev) & 15) == 0, "the workspace must be 16-byte aligned");
-  const int64_t blocks = p.base * p.nsplit;
-  KH_CHECK_ARG(blocks < (int64_t)1 << 31 && rows * num_heads < (int64_t)1 << 31, "too many rows for one call");
+  const int64_t blocks = p.base * p.nsplit;  // of many rows' tiles
+  KH_CHECK_ARG((!p.many || blocks <= kGridThreads / 512) && rows * num_heads < (int64_t)1 << 31,
+               "too many rows for one call");
   KH_ON_DEVICE(c->device, "the cache");
   PaArgs a;
   a.pool = c->pool;

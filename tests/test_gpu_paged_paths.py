@@ -13,31 +13,39 @@ from test_gpu_paged_attn import BF16, F32, Case
 pytestmark = pytest.mark.gpu
 
 
-def hold(c, got, causal=True, window=0, many=False, on=None):
-    """got is `out` or (out, lse) of the case's rows: every element within its own tolerance."""
-    out, lse = (None if x is None else x.double().cpu().numpy() for x in ((got, None) if torch.is_tensor(got) else got))
-    at = 0
-    for n, length, k, v in zip(c.rows, c.lens, c.k, c.v):
-        rows, at = slice(at, at + n), at + n
+def hold(c, got, causal=True, window=0, many=False, on=None, seqs=None, heads=None, status=True):
+    """got is `out` or (out, lse) of the case's rows: every element within its own tolerance, of all sequences and heads
+    or of those given."""
+    out, lse = (None if x is None else x for x in ((got, None) if torch.is_tensor(got) else got))
+    at = np.concatenate([[0], np.cumsum(c.rows)])
+    hs = list(range(c.heads)) if heads is None else heads
+    for b in range(len(c.rows)) if seqs is None else seqs:
+        n, length, rows = c.rows[b], c.lens[b], slice(at[b], at[b + 1])
         if n == 0:
             continue
         assert 1 <= n <= length
         fine = not many and min(length, window or length) <= 1024
-        o, l, to, tl = attention(c.q[rows].double().numpy(), k.float().numpy(), v.float().numpy(), c.dim ** -0.5, causal,
-                                 window, c.dtype == BF16, many, fine)
-        if on is not None:
-            off = ~on[rows]
-            o[off], l[off], to[off], tl[off] = 0, -np.inf, 0, 0
-        assert (np.isnan(out[rows]) == np.isnan(o)).all()
-        there = ~np.isnan(o)
-        d = np.abs(out[rows] - o)
-        assert (d[there] <= to[there]).all(), (length, float(np.max(np.where(there, d / np.where(to > 0, to, 1), 0))))
-        if lse is not None:
-            some = np.isfinite(l)
-            assert (np.isnan(lse[rows]) == np.isnan(l)).all()
-            assert (lse[rows][~some & ~np.isnan(l)] == -np.inf).all()
-            assert (np.abs(lse[rows][some] - l[some]) <= tl[some]).all()
-    c.cache.status()
+        y = out[rows][:, hs].double().cpu().numpy()
+        z = None if lse is None else lse[rows][:, hs].double().cpu().numpy()
+        q, k, v = c.q[rows].double().numpy(), c.k[b].float().numpy(), c.v[b].float().numpy()
+        for i, h in enumerate(hs):
+            g = slice(h * c.kv // c.heads, h * c.kv // c.heads + 1)
+            o, l, to, tl = (x[:, 0] for x in attention(q[:, h:h + 1], k[:, g], v[:, g], c.dim ** -0.5, causal, window,
+                                                       c.dtype == BF16, many, fine))
+            if on is not None:
+                off = ~on[rows, h]
+                o[off], l[off], to[off], tl[off] = 0, -np.inf, 0, 0
+            assert (np.isnan(y[:, i]) == np.isnan(o)).all(), (b, h)
+            there = ~np.isnan(o)
+            d = np.abs(y[:, i] - o)
+            assert (d[there] <= to[there]).all(), (b, length, h, float(np.max(np.where(there, d / np.where(to > 0, to, 1), 0))))
+            if z is not None:
+                some = np.isfinite(l)
+                assert (np.isnan(z[:, i]) == np.isnan(l)).all(), (b, h)
+                assert (z[:, i][~some & ~np.isnan(l)] == -np.inf).all(), (b, h)
+                assert (np.abs(z[:, i][some] - l[some]) <= tl[some]).all(), (b, h)
+    if status:
+        c.cache.status()
 
 
 @pytest.mark.parametrize("heads,kv,dim", [(4, 4, 128), (8, 2, 64), (6, 2, 256)])
@@ -90,3 +98,36 @@ def test_masks_are_written_whole(kh, dim, lse):
     for o, l in got[1:]:
         assert torch.equal(o.view(torch.int16), got[0][0].view(torch.int16)) and (l is None or torch.equal(l, got[0][1]))
     assert torch.isnan(got[0][0]).any()
+
+
+# ---------------------------------------------------------------- grids past a launch's threads
+def test_guess_of_the_rows_past_one_grid(kh):
+    """1000 sequences of 33 to 35 rows, and every row of the call as the guess of one sequence's: 2^32 threads of tiles."""
+    n = [33 + b % 3 for b in range(1000)]
+    c = Case(BF16, 64, 8, 64, 16, n, [r + b % 5 for b, r in enumerate(n)])
+    want = c.run(max_rows=35, max_len=40)
+    hold(c, want, many=True, seqs=[0, 1, 500, 998, 999], heads=[0, 20, 63])
+    for guess in (sum(n), 10 ** 6):
+        got = c.run(max_rows=guess, max_len=40)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_guess_of_the_rows_of_many_sequences(kh):
+    """20000 sequences of two rows, f32, and that guess: more row tiles than a grid's 2^31 blocks."""
+    c = Case(F32, 64, 8, 64, 16, [2] * 20000, [2 + b % 4 for b in range(20000)])
+    hold(c, c.run(max_rows=40000, max_len=16), seqs=[0, 1, 2, 9999, 19998, 19999], heads=[0, 31, 63])
+
+
+def test_padding_past_one_grid_of_the_join(kh):
+    """One row behind 2^17 rows of padding, in 17 parts: 2^24 + 128 rows of heads to join, 75 GB of workspace."""
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 100 GiB of device memory")
+    c = Case(F32, 128, 1, 64, 64, [1], [4352])
+    rows = 2 ** 17 + 1
+    assert c.cache._workspace(0, rows, 1, 128, 1, 4352, 0) == rows * 128 * 17 * (4 * 64 + 8)
+    q = c.q.cuda().expand(rows, 128, 64)
+    out = torch.full((rows, 128, 64), 7.0, device="cuda")
+    off = torch.tensor([rows - 1, rows], device="cuda")
+    c.cache.attention(q, off, c.len, c.table, max_rows=1, max_len=4352, out=out)
+    hold(c, out[-1:])
+    assert bool((out[:-1] == 7).all())
