@@ -409,8 +409,10 @@ struct GatherArgs {
 
 // The inverse: the same quads and lanes.  Of the four lanes that need the same eight
 // u16 of a value's codes each loads two, and they exchange them.  14460 rows of 8 heads of
-// 128 to BF16 (18.5 MB in, 59 MB out): 21.7 us, 3.6 TB/s, 3.6 us for one.  The rows leave
-// past the caches (22.8 us through them, and the append behind them 32.4 instead of 28.9).
+// 128 to BF16 (18.5 MB in, 59 MB out): 22.0 us, 3.5 TB/s, 3.6 us for one; to f32 (118 MB
+// out) 27.5 us, 5.0 TB/s.  The rows stay in the caches for whoever reads them next: with a
+// copy of them behind, 40.8 us and to f32 76.4, where stores past the caches took 44.9 and
+// 88.8 (alone 21.1 and 39.5).
 template <typename T, int D, bool VAL>
 __device__ __forceinline__ void gather_part(const GatherArgs& a, int units, int hpu, int* s_q, int* s_wsum, int* s_tot) {
   using P = KvParts<D>;
@@ -461,7 +463,7 @@ __device__ __forceinline__ void gather_part(const GatherArgs& a, int units, int 
           f[2 * i] = s * (float)(VAL ? (q[i] >> (4 * n)) & 15 : q[i] & 15) + m;
           f[2 * i + 1] = s * (float)(VAL ? (q[i] >> (4 * n + 16)) & 15 : (q[i] >> 4) & 15) + m;
         }
-        if (act) stream8(y0 + k * TP * srow, f);
+        if (act) store8(y0 + k * TP * srow, true, f);
       }
     }
   });

@@ -143,20 +143,4 @@ __device__ __forceinline__ void store8(float* p, bool vec, const float (&f)[8]) 
   }
 }
 
-// store8 of aligned rows that nothing on the chip reads soon.
-__device__ __forceinline__ void stream8(uint16_t* p, const float (&f)[8]) {
-  typedef uint32_t v4 __attribute__((ext_vector_type(4)));
-  v4 v;
-  v.x = f32_to_bf16(f[0]) | (uint32_t)f32_to_bf16(f[1]) << 16;
-  v.y = f32_to_bf16(f[2]) | (uint32_t)f32_to_bf16(f[3]) << 16;
-  v.z = f32_to_bf16(f[4]) | (uint32_t)f32_to_bf16(f[5]) << 16;
-  v.w = f32_to_bf16(f[6]) | (uint32_t)f32_to_bf16(f[7]) << 16;
-  __builtin_nontemporal_store(v, reinterpret_cast<v4*>(p));
-}
-__device__ __forceinline__ void stream8(float* p, const float (&f)[8]) {
-  typedef float v4 __attribute__((ext_vector_type(4)));
-  __builtin_nontemporal_store(v4{f[0], f[1], f[2], f[3]}, reinterpret_cast<v4*>(p));
-  __builtin_nontemporal_store(v4{f[4], f[5], f[6], f[7]}, reinterpret_cast<v4*>(p) + 1);
-}
-
 }  // namespace kh
