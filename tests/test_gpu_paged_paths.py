@@ -7,8 +7,8 @@ import numpy as np
 import pytest
 import torch
 
-from paged_ref import attention
-from test_gpu_paged_attn import BF16, F32, Case
+from paged_ref import attention, offsets
+from test_gpu_paged_attn import BF16, F32, SHAPES, Case
 
 pytestmark = pytest.mark.gpu
 
@@ -60,15 +60,16 @@ def test_weights_by_the_lengths(kh, heads, kv, dim, lens, window):
 
 
 # ---------------------------------------------------------------- positions unpacked ahead (BF16 tiles of many rows)
-def unpacked(c, most_rows, most_len, lse):
-    """(bytes of unpacked positions, bytes of their masks) where the plan takes that path in one part, as its workspace
-    says: steps of 64 positions (32 of 256-wide heads with the log-sum-exp) of values, and of keys in one or two terms,
-    and one bit of 32 positions for each group of 32 elements."""
+def unpacked(c, most_rows, most_len, lse, parts=0):
+    """(bytes of unpacked positions, bytes of their masks) where the plan takes that path in one part, or in so many, as
+    its workspace says: steps of 64 positions (32 of 256-wide heads with the log-sum-exp) of values, and of keys in one or
+    two terms, and one bit of 32 positions for each group of 32 elements."""
     keys = 32 if c.dim == 256 and lse else 64
     steps = -(-most_len // keys) * len(c.rows) * c.kv
     step, masks = keys * c.dim * 2 * (3 if lse else 2), c.dim // 32 * (keys // 32) * 4
     need = c.cache._workspace(2, sum(c.rows), len(c.rows), c.heads, most_rows, most_len, 1 if lse else 0)
-    assert need == steps * (step + masks), (need, steps, step, masks)
+    joined = -(-sum(c.rows) * c.heads * parts * (4 * c.dim + 8) // 16) * 16
+    assert need == joined + steps * (step + masks), (need, joined, steps, step, masks)
     return steps * step, steps * masks
 
 
@@ -98,6 +99,147 @@ def test_masks_are_written_whole(kh, dim, lse):
     for o, l in got[1:]:
         assert torch.equal(o.view(torch.int16), got[0][0].view(torch.int16)) and (l is None or torch.equal(l, got[0][1]))
     assert torch.isnan(got[0][0]).any()
+
+
+def again(c):
+    """The case's keys and values appended once more, after a change."""
+    c.cache.append(torch.cat(c.k).cuda(), torch.cat(c.v).cuda(), offsets(c.lens).cuda(),
+                   torch.zeros(len(c.lens), dtype=torch.int64).cuda(), c.table)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 70), (False, 0)])
+@pytest.mark.parametrize("lse", [False, True])
+def test_unpacked_in_one_part(kh, dim, page, causal, window, lse):
+    """Whole positions, then groups that stand for NaN; the guess covers every sequence, or all but the longest one."""
+    rows, lens, heads = [120, 0, 60, 40], [700, 9, 60, 300], [0, 127, 130, 300, 511]
+    c = Case(BF16, 512, 4, dim, page, rows, lens)
+    for bad in (False, True):
+        if bad:
+            c.v[0][690, 1, 40], c.v[0][100, 3, dim - 1] = float("nan"), float("inf")
+            c.v[2][30, 0, 33], c.k[3][280, 2, 5] = -float("inf"), float("nan")
+            again(c)
+        for guess in (704, 640):
+            unpacked(c, 120, guess, lse)
+            got = c.run(causal=causal, window=window, max_rows=120, max_len=guess, return_lse=lse)
+            hold(c, got, causal, window, many=True, heads=heads)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lse", [False, True])
+def test_unpacked_in_parts(kh, dim, lse):
+    """The same where the positions are cut in three."""
+    n = 150 if dim == 256 else 330
+    c = Case(BF16, 64, 4, dim, 32, [n], [1500])
+    c.v[0][1400, 2, 3], c.v[0][5, 0, 33] = float("nan"), float("nan")
+    again(c)
+    unpacked(c, n, 3500, lse, parts=3)
+    for window in (0, 200):
+        got = c.run(max_rows=n, max_len=3500, window=window, return_lse=lse)
+        hold(c, got, window=window, many=True, heads=[0, 15, 17, 40, 63])
+
+
+def without(c, b, first, count):
+    """The case as if sequence b had no positions first .. first + count - 1 (all its rows are behind them)."""
+    assert first + count <= c.lens[b] - c.rows[b]
+    keep = [i for i in range(c.lens[b]) if not first <= i < first + count]
+    c.k[b], c.v[b], c.lens[b] = c.k[b][keep], c.v[b][keep], len(keep)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lse", [False, True])
+@pytest.mark.parametrize("guess", [800, 2400])
+def test_tiles_past_one_round_of_pages(kh, dim, lse, guess):
+    """2400 positions in one part, where the tiles hold the pages of 1024 at a time: unpacked by each tile (a guess that
+    is too small) and ahead; then pages of the first, second and third round that are not there."""
+    from klearu_amd import KlearuError
+    c = Case(BF16, 128, 4, dim, 16, [300], [2400])
+    if guess == 2400:
+        unpacked(c, 300, guess, lse)
+    else:
+        assert c.cache._workspace(2, 300, 1, 128, 300, guess, 1 if lse else 0) == 0
+    heads, most = [0, 31, 33, 80, 127], dict(max_rows=300, max_len=guess, return_lse=lse)
+    hold(c, c.run(**most), many=True, heads=heads)
+    for at in (2064, 1520, 1024, 1008, 16):
+        c.table[0, at // 16] = c.cache.num_pages
+        got = c.run(**most)
+        with pytest.raises(KlearuError, match="page id"):
+            c.cache.status()
+        without(c, 0, at, 16)
+        hold(c, got, many=True, heads=heads, status=False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 64])
+def test_single_rows_past_one_round_of_pages(kh, dtype, dim, page):
+    """20000 and 17001 positions in one part, where a wave holds the pages of 64 of its steps at a time (8192 or 16384
+    positions of the block's); then pages of each round that are not there."""
+    from klearu_amd import KlearuError
+    c = Case(dtype, 4, 2, dim, page, [1, 3], [20000, 17001])
+    assert c.cache._workspace(0 if dtype == F32 else 2, 4, 2, 4, 3, 100, 1) == 0
+    hold(c, c.run(max_rows=3, max_len=100))
+    for at in (19904, 16384, 8128):
+        c.table[0, at // page] = -1
+        got = c.run(max_rows=3, max_len=100)
+        with pytest.raises(KlearuError, match="page id"):
+            c.cache.status()
+        without(c, 0, at, page)
+        hold(c, got, seqs=[0], heads=[0, 3], status=False)
+
+
+# ---------------------------------------------------------------- single rows, weights in one term and in two
+SHORT = [1, 2, 15, 16, 17, 31, 33, 64, 65, 128, 129, 511, 513, 1023, 1024]
+LONG = [1025, 1057, 2048, 2049]
+
+
+@pytest.mark.parametrize("heads,kv,dim", SHAPES)
+@pytest.mark.parametrize("lens", [SHORT, LONG])
+def test_terms_single_rows(kh, heads, kv, dim, lens):
+    c = Case(BF16, heads, kv, dim, 32, [1] * len(lens), lens)
+    hold(c, c.run())
+    hold(c, c.run(max_len=max(lens), return_lse=False))
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 4, 128), (8, 2, 64), (6, 2, 256), (3, 1, 128), (40, 2, 64)])
+@pytest.mark.parametrize("rows,lens", [([3, 1, 2], [3, 700, 1024]), ([1, 3, 2], [1025, 1500, 1060])])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 1024), (True, 1025), (True, 5)])
+def test_terms_few_rows(kh, heads, kv, dim, rows, lens, causal, window):
+    c = Case(BF16, heads, kv, dim, 16, rows, lens)
+    hold(c, c.run(causal=causal, window=window), causal, window)
+    n, rng = sum(rows), np.random.default_rng(3)
+    sel = np.stack([rng.permutation(heads)[: max(1, heads // 3)] for _ in range(n)]).astype(np.int32)
+    on = np.zeros((n, heads), bool)
+    np.put_along_axis(on, sel.astype(np.int64), True, 1)
+    hold(c, c.run(causal=causal, window=window, heads=torch.from_numpy(sel).cuda()), causal, window, on=on)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (4, 2, 128), (6, 2, 256)])
+@pytest.mark.parametrize("lens", [[200, 150], [1300, 1200]])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_terms_not_finite(kh, dtype, heads, kv, dim, lens, bad):
+    """A value's group and a key that are not finite, with rows before and behind them; the same pages with finite rows
+    after that, and a shorter sequence over them."""
+    c = Case(dtype, heads, kv, dim, 16, [5, 1], list(lens))
+    k, v = [x.clone() for x in c.k], [x.clone() for x in c.v]
+    c.v[0][lens[0] - 3, 1, 40], c.v[1][3, 0, 0] = bad, bad
+    again(c)
+    hold(c, c.run())
+    hold(c, c.run(window=64), window=64)
+    c.k[0][lens[0] - 2, 0, 5] = bad
+    again(c)
+    hold(c, c.run())
+    c.k, c.v = k, v
+    again(c)
+    hold(c, c.run())
+    # the pages' last positions hold NaN, and no sequence reaches them
+    c.k[0][-40:], c.v[0][-40:] = bad, bad
+    again(c)
+    c.k[0], c.v[0], c.lens[0] = c.k[0][:-40], c.v[0][:-40], lens[0] - 40
+    c.len = torch.tensor(c.lens).cuda()
+    hold(c, c.run())
 
 
 # ---------------------------------------------------------------- grids past a launch's threads
