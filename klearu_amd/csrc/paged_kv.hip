@@ -608,6 +608,8 @@ extern "C" int kh_paged_kv_status(const kh_paged_kv* c) {
   KH_HIP(hipMemcpy(&bad, c->err, sizeof(int), hipMemcpyDeviceToHost));
   if (!bad) return KH_OK;
   KH_HIP(hipMemset(c->err, 0, sizeof(int)));
+  // cleared before any other stream records again: streams need not wait for the null stream
+  KH_HIP(hipStreamSynchronize(nullptr));
   set_error("%s%s", (bad & 1) ? "a position lay outside its sequence's page table; " : "",
             (bad & 2) ? "a page id lay outside the pool; " : "");
   return KH_ERR_ARG;

@@ -250,6 +250,8 @@ extern "C" int kh_rope_status(const kh_rope* r) {
   KH_HIP(hipMemcpy(&bad, r->err, sizeof(int), hipMemcpyDeviceToHost));
   if (!bad) return KH_OK;
   KH_HIP(hipMemset(r->err, 0, sizeof(int)));
+  // cleared before any other stream records again: streams need not wait for the null stream
+  KH_HIP(hipStreamSynchronize(nullptr));
   set_error("a row's position was not below max_pos %lld", (long long)r->max_pos);
   return KH_ERR_ARG;
 }
