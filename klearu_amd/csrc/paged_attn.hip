@@ -1664,7 +1664,7 @@ extern "C" int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void
   a.gs = num_heads / c->nkv;
   a.c1 = scale * kLog2e;
   a.causal = causal ? 1 : 0;
-  a.window = window;
+  a.window = window <= INT32_MAX ? window : 0;  // wider than a table hides nothing; differences from it stay in 64 bits
   a.out = out_dev;
   a.os = out_row_stride;
   a.oh = out_head_stride;

@@ -242,6 +242,36 @@ def test_terms_not_finite(kh, dtype, heads, kv, dim, lens, bad):
     hold(c, c.run())
 
 
+@pytest.mark.parametrize("window", [2 ** 31, 2 ** 62, 2 ** 63 - 1])
+def test_windows_past_every_length(kh, window):
+    """A window as wide as its type is none, for rows before the cache's first position too."""
+    c = Case(BF16, 512, 4, 64, 16, [120, 0, 60, 40], [100, 9, 60, 300])
+    unpacked(c, 120, 704, True)
+    d = Case(F32, 8, 2, 64, 16, [5, 1, 2, 1], [2, 4000, 700, 1300])
+    for x, dt, most in ((c, 2, dict(max_rows=120, max_len=704)), (d, 0, dict(max_rows=1, max_len=4000))):
+        want = x.run(**most)
+        # the workspace's memory holds no earlier call's parts or positions
+        need = x.cache._workspace(dt, sum(x.rows), len(x.rows), x.heads, most["max_rows"], most["max_len"], 1)
+        torch.full((need,), 0xFF, dtype=torch.uint8, device="cuda")
+        got = x.run(window=window, **most)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        x.cache.status()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_single_rows_of_many_sequences_in_parts(kh, dtype, dim):
+    """More than 64 sequences, each cut in the same number of parts; all share their first pages."""
+    n = 70
+    c = Case(dtype, 3, 1, dim, 16, [1] * n, [16 + (b * 97) % 2990 for b in range(n)])
+    c.table[1:, 0] = c.table[0, 0]
+    for b in range(1, n):
+        c.k[b][:16], c.v[b][:16] = c.k[0][:16], c.v[0][:16]
+    assert c.cache._workspace(0 if dtype == F32 else 2, n, n, 3, 1, 3005, 1) > 0
+    hold(c, c.run(max_rows=1, max_len=3005))
+    hold(c, c.run(max_rows=1, max_len=3005, window=900, return_lse=False), window=900)
+
+
 # ---------------------------------------------------------------- grids past a launch's threads
 def test_guess_of_the_rows_past_one_grid(kh):
     """1000 sequences of 33 to 35 rows, and every row of the call as the guess of one sequence's: 2^32 threads of tiles."""
