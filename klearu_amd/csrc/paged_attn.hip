@@ -6,14 +6,15 @@
 // over the positions j that the row sees: j < L, with `causal` j <= p, with a
 // window w also j > p - w.  A row that sees nothing gives 0 and -inf.
 //
-// The codes go into the matrix cores as they are.  A nibble c three bits up behind the bits
-// 0x418 is the BF16 number 16 + c, so with group sums A_g = sum_d q_d (16 + c_d)
-//   q . k = sum_g s_g A_g + sum_g (m_g - 16 s_g) Q_g,   Q_g = sum_{d in g} q_d
+// The codes go into the matrix cores as they are, as BF16 numbers B + c.  For BF16 rows B is
+// 16: a nibble three bits up behind the bits 0x418.  f32 rows convert the codes (B = 0): their
+// bits do not last through sums of the size of 16s.  With group sums A_g = sum_d q_d (B + c_d)
+//   q . k = sum_g s_g A_g + sum_g (m_g - B s_g) Q_g,   Q_g = sum_{d in g} q_d
 // where the second sum is one more product, of the (s, m) pairs as they lie in
-// the page with (-16 Q_g, Q_g) in three BF16 terms.  Values alike, with R the
+// the page with (-B Q_g, Q_g) in three BF16 terms.  Values alike, with R the
 // rounded products p_j s_jg that the matrix core takes:
-//   o_d = sum_j R_jg (16 + c_jd) - 16 sum_j R_jg + sum_j p_j m_jg
-// where the rounding of R cancels in the 16s.  The middle sum is one more
+//   o_d = sum_j R_jg (B + c_jd) - B sum_j R_jg + sum_j p_j m_jg
+// where the rounding of R cancels in the Bs.  The middle sum is one more
 // product with ones, per group: a group that stands for NaN touches no other.
 //
 // Row tiles are 16 rows of one kv head: the queries of its heads, of one
@@ -135,14 +136,17 @@ __device__ __forceinline__ kh_f32x4 mfma16(const uint4& a, const uint4& b, kh_f3
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
 }
 
-// Two codes (nibble n of each half of w) as BF16 numbers kBias + c: behind the bits of 16 a
-// nibble counts ones three bits up.  The bias leaves the sums again, with the rounding errors
-// of numbers of its size: 128, which needs a shift less for one nibble in four, left the
-// log-sum-exp of few positions off by 2e-6 of itself (16: under 1e-6 in 100 drawn calls, at
-// 1 to 2 % of the time of single rows).
-constexpr int kBias = 16;
+// Two codes (nibble n of each half of w) as BF16 numbers BIAS + c: two instructions a pair
+// behind the bits of 16, where a nibble counts ones three bits up, four by conversion.  The bias
+// leaves the sums again, with the rounding errors of numbers of its size.  Errors of 150 drawn
+// calls against 64 bits: f32 rows with 16 up to 1.2e-6 of the result where plain f32 has 4e-7,
+// with 0 up to 4.7e-7 at 1 to 3 % more time (1024 f32 rows of 32 heads of 128: 132 us, 129 with
+// 16); log-sum-exps of BF16 rows with 128 up to 2.3e-6, with 16 below 1e-6 at 1 to 2 %.
+template <int BIAS>
 __device__ __forceinline__ uint32_t codes2(uint32_t w, int n) {
-  return ((n == 0 ? w << 3 : w >> (4 * n - 3)) & 0x00780078u) | 0x41804180u;
+  if constexpr (BIAS == 16) return ((n == 0 ? w << 3 : w >> (4 * n - 3)) & 0x00780078u) | 0x41804180u;
+  const uint32_t x = (n & 1 ? w >> 4 : w) & 0x0f0f0f0fu;
+  return cvt_bf16x2((float)(x >> (n & 2 ? 8 : 0) & 0xffu), (float)(x >> (n & 2 ? 24 : 16) & 0xffu));
 }
 
 // Eight f32 in BF16 terms: x = t[0] + t[1] + ... to 8 more bits each.
@@ -301,6 +305,7 @@ template <int D, typename T, int NP>
 __device__ __forceinline__ void pa_tiles(const PaArgs& a, float* s_o, const PaLane<D>& lo_, const int32_t* __restrict__ table,
                                          int pre, int h, int split, int parts, int tile0, int64_t o0, int n, int64_t L) {
   constexpr int NG = D / kKvGroup, HN = D / 64, NF = D / 16, NW = PaShape<D, T>::NW;
+  constexpr int BIAS = sizeof(T) == 4 ? 0 : 16;
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1;  // terms of q: all of its bits
   constexpr int OS = PaShape<D, T>::kOS;
   float* s_m = s_o + NW * 16 * OS;
@@ -340,7 +345,7 @@ __device__ __forceinline__ void pa_tiles(const PaArgs& a, float* s_o, const PaLa
 
     float m = -INFINITY, l = 0.0f;
     kh_f32x4 o[NF], om;
-    float os[NG];  // of the lane's positions
+    float os[NG];  // sums of R of the lane's positions, where there is a bias
 #pragma unroll
     for (int f = 0; f < NF; ++f) o[f] = kh_f32x4{0, 0, 0, 0};
     om = kh_f32x4{0, 0, 0, 0};
@@ -405,7 +410,7 @@ __device__ __forceinline__ void pa_tiles(const PaArgs& a, float* s_o, const PaLa
           for (int j = 0; j < 4; ++j) {
             const float s = 4 * k + j < NG ? qsum[4 * k + j < NG ? 4 * k + j : 0] : 0.0f;
             e[2 * j] = s;
-            e[2 * j + 1] = -(float)kBias * s;
+            e[2 * j + 1] = -(float)BIAS * s;
           }
           uint4 tm[3];
           terms8<3>(e, tm);
@@ -434,7 +439,7 @@ __device__ __forceinline__ void pa_tiles(const PaArgs& a, float* s_o, const PaLa
 #pragma unroll
           for (int j = 0; j < NG; ++j) {
             const uint32_t w = x.kw[tt][j];
-            const uint4 kf = make_uint4(codes2(w, 0), codes2(w, 1), codes2(w, 2), codes2(w, 3));
+            const uint4 kf = make_uint4(codes2<BIAS>(w, 0), codes2<BIAS>(w, 1), codes2<BIAS>(w, 2), codes2<BIAS>(w, 3));
             kh_f32x4 c = {0, 0, 0, 0};
 #pragma unroll
             for (int k = NQ - 1; k >= 0; --k) c = mfma16(kf, qf[j][k], c);
@@ -464,8 +469,10 @@ __device__ __forceinline__ void pa_tiles(const PaArgs& a, float* s_o, const PaLa
           const float alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.c1);
           l *= alpha;
           om *= alpha;
+          if constexpr (BIAS != 0) {
 #pragma unroll
-          for (int j = 0; j < NG; ++j) os[j] *= alpha;
+            for (int j = 0; j < NG; ++j) os[j] *= alpha;
+          }
 #pragma unroll
           for (int f = 0; f < NF; ++f) o[f] *= alpha;
           m = mn;
@@ -499,14 +506,16 @@ __device__ __forceinline__ void pa_tiles(const PaArgs& a, float* s_o, const PaLa
           }
           uint4 pg[NP];
           terms8<NP>(ps8, pg);
+          if constexpr (BIAS != 0) {
 #pragma unroll
-          for (int k = NP - 1; k >= 0; --k)
-            os[gi] = add2(pg[k].w, add2(pg[k].z, add2(pg[k].y, add2(pg[k].x, os[gi]))));
+            for (int k = NP - 1; k >= 0; --k)
+              os[gi] = add2(pg[k].w, add2(pg[k].z, add2(pg[k].y, add2(pg[k].x, os[gi]))));
+          }
 #pragma unroll
           for (int ff = 0; ff < 2; ++ff) {
             const int f = 2 * gi + ff, hf = f >> 2, nb = f & 3;
-            const uint4 vf = make_uint4(codes2(x.vw[0][hf], nb), codes2(x.vw[0][HN + hf], nb),
-                                        codes2(x.vw[1][hf], nb), codes2(x.vw[1][HN + hf], nb));
+            const uint4 vf = make_uint4(codes2<BIAS>(x.vw[0][hf], nb), codes2<BIAS>(x.vw[0][HN + hf], nb),
+                                        codes2<BIAS>(x.vw[1][hf], nb), codes2<BIAS>(x.vw[1][HN + hf], nb));
 #pragma unroll
             for (int k = NP - 1; k >= 0; --k) o[f] = mfma16(vf, pg[k], o[f]);
           }
@@ -553,13 +562,13 @@ __device__ __forceinline__ void pa_tiles(const PaArgs& a, float* s_o, const PaLa
       }
     }
 
-    // -16 sum R + sum p m: row j of om lies with lane group j / 4
+    // -B sum R + sum p m: row j of om lies with lane group j / 4
     l = across_groups_sum(l);
     {
 #pragma unroll
       for (int gi = 0; gi < NG; ++gi) {
-        const float c = __shfl(om[gi & 3], (gi >> 2) * 16 + col) -
-                        (float)kBias * across_groups_sum(os[gi]);
+        float c = __shfl(om[gi & 3], (gi >> 2) * 16 + col);
+        if constexpr (BIAS != 0) c -= (float)BIAS * across_groups_sum(os[gi]);
 #pragma unroll
         for (int ff = 0; ff < 2; ++ff)
 #pragma unroll

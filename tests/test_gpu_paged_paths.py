@@ -277,21 +277,21 @@ def test_single_rows_of_many_sequences_in_parts(kh, dtype, dim):
 def test_log_sums_of_one_position(kh, dtype, heads, kv, dim):
     """The log-sum-exp of one position is its score, held to the roundings that the method's own numbers have.
 
-    A score sums, group by group, s q (16 + c) over 32 elements, and s, m against sums of q: f32 additions, each off by
+    A score sums, group by group, s q (B + c) over 32 elements (B = 16 in BF16, 0 in f32), and s, m against sums of q: f32 additions, each off by
     u / sqrt(3) of its partial sum in the root mean square, u = 2^-24.  A group's 32 additions have partial sums of at
-    most P = |q (16 + c)| (2-norm, signs being independent), so they are off by u sqrt(32 / 3) s P together; its share of
-    the second sum, of sizes 16 s |Q| and |m Q|, is added by some 8 at most: u sqrt(8 / 3) of those; the groups'
+    most P = |q (B + c)| (2-norm, signs being independent), so they are off by u sqrt(32 / 3) s P together; its share of
+    the second sum, of sizes B s |Q| and |m Q|, is added by some 8 at most: u sqrt(8 / 3) of those; the groups'
     sums are added once each, to a total within their 2-norm, and the score is scaled and turned to natural logarithms by
     four more roundings of itself."""
-    n, u = 300, 2.0 ** -24
+    n, u, bias = 300, 2.0 ** -24, 16 if dtype == BF16 else 0
     c = Case(dtype, heads, kv, dim, 16, [1] * n, [1] * n)
     _, lse = c.run(max_rows=1, max_len=1)
     q, k = c.q.double().numpy(), np.stack([x[0].float().numpy() for x in c.k])  # [n, heads, dim], [n, kv, dim]
     kc, ks, km = (np.repeat(x, heads // kv, 1).reshape(n, heads, dim // 32, 32) for x in quantize(k))
     q, s, m = q.reshape(n, heads, -1, 32), ks[..., 0], km[..., 0]
     want = ((q * (ks * kc + km)).sum((-2, -1))) * dim ** -0.5
-    p, total = s * np.sqrt((q * q * (16 + kc) ** 2).sum(-1)), np.abs(q.sum(-1))
-    each = 32 / 3 * p ** 2 + 8 / 3 * ((16 * s * total) ** 2 + (m * total) ** 2) + p ** 2 / 3
+    p, total = s * np.sqrt((q * q * (bias + kc) ** 2).sum(-1)), np.abs(q.sum(-1))
+    each = 32 / 3 * p ** 2 + 8 / 3 * ((bias * s * total) ** 2 + (m * total) ** 2) + p ** 2 / 3
     bound = u * np.sqrt(each.sum(-1) / dim + 4 * want ** 2)
     off = lse.double().cpu().numpy() - want
     ratio = np.sqrt((off ** 2).mean() / (bound ** 2).mean())
