@@ -26,9 +26,13 @@
 // Few rows (paged_rows_kernel) are bound by the cache's bytes where it is long and by a
 // chain of some 6.5 us where it is short: launch, lengths, pages, codes, one step, the
 // join of the waves.  32 heads of 128, BF16: eight sequences of 2048 positions (84 MB)
-// 24.4 us, 131072 positions of 8 kv heads (168 MB) 44.4 + 5.2 us of join (3.7 TB/s; a copy
+// 25.4 us, 131072 positions of 8 kv heads (168 MB) 48.0 + 4.6 us of join (3.5 TB/s; a copy
 // runs at 4.8, read and write), 64 positions 7 us.  16 of 32 heads, f32, 2000 positions:
-// 11.3 + 3.7 us.  Many rows: below.
+// 11.8 + 3.9 us (parts are cut as if all heads had work: blocks of unlisted heads stay idle).
+// 16 heads of 256 over 8, eight sequences of 2048: 21.6 + 4.0 us, f32 27.5 + 4.1; no step is
+// loaded ahead there, the sums and a step fill the registers.  Many f32 rows run here too: 1024
+// causal rows of 32 heads of 128 over 8 take 130 us, each tile unpacks its positions for itself
+// and every product has three or more terms.  Many BF16 rows: below.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -685,17 +689,17 @@ __global__ __launch_bounds__((64 * PaShape<D, T>::NW), (PaShape<D, T>::kPerSimd)
 //
 // Where three row tiles or more see the same positions, a kernel unpacks them once into
 // the workspace and the tiles copy them to LDS as they are: 4096 causal rows of 32 heads
-// of 128 take 13 + 166 us so, 210 us where each tile unpacks them (at 137 GFLOP 0.83
+// of 128 take 13 + 161 us so, 210 us where each tile unpacks them (at 137 GFLOP 0.85
 // PFLOP/s; a call in a stream of them 149 us).  The copies go through registers: for a
 // load straight to LDS the compiler waits before the next read of any LDS (178 us).
 //
 // A value's group that stands for NaN is unpacked as 0 and marked in a mask of its
 // positions: rows that see one of them get their NaN from the mask.
 //
-// Bound by its own latency: two waves a SIMD (registers), each with its products (42% of
-// the time), other vector instructions (29%) and waits one after the other; at D = 256 by
-// reading LDS, where a fragment feeds one product a wave (four chunks of 41 to 331 rows of
-// 16 heads over 2, window 1024: 11 + 41 us and 8 of join).  Half of the
+// Bound by its own latency: two waves a SIMD (registers), each with its products (41% of
+// the time), other vector instructions (39%) and waits (29% of its cycles) one after the other;
+// at D = 256 by reading LDS, where a fragment feeds one product a wave (four chunks of 41 to
+// 331 rows of 16 heads over 2, window 1024: 11 + 42 us and 8 of join).  Half of the
 // waves a phase later (177 us), exponentials between the products of the step before
 // (spills), blocks of four waves (187 us) and raised priority for products (no change)
 // did not help.
@@ -1271,7 +1275,7 @@ __device__ __forceinline__ void pt_tiles(const PaArgs& a, char* s_buf, int* s_lo
 // The u-th row tile of up to 64 sequences, the last tiles (which see the most) of all of
 // them first: false where there are no more.  Grids of every sequence's most tiles left
 // compute units empty behind blocks without rows (chunks of 331, 255, 41 and 286 rows:
-// 232 blocks with rows among 336 began in two rounds, 71 us instead of 37).
+// 232 blocks with rows among 336 began in two rounds, 71 us instead of 42).
 __device__ __forceinline__ bool pt_tile(const PaArgs& a, int lane, int rb, uint32_t u, int* b, int* tile) {
   uint32_t n = 0;
   if (lane < a.batch) {

@@ -250,9 +250,11 @@ struct QuadLanes {
 // share 16-byte pieces: they are put together in LDS and stored whole where all
 // four are appended, and as u16 where they are not.
 //
-// 14460 BF16 rows of 8 heads of 128 (59 MB in, 18.5 MB out, interleaved rotation): 28.9 us,
-// 2.7 TB/s.  28 vector instructions a value, for ranges, quotients, codes and their places,
-// take 60% of the issue slots, and loads wait behind them (a position a lane took 77 us;
+// 14460 BF16 rows of 8 heads of 128 (59 MB in, 18.5 MB out, interleaved rotation): 32.6 us
+// behind a gather, 2.4 TB/s, 28.9 where the input lies in the caches; f32 (118 MB in) 37.6.
+// Latency: a wave loads, codes and stores one head after the other, so that 28 vector
+// instructions a value (ranges, quotients, codes, places), 55% of the issue slots, and waits,
+// 53% of its cycles, do not overlap enough (a position a lane took 77 us;
 // quads with correctly rounded quotients by a division 38, by a corrected reciprocal 33).
 // One row: 4 us, the chain of offsets, page id and table.
 template <typename T, int D, int MODE, bool VAL>
@@ -409,8 +411,9 @@ struct GatherArgs {
 
 // The inverse: the same quads and lanes.  Of the four lanes that need the same eight
 // u16 of a value's codes each loads two, and they exchange them.  14460 rows of 8 heads of
-// 128 to BF16 (18.5 MB in, 59 MB out): 22.0 us, 3.5 TB/s, 3.6 us for one; to f32 (118 MB
-// out) 27.5 us, 5.0 TB/s.  The rows stay in the caches for whoever reads them next: with a
+// 128 to BF16 (18.5 MB in, 59 MB out): 22.0 us, 3.5 TB/s (23.7 behind an append), 3.6 us for
+// one; to f32 (118 MB out) 27.5 us, 5.0 TB/s.  Waits are 57% of a wave's cycles: the next
+// head's loads are not under way.  The rows stay in the caches for whoever reads them next: with a
 // copy of them behind, 40.8 us and to f32 76.4, where stores past the caches took 44.9 and
 // 88.8 (alone 21.1 and 39.5).
 template <typename T, int D, bool VAL>

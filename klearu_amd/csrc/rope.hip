@@ -11,7 +11,7 @@
 // of a pair in one thread: bounded by memory for many rows (8191 BF16 rows of 32 heads of
 // 128, 138 MB with the table: 24.7 us, 5.6 TB/s, a copy of 4 GiB runs at 4.8; 2049 f32 rows
 // of 32 heads of 64, interleaved, half of a head rotated: 7.5 us) and by the launch for one
-// (2.2 us of kernel, 6.8 us a call).
+// (2.4 us of kernel, 6.8 us a call).
 #include <algorithm>
 #include <cmath>
 #include <new>
