@@ -319,6 +319,7 @@ def test_guess_of_the_rows_of_many_sequences(kh):
 
 def test_padding_past_one_grid_of_the_join(kh):
     """One row behind 2^17 rows of padding, in 17 parts: 2^24 + 128 rows of heads to join, 75 GB of workspace."""
+    torch.cuda.empty_cache()
     if torch.cuda.mem_get_info()[0] < 100 << 30:
         pytest.skip("needs 100 GiB of device memory")
     c = Case(F32, 128, 1, 64, 64, [1], [4352])
@@ -330,3 +331,5 @@ def test_padding_past_one_grid_of_the_join(kh):
     c.cache.attention(q, off, c.len, c.table, max_rows=1, max_len=4352, out=out)
     hold(c, out[-1:])
     assert bool((out[:-1] == 7).all())
+    del q, out
+    torch.cuda.empty_cache()
