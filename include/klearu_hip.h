@@ -711,12 +711,22 @@ typedef struct kh_rope kh_rope;
  * rot_dim even, 2..1024.  Keeps max_pos * rot_dim * 4 bytes.  Synchronous. */
 int kh_rope_create(int rot_dim, int64_t max_pos, int layout, double theta, int scaling, double factor,
                    int64_t original_len, double low, double high, double magnitude, kh_rope** out);
+/* The same with positions along 1 to 4 axes (time, height and width of a video's
+ * patches): pairs i = 0 .. rot_dim / 2 - 1 go to the axes section by section,
+ * sections_host[a] of them to axis a, and pair i of a row turns by the row's
+ * position along its axis.  Positions are pos_dev[axes][rows] then, wherever a
+ * call takes them.  Frequencies run on over all pairs, or begin again in each
+ * section (restart: f of a section of n pairs are those of rot_dim = 2 n). */
+#define KH_ROPE_MAX_AXES 4
+int kh_rope_create_axes(int rot_dim, int64_t max_pos, int layout, double theta, int scaling, double factor,
+                        int64_t original_len, double low, double high, double magnitude, int axes,
+                        const int32_t* sections_host, int restart, kh_rope** out);
 int kh_rope_destroy(kh_rope* r);
 /* Rotates the first rot_dim elements of every head of row t by position
- * pos_dev[t] and copies the others: y = R x, or y = R^T x with `transpose`, which
+ * pos_dev[t] (of several axes: pos_dev[a][t]) and copies the others: y = R x, or y = R^T x with `transpose`, which
  * takes the gradient with respect to y to the one with respect to x.  A row
- * with a negative position is padding and left as it was; so is one with a
- * position past the table, which kh_rope_status reports.  y may be x itself
+ * with a negative position (along any axis) is padding and left as it was; so is
+ * one with a position past the table, which kh_rope_status reports.  y may be x itself
  * (with the same strides); otherwise the two must not overlap. */
 int kh_rope_apply(const kh_rope* r, int dtype, const void* x_dev, int64_t x_row_stride,
                   int64_t x_head_stride, int64_t rows, int heads, int head_dim, const int64_t* pos_dev,
@@ -752,8 +762,8 @@ int kh_paged_kv_status(const kh_paged_kv* c);
 /* Puts keys and values k, v [rows][kv heads][head_dim] into the cache: row
  * off[b] + i at position start_dev[b] + i of sequence b.  With a rotation the
  * keys are rotated on the way, in f32 and before they are held in 4 bits, by
- * pos_dev[row], or by their positions in the cache where pos_dev is NULL; rows
- * whose rotary position is negative or past the rotation's table are not
+ * pos_dev[row] (of several axes: [axes][rows]), or by their positions in the cache
+ * (along every axis) where pos_dev is NULL; rows whose rotary position is negative or past the rotation's table are not
  * appended (kh_rope_status reports them).  Two rows of one call must not have the
  * same place (two sequences may share pages, but not write to them). */
 int kh_paged_kv_append(kh_paged_kv* c, const kh_rope* rope, int dtype, const void* k_dev,
@@ -800,6 +810,87 @@ int kh_paged_kv_attention(const kh_paged_kv* c, int dtype, const void* q_dev, in
                           float scale, int causal, int64_t window, const int32_t* heads_dev, int n_heads,
                           void* out_dev, int64_t out_row_stride, int64_t out_head_stride, float* lse_dev,
                           void* ws_dev, int64_t ws_bytes, void* stream);
+
+/* What a decoder does around that cache: the attention weights of its positions,
+ * eviction by them, beams over its pages. */
+
+/* Adds up the attention weight that the positions of the cache get from rows q
+ * whose log-sum-exp is known (kh_paged_kv_attention's lse_dev, [rows][num_heads]):
+ *   acc[b][h][j] += sum over the rows i of sequence b and the query heads g of kv head h
+ *                   of exp(scale q_ig . k_j - lse_ig)
+ * over the rows that see j (causal, window: as there).  A row whose lse is -inf (it
+ * saw nothing, or does not list the head) adds nothing.  acc_dev: f32
+ * [batch][kv heads][acc_cols]; positions past acc_cols are not added up, which
+ * kh_paged_kv_status reports as a place outside the table.  Scores and sums are f32, the keys
+ * exactly those that the cache stands for; a position whose key holds a NaN group gets NaN.
+ * The result does not depend on the run.  max_rows and max_len are guesses as for the attention, and so is
+ * ws_dev (kh_paged_kv_weights_workspace bytes). */
+int kh_paged_kv_weights_workspace(const kh_paged_kv* c, int dtype, int64_t rows, int64_t batch,
+                                  int num_heads, int64_t max_rows, int64_t max_len, int64_t* bytes);
+int kh_paged_kv_weights(const kh_paged_kv* c, int dtype, const void* q_dev, int64_t q_row_stride,
+                        int64_t q_head_stride, int num_heads, int64_t rows, const int64_t* off_dev,
+                        int64_t batch, const int64_t* len_dev, const int32_t* table_dev,
+                        int64_t table_cols, int64_t table_stride, int64_t max_rows, int64_t max_len,
+                        float scale, int causal, int64_t window, const float* lse_dev, float* acc_dev,
+                        int64_t acc_cols, void* ws_dev, int64_t ws_bytes, void* stream);
+
+/* Evicts positions: of a sequence with len > keep positions every kv head keeps
+ * `keep`, the first `first`, the last `recent` (first + recent <= keep) and of the others
+ * those with the largest acc (f32 [batch][kv heads][acc_cols]; of equal ones the
+ * first, a NaN counts as larger than every number), and the kept ones move, in their
+ * order, to positions 0 .. keep - 1 of the cache.  Places from keep on keep what
+ * they held; pages that lie there whole are the caller's again.  Shorter sequences stay as
+ * they are.  Writes
+ *   kept_dev    int32 [batch][kv heads][keep]: where each position was (its own place
+ *               where nothing was evicted), -1 past the sequence's end;
+ *   acc_out_dev f32 [batch][kv heads][acc_cols]: acc of the positions that are left,
+ *               then 0 (may be acc_dev itself);
+ *   len_out_dev int64 [batch]: min(len, keep) (not len_dev itself).
+ * Positions past acc_cols or the table are evicted and reported by kh_paged_kv_status,
+ * as are page ids outside the pool, whose positions do not move.  Sequences that are
+ * cut must not share pages with any other (as none that two beams go on from).
+ * ws_dev: 16-byte aligned, kh_paged_kv_evict_workspace bytes, not shared by calls that may run at once. */
+int kh_paged_kv_evict_workspace(const kh_paged_kv* c, int64_t batch, int64_t keep, int64_t acc_cols,
+                                int64_t* bytes);
+int kh_paged_kv_evict(kh_paged_kv* c, const float* acc_dev, int64_t acc_cols, const int64_t* len_dev,
+                      int64_t batch, const int32_t* table_dev, int64_t table_cols, int64_t table_stride,
+                      int64_t keep, int64_t recent, int64_t first, int32_t* kept_dev, float* acc_out_dev,
+                      int64_t* len_out_dev, void* ws_dev, int64_t ws_bytes, void* stream);
+
+/* Continuations of beams: row b * beams + i of the page table is beam i of
+ * sequence b, len_dev[b] positions long as all of its beams are, and beam i goes on
+ * from beam parent_dev[b][i] (int32, 0 .. beams - 1).  Row b * beams + i of
+ * out_table lists the parent's pages in its columns c < len / page_size: whole
+ * pages, which beams share.  Behind those each beam needs pages of its own to write to:
+ * the first beam that goes on from a parent takes over the parent's, the others
+ * those of the beams that nobody goes on from, in order, and get a copy of the
+ * parent's rows in the page that is not whole.  (A sequence whose beams all begin as one: every
+ * parent 0, and pages of its own in every row from column len / page_size on.)
+ * out_table_dev must not overlap table_dev.  A whole page that no row lists any more is the caller's
+ * again.  A parent outside 0 .. beams - 1 counts as the beam itself, and kh_paged_kv_status reports it. */
+#define KH_MAX_BEAMS 64
+int kh_paged_kv_reorder(kh_paged_kv* c, const int32_t* table_dev, int64_t table_cols, int64_t table_stride,
+                        const int64_t* len_dev, int64_t batch, int beams, const int32_t* parent_dev,
+                        int32_t* out_table_dev, int64_t out_stride, void* stream);
+
+/* The k best continuations of each sequence's beams: of the scores
+ *   y[i][v] = scores[i] + logits[i][v] - log sum_w exp(logits[i][w]),  i < beams, v < vocab,
+ * the k largest, in descending order; of equal ones the first by (i, v).  logits_dev: KH_DT_F32
+ * or KH_DT_BF16 rows [batch * beams][vocab], row_stride elements apart; scores_dev: f32
+ * [batch][beams].  A beam whose done_dev (NULL, or uint8 [batch][beams]) is not 0 has ended: its
+ * one continuation is token `end`, with the beam's score, the others have -inf.  So have all of a beam whose
+ * score is not finite, or whose log-sum-exp is not (a NaN or +inf among its logits, or
+ * nothing but -inf).  Log-sum-exps and scores are f64 (exponentials f32 with a correction, their
+ * sums within 1e-8), rounded to f32 where they are written: continuations of one beam are ordered by
+ * their logits.  Writes y, i and v, [batch][k] each.  k <= 64, k <= beams * vocab,
+ * beams <= KH_MAX_BEAMS.  ws_dev: 16-byte aligned, kh_beam_select_workspace bytes, not shared by
+ * calls that may run at once.  The stream's device must be the current one. */
+#define KH_MAX_BEAM_K 64
+int kh_beam_select_workspace(int64_t batch, int beams, int64_t vocab, int k, int64_t* bytes);
+int kh_beam_select(int dtype, const void* logits_dev, int64_t row_stride, int64_t batch, int beams,
+                   int64_t vocab, const float* scores_dev, const uint8_t* done_dev, int64_t end, int k,
+                   float* out_scores_dev, int32_t* out_beams_dev, int32_t* out_tokens_dev, void* ws_dev,
+                   int64_t ws_bytes, void* stream);
 
 /* ======================================================================== */
 /* On-disk formats: safetensors weights and predictor JSON files            */

@@ -153,6 +153,8 @@ SIGS = {
     "kh_sparse_attn_clear": (I, [P, P]),
     "kh_sparse_attn_forward": (I, [P, P, I64, P, P, I, P, I, P]),
     "kh_rope_create": (I, [I, I64, I, C.c_double, I, C.c_double, I64, C.c_double, C.c_double, C.c_double, PP]),
+    "kh_rope_create_axes": (I, [I, I64, I, C.c_double, I, C.c_double, I64, C.c_double, C.c_double, C.c_double, I, P, I,
+                                PP]),
     "kh_rope_destroy": (I, [P]),
     "kh_rope_apply": (I, [P, I, P, I64, I64, I64, I, I, P, P, I64, I64, I, P]),
     "kh_rope_status": (I, [P]),
@@ -164,6 +166,14 @@ SIGS = {
     "kh_paged_kv_attention_workspace": (I, [P, I, I64, I64, I, I64, I64, I, P]),
     "kh_paged_kv_attention": (I, [P, I, P, I64, I64, I, I64, P, I64, P, P, I64, I64, I64, I64, F, I, I64, P, I, P,
                                   I64, I64, P, P, I64, P]),
+    "kh_paged_kv_weights_workspace": (I, [P, I, I64, I64, I, I64, I64, P]),
+    "kh_paged_kv_weights": (I, [P, I, P, I64, I64, I, I64, P, I64, P, P, I64, I64, I64, I64, F, I, I64, P, P, I64, P, I64,
+                                P]),
+    "kh_paged_kv_evict_workspace": (I, [P, I64, I64, I64, P]),
+    "kh_paged_kv_evict": (I, [P, P, I64, P, I64, P, I64, I64, I64, I64, I64, P, P, P, P, I64, P]),
+    "kh_paged_kv_reorder": (I, [P, P, I64, I64, P, I64, I, P, P, I64, P]),
+    "kh_beam_select_workspace": (I, [I64, I, I64, I, P]),
+    "kh_beam_select": (I, [I, P, I64, I64, I, I64, P, P, I64, I, P, P, P, P, I64, P]),
     "kh_safetensors_open": (I, [S, PP]),
     "kh_safetensors_close": (I, [P]),
     "kh_safetensors_count": (I, [P, C.POINTER(I64)]),

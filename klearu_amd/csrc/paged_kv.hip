@@ -78,6 +78,7 @@ struct AppendArgs {
   int rot, half_layout, mode;
   int* rope_err;
   int kvec, vvec;  // 16-byte loads
+  RopeAxes ax;
 };
 
 // The key's elements d .. d + 7 after the rotation, in f32.
@@ -121,6 +122,25 @@ __device__ __forceinline__ void rotated8(const T* __restrict__ x, int d, int rot
   }
 }
 
+// The same with several axes, element by element; row(a): the table's row at the key's position along axis a.
+template <typename T, typename F>
+__device__ __forceinline__ void rotated8_axes(const T* __restrict__ x, int d, int rot, int half_layout, bool vec,
+                                              const RopeAxes& ax, F row, float (&f)[8]) {
+  load8(x + d, vec, f);
+  if (d >= rot) return;
+  const int half = rot >> 1;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int e = d + i;
+    if (e >= rot) break;
+    const bool second = half_layout ? e >= half : e & 1;
+    const int pair = half_layout ? (second ? e - half : e) : e >> 1;
+    const float o = load_f32(x + (half_layout ? (second ? e - half : e + half) : e ^ 1));
+    const float2 cs = row(ax.of(pair))[pair];
+    f[i] = second ? f[i] * cs.x + o * cs.y : f[i] * cs.x - o * cs.y;
+  }
+}
+
 // The quads (four positions that share bytes) that the rows of sequences c0 ..
 // c0 + nb - 1 touch: s_q[i] of them lie before sequence c0 + i.  The whole block
 // takes part; returns their number.
@@ -154,8 +174,8 @@ __device__ __forceinline__ int stage_quads(const KvRows& a, int64_t c0, int nb, 
 }
 
 // How the rows' keys are rotated: not at all, pieces of eight elements by their
-// pairs, or element by element (any rot).
-constexpr int kRotNone = 0, kRotHalf = 1, kRotInterleaved = 2, kRotAny = 3;
+// pairs, or element by element (any rot; any sections of several axes).
+constexpr int kRotNone = 0, kRotHalf = 1, kRotInterleaved = 2, kRotAny = 3, kRotAxes = 4;
 
 // Up to 64 sequences: lane i holds sequence i's quads and those before it.
 struct WaveSeqs {
@@ -272,6 +292,9 @@ __device__ __forceinline__ void append_part(const AppendArgs& a, int units, int 
   const bool first_half = 8 * c < (a.rot >> 1);
   const bool turns = MODE == kRotHalf || MODE == kRotInterleaved ? 8 * c < a.rot : false;
   const int other = first_half ? a.rot >> 1 : -(a.rot >> 1);  // the pairs' other elements (kRotHalf)
+  // several axes: where the positions along the axis of the lane's pairs lie
+  const int64_t mine_axis =
+      a.ax.n > 1 && turns ? a.ax.of(MODE == kRotInterleaved ? 4 * c : first_half ? 8 * c : 8 * c - (a.rot >> 1)) * a.ax.stride : 0;
   walk_quads(a.r, units, hpu, s_q, s_wsum, s_tot, [&](int64_t p0, int t0, int o0, int o1, int pg, int h0, int nh) {
       const int at0 = (int)(p0 & (ps - 1));
       // the lane's positions
@@ -285,8 +308,15 @@ __device__ __forceinline__ void append_part(const AppendArgs& a, int units, int 
         on[k] = t >= o0 && t < o1;
         tab[k] = nullptr;
         if (a.table && on[k]) {  // a row without a rotation is not appended at all
-          const int64_t r = a.pos ? a.pos[t] : p0 + k * TP + tp;
-          if (r < 0 || r >= a.max_pos) {
+          const int64_t r = a.pos ? a.pos[mine_axis + t] : p0 + k * TP + tp;
+          bool out = r < 0 || r >= a.max_pos;
+          if (a.ax.n > 1 && a.pos) {  // a row is appended whole or not at all
+            for (int i = 0; i < a.ax.n; ++i) {
+              const int64_t ri = a.pos[i * a.ax.stride + t];
+              out = out || ri < 0 || ri >= a.max_pos;
+            }
+          }
+          if (out) {
             if (!VAL) atomicOr(a.rope_err, 1);
             on[k] = false;
           } else
@@ -321,6 +351,13 @@ __device__ __forceinline__ void append_part(const AppendArgs& a, int units, int 
             const T* x = x0 + k * TP * srow;
             if (MODE == kRotAny) {
               rotated8(x - 8 * c, 8 * c, a.rot, a.half_layout, vec, tab[k], f);
+            } else if (MODE == kRotAxes) {
+              const int t = t0 + k * TP + tp;
+              rotated8_axes(x - 8 * c, 8 * c, a.rot, a.half_layout, vec, a.ax,
+                            [&](int i) {
+                              const int64_t r = a.pos ? a.pos[i * a.ax.stride + t] : p0 + k * TP + tp;
+                              return a.table + r * (a.rot >> 1);
+                            }, f);
             } else {
               load8(x, vec, f);
               if (MODE == kRotHalf && turns) {
@@ -486,6 +523,7 @@ static void append_launch_m(const AppendArgs& a, dim3 g, int units, int hpu, hip
   else if (a.mode == kRotHalf) hipLaunchKernelGGL((kv_append_kernel<T, D, kRotHalf>), g, blk, 0, st, a, units, hpu);
   else if (a.mode == kRotInterleaved)
     hipLaunchKernelGGL((kv_append_kernel<T, D, kRotInterleaved>), g, blk, 0, st, a, units, hpu);
+  else if (a.mode == kRotAxes) hipLaunchKernelGGL((kv_append_kernel<T, D, kRotAxes>), g, blk, 0, st, a, units, hpu);
   else hipLaunchKernelGGL((kv_append_kernel<T, D, kRotAny>), g, blk, 0, st, a, units, hpu);
 }
 template <typename T>
@@ -613,8 +651,8 @@ extern "C" int kh_paged_kv_status(const kh_paged_kv* c) {
   KH_HIP(hipMemset(c->err, 0, sizeof(int)));
   // cleared before any other stream records again: streams need not wait for the null stream
   KH_HIP(hipStreamSynchronize(nullptr));
-  set_error("%s%s", (bad & 1) ? "a position lay outside its sequence's page table; " : "",
-            (bad & 2) ? "a page id lay outside the pool; " : "");
+  set_error("%s%s%s", (bad & 1) ? "a position lay outside its sequence's page table; " : "",
+            (bad & 2) ? "a page id lay outside the pool; " : "", (bad & 4) ? "a beam's parent was none of its beams; " : "");
   return KH_ERR_ARG;
 }
 
@@ -651,6 +689,12 @@ extern "C" int kh_paged_kv_append(kh_paged_kv* c, const kh_rope* rope, int dtype
   a.mode = !rope ? kRotNone
            : rope->rot % (a.half_layout ? 16 : 8) ? kRotAny
            : a.half_layout ? kRotHalf : kRotInterleaved;
+  a.ax = RopeAxes{1, {0, 0, 0, 0}, 0};
+  if (rope && rope->axes > 1) {
+    a.ax = rope_axes(rope, rows);
+    // sections that end inside a lane's piece
+    if (a.mode == kRotAny || !rope_axes_whole(rope, a.half_layout ? 8 : 4)) a.mode = kRotAxes;
+  }
   a.rope_err = rope ? rope->err : nullptr;
   a.kvec = aligned16(k_dev, dtype, k_row_stride, k_head_stride) ? 1 : 0;
   a.vvec = aligned16(v_dev, dtype, v_row_stride, v_head_stride) ? 1 : 0;

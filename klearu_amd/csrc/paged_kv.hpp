@@ -27,6 +27,9 @@ struct kh_rope {
   int device = 0;
   float2* table = nullptr;  // [max_pos][rot / 2] (cos, sin), both times the magnitude
   int* err = nullptr;
+  // several axes: pairs end[a - 1] .. end[a] - 1 turn by the row's position along axis a
+  int axes = 1;
+  int end[KH_ROPE_MAX_AXES] = {0, 0, 0, 0};
 };
 
 struct kh_paged_kv {
@@ -39,6 +42,32 @@ struct kh_paged_kv {
 };
 
 namespace kh {
+
+// The pairs' axes of a rotation, and where the positions along the others lie behind the first one's.
+struct RopeAxes {
+  int n;
+  int end[KH_ROPE_MAX_AXES];  // of unused axes: the number of pairs
+  int64_t stride;
+  __device__ __forceinline__ int of(int pair) const {
+    int a = 0;
+#pragma unroll
+    for (int i = 0; i + 1 < KH_ROPE_MAX_AXES; ++i) a += pair >= end[i] ? 1 : 0;
+    return a;
+  }
+};
+inline RopeAxes rope_axes(const kh_rope* r, int64_t stride) {
+  RopeAxes x;
+  x.n = r->axes;
+  x.stride = stride;
+  for (int i = 0; i < KH_ROPE_MAX_AXES; ++i) x.end[i] = i < r->axes ? r->end[i] : r->rot / 2;
+  return x;
+}
+// Whether no section ends inside a piece of n pairs.
+inline bool rope_axes_whole(const kh_rope* r, int n) {
+  for (int i = 0; i < r->axes; ++i)
+    if (r->end[i] % n) return false;
+  return true;
+}
 
 constexpr int kKvGroup = 32;  // values that share a scale and a minimum
 

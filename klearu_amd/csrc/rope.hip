@@ -43,6 +43,7 @@ struct RopeArgs {
   int heads, dim, rot;
   float sgn;  // of the sine: -1 for the transposed rotation
   int copy;   // the elements past rot are copied (y is not x)
+  RopeAxes ax;
 };
 
 // The row's table entries, or nullptr for a row that is skipped: negative
@@ -57,6 +58,25 @@ __device__ __forceinline__ const float2* rope_row(const RopeArgs& a, int64_t t) 
   return a.table + p * (a.rot >> 1);
 }
 
+// Several axes: whether the row is rotated (any negative position makes it padding), and its positions.
+__device__ __forceinline__ bool rope_row_axes(const RopeArgs& a, int64_t t, int64_t (&p)[KH_ROPE_MAX_AXES]) {
+  bool pad = false, past = false;
+#pragma unroll
+  for (int i = 0; i < KH_ROPE_MAX_AXES; ++i) {
+    p[i] = i < a.ax.n ? a.pos[i * a.ax.stride + t] : 0;
+    pad = pad || p[i] < 0;
+    past = past || p[i] >= a.max_pos;
+  }
+  if (!pad && past) atomicOr(a.err, 1);
+  return !pad && !past;
+}
+// The table's row that pair i of the row reads.
+__device__ __forceinline__ const float2* rope_axis(const RopeArgs& a, const int64_t (&p)[KH_ROPE_MAX_AXES], int i) {
+  const int x = a.ax.of(i);
+  const int64_t r = x == 0 ? p[0] : x == 1 ? p[1] : x == 2 ? p[2] : p[3];
+  return a.table + r * (a.rot >> 1);
+}
+
 __device__ __forceinline__ void rope_pair(float& x0, float& x1, float c, float s) {
   const float y0 = x0 * c - x1 * s, y1 = x1 * c + x0 * s;
   x0 = y0;
@@ -64,15 +84,26 @@ __device__ __forceinline__ void rope_pair(float& x0, float& x1, float c, float s
 }
 
 // One thread: one piece of eight pairs (or eight elements of four pairs, or
-// eight elements past rot) of one head of one row.
-template <typename T, bool HALF>
+// eight elements past rot) of one head of one row.  AXES: several of them; a piece
+// that two sections share looks its rows up pair by pair.
+template <typename T, bool HALF, bool AXES>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pieces) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t per_row = (int64_t)pieces * a.heads;
   const int64_t t = id / per_row;
   if (t >= a.rows) return;
-  const float2* __restrict__ tab = rope_row(a, t);
-  if (!tab) return;
+  const float2* __restrict__ tab = nullptr;
+  int64_t p[KH_ROPE_MAX_AXES];
+  if (AXES) {
+    if (!rope_row_axes(a, t, p)) return;
+  } else {
+    tab = rope_row(a, t);
+    if (!tab) return;
+  }
+  const auto pair = [&](int i) -> float2 {
+    if (!AXES) return tab[i];
+    return rope_axis(a, p, i)[i];
+  };
   const int rem = (int)(id - t * per_row), h = rem / pieces, u = rem - h * pieces;
   const T* x = static_cast<const T*>(a.x) + t * a.xs + h * a.xh;
   T* y = static_cast<T*>(a.y) + t * a.ys + h * a.yh;
@@ -85,7 +116,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pieces) {
       load8(x + half + 8 * u, true, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float2 cs = tab[8 * u + i];
+        const float2 cs = pair(8 * u + i);
         rope_pair(v[i], w[i], cs.x, a.sgn * cs.y);
       }
       store8(y + 8 * u, true, v);
@@ -101,7 +132,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pieces) {
     if (d < a.rot) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 cs = tab[4 * u + i];
+        const float2 cs = pair(4 * u + i);
         rope_pair(v[2 * i], v[2 * i + 1], cs.x, a.sgn * cs.y);
       }
     }
@@ -111,14 +142,20 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int pieces) {
 
 // Any alignment and any even rot: one thread per pair, then one per copied
 // element.
-template <typename T>
+template <typename T, bool AXES>
 __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a, int half_layout, int units) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t per_row = (int64_t)units * a.heads;
   const int64_t t = id / per_row;
   if (t >= a.rows) return;
-  const float2* __restrict__ tab = rope_row(a, t);
-  if (!tab) return;
+  const float2* __restrict__ tab = nullptr;
+  int64_t p[KH_ROPE_MAX_AXES];
+  if (AXES) {
+    if (!rope_row_axes(a, t, p)) return;
+  } else {
+    tab = rope_row(a, t);
+    if (!tab) return;
+  }
   const int rem = (int)(id - t * per_row), h = rem / units, u = rem - h * units;
   const T* x = static_cast<const T*>(a.x) + t * a.xs + h * a.xh;
   T* y = static_cast<T*>(a.y) + t * a.ys + h * a.yh;
@@ -126,7 +163,7 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a, int half_layo
   if (u < half) {
     const int i0 = half_layout ? u : 2 * u, i1 = half_layout ? u + half : 2 * u + 1;
     float v = load_f32(x + i0), w = load_f32(x + i1);
-    const float2 cs = tab[u];
+    const float2 cs = AXES ? rope_axis(a, p, u)[u] : tab[u];
     rope_pair(v, w, cs.x, a.sgn * cs.y);
     store_f32(y + i0, v);
     store_f32(y + i1, w);
@@ -136,7 +173,7 @@ __global__ __launch_bounds__(256) void rope_any_kernel(RopeArgs a, int half_layo
   }
 }
 
-template <typename T>
+template <typename T, bool AXES>
 static int rope_launch(const RopeArgs& all, int layout, bool vec, hipStream_t st) {
   const int pieces = !vec ? all.rot / 2 + (all.copy ? all.dim - all.rot : 0)
                      : layout == KH_ROPE_HALF ? all.rot / 16 + (all.copy ? (all.dim - all.rot) / 8 : 0)
@@ -151,11 +188,11 @@ static int rope_launch(const RopeArgs& all, int layout, bool vec, hipStream_t st
     a.pos = all.pos + t0;
     const unsigned blocks = (unsigned)((a.rows * a.heads * pieces + 255) / 256);
     if (!vec)
-      hipLaunchKernelGGL(rope_any_kernel<T>, dim3(blocks), dim3(256), 0, st, a, layout == KH_ROPE_HALF ? 1 : 0, pieces);
+      hipLaunchKernelGGL((rope_any_kernel<T, AXES>), dim3(blocks), dim3(256), 0, st, a, layout == KH_ROPE_HALF ? 1 : 0, pieces);
     else if (layout == KH_ROPE_HALF)
-      hipLaunchKernelGGL((rope_kernel<T, true>), dim3(blocks), dim3(256), 0, st, a, pieces);
+      hipLaunchKernelGGL((rope_kernel<T, true, AXES>), dim3(blocks), dim3(256), 0, st, a, pieces);
     else
-      hipLaunchKernelGGL((rope_kernel<T, false>), dim3(blocks), dim3(256), 0, st, a, pieces);
+      hipLaunchKernelGGL((rope_kernel<T, false, AXES>), dim3(blocks), dim3(256), 0, st, a, pieces);
     KH_LAUNCHED();
   }
   return KH_OK;
@@ -175,6 +212,14 @@ extern "C" int kh_rope_destroy(kh_rope* r) {
 
 extern "C" int kh_rope_create(int rot_dim, int64_t max_pos, int layout, double theta, int scaling, double factor,
                               int64_t original_len, double low, double high, double magnitude, kh_rope** out) {
+  const int all = rot_dim / 2;
+  return kh_rope_create_axes(rot_dim, max_pos, layout, theta, scaling, factor, original_len, low, high, magnitude, 1,
+                             &all, 0, out);
+}
+
+extern "C" int kh_rope_create_axes(int rot_dim, int64_t max_pos, int layout, double theta, int scaling, double factor,
+                                   int64_t original_len, double low, double high, double magnitude, int axes,
+                                   const int32_t* sections_host, int restart, kh_rope** out) {
   KH_CHECK_ARG(out != nullptr, "null output");
   *out = nullptr;
   KH_CHECK_ARG(rot_dim >= 2 && rot_dim <= 1024 && rot_dim % 2 == 0, "rot_dim %d not an even number in [2,1024]",
@@ -190,11 +235,24 @@ extern "C" int kh_rope_create(int rot_dim, int64_t max_pos, int layout, double t
   if (scaling == KH_ROPE_SCALE_BY_PARTS)
     KH_CHECK_ARG(original_len >= 1 && std::isfinite(low) && std::isfinite(high) && high > low,
                  "scaling by parts needs original_len >= 1 and low < high");
+  KH_CHECK_ARG(axes >= 1 && axes <= KH_ROPE_MAX_AXES, "%d axes: 1 to %d are supported", axes, KH_ROPE_MAX_AXES);
+  KH_CHECK_ARG(sections_host != nullptr, "null sections");
   const int half = rot_dim / 2;
+  int64_t pairs = 0;
+  for (int x = 0; x < axes; ++x) {
+    KH_CHECK_ARG(sections_host[x] >= 1, "section %d has %d pairs", x, sections_host[x]);
+    KH_CHECK_ARG(!restart || scaling != KH_ROPE_SCALE_BASE || sections_host[x] > 1,
+                 "a changed base needs sections of more than one pair");
+    pairs += sections_host[x];
+  }
+  KH_CHECK_ARG(pairs == half, "the sections have %lld pairs, rot_dim %d", (long long)pairs, rot_dim);
   double freq[512];
-  const double base = scaling == KH_ROPE_SCALE_BASE ? theta * std::pow(factor, (double)rot_dim / (rot_dim - 2)) : theta;
+  int first = 0, axis = 0;  // of the section whose frequencies pair i's are: its first pair, its axis
   for (int i = 0; i < half; ++i) {
-    double f = std::pow(base, -2.0 * i / rot_dim);
+    if (restart && i == first + sections_host[axis]) first = i, ++axis;
+    const int r = restart ? 2 * sections_host[axis] : rot_dim;
+    const double base = scaling == KH_ROPE_SCALE_BASE ? theta * std::pow(factor, (double)r / (r - 2)) : theta;
+    double f = std::pow(base, -2.0 * (i - first) / r);
     if (scaling == KH_ROPE_SCALE_LINEAR) f /= factor;
     if (scaling == KH_ROPE_SCALE_BY_PARTS) {
       const double turns = f * (double)original_len / (2.0 * 3.14159265358979323846);
@@ -212,6 +270,8 @@ extern "C" int kh_rope_create(int rot_dim, int64_t max_pos, int layout, double t
   r->rot = rot_dim;
   r->layout = layout;
   r->max_pos = max_pos;
+  r->axes = axes;
+  for (int x = 0, n = 0; x < axes; ++x) r->end[x] = n += sections_host[x];
   double* freq_dev = nullptr;
   int rc = KH_OK;
   const int64_t n = max_pos * half;
@@ -291,9 +351,12 @@ extern "C" int kh_rope_apply(const kh_rope* r, int dtype, const void* x_dev, int
   a.rot = r->rot;
   a.sgn = transpose ? -1.0f : 1.0f;
   a.copy = in_place ? 0 : 1;
+  a.ax = rope_axes(r, rows);
   const bool vec = aligned16(x_dev, dtype, x_row_stride, x_head_stride) &&
                    aligned16(y_dev, dtype, y_row_stride, y_head_stride) && head_dim % 8 == 0 &&
                    r->rot % (r->layout == KH_ROPE_HALF ? 16 : 8) == 0;
-  return dtype == KH_DT_F32 ? rope_launch<float>(a, r->layout, vec, as_stream(stream))
-                            : rope_launch<uint16_t>(a, r->layout, vec, as_stream(stream));
+  const hipStream_t st = as_stream(stream);
+  if (r->axes > 1)
+    return dtype == KH_DT_F32 ? rope_launch<float, true>(a, r->layout, vec, st) : rope_launch<uint16_t, true>(a, r->layout, vec, st);
+  return dtype == KH_DT_F32 ? rope_launch<float, false>(a, r->layout, vec, st) : rope_launch<uint16_t, false>(a, r->layout, vec, st);
 }

@@ -11,6 +11,13 @@ way, and attention takes any number of rows per sequence: prompts, chunks of the
     q = rope.apply(q, pos)
     y = cache.attention(q, off, start + n_new, table)
 
+Positions may be evicted by the attention weight that they got, and beams share pages:
+
+    y, lse = cache.attention(q, off, lens, table, return_lse=True)
+    cache.attention_weights(q, lse, off, lens, table, acc)      # every step, or some
+    kept, lens, acc = cache.evict(acc, lens, table, keep=2048, recent=512)
+    table = cache.reorder(table, lens, parent)                  # parent: beam.select's
+
 All compute runs in libklearu_hip.so on the current torch stream of the tensors' device (or
 `stream`).  Rows are tensors [rows, heads, head_dim], f32 or bfloat16, of any non-negative strides
 but 1 along the last dimension.
@@ -146,28 +153,40 @@ class Rope(_Handle):
     INTERLEAVED 2 i with 2 i + 1.  Frequencies theta^(-2 i / rot_dim) are stretched for contexts
     longer than the trained one by `factor`: SCALE_LINEAR all of them, SCALE_BASE through theta,
     SCALE_BY_PARTS those that turn less than `low` times over `original_len` positions, those
-    over `high` turns not, in between in proportion.  `magnitude` scales the rotated elements."""
+    over `high` turns not, in between in proportion.  `magnitude` scales the rotated elements.
+
+    `sections` (up to four numbers of pairs, rot_dim / 2 in all) gives a row a position along as
+    many axes, as images and videos have them: the first sections[0] pairs turn by the first, and
+    so on, and positions are [axes, rows].  Frequencies run on over the sections, or begin again
+    in each (`restart`)."""
 
     _destroy = "kh_rope_destroy"
 
     def __init__(self, rot_dim, max_pos, layout=HALF, theta=10000.0, scaling=SCALE_NONE, factor=1.0, original_len=0,
-                 low=1.0, high=32.0, magnitude=1.0):
+                 low=1.0, high=32.0, magnitude=1.0, sections=None, restart=False):
         h = C.c_void_p()
-        _lib.call("kh_rope_create", rot_dim, max_pos, layout, theta, scaling, factor, original_len, low, high,
-                  magnitude, C.byref(h))
+        sections = (rot_dim // 2,) if sections is None else tuple(sections)
+        if any(not -1 << 31 <= n < 1 << 31 for n in sections):
+            raise ValueError(f"sections: {sections}")
+        _lib.call("kh_rope_create_axes", rot_dim, max_pos, layout, theta, scaling, factor, original_len, low, high,
+                  magnitude, len(sections), (C.c_int32 * len(sections))(*sections), 1 if restart else 0, C.byref(h))
         self._adopt(h)
-        self.rot_dim, self.max_pos, self.layout = rot_dim, max_pos, layout
+        self.rot_dim, self.max_pos, self.layout, self.axes = rot_dim, max_pos, layout, len(sections)
+
+    def _pos(self, n):
+        """The shape of n rows' positions."""
+        return (n,) if self.axes == 1 else (self.axes, n)
 
     def apply(self, x: torch.Tensor, pos: torch.Tensor, out: torch.Tensor | None = None, transpose: bool = False,
               stream=None) -> torch.Tensor:
-        """x [rows, heads, head_dim] rotated by pos [rows] (int64), into `out` (x itself rotates in
-        place) or a new tensor.  `transpose` takes gradients back: the transposed rotation.  Rows of
-        a negative position are padding and left as they were, as are (reported by status()) rows
-        past max_pos; in a new tensor those hold no value."""
+        """x [rows, heads, head_dim] rotated by pos [rows] (int64; with sections [axes, rows]), into
+        `out` (x itself rotates in place) or a new tensor.  `transpose` takes gradients back: the
+        transposed rotation.  Rows of a negative position are padding and left as they were, as are
+        (reported by status()) rows past max_pos; in a new tensor those hold no value."""
         dev = self._dev
         xp, x0, x1, dt = _rows(x, "x", dev)
         n, heads, dim = x.shape
-        pp = _index(pos, "pos", dev, _I64, (n,))
+        pp = _index(pos, "pos", dev, _I64, self._pos(n))
         if stream is not None or _raw_device() != dev:
             with _On(self.device, stream, (x, pos, out)):
                 return self.apply(x, pos, out, transpose)
@@ -213,8 +232,8 @@ class PagedKv(_Handle):
     def append(self, k: torch.Tensor, v: torch.Tensor, off: torch.Tensor, start: torch.Tensor, table: torch.Tensor,
                rope: Rope | None = None, pos: torch.Tensor | None = None, stream=None) -> None:
         """Row off[b] + i of k and v [rows, num_kv_heads, head_dim] becomes position start[b] + i of
-        sequence b; `rope` rotates the keys on the way, by pos [rows] or by their places in the
-        cache.  Two rows of one call must not have the same place."""
+        sequence b; `rope` rotates the keys on the way, by pos [rows] (with sections [axes, rows]) or
+        by their places in the cache.  Two rows of one call must not have the same place."""
         dev = self._dev
         kp, k0, k1, dt = _rows(k, "k", dev)
         vp, v0, v1, _ = _rows(v, "v", dev, k.dtype)
@@ -225,7 +244,7 @@ class PagedKv(_Handle):
         batch, op, sp, tp, cols, ts = self._places(off, start, table)
         if pos is not None and rope is None:
             raise ValueError("pos: rotary positions without a rotation")
-        pp = None if pos is None else _index(pos, "pos", dev, _I64, (n,))
+        pp = None if pos is None else _index(pos, "pos", dev, _I64, rope._pos(n))
         if stream is not None or _raw_device() != dev:
             with _On(self.device, stream, (k, v, off, start, table, pos)):
                 return self.append(k, v, off, start, table, rope, pos)
@@ -306,15 +325,115 @@ class PagedKv(_Handle):
             need, _raw_stream(dev)))
         return (out, lse) if return_lse else out
 
-    def _workspace(self, *sizes) -> int:
-        """kh_paged_kv_attention_workspace: bytes by the call's sizes."""
-        need = self._ws.get(sizes)
+    def attention_weights(self, q: torch.Tensor, lse: torch.Tensor, off: torch.Tensor, lens: torch.Tensor,
+                          table: torch.Tensor, acc: torch.Tensor | None = None, scale: float | None = None,
+                          causal: bool = True, window: int = 0, max_rows: int | None = None, max_len: int | None = None,
+                          stream=None) -> torch.Tensor:
+        """Adds the attention weight that each cached position gets from rows q to acc [batch,
+        num_kv_heads, columns] (f32; default: zeros for the table's reach), summed over the rows and
+        the query heads of a kv head.  lse [rows, num_heads] is attention(return_lse=True)'s of the
+        same rows and arguments: heads that it gave -inf (not listed, nothing seen) add nothing.
+        Returns acc.  evict() takes it."""
+        dev = self._dev
+        qp, q0, q1, dt = _rows(q, "q", dev)
+        n, nh, dim = q.shape
+        if dim != self.head_dim:
+            raise ValueError(f"q: head_dim {dim}, expected {self.head_dim}")
+        batch, op, lp, tp, cols, ts = self._places(off, lens, table)
+        sp = _index(lse, "lse", dev, torch.float32, (n, nh))
+        if acc is not None:
+            self._weights(acc, "acc", batch)
+        if stream is not None or _raw_device() != dev:
+            with _On(self.device, stream, (q, lse, off, lens, table, acc)):
+                return self.attention_weights(q, lse, off, lens, table, acc, scale, causal, window, max_rows, max_len)
+        if max_rows is None:
+            max_rows = -(-n // max(1, batch))
+        if max_len is None:
+            max_len = cols * self.page_size
+        if scale is None:
+            scale = dim ** -0.5
+        need = self._workspace(dt, n, batch, nh, max_rows, max_len, name="kh_paged_kv_weights_workspace")
+        if acc is None:
+            acc = torch.zeros((batch, self.num_kv_heads, cols * self.page_size), dtype=torch.float32, device=self.device)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        _check(self._lib.kh_paged_kv_weights(
+            self._h, dt, qp, q0, q1, nh, n, op, batch, lp, tp, cols, ts, max_rows, max_len, scale, 1 if causal else 0, window,
+            sp, acc.data_ptr(), acc.shape[2], None if ws is None else ws.data_ptr(), need, _raw_stream(dev)))
+        return acc
+
+    def evict(self, acc: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, keep: int, recent: int = 0,
+              first: int = 0, out: torch.Tensor | None = None, stream=None):
+        """Cuts sequences of more than `keep` positions to that: every kv head keeps its `first` and
+        `recent` (last) positions and, of the others, those with the largest acc [batch,
+        num_kv_heads, columns] (of equal ones the first), moved together in their order; what lies
+        behind them is free.  A sequence's pages must be its own, as for append.  Their places are no longer their positions in the text: append(pos=...)
+        and apply() take those.  Returns (kept, lens, acc): kept [batch, num_kv_heads, keep] (int32)
+        where each position was, -1 past a sequence's end; the new lengths; the weights of
+        what is left, then 0, in `out` (acc itself may be it) or a new tensor."""
+        dev = self._dev
+        batch = lens.shape[0]
+        lp = _index(lens, "lens", dev, _I64, (batch,))
+        tp, cols, ts = _table(table, dev, batch)
+        ap, n = self._weights(acc, "acc", batch)
+        if out is not None and out.shape != acc.shape:
+            raise ValueError(f"out: shape {tuple(out.shape)}, expected {tuple(acc.shape)}")
+        yp = None if out is None else self._weights(out, "out", batch)[0]
+        if stream is not None or _raw_device() != dev:
+            with _On(self.device, stream, (acc, lens, table, out)):
+                return self.evict(acc, lens, table, keep, recent, first, out)
+        need = self._workspace(batch, keep, n, name="kh_paged_kv_evict_workspace")
+        if out is None:
+            out = torch.empty_like(acc)
+            yp = out.data_ptr()
+        kept = torch.empty((batch, self.num_kv_heads, keep), dtype=_I32, device=self.device)
+        left = torch.empty_like(lens)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        _check(self._lib.kh_paged_kv_evict(self._h, ap, n, lp, batch, tp, cols, ts, keep, recent, first, kept.data_ptr(),
+                                           yp, left.data_ptr(), None if ws is None else ws.data_ptr(), need,
+                                           _raw_stream(dev)))
+        return kept, left, out
+
+    def reorder(self, table: torch.Tensor, lens: torch.Tensor, parent: torch.Tensor, out: torch.Tensor | None = None,
+                stream=None) -> torch.Tensor:
+        """The page table of beams that go on from others: row b * beams + i of table [batch *
+        beams, columns] is beam i of sequence b, whose beams are lens[b] positions long, and goes on
+        from beam parent[b, i] (int32, [batch, beams]).  Whole pages are shared; of the others each
+        beam has its own again, with a copy of what its parent held in the one that is begun (beams
+        that nobody goes on from give theirs).  Returns the new table, in `out` or a new tensor."""
+        dev = self._dev
+        if parent.dim() != 2:
+            raise ValueError(f"parent: expected [batch, beams], got {tuple(parent.shape)}")
+        batch, beams = parent.shape
+        pp = _index(parent, "parent", dev, _I32, (batch, beams))
+        lp = _index(lens, "lens", dev, _I64, (batch,))
+        tp, cols, ts = _table(table, dev, batch * beams)
+        if out is not None:
+            yp, ocols, ys = _table(out, dev, batch * beams)
+            if ocols != cols:
+                raise ValueError(f"out: {ocols} columns, expected {cols}")
+        if stream is not None or _raw_device() != dev:
+            with _On(self.device, stream, (table, lens, parent, out)):
+                return self.reorder(table, lens, parent, out)
+        if out is None:
+            out = torch.empty_strided((batch * beams, cols), (cols, 1), dtype=_I32, device=self.device)
+            yp, ys = out.data_ptr(), cols
+        _check(self._lib.kh_paged_kv_reorder(self._h, tp, cols, ts, lp, batch, beams, pp, yp, ys, _raw_stream(dev)))
+        return out
+
+    def _weights(self, t: torch.Tensor, what: str, batch: int):
+        """(pointer, columns) of weights [batch, num_kv_heads, columns]."""
+        n = t.shape[-1] if t.dim() == 3 else 0
+        return _index(t, what, self._dev, torch.float32, (batch, self.num_kv_heads, n)), n
+
+    def _workspace(self, *sizes, name="kh_paged_kv_attention_workspace") -> int:
+        """What the entry point `name` says: bytes by the call's sizes."""
+        need = self._ws.get((name, sizes))
         if need is None:
             x = C.c_int64()
-            _check(self._lib.kh_paged_kv_attention_workspace(self._h, *sizes, C.byref(x)))
+            _check(getattr(self._lib, name)(self._h, *sizes, C.byref(x)))
             if len(self._ws) >= 1024:
                 self._ws.clear()
-            need = self._ws[sizes] = x.value
+            need = self._ws[name, sizes] = x.value
         return need
 
     def status(self):
