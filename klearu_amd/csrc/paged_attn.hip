@@ -618,15 +618,6 @@ struct PtShape {
 };
 
 typedef int kh_i32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 kh_f16x2 __attribute__((ext_vector_type(2)));
-
-// Nibble n of each half of w as 16 + c, a pair of f16: six bits up it counts ones
-// behind the bits of 16.
-__device__ __forceinline__ kh_f16x2 codes_f16(uint32_t w, int n) {
-  const uint32_t x = n == 0 ? w << 6 : n == 1 ? w << 2 : n == 2 ? w >> 2 : w >> 6;
-  return __builtin_bit_cast(kh_f16x2, (x & 0x03c003c0u) | 0x4c004c00u);
-}
-
 template <int D, int KT>
 struct PtCodes {
   using S = PtShape<D, KT>;

@@ -630,7 +630,8 @@ extern "C" int kh_paged_kv_create(int num_kv_heads, int head_dim, int page_size,
     KH_HIP(hipMemset(c->pool, 0, bytes));
     KH_HIP(hipMemset(c->err, 0, sizeof(int)));
     KH_HIP(hipStreamSynchronize(nullptr));
-    return paged_attn_prepare(c->d);
+    const int rc = paged_attn_prepare(c->d);
+    return rc != KH_OK ? rc : paged_weights_prepare(c->d);
   };
   const int rc = fill();
   if (rc != KH_OK) {

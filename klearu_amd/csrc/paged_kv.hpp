@@ -103,6 +103,7 @@ constexpr int64_t kGridThreads = ((int64_t)1 << 32) - 1;
 
 // What the attention kernels of a head_dim need of the current device.
 int paged_attn_prepare(int d);
+int paged_weights_prepare(int d);
 
 inline size_t dtype_bytes(int dtype) { return dtype == KH_DT_F32 ? 4 : 2; }
 

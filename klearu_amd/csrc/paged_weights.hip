@@ -2,16 +2,19 @@
 //
 //   acc[j] += sum_i exp(c q_i . k_j - lse_i)   over the rows i (and query heads) that see position j
 //
-// The log-sum-exps are known, so positions are independent of each other: a wave holds the keys of
-// its positions in registers and runs the rows over them; nothing is joined, and each
-// sum has one owner and one order.  With group sums A_g = sum_{d in g} q_d c_d of the codes, which
-// are exact BF16 numbers,
-//   log2(e) (c q . k - lse) = sum_g (c' s_g) A_g + [sum_g m_g (c' Q_g) - lse'],   Q_g = sum_{d in g} q_d
-// where the bracket is one more matrix product, of the BF16 minima with three BF16 terms of c' Q_g
-// and of lse' (three hold all bits of an f32; c' = c log2 e).
+// The log-sum-exps are known, so positions are independent of each other: nothing is carried
+// from one to the next, and each sum has one owner and one order.
 //
-// Scores come out of the matrix core with positions along lanes and rows along registers, so a
-// sum over rows stays in its lane until the end.
+// Scores come from the f16 matrix core without a rounding of either side that an f32 would not have:
+// with codes c, scale s and minimum m of a group, k = s (c - 8) + m + 8 s, where s (c - 8) has 11
+// significant bits, as f16 has, and
+//   q . k = sum_g [sum_{d in g} q_d s_g (c_d - 8)] + sum_g m_g Q_g + sum_g 8 s_g Q_g,   Q_g = sum_{d in g} q_d
+// is one chain of products, the last two sums with Q_g in three f16 terms.  A position's numbers are scaled by
+// a power of two of its own, and a row's by one of its own (of its tile of 16 rows, where those are alike),
+// so that what falls below f16's smallest number is less than 2^-32 of the largest.  f32 rows take three terms.
+//
+// Rows lie along the registers of a product and positions along its lanes, so that a sum over
+// rows stays in its lane until the end.
 #include <algorithm>
 #include <cmath>
 
@@ -21,6 +24,7 @@ namespace kh {
 
 constexpr int kWtWaves = 4;
 constexpr float kWtNone = 0x1p100f;  // a log-sum-exp whose rows add nothing
+constexpr int kWtNear = 7;           // powers of two between the largest and the smallest row of a tile with one scale
 
 struct WtArgs {
   const char* pool;
@@ -41,192 +45,567 @@ struct WtArgs {
   float* acc;
   int64_t acc_cols;
   int qvec;
+  char* tiles;      // row tiles as WtTile lays them out
+  float* part;      // [batch][kv heads][chunks][part_len] sums of chunks of rows
+  int chunks, chunk, part_len;  // chunks of a sequence's rows, their row tiles, and the positions that have them
 };
 
-// A tile of 16 rows (of the heads of a kv head, row after row) as first operands: the
-// queries' terms, slots (0,4,1,5,2,6,3,7) of eight neighbouring elements as codes2 gives the codes, and the bracket's.
+typedef _Float16 kh_f16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ kh_f32x4 mfma16h(const uint4& a, const uint4& b, kh_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(kh_f16x8, a), __builtin_bit_cast(kh_f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t f16x2(float x, float y) {
+  const kh_f16x2 h = {(_Float16)x, (_Float16)y};
+  return __builtin_bit_cast(uint32_t, h);
+}
+// Eight f32 in f16 terms: x = t[0] + t[1] + ...
+template <int NT>
+__device__ __forceinline__ void terms8h(const float (&f)[8], uint4 (&t)[NT]) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = f[i];
+#pragma unroll
+  for (int k = 0; k < NT; ++k) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = f16x2(r[2 * i], r[2 * i + 1]);
+      const kh_f16x2 h = __builtin_bit_cast(kh_f16x2, w[i]);
+      r[2 * i] -= (float)h.x;
+      r[2 * i + 1] -= (float)h.y;
+    }
+    t[k] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+// The power of two that a number's exponent is, between 2^lo and 2^hi; 0 and subnormals: 2^lo.
+__device__ __forceinline__ int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23 & 0xff) - 127; }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// A tile of 16 rows (of the heads of a kv head, row after row) as first operands, lane by lane.
 template <int D, typename T>
 struct WtRows {
   static constexpr int NG = D / kKvGroup, NQ = sizeof(T) == 4 ? 3 : 1;
-  uint4 q[NG][NQ], base;
+  static constexpr int NB = NG == 8 ? 2 : 1;  // operands of the sums over groups: eight numbers each
+  static constexpr int NF = NG * NQ + NB;
+  static constexpr int kBytes = NF * 1024 + 256;  // in memory: the operands, scales and log-sum-exps of 16 rows, `one`
+  uint4 x[NF];      // the groups' terms, slots (0,4,1,5,2,6,3,7) of eight elements as codes_f16 gives codes; sums
+  float r, nl;      // of row lane % 16: its scale, and minus its log-sum-exp in powers of two
+  bool one;         // all rows have the first one's scale
   __device__ __forceinline__ void load(const WtArgs& a, int64_t o0, int nr, int h, int tile, int lane) {
     const int g = lane >> 4, rr = tile * 16 + (lane & 15);
     const bool inside = rr < nr;
     const int i = (int)((uint32_t)(inside ? rr : 0) / (uint32_t)a.gs);
     const int head = h * a.gs + ((inside ? rr : 0) - i * a.gs);
     const int64_t t = o0 + i;
-    const T* x = static_cast<const T*>(a.q) + t * a.qs + head * a.qh;
+    const T* q = static_cast<const T*>(a.q) + t * a.qs + head * a.qh;
     Raw8<T> raw[NG];
 #pragma unroll
-    for (int j = 0; j < NG; ++j) raw[j].load(x + 32 * j + 8 * g, a.qvec);
+    for (int j = 0; j < NG; ++j) raw[j].load(q + 32 * j + 8 * g, a.qvec);
     const float lse = a.lse[t * a.nh + head];
     const bool on = inside && !__builtin_isinf(lse);
-    float e[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    nl = on ? -lse * kLog2e : -kWtNone;
+    float top = 0.0f;  // of the row's finite elements
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       float f[8];
       raw[j].get(f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = on ? f[k] : 0.0f;
+      for (int k = 0; k < 8; ++k) {
+        const float y = __builtin_fabsf(f[k]);
+        top = on && y < INFINITY ? fmaxf(top, y) : top;
+      }
+    }
+    top = across_groups_max(top);
+    // elements below 2^9, so that sums of 32 are below 2^14
+    int e = min(max(exponent_of(top) - 8, -100), 118);
+    const int most = (int)wave_max_u32((uint32_t)(top > 0.0f ? e + 128 : 0)) - 128;
+    one = __ballot(top > 0.0f && e < most - kWtNear) == 0;
+    if (one) e = max(most, -100);
+    r = pow2(e);
+    const float down = pow2(-e);
+    float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      float f[8];
+      raw[j].get(f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = on ? f[k] * down : 0.0f;
       const float s[8] = {f[0], f[4], f[1], f[5], f[2], f[6], f[3], f[7]};
-      terms8<NQ>(s, q[j]);
-      e[j] = a.c1 * across_groups_sum(((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7])));
+      uint4 tm[NQ];
+      terms8h<NQ>(s, tm);
+#pragma unroll
+      for (int k = 0; k < NQ; ++k) x[j * NQ + k] = tm[k];
+      sums[j] = across_groups_sum(((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7])));
+    }
+    if constexpr (NB == 1) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sums[j + NG] = sums[j];  // NG is 4 or 2: of eight numbers, the minima's and the scales'
     }
     uint4 tm[3];
-    terms8<3>(e, tm);
-    const float l0 = on ? -lse * kLog2e : -kWtNone;
-    const float t0 = bf16_to_f32(f32_to_bf16(l0)), t1 = bf16_to_f32(f32_to_bf16(l0 - t0)), t2 = l0 - t0 - t1;
-    const uint4 tl = make_uint4(cvt_bf16x2(t0, t1), cvt_bf16x2(t2, 0.0f), 0, 0);
-    base = g == 0 ? tm[0] : g == 1 ? tm[1] : g == 2 ? tm[2] : tl;
+    terms8h<3>(sums, tm);
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < NB; ++k) x[NG * NQ + k] = g == 0 ? tm[0] : g == 1 ? tm[1] : g == 2 ? tm[2] : zero;
   }
 };
 
 // The keys of 16 positions as second operands, a position a column.
 template <int D>
 struct WtKeys {
-  static constexpr int NG = D / kKvGroup;
-  uint4 c[NG], m;
-  float s[NG];
+  static constexpr int NG = D / kKvGroup, NB = NG == 8 ? 2 : 1;
+  uint4 c[NG], b[NB];
+  float f;  // the position's scale, times c1
   __device__ __forceinline__ void put(const uint32_t (&w)[NG], const uint32_t (&p)[NG], float c1, int g) {
-    uint32_t e[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    float top = 0.0f, s[NG], m[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      c[j] = make_uint4(codes2<0>(w[j], 0), codes2<0>(w[j], 1), codes2<0>(w[j], 2), codes2<0>(w[j], 3));
-      s[j] = c1 * __uint_as_float(p[j] & 0xffff0000u);
-      e[j] = p[j] & 0xffffu;
+      s[j] = __uint_as_float(p[j] & 0xffff0000u);
+      m[j] = __uint_as_float(p[j] << 16);
+      top = fmaxf(top, fmaxf(8.0f * s[j], __builtin_fabsf(m[j])));  // a NaN is passed over
     }
-    m = g == 3 ? make_uint4(0x3f803f80u, 0x00003f80u, 0, 0)
-               : make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+    const int e = max(exponent_of(top) - 13, -100);
+    const float down = pow2(-e);
+    f = c1 * pow2(e);
+    uint32_t mh[NG], sh[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const float sd = s[j] * down;
+      const _Float16 s1 = (_Float16)sd;
+      const kh_f16x2 s2 = {s1, s1}, eight = {(_Float16)-24.0f, (_Float16)-24.0f};
+      uint32_t v[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) v[n] = __builtin_bit_cast(uint32_t, (codes_f16(w[j], n) + eight) * s2);
+      c[j] = make_uint4(v[0], v[1], v[2], v[3]);
+      mh[j] = f16x2(m[j] * down, 0.0f);
+      sh[j] = f16x2(8.0f * sd, 0.0f);
+    }
+    if constexpr (NG == 2) {
+      b[0] = make_uint4(mh[0] | mh[1] << 16, sh[0] | sh[1] << 16, 0, 0);
+    } else if constexpr (NG == 4) {
+      b[0] = make_uint4(mh[0] | mh[1] << 16, mh[2] | mh[3] << 16, sh[0] | sh[1] << 16, sh[2] | sh[3] << 16);
+    } else {
+      b[0] = make_uint4(mh[0] | mh[1] << 16, mh[2] | mh[3] << 16, mh[4] | mh[5] << 16, mh[6] | mh[7] << 16);
+      b[1] = make_uint4(sh[0] | sh[1] << 16, sh[2] | sh[3] << 16, sh[4] | sh[5] << 16, sh[6] | sh[7] << 16);
+    }
+    // the terms' slots: group 3 of the lanes has none (a NaN scale is a NaN in the codes' products)
+    if (g == 3) {
+#pragma unroll
+      for (int k = 0; k < NB; ++k) b[k] = make_uint4(0, 0, 0, 0);
+    }
   }
 };
 
-// Block: 4 waves with NPT tiles of 16 positions each, of one kv head of one sequence.
+// q . k of a tile of rows and one of positions, both scaled.
+template <int D, typename T>
+__device__ __forceinline__ kh_f32x4 wt_scores(const uint4 (&x)[WtRows<D, T>::NF], const WtKeys<D>& k) {
+  using R = WtRows<D, T>;
+  kh_f32x4 y = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < R::NB; ++i) y = mfma16h(x[R::NG * R::NQ + i], k.b[i], y);
+#pragma unroll
+  for (int j = 0; j < R::NG; ++j)
+#pragma unroll
+    for (int i = R::NQ - 1; i >= 0; --i) y = mfma16h(x[j * R::NQ + i], k.c[j], y);
+  return y;
+}
+// The weights of four rows for the lane's position.
+__device__ __forceinline__ void wt_weights(const kh_f32x4& y, float f, bool one, const float (&r)[4], const float (&nl)[4], float (&w)[4]) {
+  if (one) {
+    const float fr = f * r[0];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(y[i], fr, nl[i]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(y[i] * f, r[i], nl[i]));
+  }
+}
+
+// A sequence of the call.
+struct WtSeq {
+  const int32_t* table;
+  int64_t o0, before;  // its first row; that row's position
+  int n, nr, E;        // rows, times heads; positions that are added up
+};
+__device__ __forceinline__ bool wt_seq(const WtArgs& a, int64_t b, bool tell, WtSeq& s) {
+  int64_t o0 = a.off[b], o1 = a.off[b + 1], L = a.len[b];
+  const int64_t cap = a.cols << a.ps_log2;
+  o0 = o0 < 0 ? 0 : o0;
+  o1 = o1 > a.rows ? a.rows : o1;
+  if (o1 <= o0) return false;
+  if (L < 0 || L > min(cap, a.acc_cols)) {
+    if (tell) atomicOr(a.err, 1);
+    L = L < 0 ? 0 : min(L, cap);
+  }
+  s.table = a.table + b * a.table_stride;
+  s.o0 = o0;
+  s.n = (int)(o1 - o0);
+  s.nr = s.n * a.gs;
+  s.before = L - s.n;
+  s.E = (int)min(L, a.acc_cols);
+  return true;
+}
+// The rows (times heads) that see position j: [lo, hi).
+__device__ __forceinline__ void wt_span(const WtArgs& a, const WtSeq& s, int j, int& lo, int& hi) {
+  const int64_t x = a.causal ? max(j - s.before, (int64_t)0) : 0;
+  const int64_t y = a.window > 0 ? min(j + a.window - s.before, (int64_t)s.n) : s.n;
+  const bool some = y > x;
+  lo = some ? (int)(x * a.gs) : 0;
+  hi = some ? (int)(y * a.gs) : 0;
+}
+
+// NPT tiles of 16 positions from `base` on: their keys, who sees them, and the ranges of that.
+template <int D, int NPT>
+struct WtCols {
+  WtKeys<D> x[NPT];
+  int lo[NPT], hi[NPT];
+  int all_lo, all_hi, some_lo, some_hi;  // all_lo > all_hi where a key holds a NaN: see wt_hide
+  __device__ __forceinline__ void load(const WtArgs& a, const WtSeq& s, int h, int base, int lane) {
+    using P = KvParts<D>;
+    constexpr int NG = P::NG;
+    const int g = lane >> 4, col = lane & 15, ps = 1 << a.ps_log2;
+    uint32_t al = 0, ah = 0x7fffffffu, sl = 0x7fffffffu, sh = 0;
+    uint32_t w[NPT][NG], p[NPT][NG];
+#pragma unroll
+    for (int t = 0; t < NPT; ++t) {
+      const int tok = base + 16 * t, j = tok + col;
+      wt_span(a, s, j, lo[t], hi[t]);
+      if (j >= s.E) lo[t] = hi[t] = 0;
+#pragma unroll
+      for (int k = 0; k < NG; ++k) w[t][k] = p[t][k] = 0;
+      if (__ballot(hi[t] > lo[t])) {  // tables need not name pages that no row sees
+        const int pg = __builtin_amdgcn_readfirstlane(s.table[tok >> a.ps_log2]);
+        if (pg >= 0 && pg < a.pages) {
+          const char* blk = a.pool + ((int64_t)pg * a.nkv + h) * a.block;
+          const int at = (tok & (ps - 1)) + col;
+          ld_words<NG>(blk + P::kc() + at * (D / 2) + g * NG * 4, w[t]);
+          ld_words<NG>(blk + P::kp(ps) + at * NG * 4, p[t]);
+        } else {
+          if (lane == 0) atomicOr(a.err, 2);
+          lo[t] = hi[t] = 0;
+        }
+      }
+      if (hi[t] > lo[t]) sl = min(sl, (uint32_t)lo[t]), sh = max(sh, (uint32_t)hi[t]);
+      if (j < s.E) al = max(al, (uint32_t)lo[t]), ah = min(ah, (uint32_t)hi[t]);  // other columns' sums go nowhere
+    }
+#pragma unroll
+    for (int t = 0; t < NPT; ++t) x[t].put(w[t], p[t], a.c1, g);
+    all_lo = (int)wave_max_u32(al);
+    all_hi = (int)wave_min_u32(ah);
+    some_lo = (int)wave_min_u32(sl);
+    some_hi = (int)wave_max_u32(sh);
+    uint32_t nan = 0;
+#pragma unroll
+    for (int t = 0; t < NPT; ++t)
+#pragma unroll
+      for (int k = 0; k < NG; ++k) nan = max(nan, p[t][k]);
+    if (__ballot(nan >= 0x7f800000u)) all_lo = 0x7fffffff;
+  }
+};
+// Leaves the weights of rows that see the lane's position, and that add anything: 0 times a NaN is one.
+__device__ __forceinline__ void wt_hide(int r0, int g, int lo, int hi, const float (&nl)[4], float (&w)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int rr = r0 + 4 * g + i;
+    w[i] = rr >= lo && rr < hi && nl[i] != -kWtNone ? w[i] : 0.0f;
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+// A wave keeps a tile of rows and takes the positions of its part, NPT tiles at a time.
 template <int D, typename T, int NPT>
 __global__ __launch_bounds__(64 * kWtWaves) void paged_weights_kernel(WtArgs a) {
-  using P = KvParts<D>;
-  constexpr int NG = D / kKvGroup, NQ = WtRows<D, T>::NQ, BP = 16 * NPT * kWtWaves;
+  constexpr int STEP = 16 * NPT;
   const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.y, ps = 1 << a.ps_log2;
-  const int64_t cap = a.cols << a.ps_log2;
+  const int h = blockIdx.y;
   for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
-    const int32_t* __restrict__ table = a.table + b * a.table_stride;
-    int64_t o0 = a.off[b], o1 = a.off[b + 1], L = a.len[b];
-    o0 = o0 < 0 ? 0 : o0;
-    o1 = o1 > a.rows ? a.rows : o1;
-    if (o1 <= o0) continue;
-    const int n = (int)(o1 - o0), nr = n * a.gs;
-    if (L < 0 || L > min(cap, a.acc_cols)) {
-      if (threadIdx.x == 0) atomicOr(a.err, 1);
-      L = L < 0 ? 0 : min(L, cap);
-    }
-    const int64_t before = L - n;  // the first row's position
-    const int E = (int)min(L, a.acc_cols);
+    WtSeq s;
+    if (!wt_seq(a, b, threadIdx.x == 0 && blockIdx.x == 0 && h == 0, s)) continue;
     float* acc = a.acc + (b * a.nkv + h) * a.acc_cols;
-    for (int64_t pb = blockIdx.x; pb * BP < E; pb += gridDim.x) {
-      const int base = (int)(pb * BP) + wave * 16 * NPT;
-      WtKeys<D> x[NPT];
-      int rlo[NPT], rhi[NPT];  // the rows (times heads) that see the lane's position
-      float sum[NPT], old[NPT];
-      uint32_t all_lo = 0, all_hi = 0x7fffffffu, some_lo = 0x7fffffffu, some_hi = 0;
+    for (int tile = 0; tile * 16 < s.nr; ++tile) {
+      WtRows<D, T> q;
+      q.load(a, s.o0, s.nr, h, tile, lane);
+      float r[4], nl[4];
 #pragma unroll
-      for (int t = 0; t < NPT; ++t) {
-        const int tok = base + 16 * t, j = tok + col;
-        sum[t] = old[t] = 0.0f;
-        rlo[t] = 0;
-        rhi[t] = 0x7fffffff;  // a column that is no position: its sum goes nowhere
-        int64_t lo = a.causal ? max(j - before, (int64_t)0) : 0;
-        int64_t hi = a.window > 0 ? min(j + a.window - before, (int64_t)n) : n;
-        if (hi <= lo) lo = hi = 0;
-        uint32_t w[NG], p[NG];
-#pragma unroll
-        for (int k = 0; k < NG; ++k) w[k] = p[k] = 0;
-        if (__ballot(j < E && hi > lo)) {  // tables need not name pages that no row sees
-          const int pg = __builtin_amdgcn_readfirstlane(table[tok >> a.ps_log2]);
-          if (pg >= 0 && pg < a.pages) {
-            const char* blk = a.pool + ((int64_t)pg * a.nkv + h) * a.block;
-            const int at = (tok & (ps - 1)) + col;
-            ld_words<NG>(blk + P::kc() + at * (D / 2) + g * NG * 4, w);
-            ld_words<NG>(blk + P::kp(ps) + at * NG * 4, p);
-            if (j < E) {
-              old[t] = acc[j];
-              some_lo = min(some_lo, hi > lo ? (uint32_t)(lo * a.gs) : 0x7fffffffu);
-              some_hi = max(some_hi, (uint32_t)(hi * a.gs));
-            }
-          } else {
-            if (lane == 0) atomicOr(a.err, 2);
-            lo = hi = 0;
-          }
-        } else {
-          lo = hi = 0;
-        }
-        if (j < E) {
-          rlo[t] = (int)(lo * a.gs);
-          rhi[t] = (int)(hi * a.gs);
-        }
-        all_lo = max(all_lo, (uint32_t)rlo[t]);
-        all_hi = min(all_hi, (uint32_t)rhi[t]);
-        x[t].put(w, p, a.c1, g);
+      for (int i = 0; i < 4; ++i) {
+        r[i] = __shfl(q.r, 4 * g + i);
+        nl[i] = __shfl(q.nl, 4 * g + i);
       }
-      all_lo = wave_max_u32(all_lo);
-      all_hi = wave_min_u32(all_hi);
-      some_lo = wave_min_u32(some_lo);
-      some_hi = wave_max_u32(some_hi);
-      for (int rt = (int)(some_lo >> 4); rt * 16 < (int)some_hi; ++rt) {
-        WtRows<D, T> r;
-        r.load(a, o0, nr, h, rt, lane);
-        const bool whole = rt * 16 >= (int)all_lo && min(rt * 16 + 16, nr) <= (int)all_hi;
+      const int r0 = tile * 16, r1 = min(r0 + 16, s.nr);
+      for (int base = (blockIdx.x * kWtWaves + wave) * STEP; base < s.E; base += gridDim.x * kWtWaves * STEP) {
+        WtCols<D, NPT> k;
+        float old[NPT];
+#pragma unroll
+        for (int t = 0; t < NPT; ++t) old[t] = acc[min(base + 16 * t + col, s.E - 1)];
+        k.load(a, s, h, base, lane);
+        const bool whole = r0 >= k.all_lo && r1 <= k.all_hi;
 #pragma unroll
         for (int t = 0; t < NPT; ++t) {
-          const kh_f32x4 zero = {0, 0, 0, 0};
-          kh_f32x4 y = mfma16(r.base, x[t].m, zero);
-#pragma unroll
-          for (int j = 0; j < NG; ++j) {
-            kh_f32x4 c = zero;
-#pragma unroll
-            for (int k = NQ - 1; k >= 0; --k) c = mfma16(r.q[j][k], x[t].c[j], c);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = fmaf(x[t].s[j], c[i], y[i]);
-          }
           float w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(y[i]);
-          if (!whole) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int rr = rt * 16 + 4 * g + i;
-              w[i] = rr >= rlo[t] && rr < rhi[t] ? w[i] : 0.0f;
-            }
-          }
-          sum[t] += (w[0] + w[1]) + (w[2] + w[3]);
+          wt_weights(wt_scores<D, T>(q.x, k.x[t]), k.x[t].f, q.one, r, nl, w);
+          if (!whole) wt_hide(r0, g, k.lo[t], k.hi[t], nl, w);
+          const float sum = across_groups_sum((w[0] + w[1]) + (w[2] + w[3]));
+          const int j = base + 16 * t + col;
+          if (g == 0 && j < s.E && sum != 0.0f) acc[j] = old[t] + sum;
         }
       }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- many rows
+// Row tiles go to the workspace as operands once, and the blocks of positions read them from there: a
+// wave keeps the keys of its positions, and all waves of a block run the same row tiles over them through
+// LDS, kWtGroup at a time.  The place of a sequence's tiles: every sequence may begin one that is not full.
+__device__ __forceinline__ int64_t wt_slot(const WtArgs& a, int64_t b, int64_t o0, int tile) {
+  return o0 * a.gs / 16 + b + tile;
+}
+
+template <int D, typename T>
+__global__ __launch_bounds__(256) void paged_weights_rows_kernel(WtArgs a) {
+  using R = WtRows<D, T>;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y;
+  for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
+    WtSeq s;
+    if (!wt_seq(a, b, false, s)) continue;
+    for (int tile = blockIdx.x * 4 + wave; tile * 16 < s.nr; tile += gridDim.x * 4) {
+      R q;
+      q.load(a, s.o0, s.nr, h, tile, lane);
+      char* to = a.tiles + (wt_slot(a, b, s.o0, tile) * a.nkv + h) * R::kBytes;
 #pragma unroll
-      for (int t = 0; t < NPT; ++t) {
-        const int j = base + 16 * t + col;
-        const float s = across_groups_sum(sum[t]);
-        if (g == 0 && j < E && rhi[t] > rlo[t]) acc[j] = old[t] + s;
-      }
+      for (int i = 0; i < R::NF; ++i) *reinterpret_cast<uint4*>(to + i * 1024 + lane * 16) = q.x[i];
+      float* x = reinterpret_cast<float*>(to + R::NF * 1024);
+      if (lane < 16) x[lane] = q.r;
+      else if (lane < 32) x[lane] = q.nl;
+      else if (lane == 32) x[lane] = q.one ? 1.0f : 0.0f;
     }
   }
 }
 
 template <int D, typename T>
-static int wt_launch(const WtArgs& a, int64_t max_len, hipStream_t st) {
-  constexpr int NPT = 2, BP = 16 * NPT * kWtWaves;
-  const int64_t most = std::min(std::min(max_len, a.acc_cols), a.cols << a.ps_log2);
-  const dim3 g((unsigned)std::max<int64_t>(std::min<int64_t>((most + BP - 1) / BP, 65535), 1), (unsigned)a.nkv,
-               (unsigned)std::min<int64_t>(a.batch, 65535));
-  hipLaunchKernelGGL((paged_weights_kernel<D, T, NPT>), g, dim3(64 * kWtWaves), 0, st, a);
+struct WtShape {
+  static constexpr int NPT = D == 256 || sizeof(T) == 4 ? 2 : 4;
+  static constexpr int kGroup = D == 256 || sizeof(T) == 4 ? 2 : 4;  // row tiles between two barriers
+  static constexpr int kStep = kGroup * WtRows<D, T>::kBytes, kLds = 2 * kStep;
+  static constexpr int BP = 16 * NPT * kWtWaves;
+};
+
+template <int D, typename T>
+__global__ __launch_bounds__(64 * kWtWaves, 2) void paged_weights_tiles_kernel(WtArgs a) {
+  using R = WtRows<D, T>;
+  using S = WtShape<D, T>;
+  constexpr int NPT = S::NPT, BP = S::BP, G = S::kGroup;
+  constexpr int PIECES = R::kBytes / 16, NL = (G * PIECES + 64 * kWtWaves - 1) / (64 * kWtWaves);
+  extern __shared__ __align__(16) char s_rows[];
+  __shared__ int s_lo[kWtWaves], s_hi[kWtWaves];
+  const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15, tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // the kv head varies fastest: there are eight XCDs, and each keeps its heads' row tiles
+  uint32_t id = blockIdx.x;
+  const int h = (int)(id % (uint32_t)a.nkv);
+  id /= (uint32_t)a.nkv;
+  const int blocks = (a.part_len + BP - 1) / BP;
+  const int chunk = (int)(id % (uint32_t)a.chunks);
+  const int pb0 = (int)(id / (uint32_t)a.chunks);
+  for (int64_t b = blockIdx.y; b < a.batch; b += gridDim.y) {
+    WtSeq s;
+    if (!wt_seq(a, b, tid == 0 && blockIdx.x == 0, s)) continue;
+    float* acc = a.acc + (b * a.nkv + h) * a.acc_cols;
+    for (int64_t pb = pb0; pb * BP < s.E; pb += blocks) {
+      // positions past the guess have no parts: one block takes all of their rows
+      const bool parts = a.chunks > 1 && pb < blocks;
+      if (pb >= blocks && chunk > 0) break;
+      const int base = (int)(pb * BP) + wave * 16 * NPT;
+      WtCols<D, NPT> k;
+      k.load(a, s, h, base, lane);
+      float sum[NPT];
+#pragma unroll
+      for (int t = 0; t < NPT; ++t) sum[t] = 0.0f;
+      __syncthreads();
+      if (lane == 0) s_lo[wave] = k.some_lo, s_hi[wave] = k.some_hi;
+      __syncthreads();
+      int lo = 0x7fffffff, hi = 0;
+#pragma unroll
+      for (int w = 0; w < kWtWaves; ++w) lo = min(lo, s_lo[w]), hi = max(hi, s_hi[w]);
+      lo = __builtin_amdgcn_readfirstlane(lo);
+      hi = __builtin_amdgcn_readfirstlane(hi);
+      const int t_end = hi > lo ? (hi + 15) >> 4 : 0, t_begin = hi > lo ? lo >> 4 : 0;
+      const int step = parts ? a.chunks * a.chunk : t_end + 1;
+      for (int c0 = parts ? chunk * a.chunk : 0; c0 < t_end; c0 += step) {
+        const int from = max(c0, t_begin), to = parts ? min(c0 + a.chunk, t_end) : t_end;
+        if (from >= to) continue;
+        const char* rows = a.tiles + (wt_slot(a, b, s.o0, from) * a.nkv + h) * R::kBytes;
+        const int64_t apart = (int64_t)a.nkv * R::kBytes;
+        uint4 raw[NL];
+        const auto fetch = [&](int t0) {
+#pragma unroll
+          for (int i = 0; i < NL; ++i) {
+            const int x = i * 64 * kWtWaves + tid, tile = min(x / PIECES, min(G, to - from - t0) - 1);
+            raw[i] = *reinterpret_cast<const uint4*>(rows + (t0 + tile) * apart + (x % PIECES) * 16);
+          }
+        };
+        const auto place = [&](int which) {
+#pragma unroll
+          for (int i = 0; i < NL; ++i) {
+            const int x = i * 64 * kWtWaves + tid;
+            if (x < G * PIECES) *reinterpret_cast<uint4*>(s_rows + which * S::kStep + x * 16) = raw[i];
+          }
+        };
+        const int count = to - from;
+        fetch(0);
+        __syncthreads();  // the chunk before is read
+        place(0);
+        if (G < count) fetch(G);
+        for (int t0 = 0, which = 0; t0 < count; t0 += G, which ^= 1) {
+          __syncthreads();
+          if (t0 + G < count) {
+            place(which ^ 1);
+            if (t0 + 2 * G < count) fetch(t0 + 2 * G);
+          }
+#pragma unroll
+          for (int u = 0; u < G; ++u) {
+            if (t0 + u >= count) break;
+            const int r0 = (from + t0 + u) * 16;
+            if (r0 + 16 <= k.some_lo || r0 >= k.some_hi) continue;
+            const char* at = s_rows + which * S::kStep + u * R::kBytes;
+            uint4 x[R::NF];
+#pragma unroll
+            for (int i = 0; i < R::NF; ++i) x[i] = *reinterpret_cast<const uint4*>(at + i * 1024 + lane * 16);
+            const float* tail = reinterpret_cast<const float*>(at + R::NF * 1024);
+            float r[4], nl[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = tail[4 * g + i], nl[i] = tail[16 + 4 * g + i];
+            const bool one = __builtin_amdgcn_readfirstlane(__float_as_uint(tail[32])) != 0;
+            const bool whole = r0 >= k.all_lo && min(r0 + 16, s.nr) <= k.all_hi;
+            kh_f32x4 y[NPT];
+#pragma unroll
+            for (int t = 0; t < NPT; ++t) y[t] = wt_scores<D, T>(x, k.x[t]);
+#pragma unroll
+            for (int t = 0; t < NPT; ++t) {
+              float w[4];
+              wt_weights(y[t], k.x[t].f, one, r, nl, w);
+              if (!whole) wt_hide(r0, g, k.lo[t], k.hi[t], nl, w);
+              sum[t] += (w[0] + w[1]) + (w[2] + w[3]);
+            }
+          }
+        }
+      }
+      float* part = a.part + ((b * a.nkv + h) * a.chunks + chunk) * a.part_len;
+#pragma unroll
+      for (int t = 0; t < NPT; ++t) {
+        const int j = base + 16 * t + col;
+        const float w = across_groups_sum(sum[t]);
+        if (g != 0 || j >= s.E) continue;
+        if (parts) part[j] = w;
+        else if (w != 0.0f) acc[j] += w;
+      }
+    }
+  }
+}
+
+// Adds the chunks' sums to acc, in their order.
+__global__ __launch_bounds__(256) void paged_weights_join_kernel(WtArgs a) {
+  for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
+    WtSeq s;
+    if (!wt_seq(a, b, false, s)) continue;
+    const int64_t row = b * a.nkv + blockIdx.y;
+    const int j = blockIdx.x * 256 + threadIdx.x;
+    if (j >= min(s.E, a.part_len)) continue;
+    const float* part = a.part + row * a.chunks * a.part_len + j;
+    float w = 0.0f;
+    for (int c = 0; c < a.chunks; ++c) w += part[(int64_t)c * a.part_len];
+    if (w != 0.0f) a.acc[row * a.acc_cols + j] += w;
+  }
+}
+
+// How a call is cut.
+struct WtPlan {
+  bool many;
+  int chunks, chunk, part_len;
+  int64_t slots;  // row tiles of the workspace
+};
+static int wt_positions(int d, int dtype) {  // of a block of many rows
+  if (dtype == KH_DT_F32) return d == 64 ? WtShape<64, float>::BP : d == 128 ? WtShape<128, float>::BP : WtShape<256, float>::BP;
+  return d == 64 ? WtShape<64, uint16_t>::BP : d == 128 ? WtShape<128, uint16_t>::BP : WtShape<256, uint16_t>::BP;
+}
+static int wt_tile_bytes(int d, int dtype) {
+  if (dtype == KH_DT_F32) return d == 64 ? WtRows<64, float>::kBytes : d == 128 ? WtRows<128, float>::kBytes : WtRows<256, float>::kBytes;
+  return d == 64 ? WtRows<64, uint16_t>::kBytes : d == 128 ? WtRows<128, uint16_t>::kBytes : WtRows<256, uint16_t>::kBytes;
+}
+constexpr int64_t kWtFill = 512;              // blocks of many rows that the chip holds at once
+constexpr int64_t kWtPartMost = 1 << 28;      // sums of chunks
+constexpr int64_t kWtMostBlocks = 1 << 20;
+static WtPlan wt_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int64_t batch, int64_t max_rows, int64_t max_len) {
+  WtPlan p;
+  const int64_t gs = nh / c->nkv;
+  max_rows = std::min(max_rows, rows);
+  p.many = max_rows * gs > 16;
+  p.slots = p.many ? rows * gs / 16 + batch + 1 : 0;
+  p.chunks = 1;
+  const int bp = wt_positions(c->d, dtype);
+  const int64_t tiles = std::max<int64_t>((max_rows * gs + 15) / 16, 1);
+  // as many blocks as a grid holds: positions past them are taken by turns
+  const int64_t blocks = std::max<int64_t>(std::min((std::min<int64_t>(max_len, INT32_MAX) + bp - 1) / bp, kWtMostBlocks / c->nkv), 1);
+  p.part_len = (int)(blocks * bp);
+  // chunks of equal work, some four rounds of blocks (half of the pairs are not seen): a
+  // chunk of few row tiles does not pay for loading the positions
+  if (batch * c->nkv <= 8 * kWtFill) {
+    const int64_t base = blocks * c->nkv * batch;
+    const int64_t want = std::min(std::min(8 * kWtFill / base, tiles / 8), kWtPartMost / (batch * c->nkv * p.part_len));
+    if (want > 1) p.chunks = (int)want;
+  }
+  p.chunk = (int)((tiles + p.chunks - 1) / p.chunks);
+  p.chunks = (int)((tiles + p.chunk - 1) / p.chunk);
+  return p;
+}
+struct WtSpace {
+  int64_t part, bytes;
+};
+static WtSpace wt_space(const WtPlan& p, int dtype, int64_t batch, int nkv, int d) {
+  WtSpace s;
+  s.part = p.slots * nkv * wt_tile_bytes(d, dtype);
+  s.bytes = s.part + (p.many && p.chunks > 1 ? batch * nkv * p.chunks * (int64_t)p.part_len * 4 : 0);
+  return s;
+}
+
+template <int D, typename T>
+static int wt_launch(const WtArgs& a, const WtPlan& p, int64_t max_rows, int64_t max_len, hipStream_t st) {
+  using S = WtShape<D, T>;
+  const unsigned seqs = (unsigned)std::min<int64_t>(a.batch, 65535);
+  if (!p.many) {
+    constexpr int NPT = 2, BP = 16 * NPT * kWtWaves;
+    const int64_t most = std::min(std::min(max_len, a.acc_cols), a.cols << a.ps_log2);
+    const dim3 g((unsigned)std::max<int64_t>(std::min<int64_t>((most + BP - 1) / BP, 65535), 1), (unsigned)a.nkv, seqs);
+    hipLaunchKernelGGL((paged_weights_kernel<D, T, NPT>), g, dim3(64 * kWtWaves), 0, st, a);
+  } else {
+    const int64_t tiles = (std::min(max_rows, a.rows) * a.gs + 63) / 64;
+    hipLaunchKernelGGL((paged_weights_rows_kernel<D, T>), dim3((unsigned)std::min<int64_t>(tiles, 65535), (unsigned)a.nkv, seqs),
+                       dim3(256), 0, st, a);
+    const int64_t blocks = (int64_t)a.part_len / S::BP * a.chunks * a.nkv;
+    hipLaunchKernelGGL((paged_weights_tiles_kernel<D, T>), dim3((unsigned)blocks, seqs), dim3(64 * kWtWaves), S::kLds, st, a);
+    if (a.chunks > 1)
+      hipLaunchKernelGGL(paged_weights_join_kernel, dim3((unsigned)(a.part_len + 255) / 256, (unsigned)a.nkv, seqs), dim3(256), 0,
+                         st, a);
+  }
   KH_LAUNCHED();
   return KH_OK;
 }
 template <typename T>
-static int wt_launch_d(int d, const WtArgs& a, int64_t max_len, hipStream_t st) {
-  if (d == 64) return wt_launch<64, T>(a, max_len, st);
-  if (d == 128) return wt_launch<128, T>(a, max_len, st);
-  return wt_launch<256, T>(a, max_len, st);
+static int wt_launch_d(int d, const WtArgs& a, const WtPlan& p, int64_t max_rows, int64_t max_len, hipStream_t st) {
+  if (d == 64) return wt_launch<64, T>(a, p, max_rows, max_len, st);
+  if (d == 128) return wt_launch<128, T>(a, p, max_rows, max_len, st);
+  return wt_launch<256, T>(a, p, max_rows, max_len, st);
 }
+
+template <int D>
+static int wt_allow_lds() {
+  KH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_weights_tiles_kernel<D, float>),
+                             hipFuncAttributeMaxDynamicSharedMemorySize, WtShape<D, float>::kLds));
+  KH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_weights_tiles_kernel<D, uint16_t>),
+                             hipFuncAttributeMaxDynamicSharedMemorySize, WtShape<D, uint16_t>::kLds));
+  return KH_OK;
+}
+int paged_weights_prepare(int d) { return d == 64 ? wt_allow_lds<64>() : d == 128 ? wt_allow_lds<128>() : wt_allow_lds<256>(); }
 
 static int wt_shape(const kh_paged_kv* c, int dtype, int64_t rows, int64_t batch, int num_heads, int64_t max_rows,
                     int64_t max_len) {
@@ -252,6 +631,8 @@ extern "C" int kh_paged_kv_weights_workspace(const kh_paged_kv* c, int dtype, in
   const int rc = wt_shape(c, dtype, rows, batch, num_heads, max_rows, max_len);
   if (rc != KH_OK) return rc;
   *bytes = 0;
+  if (rows && batch)
+    *bytes = wt_space(wt_plan(c, dtype, num_heads, rows, batch, max_rows, max_len), dtype, batch, c->nkv, c->d).bytes;
   return KH_OK;
 }
 
@@ -273,6 +654,13 @@ extern "C" int kh_paged_kv_weights(const kh_paged_kv* c, int dtype, const void* 
   KH_CHECK_ARG(acc_cols >= 1, "weights of %lld columns", (long long)acc_cols);
   if (rows == 0 || batch == 0) return KH_OK;
   KH_CHECK_ARG(q_dev && off_dev && len_dev && table_dev && lse_dev && acc_dev, "null argument");
+  const WtPlan p = wt_plan(c, dtype, num_heads, rows, batch, max_rows, max_len);
+  const WtSpace sp = wt_space(p, dtype, batch, c->nkv, c->d);
+  if (sp.bytes > 0 && (!ws_dev || ws_bytes < sp.bytes)) {
+    set_error("the workspace holds %lld bytes, %lld are needed", (long long)(ws_dev ? ws_bytes : 0), (long long)sp.bytes);
+    return KH_ERR_CAPACITY;
+  }
+  KH_CHECK_ARG((reinterpret_cast<uintptr_t>(ws_dev) & 15) == 0, "the workspace must be 16-byte aligned");
   KH_ON_DEVICE(c->device, "the cache");
   WtArgs a;
   a.pool = c->pool;
@@ -300,6 +688,11 @@ extern "C" int kh_paged_kv_weights(const kh_paged_kv* c, int dtype, const void* 
   a.acc = acc_dev;
   a.acc_cols = acc_cols;
   a.qvec = aligned16(q_dev, dtype, q_row_stride, q_head_stride) ? 1 : 0;
-  return dtype == KH_DT_F32 ? wt_launch_d<float>(c->d, a, max_len, as_stream(stream))
-                            : wt_launch_d<uint16_t>(c->d, a, max_len, as_stream(stream));
+  a.tiles = static_cast<char*>(ws_dev);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(ws_dev) + sp.part);
+  a.chunks = p.chunks;
+  a.chunk = p.chunk;
+  a.part_len = p.part_len;
+  return dtype == KH_DT_F32 ? wt_launch_d<float>(c->d, a, p, max_rows, max_len, as_stream(stream))
+                            : wt_launch_d<uint16_t>(c->d, a, p, max_rows, max_len, as_stream(stream));
 }

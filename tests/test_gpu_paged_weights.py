@@ -2,7 +2,8 @@
 
 A weight is exp(x), x = scale q . k - lse.  x is off by the f32 sums of the score (at most dim + 32 additions of
 magnitudes B = scale sum |q| (15 s + |m|)), by the conversion of lse to powers of two (2 * 2^-24 |lse|) and by a last
-fused addition (2^-24 |x|); the exponential by 2^-22 of itself and, through x log2 e, 2^-23 |x|.  Sums of R weights take at most
+fused addition (2^-24 |x|), by d in all: exp(x + d) - exp(x) = exp(x) (exp(d) - 1), so the weight by that (scores of 1e8 and
+more have no f32 digits behind the point: d passes 1, and the tolerance says nothing there); the exponential by 2^-22 of itself and, through x log2 e, 2^-23 |x|.  Sums of R weights take at most
 R / 4 + 64 additions in a row, each off by 2^-24 of the sum, and acc itself is rounded once."""
 import numpy as np
 import pytest
@@ -30,7 +31,8 @@ def reference(q, lse, kraw, scale, causal, window):
             big = scale * (np.abs(q[:, h]) @ (15 * s[:, g] + np.abs(m[:, g])).T)
             err = np.where(on, ((dim + 32) * big + 2 * np.abs(l) + 3 * np.abs(x) + 4) * U, 0.0)
         out[g] += np.where(on, p, 0.0).sum(0)
-        tol[g] += (np.where(on, p, 0.0) * np.nan_to_num(err)).sum(0)
+        err = np.nan_to_num(err)
+        tol[g] += np.where(err > 1, np.inf, np.where(on, p, 0.0) * np.expm1(np.minimum(err, 1.0))).sum(0)
     return out, tol + (n * heads / kv / 4 + 64) * U * out
 
 
@@ -151,6 +153,32 @@ def test_keys_that_are_not_finite(kh, dtype, rows):
     got = bad.run(lse=lse)
     bad.check(got, lse=lse)
     assert got.isnan().sum().item() == 3
+    lse[:, :2] = -np.inf  # rows that add nothing add no NaN either
+    got = bad.run(lse=lse)
+    bad.check(got, lse=lse)
+    assert not got[0, 0].isnan().any() and got[0, 1].isnan().sum().item() == 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [[3], [150]])
+@pytest.mark.parametrize("lo,hi", [(0, 0), (-3, 3), (-30, 30)])
+def test_sizes_of_rows_and_keys(kh, dtype, rows, lo, hi):
+    """Rows and keys of sizes that are powers of two apart, single large elements and zero rows, each position and row to
+    its own tolerance (scales are chosen per position and row)."""
+    rng = np.random.default_rng(hi)
+    k = keys(rng, 400, 2, 128) * 2.0 ** rng.integers(lo, hi + 1, (400, 2, 1))
+    k[7], k[300, 0, 5] = 0, 1000.0
+    c = Call(4, 2, 128, rows, [400], 32, dtype, k=[k.astype(np.float32)])
+    q = c.q.float() * torch.from_numpy(2.0 ** rng.integers(lo, hi + 1, c.q.shape[:2] + (1,))).float() * 2.0 ** -hi
+    q[-1, 1], q[0, 3, 77] = 0, 8 * 2.0 ** -hi
+    c.q = q.to(dtype)
+    lse = np.zeros_like(c.lse)
+    for h in range(4):  # a weight of at most 1 for each row
+        x = np.where(seen(rows[0], 400, True, 0), c.q[:, h].double().numpy() @ values(c.k[0])[:, h // 2].T * c.scale, -np.inf)
+        lse[:, h] = x.max(-1) + 1
+    c.check(c.run(lse=lse), lse=lse)
+    lse[lse > 1e4] = -np.inf  # without the rows whose scores have no digits left
+    c.check(c.run(lse=lse), lse=lse)
 
 
 @pytest.mark.parametrize("rows,lens", [([1, 1], [130, 77]), ([200, 60], [300, 400])])
