@@ -23,6 +23,22 @@ __device__ __forceinline__ void ld_words(const char* p, uint32_t (&w)[N]) {
   }
 }
 
+template <int N>
+__device__ __forceinline__ void ld_n(const char* p, uint32_t* w) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  }
+}
+
 // Eight neighbouring elements as they lie in memory.
 template <typename T>
 struct Raw8 {

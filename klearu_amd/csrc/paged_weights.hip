@@ -45,9 +45,8 @@ struct WtArgs {
   float* acc;
   int64_t acc_cols;
   int qvec;
-  char* tiles;      // row tiles as WtTile lays them out
-  float* part;      // [batch][kv heads][chunks][part_len] sums of chunks of rows
-  int chunks, chunk, part_len;  // chunks of a sequence's rows, their row tiles, and the positions that have them
+  float* sums;      // [batch][kv heads][chunks][parts * part] sums of chunks of rows
+  int chunks, parts, part;  // chunks of a sequence's rows, parts of its positions, positions of a part
 };
 
 typedef _Float16 kh_f16x8 __attribute__((ext_vector_type(8)));
@@ -87,7 +86,6 @@ struct WtRows {
   static constexpr int NG = D / kKvGroup, NQ = sizeof(T) == 4 ? 3 : 1;
   static constexpr int NB = NG == 8 ? 2 : 1;  // operands of the sums over groups: eight numbers each
   static constexpr int NF = NG * NQ + NB;
-  static constexpr int kBytes = NF * 1024 + 256;  // in memory: the operands, scales and log-sum-exps of 16 rows, `one`
   uint4 x[NF];      // the groups' terms, slots (0,4,1,5,2,6,3,7) of eight elements as codes_f16 gives codes; sums
   float r, nl;      // of row lane % 16: its scale, and minus its log-sum-exp in powers of two
   bool one;         // all rows have the first one's scale
@@ -149,49 +147,54 @@ struct WtRows {
   }
 };
 
-// The keys of 16 positions as second operands, a position a column.
+// The keys of 16 positions as second operands, a position a column: groups g0 .. g0 + N - 1 of the
+// codes w, all of the pairs p; f: the position's scale, times c1.
+template <int D, int N>
+__device__ __forceinline__ void wt_unpack(const uint32_t (&w)[N], const uint32_t (&p)[D / kKvGroup], int g0, float c1, int g,
+                                          uint4 (&c)[N], uint4 (&b)[D == 256 ? 2 : 1], float& f) {
+  constexpr int NG = D / kKvGroup, NB = NG == 8 ? 2 : 1;
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NG; ++j)  // a NaN is passed over
+    top = fmaxf(top, fmaxf(8.0f * __uint_as_float(p[j] & 0xffff0000u), __builtin_fabsf(__uint_as_float(p[j] << 16))));
+  const int e = max(exponent_of(top) - 13, -100);
+  const float down = pow2(-e);
+  f = c1 * pow2(e);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const uint32_t pj = N == NG ? p[j] : g0 == 0 ? p[j] : p[j + NG - N];
+    const _Float16 s1 = (_Float16)(__uint_as_float(pj & 0xffff0000u) * down);
+    const kh_f16x2 s2 = {s1, s1}, off = {(_Float16)-24.0f, (_Float16)-24.0f};
+    uint32_t v[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) v[n] = __builtin_bit_cast(uint32_t, (codes_f16(w[j], n) + off) * s2);
+    c[j] = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+  uint32_t mh[NG / 2], sh[NG / 2];  // minima and 8 scales, pairs of groups
+#pragma unroll
+  for (int j = 0; j < NG / 2; ++j) {
+    mh[j] = f16x2(__uint_as_float(p[2 * j] << 16) * down, __uint_as_float(p[2 * j + 1] << 16) * down);
+    sh[j] = f16x2(__uint_as_float(p[2 * j] & 0xffff0000u) * down * 8.0f, __uint_as_float(p[2 * j + 1] & 0xffff0000u) * down * 8.0f);
+  }
+  if constexpr (NG == 2) b[0] = make_uint4(mh[0], sh[0], 0, 0);
+  if constexpr (NG == 4) b[0] = make_uint4(mh[0], mh[1], sh[0], sh[1]);
+  if constexpr (NG == 8) {
+    b[0] = make_uint4(mh[0], mh[1], mh[2], mh[3]);
+    b[1] = make_uint4(sh[0], sh[1], sh[2], sh[3]);
+  }
+  // three terms: the lanes' last group has none
+  if (g == 3) {
+#pragma unroll
+    for (int k = 0; k < NB; ++k) b[k] = make_uint4(0, 0, 0, 0);
+  }
+}
 template <int D>
 struct WtKeys {
   static constexpr int NG = D / kKvGroup, NB = NG == 8 ? 2 : 1;
   uint4 c[NG], b[NB];
-  float f;  // the position's scale, times c1
+  float f;
   __device__ __forceinline__ void put(const uint32_t (&w)[NG], const uint32_t (&p)[NG], float c1, int g) {
-    float top = 0.0f, s[NG], m[NG];
-#pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      s[j] = __uint_as_float(p[j] & 0xffff0000u);
-      m[j] = __uint_as_float(p[j] << 16);
-      top = fmaxf(top, fmaxf(8.0f * s[j], __builtin_fabsf(m[j])));  // a NaN is passed over
-    }
-    const int e = max(exponent_of(top) - 13, -100);
-    const float down = pow2(-e);
-    f = c1 * pow2(e);
-    uint32_t mh[NG], sh[NG];
-#pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      const float sd = s[j] * down;
-      const _Float16 s1 = (_Float16)sd;
-      const kh_f16x2 s2 = {s1, s1}, eight = {(_Float16)-24.0f, (_Float16)-24.0f};
-      uint32_t v[4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) v[n] = __builtin_bit_cast(uint32_t, (codes_f16(w[j], n) + eight) * s2);
-      c[j] = make_uint4(v[0], v[1], v[2], v[3]);
-      mh[j] = f16x2(m[j] * down, 0.0f);
-      sh[j] = f16x2(8.0f * sd, 0.0f);
-    }
-    if constexpr (NG == 2) {
-      b[0] = make_uint4(mh[0] | mh[1] << 16, sh[0] | sh[1] << 16, 0, 0);
-    } else if constexpr (NG == 4) {
-      b[0] = make_uint4(mh[0] | mh[1] << 16, mh[2] | mh[3] << 16, sh[0] | sh[1] << 16, sh[2] | sh[3] << 16);
-    } else {
-      b[0] = make_uint4(mh[0] | mh[1] << 16, mh[2] | mh[3] << 16, mh[4] | mh[5] << 16, mh[6] | mh[7] << 16);
-      b[1] = make_uint4(sh[0] | sh[1] << 16, sh[2] | sh[3] << 16, sh[4] | sh[5] << 16, sh[6] | sh[7] << 16);
-    }
-    // the terms' slots: group 3 of the lanes has none (a NaN scale is a NaN in the codes' products)
-    if (g == 3) {
-#pragma unroll
-      for (int k = 0; k < NB; ++k) b[k] = make_uint4(0, 0, 0, 0);
-    }
+    wt_unpack<D, NG>(w, p, 0, c1, g, c, b, f);
   }
 };
 
@@ -208,16 +211,12 @@ __device__ __forceinline__ kh_f32x4 wt_scores(const uint4 (&x)[WtRows<D, T>::NF]
     for (int i = R::NQ - 1; i >= 0; --i) y = mfma16h(x[j * R::NQ + i], k.c[j], y);
   return y;
 }
+// The two scales together: products of powers of two, so that it does not matter which rows share one.
+__device__ __forceinline__ float wt_scale(float f, float r) { return fminf(f * r, 0x1.fffffep127f); }
 // The weights of four rows for the lane's position.
-__device__ __forceinline__ void wt_weights(const kh_f32x4& y, float f, bool one, const float (&r)[4], const float (&nl)[4], float (&w)[4]) {
-  if (one) {
-    const float fr = f * r[0];
+__device__ __forceinline__ void wt_weights(const kh_f32x4& y, float f, const float (&r)[4], const float (&nl)[4], float (&w)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(y[i], fr, nl[i]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(y[i] * f, r[i], nl[i]));
-  }
+  for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(y[i], wt_scale(f, r[i]), nl[i]));
 }
 
 // A sequence of the call.
@@ -342,7 +341,7 @@ __global__ __launch_bounds__(64 * kWtWaves) void paged_weights_kernel(WtArgs a) 
 #pragma unroll
         for (int t = 0; t < NPT; ++t) {
           float w[4];
-          wt_weights(wt_scores<D, T>(q.x, k.x[t]), k.x[t].f, q.one, r, nl, w);
+          wt_weights(wt_scores<D, T>(q.x, k.x[t]), k.x[t].f, r, nl, w);
           if (!whole) wt_hide(r0, g, k.lo[t], k.hi[t], nl, w);
           const float sum = across_groups_sum((w[0] + w[1]) + (w[2] + w[3]));
           const int j = base + 16 * t + col;
@@ -354,166 +353,242 @@ __global__ __launch_bounds__(64 * kWtWaves) void paged_weights_kernel(WtArgs a) 
 }
 
 // ---------------------------------------------------------------- many rows
-// Row tiles go to the workspace as operands once, and the blocks of positions read them from there: a
-// wave keeps the keys of its positions, and all waves of a block run the same row tiles over them through
-// LDS, kWtGroup at a time.  The place of a sequence's tiles: every sequence may begin one that is not full.
-__device__ __forceinline__ int64_t wt_slot(const WtArgs& a, int64_t b, int64_t o0, int tile) {
-  return o0 * a.gs / 16 + b + tile;
-}
-
-template <int D, typename T>
-__global__ __launch_bounds__(256) void paged_weights_rows_kernel(WtArgs a) {
-  using R = WtRows<D, T>;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y;
-  for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
-    WtSeq s;
-    if (!wt_seq(a, b, false, s)) continue;
-    for (int tile = blockIdx.x * 4 + wave; tile * 16 < s.nr; tile += gridDim.x * 4) {
-      R q;
-      q.load(a, s.o0, s.nr, h, tile, lane);
-      char* to = a.tiles + (wt_slot(a, b, s.o0, tile) * a.nkv + h) * R::kBytes;
-#pragma unroll
-      for (int i = 0; i < R::NF; ++i) *reinterpret_cast<uint4*>(to + i * 1024 + lane * 16) = q.x[i];
-      float* x = reinterpret_cast<float*>(to + R::NF * 1024);
-      if (lane < 16) x[lane] = q.r;
-      else if (lane < 32) x[lane] = q.nl;
-      else if (lane == 32) x[lane] = q.one ? 1.0f : 0.0f;
-    }
-  }
-}
-
+// A wave keeps RT tiles of rows, and the waves of a block run the same positions: a step's 64
+// are unpacked once for all of them, to LDS as operands, while the step before is worked on.  The
+// waves' sums of a step meet in LDS, and 64 threads add them up in the order of the waves.
+//
+// A block takes every chunks-th block of rows and one part of the positions, and has sums of its own in
+// the workspace; a second kernel adds those to acc in the order of the chunks.
 template <int D, typename T>
 struct WtShape {
-  static constexpr int NPT = D == 256 || sizeof(T) == 4 ? 2 : 4;
-  static constexpr int kGroup = D == 256 || sizeof(T) == 4 ? 2 : 4;  // row tiles between two barriers
-  static constexpr int kStep = kGroup * WtRows<D, T>::kBytes, kLds = 2 * kStep;
-  static constexpr int BP = 16 * NPT * kWtWaves;
+  using R = WtRows<D, T>;
+  static constexpr int NW = 8, KEYS = 64, TK = KEYS / 16;
+  static constexpr int RT = R::NF <= 7 ? 4 : R::NF <= 13 ? 2 : 1;
+  static constexpr int RB = 16 * RT * NW;                 // rows of a block
+  static constexpr int NK = R::NG + R::NB;                // operands of a tile of positions
+  static constexpr int kStep = TK * NK * 1024;            // bytes of a step
+  static constexpr int kLds = 2 * kStep + 2 * KEYS * 4 + 2 * NW * KEYS * 4;  // and the scales, and the waves' sums
 };
 
 template <int D, typename T>
-__global__ __launch_bounds__(64 * kWtWaves, 2) void paged_weights_tiles_kernel(WtArgs a) {
+__global__ __launch_bounds__((64 * WtShape<D, T>::NW), 2) void paged_weights_tiles_kernel(WtArgs a) {
   using R = WtRows<D, T>;
   using S = WtShape<D, T>;
-  constexpr int NPT = S::NPT, BP = S::BP, G = S::kGroup;
-  constexpr int PIECES = R::kBytes / 16, NL = (G * PIECES + 64 * kWtWaves - 1) / (64 * kWtWaves);
-  extern __shared__ __align__(16) char s_rows[];
-  __shared__ int s_lo[kWtWaves], s_hi[kWtWaves];
+  using P = KvParts<D>;
+  constexpr int NG = R::NG, NB = R::NB, NW = S::NW, KEYS = S::KEYS, TK = S::TK, RT = S::RT, RB = S::RB, NK = S::NK;
+  constexpr int HALF = NG / 2;  // groups of a position that a wave unpacks
+  extern __shared__ __align__(16) char s_buf[];
+  float* s_f = reinterpret_cast<float*>(s_buf + 2 * S::kStep);  // [2][KEYS]
+  float* s_sum = s_f + 2 * KEYS;                                // [2][NW][KEYS]
+  __shared__ int s_lo[NW], s_hi[NW];
+  __shared__ int s_state[2][TK];  // of a step's tiles: 0, 1 where a key holds a NaN, 2 where there is no page
   const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15, tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // the kv head varies fastest: there are eight XCDs, and each keeps its heads' row tiles
+  const int ps = 1 << a.ps_log2, utile = wave >> 1, uhalf = wave & 1;
+  // the kv head varies fastest: there are eight XCDs, and each keeps its heads' pages
   uint32_t id = blockIdx.x;
   const int h = (int)(id % (uint32_t)a.nkv);
   id /= (uint32_t)a.nkv;
-  const int blocks = (a.part_len + BP - 1) / BP;
-  const int chunk = (int)(id % (uint32_t)a.chunks);
-  const int pb0 = (int)(id / (uint32_t)a.chunks);
+  const int part = (int)(id % (uint32_t)a.parts), chunk = a.chunks - 1 - (int)(id / (uint32_t)a.parts);
   for (int64_t b = blockIdx.y; b < a.batch; b += gridDim.y) {
     WtSeq s;
     if (!wt_seq(a, b, tid == 0 && blockIdx.x == 0, s)) continue;
     float* acc = a.acc + (b * a.nkv + h) * a.acc_cols;
-    for (int64_t pb = pb0; pb * BP < s.E; pb += blocks) {
-      // positions past the guess have no parts: one block takes all of their rows
-      const bool parts = a.chunks > 1 && pb < blocks;
-      if (pb >= blocks && chunk > 0) break;
-      const int base = (int)(pb * BP) + wave * 16 * NPT;
-      WtCols<D, NPT> k;
-      k.load(a, s, h, base, lane);
-      float sum[NPT];
+    for (int64_t p0 = (int64_t)part * a.part; p0 < s.E; p0 += (int64_t)a.parts * a.part) {
+      // positions past the guess have no sums of their own: one block takes all of their rows
+      const bool own = a.chunks > 1 && p0 < (int64_t)a.parts * a.part;
+      if (a.chunks > 1 && !own && chunk > 0) break;
+      const int p1 = (int)min(p0 + a.part, (int64_t)s.E);
+      // sums go to out[j], by the same thread each time
+      float* out = own ? a.sums + ((b * a.nkv + h) * a.chunks + chunk) * ((int64_t)a.parts * a.part) : acc;
+      if (own && tid < KEYS)
+        for (int j = (int)p0 + tid; j < p1; j += KEYS) out[j] = 0.0f;
+      for (int rb = own ? chunk : 0; (int64_t)rb * RB < s.nr; rb += own ? a.chunks : 1) {
+        const int w0 = (rb * NW + wave) * RT * 16;  // the wave's first row
+        // positions that some of the wave's rows see, and those that all of them see
+        uint32_t lo = 0x7fffffffu, hi = 0, all_lo = 0, all_hi = 0x7fffffffu;
+        if (w0 < s.nr) {
+          const int64_t i0 = w0 / a.gs, i1 = (min(w0 + RT * 16, s.nr) - 1) / a.gs;
+          const int64_t L = s.before + s.n, q0 = s.before + i0, q1 = s.before + i1;
+          const int64_t x = a.window > 0 ? max(q0 - a.window + 1, (int64_t)0) : 0, xa = a.window > 0 ? max(q1 - a.window + 1, (int64_t)0) : 0;
+          const int64_t y = a.causal ? min(q1 + 1, L) : L, ya = a.causal ? min(q0 + 1, L) : L;
+          if (y > x) lo = (uint32_t)x, hi = (uint32_t)y;
+          all_lo = (uint32_t)xa;
+          all_hi = (uint32_t)max(ya, (int64_t)0);
+        }
+        __syncthreads();  // the last block of rows is done with LDS
+        if (lane == 0) s_lo[wave] = (int)lo, s_hi[wave] = (int)hi;
+        __syncthreads();
+        int tlo = 0x7fffffff, thi = 0;
 #pragma unroll
-      for (int t = 0; t < NPT; ++t) sum[t] = 0.0f;
-      __syncthreads();
-      if (lane == 0) s_lo[wave] = k.some_lo, s_hi[wave] = k.some_hi;
-      __syncthreads();
-      int lo = 0x7fffffff, hi = 0;
-#pragma unroll
-      for (int w = 0; w < kWtWaves; ++w) lo = min(lo, s_lo[w]), hi = max(hi, s_hi[w]);
-      lo = __builtin_amdgcn_readfirstlane(lo);
-      hi = __builtin_amdgcn_readfirstlane(hi);
-      const int t_end = hi > lo ? (hi + 15) >> 4 : 0, t_begin = hi > lo ? lo >> 4 : 0;
-      const int step = parts ? a.chunks * a.chunk : t_end + 1;
-      for (int c0 = parts ? chunk * a.chunk : 0; c0 < t_end; c0 += step) {
-        const int from = max(c0, t_begin), to = parts ? min(c0 + a.chunk, t_end) : t_end;
-        if (from >= to) continue;
-        const char* rows = a.tiles + (wt_slot(a, b, s.o0, from) * a.nkv + h) * R::kBytes;
-        const int64_t apart = (int64_t)a.nkv * R::kBytes;
-        uint4 raw[NL];
-        const auto fetch = [&](int t0) {
-#pragma unroll
-          for (int i = 0; i < NL; ++i) {
-            const int x = i * 64 * kWtWaves + tid, tile = min(x / PIECES, min(G, to - from - t0) - 1);
-            raw[i] = *reinterpret_cast<const uint4*>(rows + (t0 + tile) * apart + (x % PIECES) * 16);
+        for (int w = 0; w < NW; ++w) tlo = min(tlo, s_lo[w]), thi = max(thi, s_hi[w]);
+        tlo = __builtin_amdgcn_readfirstlane(max(tlo, (int)p0));
+        thi = __builtin_amdgcn_readfirstlane(min(thi, p1));
+        if (thi <= tlo) continue;
+        const int sb = tlo / KEYS, se = (thi + KEYS - 1) / KEYS;
+
+        // lane i holds the page of the wave's tile of the i-th of 64 steps
+        int pages = 0;
+        const auto find = [&](int st) {
+          const int tok = (st + lane) * KEYS + utile * 16;
+          pages = tok + 16 > tlo && tok < thi ? s.table[max(tok, tlo) >> a.ps_log2] : 0;
+          if (tok + 16 > tlo && tok < thi && (pages < 0 || pages >= a.pages)) {
+            atomicOr(a.err, 2);
+            pages = -1;
           }
         };
-        const auto place = [&](int which) {
+        uint32_t kw[HALF], kp[NG];
+        int pg = 0;
+        const auto load = [&](int st) {
+          pg = __builtin_amdgcn_readlane(pages, (st - sb) & 63);
+          const int tok = st * KEYS + utile * 16;
+          const char* blk = a.pool + ((int64_t)max(pg, 0) * a.nkv + h) * a.block;
+          const int at = (tok & (ps - 1)) + col;
+          ld_n<HALF>(blk + P::kc() + at * (D / 2) + (g * NG + uhalf * HALF) * 4, kw);
+          ld_words<NG>(blk + P::kp(ps) + at * NG * 4, kp);
+        };
+        const auto unpack = [&](int st) {
+          char* to = s_buf + (st & 1) * S::kStep + utile * NK * 1024 + lane * 16;
+          float f;
+          uint4 c[HALF], bb[NB];
+          wt_unpack<D, HALF>(kw, kp, uhalf * HALF, a.c1, g, c, bb, f);
 #pragma unroll
-          for (int i = 0; i < NL; ++i) {
-            const int x = i * 64 * kWtWaves + tid;
-            if (x < G * PIECES) *reinterpret_cast<uint4*>(s_rows + which * S::kStep + x * 16) = raw[i];
+          for (int k = 0; k < HALF; ++k) *reinterpret_cast<uint4*>(to + (uhalf * HALF + k) * 1024) = c[k];
+          if (uhalf == 0) {
+#pragma unroll
+            for (int k = 0; k < NB; ++k) *reinterpret_cast<uint4*>(to + (NG + k) * 1024) = bb[k];
+            if (g == 0) s_f[(st & 1) * KEYS + utile * 16 + col] = f;
+            uint32_t nan = 0;
+#pragma unroll
+            for (int k = 0; k < NG; ++k) nan = max(nan, kp[k]);
+            const int state = pg < 0 ? 2 : __ballot(nan >= 0x7f800000u) ? 1 : 0;
+            if (lane == 0) s_state[st & 1][utile] = state;
           }
         };
-        const int count = to - from;
-        fetch(0);
-        __syncthreads();  // the chunk before is read
-        place(0);
-        if (G < count) fetch(G);
-        for (int t0 = 0, which = 0; t0 < count; t0 += G, which ^= 1) {
+        find(sb);
+        load(sb);
+
+        R q[RT];
+        bool one = true;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          q[t].load(a, s.o0, s.nr, h, w0 / 16 + t, lane);
+          one = one && q[t].one;
+        }
+        float nl[RT][4], r[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          r[t] = __shfl(q[t].r, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) nl[t][i] = __shfl(q[t].nl, 4 * g + i);
+        }
+        unpack(sb);
+        if (sb + 1 < se) load(sb + 1);
+
+        for (int st = sb; st < se; ++st) {
           __syncthreads();
-          if (t0 + G < count) {
-            place(which ^ 1);
-            if (t0 + 2 * G < count) fetch(t0 + 2 * G);
+          if (st > sb && tid < KEYS) {
+            const float* x = s_sum + ((st - 1) & 1) * NW * KEYS + tid;
+            float w = 0.0f;
+#pragma unroll
+            for (int k = 0; k < NW; ++k) w += x[k * KEYS];
+            const int j = (st - 1) * KEYS + tid;
+            if (j >= p0 && j < p1 && w != 0.0f) out[j] += w;
           }
+          const int first = st * KEYS;
+          const char* buf = s_buf + (st & 1) * S::kStep + lane * 16;
+          const float* fs = s_f + (st & 1) * KEYS;
+          float* sums = s_sum + ((st & 1) * NW + wave) * KEYS;
+          int state = 0;
 #pragma unroll
-          for (int u = 0; u < G; ++u) {
-            if (t0 + u >= count) break;
-            const int r0 = (from + t0 + u) * 16;
-            if (r0 + 16 <= k.some_lo || r0 >= k.some_hi) continue;
-            const char* at = s_rows + which * S::kStep + u * R::kBytes;
-            uint4 x[R::NF];
+          for (int k = 0; k < TK; ++k) state |= s_state[st & 1][k];
+          state = __builtin_amdgcn_readfirstlane(state);
+          if (st + 1 < se) {
+            unpack(st + 1);
+            if (st + 2 < se) {
+              if (((st + 2 - sb) & 63) == 0) find(st + 2);
+              load(st + 2);
+            }
+          }
+          const auto scores = [&](int k, int t) {
+            kh_f32x4 y = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < R::NF; ++i) x[i] = *reinterpret_cast<const uint4*>(at + i * 1024 + lane * 16);
-            const float* tail = reinterpret_cast<const float*>(at + R::NF * 1024);
-            float r[4], nl[4];
+            for (int i = 0; i < NB; ++i) y = mfma16h(q[t].x[NG * R::NQ + i], *reinterpret_cast<const uint4*>(buf + (k * NK + NG + i) * 1024), y);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = tail[4 * g + i], nl[i] = tail[16 + 4 * g + i];
-            const bool one = __builtin_amdgcn_readfirstlane(__float_as_uint(tail[32])) != 0;
-            const bool whole = r0 >= k.all_lo && min(r0 + 16, s.nr) <= k.all_hi;
-            kh_f32x4 y[NPT];
+            for (int j = 0; j < NG; ++j) {
+              const uint4 c = *reinterpret_cast<const uint4*>(buf + (k * NK + j) * 1024);
 #pragma unroll
-            for (int t = 0; t < NPT; ++t) y[t] = wt_scores<D, T>(x, k.x[t]);
+              for (int i = R::NQ - 1; i >= 0; --i) y = mfma16h(q[t].x[j * R::NQ + i], c, y);
+            }
+            return y;
+          };
+          if (first >= (int)hi || first + KEYS <= (int)lo) {  // the wave's rows see nothing of it
+            sums[lane] = 0.0f;
+          } else if (one && state == 0 && first >= (int)all_lo && first + KEYS <= (int)all_hi) {
+            // every row sees every position
 #pragma unroll
-            for (int t = 0; t < NPT; ++t) {
-              float w[4];
-              wt_weights(y[t], k.x[t].f, one, r, nl, w);
-              if (!whole) wt_hide(r0, g, k.lo[t], k.hi[t], nl, w);
-              sum[t] += (w[0] + w[1]) + (w[2] + w[3]);
+            for (int k = 0; k < TK; ++k) {
+              const float f = fs[k * 16 + col];
+              float sum = 0.0f;
+#pragma unroll
+              for (int t = 0; t < RT; ++t) {
+                const kh_f32x4 y = scores(k, t);
+                const float fr = wt_scale(f, r[t]);
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(y[i], fr, nl[t][i]));
+                sum += (w[0] + w[1]) + (w[2] + w[3]);
+              }
+              sum = across_groups_sum(sum);
+              if (g == 0) sums[k * 16 + col] = sum;
+            }
+          } else {
+            for (int k = 0; k < TK; ++k) {
+              const float f = fs[k * 16 + col];
+              int from, to;
+              wt_span(a, s, first + k * 16 + col, from, to);
+              float sum = 0.0f;
+#pragma unroll
+              for (int t = 0; t < RT; ++t) {
+                const kh_f32x4 y = scores(k, t);
+                float w[4], rt[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) rt[i] = __shfl(q[t].r, 4 * g + i);
+                wt_weights(y, f, rt, nl[t], w);
+                wt_hide(w0 + 16 * t, g, from, to, nl[t], w);
+                sum += (w[0] + w[1]) + (w[2] + w[3]);
+              }
+              sum = across_groups_sum(sum);
+              if (g == 0) sums[k * 16 + col] = s_state[st & 1][k] == 2 ? 0.0f : sum;
             }
           }
         }
-      }
-      float* part = a.part + ((b * a.nkv + h) * a.chunks + chunk) * a.part_len;
+        __syncthreads();
+        if (tid < KEYS) {
+          const float* x = s_sum + ((se - 1) & 1) * NW * KEYS + tid;
+          float w = 0.0f;
 #pragma unroll
-      for (int t = 0; t < NPT; ++t) {
-        const int j = base + 16 * t + col;
-        const float w = across_groups_sum(sum[t]);
-        if (g != 0 || j >= s.E) continue;
-        if (parts) part[j] = w;
-        else if (w != 0.0f) acc[j] += w;
+          for (int k = 0; k < NW; ++k) w += x[k * KEYS];
+          const int j = (se - 1) * KEYS + tid;
+          if (j >= p0 && j < p1 && w != 0.0f) out[j] += w;
+        }
       }
     }
   }
 }
 
 // Adds the chunks' sums to acc, in their order.
-__global__ __launch_bounds__(256) void paged_weights_join_kernel(WtArgs a) {
+__global__ __launch_bounds__(64) void paged_weights_join_kernel(WtArgs a) {
+  const int64_t apart = (int64_t)a.parts * a.part;
   for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
     WtSeq s;
     if (!wt_seq(a, b, false, s)) continue;
-    const int64_t row = b * a.nkv + blockIdx.y;
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    if (j >= min(s.E, a.part_len)) continue;
-    const float* part = a.part + row * a.chunks * a.part_len + j;
+    const int64_t row = b * a.nkv + blockIdx.y, j = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    if (j >= min((int64_t)s.E, apart)) continue;
+    const float* sums = a.sums + row * a.chunks * apart + j;
     float w = 0.0f;
-    for (int c = 0; c < a.chunks; ++c) w += part[(int64_t)c * a.part_len];
+#pragma unroll 8
+    for (int c = 0; c < a.chunks; ++c) w += sums[c * apart];
     if (w != 0.0f) a.acc[row * a.acc_cols + j] += w;
   }
 }
@@ -521,80 +596,62 @@ __global__ __launch_bounds__(256) void paged_weights_join_kernel(WtArgs a) {
 // How a call is cut.
 struct WtPlan {
   bool many;
-  int chunks, chunk, part_len;
-  int64_t slots;  // row tiles of the workspace
+  int chunks, parts, part;
 };
-static int wt_positions(int d, int dtype) {  // of a block of many rows
-  if (dtype == KH_DT_F32) return d == 64 ? WtShape<64, float>::BP : d == 128 ? WtShape<128, float>::BP : WtShape<256, float>::BP;
-  return d == 64 ? WtShape<64, uint16_t>::BP : d == 128 ? WtShape<128, uint16_t>::BP : WtShape<256, uint16_t>::BP;
+static int wt_block_rows(int d, int dtype) {
+  if (dtype == KH_DT_F32) return d == 64 ? WtShape<64, float>::RB : d == 128 ? WtShape<128, float>::RB : WtShape<256, float>::RB;
+  return d == 64 ? WtShape<64, uint16_t>::RB : d == 128 ? WtShape<128, uint16_t>::RB : WtShape<256, uint16_t>::RB;
 }
-static int wt_tile_bytes(int d, int dtype) {
-  if (dtype == KH_DT_F32) return d == 64 ? WtRows<64, float>::kBytes : d == 128 ? WtRows<128, float>::kBytes : WtRows<256, float>::kBytes;
-  return d == 64 ? WtRows<64, uint16_t>::kBytes : d == 128 ? WtRows<128, uint16_t>::kBytes : WtRows<256, uint16_t>::kBytes;
-}
-constexpr int64_t kWtFill = 512;              // blocks of many rows that the chip holds at once
-constexpr int64_t kWtPartMost = 1 << 28;      // sums of chunks
-constexpr int64_t kWtMostBlocks = 1 << 20;
+constexpr int64_t kWtFill = 256;          // blocks of many rows that the chip holds at once
+constexpr int64_t kWtMost = 1 << 26;      // sums of chunks
+constexpr int kWtMostChunks = 64, kWtPart = 512;
 static WtPlan wt_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int64_t batch, int64_t max_rows, int64_t max_len) {
   WtPlan p;
-  const int64_t gs = nh / c->nkv;
+  const int64_t gs = nh / c->nkv, rb = wt_block_rows(c->d, dtype);
   max_rows = std::min(max_rows, rows);
+  max_len = std::max<int64_t>(std::min<int64_t>(max_len, INT32_MAX), 1);
   p.many = max_rows * gs > 16;
-  p.slots = p.many ? rows * gs / 16 + batch + 1 : 0;
-  p.chunks = 1;
-  const int bp = wt_positions(c->d, dtype);
-  const int64_t tiles = std::max<int64_t>((max_rows * gs + 15) / 16, 1);
-  // as many blocks as a grid holds: positions past them are taken by turns
-  const int64_t blocks = std::max<int64_t>(std::min((std::min<int64_t>(max_len, INT32_MAX) + bp - 1) / bp, kWtMostBlocks / c->nkv), 1);
-  p.part_len = (int)(blocks * bp);
-  // chunks of equal work, some four rounds of blocks (half of the pairs are not seen): a
-  // chunk of few row tiles does not pay for loading the positions
-  if (batch * c->nkv <= 8 * kWtFill) {
-    const int64_t base = blocks * c->nkv * batch;
-    const int64_t want = std::min(std::min(8 * kWtFill / base, tiles / 8), kWtPartMost / (batch * c->nkv * p.part_len));
-    if (want > 1) p.chunks = (int)want;
-  }
-  p.chunk = (int)((tiles + p.chunks - 1) / p.chunks);
-  p.chunks = (int)((tiles + p.chunk - 1) / p.chunk);
+  // parts of the positions, and chunks of the rows where those alone do not fill the chip four times over
+  const int64_t heads = batch * c->nkv;
+  p.part = kWtPart;
+  int64_t parts = (max_len + kWtPart - 1) / kWtPart;
+  const int64_t most = std::max<int64_t>(((int64_t)1 << 20) / c->nkv, 1);
+  if (parts > most) parts = most;  // a grid's: the others are taken by turns
+  int64_t chunks = std::min<int64_t>((max_rows * gs + rb - 1) / rb, kWtMostChunks);
+  if (heads > 8 * kWtFill) chunks = 1;
+  else chunks = std::min(std::min(chunks, 8 * kWtFill / (heads * std::min(parts, 8 * kWtFill)) + 1), kWtMost / (heads * parts * kWtPart));
+  p.parts = (int)parts;
+  p.chunks = (int)std::max<int64_t>(chunks, 1);
   return p;
 }
-struct WtSpace {
-  int64_t part, bytes;
-};
-static WtSpace wt_space(const WtPlan& p, int dtype, int64_t batch, int nkv, int d) {
-  WtSpace s;
-  s.part = p.slots * nkv * wt_tile_bytes(d, dtype);
-  s.bytes = s.part + (p.many && p.chunks > 1 ? batch * nkv * p.chunks * (int64_t)p.part_len * 4 : 0);
-  return s;
+static int64_t wt_space(const WtPlan& p, int64_t heads) {
+  return p.many && p.chunks > 1 ? heads * p.chunks * p.parts * (int64_t)p.part * 4 : 0;
 }
 
 template <int D, typename T>
-static int wt_launch(const WtArgs& a, const WtPlan& p, int64_t max_rows, int64_t max_len, hipStream_t st) {
-  using S = WtShape<D, T>;
+static int wt_launch(const WtArgs& a, bool many, int64_t max_len, hipStream_t st) {
   const unsigned seqs = (unsigned)std::min<int64_t>(a.batch, 65535);
-  if (!p.many) {
+  if (!many) {
     constexpr int NPT = 2, BP = 16 * NPT * kWtWaves;
     const int64_t most = std::min(std::min(max_len, a.acc_cols), a.cols << a.ps_log2);
     const dim3 g((unsigned)std::max<int64_t>(std::min<int64_t>((most + BP - 1) / BP, 65535), 1), (unsigned)a.nkv, seqs);
     hipLaunchKernelGGL((paged_weights_kernel<D, T, NPT>), g, dim3(64 * kWtWaves), 0, st, a);
   } else {
-    const int64_t tiles = (std::min(max_rows, a.rows) * a.gs + 63) / 64;
-    hipLaunchKernelGGL((paged_weights_rows_kernel<D, T>), dim3((unsigned)std::min<int64_t>(tiles, 65535), (unsigned)a.nkv, seqs),
-                       dim3(256), 0, st, a);
-    const int64_t blocks = (int64_t)a.part_len / S::BP * a.chunks * a.nkv;
-    hipLaunchKernelGGL((paged_weights_tiles_kernel<D, T>), dim3((unsigned)blocks, seqs), dim3(64 * kWtWaves), S::kLds, st, a);
+    const int64_t blocks = (int64_t)a.parts * a.chunks * a.nkv;
+    hipLaunchKernelGGL((paged_weights_tiles_kernel<D, T>), dim3((unsigned)blocks, seqs), dim3((64 * WtShape<D, T>::NW)),
+                       (WtShape<D, T>::kLds), st, a);
     if (a.chunks > 1)
-      hipLaunchKernelGGL(paged_weights_join_kernel, dim3((unsigned)(a.part_len + 255) / 256, (unsigned)a.nkv, seqs), dim3(256), 0,
-                         st, a);
+      hipLaunchKernelGGL(paged_weights_join_kernel, dim3((unsigned)((int64_t)a.parts * a.part / 64), (unsigned)a.nkv, seqs), dim3(64),
+                         0, st, a);
   }
   KH_LAUNCHED();
   return KH_OK;
 }
 template <typename T>
-static int wt_launch_d(int d, const WtArgs& a, const WtPlan& p, int64_t max_rows, int64_t max_len, hipStream_t st) {
-  if (d == 64) return wt_launch<64, T>(a, p, max_rows, max_len, st);
-  if (d == 128) return wt_launch<128, T>(a, p, max_rows, max_len, st);
-  return wt_launch<256, T>(a, p, max_rows, max_len, st);
+static int wt_launch_d(int d, const WtArgs& a, bool many, int64_t max_len, hipStream_t st) {
+  if (d == 64) return wt_launch<64, T>(a, many, max_len, st);
+  if (d == 128) return wt_launch<128, T>(a, many, max_len, st);
+  return wt_launch<256, T>(a, many, max_len, st);
 }
 
 template <int D>
@@ -631,8 +688,7 @@ extern "C" int kh_paged_kv_weights_workspace(const kh_paged_kv* c, int dtype, in
   const int rc = wt_shape(c, dtype, rows, batch, num_heads, max_rows, max_len);
   if (rc != KH_OK) return rc;
   *bytes = 0;
-  if (rows && batch)
-    *bytes = wt_space(wt_plan(c, dtype, num_heads, rows, batch, max_rows, max_len), dtype, batch, c->nkv, c->d).bytes;
+  if (rows && batch) *bytes = wt_space(wt_plan(c, dtype, num_heads, rows, batch, max_rows, max_len), batch * c->nkv);
   return KH_OK;
 }
 
@@ -655,9 +711,9 @@ extern "C" int kh_paged_kv_weights(const kh_paged_kv* c, int dtype, const void* 
   if (rows == 0 || batch == 0) return KH_OK;
   KH_CHECK_ARG(q_dev && off_dev && len_dev && table_dev && lse_dev && acc_dev, "null argument");
   const WtPlan p = wt_plan(c, dtype, num_heads, rows, batch, max_rows, max_len);
-  const WtSpace sp = wt_space(p, dtype, batch, c->nkv, c->d);
-  if (sp.bytes > 0 && (!ws_dev || ws_bytes < sp.bytes)) {
-    set_error("the workspace holds %lld bytes, %lld are needed", (long long)(ws_dev ? ws_bytes : 0), (long long)sp.bytes);
+  const int64_t need = wt_space(p, batch * c->nkv);
+  if (need > 0 && (!ws_dev || ws_bytes < need)) {
+    set_error("the workspace holds %lld bytes, %lld are needed", (long long)(ws_dev ? ws_bytes : 0), (long long)need);
     return KH_ERR_CAPACITY;
   }
   KH_CHECK_ARG((reinterpret_cast<uintptr_t>(ws_dev) & 15) == 0, "the workspace must be 16-byte aligned");
@@ -688,11 +744,10 @@ extern "C" int kh_paged_kv_weights(const kh_paged_kv* c, int dtype, const void* 
   a.acc = acc_dev;
   a.acc_cols = acc_cols;
   a.qvec = aligned16(q_dev, dtype, q_row_stride, q_head_stride) ? 1 : 0;
-  a.tiles = static_cast<char*>(ws_dev);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(ws_dev) + sp.part);
+  a.sums = static_cast<float*>(ws_dev);
   a.chunks = p.chunks;
-  a.chunk = p.chunk;
-  a.part_len = p.part_len;
-  return dtype == KH_DT_F32 ? wt_launch_d<float>(c->d, a, p, max_rows, max_len, as_stream(stream))
-                            : wt_launch_d<uint16_t>(c->d, a, p, max_rows, max_len, as_stream(stream));
+  a.parts = p.parts;
+  a.part = p.part;
+  return dtype == KH_DT_F32 ? wt_launch_d<float>(c->d, a, p.many, max_len, as_stream(stream))
+                            : wt_launch_d<uint16_t>(c->d, a, p.many, max_len, as_stream(stream));
 }
