@@ -2,36 +2,37 @@
 //
 //   y[i][v] = scores[i] + x[i][v] - log sum_w exp(x[i][w]),   top k of y over (i, v)
 //
-// One pass over the logits: a block takes a chunk of a row, and leaves its maximum M, the sum of
-// exp(x - M) and its k largest logits; a second kernel joins a sequence's chunks.  Within a beam y orders
-// as x does, so chunks compare logits as integers.  Between beams the log-sum-exps decide: they are f64,
-// of f32 exponentials with the rounding of their arguments put back (log2 e in two
-// parts), since sums that are 1e-7 off swap continuations of a batch of beams now and then.
+// One pass over the logits: a wave takes a part of a row and leaves the sum of exp(x - m) and its
+// k largest logits; a second kernel joins a sequence's parts.  Within a beam y orders as x does, so
+// parts compare logits as integers, of equal ones the first.  Between beams the log-sum-exps
+// decide: they are f64, of f32 exponentials with the rounding of their arguments put back (log2 e
+// in two parts), since sums that are 1e-7 off swap continuations of a batch of beams now and then.
 //
-// The k largest of a chunk: the k-th largest T of the threads' own maxima has k logits at
-// or above it, so the k largest are among those, few, which are ranked by counting.
+// The k largest: the k-th largest of the lanes' own maxima, T, has k logits at or above it, so only
+// those can be among the k largest (16 a lane at most), and of later logits only those above T.  They go to a list in LDS, which is
+// cut to k when it fills and at the end: its k-th largest is found bit by bit, counted with ballots.
 #include <algorithm>
 
 #include "paged_kv.hpp"
 
 namespace kh {
 
-constexpr int kBmThreads = 256;
-constexpr int kBmEach = 16;                       // logits of a thread
-constexpr int kBmChunk = kBmThreads * kBmEach;
-constexpr int kBmList = 512;                      // of a chunk, that are ranked by counting
+constexpr int kBmThreads = 256, kBmWaves = kBmThreads / 64;
+constexpr int kBmEach = 16;             // logits of a lane
+constexpr int kBmTile = 64 * kBmEach;   // of a wave
+constexpr int64_t kBmFill = 8192;       // waves that the chip holds at once
 
 struct BeamArgs {
   const void* x;
   int64_t row_stride, batch, vocab;
-  int beams, k, chunks;
+  int beams, k, parts, tiles;  // parts of a row, tiles of a part
   const float* scores;
   const uint8_t* done;
   int64_t end;
   float* out_y;
   int32_t *out_i, *out_v;
-  uint64_t* top;  // [rows][chunks][k] f32_key << 32 | ~token, descending; 0: none
-  double* sum;    // [rows][chunks]
+  uint64_t* top;  // [rows][parts][k] f32_key << 32 | ~token; 0: none
+  double* sum;    // [rows][parts] of exp(x - max)
   float* max;
 };
 
@@ -40,145 +41,189 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
   for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
   return v;
 }
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) {
-    const uint64_t o = __shfl_xor((unsigned long long)v, m);
-    v = o > v ? o : v;
-  }
-  return v;
-}
 
-// exp(t), t <= 0, within 1e-7 and without a bias: log2 e is 0x1.715476p+0f and 1.9e-8 more.
+// exp(t), t <= 88, within 1e-7 and without a bias: log2 e is 0x1.715476p+0f and 1.9e-8 more.  Not for -inf.
 __device__ __forceinline__ float beam_exp(float t) {
   const float hi = 0x1.715476p+0f, lo = 0x1.4ae0cp-26f;
-  const float y = t * hi, r = fmaf(t, hi, -y) + t * lo;
+  const float y = t * hi, r = fmaf(t, lo, fmaf(t, hi, -y));
   const float e = __builtin_amdgcn_exp2f(y);
-  return y < -126.0f ? 0.0f : fmaf(e, r * 0x1.62e43p-1f, e);
+  return fmaf(e, r * 0x1.62e43p-1f, e);
 }
 
-// Elements i0 .. i0 + N - 1 of a row that starts `shift` elements behind a 16-byte
-// border, counted from that border: a vector load where all of them are the row's.
-template <typename T, int N>
-__device__ __forceinline__ void beam_load(const T* row, int shift, int64_t n, int64_t i0, float (&f)[N]) {
-  const int64_t v0 = i0 - shift;
-  if (v0 >= 0 && v0 + N <= n) {
-    const uint4 w = *reinterpret_cast<const uint4*>(row + v0);
-    if constexpr (sizeof(T) == 4) {
-      f[0] = __uint_as_float(w.x); f[1] = __uint_as_float(w.y); f[2] = __uint_as_float(w.z); f[3] = __uint_as_float(w.w);
-    } else {
-      f[0] = bf16_lo(w.x); f[1] = bf16_hi(w.x); f[2] = bf16_lo(w.y); f[3] = bf16_hi(w.y);
-      f[4] = bf16_lo(w.z); f[5] = bf16_hi(w.z); f[6] = bf16_lo(w.w); f[7] = bf16_hi(w.w);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = v0 + i >= 0 && v0 + i < n ? load_f32(row + v0 + i) : -INFINITY;
+// The largest T of which `count(T)` entries are at or above it: the k-th largest of 32-bit entries; all
+// bits below `last` are zero in T (they say nothing of the entries).
+template <typename F>
+__device__ __forceinline__ uint32_t kth_largest(int k, int last, F count) {
+  uint32_t T = 0;
+  for (int bit = 31; bit >= last; --bit) {
+    const uint32_t c = T | 1u << bit;
+    if (count(c) >= k) T = c;
   }
+  return T;
+}
+__device__ __forceinline__ int ballots(bool p) { return __popcll(__ballot(p)); }
+
+// Cuts a wave's list of `n` different entries to its k largest, in any order; returns their number.
+template <int KC>
+__device__ __forceinline__ int beam_cut(uint64_t* list, int n, int k, int last, int lane) {
+  if (n <= k) return n;
+  constexpr int C = KC / 2;  // entries of a lane
+  uint64_t x[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) x[c] = c * 64 + lane < n ? list[c * 64 + lane] : 0;
+  const uint32_t T = kth_largest(k, last, [&](uint32_t v) {
+    int m = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (c * 64 < n) m += ballots((uint32_t)(x[c] >> 32) >= v);
+    return m;
+  });
+  const auto high = [&](uint64_t y) { return (uint32_t)(y >> 32) >> last; };
+  int above = 0, same = 0;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (c * 64 < n) {
+      above += ballots(high(x[c]) > T >> last);
+      same += ballots(x[c] != 0 && high(x[c]) == T >> last);
+    }
+  uint32_t least = 0;  // of those equal to T, the lower word that the last one kept has
+  if (same > k - above)
+    least = kth_largest(k - above, 0, [&](uint32_t v) {
+      int m = 0;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (c * 64 < n) m += ballots(x[c] != 0 && high(x[c]) == T >> last && (uint32_t)x[c] >= v);
+      return m;
+    });
+  int at = 0;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (c * 64 < n) {
+      const bool keep = x[c] != 0 && (high(x[c]) > T >> last || (high(x[c]) == T >> last && (uint32_t)x[c] >= least));
+      const uint64_t b = __ballot(keep);
+      if (keep) list[at + __popcll(b & ((1ull << lane) - 1))] = x[c];
+      at += __popcll(b);
+    }
+  return at;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kBmThreads) void beam_chunk_kernel(BeamArgs a) {
-  constexpr int V = 16 / sizeof(T), W = kBmThreads / 64;
-  __shared__ __align__(16) uint32_t s_max[kBmThreads];
-  __shared__ uint64_t s_list[kBmList], s_best[W];
-  __shared__ float s_m[W];
-  __shared__ double s_sum[W];
-  __shared__ uint32_t s_t;
-  __shared__ int s_n;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  for (int64_t id = blockIdx.x; id < a.batch * a.beams * a.chunks; id += gridDim.x) {
-    const int64_t r = id / a.chunks, c0 = (id - r * a.chunks) * kBmChunk;
+// KC: at least k; a tile adds no more than 16 k entries to the list, which is cut above 16 KC.
+template <typename T, int KC>
+__global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
+  constexpr int V = 16 / sizeof(T), Q = kBmEach / V, LAST = sizeof(T) == 2 ? 16 : 0;
+  extern __shared__ __align__(16) uint64_t s_lists[];  // [waves][32 KC]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint64_t* list = s_lists + wave * (32 * KC);
+  const int64_t waves = a.batch * a.beams * a.parts;
+  for (int64_t id = (int64_t)blockIdx.x * kBmWaves + wave; id < waves; id += (int64_t)gridDim.x * kBmWaves) {
+    const int64_t r = id / a.parts;
+    const int part = (int)(id - r * a.parts);
     const T* row = static_cast<const T*>(a.x) + r * a.row_stride;
+    // positions are counted from the 16-byte border before the row
     const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-    float x[kBmEach];
-    // element e of thread t: (e / V * 256 + t) V + e % V of the chunk
-#pragma unroll
-    for (int q = 0; q < kBmEach / V; ++q) {
-      float f[V];
-      beam_load<T, V>(row, shift, a.vocab, c0 + (q * kBmThreads + t) * V, f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[q * V + i] = f[i];
-    }
-    const auto token = [&](int e) { return (uint32_t)(c0 + ((e / V) * kBmThreads + t) * V + e % V - shift); };
-    const auto there = [&](int e) { return token(e) < (uint32_t)a.vocab; };
-    float m = x[0];
-#pragma unroll
-    for (int e = 1; e < kBmEach; ++e) m = fmaxf(m, x[e]);
-    // a thread of nothing but NaN has no maximum: its NaN go into the sum
-    uint32_t key = 0;
-#pragma unroll
-    for (int e = 0; e < kBmEach; ++e)
-      if (there(e)) key = max(key, f32_key(x[e]));
-    s_max[t] = key;
-    m = wave_max(m);
-    if (lane == 0) s_m[wave] = m;
-    if (t == 0) s_n = 0, s_t = 1;
-    __syncthreads();
-    m = s_m[0];
-#pragma unroll
-    for (int w = 1; w < W; ++w) m = fmaxf(m, s_m[w]);
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < kBmEach; ++e) s += x[e] == -INFINITY ? 0.0f : beam_exp(x[e] - m);
-    const double d = wave_sum_f64((double)s);
-    if (lane == 0) s_sum[wave] = d;
-    // the rank of the thread's maximum
-    int rank = 0;
-    for (int i = 0; i < kBmThreads; i += 4) {
-      const uint4 o = *reinterpret_cast<const uint4*>(&s_max[i]);
-      rank += (o.x > key || (o.x == key && i < t)) + (o.y > key || (o.y == key && i + 1 < t)) +
-              (o.z > key || (o.z == key && i + 2 < t)) + (o.w > key || (o.w == key && i + 3 < t));
-    }
-    if (rank == a.k - 1 && key > 0) s_t = key;
-    __syncthreads();
-    if (t == 0) {
-      a.max[id] = m;
-      a.sum[id] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-    }
-    const uint32_t T0 = s_t;
+    const int end = shift + (int)a.vocab;
+    const int first = part * a.tiles * kBmTile, last = min(first + a.tiles * kBmTile, end);
+    float ref = -INFINITY;  // what exponentials of the lane's logits are taken from
+    double sum = 0.0;
     int n = 0;
+    uint32_t tk = 0, tv = 0;  // T, and its token (inverted): entries below it are of no use
+    uint4 next[Q];
+    const auto inside = [&](int p) { return p >= shift && p + kBmTile <= end; };
+    const auto fetch = [&](int p) {
+      if (inside(p)) {
 #pragma unroll
-    for (int e = 0; e < kBmEach; ++e) n += there(e) && f32_key(x[e]) >= T0 ? 1 : 0;
-    if (n) {
-      int at = atomicAdd(&s_n, n);
-#pragma unroll
-      for (int e = 0; e < kBmEach; ++e)
-        if (there(e) && f32_key(x[e]) >= T0) {
-          if (at < kBmList) s_list[at] = (uint64_t)f32_key(x[e]) << 32 | ~token(e);
-          ++at;
-        }
-    }
-    __syncthreads();
-    n = s_n;
-    uint64_t* top = a.top + id * a.k;
-    if (n <= kBmList) {
-      for (int i = t; i < n; i += kBmThreads) {
-        const uint64_t me = s_list[i];
-        int above = 0;
-        for (int j = 0; j < n; ++j) above += s_list[j] > me ? 1 : 0;
-        if (above < a.k) top[above] = me;
+        for (int q = 0; q < Q; ++q) next[q] = *reinterpret_cast<const uint4*>(row + (p - shift) + (q * 64 + lane) * V);
       }
-      if (t >= n && t < a.k) top[t] = 0;
-    } else {  // many equal logits: the largest, time after time
-      uint64_t last = ~0ull;
-      for (int i = 0; i < a.k; ++i) {
-        uint64_t best = 0;
+    };
+    if (first < last) fetch(first);
+    for (int p = first; p < last; p += kBmTile) {
+      float x[kBmEach];
+      const bool whole = inside(p);
+      if (whole) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const uint4 w = next[q];
+          if constexpr (V == 4) {
+            x[4 * q] = __uint_as_float(w.x); x[4 * q + 1] = __uint_as_float(w.y);
+            x[4 * q + 2] = __uint_as_float(w.z); x[4 * q + 3] = __uint_as_float(w.w);
+          } else {
+            x[8 * q] = bf16_lo(w.x); x[8 * q + 1] = bf16_hi(w.x); x[8 * q + 2] = bf16_lo(w.y); x[8 * q + 3] = bf16_hi(w.y);
+            x[8 * q + 4] = bf16_lo(w.z); x[8 * q + 5] = bf16_hi(w.z); x[8 * q + 6] = bf16_lo(w.w); x[8 * q + 7] = bf16_hi(w.w);
+          }
+        }
+        if (p + kBmTile < last) fetch(p + kBmTile);
+      } else {
 #pragma unroll
         for (int e = 0; e < kBmEach; ++e) {
-          const uint64_t y = (uint64_t)f32_key(x[e]) << 32 | ~token(e);
-          if (there(e) && y < last && y > best) best = y;
+          const int at = p + (e / V * 64 + lane) * V + e % V;
+          x[e] = at >= shift && at < end ? load_f32(row + (at - shift)) : -INFINITY;
         }
-        best = wave_max_u64(best);
-        __syncthreads();
-        if (lane == 0) s_best[wave] = best;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < W; ++w) best = s_best[w] > best ? s_best[w] : best;
-        last = best;
-        if (t == 0) top[i] = best;
+        if (p + kBmTile < last) fetch(p + kBmTile);
       }
+      float m = x[0];
+#pragma unroll
+      for (int e = 1; e < kBmEach; ++e) m = fmaxf(m, x[e]);
+      if (m > ref + 60.0f) {  // sums of 2^24 exp(60) fit in f32
+        sum = sum == 0.0 ? 0.0 : sum * exp((double)ref - (double)m);
+        ref = m;
+      }
+      float s = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kBmEach; ++e) s += beam_exp(x[e] - ref);
+      if (s != s) {  // -inf or the type's lowest value among them, or what makes the sum NaN
+        s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < kBmEach; ++e) s += x[e] == -INFINITY || x[e] - ref < -150.0f ? 0.0f : beam_exp(x[e] - ref);
+      }
+      sum += (double)s;
+
+      // the lane's largest (of the row's own: those past its ends are -inf, too, but no entries)
+      const uint32_t mk = f32_key(m);
+      bool mine = n == 0 || mk > tk;
+      const uint64_t better = __ballot(mine);
+      if (!better) continue;
+      const auto there = [&](int e) {
+        const int at = p + (e / V * 64 + lane) * V + e % V;
+        return whole || (at >= shift && at < end);
+      };
+      const auto token = [&](int e) { return ~(uint32_t)(p + (e / V * 64 + lane) * V + e % V - shift); };
+      if (__popcll(better) >= a.k) {
+        uint32_t bk = 0, bv = 0;
+#pragma unroll
+        for (int e = 0; e < kBmEach; ++e) {
+          const uint32_t key = f32_key(x[e]);
+          if (there(e) && key > bk) bk = key, bv = token(e);
+        }
+        const uint32_t kth = kth_largest(a.k, LAST, [&](uint32_t v) { return ballots(bk >= v); }) >> LAST;
+        if (kth != 0 && (n == 0 || kth > tk >> LAST)) {
+          // of the lanes whose maximum is T the first ones, by their tokens
+          const int above = ballots(bk >> LAST > kth);
+          tv = kth_largest(a.k - above, 0, [&](uint32_t v) { return ballots(bk >> LAST == kth && bv >= v); });
+          tk = __builtin_amdgcn_readlane(bk, __builtin_ctzll(__ballot(bk >> LAST == kth)));
+          mine = true;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kBmEach; ++e) {
+        const uint32_t key = f32_key(x[e]);
+        const bool take = mine && there(e) && (key > tk || (key == tk && token(e) >= tv));
+        const uint64_t b = __ballot(take);
+        if (b) {
+          if (take) list[n + __popcll(b & ((1ull << lane) - 1))] = (uint64_t)key << 32 | token(e);
+          n += __popcll(b);
+        }
+      }
+      if (n > 16 * KC) n = beam_cut<KC>(list, n, a.k, LAST, lane);
     }
-    __syncthreads();
+    n = beam_cut<KC>(list, n, a.k, LAST, lane);
+    uint64_t* top = a.top + id * a.k;
+    if (lane < a.k) top[lane] = lane < n ? list[lane] : 0;
+    const float all = wave_max(ref);
+    const double total = wave_sum_f64(sum == 0.0 ? 0.0 : sum * exp((double)ref - (double)all));
+    if (lane == 0) {
+      a.max[id] = all;
+      a.sum[id] = total;
+    }
   }
 }
 
@@ -197,21 +242,22 @@ constexpr int kBjThreads = 256, kBjList = 1024;
 __global__ __launch_bounds__(kBjThreads) void beam_join_kernel(BeamArgs a) {
   constexpr int W = kBjThreads / 64;
   __shared__ double s_score[KH_MAX_BEAMS], s_top[KH_MAX_BEAMS], s_log[KH_MAX_BEAMS];  // and the log-sum-exp's parts
-  __shared__ int s_kind[KH_MAX_BEAMS];  // 0: its chunks' logits, 1: none, 2: at its end
-  __shared__ __align__(16) uint64_t s_max[kBjThreads];
-  __shared__ uint64_t s_key[kBjList], s_flat[kBjList], s_bk[W], s_bf[W], s_t;
+  __shared__ int s_kind[KH_MAX_BEAMS];  // 0: its parts' logits, 1: none, 2: at its end
+  __shared__ uint64_t s_key[kBjList], s_flat[kBjList], s_bk[W], s_bf[W];
+  __shared__ uint32_t s_t;
   __shared__ int s_n;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
     for (int i = wave; i < a.beams; i += W) {
-      const int64_t r = b * a.beams + i, at = r * a.chunks;
+      const int64_t r = b * a.beams + i, at = r * a.parts;
       float m = -INFINITY;
-      for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, a.max[at + c]);
+      for (int c = lane; c < a.parts; c += 64) m = fmaxf(m, a.max[at + c]);
       m = wave_max(m);
       double s = 0.0;
-      for (int c = lane; c < a.chunks; c += 64) {
+      for (int c = lane; c < a.parts; c += 64) {
         const float mc = a.max[at + c];
-        s += mc == -INFINITY ? a.sum[at + c] : a.sum[at + c] * exp((double)mc - (double)m);
+        const double sc = a.sum[at + c];
+        s += sc == 0.0 ? 0.0 : sc * exp((double)mc - (double)m);
       }
       s = wave_sum_f64(s);
       if (lane == 0) {
@@ -225,14 +271,14 @@ __global__ __launch_bounds__(kBjThreads) void beam_join_kernel(BeamArgs a) {
     }
     if (t == 0) s_n = 0, s_t = 0;
     __syncthreads();
-    const int each = a.chunks * a.k, all = a.beams * each;
+    const int each = a.parts * a.k, all = a.beams * each;
     // continuation j: its key and its place among all; false: there is none
     const auto get = [&](int j, uint64_t& key, uint64_t& flat) {
       const int i = j / each, e = j - i * each;
       const uint64_t base = (uint64_t)i * (uint64_t)a.vocab;
       const int kind = s_kind[i];
       if (kind == 0) {
-        const uint64_t w = a.top[((b * a.beams + i) * a.chunks) * a.k + e];
+        const uint64_t w = a.top[((b * a.beams + i) * a.parts) * a.k + e];
         const uint32_t k32 = (uint32_t)(w >> 32);
         const double x = (double)__uint_as_float(k32 >> 31 ? k32 & 0x7fffffffu : ~k32);
         key = f64_key(s_score[i] + ((x - s_top[i]) - s_log[i]));  // logits of any size leave the score its bits
@@ -249,21 +295,19 @@ __global__ __launch_bounds__(kBjThreads) void beam_join_kernel(BeamArgs a) {
       flat = base + (uint64_t)v;
       return e < a.k && e < a.vocab;
     };
-    uint64_t mine = 0;
+    // the k-th largest of the lanes' own maxima, by their upper words
+    uint32_t mine = 0;
     for (int j = t; j < all; j += kBjThreads) {
       uint64_t key, flat;
-      if (get(j, key, flat) && key > mine) mine = key;
+      if (get(j, key, flat)) mine = max(mine, (uint32_t)(key >> 32));
     }
-    s_max[t] = mine;
+    const uint32_t Tw = kth_largest(a.k, 0, [&](uint32_t v) { return ballots(mine >= v); });
+    if (lane == 0) atomicMax(&s_t, Tw);
     __syncthreads();
-    int rank = 0;
-    for (int i = 0; i < kBjThreads; ++i) rank += s_max[i] > mine || (s_max[i] == mine && i < t) ? 1 : 0;
-    if (rank == a.k - 1) s_t = mine;
-    __syncthreads();
-    const uint64_t T = s_t;
+    const uint32_t T = s_t;
     for (int j = t; j < all; j += kBjThreads) {
       uint64_t key, flat;
-      if (get(j, key, flat) && key >= T) {
+      if (get(j, key, flat) && (uint32_t)(key >> 32) >= T) {
         const int at = atomicAdd(&s_n, 1);
         if (at < kBjList) s_key[at] = key, s_flat[at] = flat;
       }
@@ -319,10 +363,32 @@ static int beam_shape(int64_t batch, int beams, int64_t vocab, int k) {
                KH_MAX_BEAM_K);
   return KH_OK;
 }
-// Chunks of a row, wherever it starts between two 16-byte borders.
-static int beam_chunks(int64_t vocab) { return ceil_div(vocab + 7, kBmChunk); }
+// Parts of a row (tiles of a part), wherever it starts between two 16-byte borders: as many waves as the chip holds.
+struct BeamPlan {
+  int parts, tiles;
+};
+static BeamPlan beam_plan(int64_t rows, int64_t vocab) {
+  const int64_t all = (vocab + 7 + kBmTile - 1) / kBmTile;
+  const int64_t want = std::max<int64_t>(std::min(kBmFill / std::max<int64_t>(rows, 1), all), 1);
+  BeamPlan p;
+  p.tiles = (int)((all + want - 1) / want);
+  p.parts = (int)((all + p.tiles - 1) / p.tiles);
+  return p;
+}
 static int64_t beam_space(int64_t batch, int beams, int64_t vocab, int k) {
-  return batch * beams * beam_chunks(vocab) * (8 * (int64_t)k + 8 + 4);
+  return batch * beams * beam_plan(batch * beams, vocab).parts * (8 * (int64_t)k + 8 + 4);
+}
+template <typename T, int KC>
+static void beam_launch_k(const BeamArgs& a, hipStream_t st) {
+  const int64_t blocks = (a.batch * a.beams * a.parts + kBmWaves - 1) / kBmWaves;
+  hipLaunchKernelGGL((beam_part_kernel<T, KC>), dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(kBmThreads),
+                     kBmWaves * 32 * KC * 8, st, a);
+}
+template <typename T>
+static void beam_launch(const BeamArgs& a, hipStream_t st) {
+  if (a.k <= 16) beam_launch_k<T, 16>(a, st);
+  else if (a.k <= 32) beam_launch_k<T, 32>(a, st);
+  else beam_launch_k<T, 64>(a, st);
 }
 
 }  // namespace kh
@@ -362,7 +428,9 @@ extern "C" int kh_beam_select(int dtype, const void* logits_dev, int64_t row_str
   a.vocab = vocab;
   a.beams = beams;
   a.k = k;
-  a.chunks = beam_chunks(vocab);
+  const BeamPlan p = beam_plan(rows, vocab);
+  a.parts = p.parts;
+  a.tiles = p.tiles;
   a.scores = scores_dev;
   a.done = done_dev;
   a.end = end;
@@ -370,12 +438,11 @@ extern "C" int kh_beam_select(int dtype, const void* logits_dev, int64_t row_str
   a.out_i = out_beams_dev;
   a.out_v = out_tokens_dev;
   a.top = static_cast<uint64_t*>(ws_dev);
-  a.sum = reinterpret_cast<double*>(a.top + rows * a.chunks * k);
-  a.max = reinterpret_cast<float*>(a.sum + rows * a.chunks);
+  a.sum = reinterpret_cast<double*>(a.top + rows * a.parts * k);
+  a.max = reinterpret_cast<float*>(a.sum + rows * a.parts);
   const hipStream_t st = as_stream(stream);
-  const dim3 g((unsigned)std::min<int64_t>(rows * a.chunks, 1 << 20));
-  if (dtype == KH_DT_F32) hipLaunchKernelGGL(beam_chunk_kernel<float>, g, dim3(kBmThreads), 0, st, a);
-  else hipLaunchKernelGGL(beam_chunk_kernel<uint16_t>, g, dim3(kBmThreads), 0, st, a);
+  if (dtype == KH_DT_F32) beam_launch<float>(a, st);
+  else beam_launch<uint16_t>(a, st);
   hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)std::min<int64_t>(batch, 1 << 20)), dim3(kBjThreads), 0, st, a);
   KH_LAUNCHED();
   return KH_OK;

@@ -24,9 +24,9 @@ def scores_of(x, s, done, end):
                 continue
             top = x[b, i].max()
             with np.errstate(all="ignore"):
-                lse = top + np.log(np.exp(x[b, i] - top).sum())
-            if np.isfinite(lse):
-                y[b, i] = np.float64(s[b, i]) + (x[b, i] - lse)
+                log = np.log(np.exp(x[b, i] - top).sum())
+            if np.isfinite(top) and np.isfinite(log):  # beside a `top` of 1e38 the logarithm would be lost, to 64 bits too
+                y[b, i] = np.float64(s[b, i]) + ((x[b, i] - top) - log)
     return y.reshape(batch, -1)
 
 
@@ -115,6 +115,56 @@ def test_ties(kh, vocab, kind):
             for r in range(1, k):
                 if i[r] == i[r - 1] and y[r] > -np.inf and xs[b, i[r], v[r]] == xs[b, i[r - 1], v[r - 1]]:
                     assert v[r] > v[r - 1]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab,left", [(3000, 5), (40000, 3), (40000, 20000), (40000, 0)])
+def test_masks(kh, dtype, vocab, left):
+    """Masked tokens at -inf or at the type's lowest value; all but a few, all of a beam, the first or the last ones."""
+    rng = np.random.default_rng(left)
+    for low in (-np.inf, float(torch.finfo(dtype).min)):
+        x, s = logits(rng, 2, 3, vocab)
+        for b in range(2):
+            for i in range(3):
+                gone = rng.permutation(vocab)[left:] if i < 2 else np.arange(vocab)[-(vocab - left):]
+                x[b, i, gone] = low
+        for k in (4, 17, 64):
+            xs, got = run(x, s, k, dtype=dtype)
+            check(got, xs, s, k)
+
+
+@pytest.mark.parametrize("vocab", [5000, 70000])
+@pytest.mark.parametrize("way", ["up", "down", "steps", "late"])
+@pytest.mark.parametrize("k", [1, 16, 31, 64])
+def test_orders_of_logits(kh, vocab, way, k):
+    """Logits that rise or fall along the vocabulary (every next one is a better one), in steps of equal ones, or far
+    larger at the end."""
+    rng = np.random.default_rng(k)
+    x, s = logits(rng, 1, 2, vocab)
+    x = np.sort(x, -1)
+    if way == "down":
+        x = x[..., ::-1].copy()
+    if way == "steps":
+        x = np.floor(x * 2).astype(np.float32)
+    if way == "late":
+        x[..., -vocab // 3:] += 500
+        x[..., -3:] += 5e4
+    xs, got = run(x, s, k)
+    check(got, xs, s, k)
+
+
+def test_nan_among_others(kh):
+    """A beam with NaN here and there has no continuation, however many there are; its neighbours lose nothing."""
+    rng = np.random.default_rng(4)
+    x, s = logits(rng, 2, 4, 9000)
+    x[0, 1][rng.random(9000) < 0.9] = np.nan
+    x[0, 2, 1:] = np.nan
+    x[1, 3][rng.random(9000) < 0.3] = -np.float32(np.nan)
+    x[1, 0, 17] = np.nan
+    for k in (8, 64):
+        xs, got = run(x, s, k)
+        check(got, xs, s, k)
+        assert not np.isin(got[1][0].cpu().numpy(), (1, 2)).any() and not np.isin(got[1][1].cpu().numpy(), (0, 3)).any()
 
 
 def test_values_that_are_not_finite(kh):
