@@ -170,10 +170,12 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
       float s = 0.0f;
 #pragma unroll
       for (int e = 0; e < kBmEach; ++e) s += beam_exp(x[e] - ref);
-      if (s != s) {  // -inf or the type's lowest value among them, or what makes the sum NaN
+      if (__ballot(s != s)) {  // -inf or the type's lowest value among them, or what makes the sum NaN
+        float none = -150.0f;
+        asm volatile("" : "+v"(none));  // keeps this behind its branch
         s = 0.0f;
 #pragma unroll
-        for (int e = 0; e < kBmEach; ++e) s += x[e] == -INFINITY || x[e] - ref < -150.0f ? 0.0f : beam_exp(x[e] - ref);
+        for (int e = 0; e < kBmEach; ++e) s += x[e] == -INFINITY || x[e] - ref < none ? 0.0f : beam_exp(x[e] - ref);
       }
       sum += (double)s;
 
@@ -198,15 +200,21 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
         if (kth != 0 && (n == 0 || kth > tk >> LAST)) {
           // of the lanes whose maximum is T the first ones, by their tokens
           const int above = ballots(bk >> LAST > kth);
-          tv = kth_largest(a.k - above, 0, [&](uint32_t v) { return ballots(bk >> LAST == kth && bv >= v); });
-          tk = __builtin_amdgcn_readlane(bk, __builtin_ctzll(__ballot(bk >> LAST == kth)));
+          const uint64_t same = __ballot(bk >> LAST == kth);
+          tv = 0;
+          if (__popcll(same) > a.k - above)
+            tv = kth_largest(a.k - above, 0, [&](uint32_t v) { return ballots(bk >> LAST == kth && bv >= v); });
+          tk = __builtin_amdgcn_readlane(bk, __builtin_ctzll(same));
           mine = true;
         }
       }
+      // at or above T, as floats (a NaN is not); then exactly
+      const float from = !mine ? INFINITY : tk == 0 ? -INFINITY : __uint_as_float(tk >> 31 ? tk & 0x7fffffffu : ~tk);
 #pragma unroll
       for (int e = 0; e < kBmEach; ++e) {
+        if (!__ballot(x[e] >= from)) continue;
         const uint32_t key = f32_key(x[e]);
-        const bool take = mine && there(e) && (key > tk || (key == tk && token(e) >= tv));
+        const bool take = mine && x[e] >= from && there(e) && (key > tk || token(e) >= tv);
         const uint64_t b = __ballot(take);
         if (b) {
           if (take) list[n + __popcll(b & ((1ull << lane) - 1))] = (uint64_t)key << 32 | token(e);
@@ -236,34 +244,43 @@ __device__ __forceinline__ double key_f64(uint64_t k) {
   return __longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
 }
 
-constexpr int kBjThreads = 256, kBjList = 1024;
+// Block: a sequence.  A chain of loads: what its threads need of the parts is asked for at once, before
+// the log-sum-exps that it is scored with.
+constexpr int kBjThreads = 512, kBjEach = 4, kBjList = 1024;
 
-// Block: a sequence.
 __global__ __launch_bounds__(kBjThreads) void beam_join_kernel(BeamArgs a) {
   constexpr int W = kBjThreads / 64;
   __shared__ double s_score[KH_MAX_BEAMS], s_top[KH_MAX_BEAMS], s_log[KH_MAX_BEAMS];  // and the log-sum-exp's parts
   __shared__ int s_kind[KH_MAX_BEAMS];  // 0: its parts' logits, 1: none, 2: at its end
-  __shared__ uint64_t s_key[kBjList], s_flat[kBjList], s_bk[W], s_bf[W];
-  __shared__ uint32_t s_t;
+  __shared__ uint64_t s_key[kBjList], s_bk[W];
+  __shared__ uint32_t s_flat[kBjList], s_bf[W], s_t;
   __shared__ int s_n;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int each = a.parts * a.k, all = a.beams * each;
   for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    const uint64_t* top = a.top + b * all;
+    uint64_t mine[kBjEach];
+#pragma unroll
+    for (int c = 0; c < kBjEach; ++c) mine[c] = top[min(t + c * kBjThreads, all - 1)];
     for (int i = wave; i < a.beams; i += W) {
       const int64_t r = b * a.beams + i, at = r * a.parts;
-      float m = -INFINITY;
-      for (int c = lane; c < a.parts; c += 64) m = fmaxf(m, a.max[at + c]);
+      const float m0 = lane < a.parts ? a.max[at + lane] : -INFINITY;
+      const double d0 = lane < a.parts ? a.sum[at + lane] : 0.0;
+      const double score = (double)a.scores[r];
+      const bool ended = a.done && a.done[r];
+      float m = m0;
+      for (int c = 64 + lane; c < a.parts; c += 64) m = fmaxf(m, a.max[at + c]);
       m = wave_max(m);
-      double s = 0.0;
-      for (int c = lane; c < a.parts; c += 64) {
-        const float mc = a.max[at + c];
-        const double sc = a.sum[at + c];
-        s += sc == 0.0 ? 0.0 : sc * exp((double)mc - (double)m);
+      double s = d0 == 0.0 ? 0.0 : d0 * exp((double)m0 - (double)m);
+      for (int c = 64 + lane; c < a.parts; c += 64) {
+        const double d = a.sum[at + c];
+        s += d == 0.0 ? 0.0 : d * exp((double)a.max[at + c] - (double)m);
       }
       s = wave_sum_f64(s);
       if (lane == 0) {
-        const double score = (double)a.scores[r], l = log(s);
+        const double l = log(s);
         const bool fine = __builtin_isfinite(score), has = __builtin_isfinite(m) && __builtin_isfinite(l);
-        s_kind[i] = !fine ? 1 : a.done && a.done[r] ? 2 : has ? 0 : 1;
+        s_kind[i] = !fine ? 1 : ended ? 2 : has ? 0 : 1;
         s_score[i] = score;
         s_top[i] = (double)m;
         s_log[i] = l;
@@ -271,73 +288,82 @@ __global__ __launch_bounds__(kBjThreads) void beam_join_kernel(BeamArgs a) {
     }
     if (t == 0) s_n = 0, s_t = 0;
     __syncthreads();
-    const int each = a.parts * a.k, all = a.beams * each;
-    // continuation j: its key and its place among all; false: there is none
-    const auto get = [&](int j, uint64_t& key, uint64_t& flat) {
-      const int i = j / each, e = j - i * each;
-      const uint64_t base = (uint64_t)i * (uint64_t)a.vocab;
-      const int kind = s_kind[i];
+    // continuation j with entry w of its part: its key (0: there is none) and its place among all
+    const auto get = [&](int j, uint64_t w, uint32_t& flat) -> uint64_t {
+      const int i = (int)((uint32_t)j / (uint32_t)each), e = j - i * each, kind = s_kind[i];
+      flat = (uint32_t)i * (uint32_t)a.vocab;
       if (kind == 0) {
-        const uint64_t w = a.top[((b * a.beams + i) * a.parts) * a.k + e];
         const uint32_t k32 = (uint32_t)(w >> 32);
         const double x = (double)__uint_as_float(k32 >> 31 ? k32 & 0x7fffffffu : ~k32);
-        key = f64_key(s_score[i] + ((x - s_top[i]) - s_log[i]));  // logits of any size leave the score its bits
-        flat = base + (uint32_t)~(uint32_t)w;
-        return w != 0;
+        flat += ~(uint32_t)w;
+        return w ? f64_key(s_score[i] + ((x - s_top[i]) - s_log[i])) : 0;  // logits of any size leave the score its bits
       }
       // the first tokens, all of them -inf, but for the end
-      key = f64_key(-INFINITY);
-      int64_t v = e;
-      if (kind == 2) {
-        if (e == 0) key = f64_key(s_score[i]), v = a.end;
-        else if (e <= a.end) v = e - 1;
-      }
-      flat = base + (uint64_t)v;
-      return e < a.k && e < a.vocab;
+      if (e >= a.k || e >= a.vocab) return 0;
+      flat += kind == 1 || e > a.end ? e : e == 0 ? (uint32_t)a.end : e - 1;
+      return f64_key(kind == 2 && e == 0 ? s_score[i] : -INFINITY);
     };
+    uint64_t key[kBjEach];
+    uint32_t flat[kBjEach];
     // the k-th largest of the lanes' own maxima, by their upper words
-    uint32_t mine = 0;
-    for (int j = t; j < all; j += kBjThreads) {
-      uint64_t key, flat;
-      if (get(j, key, flat)) mine = max(mine, (uint32_t)(key >> 32));
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < kBjEach; ++c) {
+      const int j = t + c * kBjThreads;
+      key[c] = j < all ? get(j, mine[c], flat[c]) : 0;
+      most = max(most, (uint32_t)(key[c] >> 32));
     }
-    const uint32_t Tw = kth_largest(a.k, 0, [&](uint32_t v) { return ballots(mine >= v); });
+    for (int j = t + kBjEach * kBjThreads; j < all; j += kBjThreads) {
+      uint32_t f;
+      most = max(most, (uint32_t)(get(j, top[j], f) >> 32));
+    }
+    const uint32_t Tw = kth_largest(a.k, 0, [&](uint32_t v) { return ballots(most >= v); });
     if (lane == 0) atomicMax(&s_t, Tw);
     __syncthreads();
     const uint32_t T = s_t;
-    for (int j = t; j < all; j += kBjThreads) {
-      uint64_t key, flat;
-      if (get(j, key, flat) && (uint32_t)(key >> 32) >= T) {
+    const auto list = [&](uint64_t y, uint32_t f) {
+      if (y != 0 && (uint32_t)(y >> 32) >= T) {
         const int at = atomicAdd(&s_n, 1);
-        if (at < kBjList) s_key[at] = key, s_flat[at] = flat;
+        if (at < kBjList) s_key[at] = y, s_flat[at] = f;
       }
+    };
+#pragma unroll
+    for (int c = 0; c < kBjEach; ++c) list(key[c], flat[c]);
+    for (int j = t + kBjEach * kBjThreads; j < all; j += kBjThreads) {
+      uint32_t f;
+      const uint64_t y = get(j, top[j], f);
+      list(y, f);
     }
     __syncthreads();
     const int n = s_n;
-    const auto put = [&](int at, uint64_t key, uint64_t flat) {
-      a.out_y[b * a.k + at] = (float)key_f64(key);
-      a.out_i[b * a.k + at] = (int32_t)(flat / (uint64_t)a.vocab);
-      a.out_v[b * a.k + at] = (int32_t)(flat % (uint64_t)a.vocab);
+    const auto put = [&](int at, uint64_t y, uint32_t f) {
+      a.out_y[b * a.k + at] = (float)key_f64(y);
+      a.out_i[b * a.k + at] = (int32_t)(f / (uint32_t)a.vocab);
+      a.out_v[b * a.k + at] = (int32_t)(f % (uint32_t)a.vocab);
     };
     if (n <= kBjList) {
       for (int i = t; i < n; i += kBjThreads) {
-        const uint64_t key = s_key[i], flat = s_flat[i];
+        const uint64_t y = s_key[i];
+        const uint32_t f = s_flat[i];
         int above = 0;
-        for (int j = 0; j < n; ++j) above += s_key[j] > key || (s_key[j] == key && s_flat[j] < flat) ? 1 : 0;
-        if (above < a.k) put(above, key, flat);
+        for (int j = 0; j < n; ++j) above += s_key[j] > y || (s_key[j] == y && s_flat[j] < f) ? 1 : 0;
+        if (above < a.k) put(above, y, f);
       }
-    } else {
-      uint64_t lk = ~0ull, lf = 0;  // the last one written
+    } else {  // many equal scores: the best, time after time
+      uint64_t lk = ~0ull;  // the last one written
+      uint32_t lf = 0;
       for (int i = 0; i < a.k; ++i) {
-        uint64_t bk = 0, bf = ~0ull;
+        uint64_t bk = 0;
+        uint32_t bf = ~0u;
         for (int j = t; j < all; j += kBjThreads) {
-          uint64_t key, flat;
-          if (get(j, key, flat) && (key < lk || (key == lk && flat > lf)) && (key > bk || (key == bk && flat < bf)))
-            bk = key, bf = flat;
+          uint32_t f;
+          const uint64_t y = get(j, top[j], f);
+          if (y != 0 && (y < lk || (y == lk && f > lf)) && (y > bk || (y == bk && f < bf))) bk = y, bf = f;
         }
 #pragma unroll
         for (int m = 32; m > 0; m >>= 1) {
-          const uint64_t ok = __shfl_xor((unsigned long long)bk, m), of = __shfl_xor((unsigned long long)bf, m);
+          const uint64_t ok = __shfl_xor((unsigned long long)bk, m);
+          const uint32_t of = __shfl_xor(bf, m);
           if (ok > bk || (ok == bk && of < bf)) bk = ok, bf = of;
         }
         __syncthreads();
