@@ -20,7 +20,7 @@ namespace kh {
 constexpr int kBmThreads = 256, kBmWaves = kBmThreads / 64;
 constexpr int kBmEach = 16;             // logits of a lane
 constexpr int kBmTile = 64 * kBmEach;   // of a wave
-constexpr int64_t kBmFill = 8192;       // waves that the chip holds at once
+constexpr int64_t kBmFill = 4096;       // waves that the chip holds at once (512 rows of 131071: 6144 90 us, 2048 104 instead of 76)
 
 struct BeamArgs {
   const void* x;
@@ -63,11 +63,12 @@ __device__ __forceinline__ uint32_t kth_largest(int k, int last, F count) {
 }
 __device__ __forceinline__ int ballots(bool p) { return __popcll(__ballot(p)); }
 
-// Cuts a wave's list of `n` different entries to its k largest, in any order; returns their number.
+// Cuts a wave's list of n > k different entries to its k largest, in any order; returns the upper word of
+// the smallest of them.
 template <int KC>
-__device__ __forceinline__ int beam_cut(uint64_t* list, int n, int k, int last, int lane) {
-  if (n <= k) return n;
+__device__ __forceinline__ uint32_t beam_cut(uint64_t* list, int n, int k, int last, int lane) {
   constexpr int C = KC / 2;  // entries of a lane
+  __builtin_amdgcn_wave_barrier();  // the wave's writes are in order before its reads
   uint64_t x[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) x[c] = c * 64 + lane < n ? list[c * 64 + lane] : 0;
@@ -96,6 +97,7 @@ __device__ __forceinline__ int beam_cut(uint64_t* list, int n, int k, int last, 
       return m;
     });
   int at = 0;
+  uint32_t key = 0;
 #pragma unroll
   for (int c = 0; c < C; ++c)
     if (c * 64 < n) {
@@ -103,11 +105,15 @@ __device__ __forceinline__ int beam_cut(uint64_t* list, int n, int k, int last, 
       const uint64_t b = __ballot(keep);
       if (keep) list[at + __popcll(b & ((1ull << lane) - 1))] = x[c];
       at += __popcll(b);
+      const uint64_t least_ones = __ballot(keep && high(x[c]) == T >> last);
+      if (least_ones) key = __builtin_amdgcn_readlane((uint32_t)(x[c] >> 32), __builtin_ctzll(least_ones));
     }
-  return at;
+  __builtin_amdgcn_wave_barrier();
+  return key;
 }
 
-// KC: at least k; a tile adds no more than 16 k entries to the list, which is cut above 16 KC.
+// KC: at least k; a tile adds no more than 16 k entries to the list.  It is cut as soon as it holds 2 k: the
+// higher T, the fewer of the next logits pass it (with the first tile's T 16 of every tile do).
 template <typename T, int KC>
 __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
   constexpr int V = 16 / sizeof(T), Q = kBmEach / V, LAST = sizeof(T) == 2 ? 16 : 0;
@@ -221,9 +227,13 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
           n += __popcll(b);
         }
       }
-      if (n > 16 * KC) n = beam_cut<KC>(list, n, a.k, LAST, lane);
+      if (n >= 2 * a.k) {
+        tk = beam_cut<KC>(list, n, a.k, LAST, lane);
+        n = a.k;
+        tv = ~0u;  // the next ones have to be above it
+      }
     }
-    n = beam_cut<KC>(list, n, a.k, LAST, lane);
+    if (n > a.k) beam_cut<KC>(list, n, a.k, LAST, lane), n = a.k;
     uint64_t* top = a.top + id * a.k;
     if (lane < a.k) top[lane] = lane < n ? list[lane] : 0;
     const float all = wave_max(ref);
@@ -342,12 +352,16 @@ __global__ __launch_bounds__(kBjThreads) void beam_join_kernel(BeamArgs a) {
       a.out_v[b * a.k + at] = (int32_t)(f % (uint32_t)a.vocab);
     };
     if (n <= kBjList) {
-      for (int i = t; i < n; i += kBjThreads) {
+      for (int i0 = 0; i0 < n; i0 += kBjThreads / 8) {  // eight lanes an entry
+        const int i = min(i0 + (t >> 3), n - 1);
         const uint64_t y = s_key[i];
         const uint32_t f = s_flat[i];
         int above = 0;
-        for (int j = 0; j < n; ++j) above += s_key[j] > y || (s_key[j] == y && s_flat[j] < f) ? 1 : 0;
-        if (above < a.k) put(above, y, f);
+        for (int j = t & 7; j < n; j += 8) above += s_key[j] > y || (s_key[j] == y && s_flat[j] < f) ? 1 : 0;
+        above += dpp<kDppQuadSwap1>(above);
+        above += dpp<kDppQuadSwap2>(above);
+        above += dpp<kDppRowHalfMirror>(above);
+        if ((t & 7) == 0 && i0 + (t >> 3) < n && above < a.k) put(above, y, f);
       }
     } else {  // many equal scores: the best, time after time
       uint64_t lk = ~0ull;  // the last one written
