@@ -64,11 +64,15 @@ def test_evict():
                      (dict(len=None), "null"), (dict(table=None), "null"), (dict(kept=None), "null"), (dict(out=None), "null"),
                      (dict(left=None), "null"), (dict(left=P), "place of their own"), (dict(ws=P + 8), "aligned")):
         refused("kh_paged_kv_evict", change(base, **kw), ARG, text)
+    # a long sequence's rows go through the workspace, a short one's through registers
     need, lib = C.c_int64(), _lib.load()
-    assert lib.kh_paged_kv_evict_workspace(cache(), 2, 40, 100, C.byref(need)) == 0 and need.value > 0
-    refused("kh_paged_kv_evict", change(base, wsb=need.value - 1), CAP, "workspace")
-    refused("kh_paged_kv_evict", change(base, ws=None), CAP, "workspace")
-    assert lib.kh_paged_kv_evict_workspace(cache(), 2, 100, 100, C.byref(need)) == 0 and need.value == 0
+    assert lib.kh_paged_kv_evict_workspace(cache(), 2, 40, 100000, C.byref(need)) == 0 and need.value > 0
+    refused("kh_paged_kv_evict", change(base, acols=100000, wsb=need.value - 1), CAP, "workspace")
+    refused("kh_paged_kv_evict", change(base, acols=100000, ws=None), CAP, "workspace")
+    for keep, cols in ((40, 100), (100, 100), (2 ** 31 - 1, 100)):
+        assert lib.kh_paged_kv_evict_workspace(cache(), 2, keep, cols, C.byref(need)) == 0 and need.value == 0
+    for keep, cols in ((2 ** 31 - 1, 2 ** 31 - 65), (1, 2 ** 31 - 65), (2 ** 31 - 65, 2 ** 31 - 65)):
+        assert lib.kh_paged_kv_evict_workspace(cache(), 2 ** 31 - 1, keep, cols, C.byref(need)) == 0 and need.value >= 0
     refused("kh_paged_kv_evict_workspace", (cache(), 2, 0, 100, C.byref(need)), ARG, "keep")
     assert lib.kh_paged_kv_evict(*change(base, batch=0, acc=None)) == 0
 

@@ -111,11 +111,13 @@ def test_orders(kh, kind, lens, keep, recent, first, place):
     check_evicted(c, before, acc, got, keep, recent, first)
 
 
-@pytest.mark.parametrize("kv,dim,page,length,keep", [(2, 128, 64, 40000, 9000), (1, 64, 16, 70001, 20000), (1, 256, 128, 20000, 19999)])
-def test_long(kh, kv, dim, page, length, keep):
+@pytest.mark.parametrize("kv,dim,page,length,keep", [(2, 128, 64, 40000, 9000), (1, 64, 16, 70001, 20000), (1, 256, 128, 20000, 19999),
+                                                     (1, 64, 32, 16385, 600), (2, 128, 16, 20000, 30000), (1, 64, 16, 9000, 5000)])
+@pytest.mark.parametrize("kind", ["plain", "equal", "ties", "wild"])
+def test_long(kh, kv, dim, page, length, keep, kind):
     rng = np.random.default_rng(length)
     c = Cache(kv, dim, [length, 1000], page)
-    acc = weights(rng, 2, kv, c.table.shape[1] * page, "plain")
+    acc = weights(rng, 2, kv, c.table.shape[1] * page, kind)
     before = c.read()
     given = torch.from_numpy(acc).cuda()
     got = c.c.evict(given, c.len, c.table, keep, recent=500, first=4, out=given)
