@@ -5,11 +5,12 @@
 // weight T, and of those equal to T the first.  Weights are compared as integers of the same order
 // (f32_key), T is found digit by digit from histograms.
 //
-// Kept positions move towards the front of the same pages, k-th to place k, from places that are not before
-// it.  Where one block moves a kv head's rows, chunk after chunk, it reads a chunk before it
-// writes it, and nothing is lost.  Blocks of their own for parts of them could overwrite each
-// other's: long sequences' rows go to the workspace first, as images of the pages they will lie in.
+// Kept positions move towards the front of the same pages, the k-th to place k, from a place that is not
+// before it.  The 16-byte pieces of a position move alike, each among its own kind, so a block takes
+// one kind of a kv head's pieces: it has a chunk of them in registers before it writes it, from front to
+// back, and nothing is read after it was overwritten; no copy is needed.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_kv.hpp"
 #include "topk_select.hpp"
@@ -22,6 +23,7 @@ constexpr int kEvBins = 1 << kEvDigit;
 constexpr int kEvPart = 4096;         // positions of a part of a long sequence
 constexpr int kEvEach = kEvPart / kEvThreads;
 constexpr int kEvMost = 16;           // weights of a thread where a block has a whole sequence's
+
 
 struct EvictArgs {
   char* pool;
@@ -37,13 +39,11 @@ struct EvictArgs {
   int32_t* kept;
   float* acc_out;
   int64_t* len_out;
-  // long sequences: images of the pages that the kept positions will lie in, their weights,
-  // histograms of parts, and what each part begins with
-  char* images;
+  // long sequences: the kept weights, histograms of parts, and what was found of T
   float* weights;
-  uint16_t* hist;
-  int* state;  // [batch][kv heads][2 + 2 parts]: T, the ties that are kept; kept above T and ties before each part
-  int num_images, parts;
+  uint16_t* hist[3];  // of each digit, [batch][kv heads][parts][bins]
+  int* state;  // [batch][kv heads][4 + parts]: T's digits so far and the rank within, for one and two; weights of each part above two
+  int parts;
   int64_t wcols;  // weights of a kv head
 };
 
@@ -57,189 +57,37 @@ __device__ __forceinline__ int64_t evict_len(const EvictArgs& a, int64_t b, bool
 
 __device__ __forceinline__ uint32_t evict_key(float w) { return w != w ? 0xffffffffu : f32_key(w); }
 
-// ---------------------------------------------------------------- a block a kv head
-// Where position k of the kept ones comes from: its block and place; the place itself where its page is
-// none of the pool (it does not move); nullptr where that is none either.
-struct EvictFrom {
-  const char* blk;
-  int at;
-};
-__device__ __forceinline__ EvictFrom evict_from(const EvictArgs& a, const int32_t* __restrict__ table, int h, int from, int to) {
-  int pg = table[from >> a.ps_log2], at = from;
-  if (pg < 0 || pg >= a.pages) {
-    atomicOr(a.err, 2);
-    at = to;
-    pg = table[to >> a.ps_log2];
-  }
-  EvictFrom x;
-  x.blk = pg < 0 || pg >= a.pages ? nullptr : a.pool + ((int64_t)pg * a.nkv + h) * a.block;
-  x.at = at & ((1 << a.ps_log2) - 1);
-  return x;
-}
-
-// A value's codes of row r (of sixteen) of four positions, from the positions that the four
-// come from: words [position / 2][h] with a position in each half.
-template <int D, typename F>
-__device__ __forceinline__ void evict_quad(int ps, int r, F from, uint32_t (&y)[D / 32]) {
-  constexpr int HN = D / 64;
-#pragma unroll
-  for (int i = 0; i < 2 * HN; ++i) y[i] = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const EvictFrom x = from(e);
-    if (!x.blk) continue;
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(x.blk + KvParts<D>::vc(ps) + (x.at >> 2) * (2 * D)) + r * (2 * HN) + (x.at >> 1 & 1) * HN;
-#pragma unroll
-    for (int hf = 0; hf < HN; ++hf) {
-      const uint32_t u = x.at & 1 ? w[hf] >> 16 : w[hf] & 0xffffu;
-      y[(e >> 1) * HN + hf] |= e & 1 ? u << 16 : u;
-    }
-  }
-}
-
-// Moves the kept positions k0 .. n - 1 of a kv head (n of them, s_kept[k] >= k), keys (what 1) or values
-// (2) or both (3).  s_from: of a chunk.
-constexpr int kEvChunk = kEvThreads;
-template <int D>
-__device__ __forceinline__ void evict_move(const EvictArgs& a, int64_t b, int h, int n, int k0, int what, const uint16_t* s_kept,
-                                           EvictFrom* s_from) {
-  using P = KvParts<D>;
-  constexpr int NG = P::NG, HN = D / 64;
-  const int ps = 1 << a.ps_log2, t = threadIdx.x;
-  const int32_t* __restrict__ table = a.table + b * a.table_stride;
-  // place k of the chunk, or nullptr
-  const auto place = [&](int k, int& at) -> char* {
-    const int pg = table[k >> a.ps_log2];
-    at = k & (ps - 1);
-    return pg < 0 || pg >= a.pages ? nullptr : a.pool + ((int64_t)pg * a.nkv + h) * a.block;
-  };
-  for (int c0 = k0 & ~3; c0 < n; c0 += kEvChunk) {
-    const int c1 = min(c0 + kEvChunk, n), quads = (c1 - c0 + 3) >> 2;
-    // the last quad's positions past the kept ones keep what they hold
-    const int k = c0 + t;
-    if (t < 4 * quads) s_from[t] = evict_from(a, table, h, k < c1 ? s_kept[k] : k, k);
-    __syncthreads();
-    if (what & 1) {
-      constexpr int KC = D / 32;  // 16-byte pieces of a key's codes
-      uint4 c[KC];
-      uint32_t p[NG];
-#pragma unroll
-      for (int r = 0; r < KC; ++r) {
-        const int i = r * kEvChunk + t;
-        if (i < (c1 - c0) * KC) {
-          const EvictFrom x = s_from[i / KC];
-          if (x.blk) c[r] = *reinterpret_cast<const uint4*>(x.blk + P::kc() + x.at * (D / 2) + i % KC * 16);
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < NG; ++r) {
-        const int i = r * kEvChunk + t;
-        if (i < (c1 - c0) * NG) {
-          const EvictFrom x = s_from[i / NG];
-          if (x.blk) p[r] = *reinterpret_cast<const uint32_t*>(x.blk + P::kp(ps) + (x.at * NG + i % NG) * 4);
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int r = 0; r < KC; ++r) {
-        const int i = r * kEvChunk + t;
-        if (i < (c1 - c0) * KC) {
-          int at;
-          char* y = place(c0 + i / KC, at);
-          if (y && s_from[i / KC].blk) *reinterpret_cast<uint4*>(y + P::kc() + at * (D / 2) + i % KC * 16) = c[r];
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < NG; ++r) {
-        const int i = r * kEvChunk + t;
-        if (i < (c1 - c0) * NG) {
-          int at;
-          char* y = place(c0 + i / NG, at);
-          if (y && s_from[i / NG].blk) *reinterpret_cast<uint32_t*>(y + P::kp(ps) + (at * NG + i % NG) * 4) = p[r];
-        }
-      }
-    }
-    if (what & 2) {
-      constexpr int Q = 4;  // (quad, r) tasks of a thread: 16 rows of a quarter of the chunk
-      uint32_t v[Q][2 * HN], p[NG];
-#pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        const int i = q * kEvChunk + t, quad = i >> 4;
-        if (quad < quads) evict_quad<D>(ps, i & 15, [&](int e) { return s_from[quad * 4 + e]; }, v[q]);
-      }
-#pragma unroll
-      for (int j = 0; j < NG; ++j)
-        if (k < c1) {
-          const EvictFrom x = s_from[t];
-          if (x.blk) p[j] = *reinterpret_cast<const uint32_t*>(x.blk + P::vp(ps) + (j * ps + x.at) * 4);
-        }
-      __syncthreads();
-#pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        const int i = q * kEvChunk + t, quad = i >> 4;
-        if (quad < quads) {
-          int at;
-          char* y = place(c0 + quad * 4, at);
-          if (y) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(y + P::vc(ps) + (at >> 2) * (2 * D)) + (i & 15) * (2 * HN);
-#pragma unroll
-            for (int e = 0; e < 2 * HN; ++e) w[e] = v[q][e];
-          }
-        }
-      }
-      if (k < c1) {
-        int at;
-        char* y = place(k, at);
-        if (y && s_from[t].blk) {
-#pragma unroll
-          for (int j = 0; j < NG; ++j) *reinterpret_cast<uint32_t*>(y + P::vp(ps) + (j * ps + at) * 4) = p[j];
-        }
-      }
-    }
-    __syncthreads();
-  }
-}
-
+// ---------------------------------------------------------------- which positions
 // A sequence that is not cut: its weights, and its positions as they are; parts [j0, j1) of the columns.
 __device__ __forceinline__ void evict_none(const EvictArgs& a, int64_t row, int64_t L, int64_t j0, int64_t j1, int t, int nt, float* out) {
   for (int64_t j = j0 + t; j < min(j1, a.keep); j += nt) a.kept[row * a.keep + j] = j < L ? (int32_t)j : -1;
   for (int64_t j = j0 + t; j < min(j1, L); j += nt) out[j] = a.acc[row * a.acc_cols + j];
 }
 
-// Block: one kv head of one sequence, its keys or values or both (halves 2: blockIdx.z says which, and the
-// block of the keys writes what else there is).  Weights stay in registers, the kept positions in LDS.
-template <int D>
-__global__ __launch_bounds__(kEvThreads) void evict_kernel(EvictArgs a, int halves) {
+// Block: one kv head of one sequence, whose weights fit in its registers.
+__global__ __launch_bounds__(kEvThreads) void evict_whole_kernel(EvictArgs a) {
   __shared__ TopkLds<kEvThreads> sh;
-  __shared__ EvictFrom s_from[kEvChunk];
-  extern __shared__ __align__(16) uint16_t s_kept[];  // [keep]
-  const int h = blockIdx.x, t = threadIdx.x, what = halves == 1 ? 3 : blockIdx.z == 0 ? 1 : 2;
+  __shared__ uint16_t s_kept[kEvThreads * kEvMost];
+  const int h = blockIdx.x, t = threadIdx.x;
   for (int64_t b = blockIdx.y; b < a.batch; b += gridDim.y) {
-    const int64_t L = evict_len(a, b, h == 0 && t == 0 && (what & 1));
+    const int64_t L = evict_len(a, b, h == 0 && t == 0);
     const int64_t row = b * a.nkv + h, left = min(L, a.keep);
     const float* acc = a.acc + row * a.acc_cols;
     float* out = a.acc_out + row * a.acc_cols;
-    if ((what & 1) && h == 0 && t == 0) a.len_out[b] = left;
+    if (h == 0 && t == 0) a.len_out[b] = left;
     if (L <= a.keep) {
-      if (what & 1) {
-        evict_none(a, row, L, 0, max(a.acc_cols, a.keep), t, kEvThreads, out);
-        for (int64_t j = L + t; j < a.acc_cols; j += kEvThreads) out[j] = 0.0f;
-      }
-      continue;
-    }
-    const int n = (int)L - a.first - a.recent, m = (int)a.keep - a.first - a.recent, each = (n + kEvThreads - 1) / kEvThreads;
-    const int i0 = t * each, cnt = min(max(n - i0, 0), each);
-    __syncthreads();
-    if (m > 0) {
+      evict_none(a, row, L, 0, max(a.acc_cols, a.keep), t, kEvThreads, out);
+    } else {
+      const int n = (int)L - a.first - a.recent, m = (int)a.keep - a.first - a.recent, each = (n + kEvThreads - 1) / kEvThreads;
+      const int i0 = t * each, cnt = min(max(n - i0, 0), each);
       uint32_t key[kEvMost], mx = 0, mn = 0xffffffffu;
 #pragma unroll
+      for (int e = 0; e < kEvMost; ++e) key[e] = e < each ? __float_as_uint(acc[a.first + min(i0 + e, max(n - 1, 0))]) : 0;
+#pragma unroll
       for (int e = 0; e < kEvMost; ++e) {
-        key[e] = 0;
-        if (e < cnt) {
-          key[e] = evict_key(acc[a.first + i0 + e]);
-          mx = max(mx, key[e]);
-          mn = min(mn, key[e]);
-        }
+        if (e >= each) break;
+        key[e] = evict_key(__uint_as_float(key[e]));
+        if (e < cnt) mx = max(mx, key[e]), mn = min(mn, key[e]);
       }
       for (int i = t; i < (1 << kTopkDigit); i += kEvThreads) sh.hist[i] = 0;
       if (t == 0) sh.s_ncand = 0;
@@ -247,30 +95,20 @@ __global__ __launch_bounds__(kEvThreads) void evict_kernel(EvictArgs a, int halv
       mn = wave_min_u32(mn);
       if ((t & 63) == 0) sh.wmax[t >> 6] = mx, sh.wmin[t >> 6] = mn;
       __syncthreads();
+      if (m > 0) {
 #pragma unroll
-      for (int w = 0; w < kEvThreads / 64; ++w) mx = max(mx, sh.wmax[w]), mn = min(mn, sh.wmin[w]);
-      uint32_t T;
-      int ties, at;
-      topk_threshold<kEvThreads, kEvMost>(key, cnt, i0, m, mx, mn, sh, T, ties);
-      const uint32_t take = topk_select_mask<kEvThreads, kEvMost>(key, cnt, T, ties, sh, at);
+        for (int w = 0; w < kEvThreads / 64; ++w) mx = max(mx, sh.wmax[w]), mn = min(mn, sh.wmin[w]);
+        uint32_t T;
+        int ties, at;
+        topk_threshold<kEvThreads, kEvMost>(key, cnt, i0, m, mx, mn, sh, T, ties);
+        const uint32_t take = topk_select_mask<kEvThreads, kEvMost>(key, cnt, T, ties, sh, at);
 #pragma unroll
-      for (int e = 0; e < kEvMost; ++e)
-        if (take >> e & 1) s_kept[a.first + at++] = (uint16_t)(a.first + i0 + e);
-    }
-    for (int j = t; j < a.first; j += kEvThreads) s_kept[j] = (uint16_t)j;
-    for (int j = t; j < a.recent; j += kEvThreads) s_kept[a.keep - a.recent + j] = (uint16_t)(L - a.recent + j);
-    if (t == 0) sh.s_kk = (int)a.keep;
-    __syncthreads();
-    // the first one that moves: k with kept[k] > k
-    int moved = (int)a.keep;
-    for (int k = t; k < a.keep; k += kEvThreads)
-      if (s_kept[k] != k) moved = min(moved, k);
-    moved = (int)wave_min_u32((uint32_t)moved);
-    if ((t & 63) == 0) atomicMin(&sh.s_kk, moved);
-    __syncthreads();
-    moved = sh.s_kk;
-    evict_move<D>(a, b, h, (int)a.keep, moved, what, s_kept, s_from);
-    if (what & 1) {
+        for (int e = 0; e < kEvMost; ++e)
+          if (take >> e & 1) s_kept[a.first + at++] = (uint16_t)(a.first + i0 + e);
+      }
+      for (int j = t; j < a.first; j += kEvThreads) s_kept[j] = (uint16_t)j;
+      for (int j = t; j < a.recent; j += kEvThreads) s_kept[a.keep - a.recent + j] = (uint16_t)(L - a.recent + j);
+      __syncthreads();
       float w[kEvMost];
 #pragma unroll
       for (int e = 0; e < kEvMost; ++e) {
@@ -280,198 +118,404 @@ __global__ __launch_bounds__(kEvThreads) void evict_kernel(EvictArgs a, int halv
           a.kept[row * a.keep + k] = s_kept[k];
         }
       }
-      __syncthreads();
+      __syncthreads();  // out may be acc
 #pragma unroll
       for (int e = 0; e < kEvMost; ++e) {
         const int k = e * kEvThreads + t;
         if (k < a.keep) out[k] = w[e];
       }
-      for (int64_t j = a.keep + t; j < a.acc_cols; j += kEvThreads) out[j] = 0.0f;
     }
+    for (int64_t j = left + t; j < a.acc_cols; j += kEvThreads) out[j] = 0.0f;
     __syncthreads();
   }
 }
 
-// ---------------------------------------------------------------- long sequences
-// Four neighbouring weights from j on, of which those in [lo, hi) are asked for.
-__device__ __forceinline__ void evict_four(const float* __restrict__ w, int j, int lo, int hi, uint32_t (&key)[4]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) key[e] = j + e >= lo && j + e < hi ? evict_key(w[j + e]) : 0;
-}
+// Long sequences: blocks of their own for parts of kEvPart positions.
+//
+// T has three digits, of 11, 11 and 10 bits.  A launch for each makes histograms of it, one of each
+// part's weights that have T's digits before, and its blocks all find the digit before that themselves, from
+// the histograms of all parts: the launches in between would take longer.
+constexpr int kEvShift[3] = {21, 10, 0};
 
-// Histograms of the upper digit of every part's weights.
-__global__ __launch_bounds__(256) void evict_hist_kernel(EvictArgs a) {
-  __shared__ uint32_t s_hist[kEvBins];
-  const int part = blockIdx.x, h = blockIdx.y, t = threadIdx.x;
-  for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
-    const int64_t L = evict_len(a, b, false), row = b * a.nkv + h;
-    if (L <= a.keep || (int64_t)part * kEvPart >= L) continue;
-    __syncthreads();
-    for (int i = t; i < kEvBins; i += 256) s_hist[i] = 0;
-    __syncthreads();
-    const int lo = max(part * kEvPart, a.first), hi = min((part + 1) * kEvPart, (int)L - a.recent);
-    const float* acc = a.acc + row * a.acc_cols;
-#pragma unroll
-    for (int c = 0; c < kEvPart / 1024; ++c) {
-      uint32_t key[4];
-      const int j = part * kEvPart + (c * 256 + t) * 4;
-      evict_four(acc, j, lo, hi, key);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (j + e >= lo && j + e < hi) atomicAdd(&s_hist[key[e] >> (32 - kEvDigit)], 1u);
-    }
-    __syncthreads();
-    uint32_t* to = reinterpret_cast<uint32_t*>(a.hist + (row * a.parts + part) * kEvBins);
-    for (int i = t; i < kEvBins / 2; i += 256) to[i] = s_hist[2 * i] | s_hist[2 * i + 1] << 16;
-  }
-}
-
-// T from the histograms and two more digits, and what each part begins with.  Block: a kv head of a
-// sequence.
-__global__ __launch_bounds__(kEvThreads) void evict_threshold_kernel(EvictArgs a) {
-  __shared__ uint32_t hist[kEvBins];
-  __shared__ int wsum[kEvThreads / 64], total, s_kk;
-  __shared__ uint32_t s_bin;
-  const int h = blockIdx.x, t = threadIdx.x, lane = t & 63;
-  for (int64_t b = blockIdx.y; b < a.batch; b += gridDim.y) {
-    const int64_t L = evict_len(a, b, false), row = b * a.nkv + h;
-    if (L <= a.keep) continue;
-    const float* acc = a.acc + row * a.acc_cols;
-    const int lo = a.first, hi = (int)L - a.recent, parts = (int)((L + kEvPart - 1) / kEvPart);
-    int* state = a.state + row * (2 + 2 * a.parts);
-    uint32_t T = 0xffffffffu, mask = 0;
-    int kk = (int)a.keep - a.first - a.recent;
-    if (kk > 0) {
-      T = 0;
-      const uint32_t* from = reinterpret_cast<const uint32_t*>(a.hist + row * a.parts * kEvBins);
-      uint32_t x = 0, y = 0;
+struct EvictFind {
+  uint32_t hist[kEvBins];
+  int wsum[kEvThreads / 64], total, kk;
+  uint32_t bin;
+};
+// The bin that holds the kk-th largest of all parts' histograms, and its rank there; x and y: of the
+// thread's bins 2 t and 2 t + 1, what parts before `part` have.
+__device__ __forceinline__ void evict_find(const uint16_t* hists, int parts, int part, int& kk, uint32_t& bin, uint32_t& x, uint32_t& y,
+                                           EvictFind& s) {
+  const int t = threadIdx.x;
+  const uint32_t* from = reinterpret_cast<const uint32_t*>(hists) + t;
+  uint32_t u = 0, v = 0;
 #pragma unroll 8
-      for (int p = 0; p < parts; ++p) {
-        const uint32_t w = from[p * (kEvBins / 2) + t];
-        x += w & 0xffffu;
-        y += w >> 16;
-      }
-      hist[2 * t] = x;
-      hist[2 * t + 1] = y;
-      __syncthreads();
-      for (int shift = 32 - kEvDigit;;) {
-        // the bin of the kk-th largest: thread t owns two bins, thread 0 the highest
-        const int top = kEvBins - 1 - 2 * t;
-        const int n1 = (int)hist[top], n0 = (int)hist[top - 1];
-        const int above = block_excl_scan(n1 + n0, wsum, &total);
-        if (above < kk && kk <= above + n1 + n0) {
-          s_bin = kk <= above + n1 ? top : top - 1;
-          s_kk = kk - above - (kk <= above + n1 ? 0 : n1);
-        }
-        __syncthreads();
-        T |= s_bin << shift;
-        mask |= (uint32_t)(kEvBins - 1) << shift;
-        kk = s_kk;
-        if (shift == 0) break;
-        const int next = max(shift - kEvDigit, 0);  // the last digit has some bits twice: they are T's
-        for (int i = t; i < kEvBins; i += kEvThreads) hist[i] = 0;
-        __syncthreads();
-        constexpr int U = 4;
-        for (int c = lo / 4 * 4; c < hi; c += 4 * U * kEvThreads) {
-          uint32_t key[U][4];
+  for (int p = 0; p < part; ++p) {
+    const uint32_t w = from[(int64_t)p * (kEvBins / 2)];
+    u += w & 0xffffu;
+    v += w >> 16;
+  }
+  x = u;
+  y = v;
+#pragma unroll 8
+  for (int p = part; p < parts; ++p) {
+    const uint32_t w = from[(int64_t)p * (kEvBins / 2)];
+    u += w & 0xffffu;
+    v += w >> 16;
+  }
+  __syncthreads();
+  s.hist[2 * t] = u;
+  s.hist[2 * t + 1] = v;
+  __syncthreads();
+  // thread t looks at two bins, thread 0 at the highest
+  const int top = kEvBins - 1 - 2 * t, n1 = (int)s.hist[top], n0 = (int)s.hist[top - 1];
+  const int above = block_excl_scan(n1 + n0, s.wsum, &s.total);
+  if (above < kk && kk <= above + n1 + n0) {
+    s.bin = kk <= above + n1 ? top : top - 1;
+    s.kk = kk - above - (kk <= above + n1 ? 0 : n1);
+  }
+  __syncthreads();
+  kk = s.kk;
+  bin = s.bin;
+}
+
+// What a part of a long sequence has of weights that are compared, four a thread.
+struct EvictPart {
+  int64_t L, row;
+  int m, parts, lo, hi, j;
+  __device__ __forceinline__ EvictPart(const EvictArgs& a, int64_t b, int h, int part, bool tell) {
+    L = evict_len(a, b, tell);
+    row = b * a.nkv + h;
+    m = (int)a.keep - a.first - a.recent;
+    parts = (int)((L + kEvPart - 1) / kEvPart);
+    lo = a.first;
+    hi = (int)(L - a.recent);
+    j = part * kEvPart + (int)threadIdx.x * kEvEach;
+  }
+  __device__ __forceinline__ bool in(int e) const { return j + e >= lo && j + e < hi; }
+};
+
+template <int DIGIT>
+__global__ __launch_bounds__(kEvThreads) void evict_hist_kernel(EvictArgs a) {
+  __shared__ EvictFind s;
+  const int part = blockIdx.x, h = blockIdx.y, t = threadIdx.x;
+  for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
+    const EvictPart p(a, b, h, part, false);
+    if (p.L <= a.keep || part >= p.parts || p.m == 0) continue;
+    const float* acc = a.acc + p.row * a.acc_cols;
+    uint32_t key[kEvEach];
 #pragma unroll
-          for (int u = 0; u < U; ++u) evict_four(acc, c + (u * kEvThreads + t) * 4, lo, hi, key[u]);
-#pragma unroll
-          for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int j = c + (u * kEvThreads + t) * 4 + e;
-              if (j >= lo && j < hi && (key[u][e] & mask) == T) atomicAdd(&hist[(key[u][e] >> next) & (kEvBins - 1)], 1u);
-            }
-        }
-        T &= ~((uint32_t)(kEvBins - 1) << next);
-        shift = next;
-        __syncthreads();
-      }
-    }
-    // what lies before each part: counts of a wave's parts, then sums
-    for (int p = t >> 6; p < parts; p += kEvThreads / 64) {
-      int gt = 0, eq = 0;
-      const int l = max(p * kEvPart, lo), u = min((p + 1) * kEvPart, hi);
-#pragma unroll 4
-      for (int c = 0; c < kEvPart; c += 256) {
-        uint32_t key[4];
-        const int j = p * kEvPart + c + lane * 4;
-        evict_four(acc, j, l, u, key);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool in = j + e >= l && j + e < u;
-          gt += __popcll(__ballot(in && key[e] > T));
-          eq += __popcll(__ballot(in && key[e] == T));
-        }
-      }
-      if (lane == 0) state[2 + 2 * p] = gt, state[3 + 2 * p] = eq;
+    for (int e = 0; e < kEvEach; ++e) key[e] = p.in(e) ? evict_key(acc[p.j + e]) : 0;
+    int* state = a.state + p.row * (4 + a.parts);
+    uint32_t T = 0;
+    if constexpr (DIGIT > 0) {
+      int kk = DIGIT == 1 ? p.m : state[1];
+      uint32_t bin, x, y;
+      if (DIGIT == 2) T = (uint32_t)state[0];
+      evict_find(a.hist[DIGIT - 1] + p.row * a.parts * kEvBins, p.parts, 0, kk, bin, x, y, s);
+      T |= bin << kEvShift[DIGIT - 1];
+      if (part == 0 && t == 0) state[2 * DIGIT - 2] = (int)T, state[2 * DIGIT - 1] = kk;
     }
     __syncthreads();
-    if (t < 64) {
-      int g0 = 0, e0 = 0;
-      for (int c = 0; c < parts; c += 64) {
-        const int p = c + lane;
-        const int gt = p < parts ? state[2 + 2 * p] : 0, eq = p < parts ? state[3 + 2 * p] : 0;
-        const int gi = wave_incl_scan(gt), ei = wave_incl_scan(eq);
-        if (p < parts) state[2 + 2 * p] = g0 + gi - gt, state[3 + 2 * p] = e0 + ei - eq;
-        g0 += __builtin_amdgcn_readlane(gi, 63);
-        e0 += __builtin_amdgcn_readlane(ei, 63);
-      }
-      if (lane == 0) state[0] = (int)T, state[1] = (int)a.keep - a.first - a.recent > 0 ? kk : 0;
+    for (int i = t; i < kEvBins; i += kEvThreads) s.hist[i] = 0;
+    if (t == 0) s.total = 0;
+    __syncthreads();
+    int above = 0;  // of the part's, above T's digits before the last
+#pragma unroll
+    for (int e = 0; e < kEvEach; ++e) {
+      const int shift = DIGIT == 0 ? 0 : kEvShift[DIGIT == 0 ? 0 : DIGIT - 1];
+      if (p.in(e) && (DIGIT == 0 || key[e] >> shift == T >> shift)) atomicAdd(&s.hist[(key[e] >> kEvShift[DIGIT]) & (kEvBins - 1)], 1u);
+      if (DIGIT == 2) above += __popcll(__ballot(p.in(e) && key[e] >> shift > T >> shift));
     }
+    if (DIGIT == 2 && (t & 63) == 0) atomicAdd(&s.total, above);
+    __syncthreads();
+    reinterpret_cast<uint32_t*>(a.hist[DIGIT] + (p.row * a.parts + part) * kEvBins)[t] = s.hist[2 * t] | s.hist[2 * t + 1] << 16;
+    if (DIGIT == 2 && t == 0) state[4 + part] = s.total;
     __syncthreads();
   }
 }
 
-// The kept positions of a part, and their weights.
+// The last digit, then the kept positions of a part, and their weights.
 __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictArgs a) {
+  __shared__ EvictFind s;
   __shared__ uint32_t uwsum[kEvThreads / 64];
+  __shared__ int s_gt, s_eq;
   const int part = blockIdx.x, h = blockIdx.y, t = threadIdx.x;
-  const int64_t j0 = (int64_t)part * kEvPart;
   for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
-    const int64_t L = evict_len(a, b, part == 0 && h == 0 && t == 0), row = b * a.nkv + h;
+    const EvictPart p(a, b, h, part, part == 0 && h == 0 && t == 0);
+    const int64_t L = p.L, row = p.row, j0 = (int64_t)part * kEvPart;
     if (part == 0 && h == 0 && t == 0) a.len_out[b] = min(L, a.keep);
     float* weights = a.weights + row * a.wcols;
     if (L <= a.keep) {
       evict_none(a, row, L, j0, part + 1 == a.parts ? max(a.acc_cols, a.keep) : j0 + kEvPart, t, kEvThreads, weights);
       continue;
     }
-    if (j0 >= L) continue;
-    const int* state = a.state + row * (2 + 2 * a.parts);
-    const uint32_t T = (uint32_t)state[0];
-    const int ties = state[1], gt0 = state[2 + 2 * part], eq0 = state[3 + 2 * part];
+    if (part >= p.parts) continue;
     const float* acc = a.acc + row * a.acc_cols;
-    int32_t* kept = a.kept + row * a.keep;
-    const int lo = a.first, hi = (int)L - a.recent, j = (int)j0 + t * kEvEach;
     float w[kEvEach];
+#pragma unroll
+    for (int e = 0; e < kEvEach; ++e) w[e] = p.j + e < L ? acc[p.j + e] : 0.0f;
+    uint32_t T = 0xffffffffu;
+    int ties = 0, gt0 = 0, eq0 = 0;  // kept of those equal to T; above it and equal to it before the part
+    if (p.m > 0) {
+      const int* state = a.state + row * (4 + a.parts);
+      uint32_t bin, x, y;
+      ties = state[3];
+      if (t == 0) s_gt = s_eq = 0;
+      evict_find(a.hist[2] + row * a.parts * kEvBins, p.parts, part, ties, bin, x, y, s);
+      T = (uint32_t)state[2] | bin;  // the digit's upper bit is the second one's last
+      int gt = (2 * t > (int)bin ? (int)x : 0) + (2 * t + 1 > (int)bin ? (int)y : 0);
+      for (int c = t; c < part; c += kEvThreads) gt += state[4 + c];
+      gt = wave_incl_scan(gt);
+      if ((t & 63) == 63) atomicAdd(&s_gt, gt);
+      if (t == (int)(bin >> 1)) s_eq = (int)(bin & 1 ? y : x);
+      __syncthreads();
+      gt0 = s_gt;
+      eq0 = s_eq;
+    }
+    int32_t* kept = a.kept + row * a.keep;
     uint32_t gt = 0, eq = 0;
 #pragma unroll
     for (int e = 0; e < kEvEach; ++e) {
-      w[e] = j + e < L ? acc[j + e] : 0.0f;
       const uint32_t k = evict_key(w[e]);
-      const bool in = j + e >= lo && j + e < hi;
-      gt |= (in && k > T ? 1u : 0u) << e;
-      eq |= (in && k == T ? 1u : 0u) << e;
+      gt |= (p.in(e) && k > T ? 1u : 0u) << e;
+      eq |= (p.in(e) && k == T ? 1u : 0u) << e;
     }
     // both counts of a part stay below 2^16
     const uint32_t before = block_excl_scan_u32(__popc(gt) | __popc(eq) << 16, uwsum);
-    int e0 = eq0 + (int)(before >> 16), k0 = lo + gt0 + (int)(before & 0xffffu) + min(e0, ties);
+    int e0 = eq0 + (int)(before >> 16), k0 = p.lo + gt0 + (int)(before & 0xffffu) + min(e0, ties);
 #pragma unroll
     for (int e = 0; e < kEvEach; ++e) {
       const bool tie = eq >> e & 1;
       int k = -1;
       if ((gt >> e & 1) || (tie && e0 < ties)) k = k0++;
-      if (j + e < lo) k = j + e;
-      if (j + e >= hi && j + e < L) k = (int)(a.keep - (L - (j + e)));
+      if (p.j + e < p.lo) k = p.j + e;
+      if (p.j + e >= p.hi && p.j + e < L) k = (int)(a.keep - (L - (p.j + e)));
       e0 += tie ? 1 : 0;
-      if (k >= 0) kept[k] = j + e, weights[k] = w[e];
+      if (k >= 0) kept[k] = p.j + e, weights[k] = w[e];
     }
     __syncthreads();
   }
 }
 
-// The first n positions of a block of a page, to another one (or to an image of one); what lies
+// ---------------------------------------------------------------- moving them
+// Where a position comes from: its block (of page 0 where there is none) and its place there.
+struct EvictFrom {
+  const char* blk;
+  int at;
+};
+
+template <int N>
+__device__ __forceinline__ void ld_n_u32(const char* p, uint32_t* w) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  }
+}
+
+// What a block moves of a kv head's kept positions: one piece of 16 bytes of the keys' codes (D / 32
+// kinds), the keys' pairs, two of the sixteen rows of the values' codes (8 kinds), the values'
+// pairs; and, of long sequences, the kept weights to where they belong.
+template <int D>
+struct EvictKinds {
+  static constexpr int KC = D / 32, kPairs = KC, kValues = KC + 1, kValuePairs = KC + 9, kAll = KC + 10;
+};
+
+// Pieces of a thread, as its registers hold them (and places to go to).
+template <int D, int NT>
+struct EvictHold {
+  static constexpr int H = NT == 256 ? 8 : D == 256 ? 4 : 8;
+};
+// NT: threads.  1024 where much is kept: a chunk of so many positions waits for memory once.  A chunk's
+// loads are asked for together, step by step (the kept positions, their pages, the pieces), and without
+// branches: a thread without a piece loads another one's.
+template <int D, int NT>
+__global__ __launch_bounds__(NT) void evict_move_kernel(EvictArgs a) {
+  using P = KvParts<D>;
+  using K = EvictKinds<D>;
+  constexpr int NG = P::NG, HN = D / 64, H = EvictHold<D, NT>::H;
+  const int h = blockIdx.x, kind = blockIdx.z, t = threadIdx.x, lg = a.ps_log2, ps = 1 << lg;
+  for (int64_t b = blockIdx.y; b < a.batch; b += gridDim.y) {
+    const int64_t L = evict_len(a, b, false), row = b * a.nkv + h;
+    if (kind == K::kAll) {
+      float* out = a.acc_out + row * a.acc_cols;
+      const int64_t left = min(L, a.keep);
+      for (int64_t j = t; j < a.acc_cols; j += NT) out[j] = j < left ? a.weights[row * a.wcols + j] : 0.0f;
+      continue;
+    }
+    if (L <= a.keep) continue;
+    const int n = (int)a.keep;
+    const int32_t* __restrict__ kept = a.kept + row * a.keep;
+    const int32_t* __restrict__ table = a.table + b * a.table_stride;
+    const auto there = [&](int pg) { return (uint32_t)pg < (uint64_t)a.pages; };
+    const auto block = [&](int pg) { return a.pool + ((int64_t)(there(pg) ? pg : 0) * a.nkv + h) * a.block; };
+    // Of positions k[i]: where they come from (their own place if that page is none), and their place; there is none
+    // (nullptr) for what does not move.
+    const auto find = [&](auto count, const int (&k)[decltype(count)::value], const bool (&on)[decltype(count)::value],
+                          EvictFrom (&x)[decltype(count)::value], char* (&to)[decltype(count)::value]) {
+      constexpr int N = decltype(count)::value;
+      int f[N], pf[N], pt[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = kept[k[i] < n ? k[i] : n - 1];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        f[i] = k[i] < n ? f[i] : k[i];  // places past the kept ones keep what they hold
+        pf[i] = table[f[i] >> lg];
+        pt[i] = table[k[i] >> lg];
+      }
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool moves = on[i] && f[i] != k[i];
+        bad = bad || (moves && (!there(pf[i]) || !there(pt[i])));
+        to[i] = moves && there(pt[i]) ? block(pt[i]) : nullptr;
+        x[i].blk = block(there(pf[i]) ? pf[i] : pt[i]);
+        x[i].at = (there(pf[i]) ? f[i] : k[i]) & (ps - 1);
+      }
+      if (bad) atomicOr(a.err, 2);
+    };
+    if (kind < K::kValues) {
+      // a piece of the codes, or the pairs
+      const bool pairs = kind == K::kPairs;
+      const int from = pairs ? P::kp(ps) : P::kc() + kind * 16, apart = pairs ? NG * 4 : D / 2;
+      for (int c0 = 0; c0 < n; c0 += H * NT) {
+        int k[H];
+        bool on[H];
+        EvictFrom x[H];
+        char* to[H];
+        uint32_t v[H][NG > 4 ? NG : 4];
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          k[i] = c0 + i * NT + t;
+          on[i] = k[i] < n;
+          k[i] = on[i] ? k[i] : n - 1;
+        }
+        find(std::integral_constant<int, H>{}, k, on, x, to);
+        const auto move = [&](auto words) {
+          constexpr int W = decltype(words)::value;
+#pragma unroll
+          for (int i = 0; i < H; ++i)
+#pragma unroll
+            for (int w = 0; w < W; w += 4) ld_n_u32<W < 4 ? W : 4>(x[i].blk + from + x[i].at * apart + w * 4, v[i] + w);
+          __syncthreads();
+#pragma unroll
+          for (int i = 0; i < H; ++i) {
+            if (!to[i]) continue;
+            uint32_t* y = reinterpret_cast<uint32_t*>(to[i] + from + (k[i] & (ps - 1)) * apart);
+            if constexpr (W == 2) {
+              *reinterpret_cast<uint2*>(y) = make_uint2(v[i][0], v[i][1]);
+            } else {
+#pragma unroll
+              for (int w = 0; w < W; w += 4) *reinterpret_cast<uint4*>(y + w) = make_uint4(v[i][w], v[i][w + 1], v[i][w + 2], v[i][w + 3]);
+            }
+          }
+        };
+        if (pairs) move(std::integral_constant<int, NG>{});
+        else move(std::integral_constant<int, 4>{});
+      }
+    } else if (kind < K::kValuePairs) {
+      // quads of positions, two rows of the values' codes of each: words [position / 2][h] with a position in each half
+      constexpr int Q = H / 4;
+      const int r = 2 * (kind - K::kValues) + (t & 1);
+      for (int c0 = 0; c0 < n; c0 += 2 * Q * NT) {
+        uint32_t v[Q][2 * HN];
+        char* to[Q];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const int k0 = c0 + 2 * (q * NT + (t & ~1));
+          int k[4];
+          bool on[4];
+          EvictFrom x[4];
+          char* y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            on[e] = k0 < n;
+            k[e] = on[e] ? k0 + e : e;
+          }
+          find(std::integral_constant<int, 4>{}, k, on, x, y);
+          to[q] = y[0] ? y[0] : y[1] ? y[1] : y[2] ? y[2] : y[3];
+          if (to[q]) to[q] += P::vc(ps) + ((k0 & (ps - 1)) >> 2) * (2 * D) + r * (8 * HN);
+          uint32_t w[4][HN];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            ld_n_u32<HN>(x[e].blk + P::vc(ps) + (x[e].at >> 2) * (2 * D) + (r * 2 + (x[e].at >> 1 & 1)) * (HN * 4), w[e]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int hf = 0; hf < HN; ++hf) {
+              const uint32_t u = x[e].at & 1 ? w[e][hf] >> 16 : w[e][hf] & 0xffffu;
+              if (e & 1) v[q][(e >> 1) * HN + hf] |= u << 16;
+              else v[q][(e >> 1) * HN + hf] = u;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          if (!to[q]) continue;
+          uint32_t* y = reinterpret_cast<uint32_t*>(to[q]);
+#pragma unroll
+          for (int e = 0; e < 2 * HN; ++e) y[e] = v[q][e];
+        }
+      }
+    } else {
+      constexpr int HP = NG == 8 ? H / 2 : H;
+      for (int c0 = 0; c0 < n; c0 += HP * NT) {
+        int k[HP];
+        bool on[HP];
+        EvictFrom x[HP];
+        char* to[HP];
+        uint32_t v[HP][NG];
+#pragma unroll
+        for (int i = 0; i < HP; ++i) {
+          k[i] = c0 + i * NT + t;
+          on[i] = k[i] < n;
+          k[i] = on[i] ? k[i] : n - 1;
+        }
+        find(std::integral_constant<int, HP>{}, k, on, x, to);
+#pragma unroll
+        for (int i = 0; i < HP; ++i)
+#pragma unroll
+          for (int j = 0; j < NG; ++j) v[i][j] = *reinterpret_cast<const uint32_t*>(x[i].blk + P::vp(ps) + (j * ps + x[i].at) * 4);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < HP; ++i) {
+          if (!to[i]) continue;
+#pragma unroll
+          for (int j = 0; j < NG; ++j) *reinterpret_cast<uint32_t*>(to[i] + P::vp(ps) + (j * ps + (k[i] & (ps - 1))) * 4) = v[i][j];
+        }
+      }
+    }
+  }
+}
+
+template <int D>
+static int evict_launch(const EvictArgs& a, bool whole, hipStream_t st) {
+  const unsigned seqs = (unsigned)std::min<int64_t>(a.batch, 65535);
+  if (whole) {
+    hipLaunchKernelGGL(evict_whole_kernel, dim3((unsigned)a.nkv, seqs), dim3(kEvThreads), 0, st, a);
+  } else {
+    const dim3 parts((unsigned)a.parts, (unsigned)a.nkv, seqs);
+    hipLaunchKernelGGL(evict_hist_kernel<0>, parts, dim3(kEvThreads), 0, st, a);
+    hipLaunchKernelGGL(evict_hist_kernel<1>, parts, dim3(kEvThreads), 0, st, a);
+    hipLaunchKernelGGL(evict_hist_kernel<2>, parts, dim3(kEvThreads), 0, st, a);
+    hipLaunchKernelGGL(evict_select_kernel, parts, dim3(kEvThreads), 0, st, a);
+  }
+  if (a.keep < a.acc_cols || !whole) {
+    const dim3 g((unsigned)a.nkv, seqs, (unsigned)EvictKinds<D>::kAll + (whole ? 0 : 1));
+    if (a.keep <= 2048) hipLaunchKernelGGL((evict_move_kernel<D, 256>), g, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((evict_move_kernel<D, 1024>), g, dim3(1024), 0, st, a);
+  }
+  KH_LAUNCHED();
+  return KH_OK;
+}
+
+// ---------------------------------------------------------------- beams
+// The first n positions of a block of a page, to another one ; what lies
 // behind them there stays.
 template <int D>
 __device__ __forceinline__ void copy_positions(char* __restrict__ to, const char* __restrict__ from, int n, int ps, int t, int nt) {
@@ -503,101 +547,6 @@ __device__ __forceinline__ void copy_positions(char* __restrict__ to, const char
   }
 }
 
-// Images of the pages that kept positions will lie in: image i of a kv head holds positions
-// i ps .. of the kept ones.  Nothing moves in an image whose last position stays.
-__device__ __forceinline__ int evict_image(const EvictArgs& a, int64_t row, int64_t L, int image) {
-  const int ps = 1 << a.ps_log2;
-  const int64_t first = (int64_t)image << a.ps_log2;
-  if (L <= a.keep || first >= a.keep) return 0;
-  const int n = (int)min((int64_t)ps, a.keep - first);
-  return a.kept[row * a.keep + first + n - 1] == first + n - 1 ? 0 : n;
-}
-
-template <int D>
-__global__ __launch_bounds__(256) void evict_gather_kernel(EvictArgs a) {
-  using P = KvParts<D>;
-  constexpr int NG = P::NG, HN = D / 64;
-  __shared__ EvictFrom s_from[256];
-  const int h = blockIdx.y, ps = 1 << a.ps_log2, t = threadIdx.x;
-  for (int64_t bi = blockIdx.x; bi < a.batch * a.num_images; bi += gridDim.x) {
-    const int64_t b = bi / a.num_images, row = b * a.nkv + h;
-    const int image = (int)(bi - b * a.num_images), first = image << a.ps_log2;
-    const int n = evict_image(a, row, evict_len(a, b, false), image);
-    if (n == 0) continue;
-    const int32_t* __restrict__ table = a.table + b * a.table_stride;
-    __syncthreads();
-    if (t < n) s_from[t] = evict_from(a, table, h, a.kept[row * a.keep + first + t], first + t);
-    __syncthreads();
-    char* to = a.images + (row * a.num_images + image) * a.block;
-    constexpr int KC = D / 32;  // 16-byte pieces of a key
-    for (int i = t; i < n * KC; i += 256) {
-      const EvictFrom x = s_from[i / KC];
-      if (x.blk) *reinterpret_cast<uint4*>(to + P::kc() + i * 16) = *reinterpret_cast<const uint4*>(x.blk + P::kc() + x.at * (D / 2) + i % KC * 16);
-    }
-    for (int i = t; i < n * NG; i += 256) {
-      const EvictFrom x = s_from[i / NG];
-      if (x.blk) *reinterpret_cast<uint32_t*>(to + P::kp(ps) + i * 4) = *reinterpret_cast<const uint32_t*>(x.blk + P::kp(ps) + (x.at * NG + i % NG) * 4);
-    }
-    for (int i = t; i < ps * NG; i += 256) {
-      const int j = i >> a.ps_log2, k = i & (ps - 1);
-      if (k >= n) continue;
-      const EvictFrom x = s_from[k];
-      if (x.blk) *reinterpret_cast<uint32_t*>(to + P::vp(ps) + i * 4) = *reinterpret_cast<const uint32_t*>(x.blk + P::vp(ps) + (j * ps + x.at) * 4);
-    }
-    for (int i = t; i < (n + 3) / 4 * 16; i += 256) {
-      uint32_t v[2 * HN];
-      evict_quad<D>(ps, i & 15, [&](int e) { return s_from[min((i >> 4) * 4 + e, n - 1)]; }, v);
-      uint32_t* w = reinterpret_cast<uint32_t*>(to + P::vc(ps)) + i * (2 * HN);
-#pragma unroll
-      for (int e = 0; e < 2 * HN; ++e) w[e] = v[e];
-    }
-  }
-}
-
-template <int D>
-__global__ __launch_bounds__(256) void evict_place_kernel(EvictArgs a) {
-  const int h = blockIdx.y;
-  for (int64_t bi = blockIdx.x; bi < a.batch * a.num_images; bi += gridDim.x) {
-    const int64_t b = bi / a.num_images, row = b * a.nkv + h, L = evict_len(a, b, false);
-    const int image = (int)(bi - b * a.num_images);
-    // the image's share of the weights, and of the columns behind them
-    const int64_t left = min(L, a.keep), each = (a.acc_cols + a.num_images - 1) / a.num_images, to = min((image + 1) * each, a.acc_cols);
-    float* out = a.acc_out + row * a.acc_cols;
-    for (int64_t j = image * each + threadIdx.x; j < to; j += 256) out[j] = j < left ? a.weights[row * a.wcols + j] : 0.0f;
-    const int n = evict_image(a, row, L, image);
-    if (n == 0) continue;
-    const int pg = a.table[b * a.table_stride + image];
-    if (pg < 0 || pg >= a.pages) {
-      if (threadIdx.x == 0) atomicOr(a.err, 2);
-      continue;
-    }
-    copy_positions<D>(a.pool + ((int64_t)pg * a.nkv + h) * a.block, a.images + (row * a.num_images + image) * a.block, n,
-                      1 << a.ps_log2, threadIdx.x, 256);
-  }
-}
-
-template <int D>
-static int evict_launch(const EvictArgs& a, bool whole, hipStream_t st) {
-  const unsigned seqs = (unsigned)std::min<int64_t>(a.batch, 65535);
-  if (whole) {
-    // two blocks a kv head where there are few, unless one would write the weights that the other reads
-    const int halves = a.acc_out != a.acc && a.batch * a.nkv < 256 ? 2 : 1;
-    hipLaunchKernelGGL(evict_kernel<D>, dim3((unsigned)a.nkv, seqs, halves), dim3(kEvThreads),
-                       (size_t)std::min(a.keep, a.acc_cols) * 2, st, a, halves);
-    KH_LAUNCHED();
-    return KH_OK;
-  }
-  const dim3 parts((unsigned)a.parts, (unsigned)a.nkv, seqs), images((unsigned)std::min<int64_t>(a.batch * a.num_images, 1 << 20), (unsigned)a.nkv);
-  hipLaunchKernelGGL(evict_hist_kernel, parts, dim3(256), 0, st, a);
-  hipLaunchKernelGGL(evict_threshold_kernel, dim3((unsigned)a.nkv, seqs), dim3(kEvThreads), 0, st, a);
-  hipLaunchKernelGGL(evict_select_kernel, parts, dim3(kEvThreads), 0, st, a);
-  hipLaunchKernelGGL(evict_gather_kernel<D>, images, dim3(256), 0, st, a);
-  hipLaunchKernelGGL(evict_place_kernel<D>, images, dim3(256), 0, st, a);
-  KH_LAUNCHED();
-  return KH_OK;
-}
-
-// ---------------------------------------------------------------- beams
 struct ReorderArgs {
   char* pool;
   int64_t block, pages;
@@ -682,23 +631,19 @@ static int evict_shape(const kh_paged_kv* c, int64_t batch, int64_t keep, int64_
   KH_CHECK_ARG(acc_cols >= 1 && acc_cols <= INT32_MAX - 64, "weights of %lld columns", (long long)acc_cols);
   return KH_OK;
 }
-// One block a kv head takes its whole sequence where its weights fit in registers, and the rows do not
-// take it too long.
+// The workspace of long sequences, whose weights do not fit in a block's registers.
 struct EvictSpace {
   bool whole;
-  int64_t parts, images;                 // of a sequence
-  int64_t weights, hist, state, bytes;   // where they lie
+  int64_t parts, hist, state, bytes;
 };
 static EvictSpace evict_space(const kh_paged_kv* c, int64_t batch, int64_t keep, int64_t acc_cols) {
   EvictSpace s;
   const int64_t heads = batch * c->nkv;
-  s.whole = acc_cols <= kEvThreads * kEvMost && (keep <= 4096 || keep >= acc_cols || heads >= 256);
+  s.whole = acc_cols <= kEvThreads * kEvMost;
   s.parts = (acc_cols + kEvPart - 1) / kEvPart;
-  s.images = std::max<int64_t>((std::min(keep, acc_cols) + c->ps - 1) >> c->ps_log2, 1);
-  s.weights = keep >= acc_cols ? 0 : heads * s.images * c->block;  // nothing moves where all can be kept
-  s.hist = (s.weights + heads * std::min(keep, acc_cols) * 4 + 15) / 16 * 16;
-  s.state = s.hist + heads * s.parts * kEvBins * 2;
-  s.bytes = s.whole ? 0 : s.state + heads * (2 + 2 * s.parts) * 4;
+  s.hist = (heads * std::min(keep, acc_cols) * 4 + 15) / 16 * 16;
+  s.state = s.hist + 2 * heads * s.parts * kEvBins * 2;  // two digits' at a time
+  s.bytes = s.whole ? 0 : s.state + heads * (4 + s.parts) * 4;
   return s;
 }
 
@@ -758,11 +703,10 @@ extern "C" int kh_paged_kv_evict(kh_paged_kv* c, const float* acc_dev, int64_t a
   a.acc_out = acc_out_dev;
   a.len_out = len_out_dev;
   char* ws = static_cast<char*>(ws_dev);
-  a.images = ws;
-  a.weights = reinterpret_cast<float*>(ws + sp.weights);
-  a.hist = reinterpret_cast<uint16_t*>(ws + sp.hist);
+  a.weights = reinterpret_cast<float*>(ws);
+  a.hist[0] = a.hist[2] = reinterpret_cast<uint16_t*>(ws + sp.hist);
+  a.hist[1] = a.hist[0] + batch * c->nkv * sp.parts * kEvBins;
   a.state = reinterpret_cast<int*>(ws + sp.state);
-  a.num_images = (int)sp.images;
   a.parts = (int)sp.parts;
   a.wcols = std::min(keep, acc_cols);
   const hipStream_t st = as_stream(stream);
