@@ -6,9 +6,10 @@
 // (f32_key), T is found digit by digit from histograms.
 //
 // Kept positions move towards the front of the same pages, the k-th to place k, from a place that is not
-// before it.  The 16-byte pieces of a position move alike, each among its own kind, so a block takes
-// one kind of a kv head's pieces: it has a chunk of them in registers before it writes it, from front to
-// back, and nothing is read after it was overwritten; no copy is needed.
+// before it: a block that moves a kv head's keys (or values), chunk after chunk from the front, holds a
+// chunk in registers before it writes it, and nothing is read after it was overwritten.  Where few
+// kv heads keep much, such a chain takes longer than two copies: blocks of their own for pages put the rows into
+// the workspace, as images of the pages that they will lie in, and others take them there.
 #include <algorithm>
 #include <type_traits>
 
@@ -23,7 +24,6 @@ constexpr int kEvBins = 1 << kEvDigit;
 constexpr int kEvPart = 4096;         // positions of a part of a long sequence
 constexpr int kEvEach = kEvPart / kEvThreads;
 constexpr int kEvMost = 16;           // weights of a thread where a block has a whole sequence's
-
 
 struct EvictArgs {
   char* pool;
@@ -41,6 +41,8 @@ struct EvictArgs {
   int64_t* len_out;
   // long sequences: the kept weights, histograms of parts, and what was found of T
   float* weights;
+  char* images;  // of pages of kept positions
+  int num_images;
   uint16_t* hist[3];  // of each digit, [batch][kv heads][parts][bins]
   int* state;  // [batch][kv heads][4 + parts]: T's digits so far and the rank within, for one and two; weights of each part above two
   int parts;
@@ -299,12 +301,6 @@ __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictArgs a) {
 }
 
 // ---------------------------------------------------------------- moving them
-// Where a position comes from: its block (of page 0 where there is none) and its place there.
-struct EvictFrom {
-  const char* blk;
-  int at;
-};
-
 template <int N>
 __device__ __forceinline__ void ld_n_u32(const char* p, uint32_t* w) {
   if constexpr (N == 1) {
@@ -313,188 +309,243 @@ __device__ __forceinline__ void ld_n_u32(const char* p, uint32_t* w) {
     const uint2 v = *reinterpret_cast<const uint2*>(p);
     w[0] = v.x; w[1] = v.y;
   } else {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void st_n_u32(char* p, const uint32_t* w) {
+  if constexpr (N == 2) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
 }
 
-// What a block moves of a kv head's kept positions: one piece of 16 bytes of the keys' codes (D / 32
-// kinds), the keys' pairs, two of the sixteen rows of the values' codes (8 kinds), the values'
-// pairs; and, of long sequences, the kept weights to where they belong.
-template <int D>
-struct EvictKinds {
-  static constexpr int KC = D / 32, kPairs = KC, kValues = KC + 1, kValuePairs = KC + 9, kAll = KC + 10;
+// Where position k of a kv head's kept ones comes from and goes to.
+struct EvictWay {
+  int from, at, to;  // page and place that it comes from (its own place if that page is none; page 0 if that is none, too);
+                     // its place's page, -1 where there is none
+  bool moves;
 };
+__device__ __forceinline__ void evict_ways(const EvictArgs& a, const int32_t* __restrict__ kept, const int32_t* __restrict__ table, int n,
+                                           const int (&k)[2], EvictWay (&w)[2]) {
+  const int lg = a.ps_log2;
+  int f[2], pf[2], pt[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) f[i] = kept[min(k[i], n - 1)];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f[i] = k[i] < n ? f[i] : k[i];  // places past the kept ones keep what they hold
+    pf[i] = table[f[i] >> lg];
+    pt[i] = table[k[i] >> lg];
+  }
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool from = (uint32_t)pf[i] < (uint64_t)a.pages, to = (uint32_t)pt[i] < (uint64_t)a.pages;
+    w[i].moves = f[i] != k[i];
+    bad = bad || (w[i].moves && !(from && to));
+    w[i].from = from ? pf[i] : to ? pt[i] : 0;
+    w[i].at = (from ? f[i] : k[i]) & ((1 << lg) - 1);
+    w[i].to = to ? pt[i] : -1;
+  }
+  if (bad) atomicOr(a.err, 2);
+}
 
-// Pieces of a thread, as its registers hold them (and places to go to).
-template <int D, int NT>
-struct EvictHold {
-  static constexpr int H = NT == 256 ? 8 : D == 256 ? 4 : 8;
-};
-// NT: threads.  1024 where much is kept: a chunk of so many positions waits for memory once.  A chunk's
-// loads are asked for together, step by step (the kept positions, their pages, the pieces), and without
-// branches: a thread without a piece loads another one's.
-template <int D, int NT>
-__global__ __launch_bounds__(NT) void evict_move_kernel(EvictArgs a) {
+// Rows of a page (or image), as the kernels that move them see them: positions i of a chunk come from from(i)
+// (a block and a place) and go to to(i) (a block, nullptr for none) at place at(i).  A thread's pieces
+// are loaded together, without branches, and written behind `between`.
+template <int D, int NT, int CHUNK, typename F, typename G, typename A, typename B>
+__device__ __forceinline__ void evict_keys(int ps, int count, F from, G to, A at, B between) {
   using P = KvParts<D>;
-  using K = EvictKinds<D>;
-  constexpr int NG = P::NG, HN = D / 64, H = EvictHold<D, NT>::H;
-  const int h = blockIdx.x, kind = blockIdx.z, t = threadIdx.x, lg = a.ps_log2, ps = 1 << lg;
-  for (int64_t b = blockIdx.y; b < a.batch; b += gridDim.y) {
-    const int64_t L = evict_len(a, b, false), row = b * a.nkv + h;
-    if (kind == K::kAll) {
-      float* out = a.acc_out + row * a.acc_cols;
-      const int64_t left = min(L, a.keep);
-      for (int64_t j = t; j < a.acc_cols; j += NT) out[j] = j < left ? a.weights[row * a.wcols + j] : 0.0f;
-      continue;
+  constexpr int NG = P::NG, KC = D / 32, H = CHUNK * KC / NT, HP = CHUNK / NT;
+  const int t = threadIdx.x;
+  uint32_t c[H][4], p[HP][NG];
+#pragma unroll
+  for (int r = 0; r < H; ++r) {
+    const int i = r * NT + t, k = min(i / KC, count - 1);
+    int place;
+    const char* x = from(k, place);
+    ld_n_u32<4>(x + P::kc() + place * (D / 2) + i % KC * 16, c[r]);
+  }
+#pragma unroll
+  for (int r = 0; r < HP; ++r) {
+    int place;
+    const char* x = from(min(r * NT + t, count - 1), place);
+    ld_n_u32<NG>(x + P::kp(ps) + place * NG * 4, p[r]);
+  }
+  between();
+#pragma unroll
+  for (int r = 0; r < H; ++r) {
+    const int i = r * NT + t, k = i / KC;
+    char* y = k < count ? to(k) : nullptr;
+    if (y) st_n_u32<4>(y + P::kc() + at(k) * (D / 2) + i % KC * 16, c[r]);
+  }
+#pragma unroll
+  for (int r = 0; r < HP; ++r) {
+    const int k = r * NT + t;
+    char* y = k < count ? to(k) : nullptr;
+    if (y) st_n_u32<NG>(y + P::kp(ps) + at(k) * NG * 4, p[r]);
+  }
+}
+// Values: words [quad][row of sixteen][position / 2][h] of two positions' codes each.  Of the last quad's
+// positions those past `count` are the caller's, too.
+template <int D, int NT, int CHUNK, typename F, typename G, typename A, typename B>
+__device__ __forceinline__ void evict_values(int ps, int count, F from, G to, A at, B between) {
+  using P = KvParts<D>;
+  constexpr int NG = P::NG, HN = D / 64, Q = CHUNK * 4 / NT, HP = CHUNK / NT;
+  const int t = threadIdx.x, quads = (count + 3) >> 2;
+  uint32_t v[Q][2 * HN], p[HP][NG];
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    const int i = q * NT + t, r = i & 15, quad = min(i >> 4, quads - 1);
+    uint32_t w[4][HN];
+    int place[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const char* x = from(quad * 4 + e, place[e]);
+      ld_n_u32<HN>(x + P::vc(ps) + (place[e] >> 2) * (2 * D) + (r * 2 + (place[e] >> 1 & 1)) * (HN * 4), w[e]);
     }
-    if (L <= a.keep) continue;
-    const int n = (int)a.keep;
-    const int32_t* __restrict__ kept = a.kept + row * a.keep;
-    const int32_t* __restrict__ table = a.table + b * a.table_stride;
-    const auto there = [&](int pg) { return (uint32_t)pg < (uint64_t)a.pages; };
-    const auto block = [&](int pg) { return a.pool + ((int64_t)(there(pg) ? pg : 0) * a.nkv + h) * a.block; };
-    // Of positions k[i]: where they come from (their own place if that page is none), and their place; there is none
-    // (nullptr) for what does not move.
-    const auto find = [&](auto count, const int (&k)[decltype(count)::value], const bool (&on)[decltype(count)::value],
-                          EvictFrom (&x)[decltype(count)::value], char* (&to)[decltype(count)::value]) {
-      constexpr int N = decltype(count)::value;
-      int f[N], pf[N], pt[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = kept[k[i] < n ? k[i] : n - 1];
+    for (int hf = 0; hf < HN; ++hf)
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        f[i] = k[i] < n ? f[i] : k[i];  // places past the kept ones keep what they hold
-        pf[i] = table[f[i] >> lg];
-        pt[i] = table[k[i] >> lg];
-      }
-      bool bad = false;
+      for (int e = 0; e < 4; e += 2)
+        v[q][(e >> 1) * HN + hf] = (place[e] & 1 ? w[e][hf] >> 16 : w[e][hf] & 0xffffu) |
+                                   (place[e + 1] & 1 ? w[e + 1][hf] & 0xffff0000u : w[e + 1][hf] << 16);
+  }
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const bool moves = on[i] && f[i] != k[i];
-        bad = bad || (moves && (!there(pf[i]) || !there(pt[i])));
-        to[i] = moves && there(pt[i]) ? block(pt[i]) : nullptr;
-        x[i].blk = block(there(pf[i]) ? pf[i] : pt[i]);
-        x[i].at = (there(pf[i]) ? f[i] : k[i]) & (ps - 1);
-      }
-      if (bad) atomicOr(a.err, 2);
-    };
-    if (kind < K::kValues) {
-      // a piece of the codes, or the pairs
-      const bool pairs = kind == K::kPairs;
-      const int from = pairs ? P::kp(ps) : P::kc() + kind * 16, apart = pairs ? NG * 4 : D / 2;
-      for (int c0 = 0; c0 < n; c0 += H * NT) {
-        int k[H];
-        bool on[H];
-        EvictFrom x[H];
-        char* to[H];
-        uint32_t v[H][NG > 4 ? NG : 4];
+  for (int r = 0; r < HP; ++r) {
+    int place;
+    const char* x = from(min(r * NT + t, count - 1), place);
 #pragma unroll
-        for (int i = 0; i < H; ++i) {
-          k[i] = c0 + i * NT + t;
-          on[i] = k[i] < n;
-          k[i] = on[i] ? k[i] : n - 1;
-        }
-        find(std::integral_constant<int, H>{}, k, on, x, to);
-        const auto move = [&](auto words) {
-          constexpr int W = decltype(words)::value;
+    for (int j = 0; j < NG; ++j) p[r][j] = *reinterpret_cast<const uint32_t*>(x + P::vp(ps) + (j * ps + place) * 4);
+  }
+  between();
 #pragma unroll
-          for (int i = 0; i < H; ++i)
+  for (int q = 0; q < Q; ++q) {
+    const int i = q * NT + t, quad = i >> 4;
+    char* y = nullptr;
+    if (quad < quads) {
 #pragma unroll
-            for (int w = 0; w < W; w += 4) ld_n_u32<W < 4 ? W : 4>(x[i].blk + from + x[i].at * apart + w * 4, v[i] + w);
-          __syncthreads();
+      for (int e = 3; e >= 0; --e) y = quad * 4 + e < count && to(quad * 4 + e) ? to(quad * 4 + e) : y;
+    }
+    if (y) st_n_u32<2 * HN>(y + P::vc(ps) + (at(quad * 4) >> 2) * (2 * D) + (i & 15) * (8 * HN), v[q]);
+  }
 #pragma unroll
-          for (int i = 0; i < H; ++i) {
-            if (!to[i]) continue;
-            uint32_t* y = reinterpret_cast<uint32_t*>(to[i] + from + (k[i] & (ps - 1)) * apart);
-            if constexpr (W == 2) {
-              *reinterpret_cast<uint2*>(y) = make_uint2(v[i][0], v[i][1]);
-            } else {
+  for (int r = 0; r < HP; ++r) {
+    const int k = r * NT + t;
+    char* y = k < count ? to(k) : nullptr;
+    if (y) {
 #pragma unroll
-              for (int w = 0; w < W; w += 4) *reinterpret_cast<uint4*>(y + w) = make_uint4(v[i][w], v[i][w + 1], v[i][w + 2], v[i][w + 3]);
-            }
-          }
-        };
-        if (pairs) move(std::integral_constant<int, NG>{});
-        else move(std::integral_constant<int, 4>{});
-      }
-    } else if (kind < K::kValuePairs) {
-      // quads of positions, two rows of the values' codes of each: words [position / 2][h] with a position in each half
-      constexpr int Q = H / 4;
-      const int r = 2 * (kind - K::kValues) + (t & 1);
-      for (int c0 = 0; c0 < n; c0 += 2 * Q * NT) {
-        uint32_t v[Q][2 * HN];
-        char* to[Q];
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          const int k0 = c0 + 2 * (q * NT + (t & ~1));
-          int k[4];
-          bool on[4];
-          EvictFrom x[4];
-          char* y[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            on[e] = k0 < n;
-            k[e] = on[e] ? k0 + e : e;
-          }
-          find(std::integral_constant<int, 4>{}, k, on, x, y);
-          to[q] = y[0] ? y[0] : y[1] ? y[1] : y[2] ? y[2] : y[3];
-          if (to[q]) to[q] += P::vc(ps) + ((k0 & (ps - 1)) >> 2) * (2 * D) + r * (8 * HN);
-          uint32_t w[4][HN];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            ld_n_u32<HN>(x[e].blk + P::vc(ps) + (x[e].at >> 2) * (2 * D) + (r * 2 + (x[e].at >> 1 & 1)) * (HN * 4), w[e]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int hf = 0; hf < HN; ++hf) {
-              const uint32_t u = x[e].at & 1 ? w[e][hf] >> 16 : w[e][hf] & 0xffffu;
-              if (e & 1) v[q][(e >> 1) * HN + hf] |= u << 16;
-              else v[q][(e >> 1) * HN + hf] = u;
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          if (!to[q]) continue;
-          uint32_t* y = reinterpret_cast<uint32_t*>(to[q]);
-#pragma unroll
-          for (int e = 0; e < 2 * HN; ++e) y[e] = v[q][e];
-        }
-      }
-    } else {
-      constexpr int HP = NG == 8 ? H / 2 : H;
-      for (int c0 = 0; c0 < n; c0 += HP * NT) {
-        int k[HP];
-        bool on[HP];
-        EvictFrom x[HP];
-        char* to[HP];
-        uint32_t v[HP][NG];
-#pragma unroll
-        for (int i = 0; i < HP; ++i) {
-          k[i] = c0 + i * NT + t;
-          on[i] = k[i] < n;
-          k[i] = on[i] ? k[i] : n - 1;
-        }
-        find(std::integral_constant<int, HP>{}, k, on, x, to);
-#pragma unroll
-        for (int i = 0; i < HP; ++i)
-#pragma unroll
-          for (int j = 0; j < NG; ++j) v[i][j] = *reinterpret_cast<const uint32_t*>(x[i].blk + P::vp(ps) + (j * ps + x[i].at) * 4);
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < HP; ++i) {
-          if (!to[i]) continue;
-#pragma unroll
-          for (int j = 0; j < NG; ++j) *reinterpret_cast<uint32_t*>(to[i] + P::vp(ps) + (j * ps + (k[i] & (ps - 1))) * 4) = v[i][j];
-        }
-      }
+      for (int j = 0; j < NG; ++j) *reinterpret_cast<uint32_t*>(y + P::vp(ps) + (j * ps + at(k)) * 4) = p[r][j];
     }
   }
 }
 
+// Block: the keys (blockIdx.z 0) or the values of a kv head, chunk after chunk.
 template <int D>
-static int evict_launch(const EvictArgs& a, bool whole, hipStream_t st) {
+__global__ __launch_bounds__(kEvThreads) void evict_move_kernel(EvictArgs a) {
+  constexpr int CHUNK = (D == 256 ? 1 : 2) * kEvThreads;
+  __shared__ int s_from[2 * kEvThreads], s_to[2 * kEvThreads];
+  __shared__ uint8_t s_at[2 * kEvThreads];
+  const int h = blockIdx.x, t = threadIdx.x, ps = 1 << a.ps_log2;
+  char* pool = a.pool + h * a.block;
+  const int64_t apart = a.nkv * a.block;
+  for (int64_t b = blockIdx.y; b < a.batch; b += gridDim.y) {
+    if (evict_len(a, b, false) <= a.keep) continue;
+    const int n = (int)a.keep;
+    const int32_t* __restrict__ kept = a.kept + (b * a.nkv + h) * a.keep;
+    const int32_t* __restrict__ table = a.table + b * a.table_stride;
+    for (int c0 = 0; c0 < n; c0 += CHUNK) {
+      const int count = min(CHUNK, n - c0);
+      EvictWay w[2];
+      int k[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) k[i] = c0 + min(i * kEvThreads + t, (count + 3 & ~3) - 1);
+      evict_ways(a, kept, table, n, k, w);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i * kEvThreads + t >= (count + 3 & ~3)) break;
+        s_from[i * kEvThreads + t] = w[i].from;
+        s_at[i * kEvThreads + t] = (uint8_t)w[i].at;
+        s_to[i * kEvThreads + t] = w[i].moves ? w[i].to : -1;
+      }
+      __syncthreads();
+      const auto from = [&](int i, int& place) -> const char* {
+        place = s_at[i];
+        return pool + s_from[i] * apart;
+      };
+      const auto to = [&](int i) -> char* { return s_to[i] < 0 ? nullptr : pool + s_to[i] * apart; };
+      const auto at = [&](int i) { return (c0 + i) & (ps - 1); };
+      const auto between = [] { __syncthreads(); };
+      if (blockIdx.z == 0) evict_keys<D, kEvThreads, CHUNK>(ps, count, from, to, at, between);
+      else evict_values<D, kEvThreads, CHUNK>(ps, count, from, to, at, between);
+      lds_barrier();  // the tables are read; what is written need not have arrived
+    }
+  }
+}
+
+// Block: the keys (blockIdx.z 0) or the values of a kv head's positions kEvCopy c .., into images of the pages that
+// they will lie in, or from there.  Nothing moves where the last of them stays.
+constexpr int kEvCopy = 256;
+template <int D, bool BACK>
+__global__ __launch_bounds__(kEvCopy) void evict_copy_kernel(EvictArgs a) {
+  __shared__ int s_from[kEvCopy], s_to[kEvCopy];
+  __shared__ uint8_t s_at[kEvCopy];
+  const int h = blockIdx.y, ps = 1 << a.ps_log2, t = threadIdx.x, chunks = (int)((a.keep + kEvCopy - 1) / kEvCopy);
+  char* pool = a.pool + h * a.block;
+  const int64_t apart = a.nkv * a.block;
+  for (int64_t bi = blockIdx.x; bi < a.batch * chunks; bi += gridDim.x) {
+    const int64_t b = bi / chunks, row = b * a.nkv + h;
+    const int c0 = (int)(bi - b * chunks) * kEvCopy, n = (int)a.keep, count = min(kEvCopy, n - c0);
+    const int32_t* __restrict__ kept = a.kept + row * a.keep;
+    if (evict_len(a, b, false) <= n || kept[c0 + count - 1] == c0 + count - 1) continue;
+    EvictWay w[2];
+    const int k[2] = {c0 + min(t, (count + 3 & ~3) - 1), c0};
+    evict_ways(a, kept, a.table + b * a.table_stride, n, k, w);
+    __syncthreads();
+    s_from[t] = w[0].from;
+    s_at[t] = (uint8_t)w[0].at;
+    s_to[t] = w[0].to;
+    __syncthreads();
+    char* images = a.images + row * a.num_images * a.block;
+    const auto page = [&](int i) { return s_to[i] < 0 ? nullptr : pool + s_to[i] * apart; };
+    const auto moved = [&](int i, int& place) -> const char* {
+      place = s_at[i];
+      return pool + s_from[i] * apart;
+    };
+    const auto at = [&](int i) { return (c0 + i) & (ps - 1); };
+    const auto image = [&](int i) { return images + ((c0 + i) >> a.ps_log2) * a.block; };
+    const auto held = [&](int i, int& place) -> const char* {
+      place = at(i);
+      return image(i);
+    };
+    const auto copy = [&](auto from, auto to) {
+      if (blockIdx.z == 0) evict_keys<D, kEvCopy, kEvCopy>(ps, count, from, to, at, [] {});
+      else evict_values<D, kEvCopy, kEvCopy>(ps, count, from, to, at, [] {});
+    };
+    if constexpr (BACK) copy(held, page);
+    else copy(moved, image);
+  }
+}
+
+// The kept weights of long sequences, which parts found beside each other's reading, and zeros behind them.
+__global__ __launch_bounds__(256) void evict_weights_kernel(EvictArgs a) {
+  const int h = blockIdx.y;
+  const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
+    const int64_t row = b * a.nkv + h, left = min(evict_len(a, b, false), a.keep);
+    if (j < a.acc_cols) a.acc_out[row * a.acc_cols + j] = j < left ? a.weights[row * a.wcols + j] : 0.0f;
+  }
+}
+
+template <int D>
+static int evict_launch(const EvictArgs& a, bool whole, bool chain, hipStream_t st) {
   const unsigned seqs = (unsigned)std::min<int64_t>(a.batch, 65535);
   if (whole) {
     hipLaunchKernelGGL(evict_whole_kernel, dim3((unsigned)a.nkv, seqs), dim3(kEvThreads), 0, st, a);
@@ -504,18 +555,22 @@ static int evict_launch(const EvictArgs& a, bool whole, hipStream_t st) {
     hipLaunchKernelGGL(evict_hist_kernel<1>, parts, dim3(kEvThreads), 0, st, a);
     hipLaunchKernelGGL(evict_hist_kernel<2>, parts, dim3(kEvThreads), 0, st, a);
     hipLaunchKernelGGL(evict_select_kernel, parts, dim3(kEvThreads), 0, st, a);
+    hipLaunchKernelGGL(evict_weights_kernel, dim3((unsigned)((a.acc_cols + 255) / 256), (unsigned)a.nkv, seqs), dim3(256), 0, st, a);
   }
-  if (a.keep < a.acc_cols || !whole) {
-    const dim3 g((unsigned)a.nkv, seqs, (unsigned)EvictKinds<D>::kAll + (whole ? 0 : 1));
-    if (a.keep <= 2048) hipLaunchKernelGGL((evict_move_kernel<D, 256>), g, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((evict_move_kernel<D, 1024>), g, dim3(1024), 0, st, a);
+  if (a.keep >= a.acc_cols) return KH_OK;
+  if (chain) {
+    hipLaunchKernelGGL(evict_move_kernel<D>, dim3((unsigned)a.nkv, seqs, 2), dim3(kEvThreads), 0, st, a);
+  } else {
+    const dim3 g((unsigned)std::min<int64_t>(a.batch * ((a.keep + kEvCopy - 1) / kEvCopy), 1 << 20), (unsigned)a.nkv, 2);
+    hipLaunchKernelGGL((evict_copy_kernel<D, false>), g, dim3(kEvCopy), 0, st, a);
+    hipLaunchKernelGGL((evict_copy_kernel<D, true>), g, dim3(kEvCopy), 0, st, a);
   }
   KH_LAUNCHED();
   return KH_OK;
 }
 
 // ---------------------------------------------------------------- beams
-// The first n positions of a block of a page, to another one ; what lies
+// The first n positions of a block of a page, to another one; what lies
 // behind them there stays.
 template <int D>
 __device__ __forceinline__ void copy_positions(char* __restrict__ to, const char* __restrict__ from, int n, int ps, int t, int nt) {
@@ -631,19 +686,25 @@ static int evict_shape(const kh_paged_kv* c, int64_t batch, int64_t keep, int64_
   KH_CHECK_ARG(acc_cols >= 1 && acc_cols <= INT32_MAX - 64, "weights of %lld columns", (long long)acc_cols);
   return KH_OK;
 }
-// The workspace of long sequences, whose weights do not fit in a block's registers.
+// How a call is cut, and its workspace: one block a kv head selects where a sequence's weights fit in its
+// registers, and two (keys and values) move where there are enough of them or little is kept: 32 kv heads that
+// keep 2048 take 17.5 us so and 7.3 + 9.2 as two copies, 256 that keep 1024 17.2 and 14.5 + 13.4, 8 that keep
+// 32768 75 and 27.6 + 16.9.
 struct EvictSpace {
-  bool whole;
-  int64_t parts, hist, state, bytes;
+  bool whole, chain;
+  int64_t parts, images, weights, hist, state, bytes;
 };
 static EvictSpace evict_space(const kh_paged_kv* c, int64_t batch, int64_t keep, int64_t acc_cols) {
   EvictSpace s;
-  const int64_t heads = batch * c->nkv;
+  const int64_t heads = batch * c->nkv, most = std::min(keep, acc_cols);
   s.whole = acc_cols <= kEvThreads * kEvMost;
+  s.chain = keep >= acc_cols || heads >= 128 || keep <= 4096;
   s.parts = (acc_cols + kEvPart - 1) / kEvPart;
-  s.hist = (heads * std::min(keep, acc_cols) * 4 + 15) / 16 * 16;
-  s.state = s.hist + 2 * heads * s.parts * kEvBins * 2;  // two digits' at a time
-  s.bytes = s.whole ? 0 : s.state + heads * (4 + s.parts) * 4;
+  s.images = (most + c->ps - 1) >> c->ps_log2;
+  s.weights = s.chain ? 0 : heads * s.images * c->block;
+  s.hist = s.weights + (s.whole ? 0 : (heads * most * 4 + 15) / 16 * 16);
+  s.state = s.hist + (s.whole ? 0 : 2 * heads * s.parts * kEvBins * 2);  // two digits' at a time
+  s.bytes = s.state + (s.whole ? 0 : heads * (4 + s.parts) * 4);
   return s;
 }
 
@@ -703,14 +764,16 @@ extern "C" int kh_paged_kv_evict(kh_paged_kv* c, const float* acc_dev, int64_t a
   a.acc_out = acc_out_dev;
   a.len_out = len_out_dev;
   char* ws = static_cast<char*>(ws_dev);
-  a.weights = reinterpret_cast<float*>(ws);
+  a.images = ws;
+  a.num_images = (int)sp.images;
+  a.weights = reinterpret_cast<float*>(ws + sp.weights);
   a.hist[0] = a.hist[2] = reinterpret_cast<uint16_t*>(ws + sp.hist);
   a.hist[1] = a.hist[0] + batch * c->nkv * sp.parts * kEvBins;
   a.state = reinterpret_cast<int*>(ws + sp.state);
   a.parts = (int)sp.parts;
   a.wcols = std::min(keep, acc_cols);
   const hipStream_t st = as_stream(stream);
-  return c->d == 64 ? evict_launch<64>(a, sp.whole, st) : c->d == 128 ? evict_launch<128>(a, sp.whole, st) : evict_launch<256>(a, sp.whole, st);
+  return c->d == 64 ? evict_launch<64>(a, sp.whole, sp.chain, st) : c->d == 128 ? evict_launch<128>(a, sp.whole, sp.chain, st) : evict_launch<256>(a, sp.whole, sp.chain, st);
 }
 
 extern "C" int kh_paged_kv_reorder(kh_paged_kv* c, const int32_t* table_dev, int64_t table_cols, int64_t table_stride,
