@@ -62,6 +62,25 @@ struct Raw8 {
                         __float_as_uint(f[4]) >> 16 | __float_as_uint(f[5]), __float_as_uint(f[6]) >> 16 | __float_as_uint(f[7]));
     }
   }
+  // Zeros unless on.
+  __device__ __forceinline__ void keep(bool on) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = make_uint4(on ? w[i].x : 0, on ? w[i].y : 0, on ? w[i].z : 0, on ? w[i].w : 0);
+  }
+  // The largest absolute value, as an f32's bits.
+  __device__ __forceinline__ uint32_t largest() const {
+    if constexpr (sizeof(T) == 4) {
+      const auto m = [](const uint4& v) {
+        return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+      };
+      return max(m(w[0]), m(w[1]));
+    } else {
+      typedef unsigned short pair __attribute__((ext_vector_type(2)));
+      const auto p = [](uint32_t u) { return __builtin_bit_cast(pair, u & 0x7fff7fffu); };
+      const pair m = __builtin_elementwise_max(__builtin_elementwise_max(p(w[0].x), p(w[0].y)), __builtin_elementwise_max(p(w[0].z), p(w[0].w)));
+      return (uint32_t)max(m.x, m.y) << 16;
+    }
+  }
   __device__ __forceinline__ void get(float (&f)[8]) const {
     if constexpr (sizeof(T) == 4) {
       f[0] = __uint_as_float(w[0].x); f[1] = __uint_as_float(w[0].y); f[2] = __uint_as_float(w[0].z); f[3] = __uint_as_float(w[0].w);
@@ -121,6 +140,13 @@ __device__ __forceinline__ float across_groups_max(float v) {
 }
 __device__ __forceinline__ float across_groups_sum(float v) {
   return across_groups(v, [](float x, float y) { return x + y; });
+}
+
+__device__ __forceinline__ uint32_t across_groups_max_u32(uint32_t u) {
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t w = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return max(b[0], b[1]);
 }
 
 __device__ __forceinline__ uint32_t across_groups_or(uint32_t u) {

@@ -24,6 +24,7 @@ namespace kh {
 
 constexpr int kWtWaves = 4;
 constexpr float kWtNone = 0x1p100f;  // a log-sum-exp whose rows add nothing
+constexpr int kWtNew = 3;               // steps whose time a share's next block of rows costs
 constexpr int kWtNear = 7;           // powers of two between the largest and the smallest row of a tile with one scale
 
 struct WtArgs {
@@ -45,8 +46,11 @@ struct WtArgs {
   float* acc;
   int64_t acc_cols;
   int qvec;
-  float* sums;      // [batch][kv heads][chunks][parts * part] sums of chunks of rows
-  int chunks, parts, part;  // chunks of a sequence's rows, parts of its positions, positions of a part
+  // many rows: shares of a kv head's steps, their sums [batch][kv heads][shares][reach], and which of those a share has
+  float* sums;
+  int2* range;
+  int shares;
+  int64_t reach;
 };
 
 typedef _Float16 kh_f16x8 __attribute__((ext_vector_type(8)));
@@ -57,7 +61,8 @@ __device__ __forceinline__ uint32_t f16x2(float x, float y) {
   const kh_f16x2 h = {(_Float16)x, (_Float16)y};
   return __builtin_bit_cast(uint32_t, h);
 }
-// Eight f32 in f16 terms: x = t[0] + t[1] + ...
+// Eight f32 in f16 terms: x = t[0] + t[1] + ..., each towards zero (one instruction a pair): three
+// leave less than 2^-30 of x, or than f16's smallest number.
 template <int NT>
 __device__ __forceinline__ void terms8h(const float (&f)[8], uint4 (&t)[NT]) {
   float r[8];
@@ -68,7 +73,7 @@ __device__ __forceinline__ void terms8h(const float (&f)[8], uint4 (&t)[NT]) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w[i] = f16x2(r[2 * i], r[2 * i + 1]);
+      w[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r[2 * i], r[2 * i + 1]));
       const kh_f16x2 h = __builtin_bit_cast(kh_f16x2, w[i]);
       r[2 * i] -= (float)h.x;
       r[2 * i + 1] -= (float)h.y;
@@ -102,22 +107,30 @@ struct WtRows {
     const float lse = a.lse[t * a.nh + head];
     const bool on = inside && !__builtin_isinf(lse);
     nl = on ? -lse * kLog2e : -kWtNone;
-    float top = 0.0f;  // of the row's finite elements
+    uint32_t top = 0;  // of the row's finite elements, as an f32's bits
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      float f[8];
-      raw[j].get(f);
+      raw[j].keep(on);
+      top = max(top, raw[j].largest());
+    }
+    if (__ballot(top >= 0x7f800000u)) {
+      top = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float y = __builtin_fabsf(f[k]);
-        top = on && y < INFINITY ? fmaxf(top, y) : top;
+      for (int j = 0; j < NG; ++j) {
+        float f[8];
+        raw[j].get(f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t y = __float_as_uint(f[k]) & 0x7fffffffu;
+          top = y < 0x7f800000u ? max(top, y) : top;
+        }
       }
     }
-    top = across_groups_max(top);
+    top = across_groups_max_u32(top);
     // elements below 2^9, so that sums of 32 are below 2^14
-    int e = min(max(exponent_of(top) - 8, -100), 118);
-    const int most = (int)wave_max_u32((uint32_t)(top > 0.0f ? e + 128 : 0)) - 128;
-    one = __ballot(top > 0.0f && e < most - kWtNear) == 0;
+    int e = min(max((int)(top >> 23) - 135, -100), 118);
+    const int most = (int)wave_max_u32((uint32_t)(top > 0 ? e + 128 : 0)) - 128;
+    one = __ballot(top > 0 && e < most - kWtNear) == 0;
     if (one) e = max(most, -100);
     r = pow2(e);
     const float down = pow2(-e);
@@ -127,7 +140,7 @@ struct WtRows {
       float f[8];
       raw[j].get(f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = on ? f[k] * down : 0.0f;
+      for (int k = 0; k < 8; ++k) f[k] *= down;
       const float s[8] = {f[0], f[4], f[1], f[5], f[2], f[6], f[3], f[7]};
       uint4 tm[NQ];
       terms8h<NQ>(s, tm);
@@ -353,16 +366,19 @@ __global__ __launch_bounds__(64 * kWtWaves) void paged_weights_kernel(WtArgs a) 
 }
 
 // ---------------------------------------------------------------- many rows
-// A wave keeps RT tiles of rows, and the waves of a block run the same positions: a step's 64
-// are unpacked once for all of them, to LDS as operands, while the step before is worked on.  The
-// waves' sums of a step meet in LDS, and 64 threads add them up in the order of the waves.
+// A wave keeps RT tiles of rows, and the waves of a block run the same positions: a step's 128
+// (64) are unpacked once for all of them, to LDS as operands, while the step before is worked on.  The
+// waves' sums of a step meet in LDS, and as many threads as positions add them up in the order of the waves.
 //
-// A block takes every chunks-th block of rows and one part of the positions, and has sums of its own in
-// the workspace; a second kernel adds those to acc in the order of the chunks.
+// A kv head's steps, of all its blocks of rows after each other, are cut in shares of the same length for blocks, since
+// a causal mask leaves blocks of rows unlike numbers of them and since each new block of rows costs a share as
+// much as some steps (its rows become operands).  A share has sums of its own in the workspace;
+// a second kernel adds those to acc in the order of the shares.
 template <int D, typename T>
 struct WtShape {
   using R = WtRows<D, T>;
-  static constexpr int NW = 8, KEYS = 64, TK = KEYS / 16;
+  static constexpr int NW = 8, KEYS = D == 256 ? 64 : 128, TK = KEYS / 16;
+  static constexpr int PARTS = NW / TK, NGW = R::NG / PARTS;  // waves that unpack a tile, and groups that each takes
   static constexpr int RT = R::NF <= 7 ? 4 : R::NF <= 13 ? 2 : 1;
   static constexpr int RB = 16 * RT * NW;                 // rows of a block
   static constexpr int NK = R::NG + R::NB;                // operands of a tile of positions
@@ -376,256 +392,366 @@ __global__ __launch_bounds__((64 * WtShape<D, T>::NW), 2) void paged_weights_til
   using S = WtShape<D, T>;
   using P = KvParts<D>;
   constexpr int NG = R::NG, NB = R::NB, NW = S::NW, KEYS = S::KEYS, TK = S::TK, RT = S::RT, RB = S::RB, NK = S::NK;
-  constexpr int HALF = NG / 2;  // groups of a position that a wave unpacks
+  constexpr int NGW = S::NGW;
   extern __shared__ __align__(16) char s_buf[];
   float* s_f = reinterpret_cast<float*>(s_buf + 2 * S::kStep);  // [2][KEYS]
   float* s_sum = s_f + 2 * KEYS;                                // [2][NW][KEYS]
-  __shared__ int s_lo[NW], s_hi[NW];
   __shared__ int s_state[2][TK];  // of a step's tiles: 0, 1 where a key holds a NaN, 2 where there is no page
   const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15, tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int ps = 1 << a.ps_log2, utile = wave >> 1, uhalf = wave & 1;
+  const int ps = 1 << a.ps_log2, utile = wave / S::PARTS, ugroup = wave % S::PARTS * NGW;
   // the kv head varies fastest: there are eight XCDs, and each keeps its heads' pages
-  uint32_t id = blockIdx.x;
-  const int h = (int)(id % (uint32_t)a.nkv);
-  id /= (uint32_t)a.nkv;
-  const int part = (int)(id % (uint32_t)a.parts), chunk = a.chunks - 1 - (int)(id / (uint32_t)a.parts);
+  const int h = (int)(blockIdx.x % (uint32_t)a.nkv), share = (int)(blockIdx.x / (uint32_t)a.nkv);
   for (int64_t b = blockIdx.y; b < a.batch; b += gridDim.y) {
     WtSeq s;
     if (!wt_seq(a, b, tid == 0 && blockIdx.x == 0, s)) continue;
-    float* acc = a.acc + (b * a.nkv + h) * a.acc_cols;
-    for (int64_t p0 = (int64_t)part * a.part; p0 < s.E; p0 += (int64_t)a.parts * a.part) {
-      // positions past the guess have no sums of their own: one block takes all of their rows
-      const bool own = a.chunks > 1 && p0 < (int64_t)a.parts * a.part;
-      if (a.chunks > 1 && !own && chunk > 0) break;
-      const int p1 = (int)min(p0 + a.part, (int64_t)s.E);
-      // sums go to out[j], by the same thread each time
-      float* out = own ? a.sums + ((b * a.nkv + h) * a.chunks + chunk) * ((int64_t)a.parts * a.part) : acc;
-      if (own && tid < KEYS)
-        for (int j = (int)p0 + tid; j < p1; j += KEYS) out[j] = 0.0f;
-      for (int rb = own ? chunk : 0; (int64_t)rb * RB < s.nr; rb += own ? a.chunks : 1) {
-        const int w0 = (rb * NW + wave) * RT * 16;  // the wave's first row
-        // positions that some of the wave's rows see, and those that all of them see
-        uint32_t lo = 0x7fffffffu, hi = 0, all_lo = 0, all_hi = 0x7fffffffu;
-        if (w0 < s.nr) {
-          const int64_t i0 = w0 / a.gs, i1 = (min(w0 + RT * 16, s.nr) - 1) / a.gs;
-          const int64_t L = s.before + s.n, q0 = s.before + i0, q1 = s.before + i1;
-          const int64_t x = a.window > 0 ? max(q0 - a.window + 1, (int64_t)0) : 0, xa = a.window > 0 ? max(q1 - a.window + 1, (int64_t)0) : 0;
-          const int64_t y = a.causal ? min(q1 + 1, L) : L, ya = a.causal ? min(q0 + 1, L) : L;
-          if (y > x) lo = (uint32_t)x, hi = (uint32_t)y;
-          all_lo = (uint32_t)xa;
-          all_hi = (uint32_t)max(ya, (int64_t)0);
+    const int nrb = (int)(((int64_t)s.nr + RB - 1) / RB);
+    // positions [x, y) that some of rows r0 .. r1 - 1 see, and the steps that hold them
+    const auto seen = [&](int r0, int r1, int& x, int& y) {
+      const int64_t q0 = s.before + (uint32_t)r0 / (uint32_t)a.gs, q1 = s.before + ((uint32_t)r1 - 1) / (uint32_t)a.gs;
+      const int64_t lo = a.window > 0 ? max(q0 - a.window + 1, (int64_t)0) : 0;
+      const int64_t hi = min(a.causal ? q1 + 1 : (int64_t)s.E, (int64_t)s.E);
+      x = hi > lo ? (int)lo : 0;
+      y = hi > lo ? (int)hi : 0;
+    };
+    const auto steps = [&](int rb, int& x, int& y) {
+      seen(rb * RB, (int)min((int64_t)rb * RB + RB, (int64_t)s.nr), x, y);
+      return (y + KEYS - 1) / KEYS - x / KEYS;
+    };
+    // a sequence longer than the guess is one share
+    const int shares = a.shares > 1 && s.E <= a.reach ? a.shares : 1;
+    if (share >= shares) continue;
+    int rb = 0;              // the share's first block of rows,
+    int64_t from = 0, left;  // how many of its steps (and kWtNew) others have, and how many are the share's
+    if (shares == 1) {
+      left = INT64_MAX;
+    } else {
+      const auto count = [&](int c) {
+        int x, y;
+        const int of = c + lane < nrb ? steps(c + lane, x, y) : 0;
+        return of > 0 ? of + kWtNew : 0;
+      };
+      int n = count(0), upto = wave_incl_scan(n);
+      int64_t total = __builtin_amdgcn_readlane(upto, 63);
+      for (int c = 64; c < nrb; c += 64) total += __builtin_amdgcn_readlane(wave_incl_scan(count(c)), 63);
+      from = total * (uint32_t)share / (uint32_t)shares;
+      left = total * (uint32_t)(share + 1) / (uint32_t)shares - from;
+      for (;;) {
+        const uint64_t here = __ballot(upto > from);
+        if (left == 0 || here) {
+          const int i = here ? __builtin_ctzll(here) : 0;
+          rb += i;
+          from -= __builtin_amdgcn_readlane(upto - n, i);
+          break;
         }
-        __syncthreads();  // the last block of rows is done with LDS
-        if (lane == 0) s_lo[wave] = (int)lo, s_hi[wave] = (int)hi;
-        __syncthreads();
-        int tlo = 0x7fffffff, thi = 0;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) tlo = min(tlo, s_lo[w]), thi = max(thi, s_hi[w]);
-        tlo = __builtin_amdgcn_readfirstlane(max(tlo, (int)p0));
-        thi = __builtin_amdgcn_readfirstlane(min(thi, p1));
-        if (thi <= tlo) continue;
-        const int sb = tlo / KEYS, se = (thi + KEYS - 1) / KEYS;
+        from -= __builtin_amdgcn_readlane(upto, 63);
+        rb += 64;
+        n = count(rb);
+        upto = wave_incl_scan(n);
+      }
+    }
+    float* out = a.acc + (b * a.nkv + h) * a.acc_cols;
+    if (shares > 1) {
+      const int64_t row = (b * a.nkv + h) * a.shares + share;
+      out = a.sums + row * a.reach;
+      int p0 = 0x7fffffff, p1 = 0;
+      int64_t n = left, skip = from;
+      for (int i = rb; n > 0; ++i) {
+        int x, y;
+        const int of = steps(i, x, y);
+        if (of == 0) continue;
+        const int i0 = (int)min(skip, (int64_t)of), i1 = (int)min(skip + n, (int64_t)of);
+        if (i1 > i0) {
+          p0 = min(p0, (x / KEYS + i0) * KEYS);
+          p1 = max(p1, min((x / KEYS + i1) * KEYS, s.E));
+        }
+        n -= of + kWtNew - skip;
+        skip = 0;
+      }
+      p0 = min(p0, p1);  // a share may have no steps
+      if (tid == 0) a.range[row] = make_int2(p0, p1);
+      if (tid < KEYS)
+        for (int j = p0 + tid; j < p1; j += KEYS) out[j] = 0.0f;
+    }
+    // sums go to out[j], by the same thread each time
+    for (; rb < nrb && left > 0; ++rb) {
+      int tlo, thi;
+      const int of = steps(rb, tlo, thi);
+      if (of == 0) continue;
+      const int sb = tlo / KEYS + (int)min(from, (int64_t)of), se = tlo / KEYS + (int)(left < of - from ? from + left : of);
+      left -= of + kWtNew - from;
+      from = 0;
+      if (se <= sb) continue;
+      const int w0 = (rb * NW + wave) * RT * 16;  // the wave's first row
+      // positions that some of the wave's rows see, and those that all of them see
+      uint32_t lo = 0x7fffffffu, hi = 0, all_lo = 0, all_hi = 0x7fffffffu;
+      if (w0 < s.nr) {
+        const int64_t i0 = (uint32_t)w0 / (uint32_t)a.gs, i1 = (uint32_t)(min(w0 + RT * 16, s.nr) - 1) / (uint32_t)a.gs;
+        const int64_t L = s.before + s.n, q0 = s.before + i0, q1 = s.before + i1;
+        const int64_t x = a.window > 0 ? max(q0 - a.window + 1, (int64_t)0) : 0, xa = a.window > 0 ? max(q1 - a.window + 1, (int64_t)0) : 0;
+        const int64_t y = a.causal ? min(q1 + 1, L) : L, ya = a.causal ? min(q0 + 1, L) : L;
+        if (y > x) lo = (uint32_t)x, hi = (uint32_t)y;
+        all_lo = (uint32_t)xa;
+        all_hi = (uint32_t)max(ya, (int64_t)0);
+      }
+      __syncthreads();  // the last block of rows is done with LDS
 
-        // lane i holds the page of the wave's tile of the i-th of 64 steps
-        int pages = 0;
-        const auto find = [&](int st) {
-          const int tok = (st + lane) * KEYS + utile * 16;
-          pages = tok + 16 > tlo && tok < thi ? s.table[max(tok, tlo) >> a.ps_log2] : 0;
-          if (tok + 16 > tlo && tok < thi && (pages < 0 || pages >= a.pages)) {
-            atomicOr(a.err, 2);
-            pages = -1;
-          }
-        };
-        uint32_t kw[HALF], kp[NG];
-        int pg = 0;
-        const auto load = [&](int st) {
-          pg = __builtin_amdgcn_readlane(pages, (st - sb) & 63);
-          const int tok = st * KEYS + utile * 16;
-          const char* blk = a.pool + ((int64_t)max(pg, 0) * a.nkv + h) * a.block;
-          const int at = (tok & (ps - 1)) + col;
-          ld_n<HALF>(blk + P::kc() + at * (D / 2) + (g * NG + uhalf * HALF) * 4, kw);
-          ld_words<NG>(blk + P::kp(ps) + at * NG * 4, kp);
-        };
-        const auto unpack = [&](int st) {
-          char* to = s_buf + (st & 1) * S::kStep + utile * NK * 1024 + lane * 16;
-          float f;
-          uint4 c[HALF], bb[NB];
-          wt_unpack<D, HALF>(kw, kp, uhalf * HALF, a.c1, g, c, bb, f);
+      // lane i holds the page of the wave's tile of the i-th of 64 steps
+      int pages = 0;
+      const auto find = [&](int st) {
+        const int tok = (int)((uint32_t)(st + lane) * KEYS) + utile * 16;
+        pages = tok + 16 > tlo && tok < thi ? s.table[max(tok, tlo) >> a.ps_log2] : 0;
+        if (tok + 16 > tlo && tok < thi && (pages < 0 || pages >= a.pages)) {
+          atomicOr(a.err, 2);
+          pages = -1;
+        }
+      };
+      // of a step's tile: what it holds, and its page
+      struct Tile {
+        uint32_t w[NGW], p[NG];
+        int pg;
+      } now, next;
+      const auto load = [&](int st, Tile& k) {
+        k.pg = __builtin_amdgcn_readlane(pages, (st - sb) & 63);
+        const int tok = st * KEYS + utile * 16;
+        const char* blk = a.pool + ((int64_t)max(k.pg, 0) * a.nkv + h) * a.block;
+        const int at = (tok & (ps - 1)) + col;
+        ld_n<NGW>(blk + P::kc() + at * (D / 2) + (g * NG + ugroup) * 4, k.w);
+        ld_words<NG>(blk + P::kp(ps) + at * NG * 4, k.p);
+      };
+      // without branches, so that it can lie between products: all waves of a tile write what the tile has one of
+      const auto unpack = [&](int st, const Tile& k) {
+        char* to = s_buf + (st & 1) * S::kStep + utile * NK * 1024 + lane * 16;
+        float f;
+        uint4 c[NGW], bb[NB];
+        wt_unpack<D, NGW>(k.w, k.p, ugroup, a.c1, g, c, bb, f);
 #pragma unroll
-          for (int k = 0; k < HALF; ++k) *reinterpret_cast<uint4*>(to + (uhalf * HALF + k) * 1024) = c[k];
-          if (uhalf == 0) {
+        for (int i = 0; i < NGW; ++i) *reinterpret_cast<uint4*>(to + (ugroup + i) * 1024) = c[i];
 #pragma unroll
-            for (int k = 0; k < NB; ++k) *reinterpret_cast<uint4*>(to + (NG + k) * 1024) = bb[k];
-            if (g == 0) s_f[(st & 1) * KEYS + utile * 16 + col] = f;
-            uint32_t nan = 0;
+        for (int i = 0; i < NB; ++i) *reinterpret_cast<uint4*>(to + (NG + i) * 1024) = bb[i];
+        s_f[(st & 1) * KEYS + utile * 16 + col] = f;
+        uint32_t nan = 0;
 #pragma unroll
-            for (int k = 0; k < NG; ++k) nan = max(nan, kp[k]);
-            const int state = pg < 0 ? 2 : __ballot(nan >= 0x7f800000u) ? 1 : 0;
-            if (lane == 0) s_state[st & 1][utile] = state;
-          }
-        };
-        find(sb);
-        load(sb);
+        for (int i = 0; i < NG; ++i) nan = max(nan, k.p[i]);
+        s_state[st & 1][utile] = k.pg < 0 ? 2 : __ballot(nan >= 0x7f800000u) ? 1 : 0;
+      };
+      find(sb);
+      load(sb, now);
 
-        R q[RT];
-        bool one = true;
+      R q[RT];
+      bool one = true;
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          q[t].load(a, s.o0, s.nr, h, w0 / 16 + t, lane);
-          one = one && q[t].one;
-        }
-        float nl[RT][4], r[RT];
+      for (int t = 0; t < RT; ++t) {
+        q[t].load(a, s.o0, s.nr, h, w0 / 16 + t, lane);
+        one = one && q[t].one;
+      }
+      float nl[RT][4], r[RT];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          r[t] = __shfl(q[t].r, 0);
+      for (int t = 0; t < RT; ++t) {
+        r[t] = __shfl(q[t].r, 0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) nl[t][i] = __shfl(q[t].nl, 4 * g + i);
-        }
-        unpack(sb);
-        if (sb + 1 < se) load(sb + 1);
+        for (int i = 0; i < 4; ++i) nl[t][i] = __shfl(q[t].nl, 4 * g + i);
+      }
+      unpack(sb, now);
+      if (sb + 1 < se) load(sb + 1, now);
 
-        for (int st = sb; st < se; ++st) {
-          __syncthreads();
-          if (st > sb && tid < KEYS) {
-            const float* x = s_sum + ((st - 1) & 1) * NW * KEYS + tid;
-            float w = 0.0f;
+      float old = 0.0f;  // what out holds of a step's positions
+      const auto add = [&](int st) {
+        const float* x = s_sum + (st & 1) * NW * KEYS + tid;
+        float w = 0.0f;
 #pragma unroll
-            for (int k = 0; k < NW; ++k) w += x[k * KEYS];
-            const int j = (st - 1) * KEYS + tid;
-            if (j >= p0 && j < p1 && w != 0.0f) out[j] += w;
-          }
-          const int first = st * KEYS;
-          const char* buf = s_buf + (st & 1) * S::kStep + lane * 16;
-          const float* fs = s_f + (st & 1) * KEYS;
-          float* sums = s_sum + ((st & 1) * NW + wave) * KEYS;
-          int state = 0;
-#pragma unroll
-          for (int k = 0; k < TK; ++k) state |= s_state[st & 1][k];
-          state = __builtin_amdgcn_readfirstlane(state);
-          if (st + 1 < se) {
-            unpack(st + 1);
-            if (st + 2 < se) {
-              if (((st + 2 - sb) & 63) == 0) find(st + 2);
-              load(st + 2);
-            }
-          }
-          const auto scores = [&](int k, int t) {
-            kh_f32x4 y = {0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < NB; ++i) y = mfma16h(q[t].x[NG * R::NQ + i], *reinterpret_cast<const uint4*>(buf + (k * NK + NG + i) * 1024), y);
-#pragma unroll
-            for (int j = 0; j < NG; ++j) {
-              const uint4 c = *reinterpret_cast<const uint4*>(buf + (k * NK + j) * 1024);
-#pragma unroll
-              for (int i = R::NQ - 1; i >= 0; --i) y = mfma16h(q[t].x[j * R::NQ + i], c, y);
-            }
-            return y;
-          };
-          if (first >= (int)hi || first + KEYS <= (int)lo) {  // the wave's rows see nothing of it
-            sums[lane] = 0.0f;
-          } else if (one && state == 0 && first >= (int)all_lo && first + KEYS <= (int)all_hi) {
-            // every row sees every position
-#pragma unroll
-            for (int k = 0; k < TK; ++k) {
-              const float f = fs[k * 16 + col];
-              float sum = 0.0f;
-#pragma unroll
-              for (int t = 0; t < RT; ++t) {
-                const kh_f32x4 y = scores(k, t);
-                const float fr = wt_scale(f, r[t]);
-                float w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(y[i], fr, nl[t][i]));
-                sum += (w[0] + w[1]) + (w[2] + w[3]);
-              }
-              sum = across_groups_sum(sum);
-              if (g == 0) sums[k * 16 + col] = sum;
-            }
-          } else {
-            for (int k = 0; k < TK; ++k) {
-              const float f = fs[k * 16 + col];
-              int from, to;
-              wt_span(a, s, first + k * 16 + col, from, to);
-              float sum = 0.0f;
-#pragma unroll
-              for (int t = 0; t < RT; ++t) {
-                const kh_f32x4 y = scores(k, t);
-                float w[4], rt[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) rt[i] = __shfl(q[t].r, 4 * g + i);
-                wt_weights(y, f, rt, nl[t], w);
-                wt_hide(w0 + 16 * t, g, from, to, nl[t], w);
-                sum += (w[0] + w[1]) + (w[2] + w[3]);
-              }
-              sum = across_groups_sum(sum);
-              if (g == 0) sums[k * 16 + col] = s_state[st & 1][k] == 2 ? 0.0f : sum;
-            }
-          }
-        }
+        for (int k = 0; k < NW; ++k) w += x[k * KEYS];
+        const int j = st * KEYS + tid;
+        if (j < s.E && w != 0.0f) out[j] = old + w;
+      };
+      for (int st = sb; st < se; ++st) {
         __syncthreads();
         if (tid < KEYS) {
-          const float* x = s_sum + ((se - 1) & 1) * NW * KEYS + tid;
-          float w = 0.0f;
-#pragma unroll
-          for (int k = 0; k < NW; ++k) w += x[k * KEYS];
-          const int j = (se - 1) * KEYS + tid;
-          if (j >= p0 && j < p1 && w != 0.0f) out[j] += w;
+          if (st > sb) add(st - 1);
+          old = out[min(st * KEYS + tid, s.E - 1)];
         }
+        const int first = st * KEYS;
+        const char* buf = s_buf + (st & 1) * S::kStep + lane * 16;
+        const float* fs = s_f + (st & 1) * KEYS;
+        float* sums = s_sum + ((st & 1) * NW + wave) * KEYS;
+        int state = 0;
+#pragma unroll
+        for (int k = 0; k < TK; ++k) state |= s_state[st & 1][k];
+        state = __builtin_amdgcn_readfirstlane(state);
+        if (st + 2 < se) {
+          if (((st + 2 - sb) & 63) == 0) find(st + 2);
+          load(st + 2, next);
+        }
+        // The next step goes to the other buffer (after the last one, what nobody reads).
+        const auto scores = [&](int k, kh_f32x4 (&y)[RT]) {
+#pragma unroll
+          for (int t = 0; t < RT; ++t) y[t] = kh_f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            const uint4 c = *reinterpret_cast<const uint4*>(buf + (k * NK + NG + i) * 1024);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) y[t] = mfma16h(q[t].x[NG * R::NQ + i], c, y[t]);
+          }
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            const uint4 c = *reinterpret_cast<const uint4*>(buf + (k * NK + j) * 1024);
+#pragma unroll
+            for (int i = R::NQ - 1; i >= 0; --i)
+#pragma unroll
+              for (int t = 0; t < RT; ++t) y[t] = mfma16h(q[t].x[j * R::NQ + i], c, y[t]);
+          }
+        };
+        if (first >= (int)hi || first + KEYS <= (int)lo) {  // the wave's rows see nothing of it
+          unpack(st + 1, now);
+#pragma unroll
+          for (int i = lane; i < KEYS; i += 64) sums[i] = 0.0f;
+        } else if (one && state == 0 && first >= (int)all_lo && first + KEYS <= (int)all_hi) {
+          // Every row sees every position.  A tile's products lie between the rest of the work of the tile before
+          // (the first one's between the unpacking), and an operand of the next tile is asked for as soon as this
+          // tile's is used: the compiler would ask for it just before it is needed, and wait.
+          const auto at = [](int o) { return o < NB ? NG + o : o - NB; };
+          const auto operand = [&](int k, int o) { return *reinterpret_cast<const uint4*>(buf + (k * NK + at(o)) * 1024); };
+          uint4 c[NK];
+#pragma unroll
+          for (int o = 0; o < NK; ++o) c[o] = operand(0, o);
+          kh_f32x4 y[2][RT];
+          float f[2], sum = 0.0f;
+          const auto finish = [&](int k, int t) {
+            const float fr = wt_scale(f[k & 1], r[t]);
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(y[k & 1][t][i], fr, nl[t][i]));
+            sum = t == 0 ? (w[0] + w[1]) + (w[2] + w[3]) : sum + ((w[0] + w[1]) + (w[2] + w[3]));
+          };
+          __builtin_amdgcn_sched_barrier(0);
+          unpack(st + 1, now);
+#pragma unroll
+          for (int k = 0; k < TK; ++k) {
+            f[k & 1] = fs[k * 16 + col];
+#pragma unroll
+            for (int o = 0; o < NK; ++o) {
+              constexpr int NQ = R::NQ;
+#pragma unroll
+              for (int i = o < NB ? 0 : NQ - 1; i >= 0; --i)
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                  y[k & 1][t] = mfma16h(q[t].x[o < NB ? NG * NQ + o : at(o) * NQ + i], c[o], o == 0 ? kh_f32x4{0, 0, 0, 0} : y[k & 1][t]);
+              if (k + 1 < TK) c[o] = operand(k + 1, o);
+              if (k > 0) {
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                  if (t * NK / RT == o) finish(k - 1, t);
+                if (o == NK - 1) sums[(k - 1) * 16 + col] = across_groups_sum(sum);
+              }
+#pragma unroll
+              for (int i = 0; i < RT * (o < NB ? 1 : NQ); ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                if (k == 0) __builtin_amdgcn_sched_group_barrier(0x402, 7, 0);
+                else __builtin_amdgcn_sched_group_barrier(0x402, 4, 0);
+              }
+              if (k > 0 || o == NK - 1) __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < RT; ++t) finish(TK - 1, t);
+          sums[(TK - 1) * 16 + col] = across_groups_sum(sum);
+        } else {
+          unpack(st + 1, now);
+          for (int k = 0; k < TK; ++k) {
+            const int j0 = first + k * 16;
+            float sum = 0.0f;
+            if (j0 < (int)hi && j0 + 16 > (int)lo && s_state[st & 1][k] < 2) {
+              const float f = fs[k * 16 + col];
+              const bool whole = j0 >= (int)all_lo && j0 + 16 <= (int)all_hi && s_state[st & 1][k] == 0;
+              int from = 0, to = 0;
+              if (!whole) wt_span(a, s, j0 + col, from, to);
+              kh_f32x4 y[RT];
+              scores(k, y);
+#pragma unroll
+              for (int t = 0; t < RT; ++t) {
+                float w[4], rt[4] = {r[t], r[t], r[t], r[t]};
+                if (!one) {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) rt[i] = __shfl(q[t].r, 4 * g + i);
+                }
+                wt_weights(y[t], f, rt, nl[t], w);
+                if (!whole) wt_hide(w0 + 16 * t, g, from, to, nl[t], w);
+                sum += (w[0] + w[1]) + (w[2] + w[3]);
+              }
+              sum = across_groups_sum(sum);
+            }
+            sums[k * 16 + col] = sum;
+          }
+        }
+        now = next;
       }
+      __syncthreads();
+      if (tid < KEYS) add(se - 1);
     }
   }
 }
 
-// Adds the chunks' sums to acc, in their order.
-__global__ __launch_bounds__(64) void paged_weights_join_kernel(WtArgs a) {
-  const int64_t apart = (int64_t)a.parts * a.part;
+// Adds the shares' sums to acc: four neighbours of each four, in their order.
+__global__ __launch_bounds__(256) void paged_weights_join_kernel(WtArgs a) {
+  __shared__ float part[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, each = (a.shares + 3) / 4;
   for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
     WtSeq s;
-    if (!wt_seq(a, b, false, s)) continue;
-    const int64_t row = b * a.nkv + blockIdx.y, j = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (j >= min((int64_t)s.E, apart)) continue;
-    const float* sums = a.sums + row * a.chunks * apart + j;
+    if (!wt_seq(a, b, false, s) || s.E > a.reach) continue;
+    const int64_t row = b * a.nkv + blockIdx.y, j = (int64_t)blockIdx.x * 64 + lane;
+    const float* sums = a.sums + row * a.shares * a.reach + j;
+    const int2* range = a.range + row * a.shares;
     float w = 0.0f;
+    for (int c0 = wave * each; c0 < min((wave + 1) * each, a.shares); c0 += 64) {
+      const int n = min(min((wave + 1) * each, a.shares) - c0, 64);
+      const int2 p = range[c0 + min(lane, n - 1)];
 #pragma unroll 8
-    for (int c = 0; c < a.chunks; ++c) w += sums[c * apart];
-    if (w != 0.0f) a.acc[row * a.acc_cols + j] += w;
+      for (int c = 0; c < n; ++c) {
+        const int x = __builtin_amdgcn_readlane(p.x, c), y = __builtin_amdgcn_readlane(p.y, c);
+        const float v = sums[(c0 + c) * a.reach];
+        w += j >= x && j < y ? v : 0.0f;
+      }
+    }
+    part[wave][lane] = w;
+    __syncthreads();
+    w = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+    if (wave == 0 && j < s.E && w != 0.0f) a.acc[row * a.acc_cols + j] += w;
+    __syncthreads();
   }
 }
 
 // How a call is cut.
 struct WtPlan {
   bool many;
-  int chunks, parts, part;
+  int shares;
+  int64_t reach;
 };
 static int wt_block_rows(int d, int dtype) {
   if (dtype == KH_DT_F32) return d == 64 ? WtShape<64, float>::RB : d == 128 ? WtShape<128, float>::RB : WtShape<256, float>::RB;
   return d == 64 ? WtShape<64, uint16_t>::RB : d == 128 ? WtShape<128, uint16_t>::RB : WtShape<256, uint16_t>::RB;
 }
-constexpr int64_t kWtFill = 256;          // blocks of many rows that the chip holds at once
-constexpr int64_t kWtMost = 1 << 26;      // sums of chunks
-constexpr int kWtMostChunks = 64, kWtPart = 512;
+static int wt_step(int d) { return d == 64 ? WtShape<64, float>::KEYS : d == 128 ? WtShape<128, float>::KEYS : WtShape<256, float>::KEYS; }
+constexpr int64_t kWtFill = 256;      // blocks of many rows that the chip holds at once
+constexpr int64_t kWtMost = 1 << 26;  // sums of shares
 static WtPlan wt_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int64_t batch, int64_t max_rows, int64_t max_len) {
   WtPlan p;
-  const int64_t gs = nh / c->nkv, rb = wt_block_rows(c->d, dtype);
+  const int64_t gs = nh / c->nkv, rb = wt_block_rows(c->d, dtype), keys = wt_step(c->d);
   max_rows = std::min(max_rows, rows);
-  max_len = std::max<int64_t>(std::min<int64_t>(max_len, INT32_MAX), 1);
+  max_len = std::max<int64_t>(std::min<int64_t>(max_len, INT32_MAX - 64), 1);
   p.many = max_rows * gs > 16;
-  // parts of the positions, and chunks of the rows where those alone do not fill the chip four times over
-  const int64_t heads = batch * c->nkv;
-  p.part = kWtPart;
-  int64_t parts = (max_len + kWtPart - 1) / kWtPart;
-  const int64_t most = std::max<int64_t>(((int64_t)1 << 20) / c->nkv, 1);
-  if (parts > most) parts = most;  // a grid's: the others are taken by turns
-  int64_t chunks = std::min<int64_t>((max_rows * gs + rb - 1) / rb, kWtMostChunks);
-  if (heads > 8 * kWtFill) chunks = 1;
-  else chunks = std::min(std::min(chunks, 8 * kWtFill / (heads * std::min(parts, 8 * kWtFill)) + 1), kWtMost / (heads * parts * kWtPart));
-  p.parts = (int)parts;
-  p.chunks = (int)std::max<int64_t>(chunks, 1);
+  p.reach = (max_len + 63) / 64 * 64;
+  // the number of shares that lets the rounds of blocks on the chip end first
+  const int64_t heads = batch * c->nkv, steps = (max_rows * gs + rb - 1) / rb * ((max_len + keys - 1) / keys);
+  int64_t least = INT64_MAX;
+  p.shares = 1;
+  for (int64_t n = 1; n <= kWtFill && n <= steps && (n == 1 || n * heads <= std::min(4 * kWtFill, kWtMost / p.reach)); ++n) {
+    const int64_t time = (heads * n + kWtFill - 1) / kWtFill * ((steps + n - 1) / n + 2 * kWtNew);
+    if (time < least) least = time, p.shares = (int)n;
+  }
   return p;
 }
 static int64_t wt_space(const WtPlan& p, int64_t heads) {
-  return p.many && p.chunks > 1 ? heads * p.chunks * p.parts * (int64_t)p.part * 4 : 0;
+  return p.many && p.shares > 1 ? heads * p.shares * (p.reach * 4 + 8) : 0;
 }
 
 template <int D, typename T>
@@ -637,12 +763,10 @@ static int wt_launch(const WtArgs& a, bool many, int64_t max_len, hipStream_t st
     const dim3 g((unsigned)std::max<int64_t>(std::min<int64_t>((most + BP - 1) / BP, 65535), 1), (unsigned)a.nkv, seqs);
     hipLaunchKernelGGL((paged_weights_kernel<D, T, NPT>), g, dim3(64 * kWtWaves), 0, st, a);
   } else {
-    const int64_t blocks = (int64_t)a.parts * a.chunks * a.nkv;
-    hipLaunchKernelGGL((paged_weights_tiles_kernel<D, T>), dim3((unsigned)blocks, seqs), dim3((64 * WtShape<D, T>::NW)),
-                       (WtShape<D, T>::kLds), st, a);
-    if (a.chunks > 1)
-      hipLaunchKernelGGL(paged_weights_join_kernel, dim3((unsigned)((int64_t)a.parts * a.part / 64), (unsigned)a.nkv, seqs), dim3(64),
-                         0, st, a);
+    hipLaunchKernelGGL((paged_weights_tiles_kernel<D, T>), dim3((unsigned)((int64_t)a.shares * a.nkv), seqs),
+                       dim3((64 * WtShape<D, T>::NW)), (WtShape<D, T>::kLds), st, a);
+    if (a.shares > 1)
+      hipLaunchKernelGGL(paged_weights_join_kernel, dim3((unsigned)(a.reach / 64), (unsigned)a.nkv, seqs), dim3(256), 0, st, a);
   }
   KH_LAUNCHED();
   return KH_OK;
@@ -702,7 +826,7 @@ extern "C" int kh_paged_kv_weights(const kh_paged_kv* c, int dtype, const void* 
   if (rc != KH_OK) return rc;
   KH_CHECK_ARG(table_cols >= 1 && table_stride >= table_cols, "page table of %lld columns, %lld apart",
                (long long)table_cols, (long long)table_stride);
-  KH_CHECK_ARG(table_cols <= (INT32_MAX - 64) >> c->ps_log2, "a page table of %lld columns holds 2^31 positions",
+  KH_CHECK_ARG(table_cols <= (INT32_MAX - 256) >> c->ps_log2, "a page table of %lld columns holds 2^31 positions",
                (long long)table_cols);
   KH_CHECK_ARG(std::isfinite(scale * kLog2e) && scale > 0, "scale must be positive and finite");
   KH_CHECK_ARG(window >= 0 && (window == 0 || causal), "a window (%lld) needs causal attention", (long long)window);
@@ -745,9 +869,9 @@ extern "C" int kh_paged_kv_weights(const kh_paged_kv* c, int dtype, const void* 
   a.acc_cols = acc_cols;
   a.qvec = aligned16(q_dev, dtype, q_row_stride, q_head_stride) ? 1 : 0;
   a.sums = static_cast<float*>(ws_dev);
-  a.chunks = p.chunks;
-  a.parts = p.parts;
-  a.part = p.part;
+  a.range = reinterpret_cast<int2*>(a.sums + batch * c->nkv * p.shares * p.reach);
+  a.shares = p.shares;
+  a.reach = p.reach;
   return dtype == KH_DT_F32 ? wt_launch_d<float>(c->d, a, p.many, max_len, as_stream(stream))
                             : wt_launch_d<uint16_t>(c->d, a, p.many, max_len, as_stream(stream));
 }
