@@ -24,6 +24,7 @@ namespace kh {
 
 constexpr int kWtWaves = 4;
 constexpr float kWtNone = 0x1p100f;  // a log-sum-exp whose rows add nothing
+constexpr float kWtLarge = 0x1p60f;    // scales up to it have finite products
 constexpr int kWtNew = 3;               // steps whose time a share's next block of rows costs
 constexpr int kWtNear = 7;           // powers of two between the largest and the smallest row of a tile with one scale
 
@@ -196,10 +197,9 @@ __device__ __forceinline__ void wt_unpack(const uint32_t (&w)[N], const uint32_t
     b[1] = make_uint4(sh[0], sh[1], sh[2], sh[3]);
   }
   // three terms: the lanes' last group has none
-  if (g == 3) {
+  const uint32_t some = g == 3 ? 0 : 0xffffffffu;
 #pragma unroll
-    for (int k = 0; k < NB; ++k) b[k] = make_uint4(0, 0, 0, 0);
-  }
+  for (int k = 0; k < NB; ++k) b[k] = make_uint4(b[k].x & some, b[k].y & some, b[k].z & some, b[k].w & some);
 }
 template <int D>
 struct WtKeys {
@@ -396,7 +396,7 @@ __global__ __launch_bounds__((64 * WtShape<D, T>::NW), 2) void paged_weights_til
   extern __shared__ __align__(16) char s_buf[];
   float* s_f = reinterpret_cast<float*>(s_buf + 2 * S::kStep);  // [2][KEYS]
   float* s_sum = s_f + 2 * KEYS;                                // [2][NW][KEYS]
-  __shared__ int s_state[2][TK];  // of a step's tiles: 0, 1 where a key holds a NaN, 2 where there is no page
+  __shared__ int s_state[2][TK];  // of a step's tiles: 1 where a key holds a NaN or has a large scale, 2 and 3 where there is no page
   const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15, tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ps = 1 << a.ps_log2, utile = wave / S::PARTS, ugroup = wave % S::PARTS * NGW;
@@ -533,22 +533,23 @@ __global__ __launch_bounds__((64 * WtShape<D, T>::NW), 2) void paged_weights_til
         uint32_t nan = 0;
 #pragma unroll
         for (int i = 0; i < NG; ++i) nan = max(nan, k.p[i]);
-        s_state[st & 1][utile] = k.pg < 0 ? 2 : __ballot(nan >= 0x7f800000u) ? 1 : 0;
+        const uint64_t rare = __ballot(nan >= 0x7f800000u || f > kWtLarge);
+        s_state[st & 1][utile] = (k.pg >> 31 & 2) | ((uint32_t)rare | (uint32_t)(rare >> 32) ? 1 : 0);
       };
       find(sb);
       load(sb, now);
 
       R q[RT];
+      float nl[RT][4], r[RT];
       bool one = true;
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         q[t].load(a, s.o0, s.nr, h, w0 / 16 + t, lane);
-        one = one && q[t].one;
+        r[t] = __shfl(q[t].r, 0);
+        one = one && q[t].one && r[t] <= kWtLarge;
       }
-      float nl[RT][4], r[RT];
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        r[t] = __shfl(q[t].r, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) nl[t][i] = __shfl(q[t].nl, 4 * g + i);
       }
@@ -617,7 +618,7 @@ __global__ __launch_bounds__((64 * WtShape<D, T>::NW), 2) void paged_weights_til
           kh_f32x4 y[2][RT];
           float f[2], sum = 0.0f;
           const auto finish = [&](int k, int t) {
-            const float fr = wt_scale(f[k & 1], r[t]);
+            const float fr = f[k & 1] * r[t];  // finite: see `one` and the tiles' states
             float w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(y[k & 1][t][i], fr, nl[t][i]));
