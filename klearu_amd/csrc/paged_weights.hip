@@ -95,7 +95,9 @@ struct WtRows {
   uint4 x[NF];      // the groups' terms, slots (0,4,1,5,2,6,3,7) of eight elements as codes_f16 gives codes; sums
   float r, nl;      // of row lane % 16: its scale, and minus its log-sum-exp in powers of two
   bool one;         // all rows have the first one's scale
-  __device__ __forceinline__ void load(const WtArgs& a, int64_t o0, int nr, int h, int tile, int lane) {
+  // `between` runs while the rows' loads are on their way.
+  template <typename F>
+  __device__ __forceinline__ void load(const WtArgs& a, int64_t o0, int nr, int h, int tile, int lane, F between) {
     const int g = lane >> 4, rr = tile * 16 + (lane & 15);
     const bool inside = rr < nr;
     const int i = (int)((uint32_t)(inside ? rr : 0) / (uint32_t)a.gs);
@@ -106,6 +108,7 @@ struct WtRows {
 #pragma unroll
     for (int j = 0; j < NG; ++j) raw[j].load(q + 32 * j + 8 * g, a.qvec);
     const float lse = a.lse[t * a.nh + head];
+    between();
     const bool on = inside && !__builtin_isinf(lse);
     nl = on ? -lse * kLog2e : -kWtNone;
     uint32_t top = 0;  // of the row's finite elements, as an f32's bits
@@ -201,29 +204,6 @@ __device__ __forceinline__ void wt_unpack(const uint32_t (&w)[N], const uint32_t
 #pragma unroll
   for (int k = 0; k < NB; ++k) b[k] = make_uint4(b[k].x & some, b[k].y & some, b[k].z & some, b[k].w & some);
 }
-template <int D>
-struct WtKeys {
-  static constexpr int NG = D / kKvGroup, NB = NG == 8 ? 2 : 1;
-  uint4 c[NG], b[NB];
-  float f;
-  __device__ __forceinline__ void put(const uint32_t (&w)[NG], const uint32_t (&p)[NG], float c1, int g) {
-    wt_unpack<D, NG>(w, p, 0, c1, g, c, b, f);
-  }
-};
-
-// q . k of a tile of rows and one of positions, both scaled.
-template <int D, typename T>
-__device__ __forceinline__ kh_f32x4 wt_scores(const uint4 (&x)[WtRows<D, T>::NF], const WtKeys<D>& k) {
-  using R = WtRows<D, T>;
-  kh_f32x4 y = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < R::NB; ++i) y = mfma16h(x[R::NG * R::NQ + i], k.b[i], y);
-#pragma unroll
-  for (int j = 0; j < R::NG; ++j)
-#pragma unroll
-    for (int i = R::NQ - 1; i >= 0; --i) y = mfma16h(x[j * R::NQ + i], k.c[j], y);
-  return y;
-}
 // The two scales together: products of powers of two, so that it does not matter which rows share one.
 __device__ __forceinline__ float wt_scale(float f, float r) { return fminf(f * r, 0x1.fffffep127f); }
 // The weights of four rows for the lane's position.
@@ -238,8 +218,8 @@ struct WtSeq {
   int64_t o0, before;  // its first row; that row's position
   int n, nr, E;        // rows, times heads; positions that are added up
 };
-__device__ __forceinline__ bool wt_seq(const WtArgs& a, int64_t b, bool tell, WtSeq& s) {
-  int64_t o0 = a.off[b], o1 = a.off[b + 1], L = a.len[b];
+// Of rows o0 .. o1 - 1 and L cached positions, as off and len have them.
+__device__ __forceinline__ bool wt_seq(const WtArgs& a, int64_t b, int64_t o0, int64_t o1, int64_t L, bool tell, WtSeq& s) {
   const int64_t cap = a.cols << a.ps_log2;
   o0 = o0 < 0 ? 0 : o0;
   o1 = o1 > a.rows ? a.rows : o1;
@@ -256,6 +236,13 @@ __device__ __forceinline__ bool wt_seq(const WtArgs& a, int64_t b, bool tell, Wt
   s.E = (int)min(L, a.acc_cols);
   return true;
 }
+__device__ __forceinline__ bool wt_seq(const WtArgs& a, int64_t b, bool tell, WtSeq& s) {
+  return wt_seq(a, b, a.off[b], a.off[b + 1], a.len[b], tell, s);
+}
+// The first position that some row of a sequence sees; the last one is E - 1.
+__device__ __forceinline__ int wt_first(const WtArgs& a, const WtSeq& s) {
+  return a.window > 0 ? (int)min(max(s.before - a.window + 1, (int64_t)0), (int64_t)s.E) : 0;
+}
 // The rows (times heads) that see position j: [lo, hi).
 __device__ __forceinline__ void wt_span(const WtArgs& a, const WtSeq& s, int j, int& lo, int& hi) {
   const int64_t x = a.causal ? max(j - s.before, (int64_t)0) : 0;
@@ -265,54 +252,6 @@ __device__ __forceinline__ void wt_span(const WtArgs& a, const WtSeq& s, int j, 
   hi = some ? (int)(y * a.gs) : 0;
 }
 
-// NPT tiles of 16 positions from `base` on: their keys, who sees them, and the ranges of that.
-template <int D, int NPT>
-struct WtCols {
-  WtKeys<D> x[NPT];
-  int lo[NPT], hi[NPT];
-  int all_lo, all_hi, some_lo, some_hi;  // all_lo > all_hi where a key holds a NaN: see wt_hide
-  __device__ __forceinline__ void load(const WtArgs& a, const WtSeq& s, int h, int base, int lane) {
-    using P = KvParts<D>;
-    constexpr int NG = P::NG;
-    const int g = lane >> 4, col = lane & 15, ps = 1 << a.ps_log2;
-    uint32_t al = 0, ah = 0x7fffffffu, sl = 0x7fffffffu, sh = 0;
-    uint32_t w[NPT][NG], p[NPT][NG];
-#pragma unroll
-    for (int t = 0; t < NPT; ++t) {
-      const int tok = base + 16 * t, j = tok + col;
-      wt_span(a, s, j, lo[t], hi[t]);
-      if (j >= s.E) lo[t] = hi[t] = 0;
-#pragma unroll
-      for (int k = 0; k < NG; ++k) w[t][k] = p[t][k] = 0;
-      if (__ballot(hi[t] > lo[t])) {  // tables need not name pages that no row sees
-        const int pg = __builtin_amdgcn_readfirstlane(s.table[tok >> a.ps_log2]);
-        if (pg >= 0 && pg < a.pages) {
-          const char* blk = a.pool + ((int64_t)pg * a.nkv + h) * a.block;
-          const int at = (tok & (ps - 1)) + col;
-          ld_words<NG>(blk + P::kc() + at * (D / 2) + g * NG * 4, w[t]);
-          ld_words<NG>(blk + P::kp(ps) + at * NG * 4, p[t]);
-        } else {
-          if (lane == 0) atomicOr(a.err, 2);
-          lo[t] = hi[t] = 0;
-        }
-      }
-      if (hi[t] > lo[t]) sl = min(sl, (uint32_t)lo[t]), sh = max(sh, (uint32_t)hi[t]);
-      if (j < s.E) al = max(al, (uint32_t)lo[t]), ah = min(ah, (uint32_t)hi[t]);  // other columns' sums go nowhere
-    }
-#pragma unroll
-    for (int t = 0; t < NPT; ++t) x[t].put(w[t], p[t], a.c1, g);
-    all_lo = (int)wave_max_u32(al);
-    all_hi = (int)wave_min_u32(ah);
-    some_lo = (int)wave_min_u32(sl);
-    some_hi = (int)wave_max_u32(sh);
-    uint32_t nan = 0;
-#pragma unroll
-    for (int t = 0; t < NPT; ++t)
-#pragma unroll
-      for (int k = 0; k < NG; ++k) nan = max(nan, p[t][k]);
-    if (__ballot(nan >= 0x7f800000u)) all_lo = 0x7fffffff;
-  }
-};
 // Leaves the weights of rows that see the lane's position, and that add anything: 0 times a NaN is one.
 __device__ __forceinline__ void wt_hide(int r0, int g, int lo, int hi, const float (&nl)[4], float (&w)[4]) {
 #pragma unroll
@@ -323,42 +262,126 @@ __device__ __forceinline__ void wt_hide(int r0, int g, int lo, int hi, const flo
 }
 
 // ---------------------------------------------------------------- few rows
-// A wave keeps a tile of rows and takes the positions of its part, NPT tiles at a time.
+// Positions are taken in steps of 16 NPT.  A kv head's steps, of 64 sequences after each other, are cut in shares of
+// the same length for waves, since contexts have every length.  A wave keeps a tile of rows, and the loads of
+// a step are under way while it works on the step before.
 template <int D, typename T, int NPT>
 __global__ __launch_bounds__(64 * kWtWaves) void paged_weights_kernel(WtArgs a) {
-  constexpr int STEP = 16 * NPT;
+  using R = WtRows<D, T>;
+  using P = KvParts<D>;
+  constexpr int NG = R::NG, NB = R::NB, STEP = 16 * NPT;
   const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.y;
-  for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
-    WtSeq s;
-    if (!wt_seq(a, b, threadIdx.x == 0 && blockIdx.x == 0 && h == 0, s)) continue;
-    float* acc = a.acc + (b * a.nkv + h) * a.acc_cols;
-    for (int tile = 0; tile * 16 < s.nr; ++tile) {
-      WtRows<D, T> q;
-      q.load(a, s.o0, s.nr, h, tile, lane);
-      float r[4], nl[4];
+  const int h = blockIdx.y, ps = 1 << a.ps_log2;
+  struct Step {
+    uint32_t w[NPT][NG], p[NPT][NG];
+    int pg[NPT];
+    float old[NPT];
+  };
+  const uint32_t share = blockIdx.x * kWtWaves + wave, shares = gridDim.x * kWtWaves;
+  for (int64_t c = blockIdx.z * (int64_t)64; c < a.batch; c += gridDim.z * (int64_t)64) {
+    // lane i: of sequence c + i the rows, the length and the steps, and of those up to it
+    int64_t o0 = 0, o1 = 0, L = 0;
+    int of = 0;
+    if (c + lane < a.batch) {
+      o0 = a.off[c + lane];
+      o1 = a.off[c + lane + 1];
+      L = a.len[c + lane];
+      WtSeq s;
+      if (wt_seq(a, c + lane, o0, o1, L, share == 0 && h == 0, s)) of = (s.E + STEP - 1) / STEP - wt_first(a, s) / STEP;
+    }
+    const int64_t upto = ((int64_t)wave_incl_scan(of >> 16) << 16) + wave_incl_scan(of & 0xffff);
+    const auto lane_of = [](int64_t v, int i) {
+      return (int64_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, i);
+    };
+    const int64_t total = lane_of(upto, 63);
+    int64_t from = total * share / shares, left = total * (share + 1) / shares - from;
+    if (left == 0) continue;
+    for (int i = __builtin_ctzll(__ballot(upto > from)); left > 0; ++i) {
+      const int n = __builtin_amdgcn_readlane(of, i);
+      if (n == 0) continue;
+      const int64_t before = lane_of(upto, i) - n, b = c + i;
+      WtSeq s;
+      wt_seq(a, b, lane_of(o0, i), lane_of(o1, i), lane_of(L, i), false, s);
+      // positions that some row sees: tables need not name pages of others
+      const int x0 = wt_first(a, s), x1 = s.E;
+      const int skip = (int)(from - before), steps = (int)min((int64_t)(n - skip), left);
+      const int first = (x0 / STEP + skip) * STEP;
+      left -= steps;
+      from = before + n;
+      float* acc = a.acc + (b * a.nkv + h) * a.acc_cols;
+      for (int tile = 0; tile * 16 < s.nr; ++tile) {
+        // lane i holds the page of the i-th of 64 tiles of positions
+        int pages = 0;
+        const auto find = [&](int i) {
+          const int64_t tok = first + (int64_t)(i * NPT + lane) * 16;
+          pages = tok < x1 && tok + 16 > x0 ? s.table[max(tok, (int64_t)x0) >> a.ps_log2] : 0;
+          if (tok < x1 && tok + 16 > x0 && (pages < 0 || pages >= a.pages)) {
+            atomicOr(a.err, 2);
+            pages = -1;
+          }
+        };
+        const auto fetch = [&](int i, Step& k) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        r[i] = __shfl(q.r, 4 * g + i);
-        nl[i] = __shfl(q.nl, 4 * g + i);
-      }
-      const int r0 = tile * 16, r1 = min(r0 + 16, s.nr);
-      for (int base = (blockIdx.x * kWtWaves + wave) * STEP; base < s.E; base += gridDim.x * kWtWaves * STEP) {
-        WtCols<D, NPT> k;
-        float old[NPT];
+          for (int t = 0; t < NPT; ++t) {
+            const int tok = first + i * STEP + 16 * t;
+            k.pg[t] = __builtin_amdgcn_readlane(pages, i * NPT + t & 63);
+            const char* blk = a.pool + ((int64_t)max(k.pg[t], 0) * a.nkv + h) * a.block;
+            const int at = (tok & (ps - 1)) + col;
+            ld_words<NG>(blk + P::kc() + at * (D / 2) + g * NG * 4, k.w[t]);
+            ld_words<NG>(blk + P::kp(ps) + at * NG * 4, k.p[t]);
+            k.old[t] = acc[min(tok + col, s.E - 1)];
+          }
+        };
+        R q;
+        Step now, next;
+        find(0);
+        q.load(a, s.o0, s.nr, h, tile, lane, [&] { fetch(0, now); });
+        float r[4], nl[4];
 #pragma unroll
-        for (int t = 0; t < NPT; ++t) old[t] = acc[min(base + 16 * t + col, s.E - 1)];
-        k.load(a, s, h, base, lane);
-        const bool whole = r0 >= k.all_lo && r1 <= k.all_hi;
+        for (int i = 0; i < 4; ++i) {
+          r[i] = __shfl(q.r, 4 * g + i);
+          nl[i] = __shfl(q.nl, 4 * g + i);
+        }
+        // positions that all of the tile's rows see
+        const int r0 = tile * 16, r1 = min(r0 + 16, s.nr);
+        const int64_t t0 = s.before + (uint32_t)r0 / (uint32_t)a.gs, t1 = s.before + (uint32_t)(r1 - 1) / (uint32_t)a.gs;
+        const int64_t all0 = a.window > 0 ? max(t1 - a.window + 1, (int64_t)0) : 0, all1 = a.causal ? t0 + 1 : s.E;
+        for (int i = 0; i < steps; ++i) {
+          if (i + 1 < steps) {
+            if (((i + 1) * NPT & 63) == 0) find(i + 1);
+            fetch(i + 1, next);
+          }
+          const int base = first + i * STEP;
+          uint32_t nan = 0;
 #pragma unroll
-        for (int t = 0; t < NPT; ++t) {
-          float w[4];
-          wt_weights(wt_scores<D, T>(q.x, k.x[t]), k.x[t].f, r, nl, w);
-          if (!whole) wt_hide(r0, g, k.lo[t], k.hi[t], nl, w);
-          const float sum = across_groups_sum((w[0] + w[1]) + (w[2] + w[3]));
-          const int j = base + 16 * t + col;
-          if (g == 0 && j < s.E && sum != 0.0f) acc[j] = old[t] + sum;
+          for (int t = 0; t < NPT; ++t)
+#pragma unroll
+            for (int k = 0; k < NG; ++k) nan = max(nan, now.p[t][k]);
+          const bool whole = base >= all0 && min(base + STEP, s.E) <= all1 && __ballot(nan >= 0x7f800000u) == 0;
+#pragma unroll
+          for (int t = 0; t < NPT; ++t) {
+            uint4 c[NG], sums[NB];
+            float f, w[4];
+            wt_unpack<D, NG>(now.w[t], now.p[t], 0, a.c1, g, c, sums, f);
+            kh_f32x4 y = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < NB; ++k) y = mfma16h(q.x[NG * R::NQ + k], sums[k], y);
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+              for (int k = R::NQ - 1; k >= 0; --k) y = mfma16h(q.x[j * R::NQ + k], c[j], y);
+            wt_weights(y, f, r, nl, w);
+            const int j = base + 16 * t + col;
+            if (!whole) {
+              int lo, hi;
+              wt_span(a, s, j, lo, hi);
+              wt_hide(r0, g, lo, hi, nl, w);
+            }
+            const float sum = across_groups_sum((w[0] + w[1]) + (w[2] + w[3]));
+            if (g == 0 && j < s.E && now.pg[t] >= 0 && sum != 0.0f) acc[j] = now.old[t] + sum;
+          }
+          now = next;
         }
       }
     }
@@ -544,7 +567,7 @@ __global__ __launch_bounds__((64 * WtShape<D, T>::NW), 2) void paged_weights_til
       bool one = true;
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        q[t].load(a, s.o0, s.nr, h, w0 / 16 + t, lane);
+        q[t].load(a, s.o0, s.nr, h, w0 / 16 + t, lane, [] {});
         r[t] = __shfl(q[t].r, 0);
         one = one && q[t].one && r[t] <= kWtLarge;
       }
@@ -733,6 +756,7 @@ static int wt_block_rows(int d, int dtype) {
 }
 static int wt_step(int d) { return d == 64 ? WtShape<64, float>::KEYS : d == 128 ? WtShape<128, float>::KEYS : WtShape<256, float>::KEYS; }
 constexpr int64_t kWtFill = 256;      // blocks of many rows that the chip holds at once
+constexpr int64_t kWtFew = 1024;      // blocks of few rows
 constexpr int64_t kWtMost = 1 << 26;  // sums of shares
 static WtPlan wt_plan(const kh_paged_kv* c, int dtype, int nh, int64_t rows, int64_t batch, int64_t max_rows, int64_t max_len) {
   WtPlan p;
@@ -761,7 +785,10 @@ static int wt_launch(const WtArgs& a, bool many, int64_t max_len, hipStream_t st
   if (!many) {
     constexpr int NPT = 2, BP = 16 * NPT * kWtWaves;
     const int64_t most = std::min(std::min(max_len, a.acc_cols), a.cols << a.ps_log2);
-    const dim3 g((unsigned)std::max<int64_t>(std::min<int64_t>((most + BP - 1) / BP, 65535), 1), (unsigned)a.nkv, seqs);
+    // as many waves as the chip holds at once, if there are steps for them
+    const int64_t groups = std::min<int64_t>((a.batch + 63) / 64, 65535);
+    const int64_t blocks = std::min((most + BP - 1) / BP * std::min<int64_t>(a.batch, 64), std::max<int64_t>(kWtFew / (a.nkv * groups), 1));
+    const dim3 g((unsigned)std::max<int64_t>(blocks, 1), (unsigned)a.nkv, (unsigned)groups);
     hipLaunchKernelGGL((paged_weights_kernel<D, T, NPT>), g, dim3(64 * kWtWaves), 0, st, a);
   } else {
     hipLaunchKernelGGL((paged_weights_tiles_kernel<D, T>), dim3((unsigned)((int64_t)a.shares * a.nkv), seqs),
