@@ -8,16 +8,19 @@
 // decide: they are f64, of f32 exponentials with the rounding of their arguments put back (log2 e
 // in two parts), since sums that are 1e-7 off swap continuations of a batch of beams now and then.
 //
-// The k largest: the k-th largest of the lanes' own maxima, T, has k logits at or above it, so only
-// those can be among the k largest (16 a lane at most), and of later logits only those above T.  They go to a list in LDS, which is
-// cut to k when it fills and at the end: its k-th largest is found bit by bit, counted with ballots.
+// The k largest: of W waves that share a row, the smallest of their own (k / W)-th largest logits, T, has k logits at
+// or above it, so that no others can be among the k largest.  Waves tell each other theirs: of the first tile's
+// lanes' maxima before any list begins, later whenever a wave's list has doubled.  A wave's own k-th largest of its
+// lanes' maxima bounds what one tile can add (16 a lane) where the others' logits are smaller.  What passes goes to a list in
+// LDS, which is cut to k when it fills and at the end: the k-th largest is found bit by bit, counted with
+// ballots.  When a wave sees what another tells changes its list, not the k largest of all.
 #include <algorithm>
 
 #include "paged_kv.hpp"
 
 namespace kh {
 
-constexpr int kBmThreads = 256, kBmWaves = kBmThreads / 64;
+constexpr int kBmThreads = 512, kBmWaves = kBmThreads / 64;
 constexpr int kBmEach = 16;             // logits of a lane
 constexpr int kBmTile = 64 * kBmEach;   // of a wave
 constexpr int64_t kBmFill = 4096;       // waves that the chip holds at once (512 rows of 131071: 6144 90 us, 2048 104 instead of 76)
@@ -26,6 +29,7 @@ struct BeamArgs {
   const void* x;
   int64_t row_stride, batch, vocab;
   int beams, k, parts, tiles;  // parts of a row, tiles of a part
+  int slots;                   // waves of a row: parts, rounded up so that whole rows or whole blocks go together
   const float* scores;
   const uint8_t* done;
   int64_t end;
@@ -118,21 +122,39 @@ template <typename T, int KC>
 __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
   constexpr int V = 16 / sizeof(T), Q = kBmEach / V, LAST = sizeof(T) == 2 ? 16 : 0;
   extern __shared__ __align__(16) uint64_t s_lists[];  // [waves][32 KC]
+  __shared__ uint32_t s_told[2][kBmWaves];             // of a row and of the next one
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint64_t* list = s_lists + wave * (32 * KC);
-  const int64_t waves = a.batch * a.beams * a.parts;
-  for (int64_t id = (int64_t)blockIdx.x * kBmWaves + wave; id < waves; id += (int64_t)gridDim.x * kBmWaves) {
-    const int64_t r = id / a.parts;
-    const int part = (int)(id - r * a.parts);
+  const int64_t waves = a.batch * a.beams * a.slots;
+  int turn = 0;
+  for (int64_t block = (int64_t)blockIdx.x * kBmWaves; block < waves; block += (int64_t)gridDim.x * kBmWaves, turn ^= 1) {
+    const int64_t slot = block + wave, r = min(slot, waves - 1) / a.slots;
+    const int part = slot < waves ? (int)(slot - r * a.slots) : a.parts;
+    const int64_t id = r * a.parts + part;
+    // the waves of the block that share the row, and how many of their largest all of them together need
+    const int group = min(a.slots, kBmWaves), leader = wave & ~(group - 1), shared = min(group, a.parts - (part & ~(group - 1)));
+    const int few = shared > 0 ? (a.k + shared - 1) / shared : a.k;
+    uint32_t* told = s_told[turn];
     const T* row = static_cast<const T*>(a.x) + r * a.row_stride;
     // positions are counted from the 16-byte border before the row
     const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     const int end = shift + (int)a.vocab;
-    const int first = part * a.tiles * kBmTile, last = min(first + a.tiles * kBmTile, end);
+    const int first = part * a.tiles * kBmTile, last = part < a.parts ? min(first + a.tiles * kBmTile, end) : 0;
     float ref = -INFINITY;  // what exponentials of the lane's logits are taken from
     double sum = 0.0;
-    int n = 0;
+    int n = 0, next_n = 2 * few;
     uint32_t tk = 0, tv = 0;  // T, and its token (inverted): entries below it are of no use
+    const auto tell = [&](uint32_t v) { __hip_atomic_store(&told[wave], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); };
+    const auto hear = [&] {
+      const uint32_t v = __hip_atomic_load(&told[leader + min(lane, max(shared, 1) - 1)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      uint32_t all = wave_min_u32(v);
+      if (LAST == 16 && all != 0 && all >> 31 == 0) all |= 0xffffu;  // the whole key of a negative BF16
+      if (all > tk) tk = all, tv = 0;  // equal ones may come before those that were counted
+    };
+    if (first >= last) {
+      if (lane == 0) tell(0);
+      __syncthreads();
+    }
     uint4 next[Q];
     const auto inside = [&](int p) { return p >= shift && p + kBmTile <= end; };
     const auto fetch = [&](int p) {
@@ -187,7 +209,16 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
 
       // the lane's largest (of the row's own: those past its ends are -inf, too, but no entries)
       const uint32_t mk = f32_key(m);
-      bool mine = n == 0 || mk > tk;
+      const auto passes = [&] { return mk >= tk + (tv == ~0u ? 1 : 0); };
+      if (p == first) {
+        const uint32_t v = kth_largest(few, LAST, [&](uint32_t v) { return ballots(mk >= v); });
+        if (lane == 0) tell(v);
+        __syncthreads();
+        hear();
+      } else if (__ballot(passes())) {
+        hear();
+      }
+      bool mine = passes();
       const uint64_t better = __ballot(mine);
       if (!better) continue;
       const auto there = [&](int e) {
@@ -203,7 +234,7 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
           if (there(e) && key > bk) bk = key, bv = token(e);
         }
         const uint32_t kth = kth_largest(a.k, LAST, [&](uint32_t v) { return ballots(bk >= v); }) >> LAST;
-        if (kth != 0 && (n == 0 || kth > tk >> LAST)) {
+        if (kth != 0 && kth >= tk >> LAST) {
           // of the lanes whose maximum is T the first ones, by their tokens
           const int above = ballots(bk >> LAST > kth);
           const uint64_t same = __ballot(bk >> LAST == kth);
@@ -232,8 +263,16 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
         n = a.k;
         tv = ~0u;  // the next ones have to be above it
       }
+      if (n >= next_n && n <= 64) {
+        next_n = 2 * n;
+        __builtin_amdgcn_wave_barrier();
+        const uint32_t key = lane < n ? (uint32_t)(list[lane] >> 32) : 0;
+        const uint32_t v = kth_largest(few, LAST, [&](uint32_t v) { return ballots(key >= v); });
+        if (lane == 0) tell(v);
+      }
     }
     if (n > a.k) beam_cut<KC>(list, n, a.k, LAST, lane), n = a.k;
+    if (part >= a.parts) continue;
     uint64_t* top = a.top + id * a.k;
     if (lane < a.k) top[lane] = lane < n ? list[lane] : 0;
     const float all = wave_max(ref);
@@ -405,7 +444,7 @@ static int beam_shape(int64_t batch, int beams, int64_t vocab, int k) {
 }
 // Parts of a row (tiles of a part), wherever it starts between two 16-byte borders: as many waves as the chip holds.
 struct BeamPlan {
-  int parts, tiles;
+  int parts, tiles, slots;
 };
 static BeamPlan beam_plan(int64_t rows, int64_t vocab) {
   const int64_t all = (vocab + 7 + kBmTile - 1) / kBmTile;
@@ -413,6 +452,9 @@ static BeamPlan beam_plan(int64_t rows, int64_t vocab) {
   BeamPlan p;
   p.tiles = (int)((all + want - 1) / want);
   p.parts = (int)((all + p.tiles - 1) / p.tiles);
+  p.slots = 1;
+  while (p.slots < p.parts && p.slots < kBmWaves) p.slots *= 2;
+  if (p.parts > kBmWaves) p.slots = (p.parts + kBmWaves - 1) / kBmWaves * kBmWaves;
   return p;
 }
 static int64_t beam_space(int64_t batch, int beams, int64_t vocab, int k) {
@@ -420,7 +462,7 @@ static int64_t beam_space(int64_t batch, int beams, int64_t vocab, int k) {
 }
 template <typename T, int KC>
 static void beam_launch_k(const BeamArgs& a, hipStream_t st) {
-  const int64_t blocks = (a.batch * a.beams * a.parts + kBmWaves - 1) / kBmWaves;
+  const int64_t blocks = (a.batch * a.beams * a.slots + kBmWaves - 1) / kBmWaves;
   hipLaunchKernelGGL((beam_part_kernel<T, KC>), dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(kBmThreads),
                      kBmWaves * 32 * KC * 8, st, a);
 }
@@ -471,6 +513,7 @@ extern "C" int kh_beam_select(int dtype, const void* logits_dev, int64_t row_str
   const BeamPlan p = beam_plan(rows, vocab);
   a.parts = p.parts;
   a.tiles = p.tiles;
+  a.slots = p.slots;
   a.scores = scores_dev;
   a.done = done_dev;
   a.end = end;
