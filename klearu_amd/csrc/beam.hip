@@ -5,8 +5,8 @@
 // One pass over the logits: a wave takes a part of a row and leaves the sum of exp(x - m) and its
 // k largest logits; a second kernel joins a sequence's parts.  Within a beam y orders as x does, so
 // parts compare logits as integers, of equal ones the first.  Between beams the log-sum-exps
-// decide: they are f64, of f32 exponentials with the rounding of their arguments put back (log2 e
-// in two parts), since sums that are 1e-7 off swap continuations of a batch of beams now and then.
+// decide: they are f64, of f32 exponentials with what log2 e and the rounded maximum lack put back, since
+// sums that are 1e-7 off swap continuations of a batch of beams now and then.
 //
 // The k largest: of W waves that share a row, the smallest of their own (k / W)-th largest logits, T, has k logits at
 // or above it, so that no others can be among the k largest.  Waves tell each other theirs: of the first tile's
@@ -46,10 +46,14 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
   return v;
 }
 
-// exp(t), t <= 88, within 1e-7 and without a bias: log2 e is 0x1.715476p+0f and 1.9e-8 more.  Not for -inf.
+// log2 e is 0x1.715476p+0f and 1.9e-8 more.  Sums of z = exp2(y), y = x log2 e - c rounded once, have the rest of log2 e and
+// of c put back: the sum of z y times ln 2 (rest / log2 e).
+constexpr float kBmHi = 0x1.715476p+0f;
+constexpr double kBmLo = 0x1.62e42fefa39efp-1 * (0x1.4ae0bf85ddf44p-26 / 0x1.715476p+0);
+// exp(t), t <= 88, within 1e-7 and without a bias, for logits of any size.  Not for -inf.
 __device__ __forceinline__ float beam_exp(float t) {
-  const float hi = 0x1.715476p+0f, lo = 0x1.4ae0cp-26f;
-  const float y = t * hi, r = fmaf(t, lo, fmaf(t, hi, -y));
+  const float lo = 0x1.4ae0cp-26f;
+  const float y = t * kBmHi, r = fmaf(t, lo, fmaf(t, kBmHi, -y));
   const float e = __builtin_amdgcn_exp2f(y);
   return fmaf(e, r * 0x1.62e43p-1f, e);
 }
@@ -140,7 +144,10 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
     const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     const int end = shift + (int)a.vocab;
     const int first = part * a.tiles * kBmTile, last = part < a.parts ? min(first + a.tiles * kBmTile, end) : 0;
-    float ref = -INFINITY;  // what exponentials of the lane's logits are taken from
+    // What the wave's exponentials are taken from, near its largest logit, so that those that count have small exponents and
+    // small rounding errors of them; times log2 e; what its rounding makes of the sums.
+    float ref = -INFINITY, c = -INFINITY;
+    double scale = 1.0;
     double sum = 0.0;
     int n = 0, next_n = 2 * few;
     uint32_t tk = 0, tv = 0;  // T, and its token (inverted): entries below it are of no use
@@ -191,21 +198,33 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
       float m = x[0];
 #pragma unroll
       for (int e = 1; e < kBmEach; ++e) m = fmaxf(m, x[e]);
-      if (m > ref + 60.0f) {  // sums of 2^24 exp(60) fit in f32
-        sum = sum == 0.0 ? 0.0 : sum * exp((double)ref - (double)m);
-        ref = m;
+      if (__ballot(m > ref + 2.0f)) {
+        const float most = wave_max(fmaxf(m, ref));
+        sum = sum == 0.0 ? 0.0 : sum * exp((double)ref - (double)most);
+        ref = most;
+        c = ref * kBmHi;
+        const double d = (double)fmaf(ref, kBmHi, -c) * 0x1.62e42fefa39efp-1;
+        scale = 1.0 - d + 0.5 * d * d;
       }
-      float s = 0.0f;
+      float s = 0.0f, sy = 0.0f;
 #pragma unroll
-      for (int e = 0; e < kBmEach; ++e) s += beam_exp(x[e] - ref);
-      if (__ballot(s != s)) {  // -inf or the type's lowest value among them, or what makes the sum NaN
+      for (int e = 0; e < kBmEach; ++e) {
+        const float y = fmaf(x[e], kBmHi, -c), z = __builtin_amdgcn_exp2f(y);
+        s += z;
+        sy = fmaf(z, y, sy);
+      }
+      const float both = s + sy;
+      if (__ballot(both != both || !(__builtin_fabsf(ref) <= 4096.0f))) {
+        // -inf or the type's lowest value among them, or what makes the sum NaN, or large ones
         float none = -150.0f;
         asm volatile("" : "+v"(none));  // keeps this behind its branch
         s = 0.0f;
 #pragma unroll
         for (int e = 0; e < kBmEach; ++e) s += x[e] == -INFINITY || x[e] - ref < none ? 0.0f : beam_exp(x[e] - ref);
+        sum += (double)s;
+      } else {
+        sum += (double)s * scale + (double)sy * kBmLo;
       }
-      sum += (double)s;
 
       // the lane's largest (of the row's own: those past its ends are -inf, too, but no entries)
       const uint32_t mk = f32_key(m);
@@ -275,10 +294,9 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
     if (part >= a.parts) continue;
     uint64_t* top = a.top + id * a.k;
     if (lane < a.k) top[lane] = lane < n ? list[lane] : 0;
-    const float all = wave_max(ref);
-    const double total = wave_sum_f64(sum == 0.0 ? 0.0 : sum * exp((double)ref - (double)all));
+    const double total = wave_sum_f64(sum);
     if (lane == 0) {
-      a.max[id] = all;
+      a.max[id] = ref;
       a.sum[id] = total;
     }
   }
