@@ -76,11 +76,13 @@ __device__ __forceinline__ uint32_t kth_largest(int k, int last, F count) {
 }
 __device__ __forceinline__ int ballots(bool p) { return __popcll(__ballot(p)); }
 
+template <int KC>
+constexpr int kBmList = (18 * KC + 63) / 64 * 64;  // less than 2 k before a tile, and what it adds
 // Cuts a wave's list of n > k different entries to its k largest, in any order; returns the upper word of
 // the smallest of them.
 template <int KC>
 __device__ __forceinline__ uint32_t beam_cut(uint64_t* list, int n, int k, int last, int lane) {
-  constexpr int C = KC / 2;  // entries of a lane
+  constexpr int C = kBmList<KC> / 64;  // entries of a lane
   __builtin_amdgcn_wave_barrier();  // the wave's writes are in order before its reads
   uint64_t x[C];
 #pragma unroll
@@ -130,10 +132,10 @@ __device__ __forceinline__ uint32_t beam_cut(uint64_t* list, int n, int k, int l
 template <typename T, int KC>
 __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
   constexpr int V = 16 / sizeof(T), Q = kBmEach / V, LAST = sizeof(T) == 2 ? 16 : 0;
-  extern __shared__ __align__(16) uint64_t s_lists[];  // [waves][32 KC]
+  extern __shared__ __align__(16) uint64_t s_lists[];  // [waves][kBmList]
   __shared__ uint32_t s_told[2][kBmWaves];             // of a row and of the next one
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint64_t* list = s_lists + wave * (32 * KC);
+  uint64_t* list = s_lists + wave * kBmList<KC>;
   const int64_t waves = a.batch * a.beams * a.slots;
   int turn = 0;
   for (int64_t block = (int64_t)blockIdx.x * kBmWaves; block < waves; block += (int64_t)gridDim.x * kBmWaves, turn ^= 1) {
@@ -235,7 +237,7 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
       const uint32_t mk = f32_key(m);
       const auto passes = [&] { return mk >= tk + (tv == ~0u ? 1 : 0); };
       if (p == first) {
-        const uint32_t v = kth_largest(few, LAST, [&](uint32_t v) { return ballots(mk >= v); });
+        const uint32_t v = few == 1 ? wave_max_u32(mk) : kth_largest(few, LAST, [&](uint32_t v) { return ballots(mk >= v); });
         if (lane == 0) tell(v);
         __syncthreads();
         hear();
@@ -487,7 +489,7 @@ template <typename T, int KC>
 static void beam_launch_k(const BeamArgs& a, hipStream_t st) {
   const int64_t blocks = (a.batch * a.beams * a.slots + kBmWaves - 1) / kBmWaves;
   hipLaunchKernelGGL((beam_part_kernel<T, KC>), dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(kBmThreads),
-                     kBmWaves * 32 * KC * 8, st, a);
+                     kBmWaves * kBmList<KC> * 8, st, a);
 }
 template <typename T>
 static void beam_launch(const BeamArgs& a, hipStream_t st) {

@@ -701,6 +701,11 @@ static EvictSpace evict_space(const kh_paged_kv* c, int64_t batch, int64_t keep,
   s.chain = keep >= acc_cols || heads >= 128 || keep <= 4096;
   s.parts = (acc_cols + kEvPart - 1) / kEvPart;
   s.images = (most + c->ps - 1) >> c->ps_log2;
+  if (heads > ((int64_t)1 << 46) / acc_cols) {  // more than a GPU's weights: no workspace is large enough
+    s.weights = s.hist = s.state = 0;
+    s.bytes = s.whole ? 0 : INT64_MAX;
+    return s;
+  }
   s.weights = s.chain ? 0 : heads * s.images * c->block;
   s.hist = s.weights + (s.whole ? 0 : (heads * most * 4 + 15) / 16 * 16);
   s.state = s.hist + (s.whole ? 0 : 2 * heads * s.parts * kEvBins * 2);  // two digits' at a time

@@ -732,7 +732,7 @@ __global__ __launch_bounds__(256) void paged_weights_join_kernel(WtArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, each = (a.shares + 3) / 4;
   for (int64_t b = blockIdx.z; b < a.batch; b += gridDim.z) {
     WtSeq s;
-    if (!wt_seq(a, b, false, s) || s.E > a.reach) continue;
+    if (!wt_seq(a, b, false, s) || s.E > a.reach || (int64_t)blockIdx.x * 64 >= s.E) continue;
     const int64_t row = b * a.nkv + blockIdx.y, j = (int64_t)blockIdx.x * 64 + lane;
     const float* sums = a.sums + row * a.shares * a.reach + j;
     const int2* range = a.range + row * a.shares;

@@ -76,6 +76,16 @@ def test_select(kh, dtype, batch, beams, vocab, k, ends):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch,beams,vocab,k", [(1100, 4, 1500, 5), (260, 4, 5000, 9), (30, 7, 20000, 33)])
+def test_many_rows(kh, dtype, batch, beams, vocab, k):
+    """Rows that one wave takes, or some of a block, or all."""
+    rng = np.random.default_rng(batch)
+    x, s = logits(rng, batch, beams, vocab)
+    xs, got = run(x, s, k, dtype=dtype)
+    check(got, xs, s, k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_first_step_and_all_ended(kh, dtype):
     rng = np.random.default_rng(0)
     x, s = logits(rng, 3, 4, 5000)

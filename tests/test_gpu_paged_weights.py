@@ -181,6 +181,36 @@ def test_sizes_of_rows_and_keys(kh, dtype, rows, lo, hi):
     c.check(c.run(lse=lse), lse=lse)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [[3], [150]])
+@pytest.mark.parametrize("power", [-80, 80, 90])
+def test_large_scales(kh, dtype, rows, power):
+    """Keys of 2^power and queries of 2^-power: ordinary scores of numbers whose scales are far from one."""
+    rng = np.random.default_rng(power + 100)
+    c = Call(4, 2, 128, rows, [300], 32, dtype, k=[(keys(rng, 300, 2, 128) * 2.0 ** power).astype(np.float32)])
+    c.q = (c.q.double() * 2.0 ** -power).to(dtype)
+    lse = np.zeros_like(c.lse)
+    for h in range(4):
+        x = np.where(seen(rows[0], 300, True, 0), c.q[:, h].double().numpy() @ values(c.k[0])[:, h // 2].T * c.scale, -np.inf)
+        lse[:, h] = x.max(-1) + 1
+    c.check(c.run(lse=lse), lse=lse)
+
+
+@pytest.mark.parametrize("window", [0, 20])
+def test_many_sequences(kh, window):
+    """More sequences than a wave has lanes, of every length, some without rows or positions."""
+    rng = np.random.default_rng(window)
+    lens = rng.integers(0, 90, 197).tolist()
+    rows = [int(r) if n else 0 for r, n in zip(rng.integers(0, 3, 197), lens)]
+    lens[70], rows[70] = 700, 1
+    c = Call(4, 2, 64, rows, lens, 16, torch.bfloat16, True, window)
+    want = c.run()
+    c.check(want)
+    c.check(c.run(max_rows=64))
+    assert torch.equal(c.run(max_len=100000), want)
+    c.cache.status()
+
+
 @pytest.mark.parametrize("rows,lens", [([1, 1], [130, 77]), ([200, 60], [300, 400])])
 def test_guesses_padding_strides(kh, rows, lens):
     """Wrong guesses, rows of no sequence, queries inside a wider row, unaligned ones: the same bits where the cut is the
