@@ -361,10 +361,9 @@ __device__ __forceinline__ void evict_ways(const EvictArgs& a, const int32_t* __
 // (a block and a place) and go to to(i) (a block, nullptr for none) at place at(i).  A thread's pieces
 // are loaded together, without branches, and written behind `between`.
 template <int D, int NT, int CHUNK, typename F, typename G, typename A, typename B>
-__device__ __forceinline__ void evict_keys(int ps, int count, F from, G to, A at, B between) {
+__device__ __forceinline__ void move_keys(int t, int ps, int count, F from, G to, A at, B between) {
   using P = KvParts<D>;
   constexpr int NG = P::NG, KC = D / 32, H = CHUNK * KC / NT, HP = CHUNK / NT;
-  const int t = threadIdx.x;
   uint32_t c[H][4], p[HP][NG];
 #pragma unroll
   for (int r = 0; r < H; ++r) {
@@ -396,10 +395,10 @@ __device__ __forceinline__ void evict_keys(int ps, int count, F from, G to, A at
 // Values: words [quad][row of sixteen][position / 2][h] of two positions' codes each.  Of the last quad's
 // positions those past `count` are the caller's, too.
 template <int D, int NT, int CHUNK, typename F, typename G, typename A, typename B>
-__device__ __forceinline__ void evict_values(int ps, int count, F from, G to, A at, B between) {
+__device__ __forceinline__ void move_values(int t, int ps, int count, F from, G to, A at, B between) {
   using P = KvParts<D>;
   constexpr int NG = P::NG, HN = D / 64, Q = CHUNK * 4 / NT, HP = CHUNK / NT;
-  const int t = threadIdx.x, quads = (count + 3) >> 2;
+  const int quads = (count + 3) >> 2;
   uint32_t v[Q][2 * HN], p[HP][NG];
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
@@ -483,8 +482,8 @@ __global__ __launch_bounds__(kEvThreads) void evict_move_kernel(EvictArgs a) {
       const auto to = [&](int i) -> char* { return s_to[i] < 0 ? nullptr : pool + s_to[i] * apart; };
       const auto at = [&](int i) { return (c0 + i) & (ps - 1); };
       const auto between = [] { __syncthreads(); };
-      if (blockIdx.z == 0) evict_keys<D, kEvThreads, CHUNK>(ps, count, from, to, at, between);
-      else evict_values<D, kEvThreads, CHUNK>(ps, count, from, to, at, between);
+      if (blockIdx.z == 0) move_keys<D, kEvThreads, CHUNK>(t, ps, count, from, to, at, between);
+      else move_values<D, kEvThreads, CHUNK>(t, ps, count, from, to, at, between);
       lds_barrier();  // the tables are read; what is written need not have arrived
     }
   }
@@ -526,8 +525,8 @@ __global__ __launch_bounds__(kEvCopy) void evict_copy_kernel(EvictArgs a) {
       return image(i);
     };
     const auto copy = [&](auto from, auto to) {
-      if (blockIdx.z == 0) evict_keys<D, kEvCopy, kEvCopy>(ps, count, from, to, at, [] {});
-      else evict_values<D, kEvCopy, kEvCopy>(ps, count, from, to, at, [] {});
+      if (blockIdx.z == 0) move_keys<D, kEvCopy, kEvCopy>(t, ps, count, from, to, at, [] {});
+      else move_values<D, kEvCopy, kEvCopy>(t, ps, count, from, to, at, [] {});
     };
     if constexpr (BACK) copy(held, page);
     else copy(moved, image);
@@ -570,38 +569,6 @@ static int evict_launch(const EvictArgs& a, bool whole, bool chain, hipStream_t 
 }
 
 // ---------------------------------------------------------------- beams
-// The first n positions of a block of a page, to another one; what lies
-// behind them there stays.
-template <int D>
-__device__ __forceinline__ void copy_positions(char* __restrict__ to, const char* __restrict__ from, int n, int ps, int t, int nt) {
-  using P = KvParts<D>;
-  constexpr int NG = P::NG;
-  const auto words = [&](int off, int count) {
-    uint32_t* y = reinterpret_cast<uint32_t*>(to + off);
-    const uint32_t* x = reinterpret_cast<const uint32_t*>(from + off);
-    for (int i = t; i < count; i += nt) y[i] = x[i];
-  };
-  const auto pieces = [&](int off, int count) {
-    uint4* y = reinterpret_cast<uint4*>(to + off);
-    const uint4* x = reinterpret_cast<const uint4*>(from + off);
-    for (int i = t; i < count; i += nt) y[i] = x[i];
-  };
-  pieces(P::kc(), n * (D / 32));
-  pieces(P::vc(ps), (n >> 2) * (D / 8));
-  words(P::kp(ps), n * NG);
-#pragma unroll
-  for (int j = 0; j < NG; ++j) words(P::vp(ps) + j * ps * 4, n);
-  if (n & 3) {  // of the last four positions' codes: words [r][position / 2][h], a position in each half
-    uint32_t* y = reinterpret_cast<uint32_t*>(to + P::vc(ps) + (n >> 2) * (2 * D));
-    const uint32_t* x = reinterpret_cast<const uint32_t*>(from + P::vc(ps) + (n >> 2) * (2 * D));
-    for (int i = t; i < D / 2; i += nt) {
-      const int second = i / (D / 64) & 1, there = (n & 3) - 2 * second;
-      if (there <= 0) continue;
-      y[i] = there >= 2 ? x[i] : (y[i] & 0xffff0000u) | (x[i] & 0xffffu);
-    }
-  }
-}
-
 struct ReorderArgs {
   char* pool;
   int64_t block, pages;
@@ -615,7 +582,7 @@ struct ReorderArgs {
   int beams;
 };
 
-// Block: a share of one beam: of its columns, and of the kv heads whose rows it copies.  Every wave
+// Block: a share of one beam: of its columns, and, a wave each, of the kv heads' keys and values that it copies.  Every wave
 // works the beams' pages out for itself, a beam a lane: the beams that go on from an
 // earlier beam's parent (again), and those that nobody goes on from (gone), the i-th of either meeting.
 template <int D>
@@ -664,9 +631,22 @@ __global__ __launch_bounds__(256) void reorder_kernel(ReorderArgs a) {
       if (share == 0 && threadIdx.x == 0) atomicOr(a.err, 2);
       continue;
     }
-    for (int h = share; h < a.nkv; h += shares)
-      copy_positions<D>(a.pool + ((int64_t)dst * a.nkv + h) * a.block, a.pool + ((int64_t)src * a.nkv + h) * a.block, n,
-                        1 << a.ps_log2, threadIdx.x, 256);
+    // 64 positions at a time; in the last four those past n keep what the place has
+    const int wave = threadIdx.x >> 6, ps = 1 << a.ps_log2;
+    for (int task = share * 4 + wave; task < 2 * a.nkv; task += shares * 4) {
+      const char* x = a.pool + ((int64_t)src * a.nkv + (task >> 1)) * a.block;
+      char* y = a.pool + ((int64_t)dst * a.nkv + (task >> 1)) * a.block;
+      for (int c0 = 0; c0 < n; c0 += 64) {
+        const auto source = [&](int i, int& place) -> const char* {
+          place = c0 + i;
+          return place < n ? x : y;
+        };
+        const auto to = [&](int i) { return y; };
+        const auto at = [&](int i) { return c0 + i; };
+        if (task & 1) move_values<D, 64, 64>(lane, ps, min(n - c0, 64), source, to, at, [] {});
+        else move_keys<D, 64, 64>(lane, ps, min(n - c0, 64), source, to, at, [] {});
+      }
+    }
   }
 }
 
@@ -811,7 +791,7 @@ extern "C" int kh_paged_kv_reorder(kh_paged_kv* c, const int32_t* table_dev, int
   a.parent = parent_dev;
   a.beams = beams;
   const int64_t rows = batch * beams;
-  const dim3 g((unsigned)std::min<int64_t>(rows, 1 << 20), (unsigned)std::min(c->nkv, 16));
+  const dim3 g((unsigned)std::min<int64_t>(rows, 1 << 20), (unsigned)std::min((c->nkv + 1) / 2, 16));
   const hipStream_t st = as_stream(stream);
   if (c->d == 64) hipLaunchKernelGGL(reorder_kernel<64>, g, dim3(256), 0, st, a);
   else if (c->d == 128) hipLaunchKernelGGL(reorder_kernel<128>, g, dim3(256), 0, st, a);
