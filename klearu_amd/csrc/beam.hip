@@ -15,9 +15,9 @@
 // LDS, which is cut to k when it fills and at the end: the k-th largest is found bit by bit, counted with
 // ballots.  When a wave sees what another tells changes its list, not the k largest of all.
 //
-// Both kernels, 512 rows of 131071 BF16 logits, k 16: 58 us (54 and 5), 2.3 TB/s of logits.  What bounds the first one are
-// instructions (210 for 1024 logits, of which 112 are the sums') and the chains of ballots in between: the same reading alone
-// takes 28 us.  One pass is all that a row needs; waves take its tiles side by side (59 us with a range each).
+// Both kernels, 512 rows of 131071 BF16 logits, k 16: 55 us (50 and 5), 2.4 TB/s of logits.  What bounds the first one are
+// instructions (210 for 1024 logits, of which 64 are the sums') and the chains of ballots in between: a copy reads as much
+// in 28 us.  One pass is all that a row needs; waves take its tiles side by side (59 us with a range each).
 #include <algorithm>
 
 #include "paged_kv.hpp"

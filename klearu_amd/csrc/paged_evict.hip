@@ -66,7 +66,9 @@ __device__ __forceinline__ void evict_none(const EvictArgs& a, int64_t row, int6
   for (int64_t j = j0 + t; j < min(j1, L); j += nt) out[j] = a.acc[row * a.acc_cols + j];
 }
 
-// Block: one kv head of one sequence, whose weights fit in its registers.
+// Block: one kv head of one sequence, whose weights fit in its registers: one launch, and weights are read once.  A chain of
+// length, weights, histogram, candidates and places with twelve barriers bounds it, not the bytes: 12.7 us for 32 kv heads
+// of 2111 positions, 15 for 256 of up to 4099.
 __global__ __launch_bounds__(kEvThreads) void evict_whole_kernel(EvictArgs a) {
   __shared__ TopkLds<kEvThreads> sh;
   __shared__ uint16_t s_kept[kEvThreads * kEvMost];
@@ -136,7 +138,8 @@ __global__ __launch_bounds__(kEvThreads) void evict_whole_kernel(EvictArgs a) {
 //
 // T has three digits, of 11, 11 and 10 bits.  A launch for each makes histograms of it, one of each
 // part's weights that have T's digits before, and its blocks all find the digit before that themselves, from
-// the histograms of all parts: the launches in between would take longer.
+// the histograms of all parts: the launches in between would take longer.  131072 positions of eight kv heads: 4.9, 6.6 and
+// 8.2 us, and 10.2 of selecting (4 MB are read four times, from the caches).
 constexpr int kEvShift[3] = {21, 10, 0};
 
 struct EvictFind {
@@ -446,7 +449,9 @@ __device__ __forceinline__ void move_values(int t, int ps, int count, F from, G 
   }
 }
 
-// Block: the keys (blockIdx.z 0) or the values of a kv head, chunk after chunk.
+// Block: the keys (blockIdx.z 0) or the values of a kv head, chunk after chunk.  A chunk is a chain of kept positions, pages and
+// rows, so it is as long as the registers allow; 256 kv heads that keep 1024 of 64: 17.2 us, a block for each kind of
+// 16-byte pieces, which each look their rows up, 25.9.
 template <int D>
 __global__ __launch_bounds__(kEvThreads) void evict_move_kernel(EvictArgs a) {
   constexpr int CHUNK = (D == 256 ? 1 : 2) * kEvThreads;
@@ -582,7 +587,8 @@ struct ReorderArgs {
   int beams;
 };
 
-// Block: a share of one beam: of its columns, and, a wave each, of the kv heads' keys and values that it copies.  Every wave
+// Block: a share of one beam: of its columns, and, a wave each, of the kv heads' keys and values that it copies.  64 x 8 beams of eight kv
+// heads of 128 with half a page of 64 each: 10.4 us (a row of pieces after the other: 15.5), a chain of parents, tables and rows.  Every wave
 // works the beams' pages out for itself, a beam a lane: the beams that go on from an
 // earlier beam's parent (again), and those that nobody goes on from (gone), the i-th of either meeting.
 template <int D>

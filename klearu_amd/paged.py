@@ -173,10 +173,6 @@ class Rope(_Handle):
         self._adopt(h)
         self.rot_dim, self.max_pos, self.layout, self.axes = rot_dim, max_pos, layout, len(sections)
 
-    def _pos(self, n):
-        """The shape of n rows' positions."""
-        return (n,) if self.axes == 1 else (self.axes, n)
-
     def apply(self, x: torch.Tensor, pos: torch.Tensor, out: torch.Tensor | None = None, transpose: bool = False,
               stream=None) -> torch.Tensor:
         """x [rows, heads, head_dim] rotated by pos [rows] (int64; with sections [axes, rows]), into
@@ -186,7 +182,7 @@ class Rope(_Handle):
         dev = self._dev
         xp, x0, x1, dt = _rows(x, "x", dev)
         n, heads, dim = x.shape
-        pp = _index(pos, "pos", dev, _I64, self._pos(n))
+        pp = _index(pos, "pos", dev, _I64, (n,) if self.axes == 1 else (self.axes, n))
         if stream is not None or _raw_device() != dev:
             with _On(self.device, stream, (x, pos, out)):
                 return self.apply(x, pos, out, transpose)
@@ -244,7 +240,7 @@ class PagedKv(_Handle):
         batch, op, sp, tp, cols, ts = self._places(off, start, table)
         if pos is not None and rope is None:
             raise ValueError("pos: rotary positions without a rotation")
-        pp = None if pos is None else _index(pos, "pos", dev, _I64, rope._pos(n))
+        pp = None if pos is None else _index(pos, "pos", dev, _I64, (n,) if rope.axes == 1 else (rope.axes, n))
         if stream is not None or _raw_device() != dev:
             with _On(self.device, stream, (k, v, off, start, table, pos)):
                 return self.append(k, v, off, start, table, rope, pos)
