@@ -289,7 +289,7 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
         n = a.k;
         tv = ~0u;  // the next ones have to be above it
       }
-      if (n >= next_n && n <= 64) {
+      if (n >= next_n && n <= 64 && p + step < last) {
         next_n = 2 * n;
         __builtin_amdgcn_wave_barrier();
         const uint32_t key = lane < n ? (uint32_t)(list[lane] >> 32) : 0;

@@ -40,7 +40,7 @@ struct EvictArgs {
   float* acc_out;
   int64_t* len_out;
   // long sequences: the kept weights, histograms of parts, and what was found of T
-  float* weights;
+  float* weights;  // nullptr: they go to their place at once
   char* images;  // of pages of kept positions
   int num_images;
   uint16_t* hist[3];  // of each digit, [batch][kv heads][parts][bins]
@@ -250,7 +250,9 @@ __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictArgs a) {
     const EvictPart p(a, b, h, part, part == 0 && h == 0 && t == 0);
     const int64_t L = p.L, row = p.row, j0 = (int64_t)part * kEvPart;
     if (part == 0 && h == 0 && t == 0) a.len_out[b] = min(L, a.keep);
-    float* weights = a.weights + row * a.wcols;
+    float* weights = a.weights ? a.weights + row * a.wcols : a.acc_out + row * a.acc_cols;
+    if (!a.weights)
+      for (int64_t j = max(j0, min(L, a.keep)) + t; j < min(j0 + kEvPart, a.acc_cols); j += kEvThreads) weights[j] = 0.0f;
     if (L <= a.keep) {
       evict_none(a, row, L, j0, part + 1 == a.parts ? max(a.acc_cols, a.keep) : j0 + kEvPart, t, kEvThreads, weights);
       continue;
@@ -538,7 +540,7 @@ __global__ __launch_bounds__(kEvCopy) void evict_copy_kernel(EvictArgs a) {
   }
 }
 
-// The kept weights of long sequences, which parts found beside each other's reading, and zeros behind them.
+// The kept weights of long sequences whose places other parts still read, and zeros behind them.
 __global__ __launch_bounds__(256) void evict_weights_kernel(EvictArgs a) {
   const int h = blockIdx.y;
   const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -559,7 +561,8 @@ static int evict_launch(const EvictArgs& a, bool whole, bool chain, hipStream_t 
     hipLaunchKernelGGL(evict_hist_kernel<1>, parts, dim3(kEvThreads), 0, st, a);
     hipLaunchKernelGGL(evict_hist_kernel<2>, parts, dim3(kEvThreads), 0, st, a);
     hipLaunchKernelGGL(evict_select_kernel, parts, dim3(kEvThreads), 0, st, a);
-    hipLaunchKernelGGL(evict_weights_kernel, dim3((unsigned)((a.acc_cols + 255) / 256), (unsigned)a.nkv, seqs), dim3(256), 0, st, a);
+    if (a.weights)
+      hipLaunchKernelGGL(evict_weights_kernel, dim3((unsigned)((a.acc_cols + 255) / 256), (unsigned)a.nkv, seqs), dim3(256), 0, st, a);
   }
   if (a.keep >= a.acc_cols) return KH_OK;
   if (chain) {
@@ -757,7 +760,8 @@ extern "C" int kh_paged_kv_evict(kh_paged_kv* c, const float* acc_dev, int64_t a
   char* ws = static_cast<char*>(ws_dev);
   a.images = ws;
   a.num_images = (int)sp.images;
-  a.weights = reinterpret_cast<float*>(ws + sp.weights);
+  const int64_t all = batch * c->nkv * acc_cols;
+  a.weights = acc_out_dev < acc_dev + all && acc_dev < acc_out_dev + all ? reinterpret_cast<float*>(ws + sp.weights) : nullptr;
   a.hist[0] = a.hist[2] = reinterpret_cast<uint16_t*>(ws + sp.hist);
   a.hist[1] = a.hist[0] + batch * c->nkv * sp.parts * kEvBins;
   a.state = reinterpret_cast<int*>(ws + sp.state);

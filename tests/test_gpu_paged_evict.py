@@ -125,6 +125,22 @@ def test_long(kh, kv, dim, page, length, keep, kind):
     c.c.status()
 
 
+@pytest.mark.parametrize("lens,keep", [([40000, 0, 9000], 9000), ([20000, 30], 30000), ([16385], 16384)])
+@pytest.mark.parametrize("kind", ["plain", "ties"])
+def test_long_into_a_new_tensor(kh, lens, keep, kind):
+    """The weights go to their places at once where no part still reads what lies there."""
+    rng = np.random.default_rng(keep)
+    c = Cache(2, 64, lens, 64)
+    acc = weights(rng, len(lens), 2, c.table.shape[1] * 64, kind)
+    before = c.read()
+    given = torch.from_numpy(acc).cuda()
+    out = torch.full_like(given, float("nan"))
+    got = c.c.evict(given, c.len, c.table, keep, recent=500, first=4, out=out)
+    assert got[2] is out and torch.equal(given.cpu(), torch.from_numpy(acc))
+    check_evicted(c, before, acc, got, keep, 500, 4)
+    c.c.status()
+
+
 def test_weights_of_other_widths(kh):
     """Wider than the table, as wide as the length, and narrower than it: the positions past them are evicted and reported."""
     from klearu_amd import KlearuError
