@@ -768,7 +768,9 @@ extern "C" int kh_paged_kv_evict(kh_paged_kv* c, const float* acc_dev, int64_t a
   a.parts = (int)sp.parts;
   a.wcols = std::min(keep, acc_cols);
   const hipStream_t st = as_stream(stream);
-  return c->d == 64 ? evict_launch<64>(a, sp.whole, sp.chain, st) : c->d == 128 ? evict_launch<128>(a, sp.whole, sp.chain, st) : evict_launch<256>(a, sp.whole, sp.chain, st);
+  return c->d == 64    ? evict_launch<64>(a, sp.whole, sp.chain, st)
+         : c->d == 128 ? evict_launch<128>(a, sp.whole, sp.chain, st)
+                       : evict_launch<256>(a, sp.whole, sp.chain, st);
 }
 
 extern "C" int kh_paged_kv_reorder(kh_paged_kv* c, const int32_t* table_dev, int64_t table_cols, int64_t table_stride,

@@ -726,7 +726,7 @@ __global__ __launch_bounds__((64 * WtShape<D, T>::NW), 2) void paged_weights_til
   }
 }
 
-// Adds the shares' sums to acc: four neighbours of each four, in their order.
+// Adds the shares' sums to acc: each wave those of a quarter of the shares, in their order, then the four.
 __global__ __launch_bounds__(256) void paged_weights_join_kernel(WtArgs a) {
   __shared__ float part[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, each = (a.shares + 3) / 4;
@@ -835,7 +835,7 @@ static int wt_shape(const kh_paged_kv* c, int dtype, int64_t rows, int64_t batch
                "rows %lld, batch %lld not in [0,2^31)", (long long)rows, (long long)batch);
   KH_CHECK_ARG(num_heads >= c->nkv && num_heads % c->nkv == 0 && num_heads <= 65536,
                "num_heads %d is no multiple of the cache's %d", num_heads, c->nkv);
-  KH_CHECK_ARG(rows * (num_heads / c->nkv) < ((int64_t)1 << 31) - 64, "%lld rows of %d heads: too many for one call",
+  KH_CHECK_ARG(rows * (num_heads / c->nkv) < ((int64_t)1 << 31) - 1024, "%lld rows of %d heads: too many for one call",
                (long long)rows, num_heads);
   KH_CHECK_ARG(max_rows >= 0 && max_len >= 0, "max_rows %lld, max_len %lld", (long long)max_rows, (long long)max_len);
   return KH_OK;
