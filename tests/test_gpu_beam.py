@@ -86,6 +86,20 @@ def test_many_rows(kh, dtype, batch, beams, vocab, k):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("k", [6, 40])
+def test_runs_are_alike(kh, dtype, k):
+    """What waves of a row hear of each other, and when, does not change the result: many equal logits, run after run."""
+    from klearu_amd import beam
+    rng = np.random.default_rng(k)
+    x, s = logits(rng, 20, 4, 60000)
+    xd, sd = torch.from_numpy(np.floor(4 * x) / 4).to(dtype).cuda(), torch.from_numpy(s).cuda()
+    want = beam.select(xd, sd, k)
+    check(want, xd.float().cpu().numpy(), s, k)
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(beam.select(xd, sd, k), want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_first_step_and_all_ended(kh, dtype):
     rng = np.random.default_rng(0)
     x, s = logits(rng, 3, 4, 5000)
