@@ -6,7 +6,8 @@
 // k largest logits; a second kernel joins a sequence's parts.  Within a beam y orders as x does, so
 // parts compare logits as integers, of equal ones the first.  Between beams the log-sum-exps
 // decide: they are f64, of f32 exponentials with what log2 e and the rounded maximum lack put back, since
-// sums that are 1e-7 off swap continuations of a batch of beams now and then.
+// sums that are 1e-7 off swap continuations of a batch of beams now and then.  The order of a row's sums depends on
+// the call's sizes only, so that beams that are alike tie.
 //
 // The k largest: of W waves that share a row, the smallest of their own (k / W)-th largest logits, T, has k logits at
 // or above it, so that no others can be among the k largest.  Waves tell each other theirs: of the first tile's
@@ -61,6 +62,15 @@ __device__ __forceinline__ float beam_exp(float t) {
   const float y = t * kBmHi, r = fmaf(t, lo, fmaf(t, kBmHi, -y));
   const float e = __builtin_amdgcn_exp2f(y);
   return fmaf(e, r * 0x1.62e43p-1f, e);
+}
+
+// 16 bytes of a row from any element on.  Tiles begin with the row and not at a 16-byte border, so that where a row
+// starts does not change how its exponentials are grouped: beams that are alike have the same sums.
+template <typename T>
+__device__ __forceinline__ uint4 beam_load(const T* p) {
+  uint4 w;
+  __builtin_memcpy(&w, p, sizeof w);
+  return w;
 }
 
 // The largest T of which `count(T)` entries are at or above it: the k-th largest of 32-bit entries; all
@@ -147,9 +157,7 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
     const int few = shared > 0 ? (a.k + shared - 1) / shared : a.k;
     uint32_t* told = s_told[turn];
     const T* row = static_cast<const T*>(a.x) + r * a.row_stride;
-    // positions are counted from the 16-byte border before the row
-    const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-    const int end = shift + (int)a.vocab;
+    const int end = (int)a.vocab;
     const int first = part * kBmTile, last = part < a.parts ? end : 0, step = a.parts * kBmTile;  // waves side by side
     // What the wave's exponentials are taken from, near its largest logit, so that those that count have small exponents and
     // small rounding errors of them; times log2 e; what its rounding makes of the sums.
@@ -170,11 +178,11 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
       __syncthreads();
     }
     uint4 next[Q];
-    const auto inside = [&](int p) { return p >= shift && p + kBmTile <= end; };
+    const auto inside = [&](int p) { return p + kBmTile <= end; };
     const auto fetch = [&](int p) {
       if (inside(p)) {
 #pragma unroll
-        for (int q = 0; q < Q; ++q) next[q] = *reinterpret_cast<const uint4*>(row + (p - shift) + (q * 64 + lane) * V);
+        for (int q = 0; q < Q; ++q) next[q] = beam_load(row + p + (q * 64 + lane) * V);
       }
     };
     if (first < last) fetch(first);
@@ -198,7 +206,7 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
 #pragma unroll
         for (int e = 0; e < kBmEach; ++e) {
           const int at = p + (e / V * 64 + lane) * V + e % V;
-          x[e] = at >= shift && at < end ? load_f32(row + (at - shift)) : -INFINITY;
+          x[e] = at < end ? load_f32(row + at) : -INFINITY;
         }
         if (p + step < last) fetch(p + step);
       }
@@ -233,7 +241,7 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
         sum += (double)s * scale + (double)sy * kBmLo;
       }
 
-      // the lane's largest (of the row's own: those past its ends are -inf, too, but no entries)
+      // the lane's largest (of the row's own: those past its end are -inf, too, but no entries)
       const uint32_t mk = f32_key(m);
       const auto passes = [&] { return mk >= tk + (tv == ~0u ? 1 : 0); };
       if (p == first) {
@@ -249,9 +257,9 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(BeamArgs a) {
       if (!better) continue;
       const auto there = [&](int e) {
         const int at = p + (e / V * 64 + lane) * V + e % V;
-        return whole || (at >= shift && at < end);
+        return whole || at < end;
       };
-      const auto token = [&](int e) { return ~(uint32_t)(p + (e / V * 64 + lane) * V + e % V - shift); };
+      const auto token = [&](int e) { return ~(uint32_t)(p + (e / V * 64 + lane) * V + e % V); };
       if (__popcll(better) >= a.k) {
         uint32_t bk = 0, bv = 0;
 #pragma unroll
@@ -467,12 +475,12 @@ static int beam_shape(int64_t batch, int beams, int64_t vocab, int k) {
                KH_MAX_BEAM_K);
   return KH_OK;
 }
-// Parts of a row (tiles of a part), wherever it starts between two 16-byte borders: as many waves as the chip holds.
+// Parts of a row (tiles of a part): as many waves as the chip holds.
 struct BeamPlan {
   int parts, slots;
 };
 static BeamPlan beam_plan(int64_t rows, int64_t vocab) {
-  const int64_t all = (vocab + 7 + kBmTile - 1) / kBmTile;
+  const int64_t all = (vocab + kBmTile - 1) / kBmTile;
   const int64_t want = std::max<int64_t>(std::min(kBmFill / std::max<int64_t>(rows, 1), all), 1);
   BeamPlan p;
   const int64_t tiles = (all + want - 1) / want;  // of a part
