@@ -882,9 +882,9 @@ int kh_paged_kv_reorder(kh_paged_kv* c, const int32_t* table_dev, int64_t table_
  * score is not finite, or whose log-sum-exp is not (a NaN or +inf among its logits, or
  * nothing but -inf).  Log-sum-exps and scores are f64 (of f32 exponentials, each that counts within
  * 2^-21 and without a bias), compared as they are computed and rounded to f32 where they are written: continuations
- * of one beam are ordered by their logits, and beams with the same logits and score have equal scores, wherever their
- * rows start.  Writes y, i and v, [batch][k] each.  k <= 64, k <= beams * vocab,
- * beams <= KH_MAX_BEAMS.  ws_dev: 16-byte aligned, kh_beam_select_workspace bytes, not shared by
+ * of one beam are ordered by their logits, also where their scores come out equal, and beams with the same logits
+ * and score have equal scores, wherever their rows start.  Writes y, i and v, [batch][k] each.  k <= 64,
+ * k <= beams * vocab, beams <= KH_MAX_BEAMS.  ws_dev: 16-byte aligned, kh_beam_select_workspace bytes, not shared by
  * calls that may run at once.  The stream's device must be the current one. */
 #define KH_MAX_BEAM_K 64
 int kh_beam_select_workspace(int64_t batch, int beams, int64_t vocab, int k, int64_t* bytes);

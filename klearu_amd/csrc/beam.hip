@@ -334,8 +334,10 @@ __global__ __launch_bounds__(kBjThreads) void beam_join_kernel(BeamArgs a) {
   constexpr int W = kBjThreads / 64;
   __shared__ double s_score[KH_MAX_BEAMS], s_top[KH_MAX_BEAMS], s_log[KH_MAX_BEAMS];  // and the log-sum-exp's parts
   __shared__ int s_kind[KH_MAX_BEAMS];  // 0: its parts' logits, 1: none, 2: at its end
-  __shared__ uint64_t s_key[kBjList], s_bk[W];
-  __shared__ uint32_t s_flat[kBjList], s_bf[W], s_t;
+  // a continuation's score, and what orders equal ones, from the first: the beam, its logit (the largest
+  // first: a score may have no digits for the difference), the token
+  __shared__ uint64_t s_key[kBjList], s_tie[kBjList], s_bk[W], s_bt[W];
+  __shared__ uint32_t s_t;
   __shared__ int s_n;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int each = a.parts * a.k, all = a.beams * each;
@@ -370,94 +372,92 @@ __global__ __launch_bounds__(kBjThreads) void beam_join_kernel(BeamArgs a) {
     }
     if (t == 0) s_n = 0, s_t = 0;
     __syncthreads();
-    // continuation j with entry w of its part: its key (0: there is none) and its place among all
-    const auto get = [&](int j, uint64_t w, uint32_t& flat) -> uint64_t {
+    // continuation j with entry w of its part: its key (0: there is none) and its order among equal ones
+    const auto get = [&](int j, uint64_t w, uint64_t& tie) -> uint64_t {
       const int i = (int)((uint32_t)j / (uint32_t)each), e = j - i * each, kind = s_kind[i];
-      flat = (uint32_t)i * (uint32_t)a.vocab;
+      tie = (uint64_t)i << 56;
       if (kind == 0) {
         const uint32_t k32 = (uint32_t)(w >> 32);
         const double x = (double)__uint_as_float(k32 >> 31 ? k32 & 0x7fffffffu : ~k32);
-        flat += ~(uint32_t)w;
+        tie |= (uint64_t)~k32 << 24 | ~(uint32_t)w;
         return w ? f64_key(s_score[i] + ((x - s_top[i]) - s_log[i])) : 0;  // logits of any size leave the score its bits
       }
       // the first tokens, all of them -inf, but for the end
       if (e >= a.k || e >= a.vocab) return 0;
-      flat += kind == 1 || e > a.end ? e : e == 0 ? (uint32_t)a.end : e - 1;
+      tie |= kind == 1 || e > a.end ? e : e == 0 ? (uint32_t)a.end : e - 1;
       return f64_key(kind == 2 && e == 0 ? s_score[i] : -INFINITY);
     };
     uint64_t key[kBjEach];
-    uint32_t flat[kBjEach];
+    uint64_t tie[kBjEach];
     // the k-th largest of the lanes' own maxima, by their upper words
     uint32_t most = 0;
 #pragma unroll
     for (int c = 0; c < kBjEach; ++c) {
       const int j = t + c * kBjThreads;
-      key[c] = j < all ? get(j, mine[c], flat[c]) : 0;
+      key[c] = j < all ? get(j, mine[c], tie[c]) : 0;
       most = max(most, (uint32_t)(key[c] >> 32));
     }
     for (int j = t + kBjEach * kBjThreads; j < all; j += kBjThreads) {
-      uint32_t f;
+      uint64_t f;
       most = max(most, (uint32_t)(get(j, top[j], f) >> 32));
     }
     const uint32_t Tw = kth_largest(a.k, 0, [&](uint32_t v) { return ballots(most >= v); });
     if (lane == 0) atomicMax(&s_t, Tw);
     __syncthreads();
     const uint32_t T = s_t;
-    const auto list = [&](uint64_t y, uint32_t f) {
+    const auto list = [&](uint64_t y, uint64_t f) {
       if (y != 0 && (uint32_t)(y >> 32) >= T) {
         const int at = atomicAdd(&s_n, 1);
-        if (at < kBjList) s_key[at] = y, s_flat[at] = f;
+        if (at < kBjList) s_key[at] = y, s_tie[at] = f;
       }
     };
 #pragma unroll
-    for (int c = 0; c < kBjEach; ++c) list(key[c], flat[c]);
+    for (int c = 0; c < kBjEach; ++c) list(key[c], tie[c]);
     for (int j = t + kBjEach * kBjThreads; j < all; j += kBjThreads) {
-      uint32_t f;
+      uint64_t f;
       const uint64_t y = get(j, top[j], f);
       list(y, f);
     }
     __syncthreads();
     const int n = s_n;
-    const auto put = [&](int at, uint64_t y, uint32_t f) {
+    const auto put = [&](int at, uint64_t y, uint64_t f) {
       a.out_y[b * a.k + at] = (float)key_f64(y);
-      a.out_i[b * a.k + at] = (int32_t)(f / (uint32_t)a.vocab);
-      a.out_v[b * a.k + at] = (int32_t)(f % (uint32_t)a.vocab);
+      a.out_i[b * a.k + at] = (int32_t)(f >> 56);
+      a.out_v[b * a.k + at] = (int32_t)(f & 0xffffffu);
     };
     if (n <= kBjList) {
       for (int i0 = 0; i0 < n; i0 += kBjThreads / 8) {  // eight lanes an entry
         const int i = min(i0 + (t >> 3), n - 1);
         const uint64_t y = s_key[i];
-        const uint32_t f = s_flat[i];
+        const uint64_t f = s_tie[i];
         int above = 0;
-        for (int j = t & 7; j < n; j += 8) above += s_key[j] > y || (s_key[j] == y && s_flat[j] < f) ? 1 : 0;
+        for (int j = t & 7; j < n; j += 8) above += s_key[j] > y || (s_key[j] == y && s_tie[j] < f) ? 1 : 0;
         above += dpp<kDppQuadSwap1>(above);
         above += dpp<kDppQuadSwap2>(above);
         above += dpp<kDppRowHalfMirror>(above);
         if ((t & 7) == 0 && i0 + (t >> 3) < n && above < a.k) put(above, y, f);
       }
     } else {  // many equal scores: the best, time after time
-      uint64_t lk = ~0ull;  // the last one written
-      uint32_t lf = 0;
+      uint64_t lk = ~0ull, lf = 0;  // the last one written
       for (int i = 0; i < a.k; ++i) {
-        uint64_t bk = 0;
-        uint32_t bf = ~0u;
+        uint64_t bk = 0, bf = ~0ull;
         for (int j = t; j < all; j += kBjThreads) {
-          uint32_t f;
+          uint64_t f;
           const uint64_t y = get(j, top[j], f);
           if (y != 0 && (y < lk || (y == lk && f > lf)) && (y > bk || (y == bk && f < bf))) bk = y, bf = f;
         }
 #pragma unroll
         for (int m = 32; m > 0; m >>= 1) {
           const uint64_t ok = __shfl_xor((unsigned long long)bk, m);
-          const uint32_t of = __shfl_xor(bf, m);
+          const uint64_t of = __shfl_xor((unsigned long long)bf, m);
           if (ok > bk || (ok == bk && of < bf)) bk = ok, bf = of;
         }
         __syncthreads();
-        if (lane == 0) s_bk[wave] = bk, s_bf[wave] = bf;
+        if (lane == 0) s_bk[wave] = bk, s_bt[wave] = bf;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < W; ++w)
-          if (s_bk[w] > bk || (s_bk[w] == bk && s_bf[w] < bf)) bk = s_bk[w], bf = s_bf[w];
+          if (s_bk[w] > bk || (s_bk[w] == bk && s_bt[w] < bf)) bk = s_bk[w], bf = s_bt[w];
         lk = bk;
         lf = bf;
         if (t == 0) put(i, bk, bf);

@@ -1,7 +1,8 @@
-"""GPU: the order of continuations whose scores are equal.
+"""GPU: the order of continuations whose scores are equal, or come out equal.
 
 Scores are compared in f64 as they are computed.  Beams of the same logits and score have the same scores, bit for bit, wherever
-their rows start, so that the order between them is that of the beams: every place is known, without a tolerance."""
+their rows start, so that the order between them is that of the beams; within a beam larger logits come first, also where
+the score has no digits for the difference, and equal ones by their tokens.  Every place is known, without a tolerance."""
 import numpy as np
 import pytest
 import torch
@@ -44,3 +45,21 @@ def test_bits_do_not_depend_on_where_rows_start(kh, dtype, vocab, shift):
     want = beam.select(wide, s, 9)
     for got in (beam.select(x, s, 9), beam.select(odd, s, 9)):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [200, 5000, 70001])
+@pytest.mark.parametrize("top,small", [(1e20, 1.0), (5.0, 2.0 ** -70)])
+def test_logits_that_the_scores_do_not_tell_apart(kh, dtype, vocab, top, small):
+    """One logit far larger than the steps between the others: they are in their own order all the same."""
+    from klearu_amd import beam
+    rng = np.random.default_rng(vocab)
+    x = np.full((1, 2, vocab), -small * 300, np.float32)
+    at = np.stack([rng.permutation(vocab)[:121] for _ in range(2)])
+    for b in range(2):
+        x[0, b, at[b, :120]] = small * rng.permutation(np.arange(1, 121))
+        x[0, b, at[b, 120]] = top
+    s = np.array([[-20.0, -21.0 - 2.0 * top]], np.float32)  # the second beam's scores all lie below the first one's
+    for k in (3, 16, 64):
+        y, i, v = (t[0].cpu().numpy() for t in beam.select(torch.from_numpy(x).to(dtype).cuda(), torch.from_numpy(s).cuda(), k))
+        assert (i == 0).all() and v.tolist() == np.argsort(-x[0, 0], kind="stable")[:k].tolist()
