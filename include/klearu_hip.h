@@ -844,8 +844,8 @@ int kh_paged_kv_weights(const kh_paged_kv* c, int dtype, const void* q_dev, int6
  *   kept_dev    int32 [batch][kv heads][keep]: where each position was (its own place
  *               where nothing was evicted), -1 past the sequence's end;
  *   acc_out_dev f32 [batch][kv heads][acc_cols]: acc of the positions that are left,
- *               then 0 (may be acc_dev itself);
- *   len_out_dev int64 [batch]: min(len, keep) (not len_dev itself).
+ *               then 0 (may be acc_dev itself, but not lie on a part of it);
+ *   len_out_dev int64 [batch]: min(len, keep) (nowhere on len_dev).
  * Positions past acc_cols or the table are evicted and reported by kh_paged_kv_status,
  * as are page ids outside the pool, whose positions do not move.  Sequences that are
  * cut must not share pages with any other (as none that two beams go on from).

@@ -728,7 +728,7 @@ extern "C" int kh_paged_kv_evict(kh_paged_kv* c, const float* acc_dev, int64_t a
                (long long)keep);
   if (batch == 0) return KH_OK;
   KH_CHECK_ARG(acc_dev && len_dev && table_dev && kept_dev && acc_out_dev && len_out_dev, "null argument");
-  KH_CHECK_ARG(len_out_dev != len_dev, "the new lengths need a place of their own");
+  KH_CHECK_ARG(!ranges_meet(len_dev, batch * 8, len_out_dev, batch * 8), "the new lengths need a place of their own");
   const EvictSpace sp = evict_space(c, batch, keep, acc_cols);
   const int64_t need = sp.bytes;
   if (need > 0 && (!ws_dev || ws_bytes < need)) {
@@ -736,6 +736,11 @@ extern "C" int kh_paged_kv_evict(kh_paged_kv* c, const float* acc_dev, int64_t a
     return KH_ERR_CAPACITY;
   }
   KH_CHECK_ARG((reinterpret_cast<uintptr_t>(ws_dev) & 15) == 0, "the workspace must be 16-byte aligned");
+  // at most 2^59 bytes: more heads have no workspace
+  const int64_t all = batch * c->nkv * acc_cols;
+  const bool in_place = acc_out_dev == acc_dev;
+  KH_CHECK_ARG(in_place || !ranges_meet(acc_dev, all * 4, acc_out_dev, all * 4),
+               "the weights and their new place overlap and are not the same");
   KH_ON_DEVICE(c->device, "the cache");
   EvictArgs a;
   a.pool = c->pool;
@@ -760,8 +765,7 @@ extern "C" int kh_paged_kv_evict(kh_paged_kv* c, const float* acc_dev, int64_t a
   char* ws = static_cast<char*>(ws_dev);
   a.images = ws;
   a.num_images = (int)sp.images;
-  const int64_t all = batch * c->nkv * acc_cols;
-  a.weights = acc_out_dev < acc_dev + all && acc_dev < acc_out_dev + all ? reinterpret_cast<float*>(ws + sp.weights) : nullptr;
+  a.weights = in_place ? reinterpret_cast<float*>(ws + sp.weights) : nullptr;
   a.hist[0] = a.hist[2] = reinterpret_cast<uint16_t*>(ws + sp.hist);
   a.hist[1] = a.hist[0] + batch * c->nkv * sp.parts * kEvBins;
   a.state = reinterpret_cast<int*>(ws + sp.state);

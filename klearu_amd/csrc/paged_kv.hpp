@@ -105,6 +105,12 @@ constexpr int64_t kGridThreads = ((int64_t)1 << 32) - 1;
 int paged_attn_prepare(int d);
 int paged_weights_prepare(int d);
 
+// Whether two ranges of n and m bytes have one in common.
+inline bool ranges_meet(const void* a, int64_t n, const void* b, int64_t m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x <= y ? y - x < (uint64_t)n : x - y < (uint64_t)m;
+}
+
 inline size_t dtype_bytes(int dtype) { return dtype == KH_DT_F32 ? 4 : 2; }
 
 // Whether 16-byte accesses of whole 16-byte pieces are aligned: the base and

@@ -365,7 +365,7 @@ class PagedKv(_Handle):
         behind them is free.  A sequence's pages must be its own, as for append.  Their places are no longer their positions in the text: append(pos=...)
         and apply() take those.  Returns (kept, lens, acc): kept [batch, num_kv_heads, keep] (int32)
         where each position was, -1 past a sequence's end; the new lengths; the weights of
-        what is left, then 0, in `out` (acc itself may be it) or a new tensor."""
+        what is left, then 0, in `out` (acc itself may be it, but no part of it) or a new tensor."""
         dev = self._dev
         batch = lens.shape[0]
         lp = _index(lens, "lens", dev, _I64, (batch,))
