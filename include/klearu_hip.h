@@ -866,7 +866,7 @@ int kh_paged_kv_evict(kh_paged_kv* c, const float* acc_dev, int64_t acc_cols, co
  * those of the beams that nobody goes on from, in order, and get a copy of the
  * parent's rows in the page that is not whole.  (A sequence whose beams all begin as one: every
  * parent 0, and pages of its own in every row from column len / page_size on.)
- * out_table_dev must not overlap table_dev.  A whole page that no row lists any more is the caller's
+ * out_table_dev must not overlap table_dev (its rows may lie between that one's).  A whole page that no row lists any more is the caller's
  * again.  A parent outside 0 .. beams - 1 counts as the beam itself, and kh_paged_kv_status reports it. */
 #define KH_MAX_BEAMS 64
 int kh_paged_kv_reorder(kh_paged_kv* c, const int32_t* table_dev, int64_t table_cols, int64_t table_stride,

@@ -668,6 +668,18 @@ static int table_args(const kh_paged_kv* c, int64_t cols, int64_t table_stride) 
   return KH_OK;
 }
 
+// Whether two tables of the same rows and columns share an element: each one's rows come in order and apart.
+static bool tables_meet(const int32_t* a, int64_t a_stride, const int32_t* b, int64_t b_stride, int64_t rows, int64_t cols) {
+  if (!ranges_meet(a, ((rows - 1) * a_stride + cols) * 4, b, ((rows - 1) * b_stride + cols) * 4)) return false;
+  for (int64_t i = 0, j = 0; i < rows && j < rows;) {
+    const int32_t *x = a + i * a_stride, *y = b + j * b_stride;
+    if (ranges_meet(x, cols * 4, y, cols * 4)) return true;
+    if (x < y) ++i;
+    else ++j;
+  }
+  return false;
+}
+
 static int evict_shape(const kh_paged_kv* c, int64_t batch, int64_t keep, int64_t acc_cols) {
   KH_CHECK_ARG(c != nullptr, "null handle");
   KH_CHECK_ARG(batch >= 0 && batch < (int64_t)1 << 31, "batch %lld not in [0,2^31)", (long long)batch);
@@ -788,7 +800,10 @@ extern "C" int kh_paged_kv_reorder(kh_paged_kv* c, const int32_t* table_dev, int
   KH_CHECK_ARG(out_stride >= table_cols, "rows of the new table %lld apart", (long long)out_stride);
   if (batch == 0) return KH_OK;
   KH_CHECK_ARG(table_dev && len_dev && parent_dev && out_table_dev, "null argument");
-  KH_CHECK_ARG(out_table_dev != table_dev, "the new table needs a place of its own");
+  KH_CHECK_ARG(table_stride < INT64_MAX / 8 / (batch * beams) && out_stride < INT64_MAX / 8 / (batch * beams),
+               "tables of rows %lld and %lld apart", (long long)table_stride, (long long)out_stride);
+  KH_CHECK_ARG(!tables_meet(table_dev, table_stride, out_table_dev, out_stride, batch * beams, table_cols),
+               "the new table needs a place of its own");
   KH_ON_DEVICE(c->device, "the cache");
   ReorderArgs a;
   a.pool = c->pool;
