@@ -564,8 +564,8 @@ static int evict_launch(const EvictArgs& a, bool whole, bool chain, hipStream_t 
     if (a.weights)
       hipLaunchKernelGGL(evict_weights_kernel, dim3((unsigned)((a.acc_cols + 255) / 256), (unsigned)a.nkv, seqs), dim3(256), 0, st, a);
   }
-  if (a.keep >= a.acc_cols) return KH_OK;
-  if (chain) {
+  if (a.keep >= a.acc_cols) {  // nothing is cut, nothing moves
+  } else if (chain) {
     hipLaunchKernelGGL(evict_move_kernel<D>, dim3((unsigned)a.nkv, seqs, 2), dim3(kEvThreads), 0, st, a);
   } else {
     const dim3 g((unsigned)std::min<int64_t>(a.batch * ((a.keep + kEvCopy - 1) / kEvCopy), 1 << 20), (unsigned)a.nkv, 2);
