@@ -277,7 +277,10 @@ struct QuadLanes {
 // 53% of its cycles, do not overlap enough (a position a lane took 77 us;
 // quads with correctly rounded quotients by a division 38, by a corrected reciprocal 33).
 // One row: 4 us, the chain of offsets, page id and table.
-template <typename T, int D, int MODE, bool VAL>
+//
+// AXES: several positions a row, in kernels of their own: the checks of the others' kernels cost prompts 0.7 us of
+// 56 (with the gather).
+template <typename T, int D, int MODE, bool AXES, bool VAL>
 __device__ __forceinline__ void append_part(const AppendArgs& a, int units, int hpu, int* s_q, int* s_wsum, int* s_tot,
                                             uint16_t* s_v) {
   using P = KvParts<D>;
@@ -292,9 +295,9 @@ __device__ __forceinline__ void append_part(const AppendArgs& a, int units, int 
   const bool first_half = 8 * c < (a.rot >> 1);
   const bool turns = MODE == kRotHalf || MODE == kRotInterleaved ? 8 * c < a.rot : false;
   const int other = first_half ? a.rot >> 1 : -(a.rot >> 1);  // the pairs' other elements (kRotHalf)
-  // several axes: where the positions along the axis of the lane's pairs lie
+  // where the positions along the axis of the lane's pairs lie
   const int64_t mine_axis =
-      a.ax.n > 1 && turns ? a.ax.of(MODE == kRotInterleaved ? 4 * c : first_half ? 8 * c : 8 * c - (a.rot >> 1)) * a.ax.stride : 0;
+      AXES && turns ? a.ax.of(MODE == kRotInterleaved ? 4 * c : first_half ? 8 * c : 8 * c - (a.rot >> 1)) * a.ax.stride : 0;
   walk_quads(a.r, units, hpu, s_q, s_wsum, s_tot, [&](int64_t p0, int t0, int o0, int o1, int pg, int h0, int nh) {
       const int at0 = (int)(p0 & (ps - 1));
       // the lane's positions
@@ -310,7 +313,7 @@ __device__ __forceinline__ void append_part(const AppendArgs& a, int units, int 
         if (a.table && on[k]) {  // a row without a rotation is not appended at all
           const int64_t r = a.pos ? a.pos[mine_axis + t] : p0 + k * TP + tp;
           bool out = r < 0 || r >= a.max_pos;
-          if (a.ax.n > 1 && a.pos) {  // a row is appended whole or not at all
+          if (AXES && a.pos) {  // a row is appended whole or not at all
             for (int i = 0; i < a.ax.n; ++i) {
               const int64_t ri = a.pos[i * a.ax.stride + t];
               out = out || ri < 0 || ri >= a.max_pos;
@@ -433,12 +436,12 @@ __device__ __forceinline__ void append_part(const AppendArgs& a, int units, int 
   });
 }
 
-template <typename T, int D, int MODE>
+template <typename T, int D, int MODE, bool AXES>
 __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a, int units, int hpu) {
   __shared__ int s_q[kSeqChunk], s_wsum[kKvThreads / 64], s_tot;
   __shared__ __align__(16) uint16_t s_v[kKvThreads / 64][D == 64 ? 2 * D : D];
-  if (blockIdx.y == 0) append_part<T, D, MODE, false>(a, units, hpu, s_q, s_wsum, &s_tot, nullptr);
-  else append_part<T, D, kRotNone, true>(a, units, hpu, s_q, s_wsum, &s_tot, s_v[threadIdx.x >> 6]);
+  if (blockIdx.y == 0) append_part<T, D, MODE, AXES, false>(a, units, hpu, s_q, s_wsum, &s_tot, nullptr);
+  else append_part<T, D, kRotNone, AXES, true>(a, units, hpu, s_q, s_wsum, &s_tot, s_v[threadIdx.x >> 6]);
 }
 
 struct GatherArgs {
@@ -516,21 +519,30 @@ __global__ __launch_bounds__(kKvThreads) void kv_gather_kernel(GatherArgs a, int
   else gather_part<T, D, true>(a, units, hpu, s_q, s_wsum, &s_tot);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool AXES>
 static void append_launch_m(const AppendArgs& a, dim3 g, int units, int hpu, hipStream_t st) {
   const dim3 blk(kKvThreads);
-  if (a.mode == kRotNone) hipLaunchKernelGGL((kv_append_kernel<T, D, kRotNone>), g, blk, 0, st, a, units, hpu);
-  else if (a.mode == kRotHalf) hipLaunchKernelGGL((kv_append_kernel<T, D, kRotHalf>), g, blk, 0, st, a, units, hpu);
+  if (a.mode == kRotHalf)
+    hipLaunchKernelGGL((kv_append_kernel<T, D, kRotHalf, AXES>), g, blk, 0, st, a, units, hpu);
   else if (a.mode == kRotInterleaved)
-    hipLaunchKernelGGL((kv_append_kernel<T, D, kRotInterleaved>), g, blk, 0, st, a, units, hpu);
-  else if (a.mode == kRotAxes) hipLaunchKernelGGL((kv_append_kernel<T, D, kRotAxes>), g, blk, 0, st, a, units, hpu);
-  else hipLaunchKernelGGL((kv_append_kernel<T, D, kRotAny>), g, blk, 0, st, a, units, hpu);
+    hipLaunchKernelGGL((kv_append_kernel<T, D, kRotInterleaved, AXES>), g, blk, 0, st, a, units, hpu);
+  else if constexpr (AXES)
+    hipLaunchKernelGGL((kv_append_kernel<T, D, kRotAxes, true>), g, blk, 0, st, a, units, hpu);
+  else if (a.mode == kRotNone)
+    hipLaunchKernelGGL((kv_append_kernel<T, D, kRotNone, false>), g, blk, 0, st, a, units, hpu);
+  else
+    hipLaunchKernelGGL((kv_append_kernel<T, D, kRotAny, false>), g, blk, 0, st, a, units, hpu);
+}
+template <typename T, int D>
+static void append_launch_d(const AppendArgs& a, dim3 g, int units, int hpu, hipStream_t st) {
+  if (a.ax.n > 1) append_launch_m<T, D, true>(a, g, units, hpu, st);
+  else append_launch_m<T, D, false>(a, g, units, hpu, st);
 }
 template <typename T>
 static void append_launch(int d, const AppendArgs& a, dim3 g, int units, int hpu, hipStream_t st) {
-  if (d == 64) append_launch_m<T, 64>(a, g, units, hpu, st);
-  else if (d == 128) append_launch_m<T, 128>(a, g, units, hpu, st);
-  else append_launch_m<T, 256>(a, g, units, hpu, st);
+  if (d == 64) append_launch_d<T, 64>(a, g, units, hpu, st);
+  else if (d == 128) append_launch_d<T, 128>(a, g, units, hpu, st);
+  else append_launch_d<T, 256>(a, g, units, hpu, st);
 }
 template <typename T>
 static void gather_launch(int d, const GatherArgs& a, dim3 g, int units, int hpu, hipStream_t st) {
