@@ -688,9 +688,14 @@ static int evict_shape(const kh_paged_kv* c, int64_t batch, int64_t keep, int64_
   return KH_OK;
 }
 // How a call is cut, and its workspace: one block a kv head selects where a sequence's weights fit in its
-// registers, and two (keys and values) move where there are enough of them or little is kept: 32 kv heads that
-// keep 2048 take 17.5 us so and 7.3 + 9.2 as two copies, 256 that keep 1024 17.2 and 14.5 + 13.4, 8 that keep
-// 32768 75 and 27.6 + 16.9.
+// registers, and two (keys and values) move where there are enough of them or little is kept.  Whole calls that halve
+// 128-wide sequences, such a chain / two copies, in us:
+//   kv heads   keep 1024     2048          4096          8192
+//        8     22.8 / 23.5   27.2 / 26.2   41.1 / 29.6   64.7 / 35.5
+//       32     23.5 / 25.3   28.4 / 33.5   42.9 / 40.1   68.3 / 56.6
+//       64     24.3 / 28.6   30.0 / 38.6   45.3 / 55.3   73.6 / 88.0
+//      128     26.4 / 35.5   36.9 / 53.0   57.4 / 89.5   113 / 186
+// 64-wide heads (62.0 / 60.9 at 64 of 8192) and 256-wide ones (30.9 / 28.6 at 8 of 2048) change sides at the same sizes.
 struct EvictSpace {
   bool whole, chain;
   int64_t parts, images, weights, hist, state, bytes;
@@ -699,7 +704,7 @@ static EvictSpace evict_space(const kh_paged_kv* c, int64_t batch, int64_t keep,
   EvictSpace s;
   const int64_t heads = batch * c->nkv, most = std::min(keep, acc_cols);
   s.whole = acc_cols <= kEvThreads * kEvMost;
-  s.chain = keep >= acc_cols || heads >= 128 || keep <= 4096;
+  s.chain = keep >= acc_cols || heads >= 64 || keep <= 2048;
   s.parts = (acc_cols + kEvPart - 1) / kEvPart;
   s.images = (most + c->ps - 1) >> c->ps_log2;
   if (heads > ((int64_t)1 << 46) / acc_cols) {  // more than a GPU's weights: no workspace is large enough

@@ -1,7 +1,8 @@
 """GPU: kept positions that one block moves in several chunks, each over places that the chunk before has just filled from.
 
-A block of a kv head takes 2048 positions at a time (1024 at 256-wide heads) through its registers, where little is kept
-or there are many kv heads.  Everything is compared bit for bit."""
+A block of a kv head takes 2048 positions at a time (1024 at 256-wide heads) through its registers, where no more than that
+is kept or there are 64 kv heads; the same sizes at fewer heads go through the workspace.  Everything is compared
+bit for bit."""
 import numpy as np
 import pytest
 import torch
@@ -29,7 +30,7 @@ def sparse(rng, batch, kv, cols):
     (2, 256, 64, [4000], 1025, 0, 0), (2, 256, 16, [4001, 3100], 3001, 100, 3), (1, 256, 128, [3010], 3002, 7, 0),
     (1, 128, 64, [4500, 2050], 2049, 0, 0), (3, 128, 16, [5000], 4095, 500, 4), (2, 128, 32, [4110], 4094, 0, 16),
     (3, 64, 16, [4400, 2052, 100], 2050, 1, 1), (1, 64, 256, [4300], 4093, 0, 0), (2, 64, 64, [4099], 4096, 4000, 0),
-    (1, 64, 64, [17000], 4095, 33, 5), (1, 256, 64, [16500], 2047, 0, 0)])
+    (1, 64, 64, [17000], 4095, 33, 5), (1, 256, 64, [16500], 2047, 0, 0), (3, 256, 32, [2047, 2000], 1999, 4, 700)])
 def test_several_chunks(kh, kv, dim, page, lens, keep, recent, first, kind, place):
     rng = np.random.default_rng(keep + dim)
     c = Cache(kv, dim, lens, page)
@@ -44,7 +45,8 @@ def test_several_chunks(kh, kv, dim, page, lens, keep, recent, first, kind, plac
 
 @pytest.mark.parametrize("kind", ["plain", "rising", "sparse"])
 @pytest.mark.parametrize("kv,dim,page,lens,keep", [(16, 64, 16, [2600, 2051, 2500, 2100, 2600, 2055, 2300, 2599], 2050),
-                                                   (128, 64, 64, [4500], 4203), (64, 128, 32, [2200, 2100], 2051), (128, 256, 16, [1100], 1026)])
+                                                   (128, 64, 64, [4500], 4203), (64, 128, 32, [2200, 2100], 2051), (128, 256, 16, [1100], 1026),
+                                                   (64, 64, 256, [4300], 4093), (64, 128, 16, [2400], 2050), (32, 256, 64, [2500, 2100], 2049)])
 def test_many_heads(kh, kv, dim, page, lens, keep, kind):
     rng = np.random.default_rng(keep + kv)
     c = Cache(kv, dim, lens, page)
