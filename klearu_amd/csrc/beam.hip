@@ -16,9 +16,11 @@
 // LDS, which is cut to k when it fills and at the end: the k-th largest is found bit by bit, counted with
 // ballots.  When a wave sees what another tells changes its list, not the k largest of all.
 //
-// Both kernels, 512 rows of 131071 BF16 logits, k 16: 55 us (50 and 5), 2.4 TB/s of logits.  What bounds the first one are
-// instructions (210 for 1024 logits, of which 64 are the sums') and the chains of ballots in between: a copy reads as much
-// in 28 us.  One pass is all that a row needs; waves take its tiles side by side (59 us with a range each).
+// Both kernels, 512 rows of 131071 BF16 logits, k 16: 56 us (48 and 7), 2.4 TB/s of logits.  The first one's 210 instructions
+// for 1024 logits, of which 16 are exponentials at a quarter of the rate, take the SIMDs 27 us, and a copy reads as much in
+// 28: loads and work hardly overlap, with one tile ahead and chains of ballots in between.  k 32 takes 76 us, and 64,
+// which nobody has looked into, 404.  One pass is all that a row needs; waves take its tiles side by side (59 us with a
+// range each).
 #include <algorithm>
 
 #include "paged_kv.hpp"
@@ -28,7 +30,8 @@ namespace kh {
 constexpr int kBmThreads = 512, kBmWaves = kBmThreads / 64;
 constexpr int kBmEach = 16;             // logits of a lane
 constexpr int kBmTile = 64 * kBmEach;   // of a wave
-// Waves that the chip holds at once (512 rows of 131071: 2048 80 us, 8192 78, 4096 62).
+// Waves that the chip holds at once, in us with 2048 / 4096 / 8192 of them: 512 rows of 131071 BF16 logits 71 / 53 / 70, of
+// 32000 35 / 31 / 36; 64 rows of 131071 23.3 / 22.9 / 28.3; 1200 of 32000 77 / 66 / 63.
 constexpr int64_t kBmFill = 4096;
 
 struct BeamArgs {

@@ -67,7 +67,7 @@ __device__ __forceinline__ void evict_none(const EvictArgs& a, int64_t row, int6
 }
 
 // Block: one kv head of one sequence, whose weights fit in its registers: one launch, and weights are read once.  A chain of
-// length, weights, histogram, candidates and places with twelve barriers bounds it, not the bytes: 12.7 us for 32 kv heads
+// length, weights, histogram, candidates and places with twelve barriers bounds it, not the bytes: 12.8 us for 32 kv heads
 // of 2111 positions, 15 for 256 of up to 4099.
 __global__ __launch_bounds__(kEvThreads) void evict_whole_kernel(EvictArgs a) {
   __shared__ TopkLds<kEvThreads> sh;
@@ -591,7 +591,9 @@ struct ReorderArgs {
 };
 
 // Block: a share of one beam: of its columns, and, a wave each, of the kv heads' keys and values that it copies.  64 x 8 beams of eight kv
-// heads of 128 with half a page of 64 each: 10.4 us (a row of pieces after the other: 15.5), a chain of parents, tables and rows.  Every wave
+// heads of 128 with half a page of 64 each: 10.2 us (a row of pieces after the other: 15.5).  The chain of parents, tables and
+// rows takes 2.9, as four beams show; the rest are rounds: 94 registers leave five waves a SIMD for eight of them, and those that
+// have nothing to copy take their places, too.  Every wave
 // works the beams' pages out for itself, a beam a lane: the beams that go on from an
 // earlier beam's parent (again), and those that nobody goes on from (gone), the i-th of either meeting.
 template <int D>
